@@ -1,0 +1,270 @@
+// A key-value cache in pages: places for new tokens, pages given back, keys and values written to their slots.
+#include "sah_common.h"
+#include "../../include/sah_serve.h"
+
+#define PG_NT 1024
+#define PG_MAX_REQ 4096   // records of all requests fit into 48 KB of LDS
+#define PG_REFUSED INT32_MIN
+
+// Exclusive scan of one 64-bit number per thread across PG_NT threads; *total: the sum. All threads call.
+__device__ __forceinline__ int64_t pg_scan(int64_t v, int64_t* wsum, int64_t* total) {
+  constexpr int NW = PG_NT / SAH_WAVE;
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
+  int64_t incl = v;
+#pragma unroll
+  for (int d = 1; d < SAH_WAVE; d <<= 1) {
+    const int64_t up = __shfl_up((long long)incl, d);
+    if (lane >= d) incl += up;
+  }
+  __syncthreads();  // wsum may still be read from the call before
+  if (lane == SAH_WAVE - 1) wsum[wave] = incl;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const int64_t s = wsum[i];
+    before += i < wave ? s : 0;
+    all += s;
+  }
+  *total = all;
+  return before + incl - v;
+}
+
+// Row t's request among `n` whose rows end at s_end[0 .. n) (not falling): the first whose end lies behind t.
+__device__ __forceinline__ int pg_request_of(const int* s_end, int n, int t) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (s_end[mid] > t) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
+// Places of rows t = first, first + step, ... A token that opens a page (every new page has one) writes the page's entry of
+// the table. s_rec: the request's length before the step, and the place in the free list of its first new page.
+__device__ __forceinline__ void pg_place(const sah_paged_assign_args& P, const int* s_end, const int2* s_rec, int first, int step) {
+  for (int t = first; t < P.n_tokens; t += step) {
+    const int b = pg_request_of(s_end, P.n_requests, t);
+    int64_t slot = -1;
+    int pos = 0;
+    if (b < P.n_requests) {
+      const int2 rec = s_rec[b];
+      pos = (int)((uint32_t)rec.x + (uint32_t)(t - (b ? s_end[b - 1] : 0)));
+      if (rec.y != PG_REFUSED) {
+        const int j = pos / P.page_size, entry = pos - j * P.page_size;
+        const int had = (int)(((int64_t)rec.x + P.page_size - 1) / P.page_size);
+        int32_t* te = P.block_table + (int64_t)b * P.table_pitch + j;
+        int page;
+        if (j >= had) {
+          page = P.free_pages[rec.y - (j - had)];
+          if (entry == 0) *te = page;
+        } else {
+          page = *te;
+        }
+        slot = page < 0 ? -1 : (int64_t)page * P.page_size + entry;
+      }
+    }
+    P.slot_map[t] = slot;
+    P.positions[t] = pos;
+  }
+}
+
+// One workgroup goes over the requests; with ALL it also places the tokens, else it leaves the records for k_paged_place.
+template <bool ALL>
+__global__ __launch_bounds__(PG_NT) void k_paged_assign(sah_paged_assign_args P) {
+  sah_touch_kernargs<sizeof(sah_paged_assign_args)>();
+  SAH_DYNAMIC_LDS(s_dyn);
+  __shared__ int64_t s_sum[PG_NT / SAH_WAVE];
+  int2* s_rec = (int2*)s_dyn;
+  int* s_end = (int*)(s_rec + P.n_requests);
+  int64_t count = *P.free_count;
+  if (count > P.n_pages) count = P.n_pages;
+  if (count < 0) count = 0;
+  int64_t rows = 0, pages = 0;   // of the requests before this round's
+  int taken = 0;                 // this thread's last granted page
+  for (int b0 = 0; b0 < P.n_requests; b0 += PG_NT) {
+    const int b = b0 + threadIdx.x;
+    const bool live = b < P.n_requests;
+    const int given = live ? P.new_lens[b] : 0;
+    const int64_t fresh = given > 0 ? given : 0, len = live ? P.lens[b] : 0;
+    int64_t all;
+    const int64_t begin = rows + pg_scan(fresh, s_sum, &all);
+    rows += all;
+    const int64_t had = (len + P.page_size - 1) / P.page_size, has = (len + fresh + P.page_size - 1) / P.page_size;
+    const bool fits = live && len >= 0 && begin + fresh <= P.n_tokens && has <= P.table_width && len + fresh <= INT32_MAX;
+    const int64_t need = fits ? has - had : 0;
+    const int64_t off = pages + pg_scan(need, s_sum, &all);
+    pages += all;
+    const bool ok = fits && (need == 0 || off + need <= count);
+    if (live) {
+      const int64_t end = begin + fresh;
+      const int e = (int)(end < P.n_tokens ? end : P.n_tokens);
+      const int2 rec = make_int2((int)len, ok ? (int)(count - 1 - (off < count ? off : count)) : PG_REFUSED);
+      if (ALL) {
+        s_end[b] = e;
+        s_rec[b] = rec;
+      } else {
+        ((int2*)P.work)[b] = rec;
+      }
+      P.cu_new[b + 1] = e;
+      P.granted[b] = ok;
+      P.kv_lens[b] = ok ? (int)(len + fresh) : 0;
+      P.lens_out[b] = (int)(ok ? len + fresh : len);
+      if (ok && need) taken = (int)(off + need);
+    }
+  }
+  // granted requests that need pages come before the others: the list has lost what the last of them took
+  int most = taken;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const int o = __shfl_xor(most, d);
+    most = most > o ? most : o;
+  }
+  __syncthreads();
+  if ((threadIdx.x & (SAH_WAVE - 1)) == 0) s_sum[threadIdx.x / SAH_WAVE] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < PG_NT / SAH_WAVE; ++i) most = most > (int)s_sum[i] ? most : (int)s_sum[i];
+    *P.free_count_out = (int)count - most;
+    P.cu_new[0] = 0;
+  }
+  if (ALL) pg_place(P, s_end, s_rec, threadIdx.x, PG_NT);
+}
+
+__global__ __launch_bounds__(PG_NT) void k_paged_place(sah_paged_assign_args P) {
+  sah_touch_kernargs<sizeof(sah_paged_assign_args)>();
+  SAH_DYNAMIC_LDS(s_dyn);
+  int2* s_rec = (int2*)s_dyn;
+  int* s_end = (int*)(s_rec + P.n_requests);
+  for (int b = threadIdx.x; b < P.n_requests; b += PG_NT) {
+    s_rec[b] = ((const int2*)P.work)[b];
+    s_end[b] = P.cu_new[b + 1];
+  }
+  __syncthreads();
+  pg_place(P, s_end, s_rec, blockIdx.x * PG_NT + threadIdx.x, gridDim.x * PG_NT);
+}
+
+// The finished requests' pages: places in the free list, and the requests' state
+__global__ __launch_bounds__(PG_NT) void k_paged_release(sah_paged_release_args P) {
+  __shared__ int64_t s_sum[PG_NT / SAH_WAVE];
+  int64_t count = *P.free_count;
+  if (count > P.n_pages) count = P.n_pages;
+  if (count < 0) count = 0;
+  int64_t pages = 0;
+  for (int b0 = 0; b0 < P.n_requests; b0 += PG_NT) {
+    const int b = b0 + threadIdx.x;
+    const bool done = b < P.n_requests && P.finished[b];
+    int64_t has = done && P.lens[b] > 0 ? ((int64_t)P.lens[b] + P.page_size - 1) / P.page_size : 0;
+    if (has > P.table_width) has = P.table_width;
+    int64_t all;
+    const int64_t off = count + pages + pg_scan(has, s_sum, &all);
+    pages += all;
+    // what a list that is full already has no room for is not appended
+    const int64_t room = P.n_pages - off < 0 ? 0 : P.n_pages - off;
+    if (b < P.n_requests) ((int2*)P.work)[b] = make_int2((int)(off < P.n_pages ? off : P.n_pages), (int)(has < room ? has : room));
+    if (done) P.lens[b] = 0;
+  }
+  __syncthreads();  // every thread has read the count
+  if (threadIdx.x == 0) *P.free_count = (int)(count + pages < P.n_pages ? count + pages : P.n_pages);
+}
+__global__ __launch_bounds__(256) void k_paged_give_back(sah_paged_release_args P) {
+  const int b = blockIdx.y;
+  const int2 rec = ((const int2*)P.work)[b];
+  for (int j = blockIdx.x * 256 + threadIdx.x; j < rec.y; j += gridDim.x * 256) {
+    int32_t* te = P.block_table + (int64_t)b * P.table_pitch + j;
+    P.free_pages[rec.x + j] = *te;
+    *te = -1;
+  }
+}
+
+// A unit is W bytes of a token's keys or values; consecutive threads take consecutive units of a token.
+template <typename W>
+__global__ __launch_bounds__(256) void k_paged_store(sah_paged_store_args P, int units_head, int units_token, int64_t n_units) {
+  sah_touch_kernargs<sizeof(sah_paged_store_args) + 16>();
+  const int es = P.dtype == SAH_F32 ? 4 : 2;
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= n_units) return;
+  const int64_t t = u / units_token;
+  const int in = (int)(u - t * units_token);
+  const int h = in / units_head, c = in - h * units_head;
+  const int64_t slot = P.slot_map[t];
+  if (slot < 0 || slot >= (int64_t)P.n_pages * P.page_size) return;
+  const int64_t page = slot / P.page_size, entry = slot - page * P.page_size;
+  const int64_t from_k = (t * P.ks_t + h * P.ks_h) * es, from_v = (t * P.vs_t + h * P.vs_h) * es;
+  const W kx = ((const W*)((const char*)P.k + from_k))[c], vx = ((const W*)((const char*)P.v + from_v))[c];
+  ((W*)((char*)P.k_cache + (page * P.kcs_p + entry * P.kcs_t + h * P.kcs_h) * es))[c] = kx;
+  ((W*)((char*)P.v_cache + (page * P.vcs_p + entry * P.vcs_t + h * P.vcs_h) * es))[c] = vx;
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+extern "C" int sah_paged_assign(const sah_paged_assign_args* a) {
+  if (!a) return sah_fail(SAH_ENULL, "sah_paged_assign: args is NULL");
+  if (a->n_requests <= 0 || a->page_size <= 0 || a->table_width <= 0 || a->n_pages <= 0 || a->n_tokens < 0)
+    return sah_fail(SAH_EINVAL, "sah_paged_assign: n_requests, page_size, table_width and n_pages must be > 0, n_tokens >= 0");
+  if (a->n_requests > PG_MAX_REQ) return sah_fail(SAH_ESHAPE, "sah_paged_assign: %d requests; at most %d", a->n_requests, PG_MAX_REQ);
+  if (a->table_pitch < a->table_width) return sah_fail(SAH_EINVAL, "sah_paged_assign: table_pitch is less than table_width");
+  if (!a->new_lens || !a->lens || !a->block_table || !a->free_pages || !a->free_count || !a->cu_new || !a->kv_lens || !a->granted ||
+      !a->lens_out || !a->free_count_out || !a->work || (a->n_tokens && (!a->slot_map || !a->positions)))
+    return sah_fail(SAH_ENULL, "sah_paged_assign: NULL pointer");
+  const size_t lds = (size_t)a->n_requests * 12;
+  hipStream_t st = (hipStream_t)a->stream;
+  if (a->n_tokens <= 4 * PG_NT) {
+    sah_timed timed("k_paged_assign", a->stream);
+    hipLaunchKernelGGL(k_paged_assign<true>, dim3(1), dim3(PG_NT), lds, st, *a);
+    return sah_launch_status("sah_paged_assign");
+  }
+  {
+    sah_timed timed("k_paged_assign", a->stream);
+    hipLaunchKernelGGL(k_paged_assign<false>, dim3(1), dim3(PG_NT), 0, st, *a);
+    if (int rc = sah_launch_status("sah_paged_assign")) return rc;
+  }
+  sah_timed timed("k_paged_place", a->stream);
+  int64_t wgs = ((int64_t)a->n_tokens + PG_NT - 1) / PG_NT;
+  hipLaunchKernelGGL(k_paged_place, dim3((unsigned)(wgs < 1024 ? wgs : 1024)), dim3(PG_NT), lds, st, *a);
+  return sah_launch_status("sah_paged_assign(place)");
+}
+
+extern "C" int sah_paged_release(const sah_paged_release_args* a) {
+  if (!a) return sah_fail(SAH_ENULL, "sah_paged_release: args is NULL");
+  if (a->n_requests <= 0 || a->page_size <= 0 || a->table_width <= 0 || a->n_pages <= 0)
+    return sah_fail(SAH_EINVAL, "sah_paged_release: n_requests, page_size, table_width and n_pages must be > 0");
+  if (a->n_requests > PG_MAX_REQ) return sah_fail(SAH_ESHAPE, "sah_paged_release: %d requests; at most %d", a->n_requests, PG_MAX_REQ);
+  if (a->table_pitch < a->table_width) return sah_fail(SAH_EINVAL, "sah_paged_release: table_pitch is less than table_width");
+  if (!a->finished || !a->lens || !a->block_table || !a->free_pages || !a->free_count || !a->work)
+    return sah_fail(SAH_ENULL, "sah_paged_release: NULL pointer");
+  hipStream_t st = (hipStream_t)a->stream;
+  {
+    sah_timed timed("k_paged_release", a->stream);
+    hipLaunchKernelGGL(k_paged_release, dim3(1), dim3(PG_NT), 0, st, *a);
+    if (int rc = sah_launch_status("sah_paged_release")) return rc;
+  }
+  sah_timed timed("k_paged_give_back", a->stream);
+  const int x = (a->table_width + 255) / 256;
+  hipLaunchKernelGGL(k_paged_give_back, dim3(x < 16 ? x : 16, a->n_requests), dim3(256), 0, st, *a);
+  return sah_launch_status("sah_paged_release(pages)");
+}
+
+extern "C" int sah_paged_store(const sah_paged_store_args* a) {
+  if (!a) return sah_fail(SAH_ENULL, "sah_paged_store: args is NULL");
+  if (a->dtype != SAH_F32 && a->dtype != SAH_BF16 && a->dtype != SAH_F16) return sah_fail(SAH_EDTYPE, "sah_paged_store: dtype %d", a->dtype);
+  if (a->n_tokens < 0 || a->Hkv <= 0 || a->D <= 0 || a->n_pages <= 0 || a->page_size <= 0)
+    return sah_fail(SAH_EINVAL, "sah_paged_store: Hkv, D, n_pages and page_size must be > 0, n_tokens >= 0");
+  if (a->n_tokens == 0) return SAH_OK;
+  if (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->slot_map) return sah_fail(SAH_ENULL, "sah_paged_store: NULL pointer");
+  const int es = a->dtype == SAH_F32 ? 4 : 2;
+  // 16 bytes at a time where every address allows it, else an element
+  const uint64_t all = (uint64_t)a->k | (uint64_t)a->v | (uint64_t)a->k_cache | (uint64_t)a->v_cache |
+                       (uint64_t)(es * (a->ks_t | a->ks_h | a->vs_t | a->vs_h | a->kcs_p | a->kcs_t | a->kcs_h | a->vcs_p | a->vcs_t | a->vcs_h | a->D));
+  const int wide = all % 16 == 0 ? 16 : es;
+  const int64_t units_head = (int64_t)a->D * es / wide, units_token = units_head * a->Hkv, n = units_token * a->n_tokens;
+  const int64_t wgs = (n + 255) / 256;
+  if (units_token > INT32_MAX || wgs > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_paged_store: too many elements");
+  hipStream_t st = (hipStream_t)a->stream;
+  sah_timed timed("k_paged_store", a->stream);
+  if (wide == 16) hipLaunchKernelGGL(k_paged_store<uint4>, dim3((unsigned)wgs), dim3(256), 0, st, *a, (int)units_head, (int)units_token, n);
+  else if (wide == 4) hipLaunchKernelGGL(k_paged_store<uint32_t>, dim3((unsigned)wgs), dim3(256), 0, st, *a, (int)units_head, (int)units_token, n);
+  else hipLaunchKernelGGL(k_paged_store<uint16_t>, dim3((unsigned)wgs), dim3(256), 0, st, *a, (int)units_head, (int)units_token, n);
+  return sah_launch_status("sah_paged_store");
+}

@@ -1,4 +1,4 @@
-"""ctypes binding of libsah_mi355.so (declared in include/sah.h).
+"""ctypes binding of libsah_mi355.so (declared in include/sah.h, sah_ext.h and sah_serve.h).
 
 The library is the only compute back end of this package: every masker and the
 masked attention call into it, and a missing library is an error, not a reason
@@ -67,6 +67,14 @@ EXTENSION_SYMBOLS = {
     "sah_amask_answer": 1,
     "sah_hash_decode_masked": 1,
 }
+# include/sah_serve.h: entry points of one argument block each
+SERVE_SYMBOLS = (
+    "sah_paged_assign",
+    "sah_paged_release",
+    "sah_paged_store",
+    "sah_paged_attention",
+    "sah_sample_tokens",
+)
 
 
 class NativeLibraryError(RuntimeError):
@@ -426,6 +434,88 @@ class AttentionWeightsArgs(C.Structure):
     ]
 
 
+class PagedAssignArgs(C.Structure):
+    _fields_ = [
+        ("new_lens", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("block_table", C.c_void_p), ("table_pitch", C.c_int64), ("table_width", C.c_int32),
+        ("free_pages", C.c_void_p),
+        ("free_count", C.c_void_p),
+        ("n_pages", C.c_int32),
+        ("n_requests", C.c_int32), ("page_size", C.c_int32), ("n_tokens", C.c_int32),
+        ("slot_map", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("cu_new", C.c_void_p),
+        ("kv_lens", C.c_void_p),
+        ("granted", C.c_void_p),
+        ("lens_out", C.c_void_p),
+        ("free_count_out", C.c_void_p),
+        ("work", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
+class PagedReleaseArgs(C.Structure):
+    _fields_ = [
+        ("finished", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("block_table", C.c_void_p), ("table_pitch", C.c_int64), ("table_width", C.c_int32),
+        ("free_pages", C.c_void_p),
+        ("free_count", C.c_void_p),
+        ("n_pages", C.c_int32),
+        ("n_requests", C.c_int32), ("page_size", C.c_int32),
+        ("work", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
+class PagedStoreArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("ks_t", C.c_int64), ("ks_h", C.c_int64),
+        ("v", C.c_void_p), ("vs_t", C.c_int64), ("vs_h", C.c_int64),
+        ("k_cache", C.c_void_p), ("kcs_p", C.c_int64), ("kcs_t", C.c_int64), ("kcs_h", C.c_int64),
+        ("v_cache", C.c_void_p), ("vcs_p", C.c_int64), ("vcs_t", C.c_int64), ("vcs_h", C.c_int64),
+        ("slot_map", C.c_void_p),
+        ("dtype", C.c_int32),
+        ("n_tokens", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+        ("stream", C.c_void_p),
+    ]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("qs_t", C.c_int64), ("qs_h", C.c_int64),
+        ("k", C.c_void_p), ("ks_p", C.c_int64), ("ks_t", C.c_int64), ("ks_h", C.c_int64),
+        ("v", C.c_void_p), ("vs_p", C.c_int64), ("vs_t", C.c_int64), ("vs_h", C.c_int64),
+        ("block_table", C.c_void_p), ("table_pitch", C.c_int64), ("table_width", C.c_int32),
+        ("kv_lens", C.c_void_p),
+        ("cu_new", C.c_void_p),
+        ("sinks", C.c_void_p),
+        ("dtype", C.c_int32),
+        ("n_requests", C.c_int32), ("n_tokens", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("n_pages", C.c_int32), ("page_size", C.c_int32),
+        ("max_context", C.c_int32), ("sink", C.c_int32), ("window", C.c_int32),
+        ("scaling", C.c_float),
+        ("out", C.c_void_p), ("os_t", C.c_int64), ("os_h", C.c_int64),
+        ("work", C.c_void_p), ("work_floats", C.c_int64),
+        ("stream", C.c_void_p),
+    ]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("row_pitch", C.c_int64),
+        ("dtype", C.c_int32),
+        ("n_rows", C.c_int32), ("vocab", C.c_int32),
+        ("uniforms", C.c_void_p), ("uniforms_f64", C.c_int32),
+        ("temperatures", C.c_void_p), ("top_ks", C.c_void_p), ("top_ps", C.c_void_p), ("min_ps", C.c_void_p),
+        ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float),
+        ("tokens", C.c_void_p),
+        ("logprobs", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
 _lib: Optional[C.CDLL] = None
 
 
@@ -449,7 +539,7 @@ def lib() -> C.CDLL:
         handle = C.CDLL(str(path))
     except OSError as e:
         raise NativeLibraryError(f"cannot load {path}: {e}") from e
-    missing = [s for s in EXPECTED_SYMBOLS if not hasattr(handle, s)]
+    missing = [s for s in (*EXPECTED_SYMBOLS, *SERVE_SYMBOLS) if not hasattr(handle, s)]
     if missing:
         raise NativeLibraryError(f"{path} lacks symbols {missing}; rebuild it")
     handle.sah_version.restype = C.c_int
@@ -483,6 +573,11 @@ def lib() -> C.CDLL:
     for name, n_blocks in EXTENSION_SYMBOLS.items():
         getattr(handle, name).restype = C.c_int
         getattr(handle, name).argtypes = [C.c_void_p] * n_blocks
+    for name in SERVE_SYMBOLS:
+        getattr(handle, name).restype = C.c_int
+        getattr(handle, name).argtypes = [C.c_void_p]
+    handle.sah_paged_attention_work_floats.restype = C.c_int64
+    handle.sah_paged_attention_work_floats.argtypes = [C.c_void_p]
     _lib = handle
     return handle
 
@@ -509,6 +604,15 @@ def call2(name: str, a: C.Structure, b: C.Structure) -> None:
         raise NativeLibraryError(f"{name}: {msg} (code {rc})")
 
 
+def call_on(device: torch.device, name: str, args: C.Structure) -> None:
+    """`call` with `device` as the current one: a kernel is launched on a stream of the current device."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, args)
+    else:
+        with torch.cuda.device(device):
+            call(name, args)
+
+
 def timing_enable(on: bool) -> None:
     """Switch the library's per-kernel HIP-event timing on or off (benchmarks only)."""
     lib().sah_timing_enable(1 if on else 0)
@@ -531,6 +635,10 @@ def work_floats(n_rows: int, max_cnt: int, head_dim: int) -> int:
 
 def members_work_floats(B: int, Hq: int, Hkv: int, Lq: int, Lk: int, head_dim: int) -> int:
     return int(lib().sah_members_attention_work_floats(B, Hq, Hkv, Lq, Lk, head_dim))
+
+
+def paged_work_floats(args: PagedAttentionArgs) -> int:
+    return int(lib().sah_paged_attention_work_floats(C.addressof(args)))
 
 
 def require_device(t: torch.Tensor, what: str) -> None:
