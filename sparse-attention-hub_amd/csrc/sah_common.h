@@ -300,6 +300,27 @@ __device__ __forceinline__ sah_f32x4 sah_mfma_16x16x32(uint4 a, uint4 b, sah_f32
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sah_f16x8, a), __builtin_bit_cast(sah_f16x8, b), c, 0, 0, 0);
 }
 
+// 16 bytes per lane from memory straight into LDS: the wave's 64 units land one after the other at `lds` (wave-uniform)
+__device__ __forceinline__ void sah_load_lds16(const void* p, void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+#else
+  (void)p; (void)lds;
+#endif
+}
+// Transposing LDS read, one 4 x 16 block of 16-bit elements per 16 lanes (layout checked on the hardware): lane l hands in
+// the address of row (l % 16) / 4, columns 4 (l % 4) .. + 3 and receives column l % 16, rows 0 .. 3.
+typedef uint32_t sah_u2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ sah_u2 sah_read_tr16(const uint16_t* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  const v4s r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)lds);
+  return __builtin_bit_cast(sah_u2, r);
+#else
+  return *(const sah_u2*)lds;
+#endif
+}
+
 // Pins a loaded value at this point of the program: the load that produced it must have
 // been issued (and is waited for) here, so the compiler can neither sink it into a later
 // branch nor serialise a batch of independent loads one wait at a time.
@@ -491,6 +512,11 @@ __device__ __forceinline__ float sah_half_min(float v) {
   uint32_t a, b;
   sah_half_both(sah_float_to_bits(v), a, b);
   return __builtin_elementwise_minimum(sah_bits_to_float(a), sah_bits_to_float(b));
+}
+__device__ __forceinline__ float sah_half_max(float v) {
+  uint32_t a, b;
+  sah_half_both(sah_float_to_bits(v), a, b);
+  return fmaxf(sah_bits_to_float(a), sah_bits_to_float(b));
 }
 __device__ __forceinline__ float sah_half_sum(float v) {
   uint32_t a, b;

@@ -1,38 +1,671 @@
-// Attention of new tokens over a key-value cache in pages.
+// Attention of new tokens over a key-value cache in pages, on the matrix cores.
+//
+// Of a request's new tokens and a key head's query heads every (token, head) is a row; PA_ROWS rows are a tile, which reads its
+// keys once. All tiles of all requests, one after the other, are one line of work (measured in keys); every workgroup takes
+// an equal piece of it, whatever the requests' lengths, finds its place from the lengths on the device, and works through
+// tiles and parts of tiles. A part's (m, l, acc) goes to the workspace, a second kernel joins the parts of a tile.
+//
+// A wave owns 32 rows: S^T = K Q^T puts row j in lanes j and j + 32 (16 of 32 keys each), so a row's maximum and sum need one exchange
+// between two lanes, and its weights are where the second product, O^T = V^T P^T, wants its B operand, with the key slots of a
+// 16-key step taken in the order [0-3][8-11] / [4-7][12-15]. fp32: the 32 x 32 x 2 form, whose operands are single elements.
+// Masked logits are replaced, not added to, so what a hidden key holds cannot reach them; keys that are not there (behind
+// the request's last, or on a missing page) are staged from one that is. A visible row's product with a value that is
+// not finite reaches the rows of its tile that do not see it (0 times it): rows that come out not finite are done again, key by key.
 #include "sah_common.h"
 #include "../../include/sah_serve.h"
 
-#define PA_NT 256
-#define PA_NW (PA_NT / SAH_WAVE)
 #define PA_MAX_D 256
+#define PA_CUS 256
+#define PA_XCDS 8
+#define PA_TILE_COST 96   // what starting and ending a tile costs, in keys
+#define PA_MIN_COST 256   // a workgroup's piece of the work is at least this long
 
-// A workgroup per row and head; its waves take keys in turn, each with a running maximum and sum of its own, joined in LDS.
-template <int DT>
-__global__ __launch_bounds__(PA_NT) void k_paged_attn(sah_paged_attention_args P) {
-  constexpr int E = PA_MAX_D / SAH_WAVE;
-  __shared__ float s_m[PA_NW], s_l[PA_NW], s_acc[PA_NW][PA_MAX_D];
-  const int t = blockIdx.x, h = blockIdx.y, hk = h / (P.Hq / P.Hkv);
-  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
-  int lo = 0, hi = P.n_requests;  // the first request whose rows end behind t
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (P.cu_new[mid + 1] > t) hi = mid; else lo = mid + 1;
+// Shape of a launch. RW waves share the keys of a stage, each with RB times 32 rows; RW = 1: every wave has keys of its own.
+template <int DT, int DP, bool WIDE>
+struct pa_shape {
+  static constexpr int ES = DT == SAH_F32 ? 4 : 2;
+  static constexpr int ROW = DP * ES;                      // bytes of a staged key
+  static constexpr int NW = WIDE ? 4 : (ROW <= 256 ? 4 : 1024 / ROW);
+  static constexpr int NT = NW * SAH_WAVE;
+  static constexpr int RB = 1;
+  static constexpr int RW = WIDE ? 4 : 1;
+  static constexpr int ROWS = 32 * RB * RW;
+  static constexpr int WKEYS = WIDE ? (ROW <= 512 ? 64 : 32) : 32;  // keys of a stage that a wave works on
+  static constexpr int STAGE = WIDE ? WKEYS : WKEYS * NW;
+  static constexpr int LDS = 4 * STAGE * ROW;              // K and V, two buffers
+  static constexpr int PER_CU = LDS <= 80 * 1024 ? 2 : 1;
+  static constexpr int WGS = PA_CUS * PER_CU;
+  static constexpr int SLOT = ROWS * (DP + 2);             // floats of a part
+};
+
+// ---------------------------------------------------------------------------
+// where the work is
+// ---------------------------------------------------------------------------
+struct pa_request {
+  int row0, n_new;   // its rows of q
+  int kv;            // keys it has
+  int64_t base;      // row t stands at position base + t
+};
+__device__ __forceinline__ pa_request pa_read_request(const sah_paged_attention_args& P, int b) {
+  pa_request r;
+  const int begin = P.cu_new[b], end = P.cu_new[b + 1];
+  int kv = P.kv_lens[b];
+  r.base = (int64_t)kv - end;
+  r.row0 = begin < 0 ? 0 : (begin < P.n_tokens ? begin : P.n_tokens);
+  const int e = end < P.n_tokens ? end : P.n_tokens;
+  r.n_new = e > r.row0 ? e - r.row0 : 0;
+  const int most = P.table_width * P.page_size;
+  r.kv = kv < 0 ? 0 : (kv < most ? kv : most);
+  return r;
+}
+// position of the request's i-th row, within what comparisons with key numbers need
+__device__ __forceinline__ int pa_position(const pa_request& r, int i) {
+  const int64_t p = r.base + r.row0 + i;
+  return (int)(p < -1 ? -1 : (p < 0x7ffffffe ? p : 0x7ffffffe));
+}
+
+// Cost of the tiles of one request and head: tile i's is min(first + (i + 1) step, most) + PA_TILE_COST. About the keys it
+// reads; only the balance depends on it.
+struct pa_cost {
+  int64_t first, step, most;
+  int tiles;
+  __device__ __forceinline__ int64_t of(int i) const {
+    const int64_t c = first + (i + 1) * step;
+    return (c < most ? c : most) + PA_TILE_COST;
   }
-  const int b = lo;
-  if (b >= P.n_requests || t < P.cu_new[b]) return;
-  int64_t kv = P.kv_lens[b];
-  const int64_t most = (int64_t)P.table_width * P.page_size;
-  const int64_t p = kv - (P.cu_new[b + 1] - t);
-  if (kv > most) kv = most;
-  const int64_t end = p + 1 < kv ? p + 1 : kv;
+  __device__ __forceinline__ int64_t before(int i) const {  // of tiles 0 .. i - 1
+    int64_t j = most > first ? (most - first) / step : 0;
+    if (j > i) j = i;
+    return j * first + step * (j * (j + 1) / 2) + (i - j) * most + (int64_t)i * PA_TILE_COST;
+  }
+  __device__ __forceinline__ int at(int64_t y) const {  // the tile whose piece of the line holds y
+    int lo = 0, hi = tiles - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (before(mid) <= y) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  }
+};
+template <int ROWS>
+__device__ __forceinline__ pa_cost pa_cost_of(const sah_paged_attention_args& P, const pa_request& r) {
+  const int G = P.Hq / P.Hkv;
+  pa_cost c;
+  c.tiles = (int)(((int64_t)r.n_new * G + ROWS - 1) / ROWS);
+  c.step = (ROWS + G - 1) / G;
+  const int64_t p = r.base + r.row0;
+  c.first = p < 0 ? 0 : (p < r.kv ? p : r.kv);
+  c.most = P.window ? (int64_t)P.sink + P.window + c.step : (int64_t)1 << 40;
+  return c;
+}
+
+// A place on the line of work: request, head, tile, and where the tile begins
+struct pa_place {
+  int b, hk, tile;
+  int64_t begin, cost;
+  pa_request req;
+  pa_cost costs;
+};
+
+__device__ __forceinline__ int64_t pa_uniform(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// The line's length, and how many workgroups share it. All NT threads call.
+template <int NT, int ROWS>
+__device__ __forceinline__ int64_t pa_total(const sah_paged_attention_args& P, int64_t* s_sum) {
+  int64_t sum = 0;
+  for (int b = threadIdx.x; b < P.n_requests; b += NT) {
+    const pa_cost c = pa_cost_of<ROWS>(P, pa_read_request(P, b));
+    sum += c.before(c.tiles);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor((long long)sum, d);
+  if (threadIdx.x % SAH_WAVE == 0) s_sum[threadIdx.x / SAH_WAVE] = sum;
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int i = 0; i < NT / SAH_WAVE; ++i) sum += s_sum[i];
+  __syncthreads();
+  return pa_uniform(sum * P.Hkv);
+}
+__device__ __forceinline__ int pa_sharers(int64_t total, int wgs) {
+  const int64_t w = (total + PA_MIN_COST - 1) / PA_MIN_COST;
+  return (int)(w < wgs ? w : wgs);
+}
+// where workgroup w of n begins
+__device__ __forceinline__ int64_t pa_bound(int64_t total, int n, int w) { return total / n * w + total % n * w / n; }
+
+// The place that holds x, 0 <= x < total. All NT threads call; s_sum: NT / 64 + 2 words.
+template <int NT, int ROWS>
+__device__ __forceinline__ pa_place pa_find(const sah_paged_attention_args& P, int64_t x, int64_t* s_sum) {
+  constexpr int NW = NT / SAH_WAVE;
+  const int lane = threadIdx.x % SAH_WAVE, wave = sah_wave_id();
+  int64_t run = 0;
+  for (int b0 = 0; b0 < P.n_requests; b0 += NT) {
+    const int b = b0 + threadIdx.x;
+    int64_t mine = 0;
+    if (b < P.n_requests) {
+      const pa_cost c = pa_cost_of<ROWS>(P, pa_read_request(P, b));
+      mine = c.before(c.tiles) * P.Hkv;
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int d = 1; d < SAH_WAVE; d <<= 1) {
+      const int64_t up = __shfl_up((long long)incl, d);
+      if (lane >= d) incl += up;
+    }
+    if (lane == SAH_WAVE - 1) s_sum[wave] = incl;
+    __syncthreads();
+    int64_t before = run, all = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      before += i < wave ? s_sum[i] : 0;
+      all += s_sum[i];
+    }
+    incl += before;
+    if (mine && incl > x && incl - mine <= x) {  // one thread
+      s_sum[NW] = b;
+      s_sum[NW + 1] = incl - mine;
+    }
+    run += all;
+    __syncthreads();
+    if (run > x) break;
+  }
+  pa_place at;
+  at.b = __builtin_amdgcn_readfirstlane((int)s_sum[NW]);
+  const int64_t begin = pa_uniform(s_sum[NW + 1]);
+  at.req = pa_read_request(P, at.b);
+  at.costs = pa_cost_of<ROWS>(P, at.req);
+  const int64_t head = at.costs.before(at.costs.tiles);
+  at.hk = (int)((x - begin) / head);
+  const int64_t y = x - begin - at.hk * head;
+  at.tile = at.costs.at(y);
+  at.begin = begin + at.hk * head + at.costs.before(at.tile);
+  at.cost = at.costs.of(at.tile);
+  return at;
+}
+// the next tile on the line; there is one
+template <int ROWS>
+__device__ __forceinline__ void pa_next(const sah_paged_attention_args& P, pa_place& at) {
+  at.begin += at.cost;
+  if (++at.tile == at.costs.tiles) {
+    at.tile = 0;
+    if (++at.hk == P.Hkv) {
+      at.hk = 0;
+      do {
+        ++at.b;
+        at.req = pa_read_request(P, at.b);
+        at.costs = pa_cost_of<ROWS>(P, at.req);
+      } while (at.costs.tiles == 0);
+    }
+  }
+  at.cost = at.costs.of(at.tile);
+}
+
+// what a workgroup leaves for the second kernel
+struct pa_note {
+  int b, hk, tile;  // the tile it began and others went on with; b < 0: none
+  int last;         // the workgroup that ended it
+  int again;        // some row of a whole tile came out not finite
+  int pad[3];
+};
+
+// The stages that a tile's rows see: the first n_sink ones, then those from `from` on; `n` in all
+struct pa_stages {
+  int n, n_sink, from;
+  __device__ __forceinline__ int operator()(int u) const { return u < n_sink ? u : u - n_sink + from; }
+};
+template <int STAGE>
+__device__ __forceinline__ pa_stages pa_stages_of(const sah_paged_attention_args& P, const pa_request& r, int p_lo, int p_hi) {
+  pa_stages s;
+  const int hi = p_hi < r.kv - 1 ? p_hi : r.kv - 1;  // the last key that any row sees
+  s.n_sink = 0;
+  s.from = 0;
+  if (hi < 0) {
+    s.n = 0;
+    return s;
+  }
+  const int last = hi / STAGE;
+  if (P.window) {
+    const int first = p_lo >= P.window ? p_lo - P.window + 1 : 0;
+    const int sink = P.sink < hi + 1 ? P.sink : hi + 1;
+    const int sinks = (int)(((int64_t)sink + STAGE - 1) / STAGE);
+    s.from = first / STAGE;
+    if (sinks < s.from) {
+      s.n_sink = sinks;
+      s.n = sinks + (s.from <= last ? last - s.from + 1 : 0);
+      return s;
+    }
+    s.from = 0;
+  }
+  s.n = last + 1;
+  return s;
+}
+
+// How far a row's maximum may rise, in powers of two, before the row is rescaled (a rise of the maximum by a little is frequent,
+// by 2^SLACK rare), and the power of two that the weights are held above their true size by: they enter the second product in
+// the tensor's type (half a step each, of independent signs: less than the result's own rounding), and fp16 keeps all its
+// bits for weights down to 2^-22 of the row's largest that way.
+template <int DT> struct pa_weights {
+  static constexpr float SLACK = DT == SAH_F16 ? 6.0f : 8.0f;
+  static constexpr float SCALE = DT == SAH_F16 ? 8.0f : 0.0f;
+};
+
+template <int DT, int DP, bool WIDE>
+__global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WIDE>::PER_CU)) void k_paged_attn(sah_paged_attention_args P) {
+  sah_touch_kernargs<sizeof(sah_paged_attention_args)>();
+  typedef pa_shape<DT, DP, WIDE> S;
+  constexpr int ES = S::ES, NT = S::NT, RB = S::RB, UNITS = S::ROW / 16;
+  constexpr int KPI = SAH_WAVE / (UNITS < 64 ? UNITS : 64);    // keys per load instruction
+  constexpr int IW = S::WKEYS / KPI / (WIDE ? S::NW : 1);      // load instructions per wave, matrix and stage
+  constexpr int TW = S::WKEYS / 32;                            // 32-key tiles a wave works on in a stage
+  constexpr int DTL = DP / 32;
+  constexpr int KQ = DT == SAH_F32 ? DP / 8 : DP / 16;         // 16-byte pieces of a lane's query
+  static_assert(UNITS <= 64 && IW >= 1, "a key is at most one load instruction");
+  // K and V as they lie in memory, a row per key, its 16-byte units permuted against bank conflicts: K unit c of key j at
+  // place c ^ (j % 16) (8 units: c ^ (j / 2 % 8)); V of 16-bit types: groups of four units (32 dims) at place
+  // u ^ (j % 4) (8 units: u ^ (j / 2 % 2)) for the transposing reads. (An array each: the compiler then knows that what is
+  // read is not what the loads under way will write.)
+  constexpr int SB = S::STAGE * S::ROW;
+  __shared__ __align__(16) unsigned char s_k0[SB], s_k1[SB], s_v0[SB], s_v1[SB];
+  __shared__ int64_t s_sum[S::NW + 2];
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
+  const int i32 = lane & 31, g = lane >> 5;
+  const int rw = WIDE ? wave : 0;
+  const int G = P.Hq / P.Hkv;
+  // neighbours on the line of work share keys: they get the same XCD
+  const int w = (int)(blockIdx.x % PA_XCDS) * (S::WGS / PA_XCDS) + (int)(blockIdx.x / PA_XCDS);
+  pa_note* notes = (pa_note*)P.work;
+  float* parts = P.work + S::WGS * (sizeof(pa_note) / 4);
+  const int64_t total = pa_total<NT, S::ROWS>(P, s_sum);
+  const int sharers = pa_sharers(total, S::WGS);
+  if (threadIdx.x == 0) {
+    notes[w].b = -1;
+    notes[w].again = 0;
+  }
+  if (w >= sharers) return;
+  const int64_t x1 = pa_bound(total, sharers, w + 1);
+  int64_t x = pa_bound(total, sharers, w);
+  pa_place at = pa_find<NT, S::ROWS>(P, x, s_sum);
+  const int page_shift = 31 - __builtin_clz(P.page_size);
+  const float c_exp = fmaxf(fabsf(P.scaling) * 1.4426950408889634f, 1e-37f);
+
+  // this lane's share of a load instruction, and where it reads what has been staged
+  const int l_key = lane / UNITS, l_place = lane % UNITS;
+  auto f_k = [](int key) { return UNITS == 8 ? (key >> 1) & 7 : key & 15; };
+  auto f_v = [](int key) { return DT == SAH_F32 ? 0 : UNITS == 8 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); };
+  const int units_real = P.D * ES / 16;
+  const int k_at = i32 * S::ROW + 16 * (g ^ f_k(i32));
+  int v_at[DTL];
+#pragma unroll
+  for (int t = 0; t < DTL; ++t) {
+    const int row = 4 * g + ((lane & 15) >> 2);
+    v_at[t] = row * S::ROW + 16 * ((4 * t) ^ f_v(row)) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  }
+
+  bool bad = false;  // a row of a whole tile came out not finite
+  for (;;) {
+    const int64_t y0 = x - at.begin, y1 = x1 - at.begin < at.cost ? x1 - at.begin : at.cost;
+    const bool whole = y0 == 0 && y1 == at.cost;
+    const int row_first = at.tile * S::ROWS;
+    const int n_rows = at.req.n_new * G;  // (n_new <= n_tokens, and n_tokens * Hq fits: the host has checked)
+    const int row_last = row_first + S::ROWS < n_rows ? row_first + S::ROWS - 1 : n_rows - 1;
+    const pa_stages stages = pa_stages_of<S::STAGE>(P, at.req, pa_position(at.req, row_first / G), pa_position(at.req, row_last / G));
+    const int u0 = (int)(y0 * stages.n / at.cost), u1 = y1 == at.cost ? stages.n : (int)(y1 * stages.n / at.cost);
+
+    // this lane's rows; lanes beyond the last repeat it and store nothing
+    int pos[RB], tok[RB], head[RB];
+    bool live[RB];
+    uint4 qf[RB][KQ];
+    bool wave_live = false;
+    int w_lo = 0x7fffffff, w_hi = -1;  // positions of the wave's rows
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const int r0 = row_first + (rw * RB + rb) * 32;
+      if (r0 < n_rows) {
+        wave_live = true;
+        const int r1 = r0 + 31 < n_rows ? r0 + 31 : n_rows - 1;
+        const int a = pa_position(at.req, r0 / G), z = pa_position(at.req, r1 / G);
+        w_lo = a < w_lo ? a : w_lo;
+        w_hi = z > w_hi ? z : w_hi;
+      }
+      const int r = r0 + i32;
+      live[rb] = r < n_rows;
+      const int rr = live[rb] ? r : n_rows - 1;
+      const int i = rr / G;
+      head[rb] = at.hk * G + rr - i * G;
+      tok[rb] = at.req.row0 + i;
+      pos[rb] = pa_position(at.req, i);
+      const char* qp = (const char*)P.q + ((int64_t)tok[rb] * P.qs_t + (int64_t)head[rb] * P.qs_h) * ES;
+#pragma unroll
+      for (int s = 0; s < KQ; ++s) {
+        const int unit = 2 * s + g;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (unit < units_real) v = *(const uint4*)(qp + 16 * unit);
+        if (P.scaling < 0.f) {  // uniform: the sign is the query's
+          const uint32_t sign = DT == SAH_F32 ? 0x80000000u : 0x80008000u;
+          v.x ^= sign; v.y ^= sign; v.z ^= sign; v.w ^= sign;
+        }
+        qf[rb][s] = v;
+      }
+    }
+    w_lo = __builtin_amdgcn_readfirstlane(w_lo);
+    w_hi = __builtin_amdgcn_readfirstlane(w_hi);
+
+    float m_run[RB], l_run[RB];
+    sah_f32x16 acc[RB][DTL];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      m_run[rb] = -INFINITY;
+      l_run[rb] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DTL; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[rb][t][e] = 0.f;
+    }
+
+    // The keys of a stage that this wave works on: a lane holds the page of one, and a bit says which are there. Requested a
+    // stage ahead of the loads that go by it.
+    const int32_t* table = P.block_table + (int64_t)at.b * P.table_pitch;
+    int page = -1, page_next = -1;
+    auto first_key = [&](int u) { return stages(u) * S::STAGE + (WIDE ? 0 : 32 * wave); };
+    auto fetch_page = [&](int u) -> int {
+      const int key = first_key(u) + (S::WKEYS == 64 ? lane : i32);
+      return key < at.req.kv ? table[key >> page_shift] : -1;
+    };
+    auto there_of = [&](int pg) -> uint64_t {
+      const uint64_t m = __ballot(pg >= 0 && pg < P.n_pages);
+      return S::WKEYS == 64 ? m : m & 0xffffffffu;
+    };
+    const char* kbase = (const char*)P.k + (int64_t)at.hk * P.ks_h * ES;
+    const char* vbase = (const char*)P.v + (int64_t)at.hk * P.vs_h * ES;
+    auto fetch = [&](int u, int pg, uint64_t there, int buf) __attribute__((always_inline)) {
+      const int key0 = first_key(u);
+      const int spare = 63 - __builtin_clzll(there | 1);  // stands for keys that are not there
+#pragma unroll
+      for (int i = 0; i < IW; ++i) {
+        const int at_key = ((WIDE ? wave * IW : 0) + i) * KPI;  // of the wave's keys; a wave with keys of its own stages all of them
+        const int key = at_key + l_key;
+        const int src = (there >> key) & 1 ? key : spare;
+        const int64_t p = there ? __shfl(pg, src) : 0;  // (nothing there: any page, and nobody reads it)
+        const int64_t entry = (key0 + src) & (P.page_size - 1);
+        const int uk = l_place ^ f_k(key), uv = l_place ^ f_v(key);
+        const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES + 16 * (uk < units_real ? uk : 0);
+        const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES + 16 * (uv < units_real ? uv : 0);
+        const int to = ((WIDE ? 0 : 32 * wave) + at_key) * S::ROW;
+        sah_load_lds16(ka, (buf ? s_k1 : s_k0) + to);
+        sah_load_lds16(va, (buf ? s_v1 : s_v0) + to);
+      }
+    };
+
+    auto work = [&](int u, uint64_t there, int buf) __attribute__((always_inline)) {
+      const int key0 = first_key(u);
+      if (!wave_live || there == 0 || key0 > w_hi) return;  // uniform
+      const unsigned char* kp = (buf ? s_k1 : s_k0) + (WIDE ? 0 : 32 * wave * S::ROW);
+      const unsigned char* vp = (buf ? s_v1 : s_v0) + (WIDE ? 0 : 32 * wave * S::ROW);
+      sah_f32x16 s[RB][TW];
+#pragma unroll
+      for (int t = 0; t < TW; ++t) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[rb][t][e] = 0.f;
+#pragma unroll
+        for (int st = 0; st < KQ; ++st) {
+          const uint4 a = *(const uint4*)(kp + 32 * t * S::ROW + (k_at ^ (32 * st)));
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            if constexpr (DT == SAH_F32) {
+              s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(a.x), sah_bits_to_float(qf[rb][st].x), s[rb][t]);
+              s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(a.y), sah_bits_to_float(qf[rb][st].y), s[rb][t]);
+              s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(a.z), sah_bits_to_float(qf[rb][st].z), s[rb][t]);
+              s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(a.w), sah_bits_to_float(qf[rb][st].w), s[rb][t]);
+            } else {
+              s[rb][t] = sah_mfma_32x32x16<DT>(a, qf[rb][st], s[rb][t]);
+            }
+          }
+        }
+      }
+      // every row sees every key of the stage?
+      const uint64_t full = S::WKEYS == 64 ? ~0ull : 0xffffffffull;
+      const bool plain = there == full && key0 + S::WKEYS - 1 <= w_lo &&
+                         (!P.window || key0 + S::WKEYS <= P.sink || (int64_t)key0 > (int64_t)w_hi - P.window);
+      if (!plain) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          const int lo = P.window && pos[rb] >= P.window ? pos[rb] - P.window + 1 : 0;
+#pragma unroll
+          for (int t = 0; t < TW; ++t) {
+            const int k0 = key0 + 32 * t, wi = k0 / 32;
+            uint32_t word = sah_range_bits(wi, lo, pos[rb] + 1);
+            if (P.window) word |= sah_range_bits(wi, 0, P.sink < pos[rb] + 1 ? P.sink : pos[rb] + 1);
+            word &= (uint32_t)(there >> (32 * t));
+            word >>= 4 * g;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[rb][t][e] = (word >> (8 * (e / 4) + e % 4)) & 1 ? s[rb][t][e] : -INFINITY;
+          }
+        }
+      }
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        float mx = s[rb][0][0];
+#pragma unroll
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[rb][t][e]);
+        mx = sah_half_max(mx) * c_exp;
+        // (-inf - -inf is NaN: no rise)
+        if (__ballot(mx - m_run[rb] > pa_weights<DT>::SLACK) != 0) {  // uniform: some row's maximum has risen too far
+          const float m_new = fmaxf(m_run[rb], mx);
+          const float up = m_run[rb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[rb] - m_new);
+          m_run[rb] = m_new;
+          l_run[rb] *= up;
+#pragma unroll
+          for (int t = 0; t < DTL; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[rb][t][e] *= up;
+        }
+        // (a row that has seen nothing: kept in range, so that -inf comes to 0)
+        const float mc = fmaxf(m_run[rb], -1e37f) - pa_weights<DT>::SCALE;
+#pragma unroll
+        for (int t = 0; t < TW; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[rb][t][e] = __builtin_amdgcn_exp2f(fmaf(s[rb][t][e], c_exp, -mc));
+            l_run[rb] += s[rb][t][e];
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < TW; ++t) {
+        if constexpr (DT == SAH_F32) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float* row = (const float*)(vp + (32 * t + 8 * (e / 4) + e % 4 + 4 * g) * S::ROW) + i32;
+#pragma unroll
+            for (int d = 0; d < DTL; ++d) {
+              const float v = row[32 * d];
+#pragma unroll
+              for (int rb = 0; rb < RB; ++rb) acc[rb][d] = sah_mfma_32x32x2_f32(v, s[rb][t][e], acc[rb][d]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            uint4 pt[RB];
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              const auto& z = s[rb][t];
+              pt[rb] = make_uint4(sah_pack2_hw<DT>(z[8 * st], z[8 * st + 1]), sah_pack2_hw<DT>(z[8 * st + 2], z[8 * st + 3]),
+                                  sah_pack2_hw<DT>(z[8 * st + 4], z[8 * st + 5]), sah_pack2_hw<DT>(z[8 * st + 6], z[8 * st + 7]));
+            }
+#pragma unroll
+            for (int d = 0; d < DTL; ++d) {
+              const unsigned char* v = vp + (32 * t + 16 * st) * S::ROW + v_at[d];
+              const sah_u2 a0 = sah_read_tr16((const uint16_t*)v), a1 = sah_read_tr16((const uint16_t*)(v + 8 * S::ROW));
+              const uint4 va = make_uint4(a0.x, a0.y, a1.x, a1.y);
+#pragma unroll
+              for (int rb = 0; rb < RB; ++rb) acc[rb][d] = sah_mfma_32x32x16<DT>(va, pt[rb], acc[rb][d]);
+            }
+          }
+        }
+      }
+    };
+
+    auto stage = [&](int u, int buf) __attribute__((always_inline)) {  // buf: a constant in the loop below
+      const uint64_t there = there_of(page);
+      if (u + 1 < u1) {
+        page = page_next;
+        fetch(u + 1, page, there_of(page), buf ^ 1);  // the other buffer: read for the last time before the previous wait
+        if (u + 2 < u1) page_next = fetch_page(u + 2);
+      }
+      work(u, there, buf);
+      sah_stores_done();  // this wave's loads into LDS have landed
+      if (WIDE) __syncthreads();
+      else sah_wave_lds_sync();
+    };
+    if (u0 < u1) {
+      page = fetch_page(u0);
+      if (u0 + 1 < u1) page_next = fetch_page(u0 + 1);
+      fetch(u0, page, there_of(page), 0);
+      sah_stores_done();
+      if (WIDE) __syncthreads();
+      else sah_wave_lds_sync();
+      for (int u = u0; u < u1; u += 2) {
+        stage(u, 0);
+        if (u + 1 < u1) stage(u + 1, 1);
+      }
+    }
+
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) l_run[rb] = sah_half_sum(l_run[rb]);
+    if constexpr (!WIDE && S::NW > 1) {
+      // the waves' shares of the keys are joined in LDS
+      __syncthreads();  // every wave has read its stages
+      constexpr int PER = SB / (16 * DTL * SAH_WAVE * 4);  // waves' tiles, [element][lane], that a buffer holds
+      static_assert(PER >= 1 && PER * 4 >= S::NW - 1 && RB == 1, "room for the waves' tiles");
+      auto tile_of = [&](int v) -> float* {
+        unsigned char* base = v / PER == 0 ? s_k0 : v / PER == 1 ? s_k1 : v / PER == 2 ? s_v0 : s_v1;
+        return (float*)base + (v % PER) * 16 * DTL * SAH_WAVE;
+      };
+      __shared__ float s_ml[S::NW][2][SAH_WAVE];
+      if (wave) {
+        float* to = tile_of(wave - 1);
+#pragma unroll
+        for (int t = 0; t < DTL; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) to[(16 * t + e) * SAH_WAVE + lane] = acc[0][t][e];
+        s_ml[wave][0][lane] = m_run[0];
+        s_ml[wave][1][lane] = l_run[0];
+      }
+      __syncthreads();
+      if (wave == 0) {
+        float m_new = m_run[0];
+#pragma unroll
+        for (int v = 1; v < S::NW; ++v) m_new = fmaxf(m_new, s_ml[v][0][lane]);
+        float up = m_run[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[0] - m_new);
+        l_run[0] *= up;
+#pragma unroll
+        for (int t = 0; t < DTL; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[0][t][e] *= up;
+#pragma unroll
+        for (int v = 1; v < S::NW; ++v) {
+          const float mv = s_ml[v][0][lane];
+          up = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - m_new);
+          l_run[0] += s_ml[v][1][lane] * up;
+          const float* from = tile_of(v - 1);
+#pragma unroll
+          for (int t = 0; t < DTL; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[0][t][e] += from[(16 * t + e) * SAH_WAVE + lane] * up;
+        }
+        m_run[0] = m_new;
+      }
+    }
+    if (WIDE || wave == 0) {
+      if (whole) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          float l = l_run[rb];
+          if (P.sinks) {
+            // a row that has seen nothing has nothing to weigh against its sink
+            const float z = fmaf(P.sinks[head[rb]], 1.4426950408889634f, pa_weights<DT>::SCALE) - m_run[rb];
+            if (m_run[rb] != -INFINITY) l += __builtin_amdgcn_exp2f(z);
+          }
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          bool fine = true;
+          char* op = (char*)P.out + ((int64_t)tok[rb] * P.os_t + (int64_t)head[rb] * P.os_h) * ES;
+#pragma unroll
+          for (int t = 0; t < DTL; ++t)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              const int d = 32 * t + 8 * q4 + 4 * g;
+              if (d >= P.D) continue;
+              float o[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                o[e] = acc[rb][t][4 * q4 + e] * inv;
+                fine = fine && fabsf(o[e]) < INFINITY;
+              }
+              if (!live[rb]) continue;
+              if (DT == SAH_F32) *(float4*)(op + 4 * d) = make_float4(o[0], o[1], o[2], o[3]);
+              else *(uint2*)(op + 2 * d) = make_uint2(sah_pack2_hw<DT>(o[0], o[1]), sah_pack2_hw<DT>(o[2], o[3]));
+            }
+          bad = bad || (live[rb] && !fine);
+        }
+      } else {
+        // a part: to slot 0 where the tile began before this workgroup's piece, else to slot 1
+        float* to = parts + (int64_t)(2 * w + (y0 ? 0 : 1)) * S::SLOT;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          const int r = (rw * RB + rb) * 32 + i32;
+          if (!live[rb]) continue;
+          if (g == 0) ((float2*)to)[r] = make_float2(m_run[rb], l_run[rb]);
+          float* o = to + 2 * S::ROWS + r * DP;
+#pragma unroll
+          for (int t = 0; t < DTL; ++t)
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+              *(float4*)(o + 32 * t + 8 * q4 + 4 * g) = make_float4(acc[rb][t][4 * q4], acc[rb][t][4 * q4 + 1], acc[rb][t][4 * q4 + 2], acc[rb][t][4 * q4 + 3]);
+        }
+        if (y0 == 0 && threadIdx.x == 0) {
+          // the workgroup whose piece holds the tile's last key: the first whose end is not before the tile's
+          const int64_t end = at.begin + at.cost;
+          int last = (int)((end * sharers - 1) / total);
+          while (last + 1 < sharers && pa_bound(total, sharers, last + 1) < end) ++last;
+          while (last > w && pa_bound(total, sharers, last) >= end) --last;
+          notes[w].hk = at.hk;
+          notes[w].tile = at.tile;
+          notes[w].last = last;
+          notes[w].b = at.b;
+        }
+      }
+    }
+    x = at.begin + y1;
+    if (x >= x1) break;
+    if (!WIDE) __syncthreads();  // wave 0 has read the others' shares
+    pa_next<S::ROWS>(P, at);
+  }
+  if (bad) notes[w].again = 1;
+}
+
+// One row key by key, by one wave: what a row holds whose products in a tile came out not finite.
+template <int DT>
+__device__ __forceinline__ void pa_row_again(const sah_paged_attention_args& P, const pa_request& r, int b, int t, int h) {
+  constexpr int E = PA_MAX_D / SAH_WAVE;
+  const int lane = threadIdx.x & (SAH_WAVE - 1), hk = h / (P.Hq / P.Hkv);
+  const int64_t p = r.base + t;
+  const int64_t end = p + 1 < r.kv ? p + 1 : r.kv;
   float q[E], acc[E], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane + e * SAH_WAVE;
-    q[e] = d < P.D ? sah_load<DT>(P.q, (int64_t)t * P.qs_t + h * P.qs_h + d) * P.scaling : 0.f;
+    q[e] = d < P.D ? sah_load<DT>(P.q, (int64_t)t * P.qs_t + (int64_t)h * P.qs_h + d) : 0.f;
     acc[e] = 0.f;
   }
-  for (int64_t j = wave; j < end; j += PA_NW) {
+  for (int64_t j = 0; j < end; ++j) {
     if (P.window > 0 && j >= P.sink && j <= p - P.window) continue;
     const int page = P.block_table[(int64_t)b * P.table_pitch + j / P.page_size];
     if (page < 0 || page >= P.n_pages) continue;
@@ -44,7 +677,7 @@ __global__ __launch_bounds__(PA_NT) void k_paged_attn(sah_paged_attention_args P
       const int d = lane + e * SAH_WAVE;
       if (d < P.D) s = fmaf(q[e], sah_load<DT>(P.k, ka + d), s);
     }
-    s = sah_wave_sum(s);
+    s = sah_wave_sum(s) * P.scaling;
     const float m_new = fmaxf(m, s);
     if (m_new == -INFINITY && s == s) continue;  // (a NaN is no maximum, but the row's result)
     const float up = expf(m - m_new), w = expf(s - m_new);
@@ -56,28 +689,158 @@ __global__ __launch_bounds__(PA_NT) void k_paged_attn(sah_paged_attention_args P
       if (d < P.D) acc[e] = acc[e] * up + w * sah_load<DT>(P.v, va + d);
     }
   }
-  if (lane == 0) { s_m[wave] = m; s_l[wave] = l; }
+  if (P.sinks && m != -INFINITY) l += expf(P.sinks[h] - m);
 #pragma unroll
-  for (int e = 0; e < E; ++e) s_acc[wave][lane + e * SAH_WAVE] = acc[e];
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= P.D) return;
-  const float sink = P.sinks ? P.sinks[h] : -INFINITY;
-  float M = sink;
-  for (int w = 0; w < PA_NW; ++w) M = fmaxf(M, s_m[w]);
-  float L = sink == -INFINITY ? 0.f : expf(sink - M), o = 0.f;
-  for (int w = 0; w < PA_NW; ++w) {
-    const float up = s_m[w] == -INFINITY ? 0.f : expf(s_m[w] - M);
-    L += s_l[w] * up;
-    o += s_acc[w][d] * up;
+  for (int e = 0; e < E; ++e) {
+    const int d = lane + e * SAH_WAVE;
+    if (d < P.D) sah_store<DT>(P.out, (int64_t)t * P.os_t + (int64_t)h * P.os_h + d, l == 0.f ? 0.f : acc[e] / l);
   }
-  sah_store<DT>(P.out, (int64_t)t * P.os_t + h * P.os_h + d, L == 0.f ? 0.f : o / L);
+}
+
+// Joins the parts of the tile that workgroup blockIdx.x of the first kernel began and did not end, a row per wave (many parts: a
+// row per workgroup, its waves taking parts in turn). Row blocks go to blockIdx.y.
+#define PA_JOIN_NT 256
+#define PA_JOIN_ROWS 8     // workgroups that share a tile's rows
+template <int DT, int DP, bool WIDE>
+__global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attention_args P) {
+  typedef pa_shape<DT, DP, WIDE> S;
+  constexpr int NW = PA_JOIN_NT / SAH_WAVE, E = DP / SAH_WAVE;
+  __shared__ float s_m[NW], s_l[NW], s_acc[NW][DP];
+  __shared__ int64_t s_sum[NW + 2];
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
+  const int w = blockIdx.x, G = P.Hq / P.Hkv;
+  const pa_note note = ((const pa_note*)P.work)[w];
+  const float* parts = P.work + S::WGS * (sizeof(pa_note) / 4);
+  if (note.b >= 0) {
+    const pa_request req = pa_read_request(P, note.b);
+    const int n_rows = req.n_new * G, n_parts = note.last - w + 1;
+    const bool many = n_parts > 8;
+    for (int i = many ? (int)blockIdx.y : (int)blockIdx.y * NW + wave; i < S::ROWS; i += many ? PA_JOIN_ROWS : PA_JOIN_ROWS * NW) {
+      const int r = note.tile * S::ROWS + i;
+      if (r >= n_rows) break;  // (uniform across the workgroup where it matters: many)
+      const int first = many ? wave : 0, step = many ? NW : 1;
+      float m = -INFINITY, l = 0.f, acc[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+      for (int p = first; p < n_parts; p += step) {
+        const float* from = parts + (int64_t)(p ? 2 * (w + p) : 2 * w + 1) * S::SLOT;
+        const float2 ml = ((const float2*)from)[i];
+        const float m_new = fmaxf(m, ml.x);
+        const float a = m == -INFINITY ? 0.f : exp2f(m - m_new), z = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m_new);
+        // (a part whose sums are NaN without a maximum: the row is done again)
+        l = l * a + (ml.y == ml.y ? ml.y * z : ml.y);
+        m = m_new;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * a + z * from[2 * S::ROWS + i * DP + lane + e * SAH_WAVE];
+      }
+      if (many) {
+        __syncthreads();
+        if (lane == 0) { s_m[wave] = m; s_l[wave] = l; }
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_acc[wave][lane + e * SAH_WAVE] = acc[e];
+        __syncthreads();
+        if (wave) continue;
+#pragma unroll
+        for (int v = 1; v < NW; ++v) {
+          const float m_new = fmaxf(m, s_m[v]);
+          const float a = m == -INFINITY ? 0.f : exp2f(m - m_new), z = s_m[v] == -INFINITY ? 0.f : exp2f(s_m[v] - m_new);
+          l = l * a + (s_l[v] == s_l[v] ? s_l[v] * z : s_l[v]);
+          m = m_new;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = acc[e] * a + z * s_acc[v][lane + e * SAH_WAVE];
+        }
+      }
+      const int tok = req.row0 + r / G, h = note.hk * G + r % G;
+      bool fine = l == l;
+      if (P.sinks && m != -INFINITY) l += exp2f(fmaf(P.sinks[h], 1.4426950408889634f, pa_weights<DT>::SCALE) - m);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int d = lane + e * SAH_WAVE;
+        if (d >= P.D) continue;
+        acc[e] *= inv;
+        fine = fine && fabsf(acc[e]) < INFINITY;
+        sah_store<DT>(P.out, (int64_t)tok * P.os_t + (int64_t)h * P.os_h + d, acc[e]);
+      }
+      if (__ballot(!fine)) pa_row_again<DT>(P, req, note.b, tok, h);
+    }
+  }
+  if (!note.again) return;  // uniform
+  // rows of whole tiles that came out not finite: the first kernel's walk once more
+  const int64_t total = pa_total<PA_JOIN_NT, S::ROWS>(P, s_sum);
+  const int sharers = pa_sharers(total, S::WGS);
+  const int64_t x0 = pa_bound(total, sharers, w), x1 = pa_bound(total, sharers, w + 1);
+  pa_place at = pa_find<PA_JOIN_NT, S::ROWS>(P, x0, s_sum);
+  for (;;) {
+    if (at.begin >= x0 && at.begin + at.cost <= x1) {
+      const int n_rows = at.req.n_new * G;
+      for (int i = (int)blockIdx.y * NW + wave; i < S::ROWS; i += PA_JOIN_ROWS * NW) {
+        const int r = at.tile * S::ROWS + i;
+        if (r >= n_rows) break;
+        const int tok = at.req.row0 + r / G, h = at.hk * G + r % G;
+        bool fine = true;
+        for (int d = lane; d < P.D; d += SAH_WAVE)
+          fine = fine && fabsf(sah_load<DT>(P.out, (int64_t)tok * P.os_t + (int64_t)h * P.os_h + d)) < INFINITY;
+        if (__ballot(!fine)) pa_row_again<DT>(P, at.req, at.b, tok, h);
+      }
+    }
+    if (at.begin + at.cost >= x1) break;
+    pa_next<S::ROWS>(P, at);
+  }
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-extern "C" int64_t sah_paged_attention_work_floats(const sah_paged_attention_args* a) { (void)a; return 0; }
+// Tiles of 128 rows whose waves share the keys, or of 32 rows whose waves each take keys of their own: by the rows per request.
+static bool pa_wide(const sah_paged_attention_args* a) {
+  return (int64_t)a->n_tokens * (a->Hq / a->Hkv) > 32 * (int64_t)a->n_requests;
+}
+
+template <int DT, int DP, bool WIDE>
+static int64_t pa_floats() {
+  typedef pa_shape<DT, DP, WIDE> S;
+  return S::WGS * (int64_t)(sizeof(pa_note) / 4) + 2 * (int64_t)S::WGS * S::SLOT;
+}
+
+template <int DT, int DP, bool WIDE>
+static int pa_launch(const sah_paged_attention_args* a) {
+  typedef pa_shape<DT, DP, WIDE> S;
+  hipStream_t st = (hipStream_t)a->stream;
+  {
+    sah_timed timed("k_paged_attn", a->stream);
+    hipLaunchKernelGGL((k_paged_attn<DT, DP, WIDE>), dim3(S::WGS), dim3(S::NT), 0, st, *a);
+    if (int rc = sah_launch_status("sah_paged_attention")) return rc;
+  }
+  sah_timed timed("k_paged_attn_join", a->stream);
+  hipLaunchKernelGGL((k_paged_attn_join<DT, DP, WIDE>), dim3(S::WGS, PA_JOIN_ROWS), dim3(PA_JOIN_NT), 0, st, *a);
+  return sah_launch_status("sah_paged_attention(join)");
+}
+
+// calls f with the instance that a call takes
+template <typename F>
+static int64_t pa_dispatch(const sah_paged_attention_args* a, F f) {
+  const bool wide = pa_wide(a);
+  const int dp = a->D <= 64 ? 64 : a->D <= 128 ? 128 : 256;
+#define PA_CASE(dt, d) if (a->dtype == dt && dp == d) return wide ? f.template operator()<dt, d, true>() : f.template operator()<dt, d, false>();
+  PA_CASE(SAH_BF16, 64) PA_CASE(SAH_BF16, 128) PA_CASE(SAH_BF16, 256)
+  PA_CASE(SAH_F16, 64) PA_CASE(SAH_F16, 128) PA_CASE(SAH_F16, 256)
+  PA_CASE(SAH_F32, 64) PA_CASE(SAH_F32, 128) PA_CASE(SAH_F32, 256)
+#undef PA_CASE
+  return 0;
+}
+struct pa_floats_fn {
+  template <int DT, int DP, bool WIDE> int64_t operator()() const { return pa_floats<DT, DP, WIDE>(); }
+};
+struct pa_launch_fn {
+  const sah_paged_attention_args* a;
+  template <int DT, int DP, bool WIDE> int64_t operator()() const { return pa_launch<DT, DP, WIDE>(a); }
+};
+
+extern "C" int64_t sah_paged_attention_work_floats(const sah_paged_attention_args* a) {
+  if (!a || a->n_tokens <= 0 || a->n_requests <= 0 || a->Hkv <= 0 || a->Hq < a->Hkv || a->D <= 0 || a->D > PA_MAX_D) return 0;
+  return pa_dispatch(a, pa_floats_fn());
+}
 
 extern "C" int sah_paged_attention(const sah_paged_attention_args* a) {
   if (!a) return sah_fail(SAH_ENULL, "sah_paged_attention: args is NULL");
@@ -89,20 +852,18 @@ extern "C" int sah_paged_attention(const sah_paged_attention_args* a) {
   if (a->D <= 0 || a->D % 8 || a->D > PA_MAX_D) return sah_fail(SAH_ESHAPE, "sah_paged_attention: head_dim %d is not a multiple of 8 up to 256", a->D);
   if (a->page_size <= 0 || (a->page_size & (a->page_size - 1))) return sah_fail(SAH_ESHAPE, "sah_paged_attention: page_size %d is not a power of two", a->page_size);
   if ((int64_t)a->table_width * a->page_size > INT32_MAX) return sah_fail(SAH_ESHAPE, "sah_paged_attention: table_width * page_size passes 2^31");
+  if ((int64_t)a->n_tokens * a->Hq > 1 << 30) return sah_fail(SAH_ESHAPE, "sah_paged_attention: n_tokens * Hq passes 2^30");
+  // the line of work is measured in 64 bits, also where running sums overlap
+  if (((double)a->n_tokens * (a->Hq / a->Hkv) / 32 + 1) * ((double)a->table_width * a->page_size + 1024) * a->Hkv * a->n_requests > 0x1p61)
+    return sah_fail(SAH_ESHAPE, "sah_paged_attention: too much work for one call");
   if (a->table_pitch < a->table_width) return sah_fail(SAH_EINVAL, "sah_paged_attention: table_pitch is less than table_width");
   if (a->n_tokens == 0) return SAH_OK;
   if (!a->q || !a->k || !a->v || !a->block_table || !a->kv_lens || !a->cu_new || !a->out) return sah_fail(SAH_ENULL, "sah_paged_attention: NULL pointer");
-  if (a->Hq > 65535) return sah_fail(SAH_ESHAPE, "sah_paged_attention: %d heads", a->Hq);
   const int es = a->dtype == SAH_F32 ? 4 : 2;
-  if (((uint64_t)a->q | (uint64_t)a->k | (uint64_t)a->v | (uint64_t)a->out |
+  if (((uint64_t)a->q | (uint64_t)a->k | (uint64_t)a->v | (uint64_t)a->out | (uint64_t)a->work |
        (uint64_t)(es * (a->qs_t | a->qs_h | a->ks_p | a->ks_t | a->ks_h | a->vs_p | a->vs_t | a->vs_h | a->os_t | a->os_h))) % 16)
     return sah_fail(SAH_EINVAL, "sah_paged_attention: addresses and strides must be multiples of 16 bytes");
-  if (!(a->scaling == a->scaling)) return sah_fail(SAH_EINVAL, "sah_paged_attention: scaling is NaN");
-  hipStream_t st = (hipStream_t)a->stream;
-  sah_timed timed("k_paged_attn", a->stream);
-  const dim3 grid(a->n_tokens, a->Hq);
-  if (a->dtype == SAH_F32) hipLaunchKernelGGL(k_paged_attn<SAH_F32>, grid, dim3(PA_NT), 0, st, *a);
-  else if (a->dtype == SAH_BF16) hipLaunchKernelGGL(k_paged_attn<SAH_BF16>, grid, dim3(PA_NT), 0, st, *a);
-  else hipLaunchKernelGGL(k_paged_attn<SAH_F16>, grid, dim3(PA_NT), 0, st, *a);
-  return sah_launch_status("sah_paged_attention");
+  if (!(a->scaling - a->scaling == 0.f)) return sah_fail(SAH_EINVAL, "sah_paged_attention: scaling is not finite");
+  if (!a->work || a->work_floats < sah_paged_attention_work_floats(a)) return sah_fail(SAH_ECAPACITY, "sah_paged_attention: work is too small");
+  return (int)pa_dispatch(a, pa_launch_fn{a});
 }

@@ -28,7 +28,7 @@
 #define QA_MIN_WGS 512   // keys are split until there are this many workgroups (two per CU: one round) ...
 #define QA_MIN_STAGES 8  // ... of at least this many stages (a partial result costs as much as half a stage to write and merge)
 typedef uint32_t qa_u4 __attribute__((ext_vector_type(4)));
-typedef uint32_t qa_u2 __attribute__((ext_vector_type(2)));
+typedef sah_u2 qa_u2;
 typedef qa_u2 qa_u2_any __attribute__((aligned(2)));  // 8 bytes at an address that is only element aligned
 typedef qa_u4 qa_u4_any __attribute__((aligned(2)));
 typedef qa_u2 qa_u2_word __attribute__((aligned(4)));
@@ -38,26 +38,6 @@ struct qa_params {
   int stages_per_split;
   int row_tiles;       // workgroups along the rows of a KV head
 };
-
-// 16 bytes per lane from memory straight into LDS: the wave's 64 units land one after the other at `lds` (wave-uniform)
-__device__ __forceinline__ void qa_load_lds(const void* p, void* lds) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
-#else
-  (void)p; (void)lds;
-#endif
-}
-// Transposing LDS read, one 4 x 16 block of 16-bit elements per 16 lanes (layout checked on the hardware): lane l hands in
-// the address of row (l % 16) / 4, columns 4 (l % 4) .. + 3 and receives column l % 16, rows 0 .. 3.
-__device__ __forceinline__ qa_u2 qa_read_tr(const uint16_t* lds) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  typedef short v4s __attribute__((ext_vector_type(4)));
-  const v4s r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s*)lds);
-  return __builtin_bit_cast(qa_u2, r);
-#else
-  return *(const qa_u2*)lds;
-#endif
-}
 
 // How far a row's maximum may rise, in powers of two, before the row is rescaled: the weights are then at most 2^SLACK
 // relative to the maximum in use, which costs a floating-point sum nothing. A row's maximum rises in most of the few
@@ -204,9 +184,9 @@ __global__ __launch_bounds__(QA_NT, 2) void k_members_attn_mfma(att_params P, qa
     const char* ks = kbase + (int64_t)st * QA_STAGE * P.ks_l * 2;
     const char* vs = vbase + (int64_t)st * QA_STAGE * P.vs_l * 2;
 #pragma unroll
-    for (int u = 0; u < UW; ++u) qa_load_lds(ks + ko[u], (buf ? s_k1 : s_k0) + (wave * UW + u) * KPW * D);
+    for (int u = 0; u < UW; ++u) sah_load_lds16(ks + ko[u], (buf ? s_k1 : s_k0) + (wave * UW + u) * KPW * D);
 #pragma unroll
-    for (int u = 0; u < UW; ++u) qa_load_lds(vs + vo[u], (buf ? s_v1 : s_v0) + (wave * UW + u) * KPW * D);
+    for (int u = 0; u < UW; ++u) sah_load_lds16(vs + vo[u], (buf ? s_v1 : s_v0) + (wave * UW + u) * KPW * D);
   };
   // where this lane reads. K: key row i32 of a tile, unit 2 s + g. V (transposed): for the four keys from 4 g on of a
   // 16-key step, row (lane % 16) / 4 of them, dims 32 t + 16 (lane / 16 % 2) + 4 (lane % 4) .. + 3
@@ -292,7 +272,7 @@ __global__ __launch_bounds__(QA_NT, 2) void k_members_attn_mfma(att_params P, qa
 #pragma unroll
       for (int t = 0; t < DTL; ++t) {
         const uint16_t* vp = (buf ? s_v1 : s_v0) + (t32 * 32 + 16 * st) * D + v_from[t];
-        const qa_u2 a0 = qa_read_tr(vp), a1 = qa_read_tr(vp + 8 * D);
+        const qa_u2 a0 = sah_read_tr16(vp), a1 = sah_read_tr16(vp + 8 * D);
         va[t] = make_uint4(a0.x, a0.y, a1.x, a1.y);
       }
       constexpr int TERMS = qa_weights<DT>::TERMS;
