@@ -1,9 +1,15 @@
 // The next token of each row of logits from one given random number.
 //
-// In the order of falling logits (ties to the lower index) top-k and top-p both keep a first part, so both are a threshold:
-// the keys (order-preserving, sah_sort_key) above one value, and of those equal to it the first few by index. Weights are
-// exp((x - m) / t) in fp64, summed as integers of 2^-43: sums of up to 2^20 of them fit 64 bits, are exact, and so do not
-// depend on who adds when.
+// In the order of falling logits (ties to the lower index) top-k and top-p both keep a first part, so both are a last kept
+// token. Weights are exp((x - m) / t) in fp64, summed as integers of 2^-43: sums of up to 2^20 of them fit 64 bits, are
+// exact, and so do not depend on who adds when.
+//
+// A workgroup has a row. Everything that decides is a selection of one kind: of weighted items in an order, the one at which the
+// running weight reaches a target: the k-th largest (weight 1), top-p's last (a token's weight), the drawn token (the same in
+// the order of the index). Weights are added up per piece of the order's range in LDS, the few items of the piece that holds the target
+// are ranked by a wave (sm_pick). It runs over a list in LDS of all tokens that may be kept, where that can hold them: what may
+// be kept is known early, since where r of 1024 threads' own largest logits reach a value, at least r of the row do, and few
+// more. Where it cannot, the row is cut into pieces of 1 / SM_FINE in (m - x) / t first, and the list holds one of them.
 #include "sah_common.h"
 #include "../../include/sah_serve.h"
 
@@ -11,83 +17,103 @@
 #define SM_NW (SM_NT / SAH_WAVE)
 #define SM_ONE 0x1p43
 #define SM_MAX_VOCAB (1 << 20)
-
-// A workgroup has a row. Everything that decides is a selection of one kind: of weighted items in an order, the one at which the
-// running weight reaches a target (sm_select: a digit at a time, weights added up per digit value in LDS): the k-th largest
-// (weight 1), top-p's border (a token's weight), the drawn token (the same in the order of the index). It runs over a list in LDS where that can
-// hold every token that may be kept, over the row itself where not. What may be kept is known early: of 1024 threads' own
-// largest logits at least r values reach the r-th largest, so at least r of the row do, and few more.
 #define SM_CAP 8192        // tokens of the list
 #define SM_BINS 2048
+#define SM_SMALL 64        // items that are ranked at once, one a lane
+#define SM_FINE 64.f
 #define SM_RANK_K 1000     // top-k up to this goes by the threads' largest logits (1024 ln(1024 / 24) = 3800 tokens on average) ...
 #define SM_RANK_P 1021     // ... and top-p tries the tokens above this one of them (6000)
+#define SM_LOWEST 0x00800000u  // order of the lowest finite logit
 typedef sah_u4 sm_vec __attribute__((aligned(2)));
 
 struct sm_shared {
-  uint2 list[SM_CAP];      // (float bits, index); or the row's segments' sums
-  uint64_t bins[SM_BINS];
-  double table[64];        // 2^(j / 64)
+  uint2 list[SM_CAP];         // (float bits, index); or the row's segments' sums
+  uint64_t bins[SM_BINS];     // zero between uses
   uint64_t wave_sum[SM_NW];
-  uint64_t found[4];
-  float wave_max[SM_NW];
+  uint64_t small_weight[SM_SMALL];
+  uint2 small[SM_SMALL];      // (order, index)
+  uint64_t found_before;
+  int found_bin;
+  int n_small[2];
+  float wave_max[SM_NW], wave_low[SM_NW];
   int wave_at[SM_NW];
   int count;
 };
 
-// order-preserving, above 0 for every logit above -inf; equal logits (0 and -0 too) share one
+// order-preserving; equal logits (0 and -0 too) share one
 __device__ __forceinline__ uint32_t sm_order(float v) { return sah_sort_key<SAH_F32>(v); }
 __device__ __forceinline__ float sm_value(uint32_t order) { return sah_bits_to_float((order & 0x80000000u) ? order ^ 0x80000000u : ~order); }
 
-// Weights of a row: exp(-d / t) = 2^(n / 64) * exp(f) with |f| <= ln 2 / 128, exp(f) by its series to the fourth power (off by 4e-14)
+// a b + c with c in a scalar register. (Left to itself the compiler accumulates onto c, a copy of it for every product.)
+__device__ __forceinline__ double sm_fma(double a, double b, double c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  double r;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+  return r;
+#else
+  return a * b + c;
+#endif
+}
+// exp((v - m) / t) = 2^n 2^f, |f| <= 1/2: 2^f by a polynomial of degree 9 (a fit for this interval, off by 1.6e-14 at most). An LDS
+// table of 2^(j / 64) and a series of degree 4 instead: 64 lanes' reads meet in the banks, no faster.
 struct sm_weights {
-  double m, c;             // the largest logit, 64 log2(e) / t
-  __device__ __forceinline__ double operator()(const double* table, float v) const {
-    // (+inf counts as a finite number, the same in every place; -inf, NaN and what is far below come to 0)
-    const double y = fmax((fmin((double)v, 0x1p1000) - m) * c, -4096.0);
-    const double n = rint(y);
-    const int i = (int)n;
-    const double f = (y - n) * 0.010830424696249145;  // ln 2 / 64
-    double p = fma(f, 1.0 / 24, 1.0 / 6);
-    p = fma(f, p, 0.5);
+  double m, c;             // the largest logit, log2(e) / t
+  __device__ __forceinline__ sm_weights(float largest, float t) {
+    // +inf is taken as a number so large that all finite ones are far below it, also where t is infinite
+    m = largest == INFINITY ? 0x1p1023 : (double)largest;
+    c = largest == INFINITY || t == INFINITY ? 1e-300 : 1.4426950408889634 / (double)t;
+  }
+  __device__ __forceinline__ double operator()(float v) const {
+    // (-inf, NaN and what is far below come to 2^-64)
+    const double y = fmin(fmax(((double)v - m) * c, -64.0), 0.0);
+    const double near = y + 0x1.8p52, n = near - 0x1.8p52, f = y - n;  // the nearest whole number, in the low bits too
+    double p = sm_fma(f, 1.0148123730040949e-07, 1.3258333889433935e-06);
+    p = sm_fma(f, p, 1.525299113787619e-05);
+    p = sm_fma(f, p, 0.0001540344088852882);
+    p = sm_fma(f, p, 0.0013333557623583215);
+    p = sm_fma(f, p, 0.009618129181165067);
+    p = sm_fma(f, p, 0.055504108668426984);
+    p = sm_fma(f, p, 0.24022650695722755);
+    p = sm_fma(f, p, 0.6931471805598848);
     p = fma(f, p, 1.0);
-    p = fma(f, p, 1.0);
-    return ldexp(table[i & 63] * p, i >> 6);
+    return ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, near));
   }
 };
-__device__ __forceinline__ uint64_t sm_fixed(double e) {  // to the nearest multiple of 2^-43 (e <= 1)
-  return __builtin_bit_cast(uint64_t, e + 512.0) - __builtin_bit_cast(uint64_t, 512.0);
-}
+// e to the nearest multiple of 2^-43 (e <= 1), above that of 0
+#define SM_ZERO 0x4080000000000000ull  // 512.0
+__device__ __forceinline__ uint64_t sm_raw(double e) { return __builtin_bit_cast(uint64_t, e + 512.0); }
+__device__ __forceinline__ uint64_t sm_fixed(double e) { return sm_raw(e) - SM_ZERO; }
 
-__device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor((unsigned long long)v, d);
+template <int CTRL, int ROW_MASK, bool BOUND>
+__device__ __forceinline__ uint64_t sm_dpp(uint64_t v) {
+  const uint32_t lo = (uint32_t)sah_dpp_i<CTRL, ROW_MASK, BOUND>((int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)sah_dpp_i<CTRL, ROW_MASK, BOUND>((int)(uint32_t)(v >> 32));
+  return ((uint64_t)hi << 32) | lo;
+}
+// inclusive scan across the wave, all lanes active (as sah_wave_incl_scan)
+__device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {
+  v += sm_dpp<0x111, 0xF, true>(v);
+  v += sm_dpp<0x112, 0xF, true>(v);
+  v += sm_dpp<0x114, 0xF, true>(v);
+  v += sm_dpp<0x118, 0xF, true>(v);
+  v += sm_dpp<0x142, 0xA, false>(v);
+  v += sm_dpp<0x143, 0xC, false>(v);
   return v;
 }
-__device__ __forceinline__ uint64_t sm_block_sum(uint64_t v, sm_shared& S) {
-  v = sm_wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & (SAH_WAVE - 1)) == 0) S.wave_sum[threadIdx.x / SAH_WAVE] = v;
-  __syncthreads();
-  uint64_t all = 0;
-#pragma unroll
-  for (int i = 0; i < SM_NW; ++i) all += S.wave_sum[i];
-  return all;
+__device__ __forceinline__ uint64_t sm_lane(uint64_t v, int lane) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
-// exclusive scan over the workgroup's threads
-__device__ __forceinline__ uint64_t sm_block_scan(uint64_t v, sm_shared& S) {
+__device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) { return sm_lane(sm_wave_scan(v), SAH_WAVE - 1); }
+
+// sum and exclusive scan over the workgroup's threads (one wait; wave_sum is free to be written when this is called)
+__device__ __forceinline__ uint64_t sm_block_scan(uint64_t v, sm_shared& S, uint64_t& all) {
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
-  uint64_t incl = v;
-#pragma unroll
-  for (int d = 1; d < SAH_WAVE; d <<= 1) {
-    const uint64_t up = __shfl_up((unsigned long long)incl, d);
-    if (lane >= d) incl += up;
-  }
+  const uint64_t incl = sm_wave_scan(v);
   if (lane == SAH_WAVE - 1) S.wave_sum[wave] = incl;
   __syncthreads();
-  uint64_t before = 0;
-#pragma unroll
-  for (int i = 0; i < SM_NW; ++i) before += i < wave ? S.wave_sum[i] : 0;
-  return before + incl - v;
+  const uint64_t sums = sm_wave_scan(lane < SM_NW ? S.wave_sum[lane] : 0);
+  all = sm_lane(sums, SM_NW - 1);
+  return (wave ? sm_lane(sums, wave - 1) : 0) + incl - v;
 }
 
 // token e of 16 bytes
@@ -98,80 +124,138 @@ __device__ __forceinline__ float sm_unpack(const sah_u4& v, int e) {
   else return sah_f16_to_float((uint16_t)(v[e / 2] >> (16 * (e & 1))));
 }
 
-// f(logit, index) for every token of the row; a thread meets its own in the order of the index
-template <int DT, typename F>
+// f(logit, index) for every token of the row; a thread meets its own in the order of the index. U: 16-byte pieces a thread
+// requests at once; 1: with the next one on its way (where f is long, so that its code is there 16 / ES times, not four times that).
+template <int DT, int U, typename F>
 __device__ __forceinline__ void sm_each(const void* x, int V, F f) {
-  constexpr int E = DT == SAH_F32 ? 4 : 8, U = 4;
-  constexpr int ES = DT == SAH_F32 ? 4 : 2;
-  for (int base = 0; base < V; base += SM_NT * E * U) {
-    sah_u4 v[U];
+  constexpr int ES = DT == SAH_F32 ? 4 : 2, E = 16 / ES;
+  auto load = [&](int i) __attribute__((always_inline)) -> sah_u4 { return *(const sm_vec*)((const char*)x + (int64_t)i * ES); };
+  const int mine = (int)threadIdx.x * E, step = SM_NT * E;
+  auto all_of = [&](const sah_u4& v, int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = base + (u * SM_NT + (int)threadIdx.x) * E;
-      if (i + E <= V) v[u] = *(const sm_vec*)((const char*)x + (int64_t)i * ES);
+    for (int e = 0; e < E; ++e) f(sm_unpack<DT>(v, e), i + e);
+  };
+  int i = mine;
+  if constexpr (U == 1) {
+    sah_u4 next = {0, 0, 0, 0};
+    if (i + E <= V) next = load(i);
+#pragma unroll 1
+    for (; i + E <= V; i += step) {
+      const sah_u4 v = next;
+      if (i + step + E <= V) next = load(i + step);
+      all_of(v, i);
     }
+  } else {
+    for (; i + (U - 1) * step + E <= V; i += U * step) {
+      sah_u4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = base + (u * SM_NT + (int)threadIdx.x) * E;
-      if (i >= V) break;
-      if (i + E <= V) {
+      for (int u = 0; u < U; ++u) v[u] = load(i + u * step);
 #pragma unroll
-        for (int e = 0; e < E; ++e) f(sm_unpack<DT>(v[u], e), i + e);
-      } else {
-        for (int e = 0; i + e < V; ++e) f(sah_load<DT>(x, i + e), i + e);
-      }
+      for (int u = 0; u < U; ++u) all_of(v[u], i + u * step);
     }
+#pragma unroll 1
+    for (; i + E <= V; i += step) all_of(load(i), i);
   }
+#pragma unroll 1
+  for (int e = i; e < V && e < i + E; ++e) f(sah_load<DT>(x, e), e);  // the row's last few
 }
 
-struct sm_found {
-  bool any;          // the weights reach the target
-  uint32_t at;       // the order of the item at which they do
-  uint64_t before;   // weight of the items above it
-  uint64_t here;     // weight of the items of this order
+struct sm_bin {
+  int at;            // the bin, -1: the weights do not reach the target
+  uint64_t before;   // weight of the bins ahead of it
 };
-// Of items (order, weight) that `each` hands to its argument, from the largest order down: where the running weight reaches
-// `target` (> 0). Orders differ in BITS leading bits, at most. All threads call.
-template <int BITS, typename EACH>
-__device__ __forceinline__ sm_found sm_select(sm_shared& S, uint64_t target, EACH each) {
-  sm_found r{true, 0, 0, 0};
-  uint32_t known = 0;  // the leading bits that are decided
-  for (int done = 0; done < BITS;) {
-    const int bits = BITS - done < 11 ? BITS - done : 11;
-    const int shift = 32 - done - bits;
-    const uint32_t digit = (1u << bits) - 1;
-    for (int b = threadIdx.x; b < SM_BINS; b += SM_NT) S.bins[b] = 0;
-    __syncthreads();
-    each([&](uint32_t order, uint64_t weight) {
-      if ((order & known) == r.at) atomicAdd((unsigned long long*)&S.bins[(order >> shift) & digit], (unsigned long long)weight);
+// Adds up what `each` hands to its argument (bin, weight) and finds where the running weight, from bin 0 on, reaches
+// target(all the weight). All threads call; ends behind a wait.
+template <typename TARGET, typename EACH>
+__device__ __forceinline__ sm_bin sm_locate(sm_shared& S, TARGET target_of, EACH each) {
+  static_assert(SM_BINS == 2 * SM_NT, "two bins a thread");
+  each([&](uint32_t bin, uint64_t weight) { atomicAdd((unsigned long long*)&S.bins[bin], (unsigned long long)weight); });
+  if (threadIdx.x == 0) S.found_bin = -1;
+  __syncthreads();
+  const int b = 2 * (int)threadIdx.x;
+  const uint64_t w0 = S.bins[b], w1 = S.bins[b + 1];
+  S.bins[b] = 0;
+  S.bins[b + 1] = 0;
+  uint64_t all;
+  const uint64_t before = sm_block_scan(w0 + w1, S, all), target = target_of(all);
+  if (before < target && target <= before + w0 + w1) {  // one thread, where the target is reached
+    const bool second = before + w0 < target;
+    S.found_bin = second ? b + 1 : b;
+    S.found_before = second ? before + w0 : before;
+  }
+  __syncthreads();
+  sm_bin r{S.found_bin, S.found_before};
+  return r;
+}
+
+struct sm_item {
+  bool any;
+  uint32_t order;
+  int index;
+};
+// Of items (order, index, weight) that `each` hands to its argument, from the largest order down, equal ones by index: the one at
+// which the running weight reaches target(all the weight) (> 0). Items outside [lo, hi] are passed over. `round` counts calls.
+template <typename TARGET, typename EACH>
+__device__ __forceinline__ sm_item sm_pick(sm_shared& S, int& round, uint32_t lo, uint32_t hi, TARGET target_of, EACH each) {
+  uint64_t before = 0, target = 0;
+  bool first = true;
+  bool ties = false;   // all that is left shares one order, `same`: the order is that of the index now
+  uint32_t same = 0;
+  for (;;) {
+    const uint32_t range = hi - lo;
+    const int bits = range ? 32 - __builtin_clz(range) : 0, shift = bits > 11 ? bits - 11 : 0;
+    auto inside = [&](auto f) __attribute__((always_inline)) {
+      each([&](uint32_t order, int index, uint64_t weight) {
+        if (ties && order != same) return;
+        const uint32_t o = ties ? ~(uint32_t)index : order;
+        if (o >= lo && o <= hi) f(o, order, index, weight);
+      });
+    };
+    const sm_bin bin = sm_locate(
+        S, [&](uint64_t all) {
+          if (first) target = target_of(all);
+          return target - before;
+        },
+        [&](auto put) { inside([&](uint32_t o, uint32_t, int, uint64_t weight) { put((hi - o) >> shift, weight); }); });
+    if (bin.at < 0) return sm_item{false, 0, 0};
+    first = false;
+    before += bin.before;
+    hi -= (uint32_t)bin.at << shift;
+    lo = hi - lo > (1u << shift) - 1 ? hi - ((1u << shift) - 1) : lo;
+    // the piece's items, if they are few
+    int* n_small = &S.n_small[round & 1];
+    inside([&](uint32_t, uint32_t order, int index, uint64_t weight) {
+      const int j = atomicAdd(n_small, 1);
+      if (j < SM_SMALL) {
+        S.small[j] = make_uint2(order, (uint32_t)index);
+        S.small_weight[j] = weight;
+      }
     });
     __syncthreads();
-    // a thread's two digit values, from the largest down
-    static_assert(SM_BINS == 2 * SM_NT, "two a thread");
-    const int b = SM_BINS - 1 - 2 * (int)threadIdx.x;
-    const uint64_t w1 = S.bins[b], w0 = S.bins[b - 1];
-    const uint64_t before = r.before + sm_block_scan(w1 + w0, S);
-    if (threadIdx.x == 0) S.found[0] = 0;
-    __syncthreads();
-    if (before < target && target <= before + w1 + w0) {  // at most one thread
-      const bool second = before + w1 < target;
-      S.found[0] = 1;
-      S.found[1] = (uint64_t)(second ? b - 1 : b);
-      S.found[2] = second ? before + w1 : before;
-      S.found[3] = second ? w0 : w1;
+    const int n = *n_small;
+    if (threadIdx.x == 0) S.n_small[~round & 1] = 0;  // (last read before the waits since)
+    ++round;
+    if (n <= SM_SMALL) {  // every wave by itself
+      const int lane = threadIdx.x & (SAH_WAVE - 1);
+      const uint2 me = lane < n ? S.small[lane] : make_uint2(0, 0);
+      const uint64_t weight = lane < n ? S.small_weight[lane] : 0;
+      uint64_t ahead = before;
+      for (int j = 0; j < n; ++j) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)me.x, j), i = (uint32_t)__builtin_amdgcn_readlane((int)me.y, j);
+        const uint64_t w = sm_lane(weight, j);
+        if (o > me.x || (o == me.x && i < me.y)) ahead += w;
+      }
+      const uint64_t hit = __ballot(lane < n && ahead < target && target <= ahead + weight);
+      const int at = hit ? __builtin_ctzll(hit) : 0;
+      return sm_item{hit != 0, (uint32_t)__builtin_amdgcn_readlane((int)me.x, at), __builtin_amdgcn_readlane((int)me.y, at)};
     }
-    __syncthreads();
-    if (!S.found[0]) {
-      r.any = false;
-      return r;
+    if (shift == 0 && !ties) {
+      ties = true;
+      same = lo;
+      lo = ~(uint32_t)(SM_MAX_VOCAB - 1);
+      hi = ~0u;
     }
-    r.at |= (uint32_t)S.found[1] << shift;
-    r.before = S.found[2];
-    r.here = S.found[3];
-    known |= digit << shift;
-    done += bits;
   }
-  return r;
 }
 
 template <int DT>
@@ -180,7 +264,6 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
   SAH_DYNAMIC_LDS(s_dyn);
   sm_shared& S = *(sm_shared*)s_dyn;
   constexpr int ES = DT == SAH_F32 ? 4 : 2, E = 16 / ES;
-  constexpr int BITS = DT == SAH_F32 ? 32 : 16 + (DT == SAH_F16 ? 3 : 0);  // fp16 as fp32: 13 of the 23 mantissa bits are 0 (or 1)
   const int r = blockIdx.x, V = P.vocab;
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
   const void* x = (const char*)P.logits + (int64_t)r * P.row_pitch * ES;
@@ -190,30 +273,34 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
   float least = P.min_ps ? P.min_ps[r] : P.min_p;
   least = least > 1.f ? 1.f : least;
   const bool use_k = k > 0 && k < V, use_p = p < 1.f, use_m = least > 0.f;
-  if (threadIdx.x < 64) S.table[threadIdx.x] = exp2(threadIdx.x / 64.0);
-  if (threadIdx.x == 0) S.count = 0;
+  for (int b = threadIdx.x; b < SM_BINS; b += SM_NT) S.bins[b] = 0;
+  if (threadIdx.x == 0) S.count = S.n_small[0] = S.n_small[1] = 0;
+  int round = 0;
 
   // the largest logit and its first place
   float best = -INFINITY;
   int best_at = INT32_MAX;
-  sm_each<DT>(x, V, [&](float v, int i) {
+  sm_each<DT, 4>(x, V, [&](float v, int i) {
     best_at = v > best ? i : best_at;
     best = v > best ? v : best;
   });
   const float own = best;
+  float low = best;  // the smallest of the threads' largest
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     const float o = __shfl_xor(best, d);
     const int oa = __shfl_xor(best_at, d);
+    low = fminf(low, __shfl_xor(low, d));
     best_at = o > best ? oa : (o == best && oa < best_at ? oa : best_at);
     best = fmaxf(o, best);
   }
-  if (lane == 0) { S.wave_max[wave] = best; S.wave_at[wave] = best_at; }
+  if (lane == 0) { S.wave_max[wave] = best; S.wave_at[wave] = best_at; S.wave_low[wave] = low; }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < SM_NW; ++i) {
     const float o = S.wave_max[i];
     const int oa = S.wave_at[i];
+    low = fminf(low, S.wave_low[i]);
     best_at = o > best ? oa : (o == best && oa < best_at ? oa : best_at);
     best = fmaxf(o, best);
   }
@@ -224,209 +311,223 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
     }
     return;
   }
-  const sm_weights weigh{fmin((double)best, 0x1p1000), 92.33248261893676 / (double)temp};  // 64 log2(e)
-  auto fixed = [&](float v) -> uint64_t { return v > -INFINITY ? sm_fixed(weigh(S.table, v)) : 0; };
+  const sm_weights weigh(best, temp);
+  auto fixed = [&](float v) -> uint64_t { return sm_fixed(weigh(v)); };
+  const uint32_t top = sm_order(best);
 
   // the tokens that may be kept, in a list, where they are not too many
   bool list = false, complete = true;  // complete: the list has every token that min-p keeps
   const bool total = use_p && !use_k && V > SM_CAP;
   uint64_t sum = 0;                    // total: of all weights
+  uint32_t lowest = SM_LOWEST;         // no token of the list is of a lower order
   if ((use_k || use_p || use_m) && (V <= SM_CAP || !use_k || k <= SM_RANK_K)) {
     float from = -INFINITY;
     if (V > SM_CAP) {
-      if (use_k || use_p) {
+      if ((use_k || use_p) && low > -INFINITY) {  // every thread has a logit
+        const uint32_t range = top - sm_order(low);
+        const int bits = range ? 32 - __builtin_clz(range) : 0, shift = bits > 11 ? bits - 11 : 0;
         const uint64_t rank = use_k ? k : SM_RANK_P;
-        const sm_found f = sm_select<22>(S, rank, [&](auto put) { if (own > -INFINITY) put(sm_order(own), 1); });
-        if (f.any) {  // (all values with these 22 bits: the smallest of them)
-          from = f.at > 0x007fffffu ? sm_value(f.at) : -INFINITY;  // (0x007fffff: the order of -inf)
-          complete = false;
-        }
+        const sm_bin b = sm_locate(S, [&](uint64_t) { return rank; }, [&](auto put) { put((top - sm_order(own)) >> shift, 1); });
+        const uint32_t down = ((uint32_t)(b.at + 1) << shift) - 1;  // to the lower end of the piece
+        from = sm_value(down < range ? top - down : top - range);
+        complete = false;
       }
       if (use_m && !use_k) {
         // e >= least where x >= m + t ln(least); a little below that, for the roundings
         const double at = weigh.m + (double)temp * log((double)least);
-        const float low = (float)(at - 1e-6 * (fabs(at) + fabs(weigh.m)) - 1e-30);
-        if (low > from || !use_p) {
-          from = low == low ? low : -INFINITY;
+        const float below = (float)(at - 1e-6 * (fabs(at) + fabs(weigh.m)) - 1e-30);
+        if (below > from || !use_p) {
+          from = below == below ? below : -INFINITY;
           complete = true;
         }
       }
+      if (from > -INFINITY && from < best) lowest = sm_order(from);
     }
-    uint64_t mine = 0;
-    sm_each<DT>(x, V, [&](float v, int i) {
+    auto enlist = [&](float v, int i) {
       if (v >= from && v > -INFINITY) {
         const int n = atomicAdd(&S.count, 1);
         if (n < SM_CAP) S.list[n] = make_uint2(sah_float_to_bits(v), (uint32_t)i);
       }
-      if (total) mine += fixed(v);
-    });
-    if (total) sum = sm_block_sum(mine, S);
+    };
+    if (total) {
+      uint64_t mine = 0, n_mine = 0;
+      sm_each<DT, 1>(x, V, [&](float v, int i) {
+        enlist(v, i);
+        mine += sm_raw(weigh(v));  // (SM_ZERO too much: all at once below)
+        ++n_mine;
+      });
+      mine -= n_mine * SM_ZERO;
+      sm_block_scan(mine, S, sum);
+    } else {
+      sm_each<DT, 4>(x, V, enlist);
+    }
     __syncthreads();
     list = S.count <= SM_CAP;
   }
-  const int n_list = list ? S.count : 0;
-  // kept: of a higher order than thr, and of those that share it the ones with an index up to last
-  uint32_t thr = 0;
-  int last = V;
-  auto kept = [&](float v, int i) {
-    const uint32_t o = sm_order(v);
-    return v > -INFINITY && (o > thr || (o == thr && i <= last));
-  };
-  auto each = [&](auto f) __attribute__((always_inline)) {
-    if (list) {
+  if (!list) lowest = SM_LOWEST;
+  int n_list = list ? S.count : 0;
+  // kept: logits above thr, and of those equal to it the ones with an index up to last
+  float thr = -INFINITY;
+  int last = -1;
+  auto kept = [&](float v, int i) { return v > thr || (v == thr && i <= last); };
+  auto each = [&](bool from_list, auto f) __attribute__((always_inline)) {
+    if (from_list) {
       for (int j = threadIdx.x; j < n_list; j += SM_NT) {
         const uint2 it = S.list[j];
         f(sah_bits_to_float(it.x), (int)it.y);
       }
     } else {
-      sm_each<DT>(x, V, f);
+      sm_each<DT, 1>(x, V, f);
     }
   };
-  // the orders of 16-bit types differ in their leading bits alone, the others are 0, of negative numbers 1
-  auto whole_order = [&](uint32_t o) { return BITS < 32 && !(o & 0x80000000u) ? o | (uint32_t)((1ull << (32 - BITS)) - 1) : o; };
-  // of those that share thr, the first n by index
-  auto first_of = [&](uint64_t n) {
-    const sm_found f = sm_select<20>(S, n, [&](auto put) {
-      each([&](float v, int i) { if (sm_order(v) == thr && kept(v, i)) put(~((uint32_t)i << 12), 1); });
-    });
-    if (f.any) last = (int)(~f.at >> 12);
-  };
-  if (use_k) {
-    const sm_found f = sm_select<BITS>(S, k, [&](auto put) { each([&](float v, int i) { if (v > -INFINITY) put(sm_order(v), 1); }); });
-    if (f.any) {
-      thr = whole_order(f.at);
-      if (f.before + f.here > (uint64_t)k) first_of(k - f.before);
-    }
-  }
-  if (use_p) {
-    if (!total) {
-      uint64_t mine = 0;
-      each([&](float v, int i) { if (kept(v, i)) mine += fixed(v); });
-      sum = sm_block_sum(mine, S);
-    }
-    // whole numbers before a token are less than p times the sum where they are less than that rounded up
-    const double limit = ceil((double)p * (double)sum);
-    const uint64_t target = limit > 1.0 ? (uint64_t)limit : 1;  // (the first is always kept)
-    auto border = [&]() {
-      return sm_select<BITS>(S, target, [&](auto put) { each([&](float v, int i) { if (kept(v, i)) put(sm_order(v), fixed(v)); }); });
+  for (int stage = 0; stage < 2; ++stage) {  // top-k, then top-p
+    if (stage ? !use_p : !use_k) continue;
+    auto weight = [&](float v) -> uint64_t { return stage ? fixed(v) : 1; };
+    auto target_of = [&](uint64_t all) -> uint64_t {
+      if (!stage) return k;
+      if (total) all = sum;
+      // whole numbers before a token are less than p times the sum where they are less than that rounded up; the first is kept
+      const double limit = ceil((double)p * (double)all);
+      return limit > 1.0 ? (uint64_t)limit : 1;
     };
-    sm_found f = border();
-    if (!f.any && list && !complete) {  // the list ends before: the whole row
-      list = false;
-      f = border();
+    auto items = [&](bool from_list) {
+      return [&, from_list](auto put) __attribute__((always_inline)) {
+        each(from_list, [&](float v, int i) { if (kept(v, i)) put(sm_order(v), i, weight(v)); });
+      };
+    };
+    sm_item found{false, 0, 0};
+    if (list) {
+      found = sm_pick(S, round, lowest, top, target_of, items(true));
+      if (!found.any && stage && !complete) list = false;  // the list ends before
+      else if (!found.any) continue;
     }
-    if (f.any) {
-      const uint32_t at = whole_order(f.at);
-      if (at != thr) last = V;
-      thr = at;
-      const uint64_t e = fixed(sm_value(at));
-      const uint64_t n = (target - f.before + e - 1) / e;  // (e > 0: the weight at `at` reaches the target)
-      if (n * e < f.here) first_of(n);
+    if (!found.any) {
+      // pieces of 1 / SM_FINE in (m - x) / t, the last one for all that is further down
+      const float fine = SM_FINE / temp;
+      auto piece = [&](float v) -> uint32_t {
+        const float d = (best - v) * fine;
+        return v == best ? 0 : d < SM_BINS - 1 ? (uint32_t)d : SM_BINS - 1;
+      };
+      uint64_t target = 0;
+      const sm_bin b = sm_locate(
+          S, [&](uint64_t all) { return target = target_of(all); },
+          [&](auto put) { each(false, [&](float v, int i) { if (kept(v, i)) put(piece(v), weight(v)); }); });
+      if (b.at < 0) continue;
+      if (threadIdx.x == 0) S.count = 0;
+      __syncthreads();
+      each(false, [&](float v, int i) {
+        if (kept(v, i) && piece(v) == (uint32_t)b.at) {
+          const int n = atomicAdd(&S.count, 1);
+          if (n < SM_CAP) S.list[n] = make_uint2(sah_float_to_bits(v), (uint32_t)i);
+        }
+      });
+      __syncthreads();
+      const int n = S.count;
+      auto rest = [&](uint64_t) { return target - b.before; };
+      if (n <= SM_CAP) {
+        n_list = n;
+        found = sm_pick(S, round, SM_LOWEST, top, rest, items(true));
+      } else {  // (thousands of logits in one piece)
+        found = sm_pick(S, round, SM_LOWEST, top, rest, [&](auto put) __attribute__((always_inline)) {
+          each(false, [&](float v, int i) { if (kept(v, i) && piece(v) == (uint32_t)b.at) put(sm_order(v), i, weight(v)); });
+        });
+      }
+    }
+    if (found.any) {
+      thr = sm_value(found.order);
+      last = found.index;
     }
   }
   auto final_weight = [&](float v, int i) -> uint64_t {
     if (!kept(v, i)) return 0;
-    const double e = weigh(S.table, v);
-    return use_m && e < (double)least ? 0 : sm_fixed(e);
+    const double e = weigh(v);
+    return use_m && e < (double)least && v != best ? 0 : sm_fixed(e);
   };
   double u = P.uniforms_f64 ? ((const double*)P.uniforms)[r] : (double)((const float*)P.uniforms)[r];
   u = u > 0.0 ? u : 0.0;
-  auto target_of = [&](uint64_t all) {
+  auto drawn = [&](uint64_t all) -> uint64_t {  // the running weight passes u times all where it reaches this
     const uint64_t t = u < 1.0 ? (uint64_t)(u * (double)all) : all;
-    return t < all ? t : all - 1;
+    return (t < all ? t : all - 1) + 1;
   };
   auto answer = [&](int i, uint64_t all) {  // one thread
     P.tokens[r] = i;
-    if (P.logprobs) P.logprobs[r] = (float)log(weigh(S.table, sah_load<DT>(x, i)) * SM_ONE / (double)all);
+    if (P.logprobs) P.logprobs[r] = (float)log(weigh(sah_load<DT>(x, i)) * SM_ONE / (double)all);
   };
   if (list) {
-    uint64_t mine = 0;
-    each([&](float v, int i) { mine += final_weight(v, i); });
-    const uint64_t all = sm_block_sum(mine, S);
-    const sm_found f = sm_select<20>(S, target_of(all) + 1, [&](auto put) {
-      each([&](float v, int i) { put(~((uint32_t)i << 12), final_weight(v, i)); });
-    });
-    if (threadIdx.x == 0) answer((int)(~f.at >> 12), all);
+    uint64_t all = 0;
+    const sm_item f = sm_pick(
+        S, round, ~(uint32_t)(V - 1), ~0u, [&](uint64_t a) { all = a; return drawn(a); },
+        [&](auto put) __attribute__((always_inline)) { each(true, [&](float v, int i) { put(~(uint32_t)i, i, final_weight(v, i)); }); });
+    if (threadIdx.x == 0) answer(f.index, all);
     return;
   }
-  // The whole row: the weights of segments of 64 E tokens, what a wave reads at once; then inside the one that holds the target.
-  constexpr int SEG = SAH_WAVE * E, U = 4;
-  static_assert(SM_MAX_VOCAB / SEG <= 4 * SM_NT && 4 * SM_NT <= SM_CAP, "four sums a thread");
+  // The whole row: the weights of segments of 4 x 64 E tokens; then inside the one that holds the target.
+  constexpr int U = 4, SEG = SAH_WAVE * E * U;
+  static_assert(SM_MAX_VOCAB / SEG <= SM_NT && SM_NT <= SM_CAP, "a sum a thread");
   uint64_t* segs = (uint64_t*)S.list;
   const int n_segs = (V + SEG - 1) / SEG;
-  auto lane_weights = [&](int seg, uint64_t (&w)[E]) __attribute__((always_inline)) {
-    const int i = seg * SEG + lane * E;
-    sah_u4 v = {0, 0, 0, 0};
-    const bool full = i + E <= V;
-    if (full) v = *(const sm_vec*)((const char*)x + (int64_t)i * ES);
-#pragma unroll
-    for (int e = 0; e < E; ++e) w[e] = full ? final_weight(sm_unpack<DT>(v, e), i + e) : i + e < V ? final_weight(sah_load<DT>(x, i + e), i + e) : 0;
-  };
   __syncthreads();  // the list is no longer read
-  for (int s0 = wave; s0 < 4 * SM_NT; s0 += SM_NW * U) {
-    if (s0 >= n_segs) {
+  auto place = [&](int j) { return (wave + j / U * SM_NW) * SEG + (j % U * SAH_WAVE + lane) * E; };  // this lane's j-th piece
+  auto load = [&](int i) __attribute__((always_inline)) -> sah_u4 { return i + E <= V ? *(const sm_vec*)((const char*)x + (int64_t)i * ES) : sah_u4{0, 0, 0, 0}; };
+  sah_u4 next = load(place(0));
+  uint64_t part = 0;
+  const bool everything = thr == -INFINITY && !use_m;
+#pragma unroll 1
+  for (int j = 0; wave + j / U * SM_NW < n_segs; ++j) {
+    const sah_u4 v = next;
+    const int i = place(j);
+    next = load(place(j + 1));
+    if (i + E <= V && everything) {
 #pragma unroll
-      for (int q = 0; q < U; ++q)
-        if (lane == 0) segs[s0 + q * SM_NW] = 0;
-      continue;
+      for (int e = 0; e < E; ++e) part += sm_raw(weigh(sm_unpack<DT>(v, e)));
+      part -= E * SM_ZERO;
+    } else if (i + E <= V) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) part += final_weight(sm_unpack<DT>(v, e), i + e);
+    } else {
+#pragma unroll 1
+      for (int e = 0; i + e < V; ++e) part += final_weight(sah_load<DT>(x, i + e), i + e);
     }
-    sah_u4 v[U];
-#pragma unroll
-    for (int q = 0; q < U; ++q) {
-      const int i = (s0 + q * SM_NW) * SEG + lane * E;
-      v[q] = sah_u4{0, 0, 0, 0};
-      if (i + E <= V) v[q] = *(const sm_vec*)((const char*)x + (int64_t)i * ES);
-    }
-#pragma unroll
-    for (int q = 0; q < U; ++q) {
-      const int seg = s0 + q * SM_NW, i = seg * SEG + lane * E;
-      uint64_t mine = 0;
-      if (i + E <= V) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) mine += final_weight(sm_unpack<DT>(v[q], e), i + e);
-      } else {
-        for (int e = 0; i + e < V; ++e) mine += final_weight(sah_load<DT>(x, i + e), i + e);
-      }
-      mine = sm_wave_sum(mine);
-      if (lane == 0) segs[seg] = mine;
+    if (j % U == U - 1) {
+      part = sm_wave_sum(part);
+      if (lane == 0) segs[wave + j / U * SM_NW] = part;
+      part = 0;
     }
   }
   __syncthreads();
-  uint64_t four[4], mine = 0;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    four[q] = segs[4 * threadIdx.x + q];
-    mine += four[q];
-  }
-  const uint64_t all = sm_block_sum(mine, S);
-  const uint64_t target = target_of(all);
-  __syncthreads();  // sums of waves are read
-  uint64_t before = sm_block_scan(mine, S);
-  if (before <= target && target < before + mine) {  // one thread
-    int q = 0;
-    for (; q < 3 && before + four[q] <= target; ++q) before += four[q];
-    S.found[0] = 4 * threadIdx.x + q;
-    S.found[1] = before;
+  uint64_t all;
+  const uint64_t mine = (int)threadIdx.x < n_segs ? segs[threadIdx.x] : 0;
+  uint64_t before = sm_block_scan(mine, S, all);
+  const uint64_t target = drawn(all);
+  if (before < target && target <= before + mine) {  // one thread
+    S.found_bin = threadIdx.x;
+    S.found_before = before;
   }
   __syncthreads();
   if (wave) return;
-  const int seg = (int)S.found[0];
-  uint64_t w[E], own_sum = 0;
-  lane_weights(seg, w);
+  before = S.found_before;
+  int hit = -1;
+#pragma unroll 1
+  for (int q = 0; q < U; ++q) {
+    const int i = S.found_bin * SEG + (q * SAH_WAVE + lane) * E;
+    uint64_t w[E], own_sum = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) own_sum += w[e];
-  uint64_t incl = own_sum;
+    for (int e = 0; e < E; ++e) {
+      w[e] = i + e < V ? final_weight(sah_load<DT>(x, i + e), i + e) : 0;
+      own_sum += w[e];
+    }
+    const uint64_t incl = sm_wave_scan(own_sum);
+    uint64_t ahead = before + incl - own_sum;
+    if (ahead < target && target <= ahead + own_sum) {  // one lane of one q
 #pragma unroll
-  for (int d = 1; d < SAH_WAVE; d <<= 1) {
-    const uint64_t up = __shfl_up((unsigned long long)incl, d);
-    if (lane >= d) incl += up;
+      for (int e = 0; e < E; ++e) {
+        if (ahead < target && target <= ahead + w[e]) hit = i + e;
+        ahead += w[e];
+      }
+    }
+    before += sm_lane(incl, SAH_WAVE - 1);
   }
-  before = S.found[1] + incl - own_sum;
-  if (before <= target && target < before + own_sum) {  // one lane
-    int e = 0;
-    for (; before + w[e] <= target; ++e) before += w[e];
-    answer(seg * SEG + lane * E + e, all);
-  }
+  if (hit >= 0) answer(hit, all);
 }
 
 // ---------------------------------------------------------------------------
