@@ -312,13 +312,42 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
     return;
   }
   const sm_weights weigh(best, temp);
-  auto fixed = [&](float v) -> uint64_t { return sm_fixed(weigh(v)); };
   const uint32_t top = sm_order(best);
+
+  // pieces of 1 / SM_FINE in (m - x) / t, the last one for all that is further down
+  const float fine = SM_FINE / temp;
+  auto piece = [&](float v) -> int {
+    const float d = (best - v) * fine;
+    return v == best ? 0 : d < SM_BINS - 1 ? (int)d : SM_BINS - 1;
+  };
+  // whole numbers before a token are less than p times the sum where they are less than that rounded up; the first is kept
+  auto nucleus = [&](uint64_t all) -> uint64_t {
+    const double limit = ceil((double)p * (double)all);
+    return limit > 1.0 ? (uint64_t)limit : 1;
+  };
+  // kept: logits above thr, and of those equal to it the ones with an index up to last
+  float thr = -INFINITY;
+  int last = -1;
+  auto kept = [&](float v, int i) { return v > thr || (v == thr && i <= last); };
+  int n_list = 0;
+  auto enlist = [&](float v, int i) {
+    const int n = atomicAdd(&S.count, 1);
+    if (n < SM_CAP) S.list[n] = make_uint2(sah_float_to_bits(v), (uint32_t)i);
+  };
+  auto list_again = [&](auto take) __attribute__((always_inline)) {  // a new list, of the kept tokens that `take` takes; whether it holds them
+    if (threadIdx.x == 0) S.count = 0;
+    __syncthreads();
+    sm_each<DT, 1>(x, V, [&](float v, int i) { if (kept(v, i) && take(v)) enlist(v, i); });
+    __syncthreads();
+    n_list = S.count;
+    return n_list <= SM_CAP;
+  };
 
   // the tokens that may be kept, in a list, where they are not too many
   bool list = false, complete = true;  // complete: the list has every token that min-p keeps
   const bool total = use_p && !use_k && V > SM_CAP;
-  uint64_t sum = 0;                    // total: of all weights
+  uint64_t whole = 0;                  // total: the weight that top-p's last token reaches ...
+  sm_bin border{0, 0};                 // ... and its piece
   uint32_t lowest = SM_LOWEST;         // no token of the list is of a lower order
   if ((use_k || use_p || use_m) && (V <= SM_CAP || !use_k || k <= SM_RANK_K)) {
     float from = -INFINITY;
@@ -343,33 +372,29 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
       }
       if (from > -INFINITY && from < best) lowest = sm_order(from);
     }
-    auto enlist = [&](float v, int i) {
-      if (v >= from && v > -INFINITY) {
-        const int n = atomicAdd(&S.count, 1);
-        if (n < SM_CAP) S.list[n] = make_uint2(sah_float_to_bits(v), (uint32_t)i);
-      }
-    };
     if (total) {
-      uint64_t mine = 0, n_mine = 0;
-      sm_each<DT, 1>(x, V, [&](float v, int i) {
-        enlist(v, i);
-        mine += sm_raw(weigh(v));  // (SM_ZERO too much: all at once below)
-        ++n_mine;
-      });
-      mine -= n_mine * SM_ZERO;
-      sm_block_scan(mine, S, sum);
+      // the weights' pass shares the row out into pieces too: if top-p's last token lies below the list, its piece is known
+      border = sm_locate(
+          S, [&](uint64_t all) { return whole = nucleus(all); },
+          [&](auto put) __attribute__((always_inline)) {
+            sm_each<DT, 1>(x, V, [&](float v, int i) {
+              if (v >= from && v > -INFINITY) enlist(v, i);
+              put(piece(v), sm_fixed(weigh(v)));
+            });
+          });
+      if (from > -INFINITY && !complete && piece(from) <= border.at) {
+        // further down than the list: all down to there, if it holds that
+        const float down = best - (border.at + 1.01f) / fine;
+        lowest = border.at < SM_BINS - 1 && down > -INFINITY && down < best ? sm_order(down) : SM_LOWEST;
+        list_again([&](float v) { return piece(v) <= border.at; });
+      }
     } else {
-      sm_each<DT, 4>(x, V, enlist);
+      sm_each<DT, 4>(x, V, [&](float v, int i) { if (v >= from && v > -INFINITY) enlist(v, i); });
     }
     __syncthreads();
-    list = S.count <= SM_CAP;
+    n_list = S.count;
+    list = n_list <= SM_CAP;
   }
-  if (!list) lowest = SM_LOWEST;
-  int n_list = list ? S.count : 0;
-  // kept: logits above thr, and of those equal to it the ones with an index up to last
-  float thr = -INFINITY;
-  int last = -1;
-  auto kept = [&](float v, int i) { return v > thr || (v == thr && i <= last); };
   auto each = [&](bool from_list, auto f) __attribute__((always_inline)) {
     if (from_list) {
       for (int j = threadIdx.x; j < n_list; j += SM_NT) {
@@ -382,14 +407,8 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
   };
   for (int stage = 0; stage < 2; ++stage) {  // top-k, then top-p
     if (stage ? !use_p : !use_k) continue;
-    auto weight = [&](float v) -> uint64_t { return stage ? fixed(v) : 1; };
-    auto target_of = [&](uint64_t all) -> uint64_t {
-      if (!stage) return k;
-      if (total) all = sum;
-      // whole numbers before a token are less than p times the sum where they are less than that rounded up; the first is kept
-      const double limit = ceil((double)p * (double)all);
-      return limit > 1.0 ? (uint64_t)limit : 1;
-    };
+    auto weight = [&](float v) -> uint64_t { return stage ? sm_fixed(weigh(v)) : 1; };
+    auto target_of = [&](uint64_t all) -> uint64_t { return !stage ? k : total ? whole : nucleus(all); };
     auto items = [&](bool from_list) {
       return [&, from_list](auto put) __attribute__((always_inline)) {
         each(from_list, [&](float v, int i) { if (kept(v, i)) put(sm_order(v), i, weight(v)); });
@@ -398,38 +417,20 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
     sm_item found{false, 0, 0};
     if (list) {
       found = sm_pick(S, round, lowest, top, target_of, items(true));
-      if (!found.any && stage && !complete) list = false;  // the list ends before
-      else if (!found.any) continue;
-    }
-    if (!found.any) {
-      // pieces of 1 / SM_FINE in (m - x) / t, the last one for all that is further down
-      const float fine = SM_FINE / temp;
-      auto piece = [&](float v) -> uint32_t {
-        const float d = (best - v) * fine;
-        return v == best ? 0 : d < SM_BINS - 1 ? (uint32_t)d : SM_BINS - 1;
-      };
-      uint64_t target = 0;
-      const sm_bin b = sm_locate(
-          S, [&](uint64_t all) { return target = target_of(all); },
-          [&](auto put) { each(false, [&](float v, int i) { if (kept(v, i)) put(piece(v), weight(v)); }); });
+    } else {
+      uint64_t target = whole;
+      sm_bin b = border;
+      if (!total)
+        b = sm_locate(
+            S, [&](uint64_t all) { return target = target_of(all); },
+            [&](auto put) __attribute__((always_inline)) { each(false, [&](float v, int i) { if (kept(v, i)) put(piece(v), weight(v)); }); });
       if (b.at < 0) continue;
-      if (threadIdx.x == 0) S.count = 0;
-      __syncthreads();
-      each(false, [&](float v, int i) {
-        if (kept(v, i) && piece(v) == (uint32_t)b.at) {
-          const int n = atomicAdd(&S.count, 1);
-          if (n < SM_CAP) S.list[n] = make_uint2(sah_float_to_bits(v), (uint32_t)i);
-        }
-      });
-      __syncthreads();
-      const int n = S.count;
       auto rest = [&](uint64_t) { return target - b.before; };
-      if (n <= SM_CAP) {
-        n_list = n;
+      if (list_again([&](float v) { return piece(v) == b.at; })) {
         found = sm_pick(S, round, SM_LOWEST, top, rest, items(true));
       } else {  // (thousands of logits in one piece)
         found = sm_pick(S, round, SM_LOWEST, top, rest, [&](auto put) __attribute__((always_inline)) {
-          each(false, [&](float v, int i) { if (kept(v, i) && piece(v) == (uint32_t)b.at) put(sm_order(v), i, weight(v)); });
+          each(false, [&](float v, int i) { if (kept(v, i) && piece(v) == b.at) put(sm_order(v), i, weight(v)); });
         });
       }
     }
