@@ -253,6 +253,13 @@ template <int DT> struct pa_weights {
   static constexpr float SCALE = DT == SAH_F16 ? 8.0f : 0.0f;
 };
 
+// Reads of LDS written above this are issued above it.
+__device__ __forceinline__ void pa_reads_stay() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" ::: "memory");
+#endif
+}
+
 template <int DT, int DP, bool WIDE>
 __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WIDE>::PER_CU)) void k_paged_attn(sah_paged_attention_args P) {
   sah_touch_kernargs<sizeof(sah_paged_attention_args)>();
@@ -296,7 +303,11 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
   const int l_key = lane / UNITS, l_place = lane % UNITS;
   auto f_k = [](int key) { return UNITS == 8 ? (key >> 1) & 7 : key & 15; };
   auto f_v = [](int key) { return DT == SAH_F32 ? 0 : UNITS == 8 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); };
+  // (places behind a shorter head's end hold its last unit again: the queries are 0 there, the results nobody's)
   const int units_real = P.D * ES / 16;
+  const uint32_t last_unit = 16u * (units_real - 1);
+  const uint32_t k_unit = 16u * (l_place ^ f_k(l_key)), v_unit = 16u * (l_place ^ f_v(l_key));
+  const uint32_t k_lane = (uint32_t)(l_key * P.ks_t * ES), v_lane = (uint32_t)(l_key * P.vs_t * ES);
   const int k_at = i32 * S::ROW + 16 * (g ^ f_k(i32));
   int v_at[DTL];
 #pragma unroll
@@ -383,20 +394,40 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     const char* vbase = (const char*)P.v + (int64_t)at.hk * P.vs_h * ES;
     auto fetch = [&](int u, int pg, uint64_t there, int buf) __attribute__((always_inline)) {
       const int key0 = first_key(u);
-      const int spare = 63 - __builtin_clzll(there | 1);  // stands for keys that are not there
+      auto stage_at = [&](int at_key) { return ((WIDE ? 0 : 32 * wave) + at_key) * S::ROW; };
+      if (there == (S::WKEYS == 64 ? ~0ull : 0xffffffffull) && P.page_size >= KPI) {  // uniform
+        // All keys are there and an instruction's lie in one page: a scalar base, and a lane's offset that stays the same but for
+        // the permutation's part of the instruction (an exclusive or: its key's bits are none of the lane's).
 #pragma unroll
+        for (int i = 0; i < IW; ++i) {
+          const int at_key = ((WIDE ? wave * IW : 0) + i) * KPI;
+          const int64_t p = __builtin_amdgcn_readlane(pg, at_key), entry = (key0 + at_key) & (P.page_size - 1);
+          const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES;
+          const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES;
+          const uint32_t uk = k_unit ^ (16u * f_k(at_key)), uv = v_unit ^ (16u * f_v(at_key));
+          sah_load_lds16(ka + (k_lane + (uk < last_unit ? uk : last_unit)), (buf ? s_k1 : s_k0) + stage_at(at_key));
+          sah_load_lds16(va + (v_lane + (uv < last_unit ? uv : last_unit)), (buf ? s_v1 : s_v0) + stage_at(at_key));
+        }
+        return;
+      }
+      const int spare = 63 - __builtin_clzll(there | 1);  // stands for keys that are not there
+      // (taken from here: a register for everything that follows from them, kept through the loop, is dearer than two instructions)
+      uint32_t lk = l_key, lp = l_place;
+      sah_keep(lk);
+      sah_keep(lp);
+#pragma unroll 1
       for (int i = 0; i < IW; ++i) {
         const int at_key = ((WIDE ? wave * IW : 0) + i) * KPI;  // of the wave's keys; a wave with keys of its own stages all of them
-        const int key = at_key + l_key;
+        const int key = at_key + (int)lk;
         const int src = (there >> key) & 1 ? key : spare;
-        const int64_t p = there ? __shfl(pg, src) : 0;  // (nothing there: any page, and nobody reads it)
+        const int page_of = __shfl(pg, src);
+        const int64_t p = there ? page_of : 0;  // (nothing there: any page, and nobody reads it)
         const int64_t entry = (key0 + src) & (P.page_size - 1);
-        const int uk = l_place ^ f_k(key), uv = l_place ^ f_v(key);
-        const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES + 16 * (uk < units_real ? uk : 0);
-        const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES + 16 * (uv < units_real ? uv : 0);
-        const int to = ((WIDE ? 0 : 32 * wave) + at_key) * S::ROW;
-        sah_load_lds16(ka, (buf ? s_k1 : s_k0) + to);
-        sah_load_lds16(va, (buf ? s_v1 : s_v0) + to);
+        const uint32_t uk = 16u * (lp ^ f_k(key)), uv = 16u * (lp ^ f_v(key));
+        const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES + (uk < last_unit ? uk : last_unit);
+        const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES + (uv < last_unit ? uv : last_unit);
+        sah_load_lds16(ka, (buf ? s_k1 : s_k0) + stage_at(at_key));
+        sah_load_lds16(va, (buf ? s_v1 : s_v0) + stage_at(at_key));
       }
     };
 
@@ -407,27 +438,61 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       const unsigned char* vp = (buf ? s_v1 : s_v0) + (WIDE ? 0 : 32 * wave * S::ROW);
       sah_f32x16 s[RB][TW];
 #pragma unroll
-      for (int t = 0; t < TW; ++t) {
+      for (int t = 0; t < TW; ++t)
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[rb][t][e] = 0.f;
+      // Four pieces of a key tile at a time are read while the four before are multiplied: the reads may not sink to where they
+      // are used (a wait for each then: 778 us of the chunk's pass instead of %QK% with both products so).
+      {
+        constexpr int C = 4, NC = TW * KQ / C;
+        uint4 a[2][C];
+        auto read = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int st = 0; st < KQ; ++st) {
-          const uint4 a = *(const uint4*)(kp + 32 * t * S::ROW + (k_at ^ (32 * st)));
+          for (int i = 0; i < C; ++i) {
+            const int t = c * C / KQ, st = c * C % KQ + i;
+            a[c & 1][i] = *(const uint4*)(kp + 32 * t * S::ROW + (k_at ^ (32 * st)));
+          }
+        };
+        read(0);
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb) {
-            if constexpr (DT == SAH_F32) {
-              s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(a.x), sah_bits_to_float(qf[rb][st].x), s[rb][t]);
-              s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(a.y), sah_bits_to_float(qf[rb][st].y), s[rb][t]);
-              s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(a.z), sah_bits_to_float(qf[rb][st].z), s[rb][t]);
-              s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(a.w), sah_bits_to_float(qf[rb][st].w), s[rb][t]);
-            } else {
-              s[rb][t] = sah_mfma_32x32x16<DT>(a, qf[rb][st], s[rb][t]);
+        for (int c = 0; c < NC; ++c) {
+          if (c + 1 < NC) read(c + 1);
+          pa_reads_stay();
+#pragma unroll
+          for (int i = 0; i < C; ++i) {
+            const int t = c * C / KQ, st = c * C % KQ + i;
+            const uint4 k = a[c & 1][i];
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+              if constexpr (DT == SAH_F32) {
+                s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.x), sah_bits_to_float(qf[rb][st].x), s[rb][t]);
+                s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.y), sah_bits_to_float(qf[rb][st].y), s[rb][t]);
+                s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.z), sah_bits_to_float(qf[rb][st].z), s[rb][t]);
+                s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.w), sah_bits_to_float(qf[rb][st].w), s[rb][t]);
+              } else {
+                s[rb][t] = sah_mfma_32x32x16<DT>(k, qf[rb][st], s[rb][t]);
+              }
             }
           }
         }
       }
+      // the first values, requested ahead of the softmax
+      constexpr int NV = 2 * TW;
+      uint4 va[2][DT == SAH_F32 ? 1 : DTL];
+      auto read_v = [&](int c) __attribute__((always_inline)) {
+        if constexpr (DT != SAH_F32) {
+#pragma unroll
+          for (int d = 0; d < DTL; ++d) {
+            const unsigned char* v = vp + 16 * c * S::ROW + v_at[d];
+            const sah_u2 a0 = sah_read_tr16((const uint16_t*)v), a1 = sah_read_tr16((const uint16_t*)(v + 8 * S::ROW));
+            va[c & 1][d] = make_uint4(a0.x, a0.y, a1.x, a1.y);
+          }
+        }
+      };
+      read_v(0);
+      pa_reads_stay();
       // every row sees every key of the stage?
       const uint64_t full = S::WKEYS == 64 ? ~0ull : 0xffffffffull;
       const bool plain = there == full && key0 + S::WKEYS - 1 <= w_lo &&
@@ -435,12 +500,15 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       if (!plain) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
-          const int lo = P.window && pos[rb] >= P.window ? pos[rb] - P.window + 1 : 0;
+          uint32_t kept_pos = pos[rb];
+          sah_keep(kept_pos);
+          const int at_pos = (int)kept_pos;
+          const int lo = P.window && at_pos >= P.window ? at_pos - P.window + 1 : 0;
 #pragma unroll
           for (int t = 0; t < TW; ++t) {
             const int k0 = key0 + 32 * t, wi = k0 / 32;
-            uint32_t word = sah_range_bits(wi, lo, pos[rb] + 1);
-            if (P.window) word |= sah_range_bits(wi, 0, P.sink < pos[rb] + 1 ? P.sink : pos[rb] + 1);
+            uint32_t word = sah_range_bits(wi, lo, at_pos + 1);
+            if (P.window) word |= sah_range_bits(wi, 0, P.sink < at_pos + 1 ? P.sink : at_pos + 1);
             word &= (uint32_t)(there >> (32 * t));
             word >>= 4 * g;
 #pragma unroll
@@ -477,9 +545,9 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
             l_run[rb] += s[rb][t][e];
           }
       }
+      if constexpr (DT == SAH_F32) {
 #pragma unroll
-      for (int t = 0; t < TW; ++t) {
-        if constexpr (DT == SAH_F32) {
+        for (int t = 0; t < TW; ++t)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float* row = (const float*)(vp + (32 * t + 8 * (e / 4) + e % 4 + 4 * g) * S::ROW) + i32;
@@ -490,24 +558,19 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
               for (int rb = 0; rb < RB; ++rb) acc[rb][d] = sah_mfma_32x32x2_f32(v, s[rb][t][e], acc[rb][d]);
             }
           }
-        } else {
+      } else {
 #pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            uint4 pt[RB];
+        for (int c = 0; c < NV; ++c) {
+          const int t = c / 2, st = c % 2;
+          if (c + 1 < NV) read_v(c + 1);
+          pa_reads_stay();
 #pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-              const auto& z = s[rb][t];
-              pt[rb] = make_uint4(sah_pack2_hw<DT>(z[8 * st], z[8 * st + 1]), sah_pack2_hw<DT>(z[8 * st + 2], z[8 * st + 3]),
-                                  sah_pack2_hw<DT>(z[8 * st + 4], z[8 * st + 5]), sah_pack2_hw<DT>(z[8 * st + 6], z[8 * st + 7]));
-            }
+          for (int rb = 0; rb < RB; ++rb) {
+            const auto& z = s[rb][t];
+            const uint4 pt = make_uint4(sah_pack2_hw<DT>(z[8 * st], z[8 * st + 1]), sah_pack2_hw<DT>(z[8 * st + 2], z[8 * st + 3]),
+                                        sah_pack2_hw<DT>(z[8 * st + 4], z[8 * st + 5]), sah_pack2_hw<DT>(z[8 * st + 6], z[8 * st + 7]));
 #pragma unroll
-            for (int d = 0; d < DTL; ++d) {
-              const unsigned char* v = vp + (32 * t + 16 * st) * S::ROW + v_at[d];
-              const sah_u2 a0 = sah_read_tr16((const uint16_t*)v), a1 = sah_read_tr16((const uint16_t*)(v + 8 * S::ROW));
-              const uint4 va = make_uint4(a0.x, a0.y, a1.x, a1.y);
-#pragma unroll
-              for (int rb = 0; rb < RB; ++rb) acc[rb][d] = sah_mfma_32x32x16<DT>(va, pt[rb], acc[rb][d]);
-            }
+            for (int d = 0; d < DTL; ++d) acc[rb][d] = sah_mfma_32x32x16<DT>(va[c & 1][d], pt, acc[rb][d]);
           }
         }
       }
@@ -697,72 +760,103 @@ __device__ __forceinline__ void pa_row_again(const sah_paged_attention_args& P, 
   }
 }
 
-// Joins the parts of the tile that workgroup blockIdx.x of the first kernel began and did not end, a row per wave (many parts: a
-// row per workgroup, its waves taking parts in turn). Row blocks go to blockIdx.y.
+// Joins the parts of the tile that workgroup blockIdx.x of the first kernel began and did not end. 16 lanes hold a row: with few parts
+// a workgroup does 16 rows at once, with many one row, whose parts its 16 groups take in turn. blockIdx.y shares the rows out.
 #define PA_JOIN_NT 256
-#define PA_JOIN_ROWS 8     // workgroups that share a tile's rows
+#define PA_JOIN_GROUPS (PA_JOIN_NT / 16)
+#define PA_JOIN_WGS 8
 template <int DT, int DP, bool WIDE>
 __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attention_args P) {
+  sah_touch_kernargs<sizeof(sah_paged_attention_args)>();
   typedef pa_shape<DT, DP, WIDE> S;
-  constexpr int NW = PA_JOIN_NT / SAH_WAVE, E = DP / SAH_WAVE;
-  __shared__ float s_m[NW], s_l[NW], s_acc[NW][DP];
+  constexpr int NW = PA_JOIN_NT / SAH_WAVE, F = DP / 64;  // float4s of a lane: dims 4 (lane % 16) + 64 f ..
+  __shared__ float s_ml[PA_JOIN_GROUPS][2];
+  __shared__ float4 s_acc[PA_JOIN_GROUPS][DP / 4];
   __shared__ int64_t s_sum[NW + 2];
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
+  const int group = threadIdx.x / 16, l16 = threadIdx.x % 16;
   const int w = blockIdx.x, G = P.Hq / P.Hkv;
   const pa_note note = ((const pa_note*)P.work)[w];
   const float* parts = P.work + S::WGS * (sizeof(pa_note) / 4);
   if (note.b >= 0) {
     const pa_request req = pa_read_request(P, note.b);
-    const int n_rows = req.n_new * G, n_parts = note.last - w + 1;
-    const bool many = n_parts > 8;
-    for (int i = many ? (int)blockIdx.y : (int)blockIdx.y * NW + wave; i < S::ROWS; i += many ? PA_JOIN_ROWS : PA_JOIN_ROWS * NW) {
-      const int r = note.tile * S::ROWS + i;
-      if (r >= n_rows) break;  // (uniform across the workgroup where it matters: many)
-      const int first = many ? wave : 0, step = many ? NW : 1;
-      float m = -INFINITY, l = 0.f, acc[E];
+    const int n_rows = req.n_new * G - note.tile * S::ROWS < S::ROWS ? req.n_new * G - note.tile * S::ROWS : S::ROWS;
+    const int n_parts = note.last - w + 1;
+    // whichever has fewer trips to memory in a row
+    const bool many = (n_parts + 3) / 4 * ((n_rows + PA_JOIN_WGS * PA_JOIN_GROUPS - 1) / (PA_JOIN_WGS * PA_JOIN_GROUPS)) >
+                      (n_rows + PA_JOIN_WGS - 1) / PA_JOIN_WGS * (n_parts / (4 * PA_JOIN_GROUPS) + 2);
+    for (int i0 = blockIdx.y * (many ? 1 : PA_JOIN_GROUPS); i0 < n_rows; i0 += PA_JOIN_WGS * (many ? 1 : PA_JOIN_GROUPS)) {  // uniform
+      const int i = many ? i0 : i0 + group < n_rows ? i0 + group : n_rows - 1;
+      const int first = many ? group : 0, step = many ? PA_JOIN_GROUPS : 1;
+      float m = -INFINITY, l = 0.f;
+      float4 acc[F];
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = 0.f;
-      for (int p = first; p < n_parts; p += step) {
-        const float* from = parts + (int64_t)(p ? 2 * (w + p) : 2 * w + 1) * S::SLOT;
-        const float2 ml = ((const float2*)from)[i];
+      for (int f = 0; f < F; ++f) acc[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto add = [&](float2 ml, const float4 (&v)[F]) __attribute__((always_inline)) {
         const float m_new = fmaxf(m, ml.x);
         const float a = m == -INFINITY ? 0.f : exp2f(m - m_new), z = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m_new);
-        // (a part whose sums are NaN without a maximum: the row is done again)
+        // (a part whose sum is NaN has no maximum, perhaps: the row is done again all the same)
         l = l * a + (ml.y == ml.y ? ml.y * z : ml.y);
         m = m_new;
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * a + z * from[2 * S::ROWS + i * DP + lane + e * SAH_WAVE];
+        for (int f = 0; f < F; ++f) {
+          acc[f].x = acc[f].x * a + v[f].x * z;
+          acc[f].y = acc[f].y * a + v[f].y * z;
+          acc[f].z = acc[f].z * a + v[f].z * z;
+          acc[f].w = acc[f].w * a + v[f].w * z;
+        }
+      };
+      constexpr int U = 4;
+      for (int p = first; p < n_parts; p += U * step) {  // four parts requested at once; behind the last one it is taken again, and not added
+        float2 ml[U];
+        float4 v[U][F];
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+          const int pp = p + q * step < n_parts ? p + q * step : n_parts - 1;
+          const float* from = parts + (int64_t)(pp ? 2 * (w + pp) : 2 * w + 1) * S::SLOT;
+          ml[q] = ((const float2*)from)[i];
+#pragma unroll
+          for (int f = 0; f < F; ++f) v[q][f] = ((const float4*)(from + 2 * S::ROWS + i * DP))[l16 + 16 * f];
+        }
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+          if (p + q * step < n_parts) add(ml[q], v[q]);
       }
       if (many) {
+        __syncthreads();  // the row before has been read
+        if (l16 == 0) { s_ml[group][0] = m; s_ml[group][1] = l; }
+#pragma unroll
+        for (int f = 0; f < F; ++f) s_acc[group][l16 + 16 * f] = acc[f];
         __syncthreads();
-        if (lane == 0) { s_m[wave] = m; s_l[wave] = l; }
+        if (group) continue;
+        for (int o = 1; o < PA_JOIN_GROUPS; ++o) {
+          float4 v[F];
 #pragma unroll
-        for (int e = 0; e < E; ++e) s_acc[wave][lane + e * SAH_WAVE] = acc[e];
-        __syncthreads();
-        if (wave) continue;
-#pragma unroll
-        for (int v = 1; v < NW; ++v) {
-          const float m_new = fmaxf(m, s_m[v]);
-          const float a = m == -INFINITY ? 0.f : exp2f(m - m_new), z = s_m[v] == -INFINITY ? 0.f : exp2f(s_m[v] - m_new);
-          l = l * a + (s_l[v] == s_l[v] ? s_l[v] * z : s_l[v]);
-          m = m_new;
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = acc[e] * a + z * s_acc[v][lane + e * SAH_WAVE];
+          for (int f = 0; f < F; ++f) v[f] = s_acc[o][l16 + 16 * f];
+          add(make_float2(s_ml[o][0], s_ml[o][1]), v);
         }
       }
-      const int tok = req.row0 + r / G, h = note.hk * G + r % G;
+      const int r = note.tile * S::ROWS + i, tok = req.row0 + r / G, h = note.hk * G + r % G;
       bool fine = l == l;
       if (P.sinks && m != -INFINITY) l += exp2f(fmaf(P.sinks[h], 1.4426950408889634f, pa_weights<DT>::SCALE) - m);
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int d = lane + e * SAH_WAVE;
+      for (int f = 0; f < F; ++f) {
+        const int d = 4 * l16 + 64 * f;
         if (d >= P.D) continue;
-        acc[e] *= inv;
-        fine = fine && fabsf(acc[e]) < INFINITY;
-        sah_store<DT>(P.out, (int64_t)tok * P.os_t + (int64_t)h * P.os_h + d, acc[e]);
+        const float4 o = make_float4(acc[f].x * inv, acc[f].y * inv, acc[f].z * inv, acc[f].w * inv);
+        fine = fine && fabsf(o.x) < INFINITY && fabsf(o.y) < INFINITY && fabsf(o.z) < INFINITY && fabsf(o.w) < INFINITY;
+        char* to = (char*)P.out + ((int64_t)tok * P.os_t + (int64_t)h * P.os_h + d) * S::ES;
+        if (DT == SAH_F32) *(float4*)to = o;
+        else *(uint2*)to = make_uint2(sah_pack2_hw<DT>(o.x, o.y), sah_pack2_hw<DT>(o.z, o.w));
       }
-      if (__ballot(!fine)) pa_row_again<DT>(P, req, note.b, tok, h);
+      // rows that are not finite are done again, one after the other, by the wave that has them
+      uint64_t again = __ballot(!fine);
+      while (again) {
+        const int from = __builtin_ctzll(again) & ~15;
+        again &= ~(0xffffull << from);
+        pa_row_again<DT>(P, req, note.b, __builtin_amdgcn_readlane(tok, from), __builtin_amdgcn_readlane(h, from));
+      }
     }
   }
   if (!note.again) return;  // uniform
@@ -774,7 +868,7 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
   for (;;) {
     if (at.begin >= x0 && at.begin + at.cost <= x1) {
       const int n_rows = at.req.n_new * G;
-      for (int i = (int)blockIdx.y * NW + wave; i < S::ROWS; i += PA_JOIN_ROWS * NW) {
+      for (int i = (int)blockIdx.y * NW + wave; i < S::ROWS; i += PA_JOIN_WGS * NW) {
         const int r = at.tile * S::ROWS + i;
         if (r >= n_rows) break;
         const int tok = at.req.row0 + r / G, h = at.hk * G + r % G;
@@ -813,7 +907,7 @@ static int pa_launch(const sah_paged_attention_args* a) {
     if (int rc = sah_launch_status("sah_paged_attention")) return rc;
   }
   sah_timed timed("k_paged_attn_join", a->stream);
-  hipLaunchKernelGGL((k_paged_attn_join<DT, DP, WIDE>), dim3(S::WGS, PA_JOIN_ROWS), dim3(PA_JOIN_NT), 0, st, *a);
+  hipLaunchKernelGGL((k_paged_attn_join<DT, DP, WIDE>), dim3(S::WGS, PA_JOIN_WGS), dim3(PA_JOIN_NT), 0, st, *a);
   return sah_launch_status("sah_paged_attention(join)");
 }
 
