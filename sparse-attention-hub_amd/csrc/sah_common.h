@@ -308,6 +308,16 @@ __device__ __forceinline__ void sah_load_lds16(const void* p, void* lds) {
   (void)p; (void)lds;
 #endif
 }
+// The same from a wave-uniform address plus a byte offset per lane, as a buffer load: the compiler counts these apart from its loads
+// through pointers, which it takes to come back out of order once they write LDS (any wait becomes one for all of them).
+__device__ __forceinline__ void sah_buffer_load_lds16(const void* base, uint32_t offset, void* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x00027000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, (int)offset, 0, 0, 0);
+#else
+  (void)base; (void)offset; (void)lds;
+#endif
+}
 // Transposing LDS read, one 4 x 16 block of 16-bit elements per 16 lanes (layout checked on the hardware): lane l hands in
 // the address of row (l % 16) / 4, columns 4 (l % 4) .. + 3 and receives column l % 16, rows 0 .. 3.
 typedef uint32_t sah_u2 __attribute__((ext_vector_type(2)));

@@ -25,16 +25,18 @@ template <int DT, int DP, bool WIDE>
 struct pa_shape {
   static constexpr int ES = DT == SAH_F32 ? 4 : 2;
   static constexpr int ROW = DP * ES;                      // bytes of a staged key
-  static constexpr int NW = WIDE ? 4 : (ROW <= 256 ? 4 : 1024 / ROW);
+  static constexpr int NW = WIDE ? 4 : ROW <= 256 ? 8 : 2048 / ROW;
   static constexpr int NT = NW * SAH_WAVE;
   static constexpr int RB = 1;
   static constexpr int RW = WIDE ? 4 : 1;
   static constexpr int ROWS = 32 * RB * RW;
-  static constexpr int WKEYS = WIDE ? (ROW <= 512 ? 64 : 32) : 32;  // keys of a stage that a wave works on
+  static constexpr int WKEYS = (WIDE ? ROW <= 512 : ROW <= 128) ? 64 : 32;  // keys of a stage that a wave works on
   static constexpr int STAGE = WIDE ? WKEYS : WKEYS * NW;
-  static constexpr int LDS = 4 * STAGE * ROW;              // K and V, two buffers
+  static constexpr int BUFFER = STAGE * ROW;
+  static constexpr int LDS = (WIDE ? 4 : 2) * BUFFER;      // K and V; where waves share them two buffers
   static constexpr int PER_CU = LDS <= 80 * 1024 ? 2 : 1;
   static constexpr int WGS = PA_CUS * PER_CU;
+  static constexpr int WAVES = NW * PER_CU >= 4 ? NW * PER_CU / 4 : 1;  // per SIMD
   static constexpr int SLOT = ROWS * (DP + 2);             // floats of a part
 };
 
@@ -260,8 +262,23 @@ __device__ __forceinline__ void pa_reads_stay() {
 #endif
 }
 
+// Waits until no more than N of this wave's loads (LDS: 15 is no wait) are under way. The builtin, not an instruction of inline asm: the
+// compiler counts loads itself, and where it does not see that staged keys have landed it waits for all loads there are.
+template <int LOADS, int LDS>
+__device__ __forceinline__ void pa_wait() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((LOADS & 15) | 7 << 4 | LDS << 8 | (LOADS >> 4) << 14);
+  asm volatile("" ::: "memory");
+#endif
+}
+template <int N>
+__device__ __forceinline__ void pa_landed() { pa_wait<N, 15>(); }
+// What this wave has asked LDS for has been read.
+__device__ __forceinline__ void pa_lds_read() { pa_wait<63, 0>(); }
+
 template <int DT, int DP, bool WIDE>
-__global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WIDE>::PER_CU)) void k_paged_attn(sah_paged_attention_args P) {
+__global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WIDE>::WAVES)) void k_paged_attn(sah_paged_attention_args P) {
   sah_touch_kernargs<sizeof(sah_paged_attention_args)>();
   typedef pa_shape<DT, DP, WIDE> S;
   constexpr int ES = S::ES, NT = S::NT, RB = S::RB, UNITS = S::ROW / 16;
@@ -275,8 +292,8 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
   // place c ^ (j % 16) (8 units: c ^ (j / 2 % 8)); V of 16-bit types: groups of four units (32 dims) at place
   // u ^ (j % 4) (8 units: u ^ (j / 2 % 2)) for the transposing reads. (An array each: the compiler then knows that what is
   // read is not what the loads under way will write.)
-  constexpr int SB = S::STAGE * S::ROW;
-  __shared__ __align__(16) unsigned char s_k0[SB], s_k1[SB], s_v0[SB], s_v1[SB];
+  constexpr int SB = S::BUFFER, SB1 = WIDE ? SB : 16;
+  __shared__ __align__(16) unsigned char s_k0[SB], s_k1[SB1], s_v0[SB], s_v1[SB1];
   __shared__ int64_t s_sum[S::NW + 2];
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
   const int i32 = lane & 31, g = lane >> 5;
@@ -380,8 +397,8 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     // The keys of a stage that this wave works on: a lane holds the page of one, and a bit says which are there. Requested a
     // stage ahead of the loads that go by it.
     const int32_t* table = P.block_table + (int64_t)at.b * P.table_pitch;
-    int page = -1, page_next = -1;
-    auto first_key = [&](int u) { return stages(u) * S::STAGE + (WIDE ? 0 : 32 * wave); };
+    [[maybe_unused]] int page = -1, page_next = -1;
+    auto first_key = [&](int u) { return stages(u) * S::STAGE + (WIDE ? 0 : S::WKEYS * wave); };
     auto fetch_page = [&](int u) -> int {
       const int key = first_key(u) + (S::WKEYS == 64 ? lane : i32);
       return key < at.req.kv ? table[key >> page_shift] : -1;
@@ -392,9 +409,9 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     };
     const char* kbase = (const char*)P.k + (int64_t)at.hk * P.ks_h * ES;
     const char* vbase = (const char*)P.v + (int64_t)at.hk * P.vs_h * ES;
-    auto fetch = [&](int u, int pg, uint64_t there, int buf) __attribute__((always_inline)) {
+    auto fetch = [&](int u, int pg, uint64_t there, int buf, bool with_k, bool with_v) __attribute__((always_inline)) {
       const int key0 = first_key(u);
-      auto stage_at = [&](int at_key) { return ((WIDE ? 0 : 32 * wave) + at_key) * S::ROW; };
+      auto stage_at = [&](int at_key) { return ((WIDE ? 0 : S::WKEYS * wave) + at_key) * S::ROW; };
       if (there == (S::WKEYS == 64 ? ~0ull : 0xffffffffull) && P.page_size >= KPI) {  // uniform
         // All keys are there and an instruction's lie in one page: a scalar base, and a lane's offset that stays the same but for
         // the permutation's part of the instruction (an exclusive or: its key's bits are none of the lane's).
@@ -402,40 +419,47 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
         for (int i = 0; i < IW; ++i) {
           const int at_key = ((WIDE ? wave * IW : 0) + i) * KPI;
           const int64_t p = __builtin_amdgcn_readlane(pg, at_key), entry = (key0 + at_key) & (P.page_size - 1);
-          const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES;
-          const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES;
-          const uint32_t uk = k_unit ^ (16u * f_k(at_key)), uv = v_unit ^ (16u * f_v(at_key));
-          sah_load_lds16(ka + (k_lane + (uk < last_unit ? uk : last_unit)), (buf ? s_k1 : s_k0) + stage_at(at_key));
-          sah_load_lds16(va + (v_lane + (uv < last_unit ? uv : last_unit)), (buf ? s_v1 : s_v0) + stage_at(at_key));
+          if (with_k) {
+            const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES;
+            const uint32_t uk = k_unit ^ (16u * f_k(at_key));
+            sah_buffer_load_lds16(ka, k_lane + (uk < last_unit ? uk : last_unit), (buf ? s_k1 : s_k0) + stage_at(at_key));
+          }
+          if (with_v) {
+            const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES;
+            const uint32_t uv = v_unit ^ (16u * f_v(at_key));
+            sah_buffer_load_lds16(va, v_lane + (uv < last_unit ? uv : last_unit), (buf ? s_v1 : s_v0) + stage_at(at_key));
+          }
         }
         return;
       }
+      // Keys that are not there, or pages smaller than an instruction's keys: every lane its own address, through registers. (A
+      // stage's K and V both come this way or neither: the count of loads under way holds.)
       const int spare = 63 - __builtin_clzll(there | 1);  // stands for keys that are not there
-      // (taken from here: a register for everything that follows from them, kept through the loop, is dearer than two instructions)
-      uint32_t lk = l_key, lp = l_place;
-      sah_keep(lk);
-      sah_keep(lp);
 #pragma unroll 1
       for (int i = 0; i < IW; ++i) {
-        const int at_key = ((WIDE ? wave * IW : 0) + i) * KPI;  // of the wave's keys; a wave with keys of its own stages all of them
-        const int key = at_key + (int)lk;
+        const int at_key = ((WIDE ? wave * IW : 0) + i) * KPI, key = at_key + l_key;
         const int src = (there >> key) & 1 ? key : spare;
         const int page_of = __shfl(pg, src);
         const int64_t p = there ? page_of : 0;  // (nothing there: any page, and nobody reads it)
         const int64_t entry = (key0 + src) & (P.page_size - 1);
-        const uint32_t uk = 16u * (lp ^ f_k(key)), uv = 16u * (lp ^ f_v(key));
-        const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES + (uk < last_unit ? uk : last_unit);
-        const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES + (uv < last_unit ? uv : last_unit);
-        sah_load_lds16(ka, (buf ? s_k1 : s_k0) + stage_at(at_key));
-        sah_load_lds16(va, (buf ? s_v1 : s_v0) + stage_at(at_key));
+        const int to = stage_at(at_key) + 16 * lane;
+        if (with_k) {
+          const uint32_t uk = 16u * (l_place ^ f_k(key));
+          *(sah_u4*)((buf ? s_k1 : s_k0) + to) = *(const sah_u4*)(kbase + (p * P.ks_p + entry * P.ks_t) * ES + (uk < last_unit ? uk : last_unit));
+        }
+        if (with_v) {
+          const uint32_t uv = 16u * (l_place ^ f_v(key));
+          *(sah_u4*)((buf ? s_v1 : s_v0) + to) = *(const sah_u4*)(vbase + (p * P.vs_p + entry * P.vs_t) * ES + (uv < last_unit ? uv : last_unit));
+        }
       }
     };
 
-    auto work = [&](int u, uint64_t there, int buf) __attribute__((always_inline)) {
+    // `between` runs when the stage's keys have been read, before its values are
+    auto work = [&](int u, uint64_t there, int buf, auto between) __attribute__((always_inline)) {
       const int key0 = first_key(u);
-      if (!wave_live || there == 0 || key0 > w_hi) return;  // uniform
-      const unsigned char* kp = (buf ? s_k1 : s_k0) + (WIDE ? 0 : 32 * wave * S::ROW);
-      const unsigned char* vp = (buf ? s_v1 : s_v0) + (WIDE ? 0 : 32 * wave * S::ROW);
+      const bool on = wave_live && there != 0 && key0 <= w_hi;  // uniform
+      const unsigned char* kp = (buf ? s_k1 : s_k0) + (WIDE ? 0 : S::WKEYS * wave * S::ROW);
+      const unsigned char* vp = (buf ? s_v1 : s_v0) + (WIDE ? 0 : S::WKEYS * wave * S::ROW);
       sah_f32x16 s[RB][TW];
 #pragma unroll
       for (int t = 0; t < TW; ++t)
@@ -445,14 +469,15 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
           for (int e = 0; e < 16; ++e) s[rb][t][e] = 0.f;
       // Four pieces of a key tile at a time are read while the four before are multiplied: the reads may not sink to where they
       // are used (a wait for each then: 778 us of the chunk's pass instead of %QK% with both products so).
-      {
+      if (on) {
         constexpr int C = 4, NC = TW * KQ / C;
         uint4 a[2][C];
         auto read = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
           for (int i = 0; i < C; ++i) {
             const int t = c * C / KQ, st = c * C % KQ + i;
-            a[c & 1][i] = *(const uint4*)(kp + 32 * t * S::ROW + (k_at ^ (32 * st)));
+            const sah_u4 v = *(const sah_u4*)(kp + 32 * t * S::ROW + (k_at ^ (32 * st)));
+            a[c & 1][i] = make_uint4(v.x, v.y, v.z, v.w);
           }
         };
         read(0);
@@ -478,6 +503,8 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
           }
         }
       }
+      between();
+      if (!on) return;
       // the first values, requested ahead of the softmax
       constexpr int NV = 2 * TW;
       uint4 va[2][DT == SAH_F32 ? 1 : DTL];
@@ -512,7 +539,10 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
             word &= (uint32_t)(there >> (32 * t));
             word >>= 4 * g;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[rb][t][e] = (word >> (8 * (e / 4) + e % 4)) & 1 ? s[rb][t][e] : -INFINITY;
+            for (int e = 0; e < 16; ++e) {
+              const uint32_t on = (uint32_t)((int)(word << (31 - (8 * (e / 4) + e % 4))) >> 31);  // all ones where the row sees the key
+              s[rb][t][e] = sah_bits_to_float((sah_float_to_bits(s[rb][t][e]) & on) | (0xff800000u & ~on));
+            }
           }
         }
       }
@@ -576,28 +606,62 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       }
     };
 
-    auto stage = [&](int u, int buf) __attribute__((always_inline)) {  // buf: a constant in the loop below
-      const uint64_t there = there_of(page);
-      if (u + 1 < u1) {
-        page = page_next;
-        fetch(u + 1, page, there_of(page), buf ^ 1);  // the other buffer: read for the last time before the previous wait
-        if (u + 2 < u1) page_next = fetch_page(u + 2);
+    if constexpr (WIDE) {
+      auto stage = [&](int u, int buf) __attribute__((always_inline)) {  // buf: a constant in the loop below
+        const uint64_t there = there_of(page);
+        if (u + 1 < u1) {
+          page = page_next;
+          fetch(u + 1, page, there_of(page), buf ^ 1, true, true);  // the other buffer: read for the last time before the previous wait
+          if (u + 2 < u1) page_next = fetch_page(u + 2);
+        }
+        work(u, there, buf, [] {});
+        sah_stores_done();  // this wave's loads into LDS have landed
+        __syncthreads();
+      };
+      if (u0 < u1) {
+        page = fetch_page(u0);
+        if (u0 + 1 < u1) page_next = fetch_page(u0 + 1);
+        fetch(u0, page, there_of(page), 0, true, true);
+        sah_stores_done();
+        __syncthreads();
+        for (int u = u0; u < u1; u += 2) {
+          stage(u, 0);
+          if (u + 1 < u1) stage(u + 1, 1);
+        }
       }
-      work(u, there, buf);
-      sah_stores_done();  // this wave's loads into LDS have landed
-      if (WIDE) __syncthreads();
-      else sah_wave_lds_sync();
-    };
-    if (u0 < u1) {
-      page = fetch_page(u0);
-      if (u0 + 1 < u1) page_next = fetch_page(u0 + 1);
-      fetch(u0, page, there_of(page), 0);
-      sah_stores_done();
-      if (WIDE) __syncthreads();
-      else sah_wave_lds_sync();
-      for (int u = u0; u < u1; u += 2) {
-        stage(u, 0);
-        if (u + 1 < u1) stage(u + 1, 1);
+    } else {
+      // A wave's own keys, with nobody to wait for: a stage's K is overwritten by the next one's as soon as it has been multiplied,
+      // its V likewise, so that half a stage of loads or more is under way all the time (8 waves of 16 KB a stage and CU at 128 x 2
+      // bytes). Loads land in the order they were asked for in: waiting for K means waiting until no more than what was
+      // requested after it is left. Pages are requested a stage ahead of the loads that go by them.
+      static_assert(IW <= 32, "counted in six bits");
+      if (u0 < u1) {
+        int pg = fetch_page(u0);
+        int pg_next = u0 + 1 < u1 ? fetch_page(u0 + 1) : -1;
+        uint64_t there = there_of(pg);
+        fetch(u0, pg, there, 0, true, false);
+        fetch(u0, pg, there, 0, false, true);
+        // (the last stage apart: a way through the loop that skips a request would have the compiler wait for all of them)
+        int u = u0;
+#pragma unroll 1
+        for (; u + 1 < u1; ++u) {
+          uint64_t there_next = 0;
+          pa_landed<IW>();  // K
+          work(u, there, 0, [&]() __attribute__((always_inline)) {
+            pg = pg_next;
+            there_next = there_of(pg);
+            pg_next = fetch_page(u + 2 < u1 ? u + 2 : u + 1);
+            pa_lds_read();
+            fetch(u + 1, pg, there_next, 0, true, false);
+            pa_landed<IW>();  // V
+          });
+          pa_lds_read();
+          fetch(u + 1, pg, there_next, 0, false, true);
+          there = there_next;
+        }
+        pa_landed<IW>();
+        work(u, there, 0, []() __attribute__((always_inline)) { pa_landed<0>(); });
+        pa_landed<0>();
       }
     }
 
@@ -607,9 +671,9 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       // the waves' shares of the keys are joined in LDS
       __syncthreads();  // every wave has read its stages
       constexpr int PER = SB / (16 * DTL * SAH_WAVE * 4);  // waves' tiles, [element][lane], that a buffer holds
-      static_assert(PER >= 1 && PER * 4 >= S::NW - 1 && RB == 1, "room for the waves' tiles");
+      static_assert(PER >= 1 && PER * 2 >= S::NW - 1 && RB == 1, "room for the waves' tiles");
       auto tile_of = [&](int v) -> float* {
-        unsigned char* base = v / PER == 0 ? s_k0 : v / PER == 1 ? s_k1 : v / PER == 2 ? s_v0 : s_v1;
+        unsigned char* base = v / PER == 0 ? s_k0 : s_v0;
         return (float*)base + (v % PER) * 16 * DTL * SAH_WAVE;
       };
       __shared__ float s_ml[S::NW][2][SAH_WAVE];
@@ -957,6 +1021,8 @@ extern "C" int sah_paged_attention(const sah_paged_attention_args* a) {
   if (((uint64_t)a->q | (uint64_t)a->k | (uint64_t)a->v | (uint64_t)a->out | (uint64_t)a->work |
        (uint64_t)(es * (a->qs_t | a->qs_h | a->ks_p | a->ks_t | a->ks_h | a->vs_p | a->vs_t | a->vs_h | a->os_t | a->os_h))) % 16)
     return sah_fail(SAH_EINVAL, "sah_paged_attention: addresses and strides must be multiples of 16 bytes");
+  if (a->ks_t < 0 || a->vs_t < 0 || a->ks_t >= 1 << 26 || a->vs_t >= 1 << 26)  // a few tokens of a page: 32-bit offsets
+    return sah_fail(SAH_ESHAPE, "sah_paged_attention: a page's tokens are 2^26 elements or more apart");
   if (!(a->scaling - a->scaling == 0.f)) return sah_fail(SAH_EINVAL, "sah_paged_attention: scaling is not finite");
   if (!a->work || a->work_floats < sah_paged_attention_work_floats(a)) return sah_fail(SAH_ECAPACITY, "sah_paged_attention: work is too small");
   return (int)pa_dispatch(a, pa_launch_fn{a});

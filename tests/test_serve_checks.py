@@ -97,7 +97,7 @@ def test_store_refuses(changes, code):
     (dict(D=0), -3), (dict(page_size=24), -3), (dict(page_size=0), -3), (dict(table_width=2 ** 28, table_pitch=2 ** 28), -3),
     (dict(table_pitch=3), -1), (dict(q=None), -2), (dict(k=None), -2), (dict(v=None), -2), (dict(block_table=None), -2),
     (dict(kv_lens=None), -2), (dict(cu_new=None), -2), (dict(out=None), -2), (dict(q=_PTR + 2), -1), (dict(k=_PTR + 8), -1), (dict(ks_t=129), -1),
-    (dict(qs_h=65), -1), (dict(os_t=257), -1), (dict(scaling=float("nan")), -1),
+    (dict(qs_h=65), -1), (dict(ks_t=2 ** 26), -3), (dict(vs_t=-64), -3), (dict(os_t=257), -1), (dict(scaling=float("nan")), -1),
 ])
 def test_attention_refuses(changes, code):
     args = N.PagedAttentionArgs(_PTR, 256, 64, _PTR, 2048, 128, 64, _PTR, 2048, 128, 64, _PTR, 4, 4, _PTR, _PTR, None, 1, 2, 3, 4, 2, 64, 8, 16,
