@@ -310,12 +310,17 @@ __device__ __forceinline__ void sah_load_lds16(const void* p, void* lds) {
 }
 // The same from a wave-uniform address plus a byte offset per lane, as a buffer load: the compiler counts these apart from its loads
 // through pointers, which it takes to come back out of order once they write LDS (any wait becomes one for all of them).
-__device__ __forceinline__ void sah_buffer_load_lds16(const void* base, uint32_t offset, void* lds) {
+// Lanes at an offset of `bytes` or more write zeros and read nothing (checked on the hardware).
+__device__ __forceinline__ void sah_buffer_load_lds16(const void* base, uint32_t bytes, uint32_t offset, void* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, -1, 0x00027000);
+  // (Said to be uniform, value by value: where the compiler is not sure it makes a loop over the lanes' values, and has put copies of
+  // registers behind that loop, where no lane is active, before the lanes are switched on again.)
+  const uint64_t at = (uint64_t)base;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)at), hi = __builtin_amdgcn_readfirstlane((int)(at >> 32));
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00027000);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, (int)offset, 0, 0, 0);
 #else
-  (void)base; (void)offset; (void)lds;
+  (void)base; (void)bytes; (void)offset; (void)lds;
 #endif
 }
 // Transposing LDS read, one 4 x 16 block of 16-bit elements per 16 lanes (layout checked on the hardware): lane l hands in
@@ -549,6 +554,26 @@ __device__ __forceinline__ int sah_wave_incl_scan(int v) {
   v += sah_dpp_i<0x142, 0xA, false>(v);  // row_bcast:15 into rows 1 and 3
   v += sah_dpp_i<0x143, 0xC, false>(v);  // row_bcast:31 into rows 2 and 3
   return v;
+}
+
+// The same of 64-bit numbers, all lanes active, and a lane's number to all of them
+template <int CTRL, int ROW_MASK, bool BOUND>
+__device__ __forceinline__ uint64_t sah_dpp_u64(uint64_t v) {
+  const uint32_t lo = (uint32_t)sah_dpp_i<CTRL, ROW_MASK, BOUND>((int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)sah_dpp_i<CTRL, ROW_MASK, BOUND>((int)(uint32_t)(v >> 32));
+  return ((uint64_t)hi << 32) | lo;
+}
+__device__ __forceinline__ uint64_t sah_wave_incl_scan_u64(uint64_t v) {
+  v += sah_dpp_u64<0x111, 0xF, true>(v);
+  v += sah_dpp_u64<0x112, 0xF, true>(v);
+  v += sah_dpp_u64<0x114, 0xF, true>(v);
+  v += sah_dpp_u64<0x118, 0xF, true>(v);
+  v += sah_dpp_u64<0x142, 0xA, false>(v);
+  v += sah_dpp_u64<0x143, 0xC, false>(v);
+  return v;
+}
+__device__ __forceinline__ uint64_t sah_lane_u64(uint64_t v, int lane) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
 
 // sum over the wave; every lane gets it

@@ -10,12 +10,7 @@
 __device__ __forceinline__ int64_t pg_scan(int64_t v, int64_t* wsum, int64_t* total) {
   constexpr int NW = PG_NT / SAH_WAVE;
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
-  int64_t incl = v;
-#pragma unroll
-  for (int d = 1; d < SAH_WAVE; d <<= 1) {
-    const int64_t up = __shfl_up((long long)incl, d);
-    if (lane >= d) incl += up;
-  }
+  const int64_t incl = (int64_t)sah_wave_incl_scan_u64((uint64_t)v);
   __syncthreads();  // wsum may still be read from the call before
   if (lane == SAH_WAVE - 1) wsum[wave] = incl;
   __syncthreads();

@@ -15,6 +15,14 @@
 #include "../../include/sah_serve.h"
 
 #define PA_MAX_D 256
+#define PA_C 4
+#define PA_V 4
+
+
+
+
+
+
 #define PA_CUS 256
 #define PA_XCDS 8
 #define PA_TILE_COST 96   // what starting and ending a tile costs, in keys
@@ -40,6 +48,21 @@ struct pa_shape {
   static constexpr int SLOT = ROWS * (DP + 2);             // floats of a part
 };
 
+// The kernel's arguments where they lie. Each call gives an address that the compiler knows nothing of, so that what is read behind it is
+// read again for every tile: all of them kept in scalar registers from the kernel's first line on, two hundred of those go
+// to vector registers and come back in the innermost loop (2048 tokens over 18432 keys: 850 us instead of %KARG%).
+typedef const sah_paged_attention_args __attribute__((address_space(4))) pa_args;
+__device__ __forceinline__ pa_args& pa_arguments() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  pa_args* p = (pa_args*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+#else
+  static pa_args* none;
+  return *none;
+#endif
+}
+
 // ---------------------------------------------------------------------------
 // where the work is
 // ---------------------------------------------------------------------------
@@ -48,7 +71,7 @@ struct pa_request {
   int kv;            // keys it has
   int64_t base;      // row t stands at position base + t
 };
-__device__ __forceinline__ pa_request pa_read_request(const sah_paged_attention_args& P, int b) {
+__device__ __forceinline__ pa_request pa_read_request(pa_args& P, int b) {
   pa_request r;
   const int begin = P.cu_new[b], end = P.cu_new[b + 1];
   int kv = P.kv_lens[b];
@@ -66,6 +89,22 @@ __device__ __forceinline__ int pa_position(const pa_request& r, int i) {
   return (int)(p < -1 ? -1 : (p < 0x7ffffffe ? p : 0x7ffffffe));
 }
 
+// What all lanes of the wave hold, in scalar registers (doubles are divided in vector ones)
+__device__ __forceinline__ int64_t pa_uniform(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// a / b for 0 <= a < 2^53, 0 < b: exact. (The 64-bit division of integers is some 150 instructions, and a dozen of them stand
+// before a workgroup's first load.)
+__device__ __forceinline__ int64_t pa_div(int64_t a, int64_t b) {
+  int64_t q = (int64_t)((double)a / (double)b);
+  const int64_t r = a - q * b;
+  q -= r < 0;
+  q += r >= b;
+  return q;
+}
+
 // Cost of the tiles of one request and head: tile i's is min(first + (i + 1) step, most) + PA_TILE_COST. About the keys it
 // reads; only the balance depends on it.
 struct pa_cost {
@@ -76,8 +115,8 @@ struct pa_cost {
     return (c < most ? c : most) + PA_TILE_COST;
   }
   __device__ __forceinline__ int64_t before(int i) const {  // of tiles 0 .. i - 1
-    int64_t j = most > first ? (most - first) / step : 0;
-    if (j > i) j = i;
+    int64_t j = i;
+    if (first + i * step > most) j = most > first ? pa_div(most - first, step) : 0;
     return j * first + step * (j * (j + 1) / 2) + (i - j) * most + (int64_t)i * PA_TILE_COST;
   }
   __device__ __forceinline__ int at(int64_t y) const {  // the tile whose piece of the line holds y
@@ -90,7 +129,7 @@ struct pa_cost {
   }
 };
 template <int ROWS>
-__device__ __forceinline__ pa_cost pa_cost_of(const sah_paged_attention_args& P, const pa_request& r) {
+__device__ __forceinline__ pa_cost pa_cost_of(pa_args& P, const pa_request& r) {
   const int G = P.Hq / P.Hkv;
   pa_cost c;
   c.tiles = (int)(((int64_t)r.n_new * G + ROWS - 1) / ROWS);
@@ -109,88 +148,97 @@ struct pa_place {
   pa_cost costs;
 };
 
-__device__ __forceinline__ int64_t pa_uniform(int64_t v) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
-  return (int64_t)(((uint64_t)hi << 32) | lo);
-}
 
-// The line's length, and how many workgroups share it. All NT threads call.
-template <int NT, int ROWS>
-__device__ __forceinline__ int64_t pa_total(const sah_paged_attention_args& P, int64_t* s_sum) {
-  int64_t sum = 0;
-  for (int b = threadIdx.x; b < P.n_requests; b += NT) {
-    const pa_cost c = pa_cost_of<ROWS>(P, pa_read_request(P, b));
-    sum += c.before(c.tiles);
-  }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor((long long)sum, d);
-  if (threadIdx.x % SAH_WAVE == 0) s_sum[threadIdx.x / SAH_WAVE] = sum;
-  __syncthreads();
-  sum = 0;
-#pragma unroll
-  for (int i = 0; i < NT / SAH_WAVE; ++i) sum += s_sum[i];
-  __syncthreads();
-  return pa_uniform(sum * P.Hkv);
-}
 __device__ __forceinline__ int pa_sharers(int64_t total, int wgs) {
   const int64_t w = (total + PA_MIN_COST - 1) / PA_MIN_COST;
   return (int)(w < wgs ? w : wgs);
 }
 // where workgroup w of n begins
-__device__ __forceinline__ int64_t pa_bound(int64_t total, int n, int w) { return total / n * w + total % n * w / n; }
+__device__ __forceinline__ int64_t pa_bound(int64_t total, int n, int w) {
+  const int64_t each = pa_uniform(pa_div(total, n));
+  return each * w + pa_uniform(pa_div((total - each * n) * w, n));
+}
 
-// The place that holds x, 0 <= x < total. All NT threads call; s_sum: NT / 64 + 2 words.
+// Workgroup w's piece of the line, [x0, x1), and the place that holds x0
+struct pa_piece {
+  int64_t total, x0, x1;
+  int sharers;   // workgroups that have a piece; without one x0 and x1 say nothing
+  pa_place at;
+};
+// s_sum: NT / 64 + 2 words. All NT threads call.
 template <int NT, int ROWS>
-__device__ __forceinline__ pa_place pa_find(const sah_paged_attention_args& P, int64_t x, int64_t* s_sum) {
+__device__ __forceinline__ pa_piece pa_start(pa_args& P, int wgs, int w, int64_t* s_sum) {
   constexpr int NW = NT / SAH_WAVE;
   const int lane = threadIdx.x % SAH_WAVE, wave = sah_wave_id();
-  int64_t run = 0;
-  for (int b0 = 0; b0 < P.n_requests; b0 += NT) {
-    const int b = b0 + threadIdx.x;
-    int64_t mine = 0;
-    if (b < P.n_requests) {
-      const pa_cost c = pa_cost_of<ROWS>(P, pa_read_request(P, b));
-      mine = c.before(c.tiles) * P.Hkv;
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int d = 1; d < SAH_WAVE; d <<= 1) {
-      const int64_t up = __shfl_up((long long)incl, d);
-      if (lane >= d) incl += up;
-    }
+  pa_piece r;
+  auto cost_of = [&](int b) -> int64_t {
+    if (b >= P.n_requests) return 0;
+    const pa_cost c = pa_cost_of<ROWS>(P, pa_read_request(P, b));
+    return c.before(c.tiles) * P.Hkv;
+  };
+  auto scan = [&](int64_t v, int64_t& all) -> int64_t {  // inclusive
+    const int64_t incl = (int64_t)sah_wave_incl_scan_u64((uint64_t)v);
     if (lane == SAH_WAVE - 1) s_sum[wave] = incl;
     __syncthreads();
-    int64_t before = run, all = 0;
+    int64_t before = 0;
+    all = 0;
 #pragma unroll
     for (int i = 0; i < NW; ++i) {
       before += i < wave ? s_sum[i] : 0;
       all += s_sum[i];
     }
-    incl += before;
-    if (mine && incl > x && incl - mine <= x) {  // one thread
+    all = pa_uniform(all);
+    return before + incl;
+  };
+  auto share = [&](int64_t total) {
+    r.total = total;
+    r.sharers = pa_sharers(total, wgs);
+    r.x0 = w < r.sharers ? pa_bound(total, r.sharers, w) : 0;
+    r.x1 = w < r.sharers ? pa_bound(total, r.sharers, w + 1) : 0;
+  };
+  auto claim = [&](int b, int64_t mine, int64_t end) {  // one thread's request holds x0
+    if (mine && end > r.x0 && end - mine <= r.x0) {
       s_sum[NW] = b;
-      s_sum[NW + 1] = incl - mine;
+      s_sum[NW + 1] = end - mine;
     }
-    run += all;
+  };
+  if (P.n_requests <= NT) {
+    const int64_t mine = cost_of(threadIdx.x);
+    int64_t all;
+    const int64_t end = scan(mine, all);
+    share(all);
+    claim(threadIdx.x, mine, end);
     __syncthreads();
-    if (run > x) break;
+  } else {
+    int64_t sum = 0, all, run = 0;
+    for (int b = threadIdx.x; b < P.n_requests; b += NT) sum += cost_of(b);
+    scan(sum, all);
+    share(all);
+    for (int b0 = 0; b0 < P.n_requests; b0 += NT) {
+      const int64_t mine = cost_of(b0 + threadIdx.x);
+      __syncthreads();
+      const int64_t end = run + scan(mine, all);
+      claim(b0 + threadIdx.x, mine, end);
+      run += all;
+    }
+    __syncthreads();
   }
-  pa_place at;
+  if (w >= r.sharers) return r;
+  pa_place& at = r.at;
   at.b = __builtin_amdgcn_readfirstlane((int)s_sum[NW]);
   const int64_t begin = pa_uniform(s_sum[NW + 1]);
   at.req = pa_read_request(P, at.b);
   at.costs = pa_cost_of<ROWS>(P, at.req);
   const int64_t head = at.costs.before(at.costs.tiles);
-  at.hk = (int)((x - begin) / head);
-  const int64_t y = x - begin - at.hk * head;
-  at.tile = at.costs.at(y);
-  at.begin = begin + at.hk * head + at.costs.before(at.tile);
-  at.cost = at.costs.of(at.tile);
-  return at;
+  at.hk = (int)pa_uniform(pa_div(r.x0 - begin, head));
+  at.tile = __builtin_amdgcn_readfirstlane(at.costs.at(r.x0 - begin - at.hk * head));
+  at.begin = pa_uniform(begin + at.hk * head + at.costs.before(at.tile));
+  at.cost = pa_uniform(at.costs.of(at.tile));
+  return r;
 }
 // the next tile on the line; there is one
 template <int ROWS>
-__device__ __forceinline__ void pa_next(const sah_paged_attention_args& P, pa_place& at) {
+__device__ __forceinline__ void pa_next(pa_args& P, pa_place& at) {
   at.begin += at.cost;
   if (++at.tile == at.costs.tiles) {
     at.tile = 0;
@@ -203,7 +251,7 @@ __device__ __forceinline__ void pa_next(const sah_paged_attention_args& P, pa_pl
       } while (at.costs.tiles == 0);
     }
   }
-  at.cost = at.costs.of(at.tile);
+  at.cost = pa_uniform(at.costs.of(at.tile));
 }
 
 // what a workgroup leaves for the second kernel
@@ -220,7 +268,7 @@ struct pa_stages {
   __device__ __forceinline__ int operator()(int u) const { return u < n_sink ? u : u - n_sink + from; }
 };
 template <int STAGE>
-__device__ __forceinline__ pa_stages pa_stages_of(const sah_paged_attention_args& P, const pa_request& r, int p_lo, int p_hi) {
+__device__ __forceinline__ pa_stages pa_stages_of(pa_args& P, const pa_request& r, int p_lo, int p_hi) {
   pa_stages s;
   const int hi = p_hi < r.kv - 1 ? p_hi : r.kv - 1;  // the last key that any row sees
   s.n_sink = 0;
@@ -278,7 +326,7 @@ __device__ __forceinline__ void pa_landed() { pa_wait<N, 15>(); }
 __device__ __forceinline__ void pa_lds_read() { pa_wait<63, 0>(); }
 
 template <int DT, int DP, bool WIDE>
-__global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WIDE>::WAVES)) void k_paged_attn(sah_paged_attention_args P) {
+__global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WIDE>::WAVES)) void k_paged_attn(sah_paged_attention_args) {
   sah_touch_kernargs<sizeof(sah_paged_attention_args)>();
   typedef pa_shape<DT, DP, WIDE> S;
   constexpr int ES = S::ES, NT = S::NT, RB = S::RB, UNITS = S::ROW / 16;
@@ -298,33 +346,23 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
   const int i32 = lane & 31, g = lane >> 5;
   const int rw = WIDE ? wave : 0;
-  const int G = P.Hq / P.Hkv;
   // neighbours on the line of work share keys: they get the same XCD
   const int w = (int)(blockIdx.x % PA_XCDS) * (S::WGS / PA_XCDS) + (int)(blockIdx.x / PA_XCDS);
-  pa_note* notes = (pa_note*)P.work;
-  float* parts = P.work + S::WGS * (sizeof(pa_note) / 4);
-  const int64_t total = pa_total<NT, S::ROWS>(P, s_sum);
-  const int sharers = pa_sharers(total, S::WGS);
   if (threadIdx.x == 0) {
-    notes[w].b = -1;
-    notes[w].again = 0;
+    pa_note* note = (pa_note*)pa_arguments().work + w;
+    note->b = -1;
+    note->again = 0;
   }
+  const pa_piece piece = pa_start<NT, S::ROWS>(pa_arguments(), S::WGS, w, s_sum);
+  const int sharers = piece.sharers;
   if (w >= sharers) return;
-  const int64_t x1 = pa_bound(total, sharers, w + 1);
-  int64_t x = pa_bound(total, sharers, w);
-  pa_place at = pa_find<NT, S::ROWS>(P, x, s_sum);
-  const int page_shift = 31 - __builtin_clz(P.page_size);
-  const float c_exp = fmaxf(fabsf(P.scaling) * 1.4426950408889634f, 1e-37f);
-
+  const int64_t total = piece.total, x1 = piece.x1;
+  int64_t x = piece.x0;
+  pa_place at = piece.at;
   // this lane's share of a load instruction, and where it reads what has been staged
   const int l_key = lane / UNITS, l_place = lane % UNITS;
   auto f_k = [](int key) { return UNITS == 8 ? (key >> 1) & 7 : key & 15; };
   auto f_v = [](int key) { return DT == SAH_F32 ? 0 : UNITS == 8 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); };
-  // (places behind a shorter head's end hold its last unit again: the queries are 0 there, the results nobody's)
-  const int units_real = P.D * ES / 16;
-  const uint32_t last_unit = 16u * (units_real - 1);
-  const uint32_t k_unit = 16u * (l_place ^ f_k(l_key)), v_unit = 16u * (l_place ^ f_v(l_key));
-  const uint32_t k_lane = (uint32_t)(l_key * P.ks_t * ES), v_lane = (uint32_t)(l_key * P.vs_t * ES);
   const int k_at = i32 * S::ROW + 16 * (g ^ f_k(i32));
   int v_at[DTL];
 #pragma unroll
@@ -335,15 +373,29 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
 
   bool bad = false;  // a row of a whole tile came out not finite
   for (;;) {
+    pa_args& P = pa_arguments();
+    const int G = P.Hq / P.Hkv, page_shift = 31 - __builtin_clz(P.page_size);
+    const float c_exp = fmaxf(fabsf(P.scaling) * 1.4426950408889634f, 1e-37f);
+    // (places behind a shorter head's end hold its last unit again: the queries are 0 there, the results nobody's)
+    const int units_real = P.D * ES / 16;
+    const uint32_t last_unit = 16u * (units_real - 1);
+    const uint32_t k_unit = 16u * (l_place ^ f_k(l_key)), v_unit = 16u * (l_place ^ f_v(l_key));
+    // an instruction's keys lie in one page, and a key's elements before the next key's
+    const bool regular = P.page_size >= KPI && P.ks_t >= P.D && P.vs_t >= P.D;
+    const uint32_t k_lane = (uint32_t)(l_key * P.ks_t * ES), v_lane = (uint32_t)(l_key * P.vs_t * ES);
     const int64_t y0 = x - at.begin, y1 = x1 - at.begin < at.cost ? x1 - at.begin : at.cost;
     const bool whole = y0 == 0 && y1 == at.cost;
     const int row_first = at.tile * S::ROWS;
     const int n_rows = at.req.n_new * G;  // (n_new <= n_tokens, and n_tokens * Hq fits: the host has checked)
     const int row_last = row_first + S::ROWS < n_rows ? row_first + S::ROWS - 1 : n_rows - 1;
     const pa_stages stages = pa_stages_of<S::STAGE>(P, at.req, pa_position(at.req, row_first / G), pa_position(at.req, row_last / G));
-    const int u0 = (int)(y0 * stages.n / at.cost), u1 = y1 == at.cost ? stages.n : (int)(y1 * stages.n / at.cost);
+    const int u0 = y0 == 0 ? 0 : (int)pa_uniform(pa_div(y0 * stages.n, at.cost)), u1 = y1 == at.cost ? stages.n : (int)pa_uniform(pa_div(y1 * stages.n, at.cost));
 
     // this lane's rows; lanes beyond the last repeat it and store nothing
+    // (its place in the wave is taken anew for every tile, as the kernel's arguments are: what follows from it, kept, is 80 registers)
+    uint32_t kept_lane = lane;
+    sah_keep(kept_lane);
+    const int i32 = kept_lane & 31, g = kept_lane >> 5;
     int pos[RB], tok[RB], head[RB];
     bool live[RB];
     uint4 qf[RB][KQ];
@@ -412,22 +464,26 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     auto fetch = [&](int u, int pg, uint64_t there, int buf, bool with_k, bool with_v) __attribute__((always_inline)) {
       const int key0 = first_key(u);
       auto stage_at = [&](int at_key) { return ((WIDE ? 0 : S::WKEYS * wave) + at_key) * S::ROW; };
-      if (there == (S::WKEYS == 64 ? ~0ull : 0xffffffffull) && P.page_size >= KPI) {  // uniform
-        // All keys are there and an instruction's lie in one page: a scalar base, and a lane's offset that stays the same but for
-        // the permutation's part of the instruction (an exclusive or: its key's bits are none of the lane's).
+      const int left = at.req.kv - key0;  // the request's keys from here on
+      const uint64_t held = left >= S::WKEYS ? (S::WKEYS == 64 ? ~0ull : 0xffffffffull) : left > 0 ? (1ull << left) - 1 : 0;
+      if (there == held && regular) {  // uniform
+        // All of them are there and an instruction's lie in one page: a scalar base, and a lane's offset that stays the same but for
+        // the permutation's part of the instruction (an exclusive or: its key's bits are none of the lane's). Keys behind
+        // the request's last come as zeros.
 #pragma unroll
         for (int i = 0; i < IW; ++i) {
           const int at_key = ((WIDE ? wave * IW : 0) + i) * KPI;
-          const int64_t p = __builtin_amdgcn_readlane(pg, at_key), entry = (key0 + at_key) & (P.page_size - 1);
+          const int here = left - at_key, page_of = __builtin_amdgcn_readlane(pg, at_key);
+          const int64_t p = here > 0 ? page_of : 0, entry = (key0 + at_key) & (P.page_size - 1);
           if (with_k) {
             const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES;
             const uint32_t uk = k_unit ^ (16u * f_k(at_key));
-            sah_buffer_load_lds16(ka, k_lane + (uk < last_unit ? uk : last_unit), (buf ? s_k1 : s_k0) + stage_at(at_key));
+            sah_buffer_load_lds16(ka, here >= KPI ? ~0u : here > 0 ? (uint32_t)(here * P.ks_t * ES) : 0u, k_lane + (uk < last_unit ? uk : last_unit), (buf ? s_k1 : s_k0) + stage_at(at_key));
           }
           if (with_v) {
             const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES;
             const uint32_t uv = v_unit ^ (16u * f_v(at_key));
-            sah_buffer_load_lds16(va, v_lane + (uv < last_unit ? uv : last_unit), (buf ? s_v1 : s_v0) + stage_at(at_key));
+            sah_buffer_load_lds16(va, here >= KPI ? ~0u : here > 0 ? (uint32_t)(here * P.vs_t * ES) : 0u, v_lane + (uv < last_unit ? uv : last_unit), (buf ? s_v1 : s_v0) + stage_at(at_key));
           }
         }
         return;
@@ -435,21 +491,26 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       // Keys that are not there, or pages smaller than an instruction's keys: every lane its own address, through registers. (A
       // stage's K and V both come this way or neither: the count of loads under way holds.)
       const int spare = 63 - __builtin_clzll(there | 1);  // stands for keys that are not there
+      constexpr int U = IW < 2 ? IW : 2;
 #pragma unroll 1
-      for (int i = 0; i < IW; ++i) {
-        const int at_key = ((WIDE ? wave * IW : 0) + i) * KPI, key = at_key + l_key;
-        const int src = (there >> key) & 1 ? key : spare;
-        const int page_of = __shfl(pg, src);
-        const int64_t p = there ? page_of : 0;  // (nothing there: any page, and nobody reads it)
-        const int64_t entry = (key0 + src) & (P.page_size - 1);
-        const int to = stage_at(at_key) + 16 * lane;
-        if (with_k) {
-          const uint32_t uk = 16u * (l_place ^ f_k(key));
-          *(sah_u4*)((buf ? s_k1 : s_k0) + to) = *(const sah_u4*)(kbase + (p * P.ks_p + entry * P.ks_t) * ES + (uk < last_unit ? uk : last_unit));
+      for (int i0 = 0; i0 < IW; i0 += U) {
+        sah_u4 k[U], v[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int key = ((WIDE ? wave * IW : 0) + i0 + i) * KPI + l_key;
+          const int src = (there >> key) & 1 ? key : spare;
+          const int page_of = __shfl(pg, src);
+          const int64_t p = there ? page_of : 0;  // (nothing there: any page, and nobody reads it)
+          const int64_t entry = (key0 + src) & (P.page_size - 1);
+          const uint32_t uk = 16u * (l_place ^ f_k(key)), uv = 16u * (l_place ^ f_v(key));
+          if (with_k) k[i] = *(const sah_u4*)(kbase + (p * P.ks_p + entry * P.ks_t) * ES + (uk < last_unit ? uk : last_unit));
+          if (with_v) v[i] = *(const sah_u4*)(vbase + (p * P.vs_p + entry * P.vs_t) * ES + (uv < last_unit ? uv : last_unit));
         }
-        if (with_v) {
-          const uint32_t uv = 16u * (l_place ^ f_v(key));
-          *(sah_u4*)((buf ? s_v1 : s_v0) + to) = *(const sah_u4*)(vbase + (p * P.vs_p + entry * P.vs_t) * ES + (uv < last_unit ? uv : last_unit));
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int to = stage_at(((WIDE ? wave * IW : 0) + i0 + i) * KPI) + 16 * lane;
+          if (with_k) *(sah_u4*)((buf ? s_k1 : s_k0) + to) = k[i];
+          if (with_v) *(sah_u4*)((buf ? s_v1 : s_v0) + to) = v[i];
         }
       }
     };
@@ -470,7 +531,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       // Four pieces of a key tile at a time are read while the four before are multiplied: the reads may not sink to where they
       // are used (a wait for each then: 778 us of the chunk's pass instead of %QK% with both products so).
       if (on) {
-        constexpr int C = 4, NC = TW * KQ / C;
+        constexpr int C = PA_C, NC = TW * KQ / C;
         uint4 a[2][C];
         auto read = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
@@ -506,13 +567,13 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       between();
       if (!on) return;
       // the first values, requested ahead of the softmax
-      constexpr int NV = 2 * TW;
-      uint4 va[2][DT == SAH_F32 ? 1 : DTL];
+      constexpr int DV = DTL < PA_V ? DTL : PA_V, NV = 2 * TW * (DTL / DV);  // 32-dim tiles of a piece, pieces
+      uint4 va[2][DT == SAH_F32 ? 1 : DV];
       auto read_v = [&](int c) __attribute__((always_inline)) {
         if constexpr (DT != SAH_F32) {
 #pragma unroll
-          for (int d = 0; d < DTL; ++d) {
-            const unsigned char* v = vp + 16 * c * S::ROW + v_at[d];
+          for (int d = 0; d < DV; ++d) {
+            const unsigned char* v = vp + 16 * (c / (DTL / DV)) * S::ROW + v_at[c % (DTL / DV) * DV + d];
             const sah_u2 a0 = sah_read_tr16((const uint16_t*)v), a1 = sah_read_tr16((const uint16_t*)(v + 8 * S::ROW));
             va[c & 1][d] = make_uint4(a0.x, a0.y, a1.x, a1.y);
           }
@@ -591,7 +652,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       } else {
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
-          const int t = c / 2, st = c % 2;
+          const int step = c / (DTL / DV), t = step / 2, st = step % 2;
           if (c + 1 < NV) read_v(c + 1);
           pa_reads_stay();
 #pragma unroll
@@ -600,7 +661,10 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
             const uint4 pt = make_uint4(sah_pack2_hw<DT>(z[8 * st], z[8 * st + 1]), sah_pack2_hw<DT>(z[8 * st + 2], z[8 * st + 3]),
                                         sah_pack2_hw<DT>(z[8 * st + 4], z[8 * st + 5]), sah_pack2_hw<DT>(z[8 * st + 6], z[8 * st + 7]));
 #pragma unroll
-            for (int d = 0; d < DTL; ++d) acc[rb][d] = sah_mfma_32x32x16<DT>(va[c & 1][d], pt, acc[rb][d]);
+            for (int d = 0; d < DV; ++d) {
+              const int to = c % (DTL / DV) * DV + d;
+              acc[rb][to] = sah_mfma_32x32x16<DT>(va[c & 1][d], pt, acc[rb][to]);
+            }
           }
         }
       }
@@ -712,6 +776,10 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       }
     }
     if (WIDE || wave == 0) {
+      pa_args& P = pa_arguments();
+      uint32_t kept_again = lane;
+      sah_keep(kept_again);
+      const int i32 = kept_again & 31, g = kept_again >> 5;
       if (whole) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
@@ -744,7 +812,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
         }
       } else {
         // a part: to slot 0 where the tile began before this workgroup's piece, else to slot 1
-        float* to = parts + (int64_t)(2 * w + (y0 ? 0 : 1)) * S::SLOT;
+        float* to = P.work + S::WGS * (sizeof(pa_note) / 4) + (int64_t)(2 * w + (y0 ? 0 : 1)) * S::SLOT;
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           const int r = (rw * RB + rb) * 32 + i32;
@@ -760,27 +828,29 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
         if (y0 == 0 && threadIdx.x == 0) {
           // the workgroup whose piece holds the tile's last key: the first whose end is not before the tile's
           const int64_t end = at.begin + at.cost;
-          int last = (int)((end * sharers - 1) / total);
+          int last = (int)((double)end / (double)total * sharers);
+          last = last < sharers ? last : sharers - 1;
           while (last + 1 < sharers && pa_bound(total, sharers, last + 1) < end) ++last;
           while (last > w && pa_bound(total, sharers, last) >= end) --last;
-          notes[w].hk = at.hk;
-          notes[w].tile = at.tile;
-          notes[w].last = last;
-          notes[w].b = at.b;
+          pa_note* note = (pa_note*)P.work + w;
+          note->hk = at.hk;
+          note->tile = at.tile;
+          note->last = last;
+          note->b = at.b;
         }
       }
     }
     x = at.begin + y1;
     if (x >= x1) break;
     if (!WIDE) __syncthreads();  // wave 0 has read the others' shares
-    pa_next<S::ROWS>(P, at);
+    pa_next<S::ROWS>(pa_arguments(), at);
   }
-  if (bad) notes[w].again = 1;
+  if (bad) ((pa_note*)pa_arguments().work)[w].again = 1;
 }
 
 // One row key by key, by one wave: what a row holds whose products in a tile came out not finite.
 template <int DT>
-__device__ __forceinline__ void pa_row_again(const sah_paged_attention_args& P, const pa_request& r, int b, int t, int h) {
+__device__ __forceinline__ void pa_row_again(pa_args& P, const pa_request& r, int b, int t, int h) {
   constexpr int E = PA_MAX_D / SAH_WAVE;
   const int lane = threadIdx.x & (SAH_WAVE - 1), hk = h / (P.Hq / P.Hkv);
   const int64_t p = r.base + t;
@@ -830,8 +900,9 @@ __device__ __forceinline__ void pa_row_again(const sah_paged_attention_args& P, 
 #define PA_JOIN_GROUPS (PA_JOIN_NT / 16)
 #define PA_JOIN_WGS 8
 template <int DT, int DP, bool WIDE>
-__global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attention_args P) {
+__global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attention_args) {
   sah_touch_kernargs<sizeof(sah_paged_attention_args)>();
+  pa_args& P = pa_arguments();
   typedef pa_shape<DT, DP, WIDE> S;
   constexpr int NW = PA_JOIN_NT / SAH_WAVE, F = DP / 64;  // float4s of a lane: dims 4 (lane % 16) + 64 f ..
   __shared__ float s_ml[PA_JOIN_GROUPS][2];
@@ -925,10 +996,9 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
   }
   if (!note.again) return;  // uniform
   // rows of whole tiles that came out not finite: the first kernel's walk once more
-  const int64_t total = pa_total<PA_JOIN_NT, S::ROWS>(P, s_sum);
-  const int sharers = pa_sharers(total, S::WGS);
-  const int64_t x0 = pa_bound(total, sharers, w), x1 = pa_bound(total, sharers, w + 1);
-  pa_place at = pa_find<PA_JOIN_NT, S::ROWS>(P, x0, s_sum);
+  const pa_piece piece = pa_start<PA_JOIN_NT, S::ROWS>(P, S::WGS, w, s_sum);
+  const int64_t x0 = piece.x0, x1 = piece.x1;
+  pa_place at = piece.at;
   for (;;) {
     if (at.begin >= x0 && at.begin + at.cost <= x1) {
       const int n_rows = at.req.n_new * G;
@@ -951,8 +1021,10 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
 // host
 // ---------------------------------------------------------------------------
 // Tiles of 128 rows whose waves share the keys, or of 32 rows whose waves each take keys of their own: by the rows per request.
+// fp32 is bound by its matrix instructions (a sixteenth of the 16-bit rate) however often keys are read: 32 rows, so that a
+// request of few rows keeps all waves busy (5 requests of 4 to 132 rows, 2000 keys on average: 59 us as tiles of 128, %F32% so).
 static bool pa_wide(const sah_paged_attention_args* a) {
-  return (int64_t)a->n_tokens * (a->Hq / a->Hkv) > 32 * (int64_t)a->n_requests;
+  return a->dtype != SAH_F32 && (int64_t)a->n_tokens * (a->Hq / a->Hkv) > 32 * (int64_t)a->n_requests;
 }
 
 template <int DT, int DP, bool WIDE>
@@ -983,9 +1055,10 @@ static int64_t pa_dispatch(const sah_paged_attention_args* a, F f) {
 #define PA_CASE(dt, d) if (a->dtype == dt && dp == d) return wide ? f.template operator()<dt, d, true>() : f.template operator()<dt, d, false>();
   PA_CASE(SAH_BF16, 64) PA_CASE(SAH_BF16, 128) PA_CASE(SAH_BF16, 256)
   PA_CASE(SAH_F16, 64) PA_CASE(SAH_F16, 128) PA_CASE(SAH_F16, 256)
-  PA_CASE(SAH_F32, 64) PA_CASE(SAH_F32, 128) PA_CASE(SAH_F32, 256)
 #undef PA_CASE
-  return 0;
+  if (dp == 64) return f.template operator()<SAH_F32, 64, false>();
+  if (dp == 128) return f.template operator()<SAH_F32, 128, false>();
+  return f.template operator()<SAH_F32, 256, false>();
 }
 struct pa_floats_fn {
   template <int DT, int DP, bool WIDE> int64_t operator()() const { return pa_floats<DT, DP, WIDE>(); }
@@ -1011,8 +1084,8 @@ extern "C" int sah_paged_attention(const sah_paged_attention_args* a) {
   if (a->page_size <= 0 || (a->page_size & (a->page_size - 1))) return sah_fail(SAH_ESHAPE, "sah_paged_attention: page_size %d is not a power of two", a->page_size);
   if ((int64_t)a->table_width * a->page_size > INT32_MAX) return sah_fail(SAH_ESHAPE, "sah_paged_attention: table_width * page_size passes 2^31");
   if ((int64_t)a->n_tokens * a->Hq > 1 << 30) return sah_fail(SAH_ESHAPE, "sah_paged_attention: n_tokens * Hq passes 2^30");
-  // the line of work is measured in 64 bits, also where running sums overlap
-  if (((double)a->n_tokens * (a->Hq / a->Hkv) / 32 + 1) * ((double)a->table_width * a->page_size + 1024) * a->Hkv * a->n_requests > 0x1p61)
+  // the line of work is divided in doubles, also where running sums overlap
+  if (((double)a->n_tokens * (a->Hq / a->Hkv) / 32 + 1) * ((double)a->table_width * a->page_size + 1024) * a->Hkv * a->n_requests > 0x1p52)
     return sah_fail(SAH_ESHAPE, "sah_paged_attention: too much work for one call");
   if (a->table_pitch < a->table_width) return sah_fail(SAH_EINVAL, "sah_paged_attention: table_pitch is less than table_width");
   if (a->n_tokens == 0) return SAH_OK;

@@ -84,36 +84,15 @@ struct sm_weights {
 __device__ __forceinline__ uint64_t sm_raw(double e) { return __builtin_bit_cast(uint64_t, e + 512.0); }
 __device__ __forceinline__ uint64_t sm_fixed(double e) { return sm_raw(e) - SM_ZERO; }
 
-template <int CTRL, int ROW_MASK, bool BOUND>
-__device__ __forceinline__ uint64_t sm_dpp(uint64_t v) {
-  const uint32_t lo = (uint32_t)sah_dpp_i<CTRL, ROW_MASK, BOUND>((int)(uint32_t)v);
-  const uint32_t hi = (uint32_t)sah_dpp_i<CTRL, ROW_MASK, BOUND>((int)(uint32_t)(v >> 32));
-  return ((uint64_t)hi << 32) | lo;
-}
-// inclusive scan across the wave, all lanes active (as sah_wave_incl_scan)
-__device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {
-  v += sm_dpp<0x111, 0xF, true>(v);
-  v += sm_dpp<0x112, 0xF, true>(v);
-  v += sm_dpp<0x114, 0xF, true>(v);
-  v += sm_dpp<0x118, 0xF, true>(v);
-  v += sm_dpp<0x142, 0xA, false>(v);
-  v += sm_dpp<0x143, 0xC, false>(v);
-  return v;
-}
-__device__ __forceinline__ uint64_t sm_lane(uint64_t v, int lane) {
-  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
-}
-__device__ __forceinline__ uint64_t sm_wave_sum(uint64_t v) { return sm_lane(sm_wave_scan(v), SAH_WAVE - 1); }
-
 // sum and exclusive scan over the workgroup's threads (one wait; wave_sum is free to be written when this is called)
 __device__ __forceinline__ uint64_t sm_block_scan(uint64_t v, sm_shared& S, uint64_t& all) {
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
-  const uint64_t incl = sm_wave_scan(v);
+  const uint64_t incl = sah_wave_incl_scan_u64(v);
   if (lane == SAH_WAVE - 1) S.wave_sum[wave] = incl;
   __syncthreads();
-  const uint64_t sums = sm_wave_scan(lane < SM_NW ? S.wave_sum[lane] : 0);
-  all = sm_lane(sums, SM_NW - 1);
-  return (wave ? sm_lane(sums, wave - 1) : 0) + incl - v;
+  const uint64_t sums = sah_wave_incl_scan_u64(lane < SM_NW ? S.wave_sum[lane] : 0);
+  all = sah_lane_u64(sums, SM_NW - 1);
+  return (wave ? sah_lane_u64(sums, wave - 1) : 0) + incl - v;
 }
 
 // token e of 16 bytes
@@ -242,7 +221,7 @@ __device__ __forceinline__ sm_item sm_pick(sm_shared& S, int& round, uint32_t lo
       uint64_t ahead = before;
       for (int j = 0; j < n; ++j) {
         const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)me.x, j), i = (uint32_t)__builtin_amdgcn_readlane((int)me.y, j);
-        const uint64_t w = sm_lane(weight, j);
+        const uint64_t w = sah_lane_u64(weight, j);
         if (o > me.x || (o == me.x && i < me.y)) ahead += w;
       }
       const uint64_t hit = __ballot(lane < n && ahead < target && target <= ahead + weight);
@@ -490,7 +469,7 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
       for (int e = 0; i + e < V; ++e) part += final_weight(sah_load<DT>(x, i + e), i + e);
     }
     if (j % U == U - 1) {
-      part = sm_wave_sum(part);
+      part = sah_lane_u64(sah_wave_incl_scan_u64(part), SAH_WAVE - 1);
       if (lane == 0) segs[wave + j / U * SM_NW] = part;
       part = 0;
     }
@@ -517,7 +496,7 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
       w[e] = i + e < V ? final_weight(sah_load<DT>(x, i + e), i + e) : 0;
       own_sum += w[e];
     }
-    const uint64_t incl = sm_wave_scan(own_sum);
+    const uint64_t incl = sah_wave_incl_scan_u64(own_sum);
     uint64_t ahead = before + incl - own_sum;
     if (ahead < target && target <= ahead + own_sum) {  // one lane of one q
 #pragma unroll
@@ -526,7 +505,7 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
         ahead += w[e];
       }
     }
-    before += sm_lane(incl, SAH_WAVE - 1);
+    before += sah_lane_u64(incl, SAH_WAVE - 1);
   }
   if (hit >= 0) answer(hit, all);
 }
