@@ -15,6 +15,7 @@
 #include "../../include/sah_serve.h"
 
 #define PA_MAX_D 256
+#define PA_PRIO 1
 #define PA_C 4
 #define PA_V 4
 
@@ -332,6 +333,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
   constexpr int ES = S::ES, NT = S::NT, RB = S::RB, UNITS = S::ROW / 16;
   constexpr int KPI = SAH_WAVE / (UNITS < 64 ? UNITS : 64);    // keys per load instruction
   constexpr int IW = S::WKEYS / KPI / (WIDE ? S::NW : 1);      // load instructions per wave, matrix and stage
+  constexpr int IG = 16 / KPI < IW ? 16 / KPI : IW;            // ... of them that are 16 keys (or all)
   constexpr int TW = S::WKEYS / 32;                            // 32-key tiles a wave works on in a stage
   constexpr int DTL = DP / 32;
   constexpr int KQ = DT == SAH_F32 ? DP / 8 : DP / 16;         // 16-byte pieces of a lane's query
@@ -382,7 +384,8 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     const uint32_t k_unit = 16u * (l_place ^ f_k(l_key)), v_unit = 16u * (l_place ^ f_v(l_key));
     // an instruction's keys lie in one page, and a key's elements before the next key's
     const bool regular = P.page_size >= KPI && P.ks_t >= P.D && P.vs_t >= P.D;
-    const uint32_t k_lane = (uint32_t)(l_key * P.ks_t * ES), v_lane = (uint32_t)(l_key * P.vs_t * ES);
+    const uint32_t k_step = (uint32_t)(KPI * P.ks_t * ES), v_step = (uint32_t)(KPI * P.vs_t * ES);  // from an instruction's keys to the next one's
+  const uint32_t k_lane = (uint32_t)(l_key * P.ks_t * ES), v_lane = (uint32_t)(l_key * P.vs_t * ES);
     const int64_t y0 = x - at.begin, y1 = x1 - at.begin < at.cost ? x1 - at.begin : at.cost;
     const bool whole = y0 == 0 && y1 == at.cost;
     const int row_first = at.tile * S::ROWS;
@@ -466,26 +469,32 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       auto stage_at = [&](int at_key) { return ((WIDE ? 0 : S::WKEYS * wave) + at_key) * S::ROW; };
       const int left = at.req.kv - key0;  // the request's keys from here on
       const uint64_t held = left >= S::WKEYS ? (S::WKEYS == 64 ? ~0ull : 0xffffffffull) : left > 0 ? (1ull << left) - 1 : 0;
-      if (there == held && regular) {  // uniform
-        // All of them are there and an instruction's lie in one page: a scalar base, and a lane's offset that stays the same but for
-        // the permutation's part of the instruction (an exclusive or: its key's bits are none of the lane's). Keys behind
-        // the request's last come as zeros.
+      // All of them are there and the keys of GI instructions lie in one page: a scalar base for these, and lanes' offsets that stay
+      // the same (the permutation's part of an instruction is an exclusive or: its key's bits are none of the lane's, and the
+      // groups' begin with 16 keys). Keys behind the request's last come as zeros.
+      auto fast = [&](auto group) __attribute__((always_inline)) {
+        constexpr int GI = decltype(group)::value;
 #pragma unroll
-        for (int i = 0; i < IW; ++i) {
-          const int at_key = ((WIDE ? wave * IW : 0) + i) * KPI;
-          const int here = left - at_key, page_of = __builtin_amdgcn_readlane(pg, at_key);
-          const int64_t p = here > 0 ? page_of : 0, entry = (key0 + at_key) & (P.page_size - 1);
-          if (with_k) {
-            const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES;
-            const uint32_t uk = k_unit ^ (16u * f_k(at_key));
-            sah_buffer_load_lds16(ka, here >= KPI ? ~0u : here > 0 ? (uint32_t)(here * P.ks_t * ES) : 0u, k_lane + (uk < last_unit ? uk : last_unit), (buf ? s_k1 : s_k0) + stage_at(at_key));
-          }
-          if (with_v) {
-            const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES;
-            const uint32_t uv = v_unit ^ (16u * f_v(at_key));
-            sah_buffer_load_lds16(va, here >= KPI ? ~0u : here > 0 ? (uint32_t)(here * P.vs_t * ES) : 0u, v_lane + (uv < last_unit ? uv : last_unit), (buf ? s_v1 : s_v0) + stage_at(at_key));
+        for (int i0 = 0; i0 < IW; i0 += GI) {
+          const int first = ((WIDE ? wave * IW : 0) + i0) * KPI;
+          const int here = left - first, page_of = __builtin_amdgcn_readlane(pg, first);
+          const int64_t p = here > 0 ? page_of : 0, entry = (key0 + first) & (P.page_size - 1);
+          const char* ka = kbase + (p * P.ks_p + entry * P.ks_t) * ES;
+          const char* va = vbase + (p * P.vs_p + entry * P.vs_t) * ES;
+          const uint32_t k_bytes = here >= GI * KPI ? ~0u : here > 0 ? (uint32_t)(here * P.ks_t * ES) : 0u;
+          const uint32_t v_bytes = here >= GI * KPI ? ~0u : here > 0 ? (uint32_t)(here * P.vs_t * ES) : 0u;
+#pragma unroll
+          for (int i = 0; i < GI; ++i) {
+            const int at_key = first + i * KPI, turn = GI == IG ? i * KPI : at_key;
+            const uint32_t uk = k_unit ^ (16u * f_k(turn)), uv = v_unit ^ (16u * f_v(turn));
+            if (with_k) sah_buffer_load_lds16(ka, k_bytes, k_lane + i * k_step + (uk < last_unit ? uk : last_unit), (buf ? s_k1 : s_k0) + stage_at(at_key));
+            if (with_v) sah_buffer_load_lds16(va, v_bytes, v_lane + i * v_step + (uv < last_unit ? uv : last_unit), (buf ? s_v1 : s_v0) + stage_at(at_key));
           }
         }
+      };
+      if (there == held && regular) {  // uniform
+        if (P.page_size >= 16) fast(std::integral_constant<int, IG>());
+        else fast(std::integral_constant<int, 1>());
         return;
       }
       // Keys that are not there, or pages smaller than an instruction's keys: every lane its own address, through registers. (A
@@ -531,6 +540,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       // Four pieces of a key tile at a time are read while the four before are multiplied: the reads may not sink to where they
       // are used (a wait for each then: 778 us of the chunk's pass instead of %QK% with both products so).
       if (on) {
+        __builtin_amdgcn_s_setprio(PA_PRIO);  // while one wave of a SIMD multiplies another finds its softmax's turns by itself
         constexpr int C = PA_C, NC = TW * KQ / C;
         uint4 a[2][C];
         auto read = [&](int c) __attribute__((always_inline)) {
@@ -564,6 +574,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
           }
         }
       }
+      __builtin_amdgcn_s_setprio(0);
       between();
       if (!on) return;
       // the first values, requested ahead of the softmax
@@ -650,6 +661,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
             }
           }
       } else {
+        __builtin_amdgcn_s_setprio(PA_PRIO);
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
           const int step = c / (DTL / DV), t = step / 2, st = step % 2;
@@ -667,6 +679,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
             }
           }
         }
+        __builtin_amdgcn_s_setprio(0);
       }
     };
 
