@@ -26,8 +26,11 @@
 
 #define PA_CUS 256
 #define PA_XCDS 8
-#define PA_TILE_COST 96   // what starting and ending a tile costs, in keys
-#define PA_MIN_COST 256   // a workgroup's piece of the work is at least this long
+#define PA_TILE_WIDE 128
+#define PA_TILE_NARROW 256
+#define PA_MIN_WIDE 256
+#define PA_MIN_NARROW 256
+#define PA_CU64 2
 
 // Shape of a launch. RW waves share the keys of a stage, each with RB times 32 rows; RW = 1: every wave has keys of its own.
 template <int DT, int DP, bool WIDE>
@@ -43,10 +46,13 @@ struct pa_shape {
   static constexpr int STAGE = WIDE ? WKEYS : WKEYS * NW;
   static constexpr int BUFFER = STAGE * ROW;
   static constexpr int LDS = (WIDE ? 4 : 2) * BUFFER;      // K and V; where waves share them two buffers
-  static constexpr int PER_CU = LDS <= 80 * 1024 ? 2 : 1;
+  static constexpr int PER_CU = WIDE && DP == 64 ? PA_CU64 : LDS <= 80 * 1024 ? 2 : 1;
   static constexpr int WGS = PA_CUS * PER_CU;
   static constexpr int WAVES = NW * PER_CU >= 4 ? NW * PER_CU / 4 : 1;  // per SIMD
   static constexpr int SLOT = ROWS * (DP + 2);             // floats of a part
+  // in keys: what starting and ending a tile takes, and the least that is worth a workgroup
+  static constexpr int TILE_COST = WIDE ? PA_TILE_WIDE : PA_TILE_NARROW;
+  static constexpr int LEAST = WIDE ? PA_MIN_WIDE : PA_MIN_NARROW;
 };
 
 // The kernel's arguments where they lie. Each call gives an address that the compiler knows nothing of, so that what is read behind it is
@@ -106,19 +112,19 @@ __device__ __forceinline__ int64_t pa_div(int64_t a, int64_t b) {
   return q;
 }
 
-// Cost of the tiles of one request and head: tile i's is min(first + (i + 1) step, most) + PA_TILE_COST. About the keys it
+// Cost of the tiles of one request and head: tile i's is min(first + (i + 1) step, most) + each. About the keys it
 // reads; only the balance depends on it.
 struct pa_cost {
   int64_t first, step, most;
-  int tiles;
+  int tiles, each;
   __device__ __forceinline__ int64_t of(int i) const {
     const int64_t c = first + (i + 1) * step;
-    return (c < most ? c : most) + PA_TILE_COST;
+    return (c < most ? c : most) + each;
   }
   __device__ __forceinline__ int64_t before(int i) const {  // of tiles 0 .. i - 1
     int64_t j = i;
     if (first + i * step > most) j = most > first ? pa_div(most - first, step) : 0;
-    return j * first + step * (j * (j + 1) / 2) + (i - j) * most + (int64_t)i * PA_TILE_COST;
+    return j * first + step * (j * (j + 1) / 2) + (i - j) * most + (int64_t)i * each;
   }
   __device__ __forceinline__ int at(int64_t y) const {  // the tile whose piece of the line holds y
     int lo = 0, hi = tiles - 1;
@@ -129,12 +135,13 @@ struct pa_cost {
     return lo;
   }
 };
-template <int ROWS>
+template <typename S>
 __device__ __forceinline__ pa_cost pa_cost_of(pa_args& P, const pa_request& r) {
   const int G = P.Hq / P.Hkv;
   pa_cost c;
-  c.tiles = (int)(((int64_t)r.n_new * G + ROWS - 1) / ROWS);
-  c.step = (ROWS + G - 1) / G;
+  c.each = S::TILE_COST;
+  c.tiles = (int)(((int64_t)r.n_new * G + S::ROWS - 1) / S::ROWS);
+  c.step = (S::ROWS + G - 1) / G;
   const int64_t p = r.base + r.row0;
   c.first = p < 0 ? 0 : (p < r.kv ? p : r.kv);
   c.most = P.window ? (int64_t)P.sink + P.window + c.step : (int64_t)1 << 40;
@@ -150,9 +157,10 @@ struct pa_place {
 };
 
 
-__device__ __forceinline__ int pa_sharers(int64_t total, int wgs) {
-  const int64_t w = (total + PA_MIN_COST - 1) / PA_MIN_COST;
-  return (int)(w < wgs ? w : wgs);
+template <typename S>
+__device__ __forceinline__ int pa_sharers(int64_t total) {
+  const int64_t w = (total + S::LEAST - 1) / S::LEAST;
+  return (int)(w < S::WGS ? w : S::WGS);
 }
 // where workgroup w of n begins
 __device__ __forceinline__ int64_t pa_bound(int64_t total, int n, int w) {
@@ -167,14 +175,14 @@ struct pa_piece {
   pa_place at;
 };
 // s_sum: NT / 64 + 2 words. All NT threads call.
-template <int NT, int ROWS>
-__device__ __forceinline__ pa_piece pa_start(pa_args& P, int wgs, int w, int64_t* s_sum) {
+template <int NT, typename S>
+__device__ __forceinline__ pa_piece pa_start(pa_args& P, int w, int64_t* s_sum) {
   constexpr int NW = NT / SAH_WAVE;
   const int lane = threadIdx.x % SAH_WAVE, wave = sah_wave_id();
   pa_piece r;
   auto cost_of = [&](int b) -> int64_t {
     if (b >= P.n_requests) return 0;
-    const pa_cost c = pa_cost_of<ROWS>(P, pa_read_request(P, b));
+    const pa_cost c = pa_cost_of<S>(P, pa_read_request(P, b));
     return c.before(c.tiles) * P.Hkv;
   };
   auto scan = [&](int64_t v, int64_t& all) -> int64_t {  // inclusive
@@ -193,7 +201,7 @@ __device__ __forceinline__ pa_piece pa_start(pa_args& P, int wgs, int w, int64_t
   };
   auto share = [&](int64_t total) {
     r.total = total;
-    r.sharers = pa_sharers(total, wgs);
+    r.sharers = pa_sharers<S>(total);
     r.x0 = w < r.sharers ? pa_bound(total, r.sharers, w) : 0;
     r.x1 = w < r.sharers ? pa_bound(total, r.sharers, w + 1) : 0;
   };
@@ -229,7 +237,7 @@ __device__ __forceinline__ pa_piece pa_start(pa_args& P, int wgs, int w, int64_t
   at.b = __builtin_amdgcn_readfirstlane((int)s_sum[NW]);
   const int64_t begin = pa_uniform(s_sum[NW + 1]);
   at.req = pa_read_request(P, at.b);
-  at.costs = pa_cost_of<ROWS>(P, at.req);
+  at.costs = pa_cost_of<S>(P, at.req);
   const int64_t head = at.costs.before(at.costs.tiles);
   at.hk = (int)pa_uniform(pa_div(r.x0 - begin, head));
   at.tile = __builtin_amdgcn_readfirstlane(at.costs.at(r.x0 - begin - at.hk * head));
@@ -238,7 +246,7 @@ __device__ __forceinline__ pa_piece pa_start(pa_args& P, int wgs, int w, int64_t
   return r;
 }
 // the next tile on the line; there is one
-template <int ROWS>
+template <typename S>
 __device__ __forceinline__ void pa_next(pa_args& P, pa_place& at) {
   at.begin += at.cost;
   if (++at.tile == at.costs.tiles) {
@@ -248,7 +256,7 @@ __device__ __forceinline__ void pa_next(pa_args& P, pa_place& at) {
       do {
         ++at.b;
         at.req = pa_read_request(P, at.b);
-        at.costs = pa_cost_of<ROWS>(P, at.req);
+        at.costs = pa_cost_of<S>(P, at.req);
       } while (at.costs.tiles == 0);
     }
   }
@@ -355,7 +363,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     note->b = -1;
     note->again = 0;
   }
-  const pa_piece piece = pa_start<NT, S::ROWS>(pa_arguments(), S::WGS, w, s_sum);
+  const pa_piece piece = pa_start<NT, S>(pa_arguments(), w, s_sum);
   const int sharers = piece.sharers;
   if (w >= sharers) return;
   const int64_t total = piece.total, x1 = piece.x1;
@@ -744,51 +752,58 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
 
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) l_run[rb] = sah_half_sum(l_run[rb]);
+    // A lane holds 4 * DTL groups of four neighbouring dims of its row. Where every wave had keys of its own, all waves' are added up in
+    // LDS, each wave taking a share of the groups (one wave doing it for all: 6.5 us of a part's end).
+    constexpr int GROUPS = 4 * DTL, MINE = WIDE ? GROUPS : GROUPS / S::NW;
+    [[maybe_unused]] float up[S::NW];
     if constexpr (!WIDE && S::NW > 1) {
-      // the waves' shares of the keys are joined in LDS
-      __syncthreads();  // every wave has read its stages
-      constexpr int PER = SB / (16 * DTL * SAH_WAVE * 4);  // waves' tiles, [element][lane], that a buffer holds
-      static_assert(PER >= 1 && PER * 2 >= S::NW - 1 && RB == 1, "room for the waves' tiles");
-      auto tile_of = [&](int v) -> float* {
-        unsigned char* base = v / PER == 0 ? s_k0 : s_v0;
-        return (float*)base + (v % PER) * 16 * DTL * SAH_WAVE;
-      };
       __shared__ float s_ml[S::NW][2][SAH_WAVE];
-      if (wave) {
-        float* to = tile_of(wave - 1);
+      constexpr int PER = SB / (GROUPS * SAH_WAVE * 16);  // waves that a buffer holds, [group][lane]
+      static_assert(PER >= 1 && PER * 2 >= S::NW && MINE * S::NW == GROUPS && RB == 1, "room for the waves' shares");
+      __syncthreads();  // every wave has read its stages
+      float4* to = (float4*)(wave < PER ? s_k0 : s_v0) + wave % PER * GROUPS * SAH_WAVE + lane;
 #pragma unroll
-        for (int t = 0; t < DTL; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) to[(16 * t + e) * SAH_WAVE + lane] = acc[0][t][e];
-        s_ml[wave][0][lane] = m_run[0];
-        s_ml[wave][1][lane] = l_run[0];
+      for (int i = 0; i < GROUPS; ++i) {
+        const auto& v = acc[0][i / 4];
+        to[i * SAH_WAVE] = make_float4(v[4 * (i % 4)], v[4 * (i % 4) + 1], v[4 * (i % 4) + 2], v[4 * (i % 4) + 3]);
       }
+      s_ml[wave][0][lane] = m_run[0];
+      s_ml[wave][1][lane] = l_run[0];
       __syncthreads();
-      if (wave == 0) {
-        float m_new = m_run[0];
+      float m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int v = 1; v < S::NW; ++v) m_new = fmaxf(m_new, s_ml[v][0][lane]);
-        float up = m_run[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[0] - m_new);
-        l_run[0] *= up;
+      for (int v = 0; v < S::NW; ++v) m = fmaxf(m, s_ml[v][0][lane]);
 #pragma unroll
-        for (int t = 0; t < DTL; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[0][t][e] *= up;
-#pragma unroll
-        for (int v = 1; v < S::NW; ++v) {
-          const float mv = s_ml[v][0][lane];
-          up = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - m_new);
-          l_run[0] += s_ml[v][1][lane] * up;
-          const float* from = tile_of(v - 1);
-#pragma unroll
-          for (int t = 0; t < DTL; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[0][t][e] += from[(16 * t + e) * SAH_WAVE + lane] * up;
-        }
-        m_run[0] = m_new;
+      for (int v = 0; v < S::NW; ++v) {
+        const float mv = s_ml[v][0][lane];
+        up[v] = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - m);
+        l += s_ml[v][1][lane] * up[v];
       }
+      m_run[0] = m;
+      l_run[0] = l;
     }
-    if (WIDE || wave == 0) {
+    // group i of this wave's, its number among all
+    auto group_of = [&](int rb, int i, int& number) __attribute__((always_inline)) -> float4 {
+      if constexpr (!WIDE && S::NW > 1) {
+        constexpr int PER = SB / (GROUPS * SAH_WAVE * 16);
+        number = wave * MINE + i;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int v = 0; v < S::NW; ++v) {
+          const float4 a = ((const float4*)(v < PER ? s_k0 : s_v0))[(v % PER * GROUPS + number) * SAH_WAVE + lane];
+          sum.x += a.x * up[v];
+          sum.y += a.y * up[v];
+          sum.z += a.z * up[v];
+          sum.w += a.w * up[v];
+        }
+        return sum;
+      } else {
+        number = i;
+        const auto& v = acc[rb][i / 4];
+        return make_float4(v[4 * (i % 4)], v[4 * (i % 4) + 1], v[4 * (i % 4) + 2], v[4 * (i % 4) + 3]);
+      }
+    };
+    {
       pa_args& P = pa_arguments();
       uint32_t kept_again = lane;
       sah_keep(kept_again);
@@ -806,21 +821,17 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
           bool fine = true;
           char* op = (char*)P.out + ((int64_t)tok[rb] * P.os_t + (int64_t)head[rb] * P.os_h) * ES;
 #pragma unroll
-          for (int t = 0; t < DTL; ++t)
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              const int d = 32 * t + 8 * q4 + 4 * g;
-              if (d >= P.D) continue;
-              float o[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                o[e] = acc[rb][t][4 * q4 + e] * inv;
-                fine = fine && fabsf(o[e]) < INFINITY;
-              }
-              if (!live[rb]) continue;
-              if (DT == SAH_F32) *(float4*)(op + 4 * d) = make_float4(o[0], o[1], o[2], o[3]);
-              else *(uint2*)(op + 2 * d) = make_uint2(sah_pack2_hw<DT>(o[0], o[1]), sah_pack2_hw<DT>(o[2], o[3]));
-            }
+          for (int i = 0; i < MINE; ++i) {
+            int number;
+            const float4 a = group_of(rb, i, number);
+            const int d = 8 * number + 4 * g;
+            if (d >= P.D) continue;
+            const float4 o = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+            fine = fine && fabsf(o.x) < INFINITY && fabsf(o.y) < INFINITY && fabsf(o.z) < INFINITY && fabsf(o.w) < INFINITY;
+            if (!live[rb]) continue;
+            if (DT == SAH_F32) *(float4*)(op + 4 * d) = o;
+            else *(uint2*)(op + 2 * d) = make_uint2(sah_pack2_hw<DT>(o.x, o.y), sah_pack2_hw<DT>(o.z, o.w));
+          }
           bad = bad || (live[rb] && !fine);
         }
       } else {
@@ -829,14 +840,14 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           const int r = (rw * RB + rb) * 32 + i32;
-          if (!live[rb]) continue;
-          if (g == 0) ((float2*)to)[r] = make_float2(m_run[rb], l_run[rb]);
+          if (live[rb] && g == 0 && (WIDE || wave == 0)) ((float2*)to)[r] = make_float2(m_run[rb], l_run[rb]);
           float* o = to + 2 * S::ROWS + r * DP;
 #pragma unroll
-          for (int t = 0; t < DTL; ++t)
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4)
-              *(float4*)(o + 32 * t + 8 * q4 + 4 * g) = make_float4(acc[rb][t][4 * q4], acc[rb][t][4 * q4 + 1], acc[rb][t][4 * q4 + 2], acc[rb][t][4 * q4 + 3]);
+          for (int i = 0; i < MINE; ++i) {
+            int number;
+            const float4 a = group_of(rb, i, number);
+            if (live[rb]) *(float4*)(o + 8 * number + 4 * g) = a;
+          }
         }
         if (y0 == 0 && threadIdx.x == 0) {
           // the workgroup whose piece holds the tile's last key: the first whose end is not before the tile's
@@ -855,8 +866,8 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     }
     x = at.begin + y1;
     if (x >= x1) break;
-    if (!WIDE) __syncthreads();  // wave 0 has read the others' shares
-    pa_next<S::ROWS>(pa_arguments(), at);
+    if (!WIDE) __syncthreads();  // all shares have been read
+    pa_next<S>(pa_arguments(), at);
   }
   if (bad) ((pa_note*)pa_arguments().work)[w].again = 1;
 }
@@ -1009,7 +1020,7 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
   }
   if (!note.again) return;  // uniform
   // rows of whole tiles that came out not finite: the first kernel's walk once more
-  const pa_piece piece = pa_start<PA_JOIN_NT, S::ROWS>(P, S::WGS, w, s_sum);
+  const pa_piece piece = pa_start<PA_JOIN_NT, S>(P, w, s_sum);
   const int64_t x0 = piece.x0, x1 = piece.x1;
   pa_place at = piece.at;
   for (;;) {
@@ -1026,7 +1037,7 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
       }
     }
     if (at.begin + at.cost >= x1) break;
-    pa_next<S::ROWS>(P, at);
+    pa_next<S>(P, at);
   }
 }
 
