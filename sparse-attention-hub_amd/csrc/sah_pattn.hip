@@ -17,7 +17,7 @@
 #define PA_MAX_D 256
 #define PA_PRIO 1
 #define PA_C 4
-#define PA_V 4
+#define PA_V 2
 
 
 
@@ -312,12 +312,19 @@ template <int DT> struct pa_weights {
   static constexpr float SCALE = DT == SAH_F16 ? 8.0f : 0.0f;
 };
 
-// Reads of LDS written above this are issued above it.
+// Reads of LDS written above this are issued above it, and x, the result of an earlier one, is used below it alone. (Left to itself the
+// compiler reads where it multiplies, one wait of LDS's latency after the other.)
 __device__ __forceinline__ void pa_reads_stay() {
 #if defined(__HIP_DEVICE_COMPILE__)
   asm volatile("" ::: "memory");
 #endif
 }
+__device__ __forceinline__ void pa_from_here(sah_u4& x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(x)::"memory");
+#endif
+}
+__device__ __forceinline__ uint4 pa_operand(const sah_u4& v) { return make_uint4(v.x, v.y, v.z, v.w); }
 
 // Waits until no more than N of this wave's loads (LDS: 15 is no wait) are under way. The builtin, not an instruction of inline asm: the
 // compiler counts loads itself, and where it does not see that staged keys have landed it waits for all loads there are.
@@ -545,29 +552,28 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[rb][t][e] = 0.f;
-      // Four pieces of a key tile at a time are read while the four before are multiplied: the reads may not sink to where they
-      // are used (a wait for each then: 778 us of the chunk's pass instead of %QK% with both products so).
+      // Four pieces of a key tile at a time are read while the four before are multiplied.
       if (on) {
         __builtin_amdgcn_s_setprio(PA_PRIO);  // while one wave of a SIMD multiplies another finds its softmax's turns by itself
         constexpr int C = PA_C, NC = TW * KQ / C;
-        uint4 a[2][C];
+        sah_u4 a[2][C];
         auto read = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
           for (int i = 0; i < C; ++i) {
             const int t = c * C / KQ, st = c * C % KQ + i;
-            const sah_u4 v = *(const sah_u4*)(kp + 32 * t * S::ROW + (k_at ^ (32 * st)));
-            a[c & 1][i] = make_uint4(v.x, v.y, v.z, v.w);
+            a[c & 1][i] = *(const sah_u4*)(kp + 32 * t * S::ROW + (k_at ^ (32 * st)));
           }
         };
         read(0);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           if (c + 1 < NC) read(c + 1);
-          pa_reads_stay();
+#pragma unroll
+          for (int i = 0; i < C; ++i) pa_from_here(a[c & 1][i]);
 #pragma unroll
           for (int i = 0; i < C; ++i) {
             const int t = c * C / KQ, st = c * C % KQ + i;
-            const uint4 k = a[c & 1][i];
+            const uint4 k = pa_operand(a[c & 1][i]);
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb) {
               if constexpr (DT == SAH_F32) {
@@ -587,14 +593,14 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       if (!on) return;
       // the first values, requested ahead of the softmax
       constexpr int DV = DTL < PA_V ? DTL : PA_V, NV = 2 * TW * (DTL / DV);  // 32-dim tiles of a piece, pieces
-      uint4 va[2][DT == SAH_F32 ? 1 : DV];
+      sah_u4 va[2][DT == SAH_F32 ? 1 : DV];
       auto read_v = [&](int c) __attribute__((always_inline)) {
         if constexpr (DT != SAH_F32) {
 #pragma unroll
           for (int d = 0; d < DV; ++d) {
             const unsigned char* v = vp + 16 * (c / (DTL / DV)) * S::ROW + v_at[c % (DTL / DV) * DV + d];
             const sah_u2 a0 = sah_read_tr16((const uint16_t*)v), a1 = sah_read_tr16((const uint16_t*)(v + 8 * S::ROW));
-            va[c & 1][d] = make_uint4(a0.x, a0.y, a1.x, a1.y);
+            va[c & 1][d] = sah_u4{a0.x, a0.y, a1.x, a1.y};
           }
         }
       };
@@ -626,6 +632,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
           }
         }
       }
+      float mc[RB];
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
         float mx = s[rb][0][0];
@@ -646,15 +653,20 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
             for (int e = 0; e < 16; ++e) acc[rb][t][e] *= up;
         }
         // (a row that has seen nothing: kept in range, so that -inf comes to 0)
-        const float mc = fmaxf(m_run[rb], -1e37f) - pa_weights<DT>::SCALE;
+        mc[rb] = fmaxf(m_run[rb], -1e37f) - pa_weights<DT>::SCALE;
+      }
+      auto weigh = [&](int t, int e0, int n) __attribute__((always_inline)) {  // n of a key tile's weights
 #pragma unroll
-        for (int t = 0; t < TW; ++t)
+        for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            s[rb][t][e] = __builtin_amdgcn_exp2f(fmaf(s[rb][t][e], c_exp, -mc));
+          for (int e = e0; e < e0 + n; ++e) {
+            s[rb][t][e] = __builtin_amdgcn_exp2f(fmaf(s[rb][t][e], c_exp, -mc[rb]));
             l_run[rb] += s[rb][t][e];
           }
-      }
+      };
+      // (16-bit types: the second key tile's weights are taken between the first one's products)
+#pragma unroll
+      for (int t = 0; t < (DT == SAH_F32 ? TW : 1); ++t) weigh(t, 0, 16);
       if constexpr (DT == SAH_F32) {
 #pragma unroll
         for (int t = 0; t < TW; ++t)
@@ -674,7 +686,8 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
         for (int c = 0; c < NV; ++c) {
           const int step = c / (DTL / DV), t = step / 2, st = step % 2;
           if (c + 1 < NV) read_v(c + 1);
-          pa_reads_stay();
+#pragma unroll
+          for (int d = 0; d < DV; ++d) pa_from_here(va[c & 1][d]);
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
             const auto& z = s[rb][t];
@@ -683,8 +696,12 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
 #pragma unroll
             for (int d = 0; d < DV; ++d) {
               const int to = c % (DTL / DV) * DV + d;
-              acc[rb][to] = sah_mfma_32x32x16<DT>(va[c & 1][d], pt, acc[rb][to]);
+              acc[rb][to] = sah_mfma_32x32x16<DT>(pa_operand(va[c & 1][d]), pt, acc[rb][to]);
             }
+          }
+          if (TW == 2 && t == 0) {
+            constexpr int N = 16 * TW / NV;
+            weigh(1, c * N, N);
           }
         }
         __builtin_amdgcn_s_setprio(0);
