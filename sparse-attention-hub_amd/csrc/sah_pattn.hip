@@ -1,6 +1,6 @@
 // Attention of new tokens over a key-value cache in pages, on the matrix cores.
 //
-// Of a request's new tokens and a key head's query heads every (token, head) is a row; PA_ROWS rows are a tile, which reads its
+// Of a request's new tokens and a key head's query heads every (token, head) is a row; 32 or 128 rows are a tile, which reads its
 // keys once. All tiles of all requests, one after the other, are one line of work (measured in keys); every workgroup takes
 // an equal piece of it, whatever the requests' lengths, finds its place from the lengths on the device, and works through
 // tiles and parts of tiles. A part's (m, l, acc) goes to the workspace, a second kernel joins the parts of a tile.
@@ -15,49 +15,39 @@
 #include "../../include/sah_serve.h"
 
 #define PA_MAX_D 256
-#define PA_PRIO 1
-#define PA_C 4
-#define PA_V 2
-
-
-
-
-
-
 #define PA_CUS 256
 #define PA_XCDS 8
-#define PA_TILE_WIDE 128
-#define PA_TILE_NARROW 256
-#define PA_MIN_WIDE 256
-#define PA_MIN_NARROW 256
-#define PA_CU64 2
+// 16-byte pieces of staged keys that are read while as many are multiplied (2048 tokens over 18432 keys: 636 us; 4: 647, 8: 650)
+// and 32-dim tiles of values (1, 2 and 4 alike)
+#define PA_LOOK 2
+#define PA_LOOK_V 2
 
-// Shape of a launch. RW waves share the keys of a stage, each with RB times 32 rows; RW = 1: every wave has keys of its own.
+// Shape of a launch. RW waves share the keys of a stage, each with 32 rows; RW = 1: every wave has keys of its own.
 template <int DT, int DP, bool WIDE>
 struct pa_shape {
   static constexpr int ES = DT == SAH_F32 ? 4 : 2;
   static constexpr int ROW = DP * ES;                      // bytes of a staged key
   static constexpr int NW = WIDE ? 4 : ROW <= 256 ? 8 : 2048 / ROW;
   static constexpr int NT = NW * SAH_WAVE;
-  static constexpr int RB = 1;
   static constexpr int RW = WIDE ? 4 : 1;
-  static constexpr int ROWS = 32 * RB * RW;
+  static constexpr int ROWS = 32 * RW;
   static constexpr int WKEYS = (WIDE ? ROW <= 512 : ROW <= 128) ? 64 : 32;  // keys of a stage that a wave works on
   static constexpr int STAGE = WIDE ? WKEYS : WKEYS * NW;
   static constexpr int BUFFER = STAGE * ROW;
   static constexpr int LDS = (WIDE ? 4 : 2) * BUFFER;      // K and V; where waves share them two buffers
-  static constexpr int PER_CU = WIDE && DP == 64 ? PA_CU64 : LDS <= 80 * 1024 ? 2 : 1;
+  static constexpr int PER_CU = LDS <= 80 * 1024 ? 2 : 1;
   static constexpr int WGS = PA_CUS * PER_CU;
   static constexpr int WAVES = NW * PER_CU >= 4 ? NW * PER_CU / 4 : 1;  // per SIMD
   static constexpr int SLOT = ROWS * (DP + 2);             // floats of a part
-  // in keys: what starting and ending a tile takes, and the least that is worth a workgroup
-  static constexpr int TILE_COST = WIDE ? PA_TILE_WIDE : PA_TILE_NARROW;
-  static constexpr int LEAST = WIDE ? PA_MIN_WIDE : PA_MIN_NARROW;
+  // In keys: what starting and ending a tile takes (256: one request of 100 keys 17 us instead of 11, its 8 heads' tiles split), and
+  // the least that is worth a workgroup (512: 5 fp32 requests of 2000 keys 43 us instead of 34; 128: no case gains, small ones lose 1).
+  static constexpr int TILE_COST = 128;
+  static constexpr int LEAST = 256;
 };
 
 // The kernel's arguments where they lie. Each call gives an address that the compiler knows nothing of, so that what is read behind it is
 // read again for every tile: all of them kept in scalar registers from the kernel's first line on, two hundred of those go
-// to vector registers and come back in the innermost loop (2048 tokens over 18432 keys: 850 us instead of %KARG%).
+// to vector registers and come back in the innermost loop (2048 tokens over 18432 keys: 666 us instead of 647).
 typedef const sah_paged_attention_args __attribute__((address_space(4))) pa_args;
 __device__ __forceinline__ pa_args& pa_arguments() {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -156,11 +146,10 @@ struct pa_place {
   pa_cost costs;
 };
 
-
 template <typename S>
 __device__ __forceinline__ int pa_sharers(int64_t total) {
   const int64_t w = (total + S::LEAST - 1) / S::LEAST;
-  return (int)(w < S::WGS ? w : S::WGS);
+  return (int)(w < (int)gridDim.x ? w : (int)gridDim.x);
 }
 // where workgroup w of n begins
 __device__ __forceinline__ int64_t pa_bound(int64_t total, int n, int w) {
@@ -345,7 +334,7 @@ template <int DT, int DP, bool WIDE>
 __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WIDE>::WAVES)) void k_paged_attn(sah_paged_attention_args) {
   sah_touch_kernargs<sizeof(sah_paged_attention_args)>();
   typedef pa_shape<DT, DP, WIDE> S;
-  constexpr int ES = S::ES, NT = S::NT, RB = S::RB, UNITS = S::ROW / 16;
+  constexpr int ES = S::ES, NT = S::NT, UNITS = S::ROW / 16;
   constexpr int KPI = SAH_WAVE / (UNITS < 64 ? UNITS : 64);    // keys per load instruction
   constexpr int IW = S::WKEYS / KPI / (WIDE ? S::NW : 1);      // load instructions per wave, matrix and stage
   constexpr int IG = 16 / KPI < IW ? 16 / KPI : IW;            // ... of them that are 16 keys (or all)
@@ -364,7 +353,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
   const int i32 = lane & 31, g = lane >> 5;
   const int rw = WIDE ? wave : 0;
   // neighbours on the line of work share keys: they get the same XCD
-  const int w = (int)(blockIdx.x % PA_XCDS) * (S::WGS / PA_XCDS) + (int)(blockIdx.x / PA_XCDS);
+  const int w = (int)(blockIdx.x % PA_XCDS) * (int)(gridDim.x / PA_XCDS) + (int)(blockIdx.x / PA_XCDS);
   if (threadIdx.x == 0) {
     pa_note* note = (pa_note*)pa_arguments().work + w;
     note->b = -1;
@@ -400,7 +389,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     // an instruction's keys lie in one page, and a key's elements before the next key's
     const bool regular = P.page_size >= KPI && P.ks_t >= P.D && P.vs_t >= P.D;
     const uint32_t k_step = (uint32_t)(KPI * P.ks_t * ES), v_step = (uint32_t)(KPI * P.vs_t * ES);  // from an instruction's keys to the next one's
-  const uint32_t k_lane = (uint32_t)(l_key * P.ks_t * ES), v_lane = (uint32_t)(l_key * P.vs_t * ES);
+    const uint32_t k_lane = (uint32_t)(l_key * P.ks_t * ES), v_lane = (uint32_t)(l_key * P.vs_t * ES);
     const int64_t y0 = x - at.begin, y1 = x1 - at.begin < at.cost ? x1 - at.begin : at.cost;
     const bool whole = y0 == 0 && y1 == at.cost;
     const int row_first = at.tile * S::ROWS;
@@ -414,55 +403,49 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     uint32_t kept_lane = lane;
     sah_keep(kept_lane);
     const int i32 = kept_lane & 31, g = kept_lane >> 5;
-    int pos[RB], tok[RB], head[RB];
-    bool live[RB];
-    uint4 qf[RB][KQ];
+    int pos, tok, head;
+    bool live;
+    uint4 qf[KQ];
     bool wave_live = false;
     int w_lo = 0x7fffffff, w_hi = -1;  // positions of the wave's rows
+    const int r0 = row_first + rw * 32;
+    if (r0 < n_rows) {
+      wave_live = true;
+      const int r1 = r0 + 31 < n_rows ? r0 + 31 : n_rows - 1;
+      const int a = pa_position(at.req, r0 / G), z = pa_position(at.req, r1 / G);
+      w_lo = a < w_lo ? a : w_lo;
+      w_hi = z > w_hi ? z : w_hi;
+    }
+    const int r = r0 + i32;
+    live = r < n_rows;
+    const int rr = live ? r : n_rows - 1;
+    const int i = rr / G;
+    head = at.hk * G + rr - i * G;
+    tok = at.req.row0 + i;
+    pos = pa_position(at.req, i);
+    const char* qp = (const char*)P.q + ((int64_t)tok * P.qs_t + (int64_t)head * P.qs_h) * ES;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const int r0 = row_first + (rw * RB + rb) * 32;
-      if (r0 < n_rows) {
-        wave_live = true;
-        const int r1 = r0 + 31 < n_rows ? r0 + 31 : n_rows - 1;
-        const int a = pa_position(at.req, r0 / G), z = pa_position(at.req, r1 / G);
-        w_lo = a < w_lo ? a : w_lo;
-        w_hi = z > w_hi ? z : w_hi;
+    for (int s = 0; s < KQ; ++s) {
+      const int unit = 2 * s + g;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (unit < units_real) v = *(const uint4*)(qp + 16 * unit);
+      if (P.scaling < 0.f) {  // uniform: the sign is the query's
+        const uint32_t sign = DT == SAH_F32 ? 0x80000000u : 0x80008000u;
+        v.x ^= sign; v.y ^= sign; v.z ^= sign; v.w ^= sign;
       }
-      const int r = r0 + i32;
-      live[rb] = r < n_rows;
-      const int rr = live[rb] ? r : n_rows - 1;
-      const int i = rr / G;
-      head[rb] = at.hk * G + rr - i * G;
-      tok[rb] = at.req.row0 + i;
-      pos[rb] = pa_position(at.req, i);
-      const char* qp = (const char*)P.q + ((int64_t)tok[rb] * P.qs_t + (int64_t)head[rb] * P.qs_h) * ES;
-#pragma unroll
-      for (int s = 0; s < KQ; ++s) {
-        const int unit = 2 * s + g;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (unit < units_real) v = *(const uint4*)(qp + 16 * unit);
-        if (P.scaling < 0.f) {  // uniform: the sign is the query's
-          const uint32_t sign = DT == SAH_F32 ? 0x80000000u : 0x80008000u;
-          v.x ^= sign; v.y ^= sign; v.z ^= sign; v.w ^= sign;
-        }
-        qf[rb][s] = v;
-      }
+      qf[s] = v;
     }
     w_lo = __builtin_amdgcn_readfirstlane(w_lo);
     w_hi = __builtin_amdgcn_readfirstlane(w_hi);
 
-    float m_run[RB], l_run[RB];
-    sah_f32x16 acc[RB][DTL];
+    float m_run, l_run;
+    sah_f32x16 acc[DTL];
+    m_run = -INFINITY;
+    l_run = 0.f;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      m_run[rb] = -INFINITY;
-      l_run[rb] = 0.f;
+    for (int t = 0; t < DTL; ++t)
 #pragma unroll
-      for (int t = 0; t < DTL; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[rb][t][e] = 0.f;
-    }
+      for (int e = 0; e < 16; ++e) acc[t][e] = 0.f;
 
     // The keys of a stage that this wave works on: a lane holds the page of one, and a bit says which are there. Requested a
     // stage ahead of the loads that go by it.
@@ -545,17 +528,15 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       const bool on = wave_live && there != 0 && key0 <= w_hi;  // uniform
       const unsigned char* kp = (buf ? s_k1 : s_k0) + (WIDE ? 0 : S::WKEYS * wave * S::ROW);
       const unsigned char* vp = (buf ? s_v1 : s_v0) + (WIDE ? 0 : S::WKEYS * wave * S::ROW);
-      sah_f32x16 s[RB][TW];
+      sah_f32x16 s[TW];
 #pragma unroll
       for (int t = 0; t < TW; ++t)
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[rb][t][e] = 0.f;
-      // Four pieces of a key tile at a time are read while the four before are multiplied.
+          for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+      // PA_LOOK pieces of a key tile at a time are read while as many before are multiplied.
       if (on) {
-        __builtin_amdgcn_s_setprio(PA_PRIO);  // while one wave of a SIMD multiplies another finds its softmax's turns by itself
-        constexpr int C = PA_C, NC = TW * KQ / C;
+        __builtin_amdgcn_s_setprio(1);  // while one wave of a SIMD multiplies another finds its softmax's turns by itself
+        constexpr int C = PA_LOOK, NC = TW * KQ / C;
         sah_u4 a[2][C];
         auto read = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
@@ -574,16 +555,13 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
           for (int i = 0; i < C; ++i) {
             const int t = c * C / KQ, st = c * C % KQ + i;
             const uint4 k = pa_operand(a[c & 1][i]);
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) {
-              if constexpr (DT == SAH_F32) {
-                s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.x), sah_bits_to_float(qf[rb][st].x), s[rb][t]);
-                s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.y), sah_bits_to_float(qf[rb][st].y), s[rb][t]);
-                s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.z), sah_bits_to_float(qf[rb][st].z), s[rb][t]);
-                s[rb][t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.w), sah_bits_to_float(qf[rb][st].w), s[rb][t]);
-              } else {
-                s[rb][t] = sah_mfma_32x32x16<DT>(k, qf[rb][st], s[rb][t]);
-              }
+            if constexpr (DT == SAH_F32) {
+              s[t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.x), sah_bits_to_float(qf[st].x), s[t]);
+              s[t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.y), sah_bits_to_float(qf[st].y), s[t]);
+              s[t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.z), sah_bits_to_float(qf[st].z), s[t]);
+              s[t] = sah_mfma_32x32x2_f32(sah_bits_to_float(k.w), sah_bits_to_float(qf[st].w), s[t]);
+            } else {
+              s[t] = sah_mfma_32x32x16<DT>(k, qf[st], s[t]);
             }
           }
         }
@@ -592,7 +570,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       between();
       if (!on) return;
       // the first values, requested ahead of the softmax
-      constexpr int DV = DTL < PA_V ? DTL : PA_V, NV = 2 * TW * (DTL / DV);  // 32-dim tiles of a piece, pieces
+      constexpr int DV = DTL < PA_LOOK_V ? DTL : PA_LOOK_V, NV = 2 * TW * (DTL / DV);  // 32-dim tiles of a piece, pieces
       sah_u4 va[2][DT == SAH_F32 ? 1 : DV];
       auto read_v = [&](int c) __attribute__((always_inline)) {
         if constexpr (DT != SAH_F32) {
@@ -611,57 +589,49 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       const bool plain = there == full && key0 + S::WKEYS - 1 <= w_lo &&
                          (!P.window || key0 + S::WKEYS <= P.sink || (int64_t)key0 > (int64_t)w_hi - P.window);
       if (!plain) {
+        uint32_t kept_pos = pos;
+        sah_keep(kept_pos);
+        const int at_pos = (int)kept_pos;
+        const int lo = P.window && at_pos >= P.window ? at_pos - P.window + 1 : 0;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          uint32_t kept_pos = pos[rb];
-          sah_keep(kept_pos);
-          const int at_pos = (int)kept_pos;
-          const int lo = P.window && at_pos >= P.window ? at_pos - P.window + 1 : 0;
+        for (int t = 0; t < TW; ++t) {
+          const int k0 = key0 + 32 * t, wi = k0 / 32;
+          uint32_t word = sah_range_bits(wi, lo, at_pos + 1);
+          if (P.window) word |= sah_range_bits(wi, 0, P.sink < at_pos + 1 ? P.sink : at_pos + 1);
+          word &= (uint32_t)(there >> (32 * t));
+          word >>= 4 * g;
 #pragma unroll
-          for (int t = 0; t < TW; ++t) {
-            const int k0 = key0 + 32 * t, wi = k0 / 32;
-            uint32_t word = sah_range_bits(wi, lo, at_pos + 1);
-            if (P.window) word |= sah_range_bits(wi, 0, P.sink < at_pos + 1 ? P.sink : at_pos + 1);
-            word &= (uint32_t)(there >> (32 * t));
-            word >>= 4 * g;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const uint32_t on = (uint32_t)((int)(word << (31 - (8 * (e / 4) + e % 4))) >> 31);  // all ones where the row sees the key
-              s[rb][t][e] = sah_bits_to_float((sah_float_to_bits(s[rb][t][e]) & on) | (0xff800000u & ~on));
-            }
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t on = (uint32_t)((int)(word << (31 - (8 * (e / 4) + e % 4))) >> 31);  // all ones where the row sees the key
+            s[t][e] = sah_bits_to_float((sah_float_to_bits(s[t][e]) & on) | (0xff800000u & ~on));
           }
         }
       }
-      float mc[RB];
+      float mc;
+      float mx = s[0][0];
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        float mx = s[rb][0][0];
+      for (int t = 0; t < TW; ++t)
 #pragma unroll
-        for (int t = 0; t < TW; ++t)
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
+      mx = sah_half_max(mx) * c_exp;
+      // (-inf - -inf is NaN: no rise)
+      if (__ballot(mx - m_run > pa_weights<DT>::SLACK) != 0) {  // uniform: some row's maximum has risen too far
+        const float m_new = fmaxf(m_run, mx);
+        const float up = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= up;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[rb][t][e]);
-        mx = sah_half_max(mx) * c_exp;
-        // (-inf - -inf is NaN: no rise)
-        if (__ballot(mx - m_run[rb] > pa_weights<DT>::SLACK) != 0) {  // uniform: some row's maximum has risen too far
-          const float m_new = fmaxf(m_run[rb], mx);
-          const float up = m_run[rb] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[rb] - m_new);
-          m_run[rb] = m_new;
-          l_run[rb] *= up;
+        for (int t = 0; t < DTL; ++t)
 #pragma unroll
-          for (int t = 0; t < DTL; ++t)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[rb][t][e] *= up;
-        }
-        // (a row that has seen nothing: kept in range, so that -inf comes to 0)
-        mc[rb] = fmaxf(m_run[rb], -1e37f) - pa_weights<DT>::SCALE;
+          for (int e = 0; e < 16; ++e) acc[t][e] *= up;
       }
+      // (a row that has seen nothing: kept in range, so that -inf comes to 0)
+      mc = fmaxf(m_run, -1e37f) - pa_weights<DT>::SCALE;
       auto weigh = [&](int t, int e0, int n) __attribute__((always_inline)) {  // n of a key tile's weights
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
           for (int e = e0; e < e0 + n; ++e) {
-            s[rb][t][e] = __builtin_amdgcn_exp2f(fmaf(s[rb][t][e], c_exp, -mc[rb]));
-            l_run[rb] += s[rb][t][e];
+            s[t][e] = __builtin_amdgcn_exp2f(fmaf(s[t][e], c_exp, -mc));
+            l_run += s[t][e];
           }
       };
       // (16-bit types: the second key tile's weights are taken between the first one's products)
@@ -676,28 +646,24 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
 #pragma unroll
             for (int d = 0; d < DTL; ++d) {
               const float v = row[32 * d];
-#pragma unroll
-              for (int rb = 0; rb < RB; ++rb) acc[rb][d] = sah_mfma_32x32x2_f32(v, s[rb][t][e], acc[rb][d]);
+              acc[d] = sah_mfma_32x32x2_f32(v, s[t][e], acc[d]);
             }
           }
       } else {
-        __builtin_amdgcn_s_setprio(PA_PRIO);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
           const int step = c / (DTL / DV), t = step / 2, st = step % 2;
           if (c + 1 < NV) read_v(c + 1);
 #pragma unroll
           for (int d = 0; d < DV; ++d) pa_from_here(va[c & 1][d]);
+          const auto& z = s[t];
+          const uint4 pt = make_uint4(sah_pack2_hw<DT>(z[8 * st], z[8 * st + 1]), sah_pack2_hw<DT>(z[8 * st + 2], z[8 * st + 3]),
+                                      sah_pack2_hw<DT>(z[8 * st + 4], z[8 * st + 5]), sah_pack2_hw<DT>(z[8 * st + 6], z[8 * st + 7]));
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb) {
-            const auto& z = s[rb][t];
-            const uint4 pt = make_uint4(sah_pack2_hw<DT>(z[8 * st], z[8 * st + 1]), sah_pack2_hw<DT>(z[8 * st + 2], z[8 * st + 3]),
-                                        sah_pack2_hw<DT>(z[8 * st + 4], z[8 * st + 5]), sah_pack2_hw<DT>(z[8 * st + 6], z[8 * st + 7]));
-#pragma unroll
-            for (int d = 0; d < DV; ++d) {
-              const int to = c % (DTL / DV) * DV + d;
-              acc[rb][to] = sah_mfma_32x32x16<DT>(pa_operand(va[c & 1][d]), pt, acc[rb][to]);
-            }
+          for (int d = 0; d < DV; ++d) {
+            const int to = c % (DTL / DV) * DV + d;
+            acc[to] = sah_mfma_32x32x16<DT>(pa_operand(va[c & 1][d]), pt, acc[to]);
           }
           if (TW == 2 && t == 0) {
             constexpr int N = 16 * TW / NV;
@@ -767,8 +733,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       }
     }
 
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) l_run[rb] = sah_half_sum(l_run[rb]);
+    l_run = sah_half_sum(l_run);
     // A lane holds 4 * DTL groups of four neighbouring dims of its row. Where every wave had keys of its own, all waves' are added up in
     // LDS, each wave taking a share of the groups (one wave doing it for all: 6.5 us of a part's end).
     constexpr int GROUPS = 4 * DTL, MINE = WIDE ? GROUPS : GROUPS / S::NW;
@@ -776,16 +741,16 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     if constexpr (!WIDE && S::NW > 1) {
       __shared__ float s_ml[S::NW][2][SAH_WAVE];
       constexpr int PER = SB / (GROUPS * SAH_WAVE * 16);  // waves that a buffer holds, [group][lane]
-      static_assert(PER >= 1 && PER * 2 >= S::NW && MINE * S::NW == GROUPS && RB == 1, "room for the waves' shares");
+      static_assert(PER >= 1 && PER * 2 >= S::NW && MINE * S::NW == GROUPS, "room for the waves' shares");
       __syncthreads();  // every wave has read its stages
       float4* to = (float4*)(wave < PER ? s_k0 : s_v0) + wave % PER * GROUPS * SAH_WAVE + lane;
 #pragma unroll
       for (int i = 0; i < GROUPS; ++i) {
-        const auto& v = acc[0][i / 4];
+        const auto& v = acc[i / 4];
         to[i * SAH_WAVE] = make_float4(v[4 * (i % 4)], v[4 * (i % 4) + 1], v[4 * (i % 4) + 2], v[4 * (i % 4) + 3]);
       }
-      s_ml[wave][0][lane] = m_run[0];
-      s_ml[wave][1][lane] = l_run[0];
+      s_ml[wave][0][lane] = m_run;
+      s_ml[wave][1][lane] = l_run;
       __syncthreads();
       float m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -796,11 +761,11 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
         up[v] = mv == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mv - m);
         l += s_ml[v][1][lane] * up[v];
       }
-      m_run[0] = m;
-      l_run[0] = l;
+      m_run = m;
+      l_run = l;
     }
     // group i of this wave's, its number among all
-    auto group_of = [&](int rb, int i, int& number) __attribute__((always_inline)) -> float4 {
+    auto group_of = [&](int i, int& number) __attribute__((always_inline)) -> float4 {
       if constexpr (!WIDE && S::NW > 1) {
         constexpr int PER = SB / (GROUPS * SAH_WAVE * 16);
         number = wave * MINE + i;
@@ -816,7 +781,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
         return sum;
       } else {
         number = i;
-        const auto& v = acc[rb][i / 4];
+        const auto& v = acc[i / 4];
         return make_float4(v[4 * (i % 4)], v[4 * (i % 4) + 1], v[4 * (i % 4) + 2], v[4 * (i % 4) + 3]);
       }
     };
@@ -826,45 +791,39 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
       sah_keep(kept_again);
       const int i32 = kept_again & 31, g = kept_again >> 5;
       if (whole) {
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          float l = l_run[rb];
-          if (P.sinks) {
-            // a row that has seen nothing has nothing to weigh against its sink
-            const float z = fmaf(P.sinks[head[rb]], 1.4426950408889634f, pa_weights<DT>::SCALE) - m_run[rb];
-            if (m_run[rb] != -INFINITY) l += __builtin_amdgcn_exp2f(z);
-          }
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          bool fine = true;
-          char* op = (char*)P.out + ((int64_t)tok[rb] * P.os_t + (int64_t)head[rb] * P.os_h) * ES;
-#pragma unroll
-          for (int i = 0; i < MINE; ++i) {
-            int number;
-            const float4 a = group_of(rb, i, number);
-            const int d = 8 * number + 4 * g;
-            if (d >= P.D) continue;
-            const float4 o = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-            fine = fine && fabsf(o.x) < INFINITY && fabsf(o.y) < INFINITY && fabsf(o.z) < INFINITY && fabsf(o.w) < INFINITY;
-            if (!live[rb]) continue;
-            if (DT == SAH_F32) *(float4*)(op + 4 * d) = o;
-            else *(uint2*)(op + 2 * d) = make_uint2(sah_pack2_hw<DT>(o.x, o.y), sah_pack2_hw<DT>(o.z, o.w));
-          }
-          bad = bad || (live[rb] && !fine);
+        float l = l_run;
+        if (P.sinks) {
+          // a row that has seen nothing has nothing to weigh against its sink
+          const float z = fmaf(P.sinks[head], 1.4426950408889634f, pa_weights<DT>::SCALE) - m_run;
+          if (m_run != -INFINITY) l += __builtin_amdgcn_exp2f(z);
         }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        bool fine = true;
+        char* op = (char*)P.out + ((int64_t)tok * P.os_t + (int64_t)head * P.os_h) * ES;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+          int number;
+          const float4 a = group_of(i, number);
+          const int d = 8 * number + 4 * g;
+          if (d >= P.D) continue;
+          const float4 o = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+          fine = fine && fabsf(o.x) < INFINITY && fabsf(o.y) < INFINITY && fabsf(o.z) < INFINITY && fabsf(o.w) < INFINITY;
+          if (!live) continue;
+          if (DT == SAH_F32) *(float4*)(op + 4 * d) = o;
+          else *(uint2*)(op + 2 * d) = make_uint2(sah_pack2_hw<DT>(o.x, o.y), sah_pack2_hw<DT>(o.z, o.w));
+        }
+        bad = bad || (live && !fine);
       } else {
         // a part: to slot 0 where the tile began before this workgroup's piece, else to slot 1
         float* to = P.work + S::WGS * (sizeof(pa_note) / 4) + (int64_t)(2 * w + (y0 ? 0 : 1)) * S::SLOT;
+        const int r = rw * 32 + i32;
+        if (live && g == 0 && (WIDE || wave == 0)) ((float2*)to)[r] = make_float2(m_run, l_run);
+        float* o = to + 2 * S::ROWS + r * DP;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          const int r = (rw * RB + rb) * 32 + i32;
-          if (live[rb] && g == 0 && (WIDE || wave == 0)) ((float2*)to)[r] = make_float2(m_run[rb], l_run[rb]);
-          float* o = to + 2 * S::ROWS + r * DP;
-#pragma unroll
-          for (int i = 0; i < MINE; ++i) {
-            int number;
-            const float4 a = group_of(rb, i, number);
-            if (live[rb]) *(float4*)(o + 8 * number + 4 * g) = a;
-          }
+        for (int i = 0; i < MINE; ++i) {
+          int number;
+          const float4 a = group_of(i, number);
+          if (live) *(float4*)(o + 8 * number + 4 * g) = a;
         }
         if (y0 == 0 && threadIdx.x == 0) {
           // the workgroup whose piece holds the tile's last key: the first whose end is not before the tile's
@@ -1063,7 +1022,7 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
 // ---------------------------------------------------------------------------
 // Tiles of 128 rows whose waves share the keys, or of 32 rows whose waves each take keys of their own: by the rows per request.
 // fp32 is bound by its matrix instructions (a sixteenth of the 16-bit rate) however often keys are read: 32 rows, so that a
-// request of few rows keeps all waves busy (5 requests of 4 to 132 rows, 2000 keys on average: 59 us as tiles of 128, %F32% so).
+// request of few rows keeps all waves busy (5 requests of 4 to 132 rows, 2000 keys on average: 66 us as tiles of 128, 34 so).
 static bool pa_wide(const sah_paged_attention_args* a) {
   return a->dtype != SAH_F32 && (int64_t)a->n_tokens * (a->Hq / a->Hkv) > 32 * (int64_t)a->n_requests;
 }
@@ -1074,17 +1033,32 @@ static int64_t pa_floats() {
   return S::WGS * (int64_t)(sizeof(pa_note) / 4) + 2 * (int64_t)S::WGS * S::SLOT;
 }
 
+// About as many workgroups as the call has work for, at most what the card holds at once: a short call's idle ones, and theirs of the
+// second kernel, cost it 0.3 to 0.6 us of 17. Only how the work is shared depends on it.
+template <typename S>
+static int pa_workgroups(const sah_paged_attention_args* a) {
+  const int G = a->Hq / a->Hkv;
+  const int64_t table = (int64_t)a->table_width * a->page_size;
+  int64_t keys = a->max_context > 0 && a->max_context < table ? a->max_context : table;
+  if (a->window && (int64_t)a->sink + a->window + S::ROWS < keys) keys = (int64_t)a->sink + a->window + S::ROWS;
+  const double tiles = ((double)a->n_tokens * G / S::ROWS + a->n_requests) * a->Hkv;
+  const double n = tiles * (double)(keys + S::TILE_COST) / S::LEAST;
+  return n < S::WGS ? ((int)n / PA_XCDS + 1) * PA_XCDS : S::WGS;
+}
+
 template <int DT, int DP, bool WIDE>
 static int pa_launch(const sah_paged_attention_args* a) {
   typedef pa_shape<DT, DP, WIDE> S;
+  static_assert(S::WGS % PA_XCDS == 0, "workgroups are dealt to the XCDs in turn");
+  const int wgs = pa_workgroups<S>(a);
   hipStream_t st = (hipStream_t)a->stream;
   {
     sah_timed timed("k_paged_attn", a->stream);
-    hipLaunchKernelGGL((k_paged_attn<DT, DP, WIDE>), dim3(S::WGS), dim3(S::NT), 0, st, *a);
+    hipLaunchKernelGGL((k_paged_attn<DT, DP, WIDE>), dim3(wgs), dim3(S::NT), 0, st, *a);
     if (int rc = sah_launch_status("sah_paged_attention")) return rc;
   }
   sah_timed timed("k_paged_attn_join", a->stream);
-  hipLaunchKernelGGL((k_paged_attn_join<DT, DP, WIDE>), dim3(S::WGS, PA_JOIN_WGS), dim3(PA_JOIN_NT), 0, st, *a);
+  hipLaunchKernelGGL((k_paged_attn_join<DT, DP, WIDE>), dim3(wgs, PA_JOIN_WGS), dim3(PA_JOIN_NT), 0, st, *a);
   return sah_launch_status("sah_paged_attention(join)");
 }
 
