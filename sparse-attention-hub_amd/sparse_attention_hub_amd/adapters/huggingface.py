@@ -12,7 +12,8 @@ adapter that touches the attention path:
   * enable_sparse_mode (:345-385): `config._attn_implementation` switched for the duration of a block;
   * process_request / _generate_response (:106-202, :387-484): the context is prefilled with the model's
     own dense attention, then - in sparse mode - the question tokens in one pass (Lq > 1) and a greedy
-    decode, one token at a time, `sparse_meta_data` carried through every forward call.
+    decode, one token at a time, `sparse_meta_data` carried through every forward call. With `sampling` the tokens
+    are drawn instead (`sample_tokens`), which the reference does not do.
 The reference's adapter also owns a model server, a tokenizer and a request type; those are outside the
 attention path. This adapter takes a loaded model and token ids instead (`process_tokens`).
 """
@@ -26,6 +27,9 @@ from typing import Any, Callable, Dict, Generator, List, Optional, Sequence, Tup
 import torch
 
 from ..sparse_attention import ResearchAttention, SparseAttention, SparseAttentionConfig
+from ..sparse_attention.utils.token_sampling import sample_tokens
+
+SAMPLING_SETTINGS = ("temperature", "top_k", "top_p", "min_p")
 
 
 class ModelAdapterHF:
@@ -138,8 +142,9 @@ class ModelAdapterHF:
 
     # ------------------------------------------------------------------ generation
     def _generate_tokens(self, question_tokens: torch.Tensor, context_outputs: Any, sparse_meta_data: Dict[str, Any],
-                         max_new_tokens: int, stop_token_ids: Sequence[int] = ()) -> torch.Tensor:
-        """Greedy continuation after the context prefill — the token-id form of _generate_response."""
+                         max_new_tokens: int, stop_token_ids: Sequence[int] = (),
+                         sampling: Optional[Dict[str, Any]] = None, generator: Optional[torch.Generator] = None) -> torch.Tensor:
+        """Continuation after the context prefill — the token-id form of _generate_response."""
         past = context_outputs.past_key_values
         last = None
 
@@ -160,20 +165,35 @@ class ModelAdapterHF:
             past = last.past_key_values
         if last is None:
             raise ValueError("Question tokens are empty; cannot generate response")
-        generated = [last.logits[0, -1].argmax()]
+
+        def choose(logits: torch.Tensor) -> torch.Tensor:
+            if sampling is None:
+                return logits.argmax()
+            uniforms = torch.rand(1, dtype=torch.float32, device=logits.device, generator=generator)
+            # a row without a logit above -inf has no token: the first one, as argmax has it
+            return sample_tokens(logits.unsqueeze(0), uniforms, **sampling)[0][0].clamp_min(0)
+
+        generated = [choose(last.logits[0, -1])]
         for _ in range(max_new_tokens - 1):
             out = forward(generated[-1].unsqueeze(0).unsqueeze(0))
             past = out.past_key_values
-            new_id = out.logits[0, -1].argmax()
+            new_id = choose(out.logits[0, -1])
             generated.append(new_id)
             if stop_token_ids and int(new_id.item()) in stop_token_ids:
                 break
         return torch.stack(generated)
 
     def process_tokens(self, context_tokens: torch.Tensor, questions: Sequence[torch.Tensor], max_new_tokens: int,
-                       stop_token_ids: Sequence[int] = ()) -> List[torch.Tensor]:
+                       stop_token_ids: Sequence[int] = (), sampling: Optional[Dict[str, Any]] = None,
+                       generator: Optional[torch.Generator] = None) -> List[torch.Tensor]:
         """The token-id form of process_request: the context is prefilled once per question with the model's own
-        attention, each question is answered independently (fresh sparse_meta_data, fresh KV cache)."""
+        attention, each question is answered independently (fresh sparse_meta_data, fresh KV cache).
+
+        `sampling`: None answers greedily; else any of `sample_tokens`' settings (`temperature`, `top_k`, `top_p`, `min_p`), with one
+        number of `generator` (on the model's device; default: that device's own) per token."""
+        unknown = sorted(set(sampling or ()) - set(SAMPLING_SETTINGS))
+        if unknown:
+            raise ValueError(f"sampling takes {', '.join(SAMPLING_SETTINGS)}; got {', '.join(map(str, unknown))}")
         self.model.eval()
         answers: List[torch.Tensor] = []
         with torch.no_grad():
@@ -184,9 +204,9 @@ class ModelAdapterHF:
                                                  sparse_meta_data=sparse_meta_data)
                     with self.enable_sparse_mode():
                         answers.append(self._generate_tokens(question_tokens, context_outputs, sparse_meta_data,
-                                                             max_new_tokens, stop_token_ids))
+                                                             max_new_tokens, stop_token_ids, sampling, generator))
                 else:
                     context_outputs = self.model(context_tokens, past_key_values=None, use_cache=True)
                     answers.append(self._generate_tokens(question_tokens, context_outputs, sparse_meta_data,
-                                                         max_new_tokens, stop_token_ids))
+                                                         max_new_tokens, stop_token_ids, sampling, generator))
         return answers
