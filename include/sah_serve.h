@@ -111,7 +111,9 @@ int sah_paged_attention(const sah_paged_attention_args* a);
  * counts as the nearest number inside, NaN as 0. t <= 0 or NaN: the largest logit's token. logprobs, optional: the logarithm of
  * the token's share of the kept weight. A row without a logit above -inf gives token -1, logprob -inf; one with logits
  * of +inf chooses among those. Weights and their sums are held in 64 bits and do not depend on the order of the sums.
- * Each of the four settings is an array of n_rows values or, where that is NULL, one value for all. vocab at most 2^20. */
+ * Each of the four settings is an array of n_rows values or, where that is NULL, one value for all. vocab at most 2^20.
+ * work: sah_sample_work_bytes(a) bytes, no particular content, 16-byte aligned: few rows are then shared by several workgroups each;
+ * NULL: every row by one. The results are the same. */
 typedef struct sah_sample_args {
   const void* logits; int64_t row_pitch;
   int32_t dtype;
@@ -122,7 +124,9 @@ typedef struct sah_sample_args {
   int64_t* tokens;
   float* logprobs;
   void* stream;
+  void* work; int64_t work_bytes;               /* optional */
 } sah_sample_args;
+int64_t sah_sample_work_bytes(const sah_sample_args* a);
 int sah_sample_tokens(const sah_sample_args* a);
 
 #ifdef __cplusplus

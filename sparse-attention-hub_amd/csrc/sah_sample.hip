@@ -22,8 +22,11 @@
 #define SM_SMALL 64        // items that are ranked at once, one a lane
 #define SM_FINE 64.f
 #define SM_RANK_K 1000     // top-k up to this goes by the threads' largest logits (1024 ln(1024 / 24) = 3800 tokens on average) ...
-#define SM_RANK_P 1021     // ... and top-p tries the tokens above this one of them (6000)
+#define SM_REST_P 3        // ... and top-p tries the tokens above all but these of them (6000)
 #define SM_LOWEST 0x00800000u  // order of the lowest finite logit
+#define SM_SPLIT_WGS 256
+#define SM_SLICE 4096
+#define SM_SLICES 16       // workgroups that share a row's passes, at most
 typedef sah_u4 sm_vec __attribute__((aligned(2)));
 
 struct sm_shared {
@@ -237,34 +240,49 @@ __device__ __forceinline__ sm_item sm_pick(sm_shared& S, int& round, uint32_t lo
   }
 }
 
+// A row: its settings, its largest logit, and the pieces of 1 / SM_FINE in (m - x) / t that it is cut into, the last one for all that is further down
 template <int DT>
-__global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
-  sah_touch_kernargs<sizeof(sah_sample_args)>();
-  SAH_DYNAMIC_LDS(s_dyn);
-  sm_shared& S = *(sm_shared*)s_dyn;
-  constexpr int ES = DT == SAH_F32 ? 4 : 2, E = 16 / ES;
-  const int r = blockIdx.x, V = P.vocab;
-  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
-  const void* x = (const char*)P.logits + (int64_t)r * P.row_pitch * ES;
-  const float temp = P.temperatures ? P.temperatures[r] : P.temperature;
-  const int k = P.top_ks ? P.top_ks[r] : P.top_k;
-  const float p = P.top_ps ? P.top_ps[r] : P.top_p;
-  float least = P.min_ps ? P.min_ps[r] : P.min_p;
-  least = least > 1.f ? 1.f : least;
-  const bool use_k = k > 0 && k < V, use_p = p < 1.f, use_m = least > 0.f;
-  for (int b = threadIdx.x; b < SM_BINS; b += SM_NT) S.bins[b] = 0;
-  if (threadIdx.x == 0) S.count = S.n_small[0] = S.n_small[1] = 0;
-  int round = 0;
+struct sm_row {
+  static constexpr int ES = DT == SAH_F32 ? 4 : 2, E = 16 / ES;
+  static constexpr int U = 4, SEG = SAH_WAVE * E * U;  // a segment: what a wave reads in U turns
+  const void* x;
+  int V, k;
+  float temp, p, least;
+  bool use_k, use_p, use_m;
+  float best, fine;
+  int best_at;
+  __device__ __forceinline__ sm_row(const sah_sample_args& P, int r) {
+    V = P.vocab;
+    x = (const char*)P.logits + (int64_t)r * P.row_pitch * ES;
+    temp = P.temperatures ? P.temperatures[r] : P.temperature;
+    k = P.top_ks ? P.top_ks[r] : P.top_k;
+    p = P.top_ps ? P.top_ps[r] : P.top_p;
+    least = P.min_ps ? P.min_ps[r] : P.min_p;
+    least = least > 1.f ? 1.f : least;
+    use_k = k > 0 && k < V;
+    use_p = p < 1.f;
+    use_m = least > 0.f;
+  }
+  __device__ __forceinline__ void largest(float value, int at) {
+    best = value;
+    best_at = at;
+    fine = SM_FINE / temp;
+  }
+  __device__ __forceinline__ bool one_answer() const { return best == -INFINITY || !(temp > 0.f); }
+  __device__ __forceinline__ bool listed() const { return (use_k || use_p || use_m) && (V <= SM_CAP || !use_k || k <= SM_RANK_K); }
+  __device__ __forceinline__ bool total() const { return use_p && !use_k && V > SM_CAP; }  // every weight is needed for top-p
+  __device__ __forceinline__ bool everything() const { return !use_k && !use_p && !use_m; }
+  __device__ __forceinline__ int piece(float v) const {
+    const float d = (best - v) * fine;
+    return v == best ? 0 : d < SM_BINS - 1 ? (int)d : SM_BINS - 1;
+  }
+};
 
-  // the largest logit and its first place
-  float best = -INFINITY;
-  int best_at = INT32_MAX;
-  sm_each<DT, 4>(x, V, [&](float v, int i) {
-    best_at = v > best ? i : best_at;
-    best = v > best ? v : best;
-  });
-  const float own = best;
-  float low = best;  // the smallest of the threads' largest
+struct sm_top { float value, low; int at; };
+// Over the workgroup: the largest value and the first place of it, and the smallest value above -inf (all -inf: +inf).
+__device__ __forceinline__ sm_top sm_largest(sm_shared& S, float best, int best_at) {
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
+  float low = best > -INFINITY ? best : INFINITY;
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     const float o = __shfl_xor(best, d);
@@ -283,22 +301,243 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
     best_at = o > best ? oa : (o == best && oa < best_at ? oa : best_at);
     best = fmaxf(o, best);
   }
-  if (best == -INFINITY || !(temp > 0.f)) {
+  return sm_top{best, low, best_at};
+}
+
+struct sm_from {
+  float value;     // the list holds the tokens of at least this
+  bool complete;   // it has every token that min-p keeps
+};
+// own: the largest logit of this thread's share of the row (-inf: it has none). All threads call.
+template <int DT>
+__device__ __forceinline__ sm_from sm_list_from(sm_shared& S, const sm_row<DT>& row, float own, float low) {
+  sm_from f{-INFINITY, true};
+  if (row.V <= SM_CAP) return f;
+  const uint32_t top = sm_order(row.best);
+  if (row.use_k || row.use_p) {
+    const uint32_t range = top - sm_order(low);
+    const int bits = range ? 32 - __builtin_clz(range) : 0, shift = bits > 11 ? bits - 11 : 0;
+    const sm_bin b = sm_locate(
+        S, [&](uint64_t all) -> uint64_t { return row.use_k ? (uint64_t)row.k : all > SM_REST_P ? all - SM_REST_P : 1; },
+        [&](auto put) { if (own > -INFINITY) put((top - sm_order(own)) >> shift, 1); });
+    if (b.at >= 0) {
+      const uint32_t down = ((uint32_t)(b.at + 1) << shift) - 1;  // to the lower end of the piece
+      f.value = sm_value(down < range ? top - down : top - range);
+      f.complete = false;
+    }
+  }
+  if (row.use_m && !row.use_k) {
+    // e >= least where x >= m + t ln(least); a little below that, for the roundings
+    const sm_weights weigh(row.best, row.temp);
+    const double at = weigh.m + (double)row.temp * log((double)row.least);
+    const float below = (float)(at - 1e-6 * (fabs(at) + fabs(weigh.m)) - 1e-30);
+    if (below > f.value || !row.use_p) {
+      f.value = below == below ? below : -INFINITY;
+      f.complete = true;
+    }
+  }
+  return f;
+}
+
+__device__ __forceinline__ void sm_enlist(sm_shared& S, float v, int i) {
+  const int n = atomicAdd(&S.count, 1);
+  if (n < SM_CAP) S.list[n] = make_uint2(sah_float_to_bits(v), (uint32_t)i);
+}
+__device__ __forceinline__ void sm_begin(sm_shared& S) {
+  for (int b = threadIdx.x; b < SM_BINS; b += SM_NT) S.bins[b] = 0;
+  if (threadIdx.x == 0) S.count = S.n_small[0] = S.n_small[1] = 0;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the passes over a whole row are shared by up to SM_SLICES workgroups, in two kernels ahead of the row's own.
+// ---------------------------------------------------------------------------
+struct sm_work {  // of a row
+  uint64_t bins[SM_BINS];    // weight of the pieces
+  uint64_t segs[SM_NT];      // weight of the segments
+  uint2 list[SM_CAP];
+  float own[SM_NT];          // the largest logits of SM_NT shares of the row, -inf where a share is empty
+  float best[SM_SLICES];     // ... of the slices
+  int best_at[SM_SLICES];
+  sm_from from;
+  int count;
+  int pad;
+};
+
+template <int DT>
+struct sm_slice {
+  int begin, n;  // tokens; n may be 0
+  __device__ __forceinline__ sm_slice(int V, int number, int slices) {
+    constexpr int SEG = sm_row<DT>::SEG;
+    const int segs = (V + SEG - 1) / SEG, each = (segs + slices - 1) / slices * SEG;
+    begin = number * each;  // (below 2^20 + 16 SEG)
+    n = begin < V ? (V - begin < each ? V - begin : each) : 0;
+  }
+};
+
+// Every slice's largest logit, and those of SM_NT / slices shares of it (slices: a power of two)
+template <int DT>
+__global__ __launch_bounds__(SM_NT, 4) void k_sample_largest(sah_sample_args P) {
+  __shared__ float s_own[SM_NT];
+  SAH_DYNAMIC_LDS(s_dyn);
+  sm_shared& S = *(sm_shared*)s_dyn;
+  const sm_row<DT> row(P, blockIdx.y);
+  const sm_slice<DT> slice(row.V, blockIdx.x, gridDim.x);
+  sm_work& W = ((sm_work*)P.work)[blockIdx.y];
+  const int bins = SM_BINS / (int)gridDim.x, shares = SM_NT / (int)gridDim.x;
+  for (int b = threadIdx.x; b < bins; b += SM_NT) W.bins[blockIdx.x * bins + b] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) W.count = 0;
+  float best = -INFINITY;
+  int best_at = INT32_MAX;
+  sm_each<DT, 4>((const char*)row.x + (int64_t)slice.begin * row.ES, slice.n, [&](float v, int i) {
+    best_at = v > best ? i + slice.begin : best_at;
+    best = v > best ? v : best;
+  });
+  s_own[threadIdx.x] = best;
+  const sm_top top = sm_largest(S, best, best_at);  // (waits)
+  if ((int)threadIdx.x < shares) {
+    float own = -INFINITY;
+    for (int t = threadIdx.x; t < SM_NT; t += shares) own = fmaxf(own, s_own[t]);
+    W.own[blockIdx.x * shares + threadIdx.x] = own;
+  }
+  if (threadIdx.x == 0) {
+    W.best[blockIdx.x] = top.value;
+    W.best_at[blockIdx.x] = top.at;
+  }
+}
+
+// the row's largest logit out of its slices'
+template <int DT>
+__device__ __forceinline__ void sm_largest_of(sm_row<DT>& row, const sm_work& W, int slices) {
+  float best = -INFINITY;
+  int at = INT32_MAX;
+  for (int i = 0; i < slices; ++i) {  // in the order of the index
+    at = W.best[i] > best ? W.best_at[i] : at;
+    best = fmaxf(best, W.best[i]);
+  }
+  row.largest(best, at);
+}
+
+// Writes the weights of the segments of [begin, begin + n), a wave's turn each. plain: weight is sm_fixed(weigh(v)).
+template <int DT, typename WEIGHT>
+__device__ __forceinline__ void sm_segments(const sm_row<DT>& row, int begin, int n, bool plain, const sm_weights& weigh, uint64_t* segs, WEIGHT weight) {
+  constexpr int ES = sm_row<DT>::ES, E = sm_row<DT>::E, U = sm_row<DT>::U, SEG = sm_row<DT>::SEG;
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id(), end = begin + n;
+  const int n_segs = (n + SEG - 1) / SEG;
+  auto place = [&](int j) { return begin + (wave + j / U * SM_NW) * SEG + (j % U * SAH_WAVE + lane) * E; };  // this lane's j-th piece
+  auto load = [&](int i) __attribute__((always_inline)) -> sah_u4 { return i + E <= end ? *(const sm_vec*)((const char*)row.x + (int64_t)i * ES) : sah_u4{0, 0, 0, 0}; };
+  sah_u4 next = load(place(0));
+  uint64_t part = 0;
+#pragma unroll 1
+  for (int j = 0; wave + j / U * SM_NW < n_segs; ++j) {
+    const sah_u4 v = next;
+    const int i = place(j);
+    next = load(place(j + 1));
+    if (i + E <= end && plain) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) part += sm_raw(weigh(sm_unpack<DT>(v, e)));
+      part -= E * SM_ZERO;
+    } else if (i + E <= end) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) part += weight(sm_unpack<DT>(v, e), i + e);
+    } else {
+#pragma unroll 1
+      for (int e = 0; i + e < end; ++e) part += weight(sah_load<DT>(row.x, i + e), i + e);
+    }
+    if (j % U == U - 1) {
+      part = sah_lane_u64(sah_wave_incl_scan_u64(part), SAH_WAVE - 1);
+      if (lane == 0) segs[begin / SEG + wave + j / U * SM_NW] = part;
+      part = 0;
+    }
+  }
+}
+
+// Every slice's tokens for the list, and the weights of its pieces or segments
+template <int DT>
+__global__ __launch_bounds__(SM_NT, 4) void k_sample_slices(sah_sample_args P) {
+  SAH_DYNAMIC_LDS(s_dyn);
+  sm_shared& S = *(sm_shared*)s_dyn;
+  sm_row<DT> row(P, blockIdx.y);
+  const sm_slice<DT> slice(row.V, blockIdx.x, gridDim.x);
+  sm_work& W = ((sm_work*)P.work)[blockIdx.y];
+  sm_largest_of(row, W, gridDim.x);
+  if (row.one_answer()) return;
+  const sm_weights weigh(row.best, row.temp);
+  if (row.everything()) {
+    sm_segments<DT>(row, slice.begin, slice.n, true, weigh, W.segs, [&](float v, int) { return sm_fixed(weigh(v)); });
+    return;
+  }
+  if (!row.listed()) return;
+  sm_begin(S);
+  const float own = W.own[threadIdx.x];
+  const sm_top top = sm_largest(S, own, 0);  // (waits)
+  const sm_from from = sm_list_from<DT>(S, row, own, top.low);
+  if (blockIdx.x == 0 && threadIdx.x == 0) W.from = from;
+  const void* x = (const char*)row.x + (int64_t)slice.begin * row.ES;
+  auto enlist = [&](float v, int i) __attribute__((always_inline)) { if (v >= from.value && v > -INFINITY) sm_enlist(S, v, i + slice.begin); };
+  if (row.total()) {
+    sm_each<DT, 1>(x, slice.n, [&](float v, int i) {
+      enlist(v, i);
+      atomicAdd((unsigned long long*)&S.bins[row.piece(v)], (unsigned long long)sm_fixed(weigh(v)));
+    });
+  } else {
+    sm_each<DT, 4>(x, slice.n, enlist);
+  }
+  __syncthreads();
+  const int n = S.count;
+  if (threadIdx.x == 0) S.found_bin = atomicAdd(&W.count, n);
+  if (row.total())
+    for (int b = threadIdx.x; b < SM_BINS; b += SM_NT)
+      if (S.bins[b]) atomicAdd((unsigned long long*)&W.bins[b], (unsigned long long)S.bins[b]);
+  __syncthreads();
+  const int at = S.found_bin;
+  if (n > SM_CAP || at > SM_CAP - n) return;  // too many: the count says so
+  for (int j = threadIdx.x; j < n; j += SM_NT) W.list[at + j] = S.list[j];
+}
+
+// SPLIT: by `slices` workgroups' work so far
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P, int slices) {
+  sah_touch_kernargs<sizeof(sah_sample_args)>();
+  SAH_DYNAMIC_LDS(s_dyn);
+  sm_shared& S = *(sm_shared*)s_dyn;
+  constexpr int E = sm_row<DT>::E, U = sm_row<DT>::U, SEG = sm_row<DT>::SEG;
+  const int r = blockIdx.x;
+  sm_row<DT> row(P, r);
+  const int V = row.V, k = row.k;
+  const void* x = row.x;
+  const float p = row.p, least = row.least;
+  const bool use_k = row.use_k, use_p = row.use_p, use_m = row.use_m;
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
+  [[maybe_unused]] const sm_work& W = ((const sm_work*)P.work)[SPLIT ? r : 0];
+  sm_begin(S);
+  int round = 0;
+
+  // the largest logit and its first place
+  [[maybe_unused]] float own = -INFINITY, low = INFINITY;
+  if constexpr (SPLIT) {
+    sm_largest_of(row, W, slices);
+    __syncthreads();
+  } else {
+    int own_at = INT32_MAX;
+    sm_each<DT, 4>(x, V, [&](float v, int i) {
+      own_at = v > own ? i : own_at;
+      own = v > own ? v : own;
+    });
+    const sm_top top = sm_largest(S, own, own_at);
+    low = top.low;
+    row.largest(top.value, top.at);
+  }
+  const float best = row.best, fine = row.fine;
+  if (row.one_answer()) {
     if (threadIdx.x == 0) {
-      P.tokens[r] = best == -INFINITY ? -1 : best_at;
+      P.tokens[r] = best == -INFINITY ? -1 : row.best_at;
       if (P.logprobs) P.logprobs[r] = best == -INFINITY ? -INFINITY : 0.f;
     }
     return;
   }
-  const sm_weights weigh(best, temp);
+  const sm_weights weigh(best, row.temp);
   const uint32_t top = sm_order(best);
-
-  // pieces of 1 / SM_FINE in (m - x) / t, the last one for all that is further down
-  const float fine = SM_FINE / temp;
-  auto piece = [&](float v) -> int {
-    const float d = (best - v) * fine;
-    return v == best ? 0 : d < SM_BINS - 1 ? (int)d : SM_BINS - 1;
-  };
+  auto piece = [&](float v) { return row.piece(v); };
   // whole numbers before a token are less than p times the sum where they are less than that rounded up; the first is kept
   auto nucleus = [&](uint64_t all) -> uint64_t {
     const double limit = ceil((double)p * (double)all);
@@ -309,69 +548,60 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
   int last = -1;
   auto kept = [&](float v, int i) { return v > thr || (v == thr && i <= last); };
   int n_list = 0;
-  auto enlist = [&](float v, int i) {
-    const int n = atomicAdd(&S.count, 1);
-    if (n < SM_CAP) S.list[n] = make_uint2(sah_float_to_bits(v), (uint32_t)i);
-  };
   auto list_again = [&](auto take) __attribute__((always_inline)) {  // a new list, of the kept tokens that `take` takes; whether it holds them
     if (threadIdx.x == 0) S.count = 0;
     __syncthreads();
-    sm_each<DT, 1>(x, V, [&](float v, int i) { if (kept(v, i) && take(v)) enlist(v, i); });
+    sm_each<DT, 1>(x, V, [&](float v, int i) { if (kept(v, i) && take(v)) sm_enlist(S, v, i); });
     __syncthreads();
     n_list = S.count;
     return n_list <= SM_CAP;
   };
 
   // the tokens that may be kept, in a list, where they are not too many
-  bool list = false, complete = true;  // complete: the list has every token that min-p keeps
-  const bool total = use_p && !use_k && V > SM_CAP;
+  bool list = false;
+  const bool total = row.total();
   uint64_t whole = 0;                  // total: the weight that top-p's last token reaches ...
   sm_bin border{0, 0};                 // ... and its piece
   uint32_t lowest = SM_LOWEST;         // no token of the list is of a lower order
-  if ((use_k || use_p || use_m) && (V <= SM_CAP || !use_k || k <= SM_RANK_K)) {
-    float from = -INFINITY;
-    if (V > SM_CAP) {
-      if ((use_k || use_p) && low > -INFINITY) {  // every thread has a logit
-        const uint32_t range = top - sm_order(low);
-        const int bits = range ? 32 - __builtin_clz(range) : 0, shift = bits > 11 ? bits - 11 : 0;
-        const uint64_t rank = use_k ? k : SM_RANK_P;
-        const sm_bin b = sm_locate(S, [&](uint64_t) { return rank; }, [&](auto put) { put((top - sm_order(own)) >> shift, 1); });
-        const uint32_t down = ((uint32_t)(b.at + 1) << shift) - 1;  // to the lower end of the piece
-        from = sm_value(down < range ? top - down : top - range);
-        complete = false;
-      }
-      if (use_m && !use_k) {
-        // e >= least where x >= m + t ln(least); a little below that, for the roundings
-        const double at = weigh.m + (double)temp * log((double)least);
-        const float below = (float)(at - 1e-6 * (fabs(at) + fabs(weigh.m)) - 1e-30);
-        if (below > from || !use_p) {
-          from = below == below ? below : -INFINITY;
-          complete = true;
-        }
-      }
-      if (from > -INFINITY && from < best) lowest = sm_order(from);
+  if (row.listed()) {
+    sm_from from;
+    if constexpr (SPLIT) {
+      from = W.from;
+      n_list = W.count;
+      if (n_list <= SM_CAP)
+        for (int j = threadIdx.x; j < n_list; j += SM_NT) S.list[j] = W.list[j];
+    } else {
+      from = sm_list_from<DT>(S, row, own, low);
     }
+    if (from.value > -INFINITY && from.value < best) lowest = sm_order(from.value);
     if (total) {
       // the weights' pass shares the row out into pieces too: if top-p's last token lies below the list, its piece is known
       border = sm_locate(
           S, [&](uint64_t all) { return whole = nucleus(all); },
           [&](auto put) __attribute__((always_inline)) {
-            sm_each<DT, 1>(x, V, [&](float v, int i) {
-              if (v >= from && v > -INFINITY) enlist(v, i);
-              put(piece(v), sm_fixed(weigh(v)));
-            });
+            if constexpr (SPLIT) {
+              const sah_u4 two = *(const sah_u4*)&W.bins[2 * threadIdx.x];
+              *(sah_u4*)&S.bins[2 * threadIdx.x] = two;
+            } else {
+              sm_each<DT, 1>(x, V, [&](float v, int i) {
+                if (v >= from.value && v > -INFINITY) sm_enlist(S, v, i);
+                put(piece(v), sm_fixed(weigh(v)));
+              });
+            }
           });
-      if (from > -INFINITY && !complete && piece(from) <= border.at) {
+      if constexpr (!SPLIT) n_list = S.count;
+      if (from.value > -INFINITY && !from.complete && piece(from.value) <= border.at) {
         // further down than the list: all down to there, if it holds that
         const float down = best - (border.at + 1.01f) / fine;
         lowest = border.at < SM_BINS - 1 && down > -INFINITY && down < best ? sm_order(down) : SM_LOWEST;
         list_again([&](float v) { return piece(v) <= border.at; });
       }
-    } else {
-      sm_each<DT, 4>(x, V, [&](float v, int i) { if (v >= from && v > -INFINITY) enlist(v, i); });
+    } else if constexpr (!SPLIT) {
+      sm_each<DT, 4>(x, V, [&](float v, int i) { if (v >= from.value && v > -INFINITY) sm_enlist(S, v, i); });
+      __syncthreads();
+      n_list = S.count;
     }
     __syncthreads();
-    n_list = S.count;
     list = n_list <= SM_CAP;
   }
   auto each = [&](bool from_list, auto f) __attribute__((always_inline)) {
@@ -441,40 +671,17 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
     if (threadIdx.x == 0) answer(f.index, all);
     return;
   }
-  // The whole row: the weights of segments of 4 x 64 E tokens; then inside the one that holds the target.
-  constexpr int U = 4, SEG = SAH_WAVE * E * U;
+  // The whole row: the weights of its segments; then inside the one that holds the target.
   static_assert(SM_MAX_VOCAB / SEG <= SM_NT && SM_NT <= SM_CAP, "a sum a thread");
-  uint64_t* segs = (uint64_t*)S.list;
   const int n_segs = (V + SEG - 1) / SEG;
-  __syncthreads();  // the list is no longer read
-  auto place = [&](int j) { return (wave + j / U * SM_NW) * SEG + (j % U * SAH_WAVE + lane) * E; };  // this lane's j-th piece
-  auto load = [&](int i) __attribute__((always_inline)) -> sah_u4 { return i + E <= V ? *(const sm_vec*)((const char*)x + (int64_t)i * ES) : sah_u4{0, 0, 0, 0}; };
-  sah_u4 next = load(place(0));
-  uint64_t part = 0;
-  const bool everything = thr == -INFINITY && !use_m;
-#pragma unroll 1
-  for (int j = 0; wave + j / U * SM_NW < n_segs; ++j) {
-    const sah_u4 v = next;
-    const int i = place(j);
-    next = load(place(j + 1));
-    if (i + E <= V && everything) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) part += sm_raw(weigh(sm_unpack<DT>(v, e)));
-      part -= E * SM_ZERO;
-    } else if (i + E <= V) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) part += final_weight(sm_unpack<DT>(v, e), i + e);
-    } else {
-#pragma unroll 1
-      for (int e = 0; i + e < V; ++e) part += final_weight(sah_load<DT>(x, i + e), i + e);
-    }
-    if (j % U == U - 1) {
-      part = sah_lane_u64(sah_wave_incl_scan_u64(part), SAH_WAVE - 1);
-      if (lane == 0) segs[wave + j / U * SM_NW] = part;
-      part = 0;
-    }
+  const uint64_t* segs = (const uint64_t*)S.list;
+  if (SPLIT && row.everything()) {
+    segs = W.segs;
+  } else {
+    __syncthreads();  // the list is no longer read
+    sm_segments<DT>(row, 0, V, thr == -INFINITY && !use_m, weigh, (uint64_t*)S.list, final_weight);
+    __syncthreads();
   }
-  __syncthreads();
   uint64_t all;
   const uint64_t mine = (int)threadIdx.x < n_segs ? segs[threadIdx.x] : 0;
   uint64_t before = sm_block_scan(mine, S, all);
@@ -513,6 +720,39 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P) {
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+// Workgroups a row: as many as fill the card, each with SM_SLICE tokens or more (a power of two).
+static int sm_slices(const sah_sample_args* a) {
+  if (a->n_rows <= 0 || (!a->temperatures && !(a->temperature > 0.f))) return 1;  // (one pass is all that is done)
+  int n = 1;
+  while (n < SM_SLICES && 2 * n * (int64_t)a->n_rows <= SM_SPLIT_WGS && a->vocab / (2 * n) >= SM_SLICE) n *= 2;
+  return n;
+}
+extern "C" int64_t sah_sample_work_bytes(const sah_sample_args* a) {
+  return a && sm_slices(a) > 1 ? (int64_t)a->n_rows * (int64_t)sizeof(sm_work) : 0;
+}
+
+template <int DT>
+static int sm_launch(const sah_sample_args* a, int slices) {
+  hipStream_t st = (hipStream_t)a->stream;
+  auto kernel = slices > 1 ? k_sample<DT, true> : k_sample<DT, false>;
+  if (int rc = sah_allow_lds((const void*)kernel, sizeof(sm_shared), "sah_sample_tokens")) return rc;
+  if (slices > 1) {
+    if (int rc = sah_allow_lds((const void*)k_sample_largest<DT>, sizeof(sm_shared), "sah_sample_tokens")) return rc;
+    if (int rc = sah_allow_lds((const void*)k_sample_slices<DT>, sizeof(sm_shared), "sah_sample_tokens")) return rc;
+    {
+      sah_timed timed("k_sample_largest", a->stream);
+      hipLaunchKernelGGL(k_sample_largest<DT>, dim3(slices, a->n_rows), dim3(SM_NT), sizeof(sm_shared), st, *a);
+      if (int rc = sah_launch_status("sah_sample_tokens(largest)")) return rc;
+    }
+    sah_timed timed("k_sample_slices", a->stream);
+    hipLaunchKernelGGL(k_sample_slices<DT>, dim3(slices, a->n_rows), dim3(SM_NT), sizeof(sm_shared), st, *a);
+    if (int rc = sah_launch_status("sah_sample_tokens(slices)")) return rc;
+  }
+  sah_timed timed("k_sample", a->stream);
+  hipLaunchKernelGGL(kernel, dim3(a->n_rows), dim3(SM_NT), sizeof(sm_shared), st, *a, slices);
+  return sah_launch_status("sah_sample_tokens");
+}
+
 extern "C" int sah_sample_tokens(const sah_sample_args* a) {
   if (!a) return sah_fail(SAH_ENULL, "sah_sample_tokens: args is NULL");
   if (a->dtype != SAH_F32 && a->dtype != SAH_BF16 && a->dtype != SAH_F16) return sah_fail(SAH_EDTYPE, "sah_sample_tokens: dtype %d", a->dtype);
@@ -521,10 +761,9 @@ extern "C" int sah_sample_tokens(const sah_sample_args* a) {
   if (a->row_pitch < a->vocab && a->n_rows > 1) return sah_fail(SAH_EINVAL, "sah_sample_tokens: row_pitch is less than vocab");
   if (a->n_rows == 0) return SAH_OK;
   if (!a->logits || !a->uniforms || !a->tokens) return sah_fail(SAH_ENULL, "sah_sample_tokens: NULL pointer");
-  hipStream_t st = (hipStream_t)a->stream;
-  auto kernel = a->dtype == SAH_F32 ? k_sample<SAH_F32> : a->dtype == SAH_BF16 ? k_sample<SAH_BF16> : k_sample<SAH_F16>;
-  if (int rc = sah_allow_lds((const void*)kernel, sizeof(sm_shared), "sah_sample_tokens")) return rc;
-  sah_timed timed("k_sample", a->stream);
-  hipLaunchKernelGGL(kernel, dim3(a->n_rows), dim3(SM_NT), sizeof(sm_shared), st, *a);
-  return sah_launch_status("sah_sample_tokens");
+  const int64_t need = sah_sample_work_bytes(a);
+  if (a->work && ((uint64_t)a->work % 16 || a->work_bytes < need)) return sah_fail(SAH_ECAPACITY, "sah_sample_tokens: work is too small, or not on a multiple of 16 bytes");
+  const int slices = a->work && need ? sm_slices(a) : 1;
+  if (a->dtype == SAH_F32) return sm_launch<SAH_F32>(a, slices);
+  return a->dtype == SAH_BF16 ? sm_launch<SAH_BF16>(a, slices) : sm_launch<SAH_F16>(a, slices);
 }

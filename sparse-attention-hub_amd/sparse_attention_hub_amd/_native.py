@@ -513,6 +513,7 @@ class SampleArgs(C.Structure):
         ("tokens", C.c_void_p),
         ("logprobs", C.c_void_p),
         ("stream", C.c_void_p),
+        ("work", C.c_void_p), ("work_bytes", C.c_int64),
     ]
 
 
@@ -578,6 +579,8 @@ def lib() -> C.CDLL:
         getattr(handle, name).argtypes = [C.c_void_p]
     handle.sah_paged_attention_work_floats.restype = C.c_int64
     handle.sah_paged_attention_work_floats.argtypes = [C.c_void_p]
+    handle.sah_sample_work_bytes.restype = C.c_int64
+    handle.sah_sample_work_bytes.argtypes = [C.c_void_p]
     _lib = handle
     return handle
 
@@ -639,6 +642,10 @@ def members_work_floats(B: int, Hq: int, Hkv: int, Lq: int, Lk: int, head_dim: i
 
 def paged_work_floats(args: PagedAttentionArgs) -> int:
     return int(lib().sah_paged_attention_work_floats(C.addressof(args)))
+
+
+def sample_work_bytes(args: SampleArgs) -> int:
+    return int(lib().sah_sample_work_bytes(C.addressof(args)))
 
 
 def require_device(t: torch.Tensor, what: str) -> None:

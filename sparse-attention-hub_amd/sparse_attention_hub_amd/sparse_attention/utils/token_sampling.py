@@ -58,8 +58,13 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Set
     m_ptr, m = _setting(min_p, "min_p", 0.0, torch.float32, rows, device)
     tokens = torch.empty(rows, dtype=torch.int64, device=device)
     logprobs = torch.empty(rows, dtype=torch.float32, device=device)
-    N.call_on(device, "sah_sample_tokens", N.SampleArgs(
+    args = N.SampleArgs(
         logits.data_ptr(), max(logits.stride(0), vocab), N.dtype_code(logits.dtype), rows, vocab,
         uniforms.data_ptr(), int(uniforms.dtype == torch.float64), t_ptr, k_ptr, p_ptr, m_ptr, t, k, p, m,
-        tokens.data_ptr(), logprobs.data_ptr(), N.stream_ptr(device)))
+        tokens.data_ptr(), logprobs.data_ptr(), N.stream_ptr(device))
+    size = N.sample_work_bytes(args)
+    if size:
+        work = torch.empty(size, dtype=torch.uint8, device=device)
+        args.work, args.work_bytes = work.data_ptr(), size
+    N.call_on(device, "sah_sample_tokens", args)
     return tokens, logprobs

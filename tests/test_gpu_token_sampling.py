@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 
+from sparse_attention_hub_amd import _native as N
 from sparse_attention_hub_amd.sparse_attention.utils.token_sampling import sample_tokens
 
 pytestmark = pytest.mark.gpu
@@ -190,6 +191,25 @@ def test_the_same_numbers_give_the_same_tokens_in_a_replayed_graph(cuda):
         want = sample_tokens(x, u, **settings)
         torch.cuda.synchronize()
         assert torch.equal(tokens, want[0]) and torch.equal(logs, want[1])
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("rows, vocab", [(1, 8192), (1, 8193), (2, 33000), (3, 32768 + 2049), (64, 50001), (128, 9001), (129, 9001)])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=1000), dict(top_k=3, top_p=0.5), dict(top_p=0.9), dict(top_p=0.999, temperature=2.0), dict(min_p=0.1),
+                                      dict(top_k=5000)])
+def test_several_workgroups_a_row_or_one(cuda, dtype, rows, vocab, settings):
+    """The results of rows shared by several workgroups are those of one workgroup each, also where a part of the row is hidden."""
+    x, u = _logits(rows, vocab, dtype, 5)
+    x, u = x.to(cuda), u.to(cuda)
+    x[0, : vocab // 2] = -math.inf
+    x[rows // 2, 1000:] = -math.inf
+    tokens, logs = sample_tokens(x, u, **settings)
+    one, one_log = torch.empty_like(tokens), torch.empty_like(logs)
+    full = dict(dict(temperature=1.0, top_k=0, top_p=1.0, min_p=0.0), **settings)
+    args = N.SampleArgs(x.data_ptr(), vocab, N.dtype_code(dtype), rows, vocab, u.data_ptr(), int(u.dtype == torch.float64), None, None, None, None,
+                        full["temperature"], full["top_k"], full["top_p"], full["min_p"], one.data_ptr(), one_log.data_ptr(), N.stream_ptr(x.device))
+    N.call_on(x.device, "sah_sample_tokens", args)
+    assert torch.equal(tokens, one) and torch.equal(logs, one_log)
 
 
 def test_shares_are_those_of_the_distribution(cuda):

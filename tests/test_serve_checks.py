@@ -32,11 +32,11 @@ def _changed(args, changes):
 def test_every_declared_symbol_is_exported_and_bound():
     text = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "sah_serve.h")).read(), flags=re.S)
     declared = set(re.findall(r"\b(?:int|int64_t)\s+(sah_\w+)\s*\(", text))
-    assert declared == set(N.SERVE_SYMBOLS) | {"sah_paged_attention_work_floats"}
+    assert declared == set(N.SERVE_SYMBOLS) | {"sah_paged_attention_work_floats", "sah_sample_work_bytes"}
     lib = N.lib()
     for fn in N.SERVE_SYMBOLS:
         assert getattr(lib, fn)(None) == -2 and fn.encode() in lib.sah_last_error(), fn
-    assert lib.sah_paged_attention_work_floats(None) == 0
+    assert lib.sah_paged_attention_work_floats(None) == 0 and lib.sah_sample_work_bytes(None) == 0
 
 
 def test_argument_blocks_are_laid_out_as_in_the_header(tmp_path):
@@ -108,6 +108,7 @@ def test_attention_refuses(changes, code):
 @pytest.mark.parametrize("changes, code", [
     (dict(dtype=7), -5), (dict(n_rows=-1), -1), (dict(vocab=0), -1), (dict(vocab=2 ** 20 + 1, row_pitch=2 ** 21), -3), (dict(row_pitch=99), -1),
     (dict(logits=None), -2), (dict(uniforms=None), -2), (dict(tokens=None), -2),
+    (dict(vocab=10000, row_pitch=10000, work=_PTR, work_bytes=1000), -4), (dict(work=_PTR + 8), -4),
 ])
 def test_sampling_refuses(changes, code):
     args = N.SampleArgs(_PTR, 100, 0, 2, 100, _PTR, 0, None, None, None, None, 1.0, 0, 1.0, 0.0, _PTR, _PTR, None)
