@@ -24,9 +24,12 @@
 #define SM_RANK_K 1000     // top-k up to this goes by the threads' largest logits (1024 ln(1024 / 24) = 3800 tokens on average) ...
 #define SM_REST_P 3        // ... and top-p tries the tokens above all but these of them (6000)
 #define SM_LOWEST 0x00800000u  // order of the lowest finite logit
+// Few rows are shared by several workgroups each, up to 16, as long as there is a CU for each of them (two do not fit into its LDS) and
+// the row is long: 1 row of 32000, in two, 17 to 18 us instead of 13 (top-k), 31 either way (top-p); of 128000 in 16: 21 either way
+// (top-k), 47 instead of 82 (top-p), 22 instead of 40 (all tokens).
 #define SM_SPLIT_WGS 256
-#define SM_SLICE 4096
-#define SM_SLICES 16       // workgroups that share a row's passes, at most
+#define SM_SPLIT_VOCAB 65536
+#define SM_SLICES 16
 typedef sah_u4 sm_vec __attribute__((aligned(2)));
 
 struct sm_shared {
@@ -175,7 +178,7 @@ struct sm_item {
   uint32_t order;
   int index;
 };
-// Of items (order, index, weight) that `each` hands to its argument, from the largest order down, equal ones by index: the one at
+// Of items (order, index, a function that gives the weight) that `each` hands to its argument, from the largest order down, equal ones by index: the one at
 // which the running weight reaches target(all the weight) (> 0). Items outside [lo, hi] are passed over. `round` counts calls.
 template <typename TARGET, typename EACH>
 __device__ __forceinline__ sm_item sm_pick(sm_shared& S, int& round, uint32_t lo, uint32_t hi, TARGET target_of, EACH each) {
@@ -187,10 +190,10 @@ __device__ __forceinline__ sm_item sm_pick(sm_shared& S, int& round, uint32_t lo
     const uint32_t range = hi - lo;
     const int bits = range ? 32 - __builtin_clz(range) : 0, shift = bits > 11 ? bits - 11 : 0;
     auto inside = [&](auto f) __attribute__((always_inline)) {
-      each([&](uint32_t order, int index, uint64_t weight) {
+      each([&](uint32_t order, int index, auto weight) __attribute__((always_inline)) {
         if (ties && order != same) return;
         const uint32_t o = ties ? ~(uint32_t)index : order;
-        if (o >= lo && o <= hi) f(o, order, index, weight);
+        if (o >= lo && o <= hi) f(o, order, index, weight());
       });
     };
     const sm_bin bin = sm_locate(
@@ -276,6 +279,20 @@ struct sm_row {
     const float d = (best - v) * fine;
     return v == best ? 0 : d < SM_BINS - 1 ? (int)d : SM_BINS - 1;
   }
+  // orders that no token of the piece is below, or above (a hundredth of a piece is more than all roundings, and these are monotonic)
+  __device__ __forceinline__ uint32_t piece_low(int at) const {
+    const float v = best - ((float)at + 1.01f) / fine;
+    return at < SM_BINS - 1 && v > -INFINITY && v < best ? sm_order(v) : SM_LOWEST;
+  }
+  __device__ __forceinline__ uint32_t piece_high(int at) const {
+    const float v = best - ((float)at - 0.01f) / fine;
+    return at > 0 && v > -INFINITY && v < best ? sm_order(v) : sm_order(best);
+  }
+  // whole numbers before a token are less than p times the sum where they are less than that rounded up; the first is kept
+  __device__ __forceinline__ uint64_t nucleus(uint64_t all) const {
+    const double limit = ceil((double)p * (double)all);
+    return limit > 1.0 ? (uint64_t)limit : 1;
+  }
 };
 
 struct sm_top { float value, low; int at; };
@@ -359,8 +376,7 @@ struct sm_work {  // of a row
   float best[SM_SLICES];     // ... of the slices
   int best_at[SM_SLICES];
   sm_from from;
-  int count;
-  int pad;
+  int count, count_again;
 };
 
 template <int DT>
@@ -385,7 +401,7 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample_largest(sah_sample_args P) 
   sm_work& W = ((sm_work*)P.work)[blockIdx.y];
   const int bins = SM_BINS / (int)gridDim.x, shares = SM_NT / (int)gridDim.x;
   for (int b = threadIdx.x; b < bins; b += SM_NT) W.bins[blockIdx.x * bins + b] = 0;
-  if (blockIdx.x == 0 && threadIdx.x == 0) W.count = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) W.count = W.count_again = 0;
   float best = -INFINITY;
   int best_at = INT32_MAX;
   sm_each<DT, 4>((const char*)row.x + (int64_t)slice.begin * row.ES, slice.n, [&](float v, int i) {
@@ -451,6 +467,42 @@ __device__ __forceinline__ void sm_segments(const sm_row<DT>& row, int begin, in
   }
 }
 
+// The slice's list to the row's; where that cannot hold all slices', `count` says so. All threads call, behind a wait.
+__device__ __forceinline__ void sm_hand_over(sm_shared& S, sm_work& W, int& count) {
+  const int n = S.count;
+  if (threadIdx.x == 0) S.found_bin = atomicAdd(&count, n);
+  __syncthreads();
+  const int at = S.found_bin;
+  if (n > SM_CAP || at > SM_CAP - n) return;
+  for (int j = threadIdx.x; j < n; j += SM_NT) W.list[at + j] = S.list[j];
+}
+// ... and from there, all requested at once; more than SM_CAP: nothing
+__device__ __forceinline__ void sm_take_list(sm_shared& S, const sm_work& W, int n) {
+  constexpr int N = SM_CAP / (2 * SM_NT);
+  if (n > SM_CAP) return;
+  sah_u4 two[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = 2 * ((int)threadIdx.x + i * SM_NT);
+    if (j < n) two[i] = *(const sah_u4*)&W.list[j];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int j = 2 * ((int)threadIdx.x + i * SM_NT);
+    if (j < n) *(sah_u4*)&S.list[j] = two[i];
+  }
+}
+// top-p's last token: the weight that it reaches, and its piece. (The bins are LDS's own again afterwards.)
+template <int DT>
+__device__ __forceinline__ sm_bin sm_border(sm_shared& S, const sm_row<DT>& row, const sm_work& W, uint64_t& whole) {
+  return sm_locate(S, [&](uint64_t all) { return whole = row.nucleus(all); },
+                   [&](auto) { *(sah_u4*)&S.bins[2 * threadIdx.x] = *(const sah_u4*)&W.bins[2 * threadIdx.x]; });
+}
+template <int DT>
+__device__ __forceinline__ bool sm_too_short(const sm_row<DT>& row, const sm_from& from, const sm_bin& border) {
+  return from.value > -INFINITY && !from.complete && row.piece(from.value) <= border.at;
+}
+
 // Every slice's tokens for the list, and the weights of its pieces or segments
 template <int DT>
 __global__ __launch_bounds__(SM_NT, 4) void k_sample_slices(sah_sample_args P) {
@@ -483,15 +535,33 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample_slices(sah_sample_args P) {
     sm_each<DT, 4>(x, slice.n, enlist);
   }
   __syncthreads();
-  const int n = S.count;
-  if (threadIdx.x == 0) S.found_bin = atomicAdd(&W.count, n);
   if (row.total())
     for (int b = threadIdx.x; b < SM_BINS; b += SM_NT)
       if (S.bins[b]) atomicAdd((unsigned long long*)&W.bins[b], (unsigned long long)S.bins[b]);
+  sm_hand_over(S, W, W.count);
+}
+
+// Rows whose top-p reaches further down than their list: the list anew, all down to there
+template <int DT>
+__global__ __launch_bounds__(SM_NT, 4) void k_sample_list(sah_sample_args P) {
+  SAH_DYNAMIC_LDS(s_dyn);
+  sm_shared& S = *(sm_shared*)s_dyn;
+  sm_row<DT> row(P, blockIdx.y);
+  if (!row.total()) return;
+  sm_work& W = ((sm_work*)P.work)[blockIdx.y];
+  sm_largest_of(row, W, gridDim.x);
+  if (row.one_answer()) return;
+  uint64_t whole;
+  const sm_bin border = sm_border(S, row, W, whole);
+  if (!sm_too_short(row, W.from, border)) return;
+  if (threadIdx.x == 0) S.count = 0;
   __syncthreads();
-  const int at = S.found_bin;
-  if (n > SM_CAP || at > SM_CAP - n) return;  // too many: the count says so
-  for (int j = threadIdx.x; j < n; j += SM_NT) W.list[at + j] = S.list[j];
+  const sm_slice<DT> slice(row.V, blockIdx.x, gridDim.x);
+  sm_each<DT, 4>((const char*)row.x + (int64_t)slice.begin * row.ES, slice.n, [&](float v, int i) __attribute__((always_inline)) {
+    if (v > -INFINITY && row.piece(v) <= border.at) sm_enlist(S, v, i + slice.begin);
+  });
+  __syncthreads();
+  sm_hand_over(S, W, W.count_again);
 }
 
 // SPLIT: by `slices` workgroups' work so far
@@ -505,7 +575,7 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P, int slic
   sm_row<DT> row(P, r);
   const int V = row.V, k = row.k;
   const void* x = row.x;
-  const float p = row.p, least = row.least;
+  const float least = row.least;
   const bool use_k = row.use_k, use_p = row.use_p, use_m = row.use_m;
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
   [[maybe_unused]] const sm_work& W = ((const sm_work*)P.work)[SPLIT ? r : 0];
@@ -527,7 +597,7 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P, int slic
     low = top.low;
     row.largest(top.value, top.at);
   }
-  const float best = row.best, fine = row.fine;
+  const float best = row.best;
   if (row.one_answer()) {
     if (threadIdx.x == 0) {
       P.tokens[r] = best == -INFINITY ? -1 : row.best_at;
@@ -538,11 +608,7 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P, int slic
   const sm_weights weigh(best, row.temp);
   const uint32_t top = sm_order(best);
   auto piece = [&](float v) { return row.piece(v); };
-  // whole numbers before a token are less than p times the sum where they are less than that rounded up; the first is kept
-  auto nucleus = [&](uint64_t all) -> uint64_t {
-    const double limit = ceil((double)p * (double)all);
-    return limit > 1.0 ? (uint64_t)limit : 1;
-  };
+  auto nucleus = [&](uint64_t all) { return row.nucleus(all); };
   // kept: logits above thr, and of those equal to it the ones with an index up to last
   float thr = -INFINITY;
   int last = -1;
@@ -568,34 +634,35 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P, int slic
     if constexpr (SPLIT) {
       from = W.from;
       n_list = W.count;
-      if (n_list <= SM_CAP)
-        for (int j = threadIdx.x; j < n_list; j += SM_NT) S.list[j] = W.list[j];
+      if (!total) sm_take_list(S, W, n_list);
     } else {
       from = sm_list_from<DT>(S, row, own, low);
     }
     if (from.value > -INFINITY && from.value < best) lowest = sm_order(from.value);
     if (total) {
       // the weights' pass shares the row out into pieces too: if top-p's last token lies below the list, its piece is known
-      border = sm_locate(
-          S, [&](uint64_t all) { return whole = nucleus(all); },
-          [&](auto put) __attribute__((always_inline)) {
-            if constexpr (SPLIT) {
-              const sah_u4 two = *(const sah_u4*)&W.bins[2 * threadIdx.x];
-              *(sah_u4*)&S.bins[2 * threadIdx.x] = two;
-            } else {
+      if constexpr (SPLIT) {
+        border = sm_border(S, row, W, whole);
+      } else {
+        border = sm_locate(
+            S, [&](uint64_t all) { return whole = nucleus(all); },
+            [&](auto put) __attribute__((always_inline)) {
               sm_each<DT, 1>(x, V, [&](float v, int i) {
                 if (v >= from.value && v > -INFINITY) sm_enlist(S, v, i);
                 put(piece(v), sm_fixed(weigh(v)));
               });
-            }
-          });
-      if constexpr (!SPLIT) n_list = S.count;
-      if (from.value > -INFINITY && !from.complete && piece(from.value) <= border.at) {
-        // further down than the list: all down to there, if it holds that
-        const float down = best - (border.at + 1.01f) / fine;
-        lowest = border.at < SM_BINS - 1 && down > -INFINITY && down < best ? sm_order(down) : SM_LOWEST;
-        list_again([&](float v) { return piece(v) <= border.at; });
+            });
+        n_list = S.count;
       }
+      if (sm_too_short(row, from, border)) {
+        // all down to there, if the list holds that
+        if constexpr (SPLIT) {
+          n_list = W.count_again;
+        } else {
+          list_again([&](float v) { return piece(v) <= border.at; });
+        }
+      }
+      if constexpr (SPLIT) sm_take_list(S, W, n_list);
     } else if constexpr (!SPLIT) {
       sm_each<DT, 4>(x, V, [&](float v, int i) { if (v >= from.value && v > -INFINITY) sm_enlist(S, v, i); });
       __syncthreads();
@@ -617,15 +684,18 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P, int slic
   for (int stage = 0; stage < 2; ++stage) {  // top-k, then top-p
     if (stage ? !use_p : !use_k) continue;
     auto weight = [&](float v) -> uint64_t { return stage ? sm_fixed(weigh(v)) : 1; };
-    auto target_of = [&](uint64_t all) -> uint64_t { return !stage ? k : total ? whole : nucleus(all); };
+    auto target_of = [&](uint64_t all) -> uint64_t { return !stage ? k : total ? whole - border.before : nucleus(all); };
     auto items = [&](bool from_list) {
       return [&, from_list](auto put) __attribute__((always_inline)) {
-        each(from_list, [&](float v, int i) { if (kept(v, i)) put(sm_order(v), i, weight(v)); });
+        // (top-p's last token lies in the border's piece)
+        each(from_list, [&](float v, int i) __attribute__((always_inline)) {
+          if (kept(v, i) && (!total || piece(v) == border.at)) put(sm_order(v), i, [&] { return weight(v); });
+        });
       };
     };
     sm_item found{false, 0, 0};
     if (list) {
-      found = sm_pick(S, round, lowest, top, target_of, items(true));
+      found = sm_pick(S, round, total ? row.piece_low(border.at) : lowest, total ? row.piece_high(border.at) : top, target_of, items(true));
     } else {
       uint64_t target = whole;
       sm_bin b = border;
@@ -636,10 +706,10 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P, int slic
       if (b.at < 0) continue;
       auto rest = [&](uint64_t) { return target - b.before; };
       if (list_again([&](float v) { return piece(v) == b.at; })) {
-        found = sm_pick(S, round, SM_LOWEST, top, rest, items(true));
+        found = sm_pick(S, round, row.piece_low(b.at), row.piece_high(b.at), rest, items(true));
       } else {  // (thousands of logits in one piece)
-        found = sm_pick(S, round, SM_LOWEST, top, rest, [&](auto put) __attribute__((always_inline)) {
-          each(false, [&](float v, int i) { if (kept(v, i) && piece(v) == b.at) put(sm_order(v), i, weight(v)); });
+        found = sm_pick(S, round, row.piece_low(b.at), row.piece_high(b.at), rest, [&](auto put) __attribute__((always_inline)) {
+          each(false, [&](float v, int i) { if (kept(v, i) && piece(v) == b.at) put(sm_order(v), i, [&] { return weight(v); }); });
         });
       }
     }
@@ -667,7 +737,7 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P, int slic
     uint64_t all = 0;
     const sm_item f = sm_pick(
         S, round, ~(uint32_t)(V - 1), ~0u, [&](uint64_t a) { all = a; return drawn(a); },
-        [&](auto put) __attribute__((always_inline)) { each(true, [&](float v, int i) { put(~(uint32_t)i, i, final_weight(v, i)); }); });
+        [&](auto put) __attribute__((always_inline)) { each(true, [&](float v, int i) { put(~(uint32_t)i, i, [&] { return final_weight(v, i); }); }); });
     if (threadIdx.x == 0) answer(f.index, all);
     return;
   }
@@ -720,11 +790,11 @@ __global__ __launch_bounds__(SM_NT, 4) void k_sample(sah_sample_args P, int slic
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-// Workgroups a row: as many as fill the card, each with SM_SLICE tokens or more (a power of two).
+// Workgroups a row (a power of two)
 static int sm_slices(const sah_sample_args* a) {
-  if (a->n_rows <= 0 || (!a->temperatures && !(a->temperature > 0.f))) return 1;  // (one pass is all that is done)
+  if (a->n_rows <= 0 || a->vocab < SM_SPLIT_VOCAB || (!a->temperatures && !(a->temperature > 0.f))) return 1;  // (one pass is all that is done)
   int n = 1;
-  while (n < SM_SLICES && 2 * n * (int64_t)a->n_rows <= SM_SPLIT_WGS && a->vocab / (2 * n) >= SM_SLICE) n *= 2;
+  while (n < SM_SLICES && 2 * n * (int64_t)a->n_rows <= SM_SPLIT_WGS) n *= 2;
   return n;
 }
 extern "C" int64_t sah_sample_work_bytes(const sah_sample_args* a) {
@@ -744,9 +814,17 @@ static int sm_launch(const sah_sample_args* a, int slices) {
       hipLaunchKernelGGL(k_sample_largest<DT>, dim3(slices, a->n_rows), dim3(SM_NT), sizeof(sm_shared), st, *a);
       if (int rc = sah_launch_status("sah_sample_tokens(largest)")) return rc;
     }
-    sah_timed timed("k_sample_slices", a->stream);
-    hipLaunchKernelGGL(k_sample_slices<DT>, dim3(slices, a->n_rows), dim3(SM_NT), sizeof(sm_shared), st, *a);
-    if (int rc = sah_launch_status("sah_sample_tokens(slices)")) return rc;
+    {
+      sah_timed timed("k_sample_slices", a->stream);
+      hipLaunchKernelGGL(k_sample_slices<DT>, dim3(slices, a->n_rows), dim3(SM_NT), sizeof(sm_shared), st, *a);
+      if (int rc = sah_launch_status("sah_sample_tokens(slices)")) return rc;
+    }
+    if ((a->top_ps || a->top_p < 1.f) && (a->top_ks || a->top_k <= 0 || a->top_k >= a->vocab)) {  // (some row may go by all its weights)
+      if (int rc = sah_allow_lds((const void*)k_sample_list<DT>, sizeof(sm_shared), "sah_sample_tokens")) return rc;
+      sah_timed timed("k_sample_list", a->stream);
+      hipLaunchKernelGGL(k_sample_list<DT>, dim3(slices, a->n_rows), dim3(SM_NT), sizeof(sm_shared), st, *a);
+      if (int rc = sah_launch_status("sah_sample_tokens(list)")) return rc;
+    }
   }
   sah_timed timed("k_sample", a->stream);
   hipLaunchKernelGGL(kernel, dim3(a->n_rows), dim3(SM_NT), sizeof(sm_shared), st, *a, slices);

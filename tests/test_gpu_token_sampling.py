@@ -194,7 +194,7 @@ def test_the_same_numbers_give_the_same_tokens_in_a_replayed_graph(cuda):
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
-@pytest.mark.parametrize("rows, vocab", [(1, 8192), (1, 8193), (2, 33000), (3, 32768 + 2049), (64, 50001), (128, 9001), (129, 9001)])
+@pytest.mark.parametrize("rows, vocab", [(1, 65535), (1, 65536), (2, 65537), (3, 65536 + 2049), (17, 70001), (64, 100001), (128, 66001), (129, 66001)])
 @pytest.mark.parametrize("settings", [dict(), dict(top_k=1000), dict(top_k=3, top_p=0.5), dict(top_p=0.9), dict(top_p=0.999, temperature=2.0), dict(min_p=0.1),
                                       dict(top_k=5000)])
 def test_several_workgroups_a_row_or_one(cuda, dtype, rows, vocab, settings):

@@ -108,7 +108,7 @@ def test_attention_refuses(changes, code):
 @pytest.mark.parametrize("changes, code", [
     (dict(dtype=7), -5), (dict(n_rows=-1), -1), (dict(vocab=0), -1), (dict(vocab=2 ** 20 + 1, row_pitch=2 ** 21), -3), (dict(row_pitch=99), -1),
     (dict(logits=None), -2), (dict(uniforms=None), -2), (dict(tokens=None), -2),
-    (dict(vocab=10000, row_pitch=10000, work=_PTR, work_bytes=1000), -4), (dict(work=_PTR + 8), -4),
+    (dict(vocab=100000, row_pitch=100000, work=_PTR, work_bytes=1000), -4), (dict(work=_PTR + 8), -4),
 ])
 def test_sampling_refuses(changes, code):
     args = N.SampleArgs(_PTR, 100, 0, 2, 100, _PTR, 0, None, None, None, None, 1.0, 0, 1.0, 0.0, _PTR, _PTR, None)
