@@ -59,6 +59,23 @@ static inline int sah_launch_status(const char* what) {
 // once per (kernel, device). Thread-safe; remembers what has been done (defined with the row builders).
 int sah_allow_lds(const void* kernel, size_t bytes, const char* what);
 
+// Whether no two rows of `inner` contiguous elements share memory, judged by strides (elements) and counts.
+template <int N>
+static inline bool sah_rows_apart(int64_t inner, const int64_t (&stride)[N], const int64_t (&count)[N]) {
+  int64_t end = inner;  // of what the dimensions so far, from the smallest stride up, take
+  bool done[N] = {};
+  for (int i = 0; i < N; ++i) {
+    int next = -1;
+    for (int j = 0; j < N; ++j)
+      if (!done[j] && (next < 0 || stride[j] < stride[next])) next = j;
+    done[next] = true;
+    if (count[next] <= 1) continue;
+    if (stride[next] < end) return false;
+    end += stride[next] * (count[next] - 1);
+  }
+  return true;
+}
+
 static inline int sah_check_rows(const sah_rows& r, const char* what, bool need_cols = true) {
   if (r.n_rows <= 0 || r.n_keys <= 0) return sah_fail(SAH_EINVAL, "%s: rows.n_rows/n_keys must be > 0", what);
   if (r.n_words != (r.n_keys + 31) / 32) return sah_fail(SAH_EINVAL, "%s: rows.n_words != ceil(n_keys/32)", what);

@@ -199,6 +199,7 @@ extern "C" int sah_paged_assign(const sah_paged_assign_args* a) {
   if (a->n_requests <= 0 || a->page_size <= 0 || a->table_width <= 0 || a->n_pages <= 0 || a->n_tokens < 0)
     return sah_fail(SAH_EINVAL, "sah_paged_assign: n_requests, page_size, table_width and n_pages must be > 0, n_tokens >= 0");
   if (a->n_requests > PG_MAX_REQ) return sah_fail(SAH_ESHAPE, "sah_paged_assign: %d requests; at most %d", a->n_requests, PG_MAX_REQ);
+  if (a->n_tokens > 1 << 30) return sah_fail(SAH_ESHAPE, "sah_paged_assign: %d tokens; at most 2^30", a->n_tokens);
   if (a->table_pitch < a->table_width) return sah_fail(SAH_EINVAL, "sah_paged_assign: table_pitch is less than table_width");
   if (!a->new_lens || !a->lens || !a->block_table || !a->free_pages || !a->free_count || !a->cu_new || !a->kv_lens || !a->granted ||
       !a->lens_out || !a->free_count_out || !a->work || (a->n_tokens && (!a->slot_map || !a->positions)))
@@ -248,6 +249,9 @@ extern "C" int sah_paged_store(const sah_paged_store_args* a) {
     return sah_fail(SAH_EINVAL, "sah_paged_store: Hkv, D, n_pages and page_size must be > 0, n_tokens >= 0");
   if (a->n_tokens == 0) return SAH_OK;
   if (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->slot_map) return sah_fail(SAH_ENULL, "sah_paged_store: NULL pointer");
+  if (!sah_rows_apart<3>(a->D, {a->kcs_p, a->kcs_t, a->kcs_h}, {a->n_pages, a->page_size, a->Hkv}) ||
+      !sah_rows_apart<3>(a->D, {a->vcs_p, a->vcs_t, a->vcs_h}, {a->n_pages, a->page_size, a->Hkv}))
+    return sah_fail(SAH_EINVAL, "sah_paged_store: rows of a cache overlap");
   const int es = a->dtype == SAH_F32 ? 4 : 2;
   // 16 bytes at a time where every address allows it, else an element
   const uint64_t all = (uint64_t)a->k | (uint64_t)a->v | (uint64_t)a->k_cache | (uint64_t)a->v_cache |

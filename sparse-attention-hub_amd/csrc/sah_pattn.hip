@@ -1097,7 +1097,8 @@ extern "C" int sah_paged_attention(const sah_paged_attention_args* a) {
                     "sink %d, window %d)", a->n_requests, a->n_tokens, a->Hq, a->Hkv, a->n_pages, a->table_width, a->max_context, a->sink, a->window);
   if (a->D <= 0 || a->D % 8 || a->D > PA_MAX_D) return sah_fail(SAH_ESHAPE, "sah_paged_attention: head_dim %d is not a multiple of 8 up to 256", a->D);
   if (a->page_size <= 0 || (a->page_size & (a->page_size - 1))) return sah_fail(SAH_ESHAPE, "sah_paged_attention: page_size %d is not a power of two", a->page_size);
-  if ((int64_t)a->table_width * a->page_size > INT32_MAX) return sah_fail(SAH_ESHAPE, "sah_paged_attention: table_width * page_size passes 2^31");
+  if ((int64_t)a->table_width * a->page_size > INT32_MAX - 4096)  // (a stage's keys reach beyond the last one)
+    return sah_fail(SAH_ESHAPE, "sah_paged_attention: table_width * page_size passes 2^31 - 4097");
   if ((int64_t)a->n_tokens * a->Hq > 1 << 30) return sah_fail(SAH_ESHAPE, "sah_paged_attention: n_tokens * Hq passes 2^30");
   // the line of work is divided in doubles, also where running sums overlap
   if (((double)a->n_tokens * (a->Hq / a->Hkv) / 32 + 1) * ((double)a->table_width * a->page_size + 1024) * a->Hkv * a->n_requests > 0x1p52)
@@ -1111,6 +1112,7 @@ extern "C" int sah_paged_attention(const sah_paged_attention_args* a) {
     return sah_fail(SAH_EINVAL, "sah_paged_attention: addresses and strides must be multiples of 16 bytes");
   if (a->ks_t < 0 || a->vs_t < 0 || a->ks_t >= 1 << 26 || a->vs_t >= 1 << 26)  // a few tokens of a page: 32-bit offsets
     return sah_fail(SAH_ESHAPE, "sah_paged_attention: a page's tokens are 2^26 elements or more apart");
+  if (!sah_rows_apart<2>(a->D, {a->os_t, a->os_h}, {a->n_tokens, a->Hq})) return sah_fail(SAH_EINVAL, "sah_paged_attention: rows of out overlap");
   if (!(a->scaling - a->scaling == 0.f)) return sah_fail(SAH_EINVAL, "sah_paged_attention: scaling is not finite");
   if (!a->work || a->work_floats < sah_paged_attention_work_floats(a)) return sah_fail(SAH_ECAPACITY, "sah_paged_attention: work is too small");
   return (int)pa_dispatch(a, pa_launch_fn{a});

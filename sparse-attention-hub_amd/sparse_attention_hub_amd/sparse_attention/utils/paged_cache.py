@@ -31,18 +31,20 @@ class PageAssignment(NamedTuple):
     granted: torch.Tensor     # bool [n_requests]
 
 
-def _check(t: torch.Tensor, what: str, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    """A contiguous tensor of this type and shape on this device (a shape's None: any size)."""
+def _check(t: torch.Tensor, what: str, dtype: torch.dtype, size: Optional[int], device: torch.device) -> None:
+    """A contiguous tensor of one dimension, of this type and size (None: any) on this device."""
+    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.dim() == 1 and t.device == device and t.is_contiguous() \
+            and (size is None or t.shape[0] == size):
+        return  # (one line for the call that is as it should be: a step makes a dozen of them)
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a tensor, got {type(t).__name__}")
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, expected {device}")
     if t.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise ValueError(f"{what} must have shape {shape}, got {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
+    if t.dim() != 1 or size is not None and t.shape[0] != size:
+        raise ValueError(f"{what} must have shape ({'n' if size is None else size},), got {tuple(t.shape)}")
+    raise ValueError(f"{what} must be contiguous")
 
 
 def _check_table(block_table: torch.Tensor, n_requests: int, device: torch.device) -> None:
@@ -85,21 +87,21 @@ def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, block_table: torch.
     device, n = new_lens.device, new_lens.shape[0] if new_lens.dim() == 1 else -1
     lens_out = lens if lens_out is None else lens_out
     free_count_out = free_count if free_count_out is None else free_count_out
-    _check(new_lens, "new_lens", torch.int32, (None,), device)
+    _check(new_lens, "new_lens", torch.int32, None, device)
     if n == 0:
         raise ValueError("assign_pages needs at least one request")
-    _check(lens, "lens", torch.int32, (n,), device)
-    _check(lens_out, "lens_out", torch.int32, (n,), device)
-    _check(free_pages, "free_pages", torch.int32, (None,), device)
-    _check(free_count, "free_count", torch.int32, (1,), device)
-    _check(free_count_out, "free_count_out", torch.int32, (1,), device)
+    _check(lens, "lens", torch.int32, n, device)
+    _check(lens_out, "lens_out", torch.int32, n, device)
+    _check(free_pages, "free_pages", torch.int32, None, device)
+    _check(free_count, "free_count", torch.int32, 1, device)
+    _check(free_count_out, "free_count_out", torch.int32, 1, device)
     _check_table(block_table, n, device)
-    if not 0 <= n_tokens < 2 ** 31:
-        raise ValueError(f"n_tokens must be in [0, 2^31), got {n_tokens}")
+    if not 0 <= n_tokens <= 2 ** 30:
+        raise ValueError(f"n_tokens must be in [0, 2^30], got {n_tokens}")
     slot_map = torch.empty(n_tokens, dtype=torch.int64, device=device)
     # one allocation for the int32 outputs and the kernels' records
-    words = torch.empty(n_tokens + 4 * n + 2, dtype=torch.int32, device=device)
-    work, cu_new, kv_lens, positions = words[:2 * n], words[2 * n:3 * n + 1], words[3 * n + 1:4 * n + 1], words[4 * n + 1:4 * n + 1 + n_tokens]
+    words = torch.empty(n_tokens + 4 * n + 1, dtype=torch.int32, device=device)
+    work, cu_new, kv_lens, positions = words.split_with_sizes((2 * n, n + 1, n, n_tokens))
     granted = torch.empty(n, dtype=torch.bool, device=device)
     N.call_on(device, "sah_paged_assign", N.PagedAssignArgs(
         new_lens.data_ptr(), lens.data_ptr(), block_table.data_ptr(), _pitch(block_table), block_table.shape[1],
@@ -115,12 +117,12 @@ def release_pages(finished: torch.Tensor, lens: torch.Tensor, block_table: torch
     and its row can serve another request."""
     N.require_device(finished, "finished")
     device, n = finished.device, finished.shape[0] if finished.dim() == 1 else -1
-    _check(finished, "finished", torch.bool, (None,), device)
+    _check(finished, "finished", torch.bool, None, device)
     if n == 0:
         raise ValueError("release_pages needs at least one request")
-    _check(lens, "lens", torch.int32, (n,), device)
-    _check(free_pages, "free_pages", torch.int32, (None,), device)
-    _check(free_count, "free_count", torch.int32, (1,), device)
+    _check(lens, "lens", torch.int32, n, device)
+    _check(free_pages, "free_pages", torch.int32, None, device)
+    _check(free_count, "free_count", torch.int32, 1, device)
     _check_table(block_table, n, device)
     work = torch.empty(2 * n, dtype=torch.int32, device=device)
     N.call_on(device, "sah_paged_release", N.PagedReleaseArgs(
@@ -136,18 +138,19 @@ def store_paged(keys: torch.Tensor, values: torch.Tensor, key_cache: torch.Tenso
     _check_cache(key_cache, value_cache)
     device = key_cache.device
     pages, page_size, heads, dim = key_cache.shape
+    rows, dtype = (keys.shape[0] if keys.dim() else 0, heads, dim), key_cache.dtype
     for t, what in ((keys, "keys"), (values, "values")):
-        if t.device != device or t.dtype != key_cache.dtype:
-            raise ValueError(f"{what} must be {key_cache.dtype} on {device}, got {t.dtype} on {t.device}")
-        if t.dim() != 3 or t.shape[1:] != (heads, dim) or t.shape[0] != keys.shape[0]:
+        if t.device != device or t.dtype != dtype:
+            raise ValueError(f"{what} must be {dtype} on {device}, got {t.dtype} on {t.device}")
+        if t.shape != rows:
             raise ValueError(f"{what} must have shape (n_tokens, {heads}, {dim}), got {tuple(t.shape)}")
         if t.stride(2) != 1:
             raise ValueError(f"{what}: the innermost stride must be 1")
-    _check(slot_map, "slot_map", torch.int64, (keys.shape[0],), device)
+    _check(slot_map, "slot_map", torch.int64, rows[0], device)
     N.call_on(device, "sah_paged_store", N.PagedStoreArgs(
         keys.data_ptr(), keys.stride(0), keys.stride(1), values.data_ptr(), values.stride(0), values.stride(1),
         key_cache.data_ptr(), *key_cache.stride()[:3], value_cache.data_ptr(), *value_cache.stride()[:3],
-        slot_map.data_ptr(), N.dtype_code(key_cache.dtype), keys.shape[0], heads, dim, pages, page_size, N.stream_ptr(device)))
+        slot_map.data_ptr(), N.dtype_code(dtype), rows[0], heads, dim, pages, page_size, N.stream_ptr(device)))
 
 
 def paged_attention(queries: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_table: torch.Tensor,
@@ -162,7 +165,7 @@ def paged_attention(queries: torch.Tensor, key_cache: torch.Tensor, value_cache:
     groups, as `repeat_kv` would have it. A row that sees nothing is 0; rows behind the last request's keep what `out` held (without
     `out`: unspecified). `max_context`, about the longest request's length, decides how work is split (default: the
     table's width); results do not depend on it beyond the order of sums. head_dim a multiple of 8 up to 256, page_size a power of two,
-    addresses and strides multiples of 16 bytes. Returns `(n_tokens, heads, head_dim)`.
+    addresses and strides multiples of 16 bytes; `out` shares no memory with the other tensors. Returns `(n_tokens, heads, head_dim)`.
     """
     _check_cache(key_cache, value_cache)
     device = key_cache.device
@@ -172,12 +175,12 @@ def paged_attention(queries: torch.Tensor, key_cache: torch.Tensor, value_cache:
     if queries.dim() != 3 or queries.shape[2] != dim or queries.stride(2) != 1:
         raise ValueError(f"queries must be (n_tokens, heads, {dim}) with innermost stride 1, got {tuple(queries.shape)}")
     tokens, heads = queries.shape[0], queries.shape[1]
-    _check(kv_lens, "kv_lens", torch.int32, (None,), device)
+    _check(kv_lens, "kv_lens", torch.int32, None, device)
     n = kv_lens.shape[0]
-    _check(cu_new, "cu_new", torch.int32, (n + 1,), device)
+    _check(cu_new, "cu_new", torch.int32, n + 1, device)
     _check_table(block_table, n, device)
     if sinks is not None:
-        _check(sinks, "sinks", torch.float32, (heads,), device)
+        _check(sinks, "sinks", torch.float32, heads, device)
     if sink_size < 0 or window_size < 0:
         raise ValueError(f"sink_size and window_size must not be negative, got {sink_size} and {window_size}")
     if sink_size and not window_size:

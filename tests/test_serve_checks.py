@@ -65,6 +65,7 @@ def test_argument_blocks_are_laid_out_as_in_the_header(tmp_path):
     (dict(n_requests=4097), -3), (dict(table_pitch=3), -1), (dict(new_lens=None), -2), (dict(lens=None), -2), (dict(block_table=None), -2),
     (dict(free_pages=None), -2), (dict(free_count=None), -2), (dict(slot_map=None), -2), (dict(positions=None), -2), (dict(cu_new=None), -2),
     (dict(kv_lens=None), -2), (dict(granted=None), -2), (dict(lens_out=None), -2), (dict(free_count_out=None), -2), (dict(work=None), -2),
+    (dict(n_tokens=2 ** 30 + 1), -3),
 ])
 def test_assign_refuses(changes, code):
     args = N.PagedAssignArgs(_PTR, _PTR, _PTR, 4, 4, _PTR, _PTR, 8, 2, 16, 5, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, _PTR, None)
@@ -84,7 +85,8 @@ def test_release_refuses(changes, code):
 @pytest.mark.parametrize("changes, code", [
     (dict(dtype=3), -5), (dict(n_tokens=-1), -1), (dict(Hkv=0), -1), (dict(D=0), -1), (dict(n_pages=0), -1), (dict(page_size=0), -1),
     (dict(k=None), -2), (dict(v=None), -2), (dict(k_cache=None), -2), (dict(v_cache=None), -2), (dict(slot_map=None), -2),
-    (dict(n_tokens=2 ** 31 - 1, Hkv=2 ** 12), -3),
+    (dict(n_tokens=2 ** 31 - 1, Hkv=2 ** 12, kcs_t=2 ** 17, kcs_p=2 ** 21, vcs_t=2 ** 17, vcs_p=2 ** 21), -3),
+    (dict(kcs_p=0), -1), (dict(vcs_t=63), -1), (dict(vcs_h=31), -1), (dict(kcs_p=-1024), -1),
 ])
 def test_store_refuses(changes, code):
     args = N.PagedStoreArgs(_PTR, 64, 32, _PTR, 64, 32, _PTR, 1024, 64, 32, _PTR, 1024, 64, 32, _PTR, 1, 3, 2, 32, 4, 16, None)
@@ -98,6 +100,7 @@ def test_store_refuses(changes, code):
     (dict(table_pitch=3), -1), (dict(q=None), -2), (dict(k=None), -2), (dict(v=None), -2), (dict(block_table=None), -2),
     (dict(kv_lens=None), -2), (dict(cu_new=None), -2), (dict(out=None), -2), (dict(q=_PTR + 2), -1), (dict(k=_PTR + 8), -1), (dict(ks_t=129), -1),
     (dict(qs_h=65), -1), (dict(ks_t=2 ** 26), -3), (dict(vs_t=-64), -3), (dict(os_t=257), -1), (dict(scaling=float("nan")), -1),
+    (dict(os_t=0), -1), (dict(os_h=0), -1), (dict(os_h=-64), -1), (dict(table_width=2 ** 27 - 255, table_pitch=2 ** 27), -3),
 ])
 def test_attention_refuses(changes, code):
     args = N.PagedAttentionArgs(_PTR, 256, 64, _PTR, 2048, 128, 64, _PTR, 2048, 128, 64, _PTR, 4, 4, _PTR, _PTR, None, 1, 2, 3, 4, 2, 64, 8, 16,
