@@ -43,6 +43,10 @@ struct pa_shape {
   // the least that is worth a workgroup (512: 5 fp32 requests of 2000 keys 43 us instead of 34; 128: no case gains, small ones lose 1).
   static constexpr int TILE_COST = 128;
   static constexpr int LEAST = 256;
+  // A tile of this many keys or fewer is not split where a workgroup's piece is no more: its joining costs more than the longer work (16
+  // requests under Sink + Local, 700 keys a tile: 36 -> 30 us, 2048 the same; 8 of one token and 200 keys: 18 -> 12). fp32, 16 times
+  // the matrix time a key: 5 requests of 2000 keys 35 us, 38 with 256 or 384.
+  static constexpr int WHOLE = DT == SAH_F32 ? 0 : WIDE ? 1024 : 512;
 };
 
 // The kernel's arguments where they lie. Each call gives an address that the compiler knows nothing of, so that what is read behind it is
@@ -157,11 +161,31 @@ __device__ __forceinline__ int64_t pa_bound(int64_t total, int n, int w) {
   return each * w + pa_uniform(pa_div((total - each * n) * w, n));
 }
 
+// the next tile on the line; there is one
+template <typename S>
+__device__ __forceinline__ void pa_next(pa_args& P, pa_place& at) {
+  at.begin += at.cost;
+  if (++at.tile == at.costs.tiles) {
+    at.tile = 0;
+    if (++at.hk == P.Hkv) {
+      at.hk = 0;
+      do {
+        ++at.b;
+        at.req = pa_read_request(P, at.b);
+        at.costs = pa_cost_of<S>(P, at.req);
+      } while (at.costs.tiles == 0);
+    }
+  }
+  at.cost = pa_uniform(at.costs.of(at.tile));
+}
+
 // Workgroup w's piece of the line, [x0, x1), and the place that holds x0
 struct pa_piece {
   int64_t total, x0, x1;
   int sharers;   // workgroups that have a piece; without one x0 and x1 say nothing
+  int whole;     // tiles of at most this cost are one workgroup's, the one whose piece they begin in: x0 lies behind another's
   pa_place at;
+  __device__ __forceinline__ bool none(int w) const { return w >= sharers || x0 >= x1; }
 };
 // s_sum: NT / 64 + 2 words. All NT threads call.
 template <int NT, typename S>
@@ -232,27 +256,14 @@ __device__ __forceinline__ pa_piece pa_start(pa_args& P, int w, int64_t* s_sum) 
   at.tile = __builtin_amdgcn_readfirstlane(at.costs.at(r.x0 - begin - at.hk * head));
   at.begin = pa_uniform(begin + at.hk * head + at.costs.before(at.tile));
   at.cost = pa_uniform(at.costs.of(at.tile));
+  r.whole = r.total <= (int64_t)S::WHOLE * r.sharers ? S::WHOLE : 0;
+  if (r.x0 > at.begin && at.cost <= r.whole) {
+    r.x0 = at.begin + at.cost;
+    if (r.x0 < r.x1) pa_next<S>(P, at);
+  }
   return r;
 }
-// the next tile on the line; there is one
-template <typename S>
-__device__ __forceinline__ void pa_next(pa_args& P, pa_place& at) {
-  at.begin += at.cost;
-  if (++at.tile == at.costs.tiles) {
-    at.tile = 0;
-    if (++at.hk == P.Hkv) {
-      at.hk = 0;
-      do {
-        ++at.b;
-        at.req = pa_read_request(P, at.b);
-        at.costs = pa_cost_of<S>(P, at.req);
-      } while (at.costs.tiles == 0);
-    }
-  }
-  at.cost = pa_uniform(at.costs.of(at.tile));
-}
-
-// what a workgroup leaves for the second kernel
+;// what a workgroup leaves for the second kernel
 struct pa_note {
   int b, hk, tile;  // the tile it began and others went on with; b < 0: none
   int last;         // the workgroup that ended it
@@ -361,7 +372,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
   }
   const pa_piece piece = pa_start<NT, S>(pa_arguments(), w, s_sum);
   const int sharers = piece.sharers;
-  if (w >= sharers) return;
+  if (piece.none(w)) return;
   const int64_t total = piece.total, x1 = piece.x1;
   int64_t x = piece.x0;
   pa_place at = piece.at;
@@ -390,7 +401,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     const bool regular = P.page_size >= KPI && P.ks_t >= P.D && P.vs_t >= P.D;
     const uint32_t k_step = (uint32_t)(KPI * P.ks_t * ES), v_step = (uint32_t)(KPI * P.vs_t * ES);  // from an instruction's keys to the next one's
     const uint32_t k_lane = (uint32_t)(l_key * P.ks_t * ES), v_lane = (uint32_t)(l_key * P.vs_t * ES);
-    const int64_t y0 = x - at.begin, y1 = x1 - at.begin < at.cost ? x1 - at.begin : at.cost;
+    const int64_t y0 = x - at.begin, y1 = x1 - at.begin < at.cost && at.cost > piece.whole ? x1 - at.begin : at.cost;
     const bool whole = y0 == 0 && y1 == at.cost;
     const int row_first = at.tile * S::ROWS;
     const int n_rows = at.req.n_new * G;  // (n_new <= n_tokens, and n_tokens * Hq fits: the host has checked)
@@ -1000,7 +1011,7 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
   const int64_t x0 = piece.x0, x1 = piece.x1;
   pa_place at = piece.at;
   for (;;) {
-    if (at.begin >= x0 && at.begin + at.cost <= x1) {
+    if (at.begin >= x0 && (at.begin + at.cost <= x1 || at.cost <= piece.whole)) {
       const int n_rows = at.req.n_new * G;
       for (int i = (int)blockIdx.y * NW + wave; i < S::ROWS; i += PA_JOIN_WGS * NW) {
         const int r = at.tile * S::ROWS + i;

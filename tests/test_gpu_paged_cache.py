@@ -346,6 +346,46 @@ def test_attention_of_large_logits(cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("dim, window", [(64, 0), (128, 0), (128, 100), (256, 0)])
+@pytest.mark.parametrize("new, cached", [
+    ([1] * 30, [7 * i for i in range(30)]),                        # short tiles only
+    ([1] * 20 + [0, 1], [90] * 20 + [500, 9000]),                  # ... and one long one
+    ([200, 1, 1, 33, 1, 300], [0, 800, 0, 100, 5000, 50]),
+    ([64] * 40, [i % 7 * 60 for i in range(40)]),
+])
+def test_attention_of_short_requests(cuda, dtype, dim, window, new, cached):
+    """Tiles that are short enough for one workgroup, alone and beside ones that are shared."""
+    _attention_case(cuda, dtype, new, cached, 8, 2, dim, 16, sink=5 if window else 0, window=window)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("new", [1, 40])
+def test_values_that_are_not_finite_among_short_requests(cuda, dtype, new):
+    """Only the request that holds them is changed, and of it only the rows that see them."""
+    n, page, dim, heads, at = 24, 16, 64, 4, 17
+    g = torch.Generator().manual_seed(9)
+    kv = [new + 20 + 9 * b for b in range(n)]
+    width = -(-max(kv) // page)
+    kc, vc = (torch.randn(n * width, page, 1, dim, generator=g).to(dtype).to(cuda) for _ in range(2))
+    table = torch.arange(n * width, dtype=torch.int32, device=cuda).view(n, width)
+    q = torch.randn(n * new, heads, dim, generator=g).to(dtype).to(cuda)
+    args = (table, _i32(kv, cuda), _i32([new * b for b in range(n + 1)], cuda), 0.125)
+    clean = P.paged_attention(q, kc, vc, *args)
+    assert bool(clean.isfinite().all())
+    for b in (0, 5, 23):
+        spoilt = vc.clone()
+        spoilt.view(n, width * page, dim)[b, at, 3] = math.nan
+        got = P.paged_attention(q, kc, spoilt, *args)
+        rows = torch.arange(new * b + max(0, at - (kv[b] - new)), new * (b + 1), device=cuda)  # they see the key
+        assert bool(got[rows, :, 3].isnan().all())
+        same = torch.ones(n * new, dtype=torch.bool, device=cuda)
+        same[new * b: new * (b + 1)] = False
+        assert torch.equal(got[same], clean[same])
+        before = torch.arange(new * b, int(rows[0]), device=cuda)
+        assert bool(got[before].isfinite().all()) and bool(got[rows][:, :, [i for i in range(dim) if i != 3]].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_attention_values_that_are_not_finite_stay_where_they_are_seen(cuda, dtype, bad):
     """A key or value that is not finite reaches the rows that see it and no other."""
