@@ -155,6 +155,12 @@ __device__ __forceinline__ int pa_sharers(int64_t total) {
   const int64_t w = (total + S::LEAST - 1) / S::LEAST;
   return (int)(w < (int)gridDim.x ? w : (int)gridDim.x);
 }
+// This workgroup's number on the line of work: neighbours share keys, and parts of a tile, so they get the same XCD (the number of workgroups is a
+// multiple of 8). The second kernel goes by the same numbers: by blockIdx.x itself the workgroups that begin a tile of 8 parts are all on
+// one XCD, and read what others' L2s hold (%JOIN%).
+__device__ __forceinline__ int pa_number() {
+  return (int)(blockIdx.x % PA_XCDS) * (int)(gridDim.x / PA_XCDS) + (int)(blockIdx.x / PA_XCDS);
+}
 // where workgroup w of n begins
 __device__ __forceinline__ int64_t pa_bound(int64_t total, int n, int w) {
   const int64_t each = pa_uniform(pa_div(total, n));
@@ -363,8 +369,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
   const int i32 = lane & 31, g = lane >> 5;
   const int rw = WIDE ? wave : 0;
-  // neighbours on the line of work share keys: they get the same XCD
-  const int w = (int)(blockIdx.x % PA_XCDS) * (int)(gridDim.x / PA_XCDS) + (int)(blockIdx.x / PA_XCDS);
+  const int w = pa_number();
   if (threadIdx.x == 0) {
     pa_note* note = (pa_note*)pa_arguments().work + w;
     note->b = -1;
@@ -905,7 +910,7 @@ __device__ __forceinline__ void pa_row_again(pa_args& P, const pa_request& r, in
   }
 }
 
-// Joins the parts of the tile that workgroup blockIdx.x of the first kernel began and did not end. 16 lanes hold a row: with few parts
+// Joins the parts of the tile that this workgroup's number in the first kernel began and did not end. 16 lanes hold a row: with few parts
 // a workgroup does 16 rows at once, with many one row, whose parts its 16 groups take in turn. blockIdx.y shares the rows out.
 #define PA_JOIN_NT 256
 #define PA_JOIN_GROUPS (PA_JOIN_NT / 16)
@@ -921,7 +926,7 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
   __shared__ int64_t s_sum[NW + 2];
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
   const int group = threadIdx.x / 16, l16 = threadIdx.x % 16;
-  const int w = blockIdx.x, G = P.Hq / P.Hkv;
+  const int w = pa_number(), G = P.Hq / P.Hkv;
   const pa_note note = ((const pa_note*)P.work)[w];
   const float* parts = P.work + S::WGS * (sizeof(pa_note) / 4);
   if (note.b >= 0) {
