@@ -157,7 +157,7 @@ __device__ __forceinline__ int pa_sharers(int64_t total) {
 }
 // This workgroup's number on the line of work: neighbours share keys, and parts of a tile, so they get the same XCD (the number of workgroups is a
 // multiple of 8). The second kernel goes by the same numbers: by blockIdx.x itself the workgroups that begin a tile of 8 parts are all on
-// one XCD, and read what others' L2s hold (%JOIN%).
+// one XCD, and read what others' L2s hold (62 us instead of 34 for 64 parts, 34 instead of 18 for 8).
 __device__ __forceinline__ int pa_number() {
   return (int)(blockIdx.x % PA_XCDS) * (int)(gridDim.x / PA_XCDS) + (int)(blockIdx.x / PA_XCDS);
 }
@@ -1036,11 +1036,17 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-// Tiles of 128 rows whose waves share the keys, or of 32 rows whose waves each take keys of their own: by the rows per request.
+// Tiles of 128 rows whose waves share the keys, or of 32 rows whose waves each take keys of their own: by the rows per request, on average.
+// Up to 32 nothing is shared. Up to 64 half of a wide tile is empty, but a narrow one's end, where 8 waves are added up, counts where there are
+// several a workgroup; up to 128 a wide tile costs nothing more, but has four times as much to join where few tiles are shared by all. In us,
+// narrow / wide, 8 key heads of 128, bf16: 1 request of 64 rows and 32768 keys 41 / 59, 16 of 64 and 4096 50 / 52, 64 of 64 and 1024 66 / 46;
+// 1 of 128 and 32768 52 / 64, 4 of 128 and 8192 49 / 47, 16 of 128 and 4096 83 / 65; 1 of 256 and 32768 79 / 69, of 8192 and 8192 434 / 260.
 // fp32 is bound by its matrix instructions (a sixteenth of the 16-bit rate) however often keys are read: 32 rows, so that a
 // request of few rows keeps all waves busy (5 requests of 4 to 132 rows, 2000 keys on average: 66 us as tiles of 128, 34 so).
 static bool pa_wide(const sah_paged_attention_args* a) {
-  return a->dtype != SAH_F32 && (int64_t)a->n_tokens * (a->Hq / a->Hkv) > 32 * (int64_t)a->n_requests;
+  const int64_t rows = (int64_t)a->n_tokens * (a->Hq / a->Hkv), n = a->n_requests, tiles = rows * a->Hkv / 32;
+  if (a->dtype == SAH_F32 || rows <= 32 * n) return false;
+  return tiles > (rows <= 64 * n ? 2 * PA_CUS : rows <= 128 * n ? PA_CUS / 4 : 0);
 }
 
 template <int DT, int DP, bool WIDE>
