@@ -64,7 +64,10 @@ __device__ __forceinline__ void pg_place(const sah_paged_assign_args& P, const i
   }
 }
 
-// One workgroup goes over the requests; with ALL it also places the tokens, else it leaves the records for k_paged_place.
+// One workgroup goes over the requests: who is granted depends on all requests before, and their running sums are two scans of up to 4096
+// numbers, latency and nothing else (64 requests: 5.4 us, of which a launch is 2). With ALL it also places the tokens, else it leaves
+// the records for k_paged_place. One kernel up to 1024 tokens, one a thread (64 requests of 16: 6.8 us, 8.0 in two); the second kernel
+// from there on (4096 tokens: 10.1 us in one, 8.4 in two; 32768: 41 and 8.5).
 template <bool ALL>
 __global__ __launch_bounds__(PG_NT) void k_paged_assign(sah_paged_assign_args P) {
   sah_touch_kernargs<sizeof(sah_paged_assign_args)>();
@@ -126,6 +129,7 @@ __global__ __launch_bounds__(PG_NT) void k_paged_assign(sah_paged_assign_args P)
   if (ALL) pg_place(P, s_end, s_rec, threadIdx.x, PG_NT);
 }
 
+// 12 bytes written per token; a search among the requests' ends, in LDS, for each: 256001 tokens of 1024 requests 4.8 us.
 __global__ __launch_bounds__(PG_NT) void k_paged_place(sah_paged_assign_args P) {
   sah_touch_kernargs<sizeof(sah_paged_assign_args)>();
   SAH_DYNAMIC_LDS(s_dyn);
@@ -139,7 +143,8 @@ __global__ __launch_bounds__(PG_NT) void k_paged_place(sah_paged_assign_args P) 
   pg_place(P, s_end, s_rec, blockIdx.x * PG_NT + threadIdx.x, gridDim.x * PG_NT);
 }
 
-// The finished requests' pages: places in the free list, and the requests' state
+// The finished requests' pages: places in the free list, and the requests' state. (Two kernels: the pages move on as many workgroups as there
+// are requests, 4 bytes read and 8 written each.)
 __global__ __launch_bounds__(PG_NT) void k_paged_release(sah_paged_release_args P) {
   __shared__ int64_t s_sum[PG_NT / SAH_WAVE];
   int64_t count = *P.free_count;
@@ -172,7 +177,9 @@ __global__ __launch_bounds__(256) void k_paged_give_back(sah_paged_release_args 
   }
 }
 
-// A unit is W bytes of a token's keys or values; consecutive threads take consecutive units of a token.
+// A unit is W bytes of a token's keys or values; consecutive threads take consecutive units of a token. Memory: 16384 tokens of 8 heads of
+// 128 (bf16, 134 MB moved) 20.6 us, 6.5 TB/s; into a cache that lies in the last-level cache still 13 us, element by element 62. No
+// staging, no reuse: nothing is read twice.
 template <typename W>
 __global__ __launch_bounds__(256) void k_paged_store(sah_paged_store_args P, int units_head, int units_token, int64_t n_units) {
   sah_touch_kernargs<sizeof(sah_paged_store_args) + 16>();
@@ -206,7 +213,7 @@ extern "C" int sah_paged_assign(const sah_paged_assign_args* a) {
     return sah_fail(SAH_ENULL, "sah_paged_assign: NULL pointer");
   const size_t lds = (size_t)a->n_requests * 12;
   hipStream_t st = (hipStream_t)a->stream;
-  if (a->n_tokens <= 4 * PG_NT) {
+  if (a->n_tokens <= PG_NT) {
     sah_timed timed("k_paged_assign", a->stream);
     hipLaunchKernelGGL(k_paged_assign<true>, dim3(1), dim3(PG_NT), lds, st, *a);
     return sah_launch_status("sah_paged_assign");

@@ -10,6 +10,11 @@
 // are ranked by a wave (sm_pick). It runs over a list in LDS of all tokens that may be kept, where that can hold them: what may
 // be kept is known early, since where r of 1024 threads' own largest logits reach a value, at least r of the row do, and few
 // more. Where it cannot, the row is cut into pieces of 1 / SM_FINE in (m - x) / t first, and the list holds one of them.
+//
+// What bounds it: 256 rows of 150001 (fp32) are read once in 24.6 us (6.2 TB/s, the answer of greedy rows), and 65 us where every
+// weight is needed (all tokens): 22 fp64 instructions each, 8 cycles a wave. So a weight is taken where it is needed only: top-k 50 and
+// min-p 0.05 of a list 50 and 47 us; top-p 0.9 needs all of them once, for the sum, 110. The list saves the passes that follow (a row of 32000
+// in one workgroup: 13 us for top-k, 27 for top-p); a nucleus of more than 8192 tokens costs them (temperature 1.5: 178 us).
 #include "sah_common.h"
 #include "../../include/sah_serve.h"
 
