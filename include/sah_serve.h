@@ -26,7 +26,7 @@ extern "C" {
  * (lens[b] + i; 0 behind the last request's rows); slot_map [n_tokens] (-1 for a request that is not granted and behind the
  * last one's rows); granted [n_requests], 0 or 1; kv_lens [n_requests], what attention may see: lens[b] + new_lens[b], or 0
  * for a request that is not granted; lens_out, which may be lens, and free_count_out, which may be free_count; the new pages'
- * entries of block_table. work: 2 * n_requests words. At most 4096 requests. */
+ * entries of block_table. work: 2 * n_requests words. At most 4096 requests and 2^30 tokens. */
 typedef struct sah_paged_assign_args {
   const int32_t* new_lens;
   const int32_t* lens;
@@ -82,7 +82,8 @@ int sah_paged_store(const sah_paged_store_args* a);
  * j < sink or j > p - window (the Sink and Local maskers' columns). sinks, optional [Hq]: a logit per head in the softmax's
  * denominator. A row that sees nothing is 0. Rows of q behind the last request's are not read and their output is left as it
  * was. Lengths beyond table_width pages count as that many. out [n_tokens, Hq, D]. max_context: about how long the longest
- * request is (0: not known); it decides how work is split, never what is computed. page_size: a power of two.
+ * request is (0: not known); it decides how work is split, never what is computed. page_size: a power of two; table_width *
+ * page_size below 2^31 - 4096. Rows of out share no memory with each other or with what is read.
  * work: sah_paged_attention_work_floats(a) floats, no particular content. */
 typedef struct sah_paged_attention_args {
   const void* q; int64_t qs_t, qs_h;

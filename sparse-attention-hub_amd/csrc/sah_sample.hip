@@ -4,7 +4,7 @@
 // token. Weights are exp((x - m) / t) in fp64, summed as integers of 2^-43: sums of up to 2^20 of them fit 64 bits, are
 // exact, and so do not depend on who adds when.
 //
-// A workgroup has a row. Everything that decides is a selection of one kind: of weighted items in an order, the one at which the
+// A workgroup has a row (few long rows: several, for the passes over all of it). Everything that decides is a selection of one kind: of weighted items in an order, the one at which the
 // running weight reaches a target: the k-th largest (weight 1), top-p's last (a token's weight), the drawn token (the same in
 // the order of the index). Weights are added up per piece of the order's range in LDS, the few items of the piece that holds the target
 // are ranked by a wave (sm_pick). It runs over a list in LDS of all tokens that may be kept, where that can hold them: what may

@@ -359,6 +359,12 @@ def test_attention_of_short_requests(cuda, dtype, dim, window, new, cached):
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("n, new", [(700, 1), (513, 0), (300, 17)])
+def test_attention_of_more_requests_than_threads(cuda, dtype, n, new):
+    _attention_case(cuda, dtype, [new if b % 9 else 1 - new for b in range(n)] if new < 2 else [new] * n, [b % 41 for b in range(n)], 4, 1, 64, 16)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
 @pytest.mark.parametrize("new", [1, 40])
 def test_values_that_are_not_finite_among_short_requests(cuda, dtype, new):
     """Only the request that holds them is changed, and of it only the rows that see them."""

@@ -212,6 +212,37 @@ def test_several_workgroups_a_row_or_one(cuda, dtype, rows, vocab, settings):
     assert torch.equal(tokens, one) and torch.equal(logs, one_log)
 
 
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=20), dict(top_p=0.95, temperature=1.3)])
+def test_rows_shared_by_workgroups_in_a_replayed_graph_and_on_two_streams(cuda, settings):
+    rows, vocab = 3, 70001
+    x, u = (t.to(cuda) for t in _logits(rows, vocab, torch.bfloat16, 40))
+    sample_tokens(x, u, **settings)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tokens, logs = sample_tokens(x, u, **settings)
+    for seed in range(4):
+        new_x, new_u = _logits(rows, vocab, torch.bfloat16, 41 + seed)
+        x.copy_(new_x)
+        u.copy_(new_u)
+        graph.replay()
+        want = sample_tokens(x, u, **settings)
+        torch.cuda.synchronize()
+        assert torch.equal(tokens, want[0]) and torch.equal(logs, want[1])
+    other = [t.to(cuda) for t in _logits(rows, vocab, torch.bfloat16, 50)]
+    want = [sample_tokens(x, u, **settings), sample_tokens(*other, **settings)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for stream, given in zip(streams, ((x, u), other)):
+            with torch.cuda.stream(stream):
+                got.append(sample_tokens(*given, **settings))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_shares_are_those_of_the_distribution(cuda):
     """200000 draws from 8 tokens: each one's share is within 5 standard deviations."""
     n, p = 200000, torch.tensor([0.4, 0.2, 0.15, 0.1, 0.08, 0.04, 0.02, 0.01], dtype=torch.float64)
