@@ -167,22 +167,23 @@ __device__ __forceinline__ int64_t pa_bound(int64_t total, int n, int w) {
   return each * w + pa_uniform(pa_div((total - each * n) * w, n));
 }
 
-// the next tile on the line; there is one
+// The next tile on the line; there is one, unless lengths changed under way (an error of the program's, but one that ends)
 template <typename S>
-__device__ __forceinline__ void pa_next(pa_args& P, pa_place& at) {
+__device__ __forceinline__ bool pa_next(pa_args& P, pa_place& at) {
   at.begin += at.cost;
   if (++at.tile == at.costs.tiles) {
     at.tile = 0;
     if (++at.hk == P.Hkv) {
       at.hk = 0;
       do {
-        ++at.b;
+        if (++at.b >= P.n_requests) return false;
         at.req = pa_read_request(P, at.b);
         at.costs = pa_cost_of<S>(P, at.req);
       } while (at.costs.tiles == 0);
     }
   }
   at.cost = pa_uniform(at.costs.of(at.tile));
+  return true;
 }
 
 // Workgroup w's piece of the line, [x0, x1), and the place that holds x0
@@ -265,7 +266,7 @@ __device__ __forceinline__ pa_piece pa_start(pa_args& P, int w, int64_t* s_sum) 
   r.whole = r.total <= (int64_t)S::WHOLE * r.sharers ? S::WHOLE : 0;
   if (r.x0 > at.begin && at.cost <= r.whole) {
     r.x0 = at.begin + at.cost;
-    if (r.x0 < r.x1) pa_next<S>(P, at);
+    if (r.x0 < r.x1 && !pa_next<S>(P, at)) r.x0 = r.x1;
   }
   return r;
 }
@@ -859,7 +860,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
     x = at.begin + y1;
     if (x >= x1) break;
     if (!WIDE) __syncthreads();  // all shares have been read
-    pa_next<S>(pa_arguments(), at);
+    if (!pa_next<S>(pa_arguments(), at)) break;
   }
   if (bad) ((pa_note*)pa_arguments().work)[w].again = 1;
 }
@@ -1029,7 +1030,7 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
       }
     }
     if (at.begin + at.cost >= x1) break;
-    pa_next<S>(P, at);
+    if (!pa_next<S>(P, at)) break;
   }
 }
 
