@@ -980,22 +980,27 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
 #pragma unroll
         for (int f = 0; f < F; ++f) s_acc[group][l16 + 16 * f] = acc[f];
         __syncthreads();
-        if (group) continue;
-        for (int o = 1; o < PA_JOIN_GROUPS; ++o) {
-          float4 v[F];
+        // The first wave ends the row, its first 16 lanes with what all groups have added up; the others stay for a row that is done again,
+        // which takes a whole wave.
+        if (wave) continue;
+        if (group == 0) {
+          for (int o = 1; o < PA_JOIN_GROUPS; ++o) {
+            float4 v[F];
 #pragma unroll
-          for (int f = 0; f < F; ++f) v[f] = s_acc[o][l16 + 16 * f];
-          add(make_float2(s_ml[o][0], s_ml[o][1]), v);
+            for (int f = 0; f < F; ++f) v[f] = s_acc[o][l16 + 16 * f];
+            add(make_float2(s_ml[o][0], s_ml[o][1]), v);
+          }
         }
       }
+      const bool holds = !many || group == 0;  // this lane has a row's sums
       const int r = note.tile * S::ROWS + i, tok = req.row0 + r / G, h = note.hk * G + r % G;
-      bool fine = l == l;
+      bool fine = !holds || l == l;
       if (P.sinks && m != -INFINITY) l += exp2f(fmaf(P.sinks[h], 1.4426950408889634f, pa_weights<DT>::SCALE) - m);
       const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
       for (int f = 0; f < F; ++f) {
         const int d = 4 * l16 + 64 * f;
-        if (d >= P.D) continue;
+        if (!holds || d >= P.D) continue;
         const float4 o = make_float4(acc[f].x * inv, acc[f].y * inv, acc[f].z * inv, acc[f].w * inv);
         fine = fine && fabsf(o.x) < INFINITY && fabsf(o.y) < INFINITY && fabsf(o.z) < INFINITY && fabsf(o.w) < INFINITY;
         char* to = (char*)P.out + ((int64_t)tok * P.os_t + (int64_t)h * P.os_h + d) * S::ES;

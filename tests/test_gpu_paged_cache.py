@@ -427,6 +427,53 @@ def test_attention_values_that_are_not_finite_stay_where_they_are_seen(cuda, dty
             assert out[at:].isnan().all()
 
 
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new, kv_heads", [(1, 1), (1, 2), (4, 2), (9, 1)])
+def test_values_that_are_not_finite_in_a_long_context(cuda, dtype, dim, new, kv_heads):
+    """Tiles of three dozen parts: a bad value spoils its own dim of the rows that see it, a bad key all of those rows, nothing else."""
+    page, n, group, bad_dim = 16, 9001, 4, 3
+    g = torch.Generator().manual_seed(dim + new)
+    k, v = (torch.randn(n, kv_heads, dim, generator=g).to(dtype) for _ in range(2))
+    q = (4 * torch.randn(new, group * kv_heads, dim, generator=g)).to(dtype)  # few keys take most of a row's weight
+    pages = -(-n // page)
+    table, kv, cu = torch.arange(pages, dtype=torch.int32, device=cuda)[None], _i32([n], cuda), _i32([0, new], cuda)
+
+    def attend(keys, values):
+        kc, vc = (torch.zeros(pages * page, kv_heads, dim, dtype=dtype, device=cuda) for _ in range(2))
+        kc[:n], vc[:n] = keys.to(cuda), values.to(cuda)
+        return P.paged_attention(q.to(cuda), kc.view(pages, page, kv_heads, dim), vc.view(pages, page, kv_heads, dim), table, kv, cu,
+                                 dim ** -0.5).double().cpu()
+
+    clean = attend(k, v)
+    want, bound = torch.empty(new, group, dim, dtype=torch.float64), torch.empty(new, group, dim, dtype=torch.float64)
+    visible = torch.arange(n)[None] <= torch.arange(n - new, n)[:, None]
+    half = _HALF_STEP[dtype]
+    for h in range(group):
+        qq, kk = q[:, h].double(), k[:, 0].double()
+        want[:, h], size = _plain_attention(qq, kk, v[:, 0].double(), visible, dim ** -0.5, None)
+        # the bound of _attention_case
+        reach = float((qq.abs() @ kk.abs().T).max()) * dim ** -0.5
+        logit_off = (dim + 4) * 2.0 ** -24 * reach + 8 * 2.0 ** -24
+        bound[:, h] = want[:, h].abs() * half + size * ((half if dtype != torch.float32 else 0.0) + 2 * logit_off + (2 * n + 16) * 2.0 ** -24)
+    others = [d for d in range(dim) if d != bad_dim]
+    for at in (0, n // 2, n - 1):
+        sees = torch.arange(n - new, n) >= at
+        for bad in (math.nan, math.inf):
+            spoilt = v.clone()
+            spoilt[at, 0, bad_dim] = bad
+            got = attend(k, spoilt)
+            assert torch.equal(got[:, group:], clean[:, group:])  # the other key heads
+            assert got[sees, :group, bad_dim].isnan().all() if bad != bad else not got[sees, :group, bad_dim].isfinite().any()
+            off = (got[:, :group] - want).abs() <= 1.001 * bound
+            assert bool(off[:, :, others].all()) and bool(off[~sees].all()), (at, bad)
+        spoilt = k.clone()
+        spoilt[at, 0, bad_dim] = math.nan
+        got = attend(spoilt, v)
+        assert got[sees, :group].isnan().all() and torch.equal(got[:, group:], clean[:, group:])
+        assert bool(((got[:, :group] - want).abs() <= 1.001 * bound)[~sees].all())
+
+
 def test_attention_offsets_beyond_32_bits(cuda):
     """Pages whose elements start past 2^31."""
     page, heads, dim, pages = 16, 8, 128, 2 ** 31 // (16 * 8 * 128) + 40
