@@ -155,13 +155,13 @@ struct sm_bin {
   uint64_t before;   // weight of the bins ahead of it
 };
 // Adds up what `each` hands to its argument (bin, weight) and finds where the running weight, from bin 0 on, reaches
-// target(all the weight). All threads call; ends behind a wait.
+// target(all the weight). All threads call; ends behind a wait, and may be called again at once.
 template <typename TARGET, typename EACH>
 __device__ __forceinline__ sm_bin sm_locate(sm_shared& S, TARGET target_of, EACH each) {
   static_assert(SM_BINS == 2 * SM_NT, "two bins a thread");
   each([&](uint32_t bin, uint64_t weight) { atomicAdd((unsigned long long*)&S.bins[bin], (unsigned long long)weight); });
-  if (threadIdx.x == 0) S.found_bin = -1;
   __syncthreads();
+  if (threadIdx.x == 0) S.found_bin = -1;  // (behind this wait all have read the call before's; the scan's comes before the bin is found)
   const int b = 2 * (int)threadIdx.x;
   const uint64_t w0 = S.bins[b], w1 = S.bins[b + 1];
   S.bins[b] = 0;

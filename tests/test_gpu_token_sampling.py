@@ -171,6 +171,21 @@ def test_more_rows_than_the_chip_holds_at_once(cuda):
     _compare(cuda, x, u, t=0.9, p=0.95)
 
 
+@pytest.mark.parametrize("vocab", [8193, 9000, 20000])
+@pytest.mark.parametrize("settings", [dict(top_p=0.9), dict(top_p=0.97, temperature=1.4), dict(top_p=0.9, min_p=0.01)])
+def test_selections_that_follow_each_other_at_once(cuda, vocab, settings):
+    """Rows just longer than the list, where a wave's pass between the list's threshold and the nucleus' border is a few loads: every run the same."""
+    x, u = _logits(1000, vocab, torch.float32, vocab)
+    x[::2] = x[::2].to(torch.bfloat16).float()
+    few = slice(0, 1000, 50)
+    _compare(cuda, x[few].contiguous(), u[few].contiguous(), t=settings.get("temperature"), p=settings["top_p"], least=settings.get("min_p"))
+    x, u = x.to(cuda), u.to(cuda)
+    tokens, logs = sample_tokens(x, u, **settings)
+    for _ in range(20):
+        again, again_logs = sample_tokens(x, u, **settings)
+        assert torch.equal(again, tokens) and torch.equal(again_logs, logs)
+
+
 def test_no_rows(cuda):
     tokens, logs = sample_tokens(torch.empty(0, 100, device=cuda), torch.empty(0, device=cuda))
     assert tokens.shape == (0,) and logs.shape == (0,)
