@@ -39,6 +39,12 @@ struct pa_shape {
   static constexpr int WGS = PA_CUS * PER_CU;
   static constexpr int WAVES = NW * PER_CU >= 4 ? NW * PER_CU / 4 : 1;  // per SIMD
   static constexpr int SLOT = ROWS * (DP + 2);             // floats of a part
+  // 16-bit terms that a weight is taken apart into for the second product. Two where every wave has keys of its own: memory bounds that
+  // form and the second term's products are free (64 single tokens, 779 us either way), the result is as exact as its own rounding (off
+  // by 0.0017 in bf16, 0.0002 in fp16; with one term 0.0023 and 0.00026). One where waves share keys: matrix and vector instructions
+  // bound it, and a second term takes 812 us instead of 639 (2048 tokens over 18432 keys) for the same gain. A weight is
+  // off by half a step then, each by one of its own sign: on average less than the result's own rounding.
+  static constexpr int TERMS = WIDE ? 1 : 2;
   // In keys: what starting and ending a tile takes (256: one request of 100 keys 17 us instead of 11, its 8 heads' tiles split), and
   // the least that is worth a workgroup (512: 5 fp32 requests of 2000 keys 43 us instead of 34; 128: no case gains, small ones lose 1).
   static constexpr int TILE_COST = 128;
@@ -312,8 +318,7 @@ __device__ __forceinline__ pa_stages pa_stages_of(pa_args& P, const pa_request& 
 
 // How far a row's maximum may rise, in powers of two, before the row is rescaled (a rise of the maximum by a little is frequent,
 // by 2^SLACK rare), and the power of two that the weights are held above their true size by: they enter the second product in
-// the tensor's type (half a step each, of independent signs: less than the result's own rounding), and fp16 keeps all its
-// bits for weights down to 2^-22 of the row's largest that way.
+// terms of the tensor's type, and fp16 keeps all its bits for weights down to 2^-22 of the row's largest that way.
 template <int DT> struct pa_weights {
   static constexpr float SLACK = DT == SAH_F16 ? 6.0f : 8.0f;
   static constexpr float SCALE = DT == SAH_F16 ? 8.0f : 0.0f;
@@ -668,6 +673,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
           }
       } else {
         __builtin_amdgcn_s_setprio(1);
+        uint32_t term[S::TERMS][4];
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
           const int step = c / (DTL / DV), t = step / 2, st = step % 2;
@@ -675,13 +681,32 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
 #pragma unroll
           for (int d = 0; d < DV; ++d) pa_from_here(va[c & 1][d]);
           const auto& z = s[t];
-          const uint4 pt = make_uint4(sah_pack2_hw<DT>(z[8 * st], z[8 * st + 1]), sah_pack2_hw<DT>(z[8 * st + 2], z[8 * st + 3]),
-                                      sah_pack2_hw<DT>(z[8 * st + 4], z[8 * st + 5]), sah_pack2_hw<DT>(z[8 * st + 6], z[8 * st + 7]));
+          if (c % (DTL / DV) == 0) {  // the step's weights: as they are rounded, and what the rounding has cut off
 #pragma unroll
-          for (int d = 0; d < DV; ++d) {
-            const int to = c % (DTL / DV) * DV + d;
-            acc[to] = sah_mfma_32x32x16<DT>(pa_operand(va[c & 1][d]), pt, acc[to]);
+            for (int p = 0; p < 4; ++p) {
+              float p0 = z[8 * st + 2 * p], p1 = z[8 * st + 2 * p + 1];
+#pragma unroll
+              for (int i = 0; i < S::TERMS; ++i) {
+                term[i][p] = sah_pack2_hw<DT>(p0, p1);
+                if (i + 1 == S::TERMS) break;
+                sah_keep(term[i][p]);  // taken apart as it is, instead of converted a second time
+                if (DT == SAH_BF16) {
+                  p0 -= sah_bits_to_float(term[i][p] << 16);
+                  p1 -= sah_bits_to_float(term[i][p] & 0xffff0000u);
+                } else {
+                  p0 -= sah_f16_to_float((uint16_t)term[i][p]);
+                  p1 -= sah_f16_to_float((uint16_t)(term[i][p] >> 16));
+                }
+              }
+            }
           }
+#pragma unroll
+          for (int i = 0; i < S::TERMS; ++i)
+#pragma unroll
+            for (int d = 0; d < DV; ++d) {
+              const int to = c % (DTL / DV) * DV + d;
+              acc[to] = sah_mfma_32x32x16<DT>(pa_operand(va[c & 1][d]), make_uint4(term[i][0], term[i][1], term[i][2], term[i][3]), acc[to]);
+            }
           if (TW == 2 && t == 0) {
             constexpr int N = 16 * TW / NV;
             weigh(1, c * N, N);

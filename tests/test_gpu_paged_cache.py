@@ -306,6 +306,39 @@ def test_attention_single_tokens(cuda, dtype, cached):
     _attention_case(cuda, dtype, [1] * 3, [cached, cached // 2, 0], 8, 2, 128, 16, seed=cached, pad=2)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("scale", [1.0, 4.0])
+def test_attention_of_few_rows_is_rounded_once(cuda, dtype, dim, scale):
+    """Up to 32 rows a request: weights are taken apart into two terms of the type, so that what is left is the result's own rounding."""
+    page, heads, kv_heads = 16, 8, 2
+    new, kv = [1, 2, 1, 8], [5000, 700, 64, 1500]
+    g = torch.Generator().manual_seed(dim)
+    width = -(-max(kv) // page)
+    kc, vc = (torch.randn(len(kv) * width * page, kv_heads, dim, generator=g).to(dtype) for _ in range(2))
+    q = (scale * torch.randn(sum(new), heads, dim, generator=g)).to(dtype)
+    cu = [sum(new[:b]) for b in range(len(new) + 1)]
+    table = torch.arange(len(kv) * width, dtype=torch.int32, device=cuda).view(len(kv), width)
+    got = P.paged_attention(q.to(cuda), kc.to(cuda).view(-1, page, kv_heads, dim), vc.to(cuda).view(-1, page, kv_heads, dim), table, _i32(kv, cuda),
+                            _i32(cu, cuda), dim ** -0.5).double().cpu()
+    half = _HALF_STEP[dtype]
+    for b, n in enumerate(kv):
+        visible = torch.arange(n)[None] <= torch.arange(n - new[b], n)[:, None]
+        at = slice(b * width * page, b * width * page + n)
+        for h in range(heads):
+            qq, kk, vv = q[cu[b]:cu[b + 1], h].double(), kc[at, h * kv_heads // heads].double(), vc[at, h * kv_heads // heads].double()
+            want, size = _plain_attention(qq, kk, vv, visible, dim ** -0.5, None)
+            # _attention_case's bound with weights off by half a step of half a step, and by what fp16's smallest number (2^-24, weights
+            # above their true size by 2^3 at least) cuts off: 2^-27 of the row's largest weight, n of them
+            reach = float((qq.abs() @ kk.abs().T).max()) * dim ** -0.5
+            logit_off = (dim + 4) * 2.0 ** -24 * reach + 8 * 2.0 ** -24
+            bound = want.abs() * half + size * (half * half + 2 * logit_off + (2 * n + 16) * 2.0 ** -24)
+            if dtype == torch.float16:
+                bound = bound + n * 2.0 ** -27 * float(vv.abs().max()) + 2.0 ** -25
+            bad = (got[cu[b]:cu[b + 1], h] - want).abs() > bound * 1.001
+            assert not bad.any(), (b, h, int(bad.sum()))
+
+
 @pytest.mark.parametrize("dtype", _TYPES)
 @pytest.mark.parametrize("new, cached", [([2], [0]), ([31, 32, 33], [1, 0, 64]), ([128], [500]), ([129, 1], [0, 3000]), ([300], [17]),
                                          ([0, 0, 3], [50, 0, 0]), ([1] * 40, list(range(40)))])
