@@ -324,6 +324,11 @@ template <int DT> struct pa_weights {
   static constexpr float SCALE = DT == SAH_F16 ? 8.0f : 0.0f;
 };
 
+// Results from here on (or NaN) are done again: the type has no finite number for them, while the average of finite values is one. (Weights
+// of one term each half a step too large reach this where all values are the type's largest.)
+template <int DT>
+__device__ __forceinline__ bool pa_fine(float v) { return fabsf(v) < (DT == SAH_F32 ? INFINITY : DT == SAH_BF16 ? 0x1.ffp127f : 65520.f); }
+
 // Reads of LDS written above this are issued above it, and x, the result of an earlier one, is used below it alone. (Left to itself the
 // compiler reads where it multiplies, one wait of LDS's latency after the other.)
 __device__ __forceinline__ void pa_reads_stay() {
@@ -849,7 +854,7 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
           const int d = 8 * number + 4 * g;
           if (d >= P.D) continue;
           const float4 o = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
-          fine = fine && fabsf(o.x) < INFINITY && fabsf(o.y) < INFINITY && fabsf(o.z) < INFINITY && fabsf(o.w) < INFINITY;
+          fine = fine && pa_fine<DT>(o.x) && pa_fine<DT>(o.y) && pa_fine<DT>(o.z) && pa_fine<DT>(o.w);
           if (!live) continue;
           if (DT == SAH_F32) *(float4*)(op + 4 * d) = o;
           else *(uint2*)(op + 2 * d) = make_uint2(sah_pack2_hw<DT>(o.x, o.y), sah_pack2_hw<DT>(o.z, o.w));
@@ -890,7 +895,8 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
   if (bad) ((pa_note*)pa_arguments().work)[w].again = 1;
 }
 
-// One row key by key, by one wave: what a row holds whose products in a tile came out not finite.
+// One row key by key, by one wave: what a row holds whose products in a tile came out not finite. The average so far is held, not the
+// sum: of finite values it is finite, however large they are.
 template <int DT>
 __device__ __forceinline__ void pa_row_again(pa_args& P, const pa_request& r, int b, int t, int h) {
   constexpr int E = PA_MAX_D / SAH_WAVE;
@@ -919,20 +925,21 @@ __device__ __forceinline__ void pa_row_again(pa_args& P, const pa_request& r, in
     s = sah_wave_sum(s) * P.scaling;
     const float m_new = fmaxf(m, s);
     if (m_new == -INFINITY && s == s) continue;  // (a NaN is no maximum, but the row's result)
-    const float up = expf(m - m_new), w = expf(s - m_new);
+    const float before = l * expf(m - m_new), w = expf(s - m_new);
     m = m_new;
-    l = l * up + w;
+    l = before + w;
+    const float old = before / l, share = w / l;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int d = lane + e * SAH_WAVE;
-      if (d < P.D) acc[e] = acc[e] * up + w * sah_load<DT>(P.v, va + d);
+      if (d < P.D) acc[e] = acc[e] * old + share * sah_load<DT>(P.v, va + d);
     }
   }
-  if (P.sinks && m != -INFINITY) l += expf(P.sinks[h] - m);
+  const float seen = P.sinks && m != -INFINITY ? l / (l + expf(P.sinks[h] - m)) : 1.f;  // all but the sink's share
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int d = lane + e * SAH_WAVE;
-    if (d < P.D) sah_store<DT>(P.out, (int64_t)t * P.os_t + (int64_t)h * P.os_h + d, l == 0.f ? 0.f : acc[e] / l);
+    if (d < P.D) sah_store<DT>(P.out, (int64_t)t * P.os_t + (int64_t)h * P.os_h + d, acc[e] * seen);
   }
 }
 
@@ -1027,7 +1034,7 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
         const int d = 4 * l16 + 64 * f;
         if (!holds || d >= P.D) continue;
         const float4 o = make_float4(acc[f].x * inv, acc[f].y * inv, acc[f].z * inv, acc[f].w * inv);
-        fine = fine && fabsf(o.x) < INFINITY && fabsf(o.y) < INFINITY && fabsf(o.z) < INFINITY && fabsf(o.w) < INFINITY;
+        fine = fine && pa_fine<DT>(o.x) && pa_fine<DT>(o.y) && pa_fine<DT>(o.z) && pa_fine<DT>(o.w);
         char* to = (char*)P.out + ((int64_t)tok * P.os_t + (int64_t)h * P.os_h + d) * S::ES;
         if (DT == SAH_F32) *(float4*)to = o;
         else *(uint2*)to = make_uint2(sah_pack2_hw<DT>(o.x, o.y), sah_pack2_hw<DT>(o.z, o.w));
@@ -1055,7 +1062,7 @@ __global__ __launch_bounds__(PA_JOIN_NT) void k_paged_attn_join(sah_paged_attent
         const int tok = at.req.row0 + r / G, h = at.hk * G + r % G;
         bool fine = true;
         for (int d = lane; d < P.D; d += SAH_WAVE)
-          fine = fine && fabsf(sah_load<DT>(P.out, (int64_t)tok * P.os_t + (int64_t)h * P.os_h + d)) < INFINITY;
+          fine = fine && pa_fine<DT>(sah_load<DT>(P.out, (int64_t)tok * P.os_t + (int64_t)h * P.os_h + d));
         if (__ballot(!fine)) pa_row_again<DT>(P, at.req, at.b, tok, h);
       }
     }

@@ -507,6 +507,33 @@ def test_values_that_are_not_finite_in_a_long_context(cuda, dtype, dim, new, kv_
         assert bool(((got[:, :group] - want).abs() <= 1.001 * bound)[~sees].all())
 
 
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("new, n", [(1, 600), (40, 600), (2, 9001), (150, 3000)])
+def test_averages_of_the_largest_values_are_finite(cuda, dtype, new, n):
+    """Values of the type's largest number: a weight that is rounded up, or a sum before it is divided, must not take a result past it."""
+    page, dim, heads = 16, 64, 4
+    most = torch.finfo(dtype).max if dtype != torch.float32 else 2.0 ** 127 * 1.9  # (fp32: its roundings' worth below the end)
+    logits = torch.linspace(0.01, 3.9, new * heads)[torch.randperm(new * heads, generator=torch.Generator().manual_seed(new))]
+    q = torch.zeros(new * heads, dim)
+    q[:, 0] = logits
+    q = q.view(new, heads, dim).to(dtype)
+    pages = -(-n // page)
+    kc = torch.zeros(pages * page, 1, dim)
+    kc[64:, 0, 0] = 1.0  # all keys but the first ones weigh the same, a row's own number of times more than those
+    signs = torch.where(torch.rand(pages * page, 1, dim, generator=torch.Generator().manual_seed(1)) < 0.5, -1.0, 1.0)
+    visible = torch.arange(n)[None] <= torch.arange(n - new, n)[:, None]
+    args = (torch.arange(pages, dtype=torch.int32, device=cuda)[None], _i32([n], cuda), _i32([0, new], cuda), 1.0)
+    half = _HALF_STEP[dtype]
+    for sign in (torch.ones_like(signs), signs):
+        vc = (sign * most).to(dtype)
+        got = P.paged_attention(q.to(cuda), kc.to(dtype).to(cuda).view(pages, page, 1, dim), vc.to(cuda).view(pages, page, 1, dim), *args).double().cpu()
+        for h in range(heads):
+            want, size = _plain_attention(q[:, h].double(), kc[:n, 0].double(), vc[:n, 0].double(), visible, 1.0, None)
+            # logits are exact; weights and sums as in _attention_case
+            bound = want.abs() * half + size * ((half if dtype != torch.float32 else 0.0) + (2 * n + 32) * 2.0 ** -24)
+            assert bool(((got[:, h] - want).abs() <= 1.001 * bound).all()), (h, float(got[:, h].abs().max()))
+
+
 def test_attention_offsets_beyond_32_bits(cuda):
     """Pages whose elements start past 2^31."""
     page, heads, dim, pages = 16, 8, 128, 2 ** 31 // (16 * 8 * 128) + 40
