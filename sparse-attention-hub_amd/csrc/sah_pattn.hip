@@ -652,8 +652,8 @@ __global__ __launch_bounds__((pa_shape<DT, DP, WIDE>::NT), (pa_shape<DT, DP, WID
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[t][e] *= up;
       }
-      // (a row that has seen nothing: kept in range, so that -inf comes to 0)
-      mc = fmaxf(m_run, -1e37f) - pa_weights<DT>::SCALE;
+      // (a row that has seen nothing: in range, so that -inf comes to 0)
+      mc = (m_run == -INFINITY ? 0.f : m_run) - pa_weights<DT>::SCALE;
       auto weigh = [&](int t, int e0, int n) __attribute__((always_inline)) {  // n of a key tile's weights
 #pragma unroll
           for (int e = e0; e < e0 + n; ++e) {

@@ -534,6 +534,27 @@ def test_averages_of_the_largest_values_are_finite(cuda, dtype, new, n):
             assert bool(((got[:, h] - want).abs() <= 1.001 * bound).all()), (h, float(got[:, h].abs().max()))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("new, n", [(1, 700), (40, 700), (1, 9001)])
+def test_logits_far_below_zero_are_logits(cuda, dtype, new, n):
+    """Every logit is one and the same number of -1e36 to -1e38: a row is the average of what it sees."""
+    page, dim, heads = 16, 64, 4
+    g = torch.Generator().manual_seed(n)
+    pages = -(-n // page)
+    q, kc = torch.zeros(new, heads, dim), torch.zeros(pages * page, 1, dim)
+    q[:, :, 0] = torch.tensor([2.0 ** 60, 2.0 ** 61, 2.0 ** 63, 2.0 ** 66])
+    kc[:, :, 0] = -2.0 ** 60
+    vc = torch.randn(pages * page, 1, dim, generator=g).to(dtype)
+    got = P.paged_attention(q.to(dtype).to(cuda), kc.to(dtype).to(cuda).view(pages, page, 1, dim), vc.to(cuda).view(pages, page, 1, dim),
+                            torch.arange(pages, dtype=torch.int32, device=cuda)[None], _i32([n], cuda), _i32([0, new], cuda), 1.0).double().cpu()
+    visible = torch.arange(n)[None] <= torch.arange(n - new, n)[:, None]
+    want, size = _plain_attention(torch.zeros(new, dim).double(), torch.zeros(n, dim).double(), vc[:n, 0].double(), visible, 1.0, None)
+    half = _HALF_STEP[dtype]
+    # equal weights are exact; sums of n of them, and the result's rounding
+    bound = want.abs() * half + size * (2 * n + 16) * 2.0 ** -24
+    assert bool(((got - want[:, None]).abs() <= 1.001 * bound[:, None]).all())
+
+
 def test_attention_offsets_beyond_32_bits(cuda):
     """Pages whose elements start past 2^31."""
     page, heads, dim, pages = 16, 8, 128, 2 ** 31 // (16 * 8 * 128) + 40
