@@ -4,7 +4,7 @@
  * there. Conventions and error codes are sah.h's.
  *
  * The cache: K and V of one layer are n_pages pages of page_size tokens each, addressed by element strides (page, token,
- * head; innermost 1). Request b's token at position p lies in page block_table[b][p / page_size], entry p % page_size; the
+ * head; innermost 1; of a dimension of one entry any number). Request b's token at position p lies in page block_table[b][p / page_size], entry p % page_size; the
  * number page * page_size + entry is its slot. A page number outside [0, n_pages) stands for no page: nothing is read or
  * written there, and the keys it would hold are not there. Several layers share one table.
  *

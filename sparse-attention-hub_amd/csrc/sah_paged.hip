@@ -249,8 +249,15 @@ extern "C" int sah_paged_release(const sah_paged_release_args* a) {
   return sah_launch_status("sah_paged_release(pages)");
 }
 
-extern "C" int sah_paged_store(const sah_paged_store_args* a) {
-  if (!a) return sah_fail(SAH_ENULL, "sah_paged_store: args is NULL");
+extern "C" int sah_paged_store(const sah_paged_store_args* given) {
+  if (!given) return sah_fail(SAH_ENULL, "sah_paged_store: args is NULL");
+  sah_paged_store_args own = *given;
+  const sah_paged_store_args* a = &own;
+  // a dimension of one entry has no stride, whatever it is said to be
+  if (own.n_tokens == 1) own.ks_t = own.vs_t = 0;
+  if (own.Hkv == 1) own.ks_h = own.vs_h = own.kcs_h = own.vcs_h = 0;
+  if (own.n_pages == 1) own.kcs_p = own.vcs_p = 0;
+  if (own.page_size == 1) own.kcs_t = own.vcs_t = 0;
   if (a->dtype != SAH_F32 && a->dtype != SAH_BF16 && a->dtype != SAH_F16) return sah_fail(SAH_EDTYPE, "sah_paged_store: dtype %d", a->dtype);
   if (a->n_tokens < 0 || a->Hkv <= 0 || a->D <= 0 || a->n_pages <= 0 || a->page_size <= 0)
     return sah_fail(SAH_EINVAL, "sah_paged_store: Hkv, D, n_pages and page_size must be > 0, n_tokens >= 0");

@@ -1148,8 +1148,16 @@ extern "C" int64_t sah_paged_attention_work_floats(const sah_paged_attention_arg
   return pa_dispatch(a, pa_floats_fn());
 }
 
-extern "C" int sah_paged_attention(const sah_paged_attention_args* a) {
-  if (!a) return sah_fail(SAH_ENULL, "sah_paged_attention: args is NULL");
+extern "C" int sah_paged_attention(const sah_paged_attention_args* given) {
+  if (!given) return sah_fail(SAH_ENULL, "sah_paged_attention: args is NULL");
+  sah_paged_attention_args own = *given;
+  const sah_paged_attention_args* a = &own;
+  // a dimension of one entry has no stride, whatever it is said to be
+  if (own.n_tokens == 1) own.qs_t = own.os_t = 0;
+  if (own.Hq == 1) own.qs_h = own.os_h = 0;
+  if (own.Hkv == 1) own.ks_h = own.vs_h = 0;
+  if (own.n_pages == 1) own.ks_p = own.vs_p = 0;
+  if (own.page_size == 1) own.ks_t = own.vs_t = own.D;
   if (a->dtype != SAH_F32 && a->dtype != SAH_BF16 && a->dtype != SAH_F16) return sah_fail(SAH_EDTYPE, "sah_paged_attention: dtype %d", a->dtype);
   if (a->n_requests <= 0 || a->n_tokens < 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->n_pages <= 0 || a->table_width <= 0 ||
       a->max_context < 0 || a->sink < 0 || a->window < 0)

@@ -52,7 +52,7 @@ def _check_table(block_table: torch.Tensor, n_requests: int, device: torch.devic
         raise ValueError(f"block_table must be int32 on {device}, got {block_table.dtype} on {block_table.device}")
     if block_table.dim() != 2 or block_table.shape[0] != n_requests or block_table.shape[1] == 0:
         raise ValueError(f"block_table must have shape ({n_requests}, pages), got {tuple(block_table.shape)}")
-    if block_table.stride(1) != 1 or (n_requests > 1 and block_table.stride(0) < block_table.shape[1]):
+    if (block_table.stride(1) != 1 and block_table.shape[1] > 1) or (n_requests > 1 and block_table.stride(0) < block_table.shape[1]):
         raise ValueError("block_table's rows must be contiguous and apart")
 
 
@@ -67,7 +67,7 @@ def _check_cache(key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
                          f"{tuple(key_cache.shape)} and {tuple(value_cache.shape)}")
     if value_cache.device != key_cache.device or value_cache.dtype != key_cache.dtype:
         raise ValueError("key_cache and value_cache must be of one type on one device")
-    if key_cache.stride(3) != 1 or value_cache.stride(3) != 1:
+    if key_cache.shape[3] > 1 and (key_cache.stride(3) != 1 or value_cache.stride(3) != 1):
         raise ValueError("the caches' innermost stride must be 1")
 
 
@@ -144,7 +144,7 @@ def store_paged(keys: torch.Tensor, values: torch.Tensor, key_cache: torch.Tenso
             raise ValueError(f"{what} must be {dtype} on {device}, got {t.dtype} on {t.device}")
         if t.shape != rows:
             raise ValueError(f"{what} must have shape (n_tokens, {heads}, {dim}), got {tuple(t.shape)}")
-        if t.stride(2) != 1:
+        if t.stride(2) != 1 and dim > 1:
             raise ValueError(f"{what}: the innermost stride must be 1")
     _check(slot_map, "slot_map", torch.int64, rows[0], device)
     N.call_on(device, "sah_paged_store", N.PagedStoreArgs(

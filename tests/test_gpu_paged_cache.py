@@ -555,6 +555,26 @@ def test_logits_far_below_zero_are_logits(cuda, dtype, new, n):
     assert bool(((got - want[:, None]).abs() <= 1.001 * bound[:, None]).all())
 
 
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("page", [1, 64])
+def test_strides_of_dimensions_of_one_entry_are_nothing(cuda, dtype, page):
+    """One token, one page, one key head: their strides may be any number, as views of such tensors have them."""
+    dim, heads, n = 64, 4, page
+    g = torch.Generator(device=cuda).manual_seed(page)
+    k, v, q = (torch.randn(m, h, dim, generator=g, device=cuda).to(dtype) for m, h in ((n, 1), (n, 1), (1, heads)))
+    q = q.as_strided((1, heads, dim), (heads * dim + 3, dim, 1))
+    caches = [torch.zeros(page * dim, dtype=dtype, device=cuda).as_strided((1, page, 1, dim), (7, dim if page > 1 else 5, 3, 1)) for _ in range(2)]
+    for t in range(n):
+        one = (x[t:t + 1].as_strided((1, 1, dim), (1, 1, 1)) for x in (k, v))
+        P.store_paged(*one, *caches, torch.tensor([t], device=cuda))
+    assert torch.equal(caches[0].reshape(n, dim), k[:, 0]) and torch.equal(caches[1].reshape(n, dim), v[:, 0])
+    table, kv, cu = _i32([0, 7, 7], cuda).as_strided((1, 1), (3, 2)), _i32([n], cuda), _i32([0, 1], cuda)
+    out = torch.empty(heads * dim, dtype=dtype, device=cuda).as_strided((1, heads, dim), (9, dim, 1))
+    P.paged_attention(q, *caches, table, kv, cu, 0.125, out=out)
+    want = P.paged_attention(q.contiguous(), k[None].contiguous(), v[None].contiguous(), table, kv, cu, 0.125)
+    assert torch.equal(out, want)
+
+
 def test_attention_offsets_beyond_32_bits(cuda):
     """Pages whose elements start past 2^31."""
     page, heads, dim, pages = 16, 8, 128, 2 ** 31 // (16 * 8 * 128) + 40

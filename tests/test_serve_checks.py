@@ -108,6 +108,17 @@ def test_attention_refuses(changes, code):
     assert _call("sah_paged_attention", _changed(args, changes)) == code
 
 
+@pytest.mark.parametrize("changes", [
+    dict(n_tokens=1, qs_t=257, os_t=3), dict(n_pages=1, ks_p=2049, vs_p=-1), dict(page_size=1, ks_t=2 ** 40 + 1, vs_t=-3),
+    dict(Hq=1, Hkv=1, qs_h=65, ks_h=3, vs_h=5, os_h=-1),
+])
+def test_attention_takes_any_stride_of_a_dimension_of_one_entry(changes):
+    """Such a dimension's stride is no address: what is refused is the workspace that is not given."""
+    args = N.PagedAttentionArgs(_PTR, 256, 64, _PTR, 2048, 128, 64, _PTR, 2048, 128, 64, _PTR, 4, 4, _PTR, _PTR, None, 1, 2, 3, 4, 2, 64, 8, 16,
+                                0, 0, 0, 0.125, _PTR, 256, 64, None, 0, None)
+    assert _call("sah_paged_attention", _changed(args, changes)) == -4
+
+
 @pytest.mark.parametrize("changes, code", [
     (dict(dtype=7), -5), (dict(n_rows=-1), -1), (dict(vocab=0), -1), (dict(vocab=2 ** 20 + 1, row_pitch=2 ** 21), -3), (dict(row_pitch=99), -1),
     (dict(logits=None), -2), (dict(uniforms=None), -2), (dict(tokens=None), -2),
