@@ -48,8 +48,9 @@ typedef struct sah_paged_assign_args {
 int sah_paged_assign(const sah_paged_assign_args* a);
 
 /* Takes the pages of every request with finished[b] != 0 back: they are appended to free_pages (in the order of requests
- * and of their pages), *free_count grows, lens[b] becomes 0 and the request's entries of block_table -1. work: 2 *
- * n_requests words. */
+ * and of their pages), *free_count grows, lens[b] becomes 0 and the entries of block_table that its length takes -1. An entry below 0 is no
+ * page and is not appended; any other number is, whatever it is. Pages that a list of n_pages entries has no room for are lost. work:
+ * 2 * n_requests words. */
 typedef struct sah_paged_release_args {
   const uint8_t* finished;
   int32_t* lens;

@@ -114,7 +114,7 @@ def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, block_table: torch.
 def release_pages(finished: torch.Tensor, lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                   free_count: torch.Tensor, page_size: int) -> None:
     """Gives the pages of every request with `finished[b]` (bool) back to `free_pages`: its length becomes 0, its table entries -1,
-    and its row can serve another request."""
+    and its row can serve another request. Entries that are negative already (no page) are not given back."""
     N.require_device(finished, "finished")
     device, n = finished.device, finished.shape[0] if finished.dim() == 1 else -1
     _check(finished, "finished", torch.bool, None, device)

@@ -136,6 +136,37 @@ def test_assign_pages_of_no_tokens(cuda):
     assert lens.tolist() == [5, 0]
 
 
+@pytest.mark.parametrize("requests, page, pages_each, room", [
+    (1, 4, 3, 100), (1, 1, 5000, 10000), (3, 16, 2048, 10000), (7, 8, 40, 150), (300, 2, 20, 10000), (4096, 16, 3, 20000), (5, 1, 4500, 9000),
+])
+def test_release_pages_that_are_not_there_and_a_list_that_is_full(cuda, requests, page, pages_each, room):
+    """Entries below 0 inside a request's length are no pages: they are not handed out again. Where the list is full the rest is lost; the
+    requests' rows are empty all the same, and other rows as they were."""
+    rng = random.Random(requests)
+    width = pages_each + 2
+    held = [rng.randrange(0, pages_each + 1) for _ in range(requests)]
+    held[-1] = pages_each
+    lens = [n * page - rng.randrange(0, page) if n else 0 for n in held]
+    table = [[rng.choice((-1, -7, 5, 1000, 2 ** 31 - 1)) if rng.random() < 0.2 else rng.randrange(0, 10 ** 6) for _ in range(width)] for _ in range(requests)]
+    finished = [rng.random() < 0.6 for _ in range(requests)]
+    finished[-1] = True
+    if requests > 2:
+        lens[0], finished[0], finished[1] = -3, True, False  # a corrupt length
+    free, count = [-9] * room, 2
+    dev_lens, dev_table, dev_free, dev_count = _i32(lens, cuda), _i32(table, cuda), _i32(free, cuda), _i32([count], cuda)
+    P.release_pages(torch.tensor(finished, device=cuda), dev_lens, dev_table, dev_free, dev_count, page)
+    for b in range(requests):
+        if finished[b]:
+            for j in range(-(-max(lens[b], 0) // page)):
+                if table[b][j] >= 0 and count < room:
+                    free[count] = table[b][j]
+                    count += 1
+                table[b][j] = -1
+            lens[b] = 0
+    assert dev_count.tolist() == [count] and dev_free.tolist() == free
+    assert dev_lens.tolist() == lens and dev_table.tolist() == table
+
+
 # -------------------------------------------------------------------------------------------------------------------- store
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("tokens, heads, dim, page, layout", [
