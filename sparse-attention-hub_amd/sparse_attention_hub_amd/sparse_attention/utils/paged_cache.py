@@ -56,6 +56,11 @@ def _check_table(block_table: torch.Tensor, n_requests: int, device: torch.devic
         raise ValueError("block_table's rows must be contiguous and apart")
 
 
+def _check_page_size(page_size: int) -> None:
+    if not 1 <= page_size < 2 ** 31:  # (a wider number would lose its upper half on the way to the kernels)
+        raise ValueError(f"page_size must be in [1, 2^31), got {page_size}")
+
+
 def _pitch(block_table: torch.Tensor) -> int:
     return max(block_table.stride(0), block_table.shape[1])  # one row: its stride says nothing
 
@@ -96,6 +101,7 @@ def assign_pages(new_lens: torch.Tensor, lens: torch.Tensor, block_table: torch.
     _check(free_count, "free_count", torch.int32, 1, device)
     _check(free_count_out, "free_count_out", torch.int32, 1, device)
     _check_table(block_table, n, device)
+    _check_page_size(page_size)
     if not 0 <= n_tokens <= 2 ** 30:
         raise ValueError(f"n_tokens must be in [0, 2^30], got {n_tokens}")
     slot_map = torch.empty(n_tokens, dtype=torch.int64, device=device)
@@ -124,6 +130,7 @@ def release_pages(finished: torch.Tensor, lens: torch.Tensor, block_table: torch
     _check(free_pages, "free_pages", torch.int32, None, device)
     _check(free_count, "free_count", torch.int32, 1, device)
     _check_table(block_table, n, device)
+    _check_page_size(page_size)
     work = torch.empty(2 * n, dtype=torch.int32, device=device)
     N.call_on(device, "sah_paged_release", N.PagedReleaseArgs(
         finished.data_ptr(), lens.data_ptr(), block_table.data_ptr(), _pitch(block_table), block_table.shape[1],

@@ -669,6 +669,16 @@ def test_tensors_that_do_not_fit_together_are_refused(cuda):
             P.paged_attention(**dict(good, **bad))
 
 
+@pytest.mark.parametrize("page_size", [0, -16, 2 ** 31, 2 ** 32 + 16])
+def test_page_sizes_that_do_not_fit_are_refused(cuda, page_size):
+    i32, table, free = (torch.zeros(s, dtype=torch.int32, device=cuda) for s in (2, (2, 4), 8))
+    with pytest.raises(ValueError, match="page_size"):
+        P.assign_pages(i32, i32, table, free, i32[:1], page_size, 3)
+    with pytest.raises(ValueError, match="page_size"):
+        P.release_pages(torch.ones(2, dtype=torch.bool, device=cuda), i32, table, free, i32[:1], page_size)
+    assert not any(t.any() for t in (i32, table, free))
+
+
 # ------------------------------------------------------------------------------------------------------ as they are used
 def _dense_reference(q, k, v, scaling):
     """One request in 64 bits: the last len(q) positions' attention over all keys; (n, heads, dim) each."""
