@@ -21,8 +21,8 @@ def _setting(value: Setting, what: str, off: float, dtype: torch.dtype, rows: in
     if not isinstance(value, torch.Tensor):
         if value != value:
             raise ValueError(f"{what} is NaN")
-        if dtype == torch.int32 and not -2 ** 31 <= value < 2 ** 31:
-            raise ValueError(f"{what} must fit 32 bits, got {value}")
+        if dtype == torch.int32 and not (value == value // 1 and -2 ** 31 <= value < 2 ** 31):
+            raise ValueError(f"{what} must be a whole number that fits 32 bits, got {value}")
         return None, int(value) if dtype == torch.int32 else float(value)
     if value.device != device or value.dtype != dtype or value.shape != (rows,) or not value.is_contiguous():
         raise ValueError(f"{what} must be a number or a contiguous {dtype} tensor of {rows} values on {device}, got {value.dtype} "

@@ -276,3 +276,11 @@ def test_tensors_that_do_not_fit_are_refused(cuda):
                 dict(temperature=math.nan), dict(top_k=2 ** 31), dict(logits=x[:, :0]), dict(logits=x[:1].expand(3, 10))):
         with pytest.raises(ValueError):
             sample_tokens(**dict(dict(logits=x, uniforms=u), **bad))
+
+
+@pytest.mark.parametrize("top_k", [1.5, 0.5, -0.1, math.inf, -math.inf, 2.0 ** 31, 10 ** 30])
+def test_numbers_that_are_no_count_are_refused(cuda, top_k):
+    x, u = torch.zeros(3, 10, device=cuda), torch.zeros(3, device=cuda)
+    with pytest.raises(ValueError, match="whole number"):
+        sample_tokens(x, u, top_k=top_k)
+    assert sample_tokens(x, u, top_k=4.0)[0].tolist() == sample_tokens(x, u, top_k=4)[0].tolist()
