@@ -84,7 +84,8 @@ int sah_paged_store(const sah_paged_store_args* a);
  * denominator. A row that sees nothing is 0. Rows of q behind the last request's are not read and their output is left as it
  * was. Lengths beyond table_width pages count as that many. out [n_tokens, Hq, D]. max_context: about how long the longest
  * request is (0: not known); it decides how work is split, never what is computed. page_size: a power of two; table_width *
- * page_size below 2^31 - 4096. Rows of out share no memory with each other or with what is read.
+ * page_size below 2^31 - 4096. Rows of out share no memory with each other or with what is read (refused, as
+ * is an out whose rows lie between those of a cache, or between q's with another qs_t than os_t).
  * work: sah_paged_attention_work_floats(a) floats, no particular content. */
 typedef struct sah_paged_attention_args {
   const void* q; int64_t qs_t, qs_h;

@@ -172,7 +172,8 @@ def paged_attention(queries: torch.Tensor, key_cache: torch.Tensor, value_cache:
     groups, as `repeat_kv` would have it. A row that sees nothing is 0; rows behind the last request's keep what `out` held (without
     `out`: unspecified). `max_context`, about the longest request's length, decides how work is split (default: the
     table's width); results do not depend on it beyond the order of sums. head_dim a multiple of 8 up to 256, page_size a power of two,
-    addresses and strides multiples of 16 bytes; `out` shares no memory with the other tensors. Returns `(n_tokens, heads, head_dim)`.
+    addresses and strides multiples of 16 bytes; `out` shares no memory with the other tensors (refused; it and
+    the queries may be slices of one buffer, their tokens equally far apart). Returns `(n_tokens, heads, head_dim)`.
     """
     _check_cache(key_cache, value_cache)
     device = key_cache.device

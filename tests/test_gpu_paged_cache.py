@@ -679,6 +679,38 @@ def test_page_sizes_that_do_not_fit_are_refused(cuda, page_size):
     assert not any(t.any() for t in (i32, table, free))
 
 
+@pytest.mark.parametrize("layout", ["beside", "interleaved", "heads_first", "same", "shifted", "cache"])
+def test_output_and_queries_of_one_buffer(cuda, layout):
+    """Slices that share nothing are what they are apart; what shares memory is refused."""
+    tokens, heads, dim, page, n = 5, 4, 64, 16, 90
+    g = torch.Generator(device=cuda).manual_seed(2)
+    kc, vc = (torch.randn(6, page, heads, dim, generator=g, device=cuda) for _ in range(2))
+    q = torch.randn(tokens, heads, dim, generator=g, device=cuda)
+    args = (kc, vc, torch.arange(6, dtype=torch.int32, device=cuda)[None], _i32([n], cuda), _i32([0, tokens], cuda), 0.125)
+    want = P.paged_attention(q, *args)
+    if layout == "beside":
+        queries, out = torch.zeros(tokens, 3 * heads, dim, device=cuda).split([heads, 2 * heads], dim=1)
+        out = out[:, heads:]
+    elif layout == "interleaved":
+        queries, out = torch.zeros(tokens, heads, 2 * dim, device=cuda).split(dim, dim=2)
+    elif layout == "heads_first":
+        queries, out = torch.zeros(2 * heads, tokens, dim, device=cuda).transpose(0, 1).split(heads, dim=1)
+    elif layout == "same":
+        queries = out = q.clone()
+    elif layout == "shifted":
+        both = torch.zeros(tokens + 1, heads, dim, device=cuda)
+        queries, out = both[:tokens], both[1:]
+    else:
+        queries, out = q.clone(), kc[0, :tokens]
+    queries.copy_(q)
+    if layout in ("same", "shifted", "cache"):
+        with pytest.raises(ValueError, match="sah_paged_attention: out"):
+            P.paged_attention(queries, *args, out=out)
+        return
+    assert P.paged_attention(queries, *args, out=out) is out
+    assert torch.equal(out, want) and torch.equal(queries, q)
+
+
 # ------------------------------------------------------------------------------------------------------ as they are used
 def _dense_reference(q, k, v, scaling):
     """One request in 64 bits: the last len(q) positions' attention over all keys; (n, heads, dim) each."""

@@ -119,6 +119,23 @@ def test_attention_takes_any_stride_of_a_dimension_of_one_entry(changes):
     assert _call("sah_paged_attention", _changed(args, changes)) == -4
 
 
+_FAR = 2 ** 40  # no two of these addresses are near each other, and none is dereferenced
+
+
+@pytest.mark.parametrize("changes, what", [
+    (dict(out=_FAR), b"with q"), (dict(out=_FAR + 2 * 256 * 2), b"with q"), (dict(out=_FAR - 2 * 256 * 2), b"with q"),
+    (dict(out=_FAR + 3 * 64 * 2), b"with q"), (dict(out=_FAR + 112), b"with q"), (dict(out=_FAR, os_h=192, os_t=64, qs_h=192, qs_t=64), b"with q"),
+    (dict(out=_FAR + 64 * 2, os_t=512), b"with q"), (dict(out=_FAR + 128, n_tokens=1), b"with q"),
+    (dict(out=2 * _FAR), b"within"), (dict(out=2 * _FAR + 8 * 2048 * 2 - 16), b"within"), (dict(out=3 * _FAR - 16), b"within"),
+    (dict(out=4 * _FAR + 16), b"within"), (dict(out=5 * _FAR), b"within"), (dict(out=6 * _FAR), b"within"), (dict(out=7 * _FAR - 256), b"within"),
+])
+def test_attention_refuses_an_output_on_what_is_read(changes, what):
+    args = N.PagedAttentionArgs(_FAR, 256, 64, 2 * _FAR, 2048, 128, 64, 3 * _FAR, 2048, 128, 64, 4 * _FAR, 4, 4, 5 * _FAR, 6 * _FAR, 7 * _FAR, 1, 2, 3, 4, 2,
+                                64, 8, 16, 0, 0, 0, 0.125, 8 * _FAR, 256, 64, 9 * _FAR, 2 ** 40, None)
+    assert _call("sah_paged_attention", _changed(args, changes)) == -1
+    assert what in N.lib().sah_last_error()
+
+
 @pytest.mark.parametrize("changes, code", [
     (dict(dtype=7), -5), (dict(n_rows=-1), -1), (dict(vocab=0), -1), (dict(vocab=2 ** 20 + 1, row_pitch=2 ** 21), -3), (dict(row_pitch=99), -1),
     (dict(logits=None), -2), (dict(uniforms=None), -2), (dict(tokens=None), -2),
