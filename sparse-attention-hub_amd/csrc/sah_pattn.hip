@@ -1087,12 +1087,6 @@ static bool pa_wide(const sah_paged_attention_args* a) {
   return tiles > (rows <= 64 * n ? 2 * PA_CUS : rows <= 128 * n ? PA_CUS / 4 : 0);
 }
 
-template <int DT, int DP, bool WIDE>
-static int64_t pa_floats() {
-  typedef pa_shape<DT, DP, WIDE> S;
-  return S::WGS * (int64_t)(sizeof(pa_note) / 4) + 2 * (int64_t)S::WGS * S::SLOT;
-}
-
 // About as many workgroups as the call has work for, at most what the card holds at once: a short call's idle ones, and theirs of the
 // second kernel, cost it 0.3 to 0.6 us of 17. Only how the work is shared depends on it.
 template <typename S>
@@ -1104,6 +1098,13 @@ static int pa_workgroups(const sah_paged_attention_args* a) {
   const double tiles = ((double)a->n_tokens * G / S::ROWS + a->n_requests) * a->Hkv;
   const double n = tiles * (double)(keys + S::TILE_COST) / S::LEAST;
   return n < S::WGS ? ((int)n / PA_XCDS + 1) * PA_XCDS : S::WGS;
+}
+
+// notes for all workgroups that fit the card, two parts for each that is launched
+template <int DT, int DP, bool WIDE>
+static int64_t pa_floats(const sah_paged_attention_args* a) {
+  typedef pa_shape<DT, DP, WIDE> S;
+  return S::WGS * (int64_t)(sizeof(pa_note) / 4) + 2 * (int64_t)pa_workgroups<S>(a) * S::SLOT;
 }
 
 template <int DT, int DP, bool WIDE>
@@ -1136,7 +1137,8 @@ static int64_t pa_dispatch(const sah_paged_attention_args* a, F f) {
   return f.template operator()<SAH_F32, 256, false>();
 }
 struct pa_floats_fn {
-  template <int DT, int DP, bool WIDE> int64_t operator()() const { return pa_floats<DT, DP, WIDE>(); }
+  const sah_paged_attention_args* a;
+  template <int DT, int DP, bool WIDE> int64_t operator()() const { return pa_floats<DT, DP, WIDE>(a); }
 };
 struct pa_launch_fn {
   const sah_paged_attention_args* a;
@@ -1144,8 +1146,10 @@ struct pa_launch_fn {
 };
 
 extern "C" int64_t sah_paged_attention_work_floats(const sah_paged_attention_args* a) {
-  if (!a || a->n_tokens <= 0 || a->n_requests <= 0 || a->Hkv <= 0 || a->Hq < a->Hkv || a->D <= 0 || a->D > PA_MAX_D) return 0;
-  return pa_dispatch(a, pa_floats_fn());
+  if (!a || a->n_tokens <= 0 || a->n_requests <= 0 || a->Hkv <= 0 || a->Hq < a->Hkv || a->D <= 0 || a->D > PA_MAX_D || a->table_width <= 0 ||
+      a->page_size <= 0)
+    return 0;
+  return pa_dispatch(a, pa_floats_fn{a});
 }
 
 // From a tensor's first byte to behind its last one, judged by strides (elements) and counts

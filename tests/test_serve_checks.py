@@ -146,6 +146,22 @@ def test_sampling_refuses(changes, code):
     assert _call("sah_sample_tokens", _changed(args, changes)) == code
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_workspaces_follow_the_work(dtype, dim):
+    """What a call needs grows with its work up to a full card's, and a short one does not hold that."""
+    def floats(tokens, context, requests=1):
+        args = N.PagedAttentionArgs(dtype=dtype, n_requests=requests, n_tokens=tokens, Hq=8, Hkv=2, D=dim, n_pages=100, page_size=16, table_width=2 ** 14,
+                                    table_pitch=2 ** 14, max_context=context)
+        return N.paged_work_floats(args)
+
+    full = floats(8192, 0)
+    assert 0 < floats(1, 100) <= floats(1, 1000) <= floats(1, 10000) <= floats(16, 100000)
+    assert floats(70, 70) * 10 < full and floats(1, 100) * 4 < 2 ** 20
+    # a length that is not known counts as the table's, and neither more requests nor longer ones need more than a full card
+    assert floats(8192, 10 ** 9) == full == floats(8192, 2 ** 18) == floats(8192, 2 ** 18, 64)
+
+
 def test_nothing_to_do_is_no_error():
     lib = N.lib()
     assert lib.sah_paged_store(ctypes.byref(N.PagedStoreArgs(Hkv=1, D=8, n_pages=1, page_size=1))) == 0
