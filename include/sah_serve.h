@@ -82,7 +82,7 @@ int sah_paged_store(const sah_paged_store_args* a);
  * p = kv_lens[b] - (cu_new[b + 1] - cu_new[b]) + i and sees the keys j <= p of its request, with window > 0 those of them with
  * j < sink or j > p - window (the Sink and Local maskers' columns). sinks, optional [Hq]: a logit per head in the softmax's
  * denominator. A row that sees nothing is 0. Rows of q behind the last request's are not read and their output is left as it
- * was. Lengths beyond table_width pages count as that many. out [n_tokens, Hq, D]. max_context: about how long the longest
+ * was. Keys beyond table_width pages are not there; positions, and so windows, go by kv_lens all the same. out [n_tokens, Hq, D]. max_context: about how long the longest
  * request is (0: not known); it decides how work is split, never what is computed. page_size: a power of two; table_width *
  * page_size below 2^31 - 4096. Rows of out share no memory with each other or with what is read (refused, as
  * is an out whose rows lie between those of a cache, or between q's with another qs_t than os_t).

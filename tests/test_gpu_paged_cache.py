@@ -641,6 +641,26 @@ def test_attention_of_lengths_that_do_not_fit_is_bounded(cuda):
         assert torch.isfinite(out.float()).all()
 
 
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("sink, window", [(0, 0), (4, 950), (4, 920), (0, 937), (4, 900), (0, 100), (64, 1), (1, 2000)])
+def test_windows_of_lengths_beyond_the_table(cuda, dtype, sink, window):
+    """Positions go by the length, keys end with the table: a window may see a few of them, or the sinks alone, or nothing."""
+    page, held, length, new, heads, dim = 16, 64, 1000, 3, 4, 64
+    g = torch.Generator().manual_seed(window)
+    q, k, v = (torch.randn(m, h, dim, generator=g).to(dtype) for m, h in ((new, heads), (held, 1), (held, 1)))
+    got = P.paged_attention(q.to(cuda), k.view(-1, page, 1, dim).to(cuda), v.view(-1, page, 1, dim).to(cuda),
+                            torch.arange(held // page, dtype=torch.int32, device=cuda)[None], _i32([length], cuda), _i32([0, new], cuda), 0.125,
+                            sink_size=sink if window else 0, window_size=window).double().cpu()
+    position, j = torch.arange(length - new, length)[:, None], torch.arange(held)[None]
+    visible = ((j < sink) | (j > position - window)) if window else torch.ones(new, held, dtype=torch.bool)
+    half = _HALF_STEP[dtype]
+    for h in range(heads):
+        want, size = _plain_attention(q[:, h].double(), k[:, 0].double(), v[:, 0].double(), visible, 0.125, None)
+        bound = want.abs() * half + size * (half + 2.0 ** -16)  # (fp32 terms of _attention_case: less than the last)
+        assert bool(((got[:, h] - want).abs() <= bound).all())
+        assert bool(got[:, h][~visible.any(1)].eq(0).all())
+
+
 # ------------------------------------------------------------------------------------------------- refusals on the device
 def test_tensors_that_do_not_fit_together_are_refused(cuda):
     i32 = torch.zeros(2, dtype=torch.int32, device=cuda)
