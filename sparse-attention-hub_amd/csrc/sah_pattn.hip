@@ -276,7 +276,8 @@ __device__ __forceinline__ pa_piece pa_start(pa_args& P, int w, int64_t* s_sum) 
   }
   return r;
 }
-;// what a workgroup leaves for the second kernel
+
+// what a workgroup leaves for the second kernel
 struct pa_note {
   int b, hk, tile;  // the tile it began and others went on with; b < 0: none
   int last;         // the workgroup that ended it
