@@ -527,8 +527,8 @@ def cold_probe(dev) -> dict:
 def hw_probe(dev) -> dict:
     """What the GPU gives to two patterns of the library (the bench-only object `bench_hw_probe.so`, built from
     `bench_hw_probe.hip` beside this file; HIP events around back-to-back launches): a 4 GiB read stream alone and with
-    1/32 of its volume written back (the exact-score pass over K at config 5), and matrix / vector / interleaved
-    instruction streams (the Lloyd assignment)."""
+    1/32 of its volume written back (the exact-score pass over K at config 5), matrix / vector / interleaved
+    instruction streams (the Lloyd assignment), and fp64 ones (the weights of the token sampling)."""
     import ctypes
 
     import torch
@@ -566,13 +566,13 @@ def hw_probe(dev) -> dict:
     for kind in (0, 1, 2, 0):
         us = timed((kind, src.data_ptr(), n, dst.data_ptr(), dst.numel(), 0, 0, stream), 10)
         out.setdefault(names[kind], []).append({"us": round(us, 1), "read_TBps": round(n / us / 1e6, 3)})
-    names = {3: "matrix_only", 4: "vector_only", 5: "matrix_and_vector_interleaved"}
+    names = {3: "matrix_only", 4: "vector_only", 5: "matrix_and_vector_interleaved", 6: "vector_fp64_only"}
     for wgs in (256, 1024):
-        for kind in (3, 4, 5):
+        for kind in (3, 4, 5, 6):
             us = timed((kind, None, 0, dst.data_ptr(), dst.numel(), 2000, wgs, stream), 5)
             out[f"{names[kind]}_{wgs // 256}_waves_per_simd_us"] = round(us, 1)
     out["note"] = ("stream kinds: 65536 workgroups x 64 KB, non-temporal 16-byte loads; issue kinds: 2000 iterations of 4 dependent "
-                   "32x32x2 fp32 matrix instructions and / or 48 vector FMAs per wave")
+                   "32x32x2 fp32 matrix instructions and / or 48 vector FMAs (fp32, fp64) per wave")
     return out
 
 

@@ -7,9 +7,10 @@
 //   kind 2  the same volume written as one 512-byte store per 16 KB;
 //   kind 3  `workgroups` workgroups of 4 waves, `iters` iterations of four dependent 32x32x2 fp32 matrix instructions;
 //   kind 4  the same loop with 48 vector instructions instead;
-//   kind 5  both, interleaved.
+//   kind 5  both, interleaved;
+//   kind 6  kind 4 with fp64 instructions (the weights of the token sampling).
 // Returns 0, or -1 for arguments outside these bounds: bytes a multiple of 65536, dst_bytes >= bytes / 32 (kinds
-// 0-2; kind 0 writes nothing) or >= 4 (kinds 3-5), iters in [1, 16384], workgroups in [1, 4096].
+// 0-2; kind 0 writes nothing) or >= 4 (kinds 3-6), iters in [1, 16384], workgroups in [1, 4096].
 #include <hip/hip_runtime.h>
 #include <cstdint>
 
@@ -72,6 +73,17 @@ __global__ __launch_bounds__(PR_NT, 2) void k_probe_issue(float* out, int iters,
   if (r == 12345.678f) out[0] = r;
 }
 
+// kind 6: 48 fp64 FMAs per iteration on four dependent chains
+__global__ __launch_bounds__(PR_NT, 2) void k_probe_issue64(float* out, int iters, double a, double b) {
+  double v0 = a + threadIdx.x, v1 = b, v2 = a + 1.0, v3 = b + 1.0;
+  for (int it = 0; it < iters; ++it) {
+#pragma unroll
+    for (int s = 0; s < 12; ++s) { v0 = fma(v0, a, b); v1 = fma(v1, a, b); v2 = fma(v2, a, b); v3 = fma(v3, a, b); }
+  }
+  const double r = v0 + v1 + v2 + v3;
+  if (r == 12345.678) out[0] = (float)r;
+}
+
 extern "C" int bench_hw_probe(int kind, const void* src, int64_t bytes, void* dst, int64_t dst_bytes, int iters,
                               int workgroups, void* stream) {
   hipStream_t st = (hipStream_t)stream;
@@ -87,12 +99,13 @@ extern "C" int bench_hw_probe(int kind, const void* src, int64_t bytes, void* ds
     else hipLaunchKernelGGL(k_probe_stream<2>, g, blk, 0, st, (const char*)src, (char*)dst, pitch);
     return hipGetLastError() == hipSuccess ? 0 : -2;
   }
-  if (kind >= 3 && kind <= 5) {
+  if (kind >= 3 && kind <= 6) {
     if (!dst || dst_bytes < 4) return -1;
     if (iters <= 0 || iters > (1 << 14) || workgroups <= 0 || workgroups > 4096) return -1;
     const dim3 g((unsigned)workgroups), blk(PR_NT);
     if (kind == 3) hipLaunchKernelGGL(k_probe_issue<3>, g, blk, 0, st, (float*)dst, iters, 1.0f, 0.5f);
     else if (kind == 4) hipLaunchKernelGGL(k_probe_issue<4>, g, blk, 0, st, (float*)dst, iters, 1.0f, 0.5f);
+    else if (kind == 6) hipLaunchKernelGGL(k_probe_issue64, g, blk, 0, st, (float*)dst, iters, 1.0, 0.5);
     else hipLaunchKernelGGL(k_probe_issue<5>, g, blk, 0, st, (float*)dst, iters, 1.0f, 0.5f);
     return hipGetLastError() == hipSuccess ? 0 : -2;
   }

@@ -20,8 +20,8 @@ extern "C" {
 /* Gives the new tokens of a step their places. Request b holds lens[b] tokens and gets new_lens[b] (negative: 0) more; the
  * pages it needs beyond those it has come off the end of the list free_pages[0 .. *free_count), request after request.
  * A request is granted all its tokens or none: none where lens[b] is negative, where its tokens would not fit into
- * table_width pages or into rows [0, n_tokens), and, among requests that need pages, from the first on for which the list is
- * too short (a request that needs no page is granted still).
+ * table_width pages or into rows [0, n_tokens) (behind requests that pass those rows also one without new tokens), and, among requests that
+ * need pages, from the first on for which the list is too short (a request that needs no page is granted still).
  * Outputs: cu_new [n_requests + 1], the running sum of all new_lens, granted or not, at most n_tokens; positions [n_tokens]
  * (lens[b] + i; 0 behind the last request's rows); slot_map [n_tokens] (-1 for a request that is not granted and behind the
  * last one's rows); granted [n_requests], 0 or 1; kv_lens [n_requests], what attention may see: lens[b] + new_lens[b], or 0

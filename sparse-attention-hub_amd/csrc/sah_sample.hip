@@ -11,10 +11,12 @@
 // be kept is known early, since where r of 1024 threads' own largest logits reach a value, at least r of the row do, and few
 // more. Where it cannot, the row is cut into pieces of 1 / SM_FINE in (m - x) / t first, and the list holds one of them.
 //
-// What bounds it: 256 rows of 150001 (fp32) are read once in 24.6 us (6.2 TB/s, the answer of greedy rows), and 65 us where every
-// weight is needed (all tokens): 22 fp64 instructions each, 8 cycles a wave. So a weight is taken where it is needed only: top-k 50 and
-// min-p 0.05 of a list 50 and 47 us; top-p 0.9 needs all of them once, for the sum, 110. The list saves the passes that follow (a row of 32000
-// in one workgroup: 13 us for top-k, 27 for top-p); a nucleus of more than 8192 tokens costs them (temperature 1.5: 178 us).
+// What bounds it, at 256 rows of 150001 (fp32, a workgroup each; greedy rows, read once, 24.6 us, 6.2 TB/s): the row is gone over twice, its
+// largest logit first. Top-k 50 and min-p 0.05 of a list take 50 and 47 us, two readings. A weight is 22 fp64 instructions (they issue as fast as
+// fp32 ones: 1.8 ns a wave and SIMD, profiles/hw_probe_stream_and_issue.txt) among some 30 in all, so it is taken where it is needed only:
+// for all tokens 69 us, of which vector instructions are 37; top-p 0.9 needs every weight too, for the sum, and its piece, an LDS
+// atomic: 115 us, 62 of instructions. The list saves the passes that follow (a row of 32000 in one workgroup: 13 us for top-k, 27 for top-p);
+// a nucleus of more than 8192 tokens costs them (temperature 1.5: 178 us).
 #include "sah_common.h"
 #include "../../include/sah_serve.h"
 
