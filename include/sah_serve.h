@@ -4,9 +4,10 @@
  * there. Conventions and error codes are sah.h's.
  *
  * The cache: K and V of one layer are n_pages pages of page_size tokens each, addressed by element strides (page, token,
- * head; innermost 1; of a dimension of one entry any number). Request b's token at position p lies in page block_table[b][p / page_size], entry p % page_size; the
- * number page * page_size + entry is its slot. A page number outside [0, n_pages) stands for no page: nothing is read or
- * written there, and the keys it would hold are not there. Several layers share one table.
+ * head; innermost 1; of a dimension of one entry any number). Request b's token at position p lies in page
+ * block_table[b][p / page_size], entry p % page_size; the number page * page_size + entry is its slot. A page number outside
+ * [0, n_pages) stands for no page: nothing is read or written there, and the keys it would hold are not there. Several layers
+ * share one table.
  *
  * One step: n_tokens rows of new tokens, request after request; request b's are rows cu_new[b] .. cu_new[b + 1] - 1. */
 #ifndef SAH_SERVE_H
@@ -20,8 +21,8 @@ extern "C" {
 /* Gives the new tokens of a step their places. Request b holds lens[b] tokens and gets new_lens[b] (negative: 0) more; the
  * pages it needs beyond those it has come off the end of the list free_pages[0 .. *free_count), request after request.
  * A request is granted all its tokens or none: none where lens[b] is negative, where its tokens would not fit into
- * table_width pages or into rows [0, n_tokens) (behind requests that pass those rows also one without new tokens), and, among requests that
- * need pages, from the first on for which the list is too short (a request that needs no page is granted still).
+ * table_width pages or into rows [0, n_tokens) (behind requests that pass those rows also one without new tokens), and, among
+ * requests that need pages, from the first on for which the list is too short (a request that needs no page is granted still).
  * Outputs: cu_new [n_requests + 1], the running sum of all new_lens, granted or not, at most n_tokens; positions [n_tokens]
  * (lens[b] + i; 0 behind the last request's rows); slot_map [n_tokens] (-1 for a request that is not granted and behind the
  * last one's rows); granted [n_requests], 0 or 1; kv_lens [n_requests], what attention may see: lens[b] + new_lens[b], or 0
@@ -48,9 +49,9 @@ typedef struct sah_paged_assign_args {
 int sah_paged_assign(const sah_paged_assign_args* a);
 
 /* Takes the pages of every request with finished[b] != 0 back: they are appended to free_pages (in the order of requests
- * and of their pages), *free_count grows, lens[b] becomes 0 and the entries of block_table that its length takes -1. An entry below 0 is no
- * page and is not appended; any other number is, whatever it is. Pages that a list of n_pages entries has no room for are lost. work:
- * 2 * n_requests words. */
+ * and of their pages), *free_count grows, lens[b] becomes 0 and the entries of block_table that its length takes -1. An entry
+ * below 0 is no page and is not appended; any other number is, whatever it is. Pages that a list of n_pages entries has no room
+ * for are lost. work: 2 * n_requests words. */
 typedef struct sah_paged_release_args {
   const uint8_t* finished;
   int32_t* lens;
@@ -65,7 +66,8 @@ typedef struct sah_paged_release_args {
 int sah_paged_release(const sah_paged_release_args* a);
 
 /* Writes row t of keys and values [n_tokens, Hkv, D] to slot slot_map[t] of the cache; a slot outside [0, n_pages *
- * page_size) is passed over. Where two rows name the same slot, which of them it holds afterwards is not defined. */
+ * page_size) is passed over. Where two rows name the same slot, which of them it holds afterwards is not defined; rows
+ * share no memory with the slots that are written. */
 typedef struct sah_paged_store_args {
   const void* k; int64_t ks_t, ks_h;
   const void* v; int64_t vs_t, vs_h;
@@ -82,10 +84,12 @@ int sah_paged_store(const sah_paged_store_args* a);
  * p = kv_lens[b] - (cu_new[b + 1] - cu_new[b]) + i and sees the keys j <= p of its request, with window > 0 those of them with
  * j < sink or j > p - window (the Sink and Local maskers' columns). sinks, optional [Hq]: a logit per head in the softmax's
  * denominator. A row that sees nothing is 0. Rows of q behind the last request's are not read and their output is left as it
- * was. Keys beyond table_width pages are not there; positions, and so windows, go by kv_lens all the same. out [n_tokens, Hq, D]. max_context: about how long the longest
- * request is (0: not known); it decides how work is split, never what is computed. page_size: a power of two; table_width *
- * page_size below 2^31 - 4096. Rows of out share no memory with each other or with what is read (refused, as
- * is an out whose rows lie between those of a cache, or between q's with another qs_t than os_t).
+ * was. Keys beyond table_width pages are not there; positions, and so windows, go by kv_lens all the same. out [n_tokens, Hq,
+ * D]. max_context: about how long the longest request is (0: not known); it decides how work is split, never what is computed.
+ * page_size: a power of two; table_width * page_size below 2^31 - 4096. Rows of out share no memory with each other or with
+ * what is read (refused, as is an out whose rows lie between those of a cache, or between q's with another qs_t than os_t).
+ * Logits, softmax statistics and sums are fp32; the weights of 16-bit types enter the second product as two terms of the type
+ * together, or, in longer chunks (tiles of 128 rows), as one.
  * work: sah_paged_attention_work_floats(a) floats, no particular content. */
 typedef struct sah_paged_attention_args {
   const void* q; int64_t qs_t, qs_h;
