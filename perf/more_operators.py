@@ -1,0 +1,546 @@
+"""What a cache in 8 bits and attention over the pages that matter cost, operator by operator.
+
+A server that holds many long contexts keeps keys and values in 8 bits (e4m3, a power of two for each token and key head as its scale)
+and lets a token read the pages whose keys can matter to it. A case is one pass of one of these:
+
+    cycle    new tokens are quantised into their slots, and the requests' whole contexts are read back as one tensor per matrix,
+             the form in which the rest of the framework takes a cache
+    attend   new tokens attend to everything their request has in the 8-bit cache
+    bounds   the smallest and largest element of every channel of the pages that a step has filled
+    sparse   every new token ranks its request's pages by how large a logit they can hold, and attends to the best
+
+Lengths inside a batch are spread evenly over a range and dealt to the requests in an order that the seed gives.
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+_DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+_SIZE = {"f32": 4, "bf16": 2, "f16": 2, "e4m3": 1}
+
+
+# ---------------------------------------------------------------------------------------------------------------- cases
+def listed():
+    return [
+        # a short request's answer: one token for each of 8, and the contexts handed to a program that wants them whole
+        _cycle("cycle_answers_8", requests=8, new=(1, 1), cached=(100, 400)),
+        # chunks of four prompts, read back behind what was there
+        _cycle("cycle_chunks_16384", requests=4, new=(4096, 4096), cached=(0, 4096)),
+        # one request alone, 32K keys: all of the chip for one row of heads
+        _attend("attend8_answer_32k", requests=1, new=(1, 1), cached=(32767, 32767)),
+        # 64 answers under way, contexts of 1K to 32K keys: the bulk of a server's time
+        _attend("attend8_answers_64", requests=64, new=(1, 1), cached=(1000, 32767), page=64),
+        # a chunk of a long prompt behind what is cached of it
+        _attend("attend8_chunk_2048", requests=1, new=(2048, 2048), cached=(16384, 16384)),
+        # a few drafted tokens a request under the Sink + Local pattern, odd group size, narrow heads
+        _attend("attend8_drafts_sink_local", requests=16, new=(1, 7), cached=(0, 8001), q_heads=12, kv_heads=4, head_dim=64, dtype="f16",
+                page=32, sink=128, window=512),
+        # a step's answers: a few of 64 requests fill a page
+        _bounds("bounds_answers_64", requests=64, new=(1, 1), cached=(1000, 32767), cache="bf16"),
+        # chunks of four prompts, 8-bit cache
+        _bounds("bounds_chunks_16384", requests=4, new=(4096, 4096), cached=(0, 4096), cache="e4m3"),
+        # one request alone, 32K keys, a thirty-second of them read
+        _sparse("sparse_answer_32k", requests=1, new=(1, 1), cached=(32767, 32767), cache="bf16", select=64),
+        # 64 answers under way on the 8-bit cache
+        _sparse("sparse_answers_64", requests=64, new=(1, 1), cached=(1000, 32767), cache="e4m3", select=64),
+        # questions of a few tokens to long texts, wide pages
+        _sparse("sparse_questions_32", requests=8, new=(1, 32), cached=(4000, 16000), cache="bf16", select=24, page=32),
+        # the type and the sizes a developer checks a model with
+        _sparse("sparse_f32", requests=5, new=(1, 9), cached=(0, 4001), q_heads=8, kv_heads=2, head_dim=96, dtype="f32", cache="f32", select=17),
+    ]
+
+
+def _named(name, case):
+    if name:
+        case["name"] = name
+    return case
+
+
+def _sizes(requests, new, cached, page):
+    return dict(requests=requests, page=page, new_lo=new[0], new_hi=new[1], cached_lo=cached[0], cached_hi=cached[1])
+
+
+def _cycle(name, requests, new, cached, kv_heads=8, head_dim=128, dtype="bf16", page=16):
+    return _named(name, dict(op="cycle", kv_heads=kv_heads, head_dim=head_dim, dtype=dtype, **_sizes(requests, new, cached, page)))
+
+
+def _attend(name, requests, new, cached, q_heads=32, kv_heads=8, head_dim=128, dtype="bf16", page=16, sink=0, window=0):
+    return _named(name, dict(op="attend", q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, dtype=dtype, sink=sink, window=window,
+                             **_sizes(requests, new, cached, page)))
+
+
+def _bounds(name, requests, new, cached, cache, kv_heads=8, head_dim=128, page=16):
+    return _named(name, dict(op="bounds", kv_heads=kv_heads, head_dim=head_dim, cache=cache, **_sizes(requests, new, cached, page)))
+
+
+def _sparse(name, requests, new, cached, cache, select, q_heads=32, kv_heads=8, head_dim=128, dtype="bf16", page=16, sink=1, window=2):
+    return _named(name, dict(op="sparse", q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, dtype=dtype, cache=cache, select=select,
+                             sink=sink, window=window, **_sizes(requests, new, cached, page)))
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(("cycle", "attend", "attend", "bounds", "sparse", "sparse"))
+    kv_heads = rng.choice((1, 2, 4, 8))
+    head_dim = rng.choice((64, 80, 96, 128, 128, 128))
+    page = rng.choice((8, 16, 16, 32, 64))
+    dtype = rng.choice(("bf16", "bf16", "bf16", "f16", "f32"))
+    heads = dict(q_heads=kv_heads * rng.choice((1, 2, 3, 4, 8) if kv_heads < 8 else (1, 2, 3, 4)), kv_heads=kv_heads)
+    if op in ("cycle", "bounds"):
+        new_hi = _log_int(rng, 1, 4096)
+        lo, hi = sorted((_log_int(rng, 1, 4097) - 1, _log_int(rng, 1, 4097) - 1))
+        requests = _log_int(rng, 1, max(1, min(64, 32768 // (new_hi + hi))))
+        new = (rng.choice((1, new_hi)), new_hi)
+        if op == "cycle":
+            return _cycle(None, requests, new, (lo, hi), kv_heads, head_dim, dtype, page)
+        return _bounds(None, requests, new, (lo, hi), rng.choice(("e4m3", dtype)), kv_heads, head_dim, page)
+    if op == "attend":
+        common = dict(head_dim=head_dim, dtype=dtype, page=page, **heads)
+        if rng.random() < 0.3:
+            common.update(sink=rng.choice((0, 4, 128)), window=_log_int(rng, 16, 2048))
+        if rng.random() < 0.5:  # answers
+            lo, hi = sorted((_log_int(rng, 1, 32767), _log_int(rng, 1, 32767)))
+            return _attend(None, _log_int(rng, 1, 64), (1, 1), (lo, hi), **common)
+        new_hi = _log_int(rng, 2, 2048 if dtype != "f32" else 256)
+        hi = _log_int(rng, 1, 16384) - 1
+        most = int(2048 * 18432 * 32 / (new_hi * (hi + new_hi) * heads["q_heads"]))  # the largest listed chunk's scores
+        return _attend(None, _log_int(rng, 1, max(1, min(16, most))), (rng.choice((1, new_hi)), new_hi), (rng.choice((0, hi)), hi), **common)
+    lo, hi = sorted((_log_int(rng, 1, 32767), _log_int(rng, 1, 32767)))
+    select = _log_int(rng, 4, max(5, 1024 // page))
+    if rng.random() < 0.6:
+        requests, new = _log_int(rng, 1, 64), (1, 1)
+    else:
+        new_hi = _log_int(rng, 2, 32)
+        requests, new, lo, hi = _log_int(rng, 1, 8), (rng.choice((1, new_hi)), new_hi), lo // 2, hi // 2
+    return _sparse(None, requests, new, (lo, hi), rng.choice(("e4m3", dtype)), select, head_dim=head_dim, dtype=dtype, page=page,
+                   sink=rng.choice((0, 1, 1)), window=rng.choice((1, 2, 2)), **heads)
+
+
+# ----------------------------------------------------------------------------------------------------------- a case's sizes
+def _spread(lo, hi, n):
+    """n lengths from lo to hi, evenly."""
+    return [lo + (hi - lo) * i // max(1, n - 1) for i in range(n)] if n > 1 else [hi]
+
+
+def _new_and_cached(case):
+    """The requests' lengths: short chunks beside long contexts and the other way round."""
+    n = case["requests"]
+    new = _spread(case["new_lo"], case["new_hi"], n)
+    cached = _spread(case["cached_lo"], case["cached_hi"], n)
+    return new, [cached[(7 * i + 3) % n] for i in range(n)] if math.gcd(7, n) == 1 else cached[::-1]
+
+
+def _visible(case, new, cached):
+    """(query, key) pairs of a request, and the keys that one of its queries at least sees."""
+    sink, window = case["sink"], case["window"]
+    kv = cached + new
+    if not window:
+        return new * cached + new * (new + 1) // 2, kv
+    pairs = 0
+    for p in range(cached, kv):
+        first = max(0, p - window + 1)
+        pairs += p + 1 - first + min(sink, first)
+    first = max(0, cached - window + 1)
+    return pairs, kv - first + min(sink, first)
+
+
+def work(case):
+    new, cached = _new_and_cached(case)
+    both = list(zip(new, cached))
+    page, d, kv_heads = case["page"], case["head_dim"], case["kv_heads"]
+    row = kv_heads * (d + 1)  # bytes of a token's keys in 8 bits, with their scales
+    if case["op"] == "cycle":
+        es = _SIZE[case["dtype"]]
+        wide = kv_heads * d * es
+        return {"bytes": sum(new) * (2 * (wide + row) + 8) + sum(c + n for n, c in both) * 2 * (row + wide), "flops": 0}
+    if case["op"] == "attend":
+        seen = [_visible(case, n, c) for n, c in both]
+        keys, pairs = sum(k for _, k in seen), sum(p for p, _ in seen)
+        return {"bytes": 2 * _SIZE[case["dtype"]] * d * case["q_heads"] * sum(new) + 2 * row * keys + 4 * keys // page,
+                "flops": 4 * case["q_heads"] * d * pairs}
+    es, held = _SIZE[case["cache"]], 2 if case["cache"] == "e4m3" else _SIZE[case["cache"]]
+    row = row if case["cache"] == "e4m3" else kv_heads * d * es
+    if case["op"] == "bounds":
+        filled = sum((c + n) // page - c // page for n, c in both)
+        return {"bytes": filled * (page * row + 2 * kv_heads * d * held) + 12 * case["requests"], "flops": 2 * filled * page * kv_heads * d}
+    # a request's bounds once; the pages its tokens attend to, all different until the context is used up
+    ranked = sum((c + n) // page for n, c in both)
+    pages = sum(min(n * case["select"], -(-(c + n) // page)) for n, c in both)
+    keys = sum(min(c + n, case["select"] * page) * n for n, c in both)
+    scored = sum(n * ((c + n) // page) for n, c in both)
+    return {"bytes": 2 * kv_heads * d * held * ranked + 2 * pages * page * row + 2 * _SIZE[case["dtype"]] * d * case["q_heads"] * sum(new)
+                     + 4 * sum(new) * kv_heads * case["select"],
+            "flops": 4 * kv_heads * d * scored + 4 * case["q_heads"] * d * keys}
+
+
+# ------------------------------------------------------------------------------------------------------------------ inputs
+def _pages_of(lens, page, width, order, device):
+    """A block table: the requests' pages lie anywhere in the cache. `order`: a permutation of the pages."""
+    table = torch.full((len(lens), width), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(lens):
+        k = -(-n // page)
+        table[b, :k] = order[at:at + k]
+        at += k
+    return table.to(device)
+
+
+def _power(exponent):
+    """2^exponent in 32 bits, exactly"""
+    return ((exponent.int() + 127) << 23).view(torch.float32)
+
+
+def _quantised(x):
+    """Rows of 32-bit numbers in e4m3 and the exponents of their scales, the least powers of two at which a row's largest fits."""
+    most = x.abs().amax(-1)
+    mantissa, exponent = torch.frexp(most)
+    exponent = torch.where(mantissa > 0.875, exponent - 8, exponent - 9)  # 448 is 0.875 * 2^9
+    exponent = torch.where(most == 0, -110, exponent).clamp(min=-110)
+    return (x * _power(-exponent)[..., None]).to(torch.float8_e4m3fn), exponent
+
+
+def _scale_bytes(exponent):
+    return (exponent + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+
+
+def _values(cache, scales):
+    """What an 8-bit cache stands for, in 32 bits: exact."""
+    return cache.float() * _power(scales.view(torch.uint8).int() - 127)[..., None]
+
+
+def prepare(case, seed):
+    device = torch.device("cuda", torch.cuda.current_device())
+    host = torch.Generator().manual_seed(seed)
+    gen = torch.Generator(device=device).manual_seed(seed)
+
+    def randn(*shape):
+        return torch.randn(shape, generator=gen, device=device, dtype=torch.float32)
+
+    page, n, kv_heads, d = case["page"], case["requests"], case["kv_heads"], case["head_dim"]
+    deal = torch.randperm(n, generator=host).tolist()
+    new, cached = ([v[i] for i in deal] for v in _new_and_cached(case))
+    kv = [a + b for a, b in zip(new, cached)]
+    width = -(-max(kv) // page)
+    pages = sum(-(-k // page) for k in kv) + 8
+    table = _pages_of(kv, page, width, torch.randperm(pages, generator=host).to(torch.int32), device)
+    cu = [0]
+    for k in new:
+        cu.append(cu[-1] + k)
+    state = dict(case=case, table=table, kv_lens=torch.tensor(kv, dtype=torch.int32, device=device),
+                 cu_new=torch.tensor(cu, dtype=torch.int32, device=device), max_context=max(kv), max_new=max(new), key_scales=None,
+                 value_scales=None)
+    kind = case.get("cache", "e4m3")
+    shape = (pages, page, kv_heads, d)
+    for name in ("key", "value"):
+        cache = torch.empty(shape, dtype=torch.float8_e4m3fn if kind == "e4m3" else _DTYPES[kind], device=device)
+        scales = torch.empty(shape[:3], dtype=torch.float8_e8m0fnu, device=device) if kind == "e4m3" else None
+        part = max(1, (1 << 27) // (page * kv_heads * d))
+        for at in range(0, pages, part):
+            count = min(part, pages - at)
+            # a text's neighbouring tokens have something in common
+            x = 0.8 * randn(count, page, kv_heads, d) + 0.6 * randn(count, 1, kv_heads, d)
+            if kind == "e4m3":
+                cache[at:at + count], exponent = _quantised(x)
+                scales[at:at + count] = _scale_bytes(exponent)
+            else:
+                cache[at:at + count] = x.to(cache.dtype)
+        state[name + "_cache"] = cache
+        if scales is not None:
+            state[name + "_scales"] = scales
+    if case["op"] == "cycle":
+        state.update(keys=randn(cu[-1], kv_heads, d).to(_DTYPES[case["dtype"]]), values=randn(cu[-1], kv_heads, d).to(_DTYPES[case["dtype"]]))
+        slots = []
+        pages_of = table.tolist()
+        for b in range(n):
+            slots += [pages_of[b][p // page] * page + p % page for p in range(cached[b], kv[b])]
+        state["slots"] = torch.tensor(slots, dtype=torch.int64, device=device)
+    if case["op"] in ("bounds", "sparse"):
+        bounds = torch.empty(pages, kv_heads, 2, d, dtype=torch.bfloat16 if kind == "e4m3" else _DTYPES[kind], device=device)
+        part = max(1, (1 << 27) // (page * kv_heads * d))
+        for at in range(0, pages, part):
+            x = state["key_cache"][at:at + part]
+            x = _values(x, state["key_scales"][at:at + part]) if kind == "e4m3" else x.float()
+            bounds[at:at + part, :, 0], bounds[at:at + part, :, 1] = x.amin(1).to(bounds.dtype), x.amax(1).to(bounds.dtype)
+        if case["op"] == "bounds":  # those of the step's pages are not known yet
+            for b in range(n):
+                bounds[table[b, cached[b] // page:kv[b] // page].long()] = 0
+        state["bounds"] = bounds
+    if case["op"] in ("attend", "sparse"):
+        state.update(queries=randn(cu[-1], case["q_heads"], d).to(_DTYPES[case["dtype"]]), scaling=d ** -0.5)
+    return state
+
+
+# ------------------------------------------------------------------------------------------------------------- plain forms
+def _plain_cycle(s):
+    page, m = s["case"]["page"], s["max_context"]
+    slots, pages = s["slots"], s["table"].long().clamp(min=0)
+    there = (torch.arange(m, device=slots.device) < s["kv_lens"][:, None])[:, None, :, None]
+    out = []
+    for name in ("key", "value"):
+        cache, scales = s[name + "_cache"], s[name + "_scales"]
+        rows, exponent = _quantised(s[name + "s"].float())
+        cache.view(-1, *cache.shape[2:]).view(torch.uint8)[slots] = rows.view(torch.uint8)
+        scales.view(torch.uint8).view(-1, cache.shape[2])[slots] = _scale_bytes(exponent).view(torch.uint8)
+        x = _values(cache.view(torch.uint8)[pages].view(torch.float8_e4m3fn), scales.view(torch.uint8)[pages])
+        x = x.reshape(pages.shape[0], -1, *cache.shape[2:])[:, :m].transpose(1, 2)
+        out.append(torch.where(there, x, 0.0).to(s[name + "s"].dtype))
+    return out
+
+
+def _rows_of(s):
+    """Rows of the packed tokens by request, padded; their positions."""
+    cu, kv = s["cu_new"].long(), s["kv_lens"].long()
+    i = torch.arange(s["max_new"], device=cu.device)
+    rows = (cu[:-1, None] + i).clamp(max=s["queries"].shape[0] - 1)
+    return rows, (kv - (cu[1:] - cu[:-1]))[:, None] + i
+
+
+def _packed(s, x):
+    """(requests, rows, ...) as packed tokens"""
+    cu = s["cu_new"].long()
+    t = torch.arange(s["queries"].shape[0], device=cu.device)
+    b = torch.searchsorted(cu[1:], t, right=True)
+    return x[b, t - cu[b]]
+
+
+def _cached(s, name, pages):
+    cache = s[name + "_cache"]
+    if s[name + "_scales"] is None:
+        return cache[pages].float()
+    return _values(cache.view(torch.uint8)[pages].view(torch.float8_e4m3fn), s[name + "_scales"].view(torch.uint8)[pages])
+
+
+def _plain_attend(s):
+    case, q = s["case"], s["queries"]
+    kv_heads, d, n, m = case["kv_heads"], case["head_dim"], s["max_new"], s["max_context"]
+    group, requests = case["q_heads"] // kv_heads, s["kv_lens"].numel()
+    rows, position = _rows_of(s)
+    qs = q[rows].float().view(requests, n, kv_heads, group, d).permute(0, 2, 3, 1, 4).reshape(requests, kv_heads, group * n, d)
+    pages = s["table"].long().clamp(min=0)
+    k = _cached(s, "key", pages).view(requests, -1, kv_heads, d)[:, :m].permute(0, 2, 3, 1).contiguous()
+    scores = torch.matmul(qs, k).view(requests, kv_heads, group, n, m)
+    del k
+    scores *= s["scaling"]
+    j = torch.arange(m, device=q.device)
+    hidden = j > position[..., None]
+    if case["window"]:
+        hidden |= (j <= position[..., None] - case["window"]) & (j >= case["sink"])
+    scores.masked_fill_(hidden[:, None, None], -math.inf)
+    scores -= scores.amax(-1, keepdim=True)
+    scores.exp_()
+    total = scores.sum(-1, keepdim=True)
+    v = _cached(s, "value", pages).view(requests, -1, kv_heads, d)[:, :m].permute(0, 2, 1, 3).contiguous()
+    out = torch.matmul(scores.view(requests, kv_heads, group * n, m), v).view(requests, kv_heads, group, n, d) / total
+    return _packed(s, out.permute(0, 3, 1, 2, 4).reshape(requests, n, case["q_heads"], d).to(q.dtype))
+
+
+def _plain_bounds(s):
+    page, bounds, cu, kv = s["case"]["page"], s["bounds"], s["cu_new"].long(), s["kv_lens"].long()
+    before = kv - (cu[1:] - cu[:-1])
+    column = torch.arange(s["table"].shape[1], device=kv.device)
+    filled = s["table"].long()[(column >= (before // page)[:, None]) & (column < (kv // page)[:, None])]
+    x = _cached(s, "key", filled)
+    bounds[filled, :, 0] = x.amin(1).to(bounds.dtype)
+    bounds[filled, :, 1] = x.amax(1).to(bounds.dtype)
+    return bounds
+
+
+def _plain_select(s):
+    """The pages each token attends to, rising, -1 behind the last: those it always sees, then the largest of
+    sum_heads sum_channels max(q * smallest, q * largest). In 64 bits: what is ranked next to each other differs by little."""
+    case, page, n = s["case"], s["case"]["page"], s["max_new"]
+    kv_heads, d, requests = case["kv_heads"], case["head_dim"], s["kv_lens"].numel()
+    rows, position = _rows_of(s)
+    q = s["queries"][rows].double().view(requests, n, kv_heads, -1, d)
+    ends = torch.cat([q.clamp(max=0).sum(3), q.clamp(min=0).sum(3)], -1).transpose(1, 2)  # (requests, kv_heads, n, 2 d)
+    table = s["table"].long().clamp(min=0)
+    width = table.shape[1]
+    bounds = s["bounds"][table].double().permute(0, 2, 3, 4, 1).reshape(requests, kv_heads, 2 * d, width)
+    scores = torch.matmul(ends, bounds)
+    j = torch.arange(width, device=table.device)
+    last = (position // page)[:, None, :, None]
+    scores.masked_fill_((j < case["sink"]) | (j > last - case["window"]), math.inf)
+    scores.masked_fill_(j > last, -math.inf)
+    ranked, order = torch.sort(scores, dim=-1, descending=True, stable=True)
+    k = min(case["select"], width)
+    pages = torch.where(ranked[..., :k] == -math.inf, width, order[..., :k])
+    pages = torch.sort(pages, dim=-1).values
+    pages = torch.where(pages == width, -1, pages)
+    pages = torch.nn.functional.pad(pages, (0, case["select"] - k), value=-1)
+    return _packed(s, pages.transpose(1, 2)).int()  # (tokens, kv_heads, select)
+
+
+def _plain_sparse(s):
+    case, page, q = s["case"], s["case"]["page"], s["queries"]
+    kv_heads, d, tokens = case["kv_heads"], case["head_dim"], q.shape[0]
+    pages = _plain_select(s)
+    cu = s["cu_new"].long()
+    b = torch.searchsorted(cu[1:], torch.arange(tokens, device=q.device), right=True)
+    position = (s["kv_lens"].long()[b] - cu[b + 1]) + torch.arange(tokens, device=q.device)
+    logical = pages.long()
+    physical = s["table"].long()[b[:, None, None], logical.clamp(min=0)].clamp(min=0)
+    head = torch.arange(kv_heads, device=q.device)[:, None]
+
+    def gathered(name):
+        cache = s[name + "_cache"]
+        if s[name + "_scales"] is None:
+            x = cache.transpose(1, 2)[physical, head].float()
+        else:
+            x = _values(cache.view(torch.uint8).transpose(1, 2)[physical, head].view(torch.float8_e4m3fn),
+                        s[name + "_scales"].view(torch.uint8).transpose(1, 2)[physical, head])
+        return x.reshape(tokens, kv_heads, -1, d)
+
+    qs = q.float().view(tokens, kv_heads, -1, d)
+    scores = torch.matmul(qs, gathered("key").transpose(2, 3).contiguous()) * s["scaling"]
+    j = (logical[..., None] * page + torch.arange(page, device=q.device)).reshape(tokens, kv_heads, 1, -1)
+    hidden = (j > position[:, None, None, None]) | (logical < 0).repeat_interleave(page, dim=2)[:, :, None]
+    scores.masked_fill_(hidden, -math.inf)
+    weights = torch.exp(scores - scores.amax(-1, keepdim=True))
+    out = torch.matmul(weights, gathered("value")) / weights.sum(-1, keepdim=True)
+    return [out.reshape(tokens, -1, d).to(q.dtype), pages]
+
+
+# ---------------------------------------------------------------------------------------------------------------- the pass
+def _framework():
+    path = os.path.join(os.getcwd(), "sparse-attention-hub_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from sparse_attention_hub_amd.sparse_attention.utils import paged_cache
+
+    return paged_cache
+
+
+def run(state):
+    s, case = state, state["case"]
+    if not own:
+        return {"cycle": _plain_cycle, "attend": _plain_attend, "bounds": _plain_bounds, "sparse": _plain_sparse}[case["op"]](s)
+    paged = _framework()
+    scales = dict(key_scales=s["key_scales"], value_scales=s["value_scales"])
+    if case["op"] == "cycle":
+        paged.store_paged(s["keys"], s["values"], s["key_cache"], s["value_cache"], s["slots"], **scales)
+        return list(paged.load_paged(s["key_cache"], s["value_cache"], s["table"], s["kv_lens"], s["max_context"], dtype=s["keys"].dtype, **scales))
+    if case["op"] == "attend":
+        return paged.paged_attention(s["queries"], s["key_cache"], s["value_cache"], s["table"], s["kv_lens"], s["cu_new"], s["scaling"],
+                                     max_context=s["max_context"], sink_size=case["sink"], window_size=case["window"], **scales)
+    if case["op"] == "bounds":
+        paged.update_page_bounds(s["bounds"], s["key_cache"], s["table"], s["kv_lens"], s["cu_new"], key_scales=s["key_scales"])
+        return s["bounds"]
+    pages = paged.select_pages(s["queries"], s["bounds"], s["table"], s["kv_lens"], s["cu_new"], case["page"], case["select"],
+                               sink_pages=case["sink"], window_pages=case["window"], max_context=s["max_context"])
+    out = paged.paged_attention(s["queries"], s["key_cache"], s["value_cache"], s["table"], s["kv_lens"], s["cu_new"], s["scaling"],
+                                max_context=s["max_context"], pages=pages, **scales)
+    return [out, pages]
+
+
+# ----------------------------------------------------------------------------------------------------------- in 64 bits
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "bounds":
+        out = s["bounds"].double()
+        cu, kv = s["cu_new"].tolist(), s["kv_lens"].tolist()
+        for b, length in enumerate(kv):
+            for j in range((length - cu[b + 1] + cu[b]) // case["page"], length // case["page"]):
+                p = int(s["table"][b, j])
+                x = _wide(s, "key", p)
+                out[p, :, 0], out[p, :, 1] = torch.min(x, dim=0).values, torch.max(x, dim=0).values
+        return out
+    if case["op"] == "cycle":
+        return _exact_cycle(case, s)
+    return _exact_attend(case, s) if case["op"] == "attend" else _exact_sparse(case, s)
+
+
+def _wide(s, name, index):
+    x = s[name + "_cache"][index].double()
+    if s[name + "_scales"] is None:
+        return x
+    return x * _two_to(s[name + "_scales"][index].view(torch.uint8).long() - 127)[..., None]
+
+
+def _two_to(exponent):
+    return ((exponent.long() + 1023) << 52).view(torch.float64)
+
+
+def _to_e4m3(x, grid):
+    """The value of e4m3 times a power of two (a tensor of them) that lies nearest, ties to the even one."""
+    size = x.abs() / grid
+    step = _two_to(torch.frexp(size.clamp(min=2.0 ** -6)).exponent - 4)
+    return torch.sign(x) * torch.round(size / step) * step * grid  # (round: ties to even)
+
+
+def _exact_cycle(case, s):
+    kv, table = s["kv_lens"].tolist(), s["table"]
+    out = []
+    for name in ("key", "value"):
+        rows = s[name + "s"].double()
+        most = rows.abs().amax(-1, keepdim=True)
+        parts = torch.frexp(most / 448)  # the least power of two that is not below
+        rows = _to_e4m3(rows, _two_to(parts.exponent - (parts.mantissa == 0.5).int()))
+        whole = torch.zeros(len(kv), case["kv_heads"], s["max_context"], case["head_dim"], dtype=torch.float64, device=rows.device)
+        at = 0
+        for b, length in enumerate(kv):
+            n = int(s["cu_new"][b + 1] - s["cu_new"][b])
+            pages = table[b, :-(-length // case["page"])].long()
+            whole[b, :, :length] = _wide(s, name, pages).flatten(0, 1)[:length].transpose(0, 1)
+            whole[b, :, length - n:length] = rows[at:at + n].transpose(0, 1)
+            at += n
+        out.append(whole)
+    return out
+
+
+def _exact_attend(case, s):
+    group, page = case["q_heads"] // case["kv_heads"], case["page"]
+    out = torch.empty(s["queries"].shape, dtype=torch.float64, device=s["queries"].device)
+    cu, kv = s["cu_new"].tolist(), s["kv_lens"].tolist()
+    for b, length in enumerate(kv):
+        first = length - (cu[b + 1] - cu[b])
+        pages = s["table"][b, :-(-length // page)].long()
+        keys, values = (_wide(s, name, pages).flatten(0, 1)[:length] for name in ("key", "value"))
+        position = torch.arange(first, length, device=out.device)[:, None]
+        j = torch.arange(length, device=out.device)[None, :]
+        seen = j <= position
+        if case["window"]:
+            seen = seen & ((j < case["sink"]) | (j > position - case["window"]))
+        for g in range(case["q_heads"]):
+            logits = (s["queries"][cu[b]:cu[b + 1], g].double() @ keys[:, g // group].T) * s["scaling"]
+            out[cu[b]:cu[b + 1], g] = torch.softmax(logits.masked_fill(~seen, -math.inf), dim=1) @ values[:, g // group]
+    return out
+
+
+def _exact_sparse(case, s):
+    group, page, k = case["q_heads"] // case["kv_heads"], case["page"], case["select"]
+    cu, kv = s["cu_new"].tolist(), s["kv_lens"].tolist()
+    tokens = s["queries"].shape[0]
+    out = torch.empty(s["queries"].shape, dtype=torch.float64, device=s["queries"].device)
+    chosen = torch.full((tokens, case["kv_heads"], k), -1, dtype=torch.int32)
+    for b, length in enumerate(kv):
+        table = s["table"][b].long()
+        for h in range(case["kv_heads"]):
+            bounds = s["bounds"][table[:-(-length // page)], h].double()
+            for t in range(cu[b], cu[b + 1]):
+                position = length - cu[b + 1] + t
+                last = position // page
+                q = s["queries"][t, h * group:(h + 1) * group].double()
+                scores = torch.stack([torch.maximum(q[g] * bounds[:, 0], q[g] * bounds[:, 1]).sum(1) for g in range(group)]).sum(0)
+                always = {j for j in range(last + 1) if j < case["sink"] or j > last - case["window"]}
+                others = [j for j in torch.argsort(scores, descending=True, stable=True).tolist() if j <= last and j not in always]
+                pages = sorted([*always, *others[:max(0, k - len(always))]])
+                chosen[t, h, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+                rows = table[pages]
+                j = (torch.tensor(pages, device=out.device)[:, None] * page + torch.arange(page, device=out.device)).flatten()
+                keys, values = (_wide_head(s, name, rows, h)[j <= position] for name in ("key", "value"))
+                out[t, h * group:(h + 1) * group] = torch.softmax((q @ keys.T) * s["scaling"], dim=1) @ values
+    return [out, chosen.to(out.device)]
+
+
+def _wide_head(s, name, pages, h):
+    x = s[name + "_cache"][pages, :, h].double()
+    if s[name + "_scales"] is not None:
+        x = x * _two_to(s[name + "_scales"][pages, :, h].view(torch.uint8).long() - 127)[..., None]
+    return x.flatten(0, 1)
