@@ -1,7 +1,7 @@
 """What a cache in 8 bits and attention over the pages that matter cost, operator by operator.
 
-A server that holds many long contexts keeps keys and values in 8 bits (e4m3, a power of two for each token and key head as its scale)
-and lets a token read the pages whose keys can matter to it. A case is one pass of one of these:
+A server that holds many long contexts keeps keys and values in 8 bits (e4m3, a power of two for each token and key head as its scale, a
+page's scales head by head) and lets a token read the pages whose keys can matter to it. A case is one pass of one of these:
 
     cycle    new tokens are quantised into their slots, and the requests' whole contexts are read back as one tensor per matrix,
              the form in which the rest of the framework takes a cache
@@ -211,8 +211,8 @@ def _scale_bytes(exponent):
 
 
 def _values(cache, scales):
-    """What an 8-bit cache stands for, in 32 bits: exact."""
-    return cache.float() * _power(scales.view(torch.uint8).int() - 127)[..., None]
+    """What an 8-bit cache (..., page, kv_heads, head_dim) stands for, in 32 bits: exact."""
+    return cache.float() * _power(scales.view(torch.uint8).int() - 127).transpose(-1, -2)[..., None]
 
 
 def prepare(case, seed):
@@ -240,7 +240,7 @@ def prepare(case, seed):
     shape = (pages, page, kv_heads, d)
     for name in ("key", "value"):
         cache = torch.empty(shape, dtype=torch.float8_e4m3fn if kind == "e4m3" else _DTYPES[kind], device=device)
-        scales = torch.empty(shape[:3], dtype=torch.float8_e8m0fnu, device=device) if kind == "e4m3" else None
+        scales = torch.empty(pages, kv_heads, page, dtype=torch.float8_e8m0fnu, device=device) if kind == "e4m3" else None
         part = max(1, (1 << 27) // (page * kv_heads * d))
         for at in range(0, pages, part):
             count = min(part, pages - at)
@@ -248,7 +248,7 @@ def prepare(case, seed):
             x = 0.8 * randn(count, page, kv_heads, d) + 0.6 * randn(count, 1, kv_heads, d)
             if kind == "e4m3":
                 cache[at:at + count], exponent = _quantised(x)
-                scales[at:at + count] = _scale_bytes(exponent)
+                scales[at:at + count] = _scale_bytes(exponent.transpose(1, 2).contiguous())
             else:
                 cache[at:at + count] = x.to(cache.dtype)
         state[name + "_cache"] = cache
@@ -287,7 +287,7 @@ def _plain_cycle(s):
         cache, scales = s[name + "_cache"], s[name + "_scales"]
         rows, exponent = _quantised(s[name + "s"].float())
         cache.view(-1, *cache.shape[2:]).view(torch.uint8)[slots] = rows.view(torch.uint8)
-        scales.view(torch.uint8).view(-1, cache.shape[2])[slots] = _scale_bytes(exponent).view(torch.uint8)
+        scales.view(torch.uint8)[slots // page, :, slots % page] = _scale_bytes(exponent).view(torch.uint8)
         x = _values(cache.view(torch.uint8)[pages].view(torch.float8_e4m3fn), scales.view(torch.uint8)[pages])
         x = x.reshape(pages.shape[0], -1, *cache.shape[2:])[:, :m].transpose(1, 2)
         out.append(torch.where(there, x, 0.0).to(s[name + "s"].dtype))
@@ -393,8 +393,8 @@ def _plain_sparse(s):
         if s[name + "_scales"] is None:
             x = cache.transpose(1, 2)[physical, head].float()
         else:
-            x = _values(cache.view(torch.uint8).transpose(1, 2)[physical, head].view(torch.float8_e4m3fn),
-                        s[name + "_scales"].view(torch.uint8).transpose(1, 2)[physical, head])
+            x = _values(cache.view(torch.uint8).transpose(1, 2)[physical, head].view(torch.float8_e4m3fn)[..., None, :],
+                        s[name + "_scales"].view(torch.uint8)[physical, head][..., None, :])
         return x.reshape(tokens, kv_heads, -1, d)
 
     qs = q.float().view(tokens, kv_heads, -1, d)
@@ -460,7 +460,7 @@ def _wide(s, name, index):
     x = s[name + "_cache"][index].double()
     if s[name + "_scales"] is None:
         return x
-    return x * _two_to(s[name + "_scales"][index].view(torch.uint8).long() - 127)[..., None]
+    return x * _two_to(s[name + "_scales"][index].view(torch.uint8).long() - 127).transpose(-1, -2)[..., None]
 
 
 def _two_to(exponent):
@@ -542,5 +542,5 @@ def _exact_sparse(case, s):
 def _wide_head(s, name, pages, h):
     x = s[name + "_cache"][pages, :, h].double()
     if s[name + "_scales"] is not None:
-        x = x * _two_to(s[name + "_scales"][pages, :, h].view(torch.uint8).long() - 127)[..., None]
+        x = x * _two_to(s[name + "_scales"][pages, h].view(torch.uint8).long() - 127)[..., None]
     return x.flatten(0, 1)
