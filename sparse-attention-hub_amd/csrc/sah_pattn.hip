@@ -12,6 +12,7 @@
 // the request's last, or on a missing page) are staged from one that is. A visible row's product with a value that is
 // not finite reaches the rows of its tile that do not see it (0 times it): rows that come out not finite are done again, key by key.
 #include "sah_common.h"
+#include "sah_spans.h"
 #include "../../include/sah_serve.h"
 
 #define PA_MAX_D 256
@@ -1153,31 +1154,6 @@ extern "C" int64_t sah_paged_attention_work_floats(const sah_paged_attention_arg
   return pa_dispatch(a, pa_floats_fn{a});
 }
 
-// From a tensor's first byte to behind its last one, judged by strides (elements) and counts
-struct pa_span { int64_t lo, hi; };
-template <int N>
-static pa_span pa_span_of(const void* p, int es, int64_t inner, const int64_t (&stride)[N], const int64_t (&count)[N]) {
-  pa_span s{0, inner};
-  for (int i = 0; i < N; ++i) (stride[i] < 0 ? s.lo : s.hi) += stride[i] * (count[i] - 1);
-  return pa_span{(int64_t)(uint64_t)p + s.lo * es, (int64_t)(uint64_t)p + s.hi * es};
-}
-static bool pa_meet(const pa_span& a, const pa_span& b) { return a.lo < b.hi && b.lo < a.hi; }
-
-// Whether a row of out shares memory with one of q. Where their tokens are equally far apart (two slices of one buffer) every pair of heads is
-// looked at: only the nearest tokens can meet. Else tensors that lie within each other count as sharing.
-static bool pa_on_queries(const sah_paged_attention_args* a, int es, const pa_span& out) {
-  if (!pa_meet(out, pa_span_of<2>(a->q, es, a->D, {a->qs_t, a->qs_h}, {a->n_tokens, a->Hq}))) return false;
-  if (a->os_t != a->qs_t || a->Hq > 1024) return true;
-  const int64_t first = (int64_t)(uint64_t)a->out - (int64_t)(uint64_t)a->q, row = (int64_t)a->D * es, step = a->os_t * es;
-  for (int ho = 0; ho < a->Hq; ++ho)
-    for (int hq = 0; hq < a->Hq; ++hq) {
-      const int64_t d = first + (ho * a->os_h - hq * a->qs_h) * es, near = step ? -d / step : 0;
-      for (int64_t i = near - 1; i <= near + 1; ++i)  // tokens that out's row is ahead of q's
-        if (i > -a->n_tokens && i < a->n_tokens && d + i * step < row && d + i * step > -row) return true;
-    }
-  return false;
-}
-
 extern "C" int sah_paged_attention(const sah_paged_attention_args* given) {
   if (!given) return sah_fail(SAH_ENULL, "sah_paged_attention: args is NULL");
   sah_paged_attention_args own = *given;
@@ -1214,13 +1190,13 @@ extern "C" int sah_paged_attention(const sah_paged_attention_args* given) {
   if (!(a->scaling - a->scaling == 0.f)) return sah_fail(SAH_EINVAL, "sah_paged_attention: scaling is not finite");
   if (!a->work || a->work_floats < sah_paged_attention_work_floats(a)) return sah_fail(SAH_ECAPACITY, "sah_paged_attention: work is too small");
   // rows are read again after others have been written
-  const pa_span out = pa_span_of<2>(a->out, es, a->D, {a->os_t, a->os_h}, {a->n_tokens, a->Hq});
-  if (pa_on_queries(a, es, out)) return sah_fail(SAH_EINVAL, "sah_paged_attention: out shares memory with q");
-  if (pa_meet(out, pa_span_of<3>(a->k, es, a->D, {a->ks_p, a->ks_t, a->ks_h}, {a->n_pages, a->page_size, a->Hkv})) ||
-      pa_meet(out, pa_span_of<3>(a->v, es, a->D, {a->vs_p, a->vs_t, a->vs_h}, {a->n_pages, a->page_size, a->Hkv})) ||
-      pa_meet(out, pa_span_of<1>(a->block_table, 4, a->table_width, {a->table_pitch}, {a->n_requests})) ||
-      pa_meet(out, pa_span_of<1>(a->kv_lens, 4, 1, {1}, {a->n_requests})) || pa_meet(out, pa_span_of<1>(a->cu_new, 4, 1, {1}, {a->n_requests + 1})) ||
-      (a->sinks && pa_meet(out, pa_span_of<1>(a->sinks, 4, 1, {1}, {a->Hq}))))
+  const sah_span out = sah_span_of<2>(a->out, es, a->D, {a->os_t, a->os_h}, {a->n_tokens, a->Hq});
+  if (sah_out_on_queries(a->q, a->qs_t, a->qs_h, a->out, a->os_t, a->os_h, a->n_tokens, a->Hq, a->D, es)) return sah_fail(SAH_EINVAL, "sah_paged_attention: out shares memory with q");
+  if (sah_meet(out, sah_span_of<3>(a->k, es, a->D, {a->ks_p, a->ks_t, a->ks_h}, {a->n_pages, a->page_size, a->Hkv})) ||
+      sah_meet(out, sah_span_of<3>(a->v, es, a->D, {a->vs_p, a->vs_t, a->vs_h}, {a->n_pages, a->page_size, a->Hkv})) ||
+      sah_meet(out, sah_span_of<1>(a->block_table, 4, a->table_width, {a->table_pitch}, {a->n_requests})) ||
+      sah_meet(out, sah_span_of<1>(a->kv_lens, 4, 1, {1}, {a->n_requests})) || sah_meet(out, sah_span_of<1>(a->cu_new, 4, 1, {1}, {a->n_requests + 1})) ||
+      (a->sinks && sah_meet(out, sah_span_of<1>(a->sinks, 4, 1, {1}, {a->Hq}))))
     return sah_fail(SAH_EINVAL, "sah_paged_attention: out lies within the cache, the table or the lengths");
   return (int)pa_dispatch(a, pa_launch_fn{a});
 }
