@@ -1,0 +1,136 @@
+// What the kernels on 8-bit pages and on pages' bounds share: a token's request, elements of e4m3, checks of arguments.
+#pragma once
+#include "sah_common.h"
+#include "../../include/sah_pages.h"
+
+#define PG_MAX_D 256
+
+// bytes of an element
+__host__ __device__ constexpr int pg_size(int dtype) { return dtype == SAH_F32 ? 4 : dtype == SAH_E4M3 ? 1 : 2; }
+
+// ---------------------------------------------------------------------------
+// elements of e4m3 and their scales
+// ---------------------------------------------------------------------------
+// 2^e of a scale's byte e + 127 (-110 <= e <= 120, so the number has no subnormal form)
+__device__ __forceinline__ float pg_scale(uint32_t byte) { return sah_bits_to_float(byte << 23); }
+// of byte i of four
+__device__ __forceinline__ float pg_scale_of(uint32_t bytes, int i) { return sah_bits_to_float(((bytes >> (8 * i)) & 0xffu) << 23); }
+
+// Two neighbouring elements of four (the lower pair, or the upper one), times a power of two, as two bf16: exact, one instruction.
+template <bool UPPER>
+__device__ __forceinline__ uint32_t pg_widen2(uint32_t four, float scale) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, scale, UPPER));
+#else
+  return 0;
+#endif
+}
+__device__ __forceinline__ void pg_widen4(uint32_t four, float scale, float (&o)[4]) {
+  const uint32_t lo = pg_widen2<false>(four, scale), hi = pg_widen2<true>(four, scale);
+  o[0] = sah_bits_to_float(lo << 16);
+  o[1] = sah_bits_to_float(lo & 0xffff0000u);
+  o[2] = sah_bits_to_float(hi << 16);
+  o[3] = sah_bits_to_float(hi & 0xffff0000u);
+}
+// element i of a row in storage type T; `scale` counts for SAH_E4M3 alone
+template <int T>
+__device__ __forceinline__ float pg_element(const void* p, int64_t i, float scale) {
+  if constexpr (T == SAH_E4M3) {
+    return sah_bits_to_float(pg_widen2<false>(((const uint8_t*)p)[i], scale) << 16);
+  } else {
+    return sah_load<T>(p, i);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// a token's request
+// ---------------------------------------------------------------------------
+struct pg_request {
+  int b;             // -1: no request has the row
+  int begin, n_new;  // its rows
+  int kv;            // keys it has
+  int64_t base;      // row t stands at position base + t
+};
+__device__ __forceinline__ pg_request pg_none() { return pg_request{-1, 0, 0, 0, 0}; }
+__device__ __forceinline__ pg_request pg_read(const sah_page_requests& R, int page_size, int b, int t) {
+  pg_request r;
+  const int begin = R.cu_new[b], end = R.cu_new[b + 1], kv = R.kv_lens[b];
+  if (begin < 0 || t < begin || t >= end) return pg_none();  // (running sums that fall: nobody's)
+  const int last = end < R.n_tokens ? end : R.n_tokens, most = R.table_width * page_size;
+  r.b = b;
+  r.begin = begin;
+  r.n_new = last - begin;
+  r.kv = kv < 0 ? 0 : (kv < most ? kv : most);
+  r.base = (int64_t)kv - end;
+  return r;
+}
+// By a whole wave, for a row that all of its lanes ask for: 64 ends are looked at in one trip to memory.
+__device__ __forceinline__ pg_request pg_find_by_wave(const sah_page_requests& R, int page_size, int t) {
+  const int lane = threadIdx.x & (SAH_WAVE - 1);
+  int lo = 0, n = R.n_requests, step;
+  do {
+    step = (n + SAH_WAVE - 1) / SAH_WAVE;
+    const int64_t i = (int64_t)(lane + 1) * step - 1;
+    const uint64_t behind = __ballot(R.cu_new[lo + (i < n ? (int)i : n - 1) + 1] > t);
+    if (!behind) return pg_none();
+    const int from = __builtin_ctzll(behind) * step;  // (at most n - 1: lanes beyond it ask what the last one before asks)
+    lo += from;
+    n = n - from < step ? n - from : step;
+  } while (step > 1);
+  return pg_read(R, page_size, __builtin_amdgcn_readfirstlane(lo), t);
+}
+// By a lane of its own, for its row
+__device__ __forceinline__ pg_request pg_find(const sah_page_requests& R, int page_size, int t) {
+  int lo = 0, hi = R.n_requests;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (R.cu_new[mid + 1] > t) hi = mid; else lo = mid + 1;
+  }
+  return lo < R.n_requests ? pg_read(R, page_size, lo, t) : pg_none();
+}
+
+// ---------------------------------------------------------------------------
+// host: checks that the entry points share. They change what has no meaning (strides of dimensions of one entry) in a copy.
+// ---------------------------------------------------------------------------
+static inline int pg_check_cache(sah_page_cache& c, bool with_v, const char* what) {
+  if (c.n_pages == 1) c.ks_p = c.vs_p = 0;
+  if (c.page_size == 1) c.ks_t = c.vs_t = c.D;
+  if (c.Hkv == 1) c.ks_h = c.vs_h = 0;
+  if (c.dtype < SAH_F32 || c.dtype > SAH_E4M3) return sah_fail(SAH_EDTYPE, "%s: cache of dtype %d", what, c.dtype);
+  if (c.n_pages <= 0 || c.Hkv <= 0) return sah_fail(SAH_EINVAL, "%s: n_pages and Hkv must be > 0", what);
+  const int unit = c.dtype == SAH_E4M3 ? 16 : 8;
+  if (c.D <= 0 || c.D % unit || c.D > PG_MAX_D) return sah_fail(SAH_ESHAPE, "%s: head_dim %d is not a multiple of %d up to 256", what, c.D, unit);
+  if (c.page_size <= 0 || (c.page_size & (c.page_size - 1))) return sah_fail(SAH_ESHAPE, "%s: page_size %d is not a power of two", what, c.page_size);
+  if (!c.k || (with_v && !c.v)) return sah_fail(SAH_ENULL, "%s: NULL pointer", what);
+  if (c.dtype == SAH_E4M3 && (!c.k_scales || (with_v && !c.v_scales))) return sah_fail(SAH_ENULL, "%s: an 8-bit cache without scales", what);
+  if (!with_v) {
+    c.v = c.k;
+    c.vs_p = c.ks_p; c.vs_t = c.ks_t; c.vs_h = c.ks_h;
+    c.v_scales = c.k_scales;
+  }
+  const int es = pg_size(c.dtype);
+  if (((uint64_t)c.k | (uint64_t)c.v | (uint64_t)(es * (c.ks_p | c.ks_t | c.ks_h | c.vs_p | c.vs_t | c.vs_h))) % 16)
+    return sah_fail(SAH_EINVAL, "%s: the cache's addresses and strides must be multiples of 16 bytes", what);
+  if (c.dtype == SAH_E4M3 && ((uint64_t)c.k_scales | (uint64_t)c.v_scales) % 4) return sah_fail(SAH_EINVAL, "%s: scales must be 4-byte aligned", what);
+  if (c.ks_t < 0 || c.vs_t < 0 || c.ks_t >= 1 << 26 || c.vs_t >= 1 << 26)  // a few tokens of a page: 32-bit offsets
+    return sah_fail(SAH_ESHAPE, "%s: a page's tokens are 2^26 elements or more apart", what);
+  return SAH_OK;
+}
+static inline int pg_check_requests(const sah_page_requests& r, int page_size, bool with_rows, const char* what) {
+  if (r.n_requests <= 0 || r.table_width <= 0 || (with_rows && r.n_tokens < 0))
+    return sah_fail(SAH_EINVAL, "%s: bad sizes (n_requests %d, table_width %d, n_tokens %d)", what, r.n_requests, r.table_width, r.n_tokens);
+  if ((int64_t)r.table_width * page_size > INT32_MAX - 4096) return sah_fail(SAH_ESHAPE, "%s: table_width * page_size passes 2^31 - 4097", what);
+  if (r.table_pitch < r.table_width) return sah_fail(SAH_EINVAL, "%s: table_pitch is less than table_width", what);
+  if (!r.block_table || !r.kv_lens || (with_rows && !r.cu_new)) return sah_fail(SAH_ENULL, "%s: NULL pointer", what);
+  return SAH_OK;
+}
+
+// Where a context's copy goes. Strides of the outputs in elements. A table, where given, names the copies' pages (of a cache whose pages follow
+// each other, table_width a request): what the attention over a copy goes by; what lies behind a context is left as it is then.
+struct pg_load_out {
+  void *k, *v;
+  int64_t s_b, s_h, s_t;
+  int length;
+  int32_t* table;
+};
+int pg_load(const sah_page_cache& c, const sah_page_requests& r, int dtype, const pg_load_out& out, void* stream, const char* what);

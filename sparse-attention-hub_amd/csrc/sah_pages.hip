@@ -1,0 +1,599 @@
+// A paged cache in 8 bits: tokens quantised into their slots, contexts read back. Bounds of pages, and the pages that a token attends to.
+#include "sah_pages.h"
+
+#define PG_NT 256
+#define PG_BOUND_WAVES 8192
+
+// ---------------------------------------------------------------------------
+// store: 16 lanes hold a row (token, key head) of one matrix, 8 elements each (16 beyond 128 dims)
+// ---------------------------------------------------------------------------
+// exponent of the scale of a row whose largest magnitude is `most`: the least e >= -110 with most <= 448 * 2^e = 1.75 * 2^(e + 8)
+__device__ __forceinline__ int pg_exponent(float most) {
+  const uint32_t bits = sah_float_to_bits(most);
+  const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u);  // (a subnormal's field is 0: far below -110)
+  return e > -110 ? e : -110;
+}
+__device__ __forceinline__ float pg_row16_max(float v) {
+  v = fmaxf(v, sah_dpp<0xB1>(v));
+  v = fmaxf(v, sah_dpp<0x4E>(v));
+  v = fmaxf(v, sah_dpp<0x141>(v));
+  return fmaxf(v, sah_dpp<0x140>(v));
+}
+// (the converter rounds to the nearest, ties to even, and gives NaN for what is not finite)
+__device__ __forceinline__ uint32_t pg_narrow4(float a, float b, float c, float d) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+#else
+  return 0;
+#endif
+}
+
+template <int T>
+__global__ __launch_bounds__(PG_NT) void k_page_store(sah_page_store_args P) {
+  sah_touch_kernargs<sizeof(sah_page_store_args)>();
+  constexpr int ES = pg_size(T);
+  const sah_page_cache& C = P.cache;
+  const int64_t row = (int64_t)blockIdx.x * (PG_NT / 16) + threadIdx.x / 16;
+  const int l16 = threadIdx.x & 15;
+  const int64_t t = row / C.Hkv;
+  const int h = (int)(row - t * C.Hkv);
+  const bool v = blockIdx.y != 0;
+  // (all 16 lanes of a row go the same way)
+  if (t >= P.n_tokens) return;
+  const int64_t slot = P.slot_map[t];
+  if (slot < 0 || slot >= (int64_t)C.n_pages * C.page_size) return;
+  const char* from = (const char*)(v ? P.v : P.k) + (t * (v ? P.vs_t : P.ks_t) + h * (v ? P.vs_h : P.ks_h)) * ES;
+  float x[2][8];
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = 8 * l16 + 128 * i;
+    if (d < C.D) {
+      sah_load8<T>(from, d, x[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = fabsf(x[i][e]);
+      most = fmaxf(most, a < INFINITY ? a : 0.f);
+    }
+  }
+  const int e = pg_exponent(pg_row16_max(most));
+  const float up = sah_bits_to_float((uint32_t)(127 - e) << 23);
+  const int64_t page = slot / C.page_size, entry = slot - page * C.page_size;
+  uint8_t* to = (uint8_t*)(v ? C.v : C.k) + page * (v ? C.vs_p : C.ks_p) + entry * (v ? C.vs_t : C.ks_t) + h * (v ? C.vs_h : C.ks_h);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = 8 * l16 + 128 * i;
+    if (d >= C.D) continue;
+    *(uint2*)(to + d) = make_uint2(pg_narrow4(x[i][0] * up, x[i][1] * up, x[i][2] * up, x[i][3] * up),
+                                   pg_narrow4(x[i][4] * up, x[i][5] * up, x[i][6] * up, x[i][7] * up));
+  }
+  if (l16 == 0) (v ? C.v_scales : C.k_scales)[(page * C.Hkv + h) * C.page_size + entry] = (uint8_t)(e + 127);
+}
+
+// ---------------------------------------------------------------------------
+// load: a thread holds 16 elements of the cache (8-bit) or 16 bytes of it (others: copied as they are)
+// ---------------------------------------------------------------------------
+// what 16 elements of e4m3 are in type T, stored at `to`
+template <int T>
+__device__ __forceinline__ void pg_put16(char* to, uint4 x, float scale) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  if constexpr (T == SAH_BF16) {
+    ((uint4*)to)[0] = make_uint4(pg_widen2<false>(w[0], scale), pg_widen2<true>(w[0], scale), pg_widen2<false>(w[1], scale), pg_widen2<true>(w[1], scale));
+    ((uint4*)to)[1] = make_uint4(pg_widen2<false>(w[2], scale), pg_widen2<true>(w[2], scale), pg_widen2<false>(w[3], scale), pg_widen2<true>(w[3], scale));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[4];
+      pg_widen4(w[i], scale, f);
+      if constexpr (T == SAH_F32) {
+        ((float4*)to)[i] = make_float4(f[0], f[1], f[2], f[3]);
+      } else {
+        // (a row's largest may have been rounded up past the type's; NaN stays)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = f[e] > 65504.f ? 65504.f : (f[e] < -65504.f ? -65504.f : f[e]);
+        ((uint2*)to)[i] = make_uint2(sah_pack2_hw<SAH_F16>(f[0], f[1]), sah_pack2_hw<SAH_F16>(f[2], f[3]));
+      }
+    }
+  }
+}
+// CT: type of the cache; OT: of the output (other caches than SAH_E4M3: the same)
+template <int CT, int OT>
+__global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_requests R, pg_load_out O, int64_t n_units) {
+  sah_touch_kernargs<sizeof(sah_page_cache) + sizeof(sah_page_requests) + sizeof(pg_load_out) + 8>();
+  constexpr int CS = pg_size(CT), OS = pg_size(OT), E = 16 / CS;  // elements of a unit
+  const int units = C.D / E, unit_h = units * C.Hkv;
+  const int64_t u = (int64_t)blockIdx.x * PG_NT + threadIdx.x;
+  if (u >= n_units) return;
+  // consecutive threads: a token's units, all heads of it, then the next token: as the cache lies
+  const int64_t token = u / unit_h;
+  const int in = (int)(u - token * unit_h), h = in / units, c = in - h * units;
+  const int b = (int)(token / O.length), t = (int)(token - (int64_t)b * O.length);
+  const int shift = 31 - __builtin_clz(C.page_size), j = t >> shift, entry = t & (C.page_size - 1);
+  const int page = t < R.kv_lens[b] && j < R.table_width ? R.block_table[(int64_t)b * R.table_pitch + j] : -1;
+  const bool there = page >= 0 && page < C.n_pages;
+  if (O.table && entry == 0 && in == 0) O.table[(int64_t)b * R.table_width + j] = there ? b * R.table_width + j : -1;
+  if (O.table && !there) return;
+  const int64_t to = (b * O.s_b + h * O.s_h + t * O.s_t + (int64_t)c * E) * OS;
+  char *ko = (char*)O.k + to, *vo = (char*)O.v + to;
+  if (!there) {
+#pragma unroll
+    for (int i = 0; i < E * OS / 16; ++i) ((uint4*)ko)[i] = ((uint4*)vo)[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const uint4 k = *(const uint4*)((const char*)C.k + (page * C.ks_p + entry * C.ks_t + h * C.ks_h) * CS + 16 * c);
+  const uint4 v = *(const uint4*)((const char*)C.v + (page * C.vs_p + entry * C.vs_t + h * C.vs_h) * CS + 16 * c);
+  if constexpr (CT == SAH_E4M3) {
+    const int64_t s = ((int64_t)page * C.Hkv + h) * C.page_size + entry;
+    const float ks = pg_scale(C.k_scales[s]), vs = pg_scale(C.v_scales[s]);
+    pg_put16<OT>(ko, k, ks);
+    pg_put16<OT>(vo, v, vs);
+  } else {
+    *(uint4*)ko = k;
+    *(uint4*)vo = v;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// bounds: a wave has every n_waves-th of the pages that a request has filled, for one key head
+// ---------------------------------------------------------------------------
+// (a NaN is kept: comparisons with it are false)
+__device__ __forceinline__ float pg_lower(float a, float b) { return b < a || b != b ? b : a; }
+__device__ __forceinline__ float pg_upper(float a, float b) { return b > a || b != b ? b : a; }
+template <int T>
+__global__ __launch_bounds__(PG_NT) void k_page_bounds(sah_page_bounds_args P, int n_waves) {
+  sah_touch_kernargs<sizeof(sah_page_bounds_args) + 4>();
+  const sah_page_cache& C = P.cache;
+  const sah_page_requests& R = P.requests;
+  constexpr int NW = PG_NT / SAH_WAVE, E = 8;
+  constexpr int BT = T == SAH_E4M3 ? SAH_BF16 : T;
+  const int lane = threadIdx.x & (SAH_WAVE - 1), l16 = lane & 15, g = lane >> 4, wave = sah_wave_id();
+  // key heads of a page next to each other
+  const int64_t item = (int64_t)blockIdx.x * NW + wave, row = item / C.Hkv;
+  const int h = (int)(item - row * C.Hkv), b = (int)(row / n_waves), turn = (int)(row - (int64_t)b * n_waves);
+  if (b >= R.n_requests) return;
+  const int shift = 31 - __builtin_clz(C.page_size), most = R.table_width << shift;
+  const int given = R.kv_lens[b];
+  const int64_t fresh = (int64_t)R.cu_new[b + 1] - R.cu_new[b];
+  const int kv = given < 0 ? 0 : (given < most ? given : most);
+  const int64_t before = (int64_t)given - (fresh > 0 ? fresh : 0);
+  const int first = before <= 0 ? 0 : (before < kv ? (int)before : kv) >> shift, end = fresh > 0 ? kv >> shift : 0;
+  for (int j = first + turn; j < end; j += n_waves) {
+    const int64_t pg = R.block_table[(int64_t)b * R.table_pitch + j];
+    if (pg < 0 || pg >= C.n_pages) continue;
+    for (int d0 = 0; d0 < C.D; d0 += 16 * E) {  // 16 lanes' dims at a time
+      const int d = d0 + l16 * E;
+      const bool on = d < C.D;
+      float lo[E], hi[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        lo[e] = INFINITY;
+        hi[e] = -INFINITY;
+      }
+      for (int i = g; i < C.page_size; i += 4) {
+        float x[E];
+        if constexpr (T == SAH_E4M3) {
+          const float scale = pg_scale(C.k_scales[(pg * C.Hkv + h) * C.page_size + i]);
+          const uint2 w = *(const uint2*)((const uint8_t*)C.k + pg * C.ks_p + i * C.ks_t + h * C.ks_h + (on ? d : 0));
+          float a[4], b[4];
+          pg_widen4(w.x, scale, a);
+          pg_widen4(w.y, scale, b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = a[e];
+            x[4 + e] = b[e];
+          }
+        } else {
+          sah_load8<T>(C.k, pg * C.ks_p + i * C.ks_t + h * C.ks_h + (on ? d : 0), x);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          lo[e] = pg_lower(lo[e], x[e]);
+          hi[e] = pg_upper(hi[e], x[e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+#pragma unroll
+        for (int m = 16; m < SAH_WAVE; m *= 2) {
+          lo[e] = pg_lower(lo[e], __shfl_xor(lo[e], m));
+          hi[e] = pg_upper(hi[e], __shfl_xor(hi[e], m));
+        }
+      }
+      if (!on || g > 1) continue;
+      const int64_t to = ((pg * C.Hkv + h) * 2 + g) * C.D + d;
+#pragma unroll
+      for (int e = 0; e < E; ++e) sah_store<BT>(P.bounds, to + e, g ? hi[e] : lo[e]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// select: a 64-bit key per candidate (larger: rather taken), then the largest of a row
+// ---------------------------------------------------------------------------
+#define PG_ALWAYS ~0ull        // pages that are taken whatever they score
+#define PG_FIRST (~0ull - 1)   // scores that are not finite
+#define PG_WAVE_PAGES 32       // pages that a wave scores
+
+__device__ __forceinline__ uint64_t pg_key(double score) {  // never 0
+  if (!(score - score == 0.0)) return PG_FIRST;
+  const uint64_t u = __builtin_bit_cast(uint64_t, score + 0.0);  // (-0 + 0 is 0)
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+template <int CTRL>
+__device__ __forceinline__ double pg_dpp(double v) {
+  return __builtin_bit_cast(double, sah_dpp_u64<CTRL, 0xF, true>(__builtin_bit_cast(uint64_t, v)));
+}
+
+struct pg_select {
+  sah_page_select_args a;
+  int pitch;    // keys of a row
+  int chunks;   // workgroups a row, which take its pages in turn
+};
+
+// BT: type of the bounds, DP: D up to 64, 128 or 256. L lanes hold a page's row of bounds, E elements of each of the two.
+template <int BT, int DP>
+__global__ __launch_bounds__(PG_NT) void k_page_scores(pg_select S) {
+  sah_touch_kernargs<sizeof(pg_select)>();
+  const sah_page_select_args& P = S.a;
+  const sah_page_requests& R = P.requests;
+  constexpr int NW = PG_NT / SAH_WAVE, ES = pg_size(BT), E = 16 / ES, L = DP / E;
+  constexpr int AT_ONCE = SAH_WAVE / L;                    // pages in a load instruction
+  constexpr int U = PG_WAVE_PAGES / AT_ONCE < 8 ? PG_WAVE_PAGES / AT_ONCE : 8;
+  const int lane = threadIdx.x & (SAH_WAVE - 1), in = lane % L, who = lane / L, wave = sah_wave_id();
+  const int64_t row = blockIdx.x / S.chunks;
+  const int chunk = (int)(blockIdx.x - row * S.chunks);
+  const int64_t t = row / P.Hkv;
+  const int h = (int)(row - t * P.Hkv);
+  const pg_request r = pg_find_by_wave(R, P.page_size, (int)t);
+  if (r.b < 0) return;
+  int64_t p = r.base + t;
+  if (p >= r.kv) p = r.kv - 1;
+  if (p < 0) return;
+  const int shift = 31 - __builtin_clz(P.page_size), n = (int)(p >> shift) + 1;
+  if ((chunk * NW + wave) * PG_WAVE_PAGES >= n) return;
+  // the group's queries, the positive and the negative ones of a channel added up (G numbers of 24 bits: exact for what is not wide apart)
+  const int G = P.Hq / P.Hkv;
+  double up[E], down[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) up[e] = down[e] = 0.0;
+  if (in * E < P.D) {
+    for (int i = 0; i < G; ++i) {
+      const int64_t at = t * P.qs_t + (int64_t)(h * G + i) * P.qs_h + in * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const double q = P.dtype == SAH_F32 ? sah_load<SAH_F32>(P.q, at + e) : P.dtype == SAH_BF16 ? sah_load<SAH_BF16>(P.q, at + e) : sah_load<SAH_F16>(P.q, at + e);
+        if (q < 0.0) down[e] += q;
+        else up[e] += q;  // (NaN too)
+      }
+    }
+  }
+  uint64_t* keys = (uint64_t*)P.work + row * S.pitch;
+  const char* base = (const char*)P.bounds + (int64_t)h * 2 * P.D * ES;
+  for (int64_t from = (chunk * NW + wave) * PG_WAVE_PAGES; from < n; from += (int64_t)S.chunks * NW * PG_WAVE_PAGES) {
+    // a lane's page
+    const int j0 = (int)from, j = j0 + lane;
+    const bool mine = lane < PG_WAVE_PAGES && j < n;
+    int page = mine ? R.block_table[(int64_t)r.b * R.table_pitch + j] : -1;
+    if (page >= P.n_pages) page = -1;
+    const bool always = j < P.sink_pages || j >= n - P.window_pages;
+    for (int i0 = 0; i0 < PG_WAVE_PAGES; i0 += U * AT_ONCE) {
+      if (j0 + i0 >= n) break;
+      uint4 lo[U], hi[U];
+      int at[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        at[i] = __shfl(always ? -1 : page, i0 + i * AT_ONCE + who);
+        lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+        if (at[i] >= 0 && in * E < P.D) {
+          const char* b = base + (int64_t)at[i] * P.Hkv * 2 * P.D * ES + 16 * in;
+          lo[i] = *(const uint4*)b;
+          hi[i] = *(const uint4*)(b + P.D * ES);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const uint32_t a[4] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w}, z[4] = {hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+        double sum = 0.0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if constexpr (BT == SAH_F32) {
+            sum = fma(down[w], (double)sah_bits_to_float(a[w]), sum);
+            sum = fma(up[w], (double)sah_bits_to_float(z[w]), sum);
+          } else {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              float x, y;
+              if constexpr (BT == SAH_BF16) {
+                x = sah_bits_to_float(half ? a[w] & 0xffff0000u : a[w] << 16);
+                y = sah_bits_to_float(half ? z[w] & 0xffff0000u : z[w] << 16);
+              } else {
+                x = sah_f16_to_float((uint16_t)(a[w] >> (16 * half)));
+                y = sah_f16_to_float((uint16_t)(z[w] >> (16 * half)));
+              }
+              sum = fma(down[2 * w + half], (double)x, sum);
+              sum = fma(up[2 * w + half], (double)y, sum);
+            }
+          }
+        }
+        if constexpr (L >= 2) sum += pg_dpp<0xB1>(sum);
+        if constexpr (L >= 4) sum += pg_dpp<0x4E>(sum);
+        if constexpr (L >= 8) sum += pg_dpp<0x141>(sum);
+        if constexpr (L >= 16) sum += pg_dpp<0x140>(sum);
+        if constexpr (L >= 32) sum += __shfl_xor(sum, 16);
+        if constexpr (L >= 64) sum += __shfl_xor(sum, 32);
+        const int to = j0 + i0 + i * AT_ONCE + who;
+        if (in == 0 && at[i] >= 0 && to < n) keys[to] = pg_key(sum);
+      }
+    }
+    if (mine && (always || page < 0)) keys[j] = page < 0 ? 0 : PG_ALWAYS;
+  }
+}
+
+// One workgroup a row: the n_select-th largest key by digits of 8 bits, from the highest bit on in which the row's keys differ, in LDS
+// histograms; then the places of what is taken, in the order of the table. A thread has neighbouring pages.
+__global__ __launch_bounds__(PG_NT) void k_page_top(pg_select S) {
+  sah_touch_kernargs<sizeof(pg_select)>();
+  const sah_page_select_args& P = S.a;
+  constexpr int NW = PG_NT / SAH_WAVE, KEEP = 8;
+  __shared__ int s_hist[256], s_scan[NW + 1];
+  __shared__ uint64_t s_min[NW], s_max[NW];
+  __shared__ int s_bin, s_above, s_count;
+  const int64_t row = blockIdx.x, t = row / P.Hkv;
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
+  const pg_request r = pg_find_by_wave(P.requests, P.page_size, (int)t);
+  int64_t p = r.b < 0 ? -1 : r.base + t;
+  if (p >= r.kv) p = r.kv - 1;
+  const int shift = 31 - __builtin_clz(P.page_size), n = p < 0 ? 0 : (int)(p >> shift) + 1;
+  int32_t* out = P.pages + row * P.n_select;
+  const uint64_t* keys = (const uint64_t*)P.work + row * S.pitch;
+  const int each = (n + PG_NT - 1) / PG_NT, first = (int)threadIdx.x * each;
+  const bool kept = each <= KEEP;  // in registers, else read again in every pass
+  uint64_t mine[KEEP];
+#pragma unroll
+  for (int i = 0; i < KEEP; ++i) mine[i] = kept && i < each && first + i < n ? keys[first + i] : 0;
+  auto visit = [&](auto f) __attribute__((always_inline)) {
+    if (kept) {
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i)
+        if (i < each) f(first + i, mine[i]);
+    } else {
+      for (int i = 0; i < each; ++i) f(first + i, first + i < n ? keys[first + i] : 0);
+    }
+  };
+  // candidates, the smallest and the largest key of them
+  uint64_t least = ~0ull, most = 0;
+  int count = 0;
+  visit([&](int, uint64_t key) {
+    if (!key) return;
+    ++count;
+    least = key < least ? key : least;
+    most = key > most ? key : most;
+  });
+#pragma unroll
+  for (int m = 1; m < SAH_WAVE; m *= 2) {
+    const uint64_t a = __shfl_xor(least, m), b = __shfl_xor(most, m);
+    least = a < least ? a : least;
+    most = b > most ? b : most;
+  }
+  if (lane == 0) {
+    s_min[wave] = least;
+    s_max[wave] = most;
+  }
+  int total;
+  (void)sah_block_excl_scan<PG_NT>(count, s_scan, &total);
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    least = s_min[i] < least ? s_min[i] : least;
+    most = s_max[i] > most ? s_max[i] : most;
+  }
+  uint64_t border = 1;         // keys above it are taken, and the first `ties` that are equal
+  int ties = total;
+  if (total > P.n_select) {
+    int want = P.n_select;
+    const uint64_t differ = least ^ most;
+    int low = differ ? 64 - __builtin_clzll(differ) : 0;  // bits below it are still to be looked at
+    uint64_t prefix = low < 64 ? most >> low : 0;
+    border = most;
+    ties = want;
+    while (low > 0) {  // (at most 8 times)
+      const int width = low < 8 ? low : 8, next = low - width;
+      for (int i = threadIdx.x; i < 256; i += PG_NT) s_hist[i] = 0;
+      __syncthreads();
+      visit([&](int, uint64_t key) {
+        if (key && (low < 64 ? key >> low : 0) == prefix) atomicAdd(&s_hist[(key >> next) & ((1u << width) - 1)], 1);
+      });
+      __syncthreads();
+      if (wave == 0) {  // the digit at which the count, from the largest down, reaches `want`: four digits a lane, the largest in lane 0
+        int c[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += c[i] = s_hist[255 - 4 * lane - i];
+        int above = sah_wave_incl_scan(sum) - sum;
+        if (above < want && want <= above + sum) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (above < want && want <= above + c[i]) {
+              s_bin = 255 - 4 * lane - i;
+              s_above = above;
+              s_count = c[i];
+            }
+            above += c[i];
+          }
+        }
+      }
+      __syncthreads();
+      want -= s_above;
+      prefix = (low < 64 ? prefix << width : 0) | (uint64_t)s_bin;
+      low = next;
+      border = prefix << low;
+      ties = want;
+      if (s_count == want) {  // all of the digit's keys: what is at least its first number
+        ties = total;
+        break;
+      }
+      // (the next write of s_bin and s_count lies behind two waits)
+    }
+  }
+  // keys above the border, and equal ones while they last; a digit that is taken whole begins at the border
+  int above = 0, equal = 0;
+  visit([&](int, uint64_t key) {
+    above += key > border;
+    equal += key == border;
+  });
+  int all_above, all_equal;
+  int before = sah_block_excl_scan<PG_NT>(above, s_scan, &all_above);
+  int ranked = sah_block_excl_scan<PG_NT>(equal, s_scan, &all_equal);
+  const int taken_equal = all_equal < ties ? all_equal : ties;
+  visit([&](int j, uint64_t key) {
+    const bool eq = key == border, take = key > border || (eq && ranked < ties);
+    if (take) out[before + (ranked < ties ? ranked : ties)] = j;
+    before += key > border;
+    ranked += eq;
+  });
+  for (int i = all_above + taken_equal + (int)threadIdx.x; i < P.n_select; i += PG_NT) out[i] = -1;
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+extern "C" int sah_page_store(const sah_page_store_args* given) {
+  static const char* what = "sah_page_store";
+  if (!given) return sah_fail(SAH_ENULL, "sah_page_store: args is NULL");
+  sah_page_store_args own = *given;
+  sah_page_store_args* a = &own;
+  sah_page_cache& c = a->cache;
+  if (int rc = pg_check_cache(c, true, what)) return rc;
+  if (c.dtype != SAH_E4M3) return sah_fail(SAH_EDTYPE, "sah_page_store: the cache's dtype is %d, not SAH_E4M3", c.dtype);
+  if (a->dtype != SAH_F32 && a->dtype != SAH_BF16 && a->dtype != SAH_F16) return sah_fail(SAH_EDTYPE, "sah_page_store: dtype %d", a->dtype);
+  if (a->n_tokens < 0) return sah_fail(SAH_EINVAL, "sah_page_store: n_tokens is negative");
+  if (a->n_tokens == 0) return SAH_OK;
+  if (!a->k || !a->v || !a->slot_map) return sah_fail(SAH_ENULL, "sah_page_store: NULL pointer");
+  if (a->n_tokens == 1) a->ks_t = a->vs_t = 0;
+  if (c.Hkv == 1) a->ks_h = a->vs_h = 0;
+  const int es = pg_size(a->dtype);
+  if (((uint64_t)a->k | (uint64_t)a->v | (uint64_t)(es * (a->ks_t | a->ks_h | a->vs_t | a->vs_h))) % 16)
+    return sah_fail(SAH_EINVAL, "sah_page_store: addresses and strides must be multiples of 16 bytes");
+  if (!sah_rows_apart<3>(c.D, {c.ks_p, c.ks_t, c.ks_h}, {c.n_pages, c.page_size, c.Hkv}) ||
+      !sah_rows_apart<3>(c.D, {c.vs_p, c.vs_t, c.vs_h}, {c.n_pages, c.page_size, c.Hkv}))
+    return sah_fail(SAH_EINVAL, "sah_page_store: rows of a cache overlap");
+  const int64_t wgs = ((int64_t)a->n_tokens * c.Hkv + PG_NT / 16 - 1) / (PG_NT / 16);
+  if (wgs > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_store: too many rows");
+  sah_timed timed("k_page_store", a->stream);
+  const dim3 grid((unsigned)wgs, 2);
+  hipStream_t st = (hipStream_t)a->stream;
+  if (a->dtype == SAH_F32) hipLaunchKernelGGL(k_page_store<SAH_F32>, grid, dim3(PG_NT), 0, st, *a);
+  else if (a->dtype == SAH_BF16) hipLaunchKernelGGL(k_page_store<SAH_BF16>, grid, dim3(PG_NT), 0, st, *a);
+  else hipLaunchKernelGGL(k_page_store<SAH_F16>, grid, dim3(PG_NT), 0, st, *a);
+  return sah_launch_status(what);
+}
+
+// (also what the attention over chunks makes its copy with)
+int pg_load(const sah_page_cache& c, const sah_page_requests& r, int dtype, const pg_load_out& out, void* stream, const char* what) {
+  const int64_t units = (int64_t)c.D * pg_size(c.dtype) / 16 * c.Hkv * out.length * r.n_requests, wgs = (units + PG_NT - 1) / PG_NT;
+  if (wgs > 0x7fffffff) return sah_fail(SAH_ESHAPE, "%s: too many elements", what);
+  sah_timed timed("k_page_load", stream);
+  const dim3 grid((unsigned)wgs);
+  hipStream_t st = (hipStream_t)stream;
+  if (c.dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_F32, SAH_F32>), grid, dim3(PG_NT), 0, st, c, r, out, units);
+  else if (c.dtype != SAH_E4M3) hipLaunchKernelGGL((k_page_load<SAH_BF16, SAH_BF16>), grid, dim3(PG_NT), 0, st, c, r, out, units);
+  else if (dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F32>), grid, dim3(PG_NT), 0, st, c, r, out, units);
+  else if (dtype == SAH_BF16) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_BF16>), grid, dim3(PG_NT), 0, st, c, r, out, units);
+  else hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F16>), grid, dim3(PG_NT), 0, st, c, r, out, units);
+  return sah_launch_status(what);
+}
+
+extern "C" int sah_page_load(const sah_page_load_args* given) {
+  static const char* what = "sah_page_load";
+  if (!given) return sah_fail(SAH_ENULL, "sah_page_load: args is NULL");
+  sah_page_load_args own = *given;
+  sah_page_load_args* a = &own;
+  sah_page_cache& c = a->cache;
+  if (int rc = pg_check_cache(c, true, what)) return rc;
+  if (int rc = pg_check_requests(a->requests, c.page_size, false, what)) return rc;
+  if (c.dtype == SAH_E4M3 ? a->dtype != SAH_F32 && a->dtype != SAH_BF16 && a->dtype != SAH_F16 : a->dtype != c.dtype)
+    return sah_fail(SAH_EDTYPE, "sah_page_load: dtype %d of a cache of dtype %d", a->dtype, c.dtype);
+  if (a->length < 0) return sah_fail(SAH_EINVAL, "sah_page_load: length is negative");
+  if (a->length == 0) return SAH_OK;
+  if (!a->k_out || !a->v_out) return sah_fail(SAH_ENULL, "sah_page_load: NULL pointer");
+  if (((uint64_t)a->k_out | (uint64_t)a->v_out) % 16) return sah_fail(SAH_EINVAL, "sah_page_load: addresses must be multiples of 16 bytes");
+  const int64_t row = c.D, head = row * a->length;
+  return pg_load(c, a->requests, a->dtype, pg_load_out{a->k_out, a->v_out, head * c.Hkv, head, row, a->length, nullptr}, a->stream, what);
+}
+
+extern "C" int sah_page_bounds(const sah_page_bounds_args* given) {
+  static const char* what = "sah_page_bounds";
+  if (!given) return sah_fail(SAH_ENULL, "sah_page_bounds: args is NULL");
+  sah_page_bounds_args own = *given;
+  sah_page_bounds_args* a = &own;
+  sah_page_cache& c = a->cache;
+  if (int rc = pg_check_cache(c, false, what)) return rc;
+  if (int rc = pg_check_requests(a->requests, c.page_size, true, what)) return rc;
+  if (!a->bounds) return sah_fail(SAH_ENULL, "sah_page_bounds: NULL pointer");
+  if ((uint64_t)a->bounds % 16) return sah_fail(SAH_EINVAL, "sah_page_bounds: addresses must be multiples of 16 bytes");
+  // Enough waves for the card where few requests have filled many pages; each of many requests' fills few.
+  const int64_t rows = (int64_t)a->requests.n_requests * c.Hkv;
+  int64_t n_waves = PG_BOUND_WAVES / rows;
+  n_waves = n_waves < 1 ? 1 : (n_waves < a->requests.table_width ? n_waves : a->requests.table_width);
+  const int64_t wgs = (rows * n_waves + PG_NT / SAH_WAVE - 1) / (PG_NT / SAH_WAVE);
+  if (wgs > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_bounds: too many rows");
+  sah_timed timed("k_page_bounds", a->stream);
+  const dim3 grid((unsigned)wgs);
+  hipStream_t st = (hipStream_t)a->stream;
+  if (c.dtype == SAH_F32) hipLaunchKernelGGL(k_page_bounds<SAH_F32>, grid, dim3(PG_NT), 0, st, *a, (int)n_waves);
+  else if (c.dtype == SAH_BF16) hipLaunchKernelGGL(k_page_bounds<SAH_BF16>, grid, dim3(PG_NT), 0, st, *a, (int)n_waves);
+  else if (c.dtype == SAH_F16) hipLaunchKernelGGL(k_page_bounds<SAH_F16>, grid, dim3(PG_NT), 0, st, *a, (int)n_waves);
+  else hipLaunchKernelGGL(k_page_bounds<SAH_E4M3>, grid, dim3(PG_NT), 0, st, *a, (int)n_waves);
+  return sah_launch_status(what);
+}
+
+extern "C" int64_t sah_page_select_work_bytes(const sah_page_select_args* a) {
+  if (!a || a->requests.n_tokens <= 0 || a->Hkv <= 0 || a->requests.table_width <= 0) return 0;
+  return (int64_t)a->requests.n_tokens * a->Hkv * a->requests.table_width * 8;
+}
+
+extern "C" int sah_page_select(const sah_page_select_args* given) {
+  if (!given) return sah_fail(SAH_ENULL, "sah_page_select: args is NULL");
+  sah_page_select_args own = *given;
+  sah_page_select_args* a = &own;
+  if (a->dtype != SAH_F32 && a->dtype != SAH_BF16 && a->dtype != SAH_F16) return sah_fail(SAH_EDTYPE, "sah_page_select: dtype %d", a->dtype);
+  if (a->bounds_dtype != SAH_F32 && a->bounds_dtype != SAH_BF16 && a->bounds_dtype != SAH_F16)
+    return sah_fail(SAH_EDTYPE, "sah_page_select: bounds of dtype %d", a->bounds_dtype);
+  if (a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->n_pages <= 0 || a->max_context < 0)
+    return sah_fail(SAH_EINVAL, "sah_page_select: bad sizes (heads %d / %d, n_pages %d, max_context %d)", a->Hq, a->Hkv, a->n_pages, a->max_context);
+  if (a->D <= 0 || a->D % 8 || a->D > PG_MAX_D) return sah_fail(SAH_ESHAPE, "sah_page_select: head_dim %d is not a multiple of 8 up to 256", a->D);
+  if (a->page_size <= 0 || (a->page_size & (a->page_size - 1))) return sah_fail(SAH_ESHAPE, "sah_page_select: page_size %d is not a power of two", a->page_size);
+  if (a->sink_pages < 0 || a->window_pages < 1 || (int64_t)a->sink_pages + a->window_pages > a->n_select)
+    return sah_fail(SAH_EINVAL, "sah_page_select: %d first and %d last pages of %d", a->sink_pages, a->window_pages, a->n_select);
+  if (int rc = pg_check_requests(a->requests, a->page_size, true, "sah_page_select")) return rc;
+  if (a->requests.n_tokens == 0) return SAH_OK;
+  if (!a->q || !a->bounds || !a->pages) return sah_fail(SAH_ENULL, "sah_page_select: NULL pointer");
+  if ((uint64_t)a->bounds % 16) return sah_fail(SAH_EINVAL, "sah_page_select: bounds must be 16-byte aligned");
+  if (!a->work || a->work_bytes < sah_page_select_work_bytes(a) || (uint64_t)a->work % 16) return sah_fail(SAH_ECAPACITY, "sah_page_select: work is too small");
+  if (a->requests.n_tokens == 1) a->qs_t = 0;
+  if (a->Hq == 1) a->qs_h = 0;
+  const int64_t rows = (int64_t)a->requests.n_tokens * a->Hkv;
+  const int per = PG_WAVE_PAGES * (PG_NT / SAH_WAVE), width = a->requests.table_width;
+  const int64_t hint = ((int64_t)a->max_context + a->page_size - 1) / a->page_size;
+  const int usual = hint > 0 && hint < width ? (int)hint : width;  // pages of the longest request, by what the caller says
+  const pg_select s{*a, width, (usual + per - 1) / per};
+  if (rows * s.chunks > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_select: too many rows");
+  hipStream_t st = (hipStream_t)a->stream;
+  const dim3 grid((unsigned)(rows * s.chunks));
+  {
+    sah_timed timed("k_page_scores", a->stream);
+    const int dp = a->D <= 64 ? 64 : a->D <= 128 ? 128 : 256;
+#define PG_CASE(bt, d) if (a->bounds_dtype == bt && dp == d) hipLaunchKernelGGL((k_page_scores<bt, d>), grid, dim3(PG_NT), 0, st, s);
+    PG_CASE(SAH_F32, 64) PG_CASE(SAH_F32, 128) PG_CASE(SAH_F32, 256)
+    PG_CASE(SAH_BF16, 64) PG_CASE(SAH_BF16, 128) PG_CASE(SAH_BF16, 256)
+    PG_CASE(SAH_F16, 64) PG_CASE(SAH_F16, 128) PG_CASE(SAH_F16, 256)
+#undef PG_CASE
+    if (int rc = sah_launch_status("sah_page_select")) return rc;
+  }
+  sah_timed timed("k_page_top", a->stream);
+  hipLaunchKernelGGL(k_page_top, dim3((unsigned)rows), dim3(PG_NT), 0, st, s);
+  return sah_launch_status("sah_page_select(top)");
+}

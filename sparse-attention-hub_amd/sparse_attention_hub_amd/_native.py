@@ -1,4 +1,4 @@
-"""ctypes binding of libsah_mi355.so (declared in include/sah.h, sah_ext.h and sah_serve.h).
+"""ctypes binding of libsah_mi355.so (declared in include/sah.h, sah_ext.h, sah_serve.h and sah_pages.h).
 
 The library is the only compute back end of this package: every masker and the
 masked attention call into it, and a missing library is an error, not a reason
@@ -75,6 +75,11 @@ SERVE_SYMBOLS = (
     "sah_paged_attention",
     "sah_sample_tokens",
 )
+
+# include/sah_pages.h: a paged cache in 8 bits, attention over selected pages
+PAGE_SYMBOLS = ("sah_page_store", "sah_page_load", "sah_page_bounds", "sah_page_select", "sah_page_attention")
+PAGE_SIZE_SYMBOLS = ("sah_page_select_work_bytes", "sah_page_attention_work_bytes")
+SAH_E4M3 = 3  # beside the types of a model: a cache's
 
 
 class NativeLibraryError(RuntimeError):
@@ -517,6 +522,78 @@ class SampleArgs(C.Structure):
     ]
 
 
+class PageCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("ks_p", C.c_int64), ("ks_t", C.c_int64), ("ks_h", C.c_int64),
+        ("v", C.c_void_p), ("vs_p", C.c_int64), ("vs_t", C.c_int64), ("vs_h", C.c_int64),
+        ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+        ("dtype", C.c_int32),
+        ("n_pages", C.c_int32), ("page_size", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+    ]
+
+
+class PageRequests(C.Structure):
+    _fields_ = [
+        ("block_table", C.c_void_p), ("table_pitch", C.c_int64), ("table_width", C.c_int32),
+        ("kv_lens", C.c_void_p),
+        ("cu_new", C.c_void_p),
+        ("n_requests", C.c_int32), ("n_tokens", C.c_int32),
+    ]
+
+
+class PageStoreArgs(C.Structure):
+    _fields_ = [
+        ("cache", PageCache),
+        ("k", C.c_void_p), ("ks_t", C.c_int64), ("ks_h", C.c_int64),
+        ("v", C.c_void_p), ("vs_t", C.c_int64), ("vs_h", C.c_int64),
+        ("slot_map", C.c_void_p),
+        ("dtype", C.c_int32), ("n_tokens", C.c_int32),
+        ("stream", C.c_void_p),
+    ]
+
+
+class PageLoadArgs(C.Structure):
+    _fields_ = [
+        ("cache", PageCache), ("requests", PageRequests),
+        ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+        ("dtype", C.c_int32), ("length", C.c_int32),
+        ("stream", C.c_void_p),
+    ]
+
+
+class PageBoundsArgs(C.Structure):
+    _fields_ = [("cache", PageCache), ("requests", PageRequests), ("bounds", C.c_void_p), ("stream", C.c_void_p)]
+
+
+class PageSelectArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("qs_t", C.c_int64), ("qs_h", C.c_int64),
+        ("bounds", C.c_void_p),
+        ("dtype", C.c_int32), ("bounds_dtype", C.c_int32),
+        ("Hq", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+        ("requests", PageRequests),
+        ("n_select", C.c_int32), ("sink_pages", C.c_int32), ("window_pages", C.c_int32), ("max_context", C.c_int32),
+        ("pages", C.c_void_p),
+        ("work", C.c_void_p), ("work_bytes", C.c_int64),
+        ("stream", C.c_void_p),
+    ]
+
+
+class PageAttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("qs_t", C.c_int64), ("qs_h", C.c_int64),
+        ("cache", PageCache), ("requests", PageRequests),
+        ("pages", C.c_void_p), ("n_select", C.c_int32),
+        ("sinks", C.c_void_p),
+        ("dtype", C.c_int32), ("Hq", C.c_int32),
+        ("max_context", C.c_int32), ("sink", C.c_int32), ("window", C.c_int32),
+        ("scaling", C.c_float),
+        ("out", C.c_void_p), ("os_t", C.c_int64), ("os_h", C.c_int64),
+        ("work", C.c_void_p), ("work_bytes", C.c_int64),
+        ("stream", C.c_void_p),
+    ]
+
+
 _lib: Optional[C.CDLL] = None
 
 
@@ -540,7 +617,7 @@ def lib() -> C.CDLL:
         handle = C.CDLL(str(path))
     except OSError as e:
         raise NativeLibraryError(f"cannot load {path}: {e}") from e
-    missing = [s for s in (*EXPECTED_SYMBOLS, *SERVE_SYMBOLS) if not hasattr(handle, s)]
+    missing = [s for s in (*EXPECTED_SYMBOLS, *SERVE_SYMBOLS, *PAGE_SYMBOLS, *PAGE_SIZE_SYMBOLS) if not hasattr(handle, s)]
     if missing:
         raise NativeLibraryError(f"{path} lacks symbols {missing}; rebuild it")
     handle.sah_version.restype = C.c_int
@@ -574,11 +651,14 @@ def lib() -> C.CDLL:
     for name, n_blocks in EXTENSION_SYMBOLS.items():
         getattr(handle, name).restype = C.c_int
         getattr(handle, name).argtypes = [C.c_void_p] * n_blocks
-    for name in SERVE_SYMBOLS:
+    for name in (*SERVE_SYMBOLS, *PAGE_SYMBOLS):
         getattr(handle, name).restype = C.c_int
         getattr(handle, name).argtypes = [C.c_void_p]
     handle.sah_paged_attention_work_floats.restype = C.c_int64
     handle.sah_paged_attention_work_floats.argtypes = [C.c_void_p]
+    for name in PAGE_SIZE_SYMBOLS:
+        getattr(handle, name).restype = C.c_int64
+        getattr(handle, name).argtypes = [C.c_void_p]
     handle.sah_sample_work_bytes.restype = C.c_int64
     handle.sah_sample_work_bytes.argtypes = [C.c_void_p]
     _lib = handle
@@ -642,6 +722,11 @@ def members_work_floats(B: int, Hq: int, Hkv: int, Lq: int, Lk: int, head_dim: i
 
 def paged_work_floats(args: PagedAttentionArgs) -> int:
     return int(lib().sah_paged_attention_work_floats(C.addressof(args)))
+
+
+def page_work_bytes(name: str, args: C.Structure) -> int:
+    """What `sah_page_<name>` needs of a workspace."""
+    return int(getattr(lib(), f"sah_page_{name}_work_bytes")(C.addressof(args)))
 
 
 def sample_work_bytes(args: SampleArgs) -> int:

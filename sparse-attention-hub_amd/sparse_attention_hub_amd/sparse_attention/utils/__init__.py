@@ -6,7 +6,17 @@ from .mask_attention_utils import (
     get_masked_attention_output,
     get_true_attention_output,
 )
-from .paged_cache import PageAssignment, PagedKVCache, assign_pages, paged_attention, release_pages, store_paged
+from .paged_cache import (
+    PageAssignment,
+    PagedKVCache,
+    assign_pages,
+    load_paged,
+    paged_attention,
+    release_pages,
+    select_pages,
+    store_paged,
+    update_page_bounds,
+)
 from .token_sampling import sample_tokens
 
 __all__ = [
@@ -21,6 +31,9 @@ __all__ = [
     "assign_pages",
     "release_pages",
     "store_paged",
+    "load_paged",
+    "update_page_bounds",
+    "select_pages",
     "paged_attention",
     "sample_tokens",
 ]

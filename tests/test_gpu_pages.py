@@ -1,0 +1,814 @@
+"""A paged cache in 8 bits, bounds of its pages, the pages a token selects and attention over them, against plain implementations in 64 bits."""
+import math
+import random
+
+import pytest
+import torch
+
+from sparse_attention_hub_amd.sparse_attention.utils import paged_cache as P
+
+pytestmark = pytest.mark.gpu
+_HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+_TYPES = [torch.float32, torch.bfloat16, torch.float16]
+_E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_KINDS = [torch.float32, torch.bfloat16, torch.float16, _E4M3]
+
+
+def _i32(v, device):
+    return torch.tensor(v, dtype=torch.int32, device=device)
+
+
+# ------------------------------------------------------------------------------------------------------------- in 64 bits
+def _plain_quantise(rows):
+    """(values, exponents) of include/sah_pages.h's rule, in 64 bits: all steps are exact there but for the one rounding."""
+    x = rows.double()
+    finite = torch.isfinite(x)
+    most = torch.where(finite, x.abs(), 0.0).amax(-1)
+    parts = torch.frexp(most / 448)
+    exponent = (parts.exponent - (parts.mantissa == 0.5).int()).clamp(min=-110)
+    exponent = torch.where(most == 0, -110, exponent)
+    grid = torch.ldexp(torch.ones_like(most), exponent)[..., None]
+    size = x.abs() / grid
+    step = torch.ldexp(torch.ones_like(size), torch.frexp(size.clamp(min=2.0 ** -6)).exponent - 4)
+    return torch.where(finite, torch.sign(x) * torch.round(size / step) * step * grid, math.nan), exponent
+
+
+def _wide(cache, scales=None):
+    """What a cache stands for, on the CPU: (pages, page, kv_heads, head_dim) in 64 bits."""
+    x = cache.cpu().float().double()
+    if scales is None:
+        return x
+    e = scales.cpu().view(torch.uint8).long() - 127
+    return x * torch.ldexp(torch.ones(e.shape, dtype=torch.float64), e).transpose(1, 2)[..., None]
+
+
+def _same_values(a, b):
+    return torch.equal(torch.nan_to_num(a, nan=12345.0), torch.nan_to_num(b, nan=12345.0))
+
+
+# ------------------------------------------------------------------------------------------------------------------ store
+def _special_rows(rows, dtype):
+    """Zeros, one element, powers of two, the type's largest and smallest numbers, ties between neighbours of e4m3, what is not finite."""
+    big, tiny = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal
+    dim = rows.shape[-1]
+    flat = rows.view(-1, dim)
+    special = [torch.zeros(dim), torch.full((dim,), big), torch.full((dim,), tiny), torch.full((dim,), -448.0), torch.full((dim,), 449.0)]
+    ties = torch.tensor([448.0, 1.0625, 1.1875, 17.0, 18.0, 19.0, 2.0 ** -9, 1.5 * 2.0 ** -9, 2.5 * 2.0 ** -9, 2.0 ** -10, 0.75 * 2.0 ** -9, 240.0, 232.0, 0.0, -17.0, -19.0])
+    special.append(ties.repeat(-(-dim // 16))[:dim])
+    one = torch.zeros(dim)
+    one[dim - 1] = -3.7
+    special.append(one)
+    for bad in (math.nan, math.inf, -math.inf):
+        row = torch.linspace(-2, 2, dim)
+        row[dim // 2] = bad
+        special.append(row)
+    special.append(torch.full((dim,), math.nan))
+    special.append(torch.tensor([big, tiny] * (dim // 2)))
+    for i, row in enumerate(special[:flat.shape[0]]):
+        flat[i] = row.to(dtype)
+    return rows
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("tokens, heads, dim, page, layout", [
+    (1, 1, 16, 1, "plain"), (1, 8, 128, 16, "plain"), (9, 3, 48, 4, "interleaved"), (77, 2, 64, 32, "heads_first"), (130, 8, 80, 16, "interleaved"),
+    (300, 4, 256, 64, "plain"), (33, 2, 144, 8, "heads_first"), (1000, 1, 96, 128, "plain"),
+])
+def test_store_quantises(cuda, dtype, tokens, heads, dim, page, layout):
+    """Element for element the rule's: one rounding, so nothing but equality will do."""
+    g = torch.Generator().manual_seed(tokens + dim)
+    pages = 2 + 2 * tokens // page
+    rows = [_special_rows((torch.randn(tokens, heads, dim, generator=g) * torch.exp2(8 * torch.randn(tokens, heads, 1, generator=g))).to(dtype), dtype)
+            for _ in range(2)]
+    slots = torch.randperm(pages * page, generator=g)[:tokens]
+    slots[::7] = torch.tensor([-1, pages * page, 2 ** 40, -2 ** 40])[torch.arange(len(slots[::7])) % 4]
+    before = [torch.randint(0, 0x7e, (pages, page, heads, dim), dtype=torch.uint8, generator=g) for _ in range(2)]
+    scales_before = [torch.randint(100, 140, (pages, heads, page), dtype=torch.uint8, generator=g) for _ in range(2)]
+    given = [r.to(cuda) for r in rows]
+    if layout == "interleaved":
+        both = torch.cat([given[0], given[1]], dim=1)
+        given = [both[:, :heads], both[:, heads:]]
+    caches, scales = [], [s.to(cuda).view(_E8M0) for s in scales_before]
+    for c in before:
+        c = c.to(cuda)
+        if layout == "heads_first":
+            c = c.transpose(1, 2).contiguous().transpose(1, 2)
+        caches.append(c.view(_E4M3))
+    P.store_paged(given[0], given[1], caches[0], caches[1], slots.to(cuda), key_scales=scales[0], value_scales=scales[1])
+    live = (slots >= 0) & (slots < pages * page)
+    for i in range(2):
+        values, exponent = _plain_quantise(rows[i][live])
+        want, want_e = _wide(before[i].view(_E4M3), scales_before[i].view(_E8M0)), scales_before[i].clone()
+        at = slots[live]
+        want[at // page, at % page] = values
+        want_e[at // page, :, at % page] = (exponent + 127).to(torch.uint8)
+        assert torch.equal(scales[i].view(torch.uint8).cpu(), want_e)
+        assert _same_values(_wide(caches[i], scales[i]), want)
+
+
+def test_store_of_no_tokens(cuda):
+    cache, scales = torch.zeros(2, 4, 2, 16, device=cuda).to(_E4M3), torch.zeros(2, 2, 4, dtype=torch.uint8, device=cuda).view(_E8M0)
+    rows = torch.zeros(0, 2, 16, device=cuda)
+    P.store_paged(rows, rows, cache, cache.clone(), torch.zeros(0, dtype=torch.int64, device=cuda), key_scales=scales, value_scales=scales)
+    assert cache.float().eq(0).all()
+
+
+# ----------------------------------------------------------------------------------------------------------- caches for tests
+class Case:
+    """Requests' keys and values in a cache of some kind, the table in disorder; the same in 64 bits."""
+
+    def __init__(self, cuda, kind, new, cached, kv_heads, dim, page, seed=0, missing=(), layout="plain", spare=3, scale=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.new, self.cached, self.page, self.kind, self.kv_heads, self.dim = new, cached, page, kind, kv_heads, dim
+        self.kv = [n + c for n, c in zip(new, cached)]
+        self.width = max(1, max(-(-k // page) for k in self.kv)) + 1
+        pages = sum(-(-k // page) for k in self.kv) + spare
+        order = torch.randperm(pages, generator=g).tolist()
+        table = torch.full((len(new), self.width), -1, dtype=torch.int32)
+        for b, k in enumerate(self.kv):
+            for j in range(-(-k // page)):
+                table[b, j] = order.pop()
+        for b, j, what in missing:
+            table[b, j] = what
+        self.table_host, self.table = table, table.to(cuda)
+        self.cu = [0]
+        for n in new:
+            self.cu.append(self.cu[-1] + n)
+        self.kv_lens, self.cu_new = _i32(self.kv, cuda), _i32(self.cu, cuda)
+        self.caches, self.scales, self.wide = [], [], []
+        for _ in range(2):
+            x = scale * (0.8 * torch.randn(pages, page, kv_heads, dim, generator=g) + 0.6 * torch.randn(pages, 1, kv_heads, dim, generator=g))
+            if kind == _E4M3:
+                e = torch.randint(-3, 4, (pages, kv_heads, page), generator=g)
+                c = x.clamp(-400, 400).to(_E4M3)
+                s = (e + 127).to(torch.uint8).view(_E8M0)
+            else:
+                c, s = x.to(kind), None
+            self._keep(c, s, layout, cuda)
+
+    def _keep(self, c, s, layout, cuda):
+        self.wide.append(_wide(c, s))
+        c = c.view(torch.uint8).to(cuda).view(c.dtype) if c.dtype == _E4M3 else c.to(cuda)
+        if layout == "heads_first":
+            raw = c.view(torch.uint8) if c.dtype == _E4M3 else c
+            raw = raw.transpose(1, 2).contiguous().transpose(1, 2)
+            c = raw.view(_E4M3) if c.dtype == _E4M3 else raw
+        self.caches.append(c)
+        self.scales.append(None if s is None else s.view(torch.uint8).to(cuda).view(_E8M0))
+
+    @property
+    def held(self):
+        return dict(key_scales=self.scales[0], value_scales=self.scales[1])
+
+    def context(self, b, which):
+        """(keys of the request, kv_heads, dim) in 64 bits, and which of them are there."""
+        n = self.kv[b]
+        j = torch.arange(n)
+        page = self.table_host[b, j // self.page].long()
+        there = (page >= 0) & (page < self.wide[which].shape[0])
+        return self.wide[which][page.clamp(0, self.wide[which].shape[0] - 1), j % self.page], there
+
+
+# ------------------------------------------------------------------------------------------------------------------- load
+@pytest.mark.parametrize("kind", _KINDS)
+@pytest.mark.parametrize("kv, heads, dim, page, length, layout", [
+    ([1], 1, 16, 1, 1, "plain"), ([5, 0, 33], 2, 48, 4, 40, "plain"), ([100, 64, 65], 8, 128, 16, 70, "heads_first"), ([300], 3, 256, 64, 300, "plain"),
+    ([17, 900], 1, 80, 128, 1000, "heads_first"),
+])
+def test_load_paged(cuda, kind, kv, heads, dim, page, length, layout):
+    case = Case(cuda, kind, kv, [0] * len(kv), heads, dim, page, seed=dim, missing=[(0, 0, -1)] if len(kv) > 1 else [], layout=layout)
+    for dtype in _TYPES if kind == _E4M3 else [kind]:
+        got = P.load_paged(*case.caches, case.table, case.kv_lens, length, dtype=dtype, **case.held)
+        for which in range(2):
+            want = torch.zeros(len(kv), heads, length, dim, dtype=torch.float64)
+            for b in range(len(kv)):
+                x, there = case.context(b, which)
+                x = torch.where(there[:, None, None], x, 0.0)[:length].transpose(0, 1)
+                want[b, :, :x.shape[1]] = x
+            assert got[which].dtype == dtype and torch.equal(got[which].double().cpu(), want.to(dtype).double())
+
+
+def test_load_paged_float16_ends_at_its_largest_number(cuda):
+    cache = torch.tensor([448.0, -448.0, 1.0, math.nan] * 4).to(_E4M3).view(1, 1, 1, 16)
+    scales = torch.tensor([127 + 9], dtype=torch.uint8).view(1, 1, 1)
+    cache, scales = cache.view(torch.uint8).to(cuda).view(_E4M3), scales.to(cuda).view(_E8M0)
+    keys, values = P.load_paged(cache, cache, _i32([[0]], cuda), _i32([1], cuda), 1, dtype=torch.float16, key_scales=scales, value_scales=scales)
+    want = torch.tensor([65504.0, -65504.0, 512.0, math.nan] * 4, dtype=torch.float64)
+    assert _same_values(keys.double().cpu().flatten(), want) and _same_values(values.double().cpu().flatten(), want)
+
+
+def test_load_of_nothing(cuda):
+    case = Case(cuda, _E4M3, [4], [0], 1, 16, 4)
+    keys, values = P.load_paged(*case.caches, case.table, case.kv_lens, 0, **case.held)
+    assert keys.shape == values.shape == (1, 1, 0, 16) and keys.dtype == torch.bfloat16
+
+
+# ----------------------------------------------------------------------------------------------------------------- bounds
+@pytest.mark.parametrize("kind", _KINDS)
+@pytest.mark.parametrize("new, cached, heads, dim, page", [
+    ([1], [0], 1, 16, 1), ([1, 1, 1, 1], [15, 16, 14, 31], 2, 64, 16), ([40, 0, 3], [5, 64, 61], 3, 128, 8), ([500], [77], 8, 128, 16),
+    ([130, 9], [0, 1], 1, 80, 2), ([300], [3], 2, 256, 64), ([1] * 70, [31] * 70, 1, 32, 32), ([5], [1], 1, 48, 256),
+])
+def test_page_bounds(cuda, kind, new, cached, heads, dim, page):
+    case = Case(cuda, kind, new, cached, heads, dim, page, seed=page, missing=[(0, 0, 10 ** 6)] if cached[0] == 5 else [])
+    pages = case.caches[0].shape[0]
+    held = torch.bfloat16 if kind == _E4M3 else kind
+    bounds = torch.full((pages, heads, 2, dim), 7.0, dtype=held, device=cuda)
+    want = bounds.double().cpu()
+    for b in range(len(new)):
+        for j in range(cached[b] // page, case.kv[b] // page):
+            at = int(case.table_host[b, j])
+            if at < pages:
+                want[at, :, 0], want[at, :, 1] = case.wide[0][at].amin(0), case.wide[0][at].amax(0)
+    P.update_page_bounds(bounds, case.caches[0], case.table, case.kv_lens, case.cu_new, key_scales=case.scales[0])
+    assert torch.equal(bounds.double().cpu(), want)
+
+
+@pytest.mark.parametrize("kind", _KINDS)
+def test_page_bounds_of_what_is_not_finite(cuda, kind):
+    case = Case(cuda, kind, [32], [0], 2, 64, 16)
+    raw = case.caches[0].float()
+    page = int(case.table_host[0, 1])
+    raw[page, 3, 1, 5] = math.nan
+    raw[page, 15, 0, 0] = -math.nan
+    if kind != _E4M3:
+        raw[page, 4, 1, 6], raw[page, 9, 1, 7] = math.inf, -math.inf
+    cache = raw.to(kind)
+    wide = _wide(cache, case.scales[0])
+    bounds = torch.zeros(cache.shape[0], 2, 2, 64, dtype=torch.bfloat16 if kind == _E4M3 else kind, device=cuda)
+    P.update_page_bounds(bounds, cache, case.table, case.kv_lens, case.cu_new, key_scales=case.scales[0])
+    for j in range(2):
+        at = int(case.table_host[0, j])
+        assert _same_values(bounds[at, :, 0].double().cpu(), wide[at].amin(0)) and _same_values(bounds[at, :, 1].double().cpu(), wide[at].amax(0))
+
+
+def test_page_bounds_of_refused_requests_and_bad_lengths(cuda):
+    """Lengths of 0 beside new tokens (a request that got no pages), a negative one, one beyond the table: no page, or those of the table."""
+    case = Case(cuda, torch.bfloat16, [20, 20, 20, 20], [0, 0, 0, 0], 1, 16, 4)
+    bounds = torch.full((case.caches[0].shape[0], 1, 2, 16), 7.0, dtype=torch.bfloat16, device=cuda)
+    P.update_page_bounds(bounds, case.caches[0], case.table, _i32([0, -5, 20, 10 ** 6], cuda), case.cu_new)
+    want = torch.full(bounds.shape, 7.0, dtype=torch.float64)
+    for j in range(5):
+        at = int(case.table_host[2, j])
+        want[at, :, 0], want[at, :, 1] = case.wide[0][at].amin(0), case.wide[0][at].amax(0)
+    assert torch.equal(bounds.double().cpu(), want)
+
+
+# ----------------------------------------------------------------------------------------------------------------- select
+def _plain_select(q, bounds, case, group, n_select, sink, window):
+    """By the rule, one row after the other. `bounds`: (pages, kv_heads, 2, dim) in 64 bits."""
+    page, kv_heads = case.page, case.kv_heads
+    out = torch.full((q.shape[0], kv_heads, n_select), -1, dtype=torch.int64)
+    for b in range(len(case.new)):
+        for t in range(case.cu[b], case.cu[b + 1]):
+            last = (case.cached[b] + t - case.cu[b]) // page
+            table = case.table_host[b, :last + 1].long()
+            there = [j for j in range(last + 1) if 0 <= table[j] < bounds.shape[0]]
+            for h in range(kv_heads):
+                qq = q[t, h * group:(h + 1) * group].double()
+                lo, hi = bounds[table.clamp(0, bounds.shape[0] - 1), h, 0], bounds[table.clamp(0, bounds.shape[0] - 1), h, 1]
+                scores = torch.maximum(qq[:, None] * lo, qq[:, None] * hi).sum((0, 2))
+                scores = torch.where(torch.isfinite(scores), scores, math.inf).tolist()
+                always = [j for j in there if j < sink or j > last - window]
+                rest = sorted((j for j in there if j not in always), key=lambda j: (-scores[j], j))
+                taken = sorted(always + rest[:n_select - len(always)])
+                out[t, h, :len(taken)] = torch.tensor(taken, dtype=torch.int64)
+    return out
+
+
+def _select_case(cuda, dtype, kind, new, cached, q_heads, kv_heads, dim, page, n_select, sink=1, window=1, seed=0, missing=(), pad=0, same=False,
+                 max_context=None):
+    case = Case(cuda, kind, new, cached, kv_heads, dim, page, seed=seed, missing=missing)
+    g = torch.Generator().manual_seed(seed + 1)
+    held = torch.bfloat16 if kind == _E4M3 else kind
+    bounds = torch.stack([case.wide[0].amin(1), case.wide[0].amax(1)], 2).to(held)
+    if same:  # only a few different pages: ties
+        bounds = bounds[torch.arange(bounds.shape[0]) % 3]
+    q = torch.randn(case.cu[-1] + pad, q_heads, dim, generator=g).to(dtype)
+    got = P.select_pages(q.to(cuda), bounds.to(cuda), case.table, case.kv_lens, case.cu_new, page, n_select, sink_pages=sink, window_pages=window,
+                         max_context=max_context)
+    want = _plain_select(q, bounds.double(), case, q_heads // kv_heads, n_select, sink, window)
+    assert got.dtype == torch.int32 and torch.equal(got.long().cpu(), want)
+
+
+@pytest.mark.parametrize("dtype, kind", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, _E4M3), (torch.float16, torch.float16), (torch.float16, _E4M3),
+                                         (torch.float32, torch.float32), (torch.float32, _E4M3)])
+@pytest.mark.parametrize("dim", [16, 48, 64, 80, 128, 144, 256])
+def test_select_types_and_head_dims(cuda, dtype, kind, dim):
+    _select_case(cuda, dtype, kind, [1, 3, 0, 2], [700, 90, 31, 0], 4, 2, dim, 8, 12, seed=dim)
+
+
+@pytest.mark.parametrize("q_heads, kv_heads", [(1, 1), (8, 8), (3, 1), (40, 2), (16, 4)])
+def test_select_head_groups(cuda, q_heads, kv_heads):
+    _select_case(cuda, torch.bfloat16, torch.bfloat16, [2, 1], [400, 1000], q_heads, kv_heads, 64, 16, 9, seed=q_heads)
+
+
+@pytest.mark.parametrize("page, n_select, sink, window", [(1, 1, 0, 1), (1, 64, 4, 4), (2, 500, 1, 1), (16, 2, 1, 1), (16, 7, 0, 7), (64, 3, 1, 2), (512, 1, 0, 1), (16, 100, 50, 50),
+                                                          (8, 5000, 1, 1)])
+@pytest.mark.parametrize("cached", [0, 1, 63, 2500])
+def test_select_page_sizes_and_numbers(cuda, page, n_select, sink, window, cached):
+    _select_case(cuda, torch.bfloat16, torch.bfloat16, [1, 2], [cached, cached // 3], 2, 1, 32, page, n_select, sink, window, seed=page + n_select)
+
+
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 5000])
+def test_select_of_many_pages(cuda, n):
+    """Beyond 2048 pages a row's keys are read again in every pass."""
+    _select_case(cuda, torch.bfloat16, _E4M3, [1], [n - 1], 4, 1, 64, 1, 100, seed=n)
+
+
+@pytest.mark.parametrize("n_select", [3, 30, 64])
+def test_select_ties_go_to_the_lower_page(cuda, n_select):
+    _select_case(cuda, torch.bfloat16, torch.bfloat16, [1, 3], [1200, 300], 4, 2, 64, 8, n_select, seed=5, same=True)
+
+
+def test_select_pages_that_are_not_there_and_rows_behind_the_last(cuda):
+    missing = [(0, 0, -1), (0, 3, 10 ** 6), (0, 50, -7), (1, 0, -1)]
+    _select_case(cuda, torch.bfloat16, torch.bfloat16, [1, 1], [500, 5], 2, 1, 64, 8, 20, sink=2, window=2, missing=missing, pad=3)
+
+
+@pytest.mark.parametrize("max_context", [1, 600, 10 ** 9])
+def test_select_does_not_depend_on_the_hint(cuda, max_context):
+    _select_case(cuda, torch.bfloat16, torch.bfloat16, [1, 2], [5000, 300], 2, 1, 64, 4, 20, max_context=max_context)
+
+
+def test_select_scores_that_are_not_finite_come_first(cuda):
+    case = Case(cuda, torch.float32, [1], [639], 1, 16, 16)
+    bounds = torch.stack([case.wide[0].amin(1), case.wide[0].amax(1)], 2).float()
+    for j, value in ((4, math.nan), (9, math.inf), (30, -math.inf)):
+        bounds[int(case.table_host[0, j]), 0, j % 2, 3] = value
+    q = torch.randn(1, 2, 16, generator=torch.Generator().manual_seed(3)).abs() + 0.1
+    q[0, 1] *= -1
+    got = P.select_pages(q.to(cuda), bounds.to(cuda), case.table, case.kv_lens, case.cu_new, 16, 5, sink_pages=0)
+    assert set(got[0, 0].tolist()) >= {4, 9, 30, 39}
+    q[0, 0, 0] = math.nan  # no score is finite: the lowest pages
+    got = P.select_pages(q.to(cuda), bounds.to(cuda), case.table, case.kv_lens, case.cu_new, 16, 5, sink_pages=0)
+    assert got[0, 0].tolist() == [0, 1, 2, 3, 39]
+
+
+# -------------------------------------------------------------------------------------------------------------- attention
+def _attention_case(cuda, dtype, kind, new, cached, q_heads, kv_heads, dim, page, sink=0, window=0, sinks=False, pad=0, seed=0, layout="plain",
+                    missing=(), lists=None, max_context=None, scaling=None, scale=1.0, stride=False):
+    """`lists`: a function (token's last page, rng) -> a token's list of pages."""
+    case = Case(cuda, kind, new, cached, kv_heads, dim, page, seed=seed, missing=missing, layout=layout, scale=scale)
+    g, rng = torch.Generator().manual_seed(seed + 7), random.Random(seed)
+    tokens, group = case.cu[-1] + pad, q_heads // kv_heads
+    q = torch.randn(tokens, q_heads, dim, generator=g).to(dtype)
+    logit = torch.randn(q_heads, generator=g) if sinks else None
+    scaling = dim ** -0.5 if scaling is None else scaling
+    out = torch.full((tokens, q_heads, dim), 7.0, dtype=dtype, device=cuda)
+    queries = q.to(cuda)
+    if stride:
+        queries = torch.cat([q, torch.full_like(q, math.nan)], dim=1).to(cuda)[:, :q_heads]
+    pages = None
+    if lists is not None:
+        rows = [[lists((cached[b] + t - case.cu[b]) // page, rng) for _ in range(kv_heads)] for b in range(len(new)) for t in range(case.cu[b], case.cu[b + 1])]
+        rows += [[[0]] * kv_heads] * pad
+        most = max(len(r) for row in rows for r in row)
+        pages = _i32([[r + [-1] * (most - len(r)) for r in row] for row in rows], cuda)
+    got = P.paged_attention(queries, *case.caches, case.table, case.kv_lens, case.cu_new, scaling, max_context=max_context, sink_size=sink,
+                            window_size=window, sinks=None if logit is None else logit.to(cuda), out=out, pages=pages, **case.held)
+    assert got is out
+    got = got.double().cpu()
+    assert got[case.cu[-1]:].eq(7).all(), "rows behind the last request's were written"
+    half = _HALF_STEP[dtype]
+    chunk = pages is None and case.cu[-1] * group > 32 * len(new)
+    off2 = norm2 = most = 0.0
+    for b in range(len(new)):
+        keys, there = case.context(b, 0)
+        values, _ = case.context(b, 1)
+        n = case.kv[b]
+        j = torch.arange(n)
+        for t in range(case.cu[b], case.cu[b + 1]):
+            p = cached[b] + t - case.cu[b]
+            for hk in range(kv_heads):
+                if pages is None:
+                    seen = there & (j <= p)
+                    if window:
+                        seen = seen & ((j < sink) | (j > p - window))
+                    at = seen.nonzero().flatten()
+                else:
+                    listed = [jj for lg in rows[t][hk] if lg >= 0 for jj in range(lg * page, (lg + 1) * page) if jj <= p and there[jj]]
+                    at = torch.tensor(listed, dtype=torch.long)
+                kk, vv = keys[at, hk], values[at, hk]
+                qq = q[t, hk * group:(hk + 1) * group].double()
+                logits = qq @ kk.T * scaling
+                if at.numel():
+                    weights = torch.exp(logits - logits.amax(1, keepdim=True))
+                    total = weights.sum(1, keepdim=True)
+                    if logit is not None:
+                        total = total + torch.exp(logit[hk * group:(hk + 1) * group].double()[:, None] - logits.amax(1, keepdim=True))
+                    weights = weights / total
+                    want, size = weights @ vv, weights @ vv.abs()
+                else:
+                    want = size = torch.zeros(group, dim, dtype=torch.float64)
+                have = got[t, hk * group:(hk + 1) * group]
+                # A product of D terms in fp32 is off by at most D 2^-24 sum |q k|, a logit by that and a rounding or two of its own size, its
+                # weight relatively by as much (exp2: a few 2^-24 more), both in a weight and in the total. Two 16-bit terms leave a weight 2^-16 of
+                # itself at most; in chunks (another kernel, one term) half a step. The sum of n weights is off by at most n 2^-24 (in parts: far less). The
+                # result is rounded once. A float16 copy of 8-bit keys and values (chunks) is exact for what these caches hold.
+                reach = float((qq.abs() @ kk.abs().T).max()) * abs(scaling) if at.numel() else 0.0
+                logit_off = (dim + 4) * 2.0 ** -24 * reach + 8 * 2.0 ** -24
+                term = (half if chunk else 2.0 ** -16) if dtype != torch.float32 else 0.0
+                bound = want.abs() * half + size * (term + 2 * logit_off + (2 * n + 16) * 2.0 ** -24) + torch.finfo(dtype).smallest_normal * half
+                off = (have - want).abs()
+                assert torch.isfinite(have).all() and not (off > bound * 1.001).any(), (b, t, hk, float((off / bound).max()))
+                most = max(most, reach)
+                off2 += float((have - want).square().sum())
+                norm2 += float(want.square().sum())
+    # Roundings of independent signs: half a step for the result, in chunks half for the weights; a logit is rounded with 2^-24 of up to `most` in each
+    # of its last few additions (4 count), and the largest one's too: 8.
+    assert math.sqrt(off2) <= math.sqrt(norm2) * ((2 if chunk else 1) * half + 2.0 ** -16 * (dtype != torch.float32) + 2.0 ** -20 + 8 * 2.0 ** -24 * most) + 1e-30
+    return got
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("dim", [16, 48, 64, 80, 96, 128, 144, 192, 256])
+def test_attention_8bit_head_dims(cuda, dtype, dim):
+    _attention_case(cuda, dtype, _E4M3, [1, 5, 3], [130, 0, 61], 6, 2, dim, 16, seed=dim)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("q_heads, kv_heads", [(1, 1), (8, 8), (3, 1), (8, 2), (16, 1), (17, 1), (40, 1), (66, 2)])
+def test_attention_8bit_head_groups(cuda, dtype, q_heads, kv_heads):
+    _attention_case(cuda, dtype, _E4M3, [1, 2, 0, 1], [63, 64, 200, 0], q_heads, kv_heads, 64, 8, seed=q_heads)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page", [1, 2, 8, 16, 32, 128, 512])
+def test_attention_8bit_page_sizes(cuda, dtype, page):
+    _attention_case(cuda, dtype, _E4M3, [1, 3, 4], [600, 97, 5], 4, 1, 128, page, seed=page, layout="heads_first" if page % 3 else "plain", stride=page > 2)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("cached", [0, 1, 15, 31, 32, 33, 127, 128, 1000, 4097])
+def test_attention_8bit_single_tokens(cuda, dtype, cached):
+    _attention_case(cuda, dtype, _E4M3, [1] * 3, [cached, cached // 2, 0], 8, 2, 128, 16, seed=cached, pad=2)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("new, cached", [([2], [0]), ([9, 8, 7], [1, 0, 64]), ([33], [100]), ([65, 1], [0, 300]), ([150], [17])])
+def test_attention_8bit_chunks(cuda, dtype, new, cached):
+    _attention_case(cuda, dtype, _E4M3, new, cached, 8, 2, 64, 16, seed=sum(new), pad=1)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("new", [[1, 4], [70, 9]])
+@pytest.mark.parametrize("sink, window", [(0, 1), (0, 64), (1, 1), (4, 63), (128, 100), (100, 100000), (5000, 7)])
+def test_attention_8bit_sink_and_window(cuda, dtype, new, sink, window):
+    for page in (8, 64):
+        _attention_case(cuda, dtype, _E4M3, new, [700, 130], 4, 2, 64, page, sink, window, seed=sink + window)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("new", [[1, 1, 2], [40, 1, 2]])
+def test_attention_8bit_sink_logits_and_missing_pages(cuda, dtype, new):
+    _attention_case(cuda, dtype, _E4M3, new, [300, 20, 0], 4, 2, 64, 16, sinks=True, missing=[(0, 2, -1), (0, 5, 10 ** 6), (1, 0, -3), (1, 1, -1), (2, 0, -1)], seed=3)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("max_context", [1, 100, 5000, 10 ** 9])
+def test_attention_8bit_does_not_depend_on_the_hint(cuda, dtype, max_context):
+    _attention_case(cuda, dtype, _E4M3, [1, 3], [5000, 77], 4, 2, 64, 16, max_context=max_context)
+
+
+@pytest.mark.parametrize("scaling", [-0.2, 0.0, 2.0])
+def test_attention_8bit_scaling(cuda, scaling):
+    _attention_case(cuda, torch.bfloat16, _E4M3, [1, 3], [500, 77], 4, 2, 64, 16, scaling=scaling)
+
+
+def _some_pages(last, rng):
+    """A token's own page and others, in disorder, one behind its position, one that does not exist, an entry of -1 in between."""
+    some = rng.sample(range(last + 1), min(last + 1, 5)) + [last + 1, 10 ** 6, -1]
+    rng.shuffle(some)
+    return some + ([last] if last not in some else [])
+
+
+@pytest.mark.parametrize("dtype, kind", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), (torch.float32, torch.float32), (torch.bfloat16, _E4M3),
+                                         (torch.float16, _E4M3), (torch.float32, _E4M3)])
+@pytest.mark.parametrize("dim", [16, 64, 80, 128, 256])
+def test_attention_over_pages_types_and_head_dims(cuda, dtype, kind, dim):
+    _attention_case(cuda, dtype, kind, [1, 4, 0, 2], [500, 30, 9, 0], 6, 2, dim, 16, seed=dim, lists=_some_pages, pad=2)
+
+
+@pytest.mark.parametrize("kind", _KINDS)
+@pytest.mark.parametrize("page", [1, 4, 8, 32, 64, 512])
+def test_attention_over_pages_page_sizes(cuda, kind, page):
+    dtype = torch.bfloat16 if kind == _E4M3 else kind
+    _attention_case(cuda, dtype, kind, [1, 2], [40 * page, 3 * page + 1], 4, 2, 64, page, seed=page, lists=_some_pages, layout="heads_first")
+
+
+@pytest.mark.parametrize("kind", _KINDS)
+def test_attention_over_many_pages(cuda, kind):
+    """Lists that several workgroups share, and the longest that one of them takes."""
+    dtype = torch.bfloat16 if kind == _E4M3 else kind
+    _attention_case(cuda, dtype, kind, [1, 1], [5000, 300], 4, 1, 128, 16, seed=1, lists=lambda last, rng: list(range(0, last + 1, 2)) + [last])
+    _attention_case(cuda, dtype, kind, [1], [2600], 2, 1, 64, 1, seed=1, lists=lambda last, rng: rng.sample(range(last + 1), 2500))
+
+
+@pytest.mark.parametrize("kind", _KINDS)
+def test_attention_over_pages_named_twice_and_over_none(cuda, kind):
+    dtype = torch.bfloat16 if kind == _E4M3 else kind
+    _attention_case(cuda, dtype, kind, [1, 2], [300, 80], 4, 2, 64, 16, sinks=True, seed=2, lists=lambda last, rng: [0, last, last, 1, 0])
+    got = _attention_case(cuda, dtype, kind, [1, 2], [300, 80], 4, 2, 64, 16, sinks=True, seed=2, lists=lambda last, rng: [-1, last + 1, 10 ** 9])
+    assert got.eq(0).all()
+
+
+@pytest.mark.parametrize("q_heads, kv_heads", [(1, 1), (16, 1), (24, 1), (12, 4)])
+def test_attention_over_pages_head_groups(cuda, q_heads, kv_heads):
+    _attention_case(cuda, torch.bfloat16, torch.bfloat16, [1, 3], [400, 20], q_heads, kv_heads, 64, 16, seed=q_heads, lists=_some_pages)
+
+
+# ------------------------------------------------------------------------------------------------------ what is not finite
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("new", [[1, 3], [1, 60]])
+def test_attention_8bit_values_that_are_not_finite_stay_where_they_are_seen(cuda, dtype, new):
+    """NaN on a page's unused end, behind a row's position, on a page of another request: no row sees it. In a visible value: that channel
+    of the rows that see it, in a visible key: all channels."""
+    cached, page, heads, dim = [100, 20], 16, 2, 64
+    case = Case(cuda, _E4M3, new, cached, 1, dim, page, seed=4)
+    keys, values = case.caches[0].view(torch.uint8), case.caches[1].view(torch.uint8)
+    for b in range(2):  # behind the last key of the last page
+        at = int(case.table_host[b, (case.kv[b] - 1) // page])
+        keys[at, (case.kv[b] - 1) % page + 1:] = 0x7f
+        values[at, (case.kv[b] - 1) % page + 1:] = 0xff
+    p = case.kv[1] - 1  # the last token's own: the rows before it do not see it
+    values[int(case.table_host[1, p // page]), p % page, 0, 5] = 0x7f
+    keys[int(case.table_host[0, 2]), 1, 0, 9] = 0x7f
+    q = torch.randn(case.cu[-1], heads, dim, generator=torch.Generator().manual_seed(1)).to(dtype).to(cuda)
+    got = P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, **case.held)
+    assert torch.isnan(got[:case.cu[1]]).all()
+    assert torch.isfinite(got[case.cu[1]:-1]).all()
+    assert torch.isnan(got[-1, :, 5]).all() and torch.isfinite(got[-1, :, :5]).all() and torch.isfinite(got[-1, :, 6:]).all()
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("n", [40, 3000])
+def test_attention_over_pages_of_values_that_are_not_finite(cuda, dtype, n):
+    """Infinite values are the result's infinities in their channel, the others' stay; keys with -inf have no weight."""
+    page, dim = 16, 64
+    case = Case(cuda, dtype, [1], [n], 1, dim, page, seed=n)
+    pages = _i32([list(range(-(-(n + 1) // page)))], cuda).view(1, 1, -1)
+    q = torch.ones(1, 2, dim, dtype=dtype, device=cuda)
+    case.caches[1][int(case.table_host[0, 1]), 3, 0, 7] = math.inf
+    case.caches[1][int(case.table_host[0, 0]), 3, 0, 9] = -math.inf
+    case.caches[0][int(case.table_host[0, 0]), 5, 0, 2] = -math.inf
+    got = P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, pages=pages)
+    assert got[0, :, 7].eq(math.inf).all() and got[0, :, 9].eq(-math.inf).all()
+    rest = [d for d in range(dim) if d not in (7, 9)]
+    assert torch.isfinite(got[0][:, rest]).all()
+    case.caches[0][int(case.table_host[0, 0]), 6, 0, 2] = math.nan
+    assert torch.isnan(P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, pages=pages)).all()
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("n", [40, 3000])
+def test_averages_of_the_largest_values_are_finite(cuda, dtype, n):
+    case = Case(cuda, dtype, [1], [n - 1], 1, 64, 16)
+    big = torch.finfo(dtype).max
+    case.caches[1].fill_(big)
+    case.caches[0].zero_()
+    q = torch.zeros(1, 2, 64, dtype=dtype, device=cuda)
+    pages = _i32([list(range(-(-n // 16)))], cuda).view(1, 1, -1)
+    got = P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, pages=pages).double()
+    # an average of n equal numbers, each share off by a few 2^-24 (n of them: at most n 2^-24), rounded once
+    assert torch.isfinite(got).all() and (got / big - 1).abs().max() <= _HALF_STEP[dtype] + (n + 8) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", [None, _E4M3])
+def test_logits_far_below_zero_are_logits(cuda, dtype, kind):
+    """All logits equal and very low: an average, not 0."""
+    case = Case(cuda, kind or dtype, [1], [99], 1, 64, 16)
+    raw = case.caches[0].float().fill_(448.0).to(case.caches[0].dtype)
+    case.caches[0].view(torch.uint8).copy_(raw.view(torch.uint8))
+    if kind:
+        case.scales[0].view(torch.uint8).fill_(127)
+    q = torch.full((1, 2, 64), -1e30, dtype=dtype, device=cuda)
+    pages = _i32([list(range(7))], cuda).view(1, 1, -1)
+    got = P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 1.0, pages=pages, **case.held).double().cpu()
+    want = case.context(0, 1)[0][:, 0].mean(0)
+    size = case.context(0, 1)[0][:, 0].abs().mean(0)
+    assert ((got[0] - want).abs() <= want.abs() * _HALF_STEP[dtype] + size * (2.0 ** -16 + 200 * 2.0 ** -24)).all()
+
+
+# --------------------------------------------------------------------------------------------------------- the whole of it
+def _plain_step(case_like, q, keys, values, scaling):
+    weights = torch.softmax(q.double() @ keys.double().T * scaling, -1)
+    return weights @ values.double()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", [None, _E4M3])
+def test_a_server_with_selected_pages(cuda, dtype, kind):
+    """Prompts in chunks, then answers by selected pages, requests that come and go, two layers: against a cache per request in 64 bits."""
+    torch.manual_seed(0)
+    layers, heads, kv_heads, dim, page, n_select = 2, 4, 2, 64, 16, 6
+    cache = P.PagedKVCache(layers, 90, page, kv_heads, dim, 3, 400, kind or dtype, cuda, page_bounds=True)
+    host = [[[torch.zeros(0, kv_heads, dim, dtype=torch.float64) for _ in range(3)] for _ in range(2)] for _ in range(layers)]
+    group, scaling = heads // kv_heads, dim ** -0.5
+    steps = [[200, 0, 37], [1, 150, 1], [1, 1, 1], [1, 1, 1], [0, 1, 3], [1, 1, 1]]
+    for i, new in enumerate(steps):
+        step = cache.assign(_i32(new, cuda), sum(new) + 2)
+        assert step.granted.all()
+        cu = [sum(new[:b]) for b in range(4)]
+        few = i > 1
+        for layer in range(layers):
+            q, k, v = (torch.randn(sum(new) + 2, n, dim, device=cuda).to(dtype) for n in (heads, kv_heads, kv_heads))
+            out = cache.attend(layer, q, k, v, step, scaling, n_select=n_select if few else None, **({} if few else {"max_context": 300})).double().cpu()
+            for which, x in enumerate((k, v)):
+                x = _plain_quantise(x.cpu())[0] if kind else x.double().cpu()
+                for b in range(3):
+                    host[layer][which][b] = torch.cat([host[layer][which][b], x[cu[b]:cu[b + 1]]])
+            for b in range(3):
+                keys, values = host[layer][0][b], host[layer][1][b]
+                for t in range(cu[b], cu[b + 1]):
+                    p = len(keys) - new[b] + t - cu[b]
+                    for h in range(kv_heads):
+                        qq = q[t, h * group:(h + 1) * group].double().cpu()
+                        at = list(range(p + 1))
+                        if few:
+                            last = p // page
+                            scores = [float(torch.maximum(qq * keys[j * page:(j + 1) * page, h].amin(0), qq * keys[j * page:(j + 1) * page, h].amax(0)).sum())
+                                      for j in range(last)]
+                            best = sorted(range(1, last), key=lambda j: -scores[j])[:n_select - 2]
+                            at = [j for j in range(p + 1) if j // page in {0, last, *best}]
+                        want = _plain_step(None, qq, keys[at, h], values[at, h], scaling)
+                        have = out[t, h * group:(h + 1) * group]
+                        # as derived for _attention_case: the weights' one term in chunks, the result's rounding, logits of a few units
+                        assert (have - want).abs().max() <= 2.2 * _HALF_STEP[dtype] * max(1.0, float(values[at, h].abs().max()))
+        if i == 3:
+            cache.release(torch.tensor([True, False, False], device=cuda))
+            for layer in range(layers):
+                for which in range(2):
+                    host[layer][which][0] = torch.zeros(0, kv_heads, dim, dtype=torch.float64)
+    for layer in range(layers):
+        got = cache.load(layer, 400, dtype)
+        for which in range(2):
+            want = torch.zeros(3, kv_heads, 400, dim, dtype=torch.float64)
+            for b in range(3):
+                want[b, :, :len(host[layer][which][b])] = host[layer][which][b].transpose(0, 1)
+            assert torch.equal(got[which].double().cpu(), want)
+
+
+def test_a_context_read_back_goes_into_research_attention(cuda):
+    """An 8-bit context as the maskers' contiguous cache: Sink + Local over it is paged attention's window over the pages."""
+    from sparse_attention_hub_amd.sparse_attention import LocalMaskerConfig, ResearchAttentionConfig, SinkMaskerConfig
+    from sparse_attention_hub_amd.sparse_attention.research_attention import ResearchAttention
+
+    torch.manual_seed(1)
+    cache = P.PagedKVCache(1, 40, 16, 2, 64, 1, 600, _E4M3, cuda)
+    q, k, v = (torch.randn(500, n, 64, device=cuda).to(torch.bfloat16) for n in (4, 2, 2))
+    cache.attend(0, q, k, v, cache.assign(_i32([500], cuda), 500), 0.125)
+    step = cache.assign(_i32([1], cuda), 1)
+    q, k, v = (torch.randn(1, n, 64, device=cuda).to(torch.bfloat16) for n in (4, 2, 2))
+    paged = cache.attend(0, q, k, v, step, 0.125, sink_size=16, window_size=64)
+    keys, values = cache.load(0, 501)
+    attention = ResearchAttention.create_from_config(ResearchAttentionConfig(masker_configs=[SinkMaskerConfig(sink_size=16), LocalMaskerConfig(window_size=64)]))
+    module = torch.nn.Module().eval()
+    module.num_key_value_groups = 2
+    out, _ = attention.custom_attention(module, q.transpose(0, 1)[None], keys, values, None, 0.125, 0.0, sparse_meta_data={}, layer_idx=0)
+    # both are the same average, each rounded once, weights of one term at most
+    assert (out[0].float() - paged.float()).abs().max() <= 4 * _HALF_STEP[torch.bfloat16] * float(values.float().abs().max())
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, _E4M3])
+def test_a_captured_step(cuda, kind):
+    """A step of store, bounds, selection and attention as a graph, replayed on changing inputs between eager work: the eager results."""
+    torch.manual_seed(2)
+
+    def fresh():
+        return P.PagedKVCache(1, 120, 16, 2, 64, 3, 600, kind, cuda, page_bounds=True)
+
+    graphed, eager = fresh(), fresh()
+    prompt = [torch.randn(900, n, 64, device=cuda).to(torch.bfloat16) for n in (4, 2, 2)]
+    new = _i32([300, 300, 300], cuda)
+    for c in (graphed, eager):
+        c.attend(0, *prompt, c.assign(new, 900), 0.125)
+    one = _i32([1, 1, 1], cuda)
+    q, k, v = (torch.randn(3, n, 64, device=cuda).to(torch.bfloat16) for n in (4, 2, 2))
+    out = torch.empty_like(q)
+
+    def step(c, o):
+        return c.attend(0, q, k, v, c.assign(one, 3), 0.125, n_select=8, out=o)
+
+    stream = torch.cuda.Stream(cuda)
+    stream.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(stream):
+        step(graphed, out)
+    torch.cuda.current_stream(cuda).wait_stream(stream)
+    step(eager, torch.empty_like(q))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(graphed, out)
+    for i in range(25):
+        for x in (q, k, v):
+            x.copy_(torch.randn_like(x))
+        graph.replay()
+        want = step(eager, torch.empty_like(q))
+        torch.cuda.synchronize(cuda)
+        assert torch.equal(out, want), i
+    assert torch.equal(graphed.lens, eager.lens)
+
+
+def test_two_streams_at_once(cuda):
+    """Calls on two streams share nothing."""
+    cases = [Case(cuda, _E4M3, [1, 2], [3000, 500], 2, 64, 16, seed=s) for s in (1, 2)]
+    q = [torch.randn(3, 4, 64, device=cuda).to(torch.bfloat16) for _ in cases]
+    pages = [_i32([[list(range(0, 30, 2))] * 2] * 3, cuda) for _ in cases]
+
+    def call(i, listed):
+        c = cases[i]
+        return P.paged_attention(q[i], *c.caches, c.table, c.kv_lens, c.cu_new, 0.125, pages=pages[i] if listed else None, **c.held)
+
+    want = [[call(i, listed) for listed in (False, True)] for i in range(2)]
+    torch.cuda.synchronize(cuda)
+    streams = [torch.cuda.Stream(cuda) for _ in cases]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append([call(i, listed) for listed in (False, True)])
+    torch.cuda.synchronize(cuda)
+    for i in range(2):
+        for pair in got[i]:
+            assert torch.equal(pair[0], want[i][0]) and torch.equal(pair[1], want[i][1])
+
+
+def test_calls_of_no_tokens(cuda):
+    case = Case(cuda, _E4M3, [0, 0], [20, 3], 2, 64, 16)
+    q = torch.zeros(0, 4, 64, dtype=torch.bfloat16, device=cuda)
+    assert P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, **case.held).shape == (0, 4, 64)
+    bounds = torch.zeros(case.caches[0].shape[0], 2, 2, 64, dtype=torch.bfloat16, device=cuda)
+    assert P.select_pages(q, bounds, case.table, case.kv_lens, case.cu_new, 16, 4).shape == (0, 2, 4)
+    P.update_page_bounds(bounds, case.caches[0], case.table, case.kv_lens, case.cu_new, key_scales=case.scales[0])
+    assert bounds.eq(0).all()
+
+
+def test_pages_beyond_32_bits(cuda):
+    """A cache of more than 2^32 bytes and elements, its last pages in use."""
+    heads, dim, page = 1, 256, 16
+    pages = (2 ** 32 // (heads * dim * page)) + 64
+    caches = [torch.empty(pages, page, heads, dim, dtype=torch.uint8, device=cuda) for _ in range(2)]
+    scales = [torch.full((pages, heads, page), 127, dtype=torch.uint8, device=cuda).view(_E8M0) for _ in range(2)]
+    g = torch.Generator().manual_seed(0)
+    n = 100
+    table = torch.arange(pages - 1, pages - 1 - 7, -1, dtype=torch.int32).view(1, 7)
+    rows = [torch.randn(n, heads, dim, generator=g).to(torch.bfloat16) for _ in range(2)]
+    slots = table[0, torch.arange(n) // page].long() * page + torch.arange(n) % page
+    kc, vc = (c.view(_E4M3) for c in caches)
+    held = dict(key_scales=scales[0], value_scales=scales[1])
+    P.store_paged(rows[0].to(cuda), rows[1].to(cuda), kc, vc, slots.to(cuda), **held)
+    keys, values = P.load_paged(kc, vc, table.to(cuda), _i32([n], cuda), n, dtype=torch.float32, **held)
+    wide = [_plain_quantise(r)[0][:, 0] for r in rows]
+    assert torch.equal(keys[0, 0].double().cpu(), wide[0]) and torch.equal(values[0, 0].double().cpu(), wide[1])
+    q = torch.randn(1, 2, dim, generator=g).to(torch.bfloat16)
+    got = P.paged_attention(q.to(cuda), kc, vc, table.to(cuda), _i32([n], cuda), _i32([0, 1], cuda), 0.0625, **held).double().cpu()
+    want = _plain_step(None, q[0], wide[0], wide[1], 0.0625)
+    assert (got[0] - want).abs().max() <= 2 * _HALF_STEP[torch.bfloat16] * float(wide[1].abs().max())
+    bounds = torch.zeros(pages, heads, 2, dim, dtype=torch.bfloat16, device=cuda)
+    P.update_page_bounds(bounds, kc, table.to(cuda), _i32([n], cuda), _i32([0, n], cuda), key_scales=scales[0])
+    assert torch.equal(bounds[pages - 1, 0, 1].double().cpu(), wide[0][:page].amax(0))
+
+
+def test_tensors_that_do_not_fit_together_are_refused(cuda):
+    i32, table = torch.zeros(2, dtype=torch.int32, device=cuda), torch.zeros(2, 4, dtype=torch.int32, device=cuda)
+    cu, slots = torch.zeros(3, dtype=torch.int32, device=cuda), torch.full((3,), -1, dtype=torch.int64, device=cuda)
+    cache = torch.zeros(8, 16, 2, 64, device=cuda).to(_E4M3)
+    plain = torch.zeros(8, 16, 2, 64, device=cuda)
+    scales = torch.zeros(8, 2, 16, dtype=torch.uint8, device=cuda).view(_E8M0)
+    rows = torch.zeros(3, 2, 64, device=cuda)
+    q = torch.zeros(3, 4, 64, device=cuda)
+    pages = torch.zeros(3, 2, 5, dtype=torch.int32, device=cuda)
+    bounds = torch.zeros(8, 2, 2, 64, dtype=torch.bfloat16, device=cuda)
+    wrong_scales = [None, scales[:7], scales.view(torch.uint8), scales.transpose(1, 2), torch.zeros(8, 16, 2, dtype=torch.uint8, device=cuda).view(_E8M0)]
+    good = dict(keys=rows, values=rows, key_cache=cache, value_cache=cache.clone(), slot_map=slots, key_scales=scales, value_scales=scales)
+    P.store_paged(**good)
+    for bad in [dict(key_scales=s) for s in wrong_scales] + [dict(value_scales=s) for s in wrong_scales] + [
+            dict(keys=rows.half()), dict(keys=rows.double(), values=rows.double()), dict(keys=rows[:, :1]), dict(value_cache=plain), dict(keys=rows[:, :, :48]),
+            dict(key_cache=plain, value_cache=plain), dict(keys=torch.zeros(3 * 128 + 1, device=cuda)[1:].view(3, 2, 64))]:
+        with pytest.raises(ValueError):
+            P.store_paged(**dict(good, **bad))
+    good = dict(key_cache=cache, value_cache=cache, block_table=table, kv_lens=i32, length=10, key_scales=scales, value_scales=scales)
+    P.load_paged(**good)
+    for bad in (dict(length=-1), dict(length=2 ** 31), dict(dtype=torch.float64), dict(kv_lens=i32.long()), dict(block_table=table[:1]), dict(key_scales=None),
+                dict(key_cache=plain, value_cache=plain), dict(key_cache=plain, value_cache=plain, key_scales=None, value_scales=None, dtype=torch.float16)):
+        with pytest.raises(ValueError):
+            P.load_paged(**dict(good, **bad))
+    good = dict(bounds=bounds, key_cache=cache, block_table=table, kv_lens=i32, cu_new=cu, key_scales=scales)
+    P.update_page_bounds(**good)
+    for bad in (dict(bounds=bounds.float()), dict(bounds=bounds[:7]), dict(bounds=bounds.transpose(1, 2)), dict(cu_new=i32), dict(key_scales=None), dict(key_cache=plain)):
+        with pytest.raises(ValueError):
+            P.update_page_bounds(**dict(good, **bad))
+    good = dict(queries=q, bounds=bounds, block_table=table, kv_lens=i32, cu_new=cu, page_size=16, n_select=4)
+    P.select_pages(**good)
+    for bad in (dict(n_select=1), dict(n_select=2 ** 31), dict(window_pages=0), dict(sink_pages=-1), dict(queries=q[:, :3]), dict(queries=q[0]), dict(bounds=bounds[0]),
+                dict(bounds=bounds.double()), dict(queries=q.double()), dict(page_size=24), dict(page_size=2 ** 32 + 16), dict(max_context=-1), dict(cu_new=i32)):
+        with pytest.raises(ValueError):
+            P.select_pages(**dict(good, **bad))
+    good = dict(queries=q, key_cache=cache, value_cache=cache, block_table=table, kv_lens=i32, cu_new=cu, scaling=1.0, key_scales=scales, value_scales=scales, pages=pages)
+    P.paged_attention(**good)
+    for bad in (dict(pages=pages.long()), dict(pages=pages[:2]), dict(pages=pages[:, :1]), dict(pages=pages[:, :, :0]), dict(pages=pages[:, :, ::2]), dict(window_size=8),
+                dict(key_scales=None), dict(queries=q.double()), dict(out=torch.zeros(3, 4, 64, dtype=torch.bfloat16, device=cuda)), dict(scaling=math.nan),
+                dict(key_cache=plain, value_cache=plain), dict(out=q)):
+        with pytest.raises(ValueError):
+            P.paged_attention(**dict(good, **bad))
