@@ -1,14 +1,17 @@
 // Attention over pages in 8 bits, or over the pages that a list names for each token: few rows a request, so that memory bounds it.
 //
-// Of a request's tokens (with a list: of one token) and a key head's query heads every (token, head) is a row; up to 16 are a tile.
-// A workgroup has a tile and a stretch of the keys that it sees, its four waves take 32 keys of it in turn. Nothing is staged: keys and values
+// Of a request's tokens (with a list: of one token) and a key head's query heads every (token, head) is a row; up to 16 are a tile. All
+// tiles of all requests are one line of work, measured in keys; every workgroup takes an equal piece of it, whatever the requests' lengths,
+// finds its place from the lengths on the device, and works through tiles and parts of tiles. A part's (m, l, acc) goes to the workspace, a second
+// kernel joins the parts of a row.
+//
+// The four waves of a workgroup take 32 keys of a tile in turn. Nothing is staged: keys and values
 // go from memory to the registers in which the matrix instructions want them. S^T = K Q^T (16 keys x 16 rows a tile of the matrix): a lane reads 16
 // bytes of a key's row, the 4 lanes of a key 64 neighbouring ones. The result has row n in lanes n + 16 g, keys 4 g .. 4 g + 3 of both key
 // tiles, which is what O^T = V^T P^T wants of P with its key slots in that order; of V lane i + 16 g then holds the 8 keys' dims
 // C i .. C i + C - 1 (a key's row is 16 lanes' pieces, one after the other), and a permutation of 16-bit halves inside the lane makes of
 // them the operand of dim C i + e, the output's tile e. 8-bit elements become bf16 on the way, their scale with them, in one instruction a pair: exact.
 // A 32-key step's K is requested as soon as the step before has been multiplied with its own, V likewise: half a step or more is under way at all times.
-// Parts of a tile (m, l, acc) are joined by a second kernel.
 #include "sah_pages.h"
 #include "sah_spans.h"
 
@@ -18,14 +21,16 @@
 #define PT_STEP 32                      // keys of a wave's step
 #define PT_ROUND (PT_STEP * PT_NW)      // of a workgroup's
 #define PT_MOST 2048                    // keys whose pages a workgroup looks up at once
-#define PT_SPLITS 256                   // workgroups that share a tile, at most
+#define PT_CUS 256
+#define PT_XCDS 8
+// In keys: what starting and ending a tile takes, and the least that is worth a workgroup.
+#define PT_TILE_COST 128
+#define PT_LEAST 256
 
 struct pt_args {
   sah_page_attention_args a;
-  int splits, stretch;    // workgroups that share a tile; keys of each, at least
   int tokens, blocks;     // tokens of a tile; tiles that a token's query heads of a key head make
   int unit;               // window: keys that begin and end with one
-  int64_t groups;         // (token, block, split)
 };
 
 template <int KT, int QT>
@@ -39,6 +44,20 @@ struct pt_types {
   static constexpr float SLACK = MT == SAH_F16 ? 6.0f : 8.0f;
   static constexpr float SCALE = MT == SAH_F16 ? 8.0f : 0.0f;
 };
+
+// The kernel's arguments where they lie. Each call gives an address that the compiler knows nothing of, so that what is read behind it is read again
+// for every tile, instead of being kept in scalar registers, of which there are too few.
+typedef const pt_args __attribute__((address_space(4))) pt_karg;
+__device__ __forceinline__ const pt_args& pt_arguments() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  pt_karg* p = (pt_karg*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const pt_args*)p;
+#else
+  static pt_args* none;
+  return *none;
+#endif
+}
 
 // From products to powers of two. The sign is the query's; 0 is a number so small that all weights are 1.
 __device__ __forceinline__ float pt_log2(float scaling) { return fmaxf(fabsf(scaling) * 1.4426950408889634f, 1e-37f); }
@@ -74,10 +93,136 @@ __device__ __forceinline__ pt_keys pt_keys_of(const pt_args& A, const pg_request
   return k;
 }
 
-// Keys of a workgroup: more than planned where a request is longer than the caller said.
-__device__ __forceinline__ int pt_stretch(const pt_args& A, int n) {
-  const int each = (int)(((int64_t)n + A.splits - 1) / A.splits);
-  return each <= A.stretch ? A.stretch : (int)(((int64_t)each + PT_ROUND - 1) / PT_ROUND * PT_ROUND);
+// ---------------------------------------------------------------------------
+// where the work is
+// ---------------------------------------------------------------------------
+// Cost of a request's tiles, all of them alike: about the keys that its last tile reads. Only the balance depends on it.
+struct pt_cost {
+  int64_t each;
+  int64_t tiles;  // of all key heads
+  __device__ __forceinline__ int64_t all() const { return each * tiles; }
+};
+struct pt_lens { int begin, end, kv; };
+__device__ __forceinline__ pt_lens pt_lens_of(const sah_page_requests& R, int b) { return pt_lens{R.cu_new[b], R.cu_new[b + 1], R.kv_lens[b]}; }
+__device__ __forceinline__ pt_cost pt_cost_of(const pt_args& A, const pt_lens& lens) {
+  const sah_page_attention_args& P = A.a;
+  const sah_page_requests& R = P.requests;
+  const int begin = lens.begin, end = lens.end, kv = lens.kv;
+  pt_cost c{PT_TILE_COST, 0};
+  const int last = end < R.n_tokens ? end : R.n_tokens;
+  if (begin < 0 || begin >= last) return c;
+  c.tiles = (int64_t)((last - begin + A.tokens - 1) / A.tokens) * A.blocks * P.cache.Hkv;
+  int64_t n = (int64_t)kv - end + last;  // keys up to the last row's position
+  const int64_t most = (int64_t)R.table_width * P.cache.page_size;
+  if (P.pages) {
+    n = n > 0 ? (int64_t)P.n_select * P.cache.page_size : 0;
+  } else {
+    n = n < most ? n : most;
+    if (P.window && (int64_t)P.sink + P.window + 2 * (int64_t)A.unit < n) n = (int64_t)P.sink + P.window + 2 * (int64_t)A.unit;
+  }
+  c.each += n > 0 ? n : 0;
+  return c;
+}
+// workgroups that have a piece, and where workgroup w's begins
+__device__ __forceinline__ int pt_sharers(int64_t total, int wgs) {
+  const int64_t w = (total + PT_LEAST - 1) / PT_LEAST;
+  return (int)(w < wgs ? w : wgs);
+}
+__device__ __forceinline__ int64_t pt_bound(int64_t total, int n, int w) {
+  const int64_t each = pg_uniform(pg_div(total, n));
+  return each * w + pg_uniform(pg_div((total - each * n) * w, n));
+}
+// Neighbours on the line share keys' cache lines (scales, and what lies between two heads), so they get the same XCD.
+__device__ __forceinline__ int pt_number() { return (int)(blockIdx.x % PT_XCDS) * (int)(gridDim.x / PT_XCDS) + (int)(blockIdx.x / PT_XCDS); }
+
+// A place on the line: request, tile of it, where the tile begins
+struct pt_place {
+  int b;
+  pt_lens lens;
+  int64_t tile, begin;
+  pt_cost cost;
+  int64_t total, x0, x1;  // the workgroup's piece
+  int sharers;
+};
+// s_sum: PT_NW + 4 words. All threads call. False: no piece.
+__device__ __forceinline__ bool pt_start(const pt_args& A, int w, int wgs, int64_t* s_sum, pt_place& at) {
+  const sah_page_requests& R = A.a.requests;
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
+  auto scan = [&](int64_t v, int64_t& all) -> int64_t {  // inclusive
+    const int64_t incl = (int64_t)sah_wave_incl_scan_u64((uint64_t)v);
+    __syncthreads();
+    if (lane == SAH_WAVE - 1) s_sum[wave] = incl;
+    __syncthreads();
+    int64_t before = 0;
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < PT_NW; ++i) {
+      before += i < wave ? s_sum[i] : 0;
+      all += s_sum[i];
+    }
+    all = pg_uniform(all);
+    return before + incl;
+  };
+  pt_lens lens{0, 0, 0};
+  auto cost_of = [&](int b) -> int64_t {
+    if (b >= R.n_requests) return 0;
+    lens = pt_lens_of(R, b);
+    return pt_cost_of(A, lens).all();
+  };
+  auto share = [&]() {
+    at.sharers = pt_sharers(at.total, wgs);
+    at.x0 = w < at.sharers ? pt_bound(at.total, at.sharers, w) : 0;
+    at.x1 = w < at.sharers ? pt_bound(at.total, at.sharers, w + 1) : 0;
+  };
+  auto claim = [&](int b, int64_t mine, int64_t end) {  // one thread's request holds x0
+    if (mine && end > at.x0 && end - mine <= at.x0) {
+      s_sum[PT_NW] = (int64_t)lens.kv << 32 | (uint32_t)b;
+      s_sum[PT_NW + 1] = end - mine;
+      s_sum[PT_NW + 2] = (int64_t)lens.end << 32 | (uint32_t)lens.begin;
+    }
+  };
+  if (R.n_requests <= PT_NT) {
+    const int64_t mine = cost_of(threadIdx.x), end = scan(mine, at.total);
+    share();
+    claim(threadIdx.x, mine, end);
+  } else {
+    int64_t sum = 0, run = 0, all;
+    for (int b = threadIdx.x; b < R.n_requests; b += PT_NT) sum += cost_of(b);
+    (void)scan(sum, at.total);
+    share();
+    for (int b0 = 0; b0 < R.n_requests; b0 += PT_NT) {
+      const int64_t mine = cost_of(b0 + threadIdx.x), end = run + scan(mine, all);
+      claim(b0 + threadIdx.x, mine, end);
+      run += all;
+    }
+  }
+  __syncthreads();
+  if (w >= at.sharers || at.x0 >= at.x1) return false;
+  const int64_t own = pg_uniform(s_sum[PT_NW]), begin = pg_uniform(s_sum[PT_NW + 1]), rows = pg_uniform(s_sum[PT_NW + 2]);
+  at.b = (int)own;
+  at.lens = pt_lens{(int)rows, (int)(rows >> 32), (int)(own >> 32)};
+  at.cost = pt_cost_of(A, at.lens);
+  at.tile = pg_uniform(pg_div(at.x0 - begin, at.cost.each));
+  at.begin = begin + at.tile * at.cost.each;
+  return true;
+}
+// The next tile on the line; there is one, unless lengths changed under way (an error of the program's, but one that ends)
+__device__ __forceinline__ bool pt_next(const pt_args& A, pt_place& at) {
+  at.begin += at.cost.each;
+  if (++at.tile < at.cost.tiles) return true;
+  at.tile = 0;
+  do {
+    if (++at.b >= A.a.requests.n_requests) return false;
+    at.lens = pt_lens_of(A.a.requests, at.b);
+    at.cost = pt_cost_of(A, at.lens);
+  } while (at.cost.tiles == 0);
+  return true;
+}
+// The key at which a tile's part ends that ends at y of its cost: the same for the one that begins there.
+__device__ __forceinline__ int pt_key_at(int64_t y, int64_t cost, int n) {
+  if (y >= cost) return n;
+  const int u = (int)((double)n * ((double)y / (double)cost));
+  return __builtin_amdgcn_readfirstlane(u / PT_ROUND * PT_ROUND);
 }
 
 // One row key by key, by one wave: what a row holds that came out not finite. The average so far is held, not the sum: of finite values it
@@ -189,12 +334,28 @@ __device__ __forceinline__ sah_f32x4 pt_mfma_f32(float a, float b, sah_f32x4 c) 
 #endif
 }
 
+// Workgroups of a CU, by the registers that an instance needs: waves of a SIMD
+__host__ __device__ constexpr int pt_per_cu(int cache_type, int dim) {
+  return cache_type == SAH_E4M3 ? (dim > 128 ? 2 : dim > 64 ? 3 : 4) : cache_type == SAH_F32 ? (dim > 64 ? 1 : 2) : dim > 128 ? 1 : dim > 64 ? 2 : 4;
+}
+
+// From a uniform address and an offset of the lane: told apart here, or the compiler adds them up in vector registers.
+template <typename W>
+__device__ __forceinline__ W pt_load(const void* base, uint32_t offset) {
+  sah_keep(offset);
+  return *(const W*)((const char*)base + offset);
+}
+
+// Where a 16-key tile (in small pages: a key) lies: bytes from the key head's first key and value, its scales, its number.
+struct __attribute__((aligned(16))) pt_where {
+  int64_t k, v, scale;
+  int first, pad;
+};
+
 // SMALL: pages of less than 16 tokens, where a 16-key tile's keys do not lie in one page
 template <int KT, int QT, int DP, bool SMALL>
-__global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
+__global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_args) {
   sah_touch_kernargs<sizeof(pt_args)>();
-  const sah_page_attention_args& P = A.a;
-  const sah_page_cache& C = P.cache;
   typedef pt_types<KT, QT> T;
   constexpr int ES = pg_size(KT), MT = T::MT;
   constexpr int KL = DP * ES / 64;                                    // 16-byte loads of a lane and key tile
@@ -203,45 +364,51 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
   constexpr int VW = NC * ES / 4;                                     // 32-bit words of a piece
   constexpr int TILES = DP / 16;
   constexpr int PITCH = DP + 4;                                       // floats of a row in LDS
-  constexpr int SLOTS = SMALL ? PT_MOST + PT_ROUND : PT_MOST / 16 + PT_ROUND / 16 + 2;
-  __shared__ int s_page[SLOTS], s_first[SLOTS];                       // of the stretch's pages: number, first key
+  // key tiles of a wave's step: fp32 rows of 256 dims leave no registers for two
+  constexpr int NA = KT == SAH_F32 && DP > 128 ? 1 : 2, STEP = 16 * NA, ROUND = STEP * PT_NW;
+  constexpr int MOST = SMALL ? PT_MOST / 4 : PT_MOST, SLOTS = SMALL ? MOST : MOST / 16;
+  __shared__ pt_where s_at[SLOTS];                                    // of the 16-key tiles (SMALL: keys) that are worked on
   __shared__ __align__(16) float s_acc[PT_NW][PT_ROWS][PITCH];
   __shared__ float s_ml[PT_NW][2][PT_ROWS];
   __shared__ uint32_t s_bad;
 
-  // The key heads of a tile and stretch, whose tokens lie side by side, are on one XCD.
-  const int64_t x = (int64_t)blockIdx.x / 8;
-  const int64_t group = x / C.Hkv * 8 + blockIdx.x % 8;
-  const int hk = (int)(x % C.Hkv);
-  if (group >= A.groups) return;
-  const int split = (int)(group % A.splits);
-  const int64_t tb = group / A.splits;
-  const int block = (int)(tb % A.blocks), t0 = (int)(tb / A.blocks);
+  __shared__ int64_t s_sum[PT_NW + 4];
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id(), i16 = lane & 15, g = lane >> 4;
-  const pg_request req = pg_find_by_wave(P.requests, C.page_size, t0);
-  if (req.b < 0) return;
-  const int G = P.Hq / C.Hkv, i0 = t0 - req.begin;
-  if (A.tokens > 1 && i0 % A.tokens) return;   // not the first of its tile
+  const int w = pt_number();
+  pt_place at;
+  if (!pt_start(pt_arguments(), w, gridDim.x, s_sum, at)) return;
+  int64_t x = at.x0;
+  for (;;) {
+  const pt_args& A = pt_arguments();
+  const sah_page_attention_args& P = A.a;
+  const sah_page_cache& C = P.cache;
+  const int G = P.Hq / C.Hkv, shift = 31 - __builtin_clz(C.page_size);
+  const float c_exp = pt_log2(P.scaling), sign = P.scaling < 0.f ? -1.f : 1.f;
+  const int64_t y0 = x - at.begin, y1 = at.x1 - at.begin < at.cost.each ? at.x1 - at.begin : at.cost.each;
+  const bool whole = y0 == 0 && y1 == at.cost.each;
+  const int tile = __builtin_amdgcn_readfirstlane((int)at.tile);  // (n_tokens * Hq fits)
+  const int tb = tile / C.Hkv, hk = tile - tb * C.Hkv, block = tb % A.blocks, i0 = tb / A.blocks * A.tokens;
+  const int t0 = at.lens.begin + i0;
+  const pg_request req = pg_make(P.requests, C.page_size, at.b, at.lens.begin, at.lens.end, at.lens.kv);
   const int n_tok = A.tokens < req.n_new - i0 ? A.tokens : req.n_new - i0;
   const int rows = A.blocks > 1 ? (G - block * PT_ROWS < PT_ROWS ? G - block * PT_ROWS : PT_ROWS) : n_tok * G;
   const int64_t p_lo = req.base + t0, p_hi = p_lo + n_tok - 1;
   const pt_keys keys = pt_keys_of(A, req, p_lo, p_hi);
-  const int stretch = pt_stretch(A, keys.n);
-  const int64_t begin = (int64_t)split * stretch;
-  if (A.splits > 1 && begin >= keys.n) return;  // (the joining knows)
-  const int u_first = (int)begin, u_end = keys.n - u_first < stretch ? keys.n : u_first + stretch;
-  const int shift = 31 - __builtin_clz(C.page_size);
+  const int u_first = y0 ? pt_key_at(y0, at.cost.each, keys.n) : 0, u_end = pt_key_at(y1, at.cost.each, keys.n);
   const bool live = i16 < rows;
   const int rr = live ? i16 : rows - 1;
   const int tok = t0 + (A.blocks > 1 ? 0 : rr / G), head = hk * G + (A.blocks > 1 ? block * PT_ROWS + rr : rr % G);
   const int64_t p = req.base + tok;
   const int last = p < keys.hi ? (p < -1 ? -1 : (int)p) : keys.hi;          // the last key that this lane's row sees
   const int least = p_lo < keys.hi ? (p_lo < -1 ? -1 : (int)p_lo) : keys.hi; // ... that all rows see
-
+  // window: where it begins for this lane's row, for some row, for all rows
+  const int sink = P.window ? P.sink : 0;
+  auto window_from = [&](int64_t at_p) { return P.window && at_p >= P.window ? (int)(at_p - P.window + 1 < keys.hi + 1 ? at_p - P.window + 1 : keys.hi + 1) : 0; };
+  const int from_own = window_from(p), from_any = window_from(p_lo), from_all = window_from(p_hi);
   if (threadIdx.x == 0) s_bad = 0;
+
   // queries as the second operand, in the order in which a lane's 16 bytes of a key come
   const char* qp = (const char*)P.q + ((int64_t)tok * P.qs_t + (int64_t)head * P.qs_h) * pg_size(QT);
-  const float sign = P.scaling < 0.f ? -1.f : 1.f;
   uint4 qf[T::NQ][KT == SAH_F32 ? KL : DP / 32];
 #pragma unroll
   for (int s = 0; s < (KT == SAH_F32 ? KL : DP / 32); ++s) {
@@ -273,7 +440,6 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
     }
   }
 
-  const float c_exp = pt_log2(P.scaling);
   float m_run = -INFINITY, l_run = 0.f;
   sah_f32x4 acc[TILES];
 #pragma unroll
@@ -281,94 +447,83 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
 
-  // what lies behind a shorter head's end is its last piece again: the queries are 0 there, the results nobody's
-  int k_in[KL];
+  // What lies behind a shorter head's end is its last piece again: the queries are 0 there, the results nobody's. Offsets of a lane from a
+  // key tile's first key (SMALL: from its own key).
+  uint32_t k_in[KL], v_in[H][4];
 #pragma unroll
   for (int s = 0; s < KL; ++s) {
-    const int at = 64 * s + 16 * g;
-    k_in[s] = at < C.D * ES ? at : C.D * ES - 16;
+    const int in = 64 * s + 16 * g;
+    k_in[s] = (uint32_t)((SMALL ? 0 : i16 * C.ks_t * ES) + (in < C.D * ES ? in : C.D * ES - 16));
   }
-  int v_in[H];
 #pragma unroll
   for (int s = 0; s < H; ++s) {
-    const int at = (s * 16 + i16) * NC;
-    v_in[s] = (at < C.D ? at : C.D - NC) * ES;
+    const int in = (s * 16 + i16) * NC;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) v_in[s][v] = (uint32_t)((SMALL ? 0 : (4 * g + v) * C.vs_t * ES) + (in < C.D ? in : C.D - NC) * ES);
   }
   const char* kbase = (const char*)C.k + (int64_t)hk * C.ks_h * ES;
   const char* vbase = (const char*)C.v + (int64_t)hk * C.vs_h * ES;
-  const int kt = (int)(C.ks_t * ES), vt = (int)(C.vs_t * ES);   // (less than 2^28)
+  const uint8_t *k_scales = C.k_scales, *v_scales = C.v_scales;
 
-  sah_u4 kr[2][KL];
-  uint32_t vr[H][8][VW];
-  uint32_t k_scale[2], v_scale[2];   // bytes: of this lane's key in a tile; of its four
-  int u0 = u_first;  // of what s_page and s_first hold
-  auto slot_of = [&](int u) { return (u - u0 + (u0 & (C.page_size - 1))) >> shift; };
-  auto in_page = [&](int u) { return u & (C.page_size - 1); };
+  sah_u4 kr[NA][KL];
+  uint32_t vr[H][4 * NA][VW];
+  uint32_t k_scale[NA], v_scale[NA];   // bytes: of four keys, this lane's among them; of the four whose values it has
+  int u0 = u_first;                  // of what s_at holds
   auto fetch_k = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const char* at;
+    for (int a = 0; a < NA; ++a) {
       if constexpr (SMALL) {
-        const int key = u + 16 * a + i16, page = s_page[slot_of(key)], in = in_page(key);
-        at = kbase + (page * C.ks_p + in * C.ks_t) * ES;
-        if constexpr (KT == SAH_E4M3) k_scale[a] = C.k_scales[((int64_t)page * C.Hkv + hk) * C.page_size + in];
-      } else {
-        const int64_t page = __builtin_amdgcn_readfirstlane(s_page[slot_of(u + 16 * a)]);
-        const int in = in_page(u + 16 * a);
-        at = kbase + (page * C.ks_p + in * C.ks_t) * ES + (int64_t)i16 * kt;
-        if constexpr (KT == SAH_E4M3) k_scale[a] = C.k_scales[(page * C.Hkv + hk) * C.page_size + in + i16];
-      }
+        const pt_where& at = s_at[u + 16 * a + i16 - u0];
+        const char* from = kbase + at.k;
+        if constexpr (KT == SAH_E4M3) k_scale[a] = k_scales[at.scale] * 0x01010101u;
 #pragma unroll
-      for (int s = 0; s < KL; ++s) kr[a][s] = *(const sah_u4*)(at + k_in[s]);
+        for (int s = 0; s < KL; ++s) kr[a][s] = *(const sah_u4*)(from + k_in[s]);
+      } else {
+        const pt_where& at = s_at[(u - u0) / 16 + a];
+        const char* from = kbase + pg_uniform(at.k);
+        if constexpr (KT == SAH_E4M3) k_scale[a] = pt_load<uint32_t>(k_scales + pg_uniform(at.scale), i16 & 12);
+#pragma unroll
+        for (int s = 0; s < KL; ++s) kr[a][s] = pt_load<sah_u4>(from, k_in[s]);
+      }
     }
   };
   auto fetch_v = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const char* at = nullptr;
+    for (int a = 0; a < NA; ++a) {
+      const char* from = nullptr;
       if constexpr (!SMALL) {
-        const int64_t page = __builtin_amdgcn_readfirstlane(s_page[slot_of(u + 16 * a)]);
-        const int in = in_page(u + 16 * a);
-        at = vbase + (page * C.vs_p + in * C.vs_t) * ES + (int64_t)(4 * g) * vt;
-        if constexpr (KT == SAH_E4M3) v_scale[a] = *(const uint32_t*)(C.v_scales + (page * C.Hkv + hk) * C.page_size + in + 4 * g);
+        const pt_where& at = s_at[(u - u0) / 16 + a];
+        from = vbase + pg_uniform(at.v);
+        if constexpr (KT == SAH_E4M3) v_scale[a] = pt_load<uint32_t>(v_scales + pg_uniform(at.scale), 4 * g);
       } else if constexpr (KT == SAH_E4M3) {
         v_scale[a] = 0;
       }
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const char* row;
         if constexpr (SMALL) {
-          const int key = u + 16 * a + 4 * g + v, page = s_page[slot_of(key)], in = in_page(key);
-          row = vbase + (page * C.vs_p + in * C.vs_t) * ES;
-          if constexpr (KT == SAH_E4M3) v_scale[a] |= (uint32_t)C.v_scales[((int64_t)page * C.Hkv + hk) * C.page_size + in] << (8 * v);
-        } else {
-          row = at + (int64_t)v * vt;
+          const pt_where& at = s_at[u + 16 * a + 4 * g + v - u0];
+          from = vbase + at.v;
+          if constexpr (KT == SAH_E4M3) v_scale[a] |= (uint32_t)v_scales[at.scale] << (8 * v);
         }
 #pragma unroll
         for (int s = 0; s < H; ++s) {
-          const char* from = row + v_in[s];
           uint32_t* to = vr[s][4 * a + v];
-          if constexpr (VW == 4) {
-            const sah_u4 w = *(const sah_u4*)from;
-            to[0] = w.x; to[1] = w.y; to[2] = w.z; to[3] = w.w;
-          } else if constexpr (VW == 2) {
-            const sah_u2 w = *(const sah_u2*)from;
-            to[0] = w.x; to[1] = w.y;
-          } else {
-            to[0] = *(const uint32_t*)from;
-          }
+          typedef uint32_t words __attribute__((ext_vector_type(VW)));
+          const words w = SMALL ? *(const words*)(from + v_in[s][v]) : pt_load<words>(from, v_in[s][v]);
+#pragma unroll
+          for (int i = 0; i < VW; ++i) to[i] = w[i];
         }
       }
     }
   };
 
   auto step = [&](int u, auto k_read, auto v_read) __attribute__((always_inline)) {
-    sah_f32x4 s[2];
+    sah_f32x4 s[NA];
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < NA; ++a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[a][e] = 0.f;
-      const float scale = KT == SAH_E4M3 ? pg_scale(k_scale[a]) : 1.f;
+      const float scale = KT == SAH_E4M3 ? pg_scale_of(k_scale[a], i16 & 3) : 1.f;
 #pragma unroll
       for (int c = 0; c < KL; ++c) {
         const sah_u4 k = kr[a][c];
@@ -392,25 +547,22 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
     }
     k_read();
     // keys that not every row sees; values of keys that no row sees are made 0
-    bool plain = true;   // uniform
+    int first[NA] = {};
+    bool plain = !SMALL;   // uniform
     if constexpr (!SMALL) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const int first = __builtin_amdgcn_readfirstlane(s_first[slot_of(u + 16 * a)]) + in_page(u + 16 * a);
-        plain = plain && first + 15 <= least && (!P.window || first + 15 < P.sink || first > p_hi - P.window);
+      for (int a = 0; a < NA; ++a) {
+        first[a] = __builtin_amdgcn_readfirstlane(s_at[(u - u0) / 16 + a].first);
+        plain = plain & (first[a] + 15 <= least) & ((first[a] >= from_all) | (first[a] + 15 < sink));
       }
-    } else {
-      plain = false;
     }
     if (!plain) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int a = 0; a < NA; ++a)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = u + 16 * a + 4 * g + e;
-          const int j = s_first[slot_of(key)] + in_page(key);
-          const bool on = j <= last && (!P.window || j < P.sink || j > p - P.window);
-          const bool some = j <= keys.hi && (!P.window || j < P.sink || j > p_lo - P.window);
+          const int j = SMALL ? s_at[u + 16 * a + 4 * g + e - u0].first : first[a] + 4 * g + e;
+          const bool on = (j <= last) & ((j >= from_own) | (j < sink)), some = (j <= keys.hi) & ((j >= from_any) | (j < sink));
           s[a][e] = on ? s[a][e] : -INFINITY;
 #pragma unroll
           for (int c = 0; c < H; ++c)
@@ -420,7 +572,7 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
       for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[a][e]);
     mx = pt_quad_max(mx);
@@ -439,7 +591,7 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
     // its own size where products are large.)
     const float m_at = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int a = 0; a < NA; ++a)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[a][e] = __builtin_amdgcn_exp2f(fmaf(s[a][e] - m_at, c_exp, T::SCALE));
@@ -447,7 +599,7 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
       }
     if constexpr (KT == SAH_F32) {
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+      for (int a = 0; a < NA; ++a)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -489,36 +641,45 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
     }
     v_read();
   };
-  for (; u0 < u_end; u0 += PT_MOST) {  // (uniform; the next one's first key fits 32 bits: the host has checked what a request can have)
-    const int u1 = u_end - u0 < PT_MOST ? u_end : u0 + PT_MOST;
-    if (u0 != u_first) __syncthreads();   // the pages before have been read
-    const int n_slots = ((u1 - u0 + PT_STEP - 1) / PT_STEP * PT_STEP - 1 + (u0 & (C.page_size - 1))) >> shift;
+  for (; u0 < u_end; u0 += MOST) {  // (uniform; the next one's first key fits 32 bits: the host has checked what a request can have)
+    const int u1 = u_end - u0 < MOST ? u_end : u0 + MOST;
+    __syncthreads();                // the places before have been read, and the sums of the tile before
+    constexpr int EACH = SMALL ? 1 : 16;
+    const int n_slots = (u1 - u0 + STEP - 1) / STEP * (STEP / EACH);
     const int32_t* list = P.pages ? P.pages + ((int64_t)t0 * C.Hkv + hk) * P.n_select : nullptr;
-    for (int s = threadIdx.x; s <= n_slots; s += PT_NT) {
-      const int e = (u0 >> shift) + s;
+    for (int s = threadIdx.x; s < n_slots; s += PT_NT) {
+      const int u = u0 + s * EACH, e = u >> shift;
+      int64_t in = u & (C.page_size - 1);
       int lg = e;
       if (list) lg = e < P.n_select ? list[e] : -1;
-      else if (keys.skip && e >= keys.sinks >> shift) lg = e + (keys.skip >> shift);
-      int page = -1;
+      else if (keys.skip && u >= keys.sinks) lg = e + (keys.skip >> shift);
+      int64_t page = -1;
       if (lg >= 0 && lg < P.requests.table_width && lg <= keys.hi >> shift) page = P.requests.block_table[(int64_t)req.b * P.requests.table_pitch + lg];
-      const bool there = page >= 0 && page < C.n_pages;
-      s_page[s] = there ? page : 0;
-      s_first[s] = there ? lg << shift : (int)(0x80000000u - (uint32_t)C.page_size);  // (behind every position: table_width pages end before it)
+      pt_where at;
+      // a page that is not there: another one's keys, behind every position (table_width pages end before that)
+      at.first = (int)(0x80000000u - (uint32_t)C.page_size + (uint32_t)in);
+      if (page >= 0 && page < C.n_pages) at.first = (lg << shift) + (int)in;
+      else page = in = 0;
+      at.k = (page * C.ks_p + in * C.ks_t) * ES;
+      at.v = (page * C.vs_p + in * C.vs_t) * ES;
+      at.scale = (page * C.Hkv + hk) * C.page_size + in;
+      s_at[s] = at;
     }
     __syncthreads();
-    int u = u0 + PT_STEP * wave;
+    int u = u0 + STEP * wave;
     if (u >= u1) continue;
     fetch_k(u);
     fetch_v(u);
     // (the last step apart: a way through the loop that skips a request would have the compiler wait for all of them)
 #pragma unroll 1
-    for (; u + PT_ROUND < u1; u += PT_ROUND)
-      step(u, [&]() __attribute__((always_inline)) { fetch_k(u + PT_ROUND); }, [&]() __attribute__((always_inline)) { fetch_v(u + PT_ROUND); });
+    for (; u + ROUND < u1; u += ROUND)
+      step(u, [&]() __attribute__((always_inline)) { fetch_k(u + ROUND); }, [&]() __attribute__((always_inline)) { fetch_v(u + ROUND); });
     step(u, [] {}, [] {});
   }
 
-  // the four waves' sums, row by row in LDS (s_bad is set behind the wait)
+  // the four waves' sums, row by row in LDS
   l_run = pt_quad_sum(l_run);
+  if (u_first >= u_end) __syncthreads();  // those of the tile before have been read (else the wait above)
   if (live) {
     if (g == 0) {
       s_ml[wave][0][i16] = m_run;
@@ -551,8 +712,8 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
       o.w += a.w * up;
     }
     const int rt = t0 + (A.blocks > 1 ? 0 : r / G), rh = hk * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G);
-    if (A.splits > 1) {
-      float* to = (float*)P.work + (((int64_t)rt * P.Hq + rh) * A.splits + split) * (DP + 4);
+    if (!whole) {  // a part: to slot 0 where the tile began before this workgroup's piece, else to slot 1
+      float* to = (float*)P.work + (((int64_t)w * 2 + (y0 ? 0 : 1)) * PT_ROWS + r) * (DP + 4);
       if (d == 0) *(float2*)to = make_float2(m, l);
       *(float4*)(to + 4 + d) = o;
       continue;
@@ -568,107 +729,160 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn(pt_args A) {
     if (QT == SAH_F32) *(float4*)to = o;
     else *(uint2*)to = make_uint2(sah_pack2_hw<QT>(o.x, o.y), sah_pack2_hw<QT>(o.z, o.w));
   }
-  if (A.splits > 1) return;
-  __syncthreads();
-  uint32_t bad = s_bad;  // rows that are not finite are done again, each by a wave
-  for (int i = 0; bad; ++i) {
-    const int r = __builtin_ctz(bad);
-    bad &= bad - 1;
-    if (i % PT_NW != wave) continue;
-    pt_row_again<KT, QT>(A, req, t0 + (A.blocks > 1 ? 0 : r / G), hk * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G));
+  if (whole) {
+    __syncthreads();
+    uint32_t bad = s_bad;  // rows that are not finite are done again, each by a wave
+    for (int i = 0; bad; ++i) {
+      const int r = __builtin_ctz(bad);
+      bad &= bad - 1;
+      if (i % PT_NW != wave) continue;
+      pt_row_again<KT, QT>(A, req, t0 + (A.blocks > 1 ? 0 : r / G), hk * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G));
+    }
+    if (at.begin + y1 < at.x1) __syncthreads();  // (s_bad has been read)
+  }
+  x = at.begin + y1;
+  if (x >= at.x1 || !pt_next(pt_arguments(), at)) break;
   }
 }
 
-// Joins the parts of the rows: a wave has a row, a lane DP / 64 of its dims.
-#define PT_JOIN_U 8
+// Joins the parts of a tile's rows, a workgroup each tile. DP / 4 lanes hold a row's dims; where a tile has fewer rows than the workgroup has
+// such groups of lanes, a row's parts are shared by several. blockIdx.y: its rows are dealt to as many workgroups.
 template <int KT, int QT, int DP>
-__global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A) {
-  sah_touch_kernargs<sizeof(pt_args)>();
+__global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A, int wgs) {
+  sah_touch_kernargs<sizeof(pt_args) + 4>();
   const sah_page_attention_args& P = A.a;
   const sah_page_cache& C = P.cache;
   typedef pt_types<KT, QT> T;
-  constexpr int F = DP / 64;
-  const int lane = threadIdx.x & (SAH_WAVE - 1);
-  const int64_t row = (int64_t)blockIdx.x * PT_NW + sah_wave_id();
-  if (row >= (int64_t)P.requests.n_tokens * P.Hq) return;
-  const int t = (int)(row / P.Hq), h = (int)(row - (int64_t)t * P.Hq);
+  constexpr int L = DP / 4, GROUPS = PT_NT / L, U = 8;
+  __shared__ __align__(16) float4 s_acc[GROUPS][L];
+  __shared__ float2 s_ml[GROUPS];
+  const int lane = threadIdx.x & (SAH_WAVE - 1), l = threadIdx.x % L, group = threadIdx.x / L;
+  const int per_token = C.Hkv * A.blocks, t = (int)(blockIdx.x / per_token), in = (int)blockIdx.x - t * per_token, hk = in % C.Hkv, block = in / C.Hkv;
   const pg_request req = pg_find_by_wave(P.requests, C.page_size, t);
   if (req.b < 0) return;
-  const int i = t - req.begin, i0 = i - i % A.tokens, n_tok = A.tokens < req.n_new - i0 ? A.tokens : req.n_new - i0;
-  const int64_t p_lo = req.base + req.begin + i0;
-  const pt_keys keys = pt_keys_of(A, req, p_lo, p_lo + n_tok - 1);
-  const int stretch = pt_stretch(A, keys.n), parts = (int)(((int64_t)keys.n + stretch - 1) / stretch);
-  const float* from = (const float*)P.work + row * A.splits * (DP + 4);
+  const int i = t - req.begin;
+  if (i % A.tokens) return;  // not the first of its tile
+  const int G = P.Hq / C.Hkv, n_tok = A.tokens < req.n_new - i ? A.tokens : req.n_new - i;
+  const int all_rows = A.blocks > 1 ? (G - block * PT_ROWS < PT_ROWS ? G - block * PT_ROWS : PT_ROWS) : n_tok * G;
+  const int rows = (all_rows - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;  // this workgroup's
+  if (rows <= 0) return;
+  // the tile on the line
+  int64_t before = 0, total = 0;
+  for (int b0 = 0; b0 < P.requests.n_requests; b0 += SAH_WAVE) {
+    const int b = b0 + lane;
+    const int64_t c = b < P.requests.n_requests ? pt_cost_of(A, pt_lens_of(P.requests, b)).all() : 0;
+    total += c;
+    before += b < req.b ? c : 0;
+  }
+  total = (int64_t)sah_lane_u64(sah_wave_incl_scan_u64((uint64_t)total), SAH_WAVE - 1);
+  before = (int64_t)sah_lane_u64(sah_wave_incl_scan_u64((uint64_t)before), SAH_WAVE - 1);
+  const pt_cost cost = pt_cost_of(A, pt_lens_of(P.requests, req.b));
+  const int64_t begin = before + (((int64_t)(i / A.tokens) * A.blocks + block) * C.Hkv + hk) * cost.each, end = begin + cost.each;
+  // the workgroups whose pieces hold its first and its last key
+  const int sharers = pt_sharers(total, wgs);
+  auto holder = [&](int64_t x) {
+    int w = __builtin_amdgcn_readfirstlane((int)((double)x / (double)total * sharers));
+    w = w < sharers ? w : sharers - 1;
+    while (w + 1 < sharers && pt_bound(total, sharers, w + 1) <= x) ++w;
+    while (w > 0 && pt_bound(total, sharers, w) > x) --w;
+    return w;
+  };
+  const int w0 = holder(begin), w1 = holder(end - 1);
+  if (w0 == w1) return;  // one workgroup's: written
+  const int parts = w1 - w0 + 1;
+  int shared_by = 1;     // groups that share a row
+  while (2 * shared_by * rows <= GROUPS) shared_by *= 2;
   const float c_exp = pt_log2(P.scaling);
-  float m = -INFINITY, l = 0.f, o[F];
+  const float* from = (const float*)P.work + (int64_t)w0 * 2 * PT_ROWS * (DP + 4);
+  float m, sum;
+  float4 o;
+  auto add = [&](float2 ml, const float4& v) __attribute__((always_inline)) {
+    const float m_new = fmaxf(m, ml.x);
+    const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * c_exp);
+    const float z = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml.x - m_new) * c_exp);
+    // (a part whose sum is NaN has no maximum, perhaps: the row is done again all the same)
+    sum = sum * a + (ml.y == ml.y ? ml.y * z : ml.y);
+    m = m_new;
+    o.x = o.x * a + v.x * z;
+    o.y = o.y * a + v.y * z;
+    o.z = o.z * a + v.z * z;
+    o.w = o.w * a + v.w * z;
+  };
+  for (int r0 = 0; r0 < rows; r0 += GROUPS / shared_by) {  // uniform
+    const int nth = r0 + group / shared_by, turn = group % shared_by, r = nth * (int)gridDim.y + (int)blockIdx.y;
+    const bool mine = nth < rows;
+    m = -INFINITY;
+    sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = turn; mine && p0 < parts; p0 += U * shared_by) {  // several parts requested at once; behind the last one it is taken again, and not added
+      float2 ml[U];
+      float4 v[U];
 #pragma unroll
-  for (int f = 0; f < F; ++f) o[f] = 0.f;
-  for (int p0 = 0; p0 < parts; p0 += PT_JOIN_U) {
-    float2 ml[PT_JOIN_U];
-    float v[PT_JOIN_U][F];
+      for (int i = 0; i < U; ++i) {
+        const int of = p0 + i * shared_by < parts ? p0 + i * shared_by : parts - 1;
+        const float* part = from + ((int64_t)(of ? 2 * of : 1) * PT_ROWS + r) * (DP + 4);
+        ml[i] = *(const float2*)part;
+        v[i] = *(const float4*)(part + 4 + 4 * l);
+      }
 #pragma unroll
-    for (int i = 0; i < PT_JOIN_U; ++i) {
-      const float* part = from + (int64_t)(p0 + i < parts ? p0 + i : parts - 1) * (DP + 4);
-      ml[i] = *(const float2*)part;
-#pragma unroll
-      for (int f = 0; f < F; ++f) v[i][f] = part[4 + lane * F + f];
+      for (int i = 0; i < U; ++i)
+        if (p0 + i * shared_by < parts) add(ml[i], v[i]);
     }
-#pragma unroll
-    for (int i = 0; i < PT_JOIN_U; ++i) {
-      if (p0 + i >= parts) continue;
-      const float m_new = fmaxf(m, ml[i].x);
-      const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * c_exp);
-      const float z = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[i].x - m_new) * c_exp);
-      l = l * a + (ml[i].y == ml[i].y ? ml[i].y * z : ml[i].y);
-      m = m_new;
-#pragma unroll
-      for (int f = 0; f < F; ++f) o[f] = o[f] * a + v[i][f] * z;
+    if (shared_by > 1) {  // (then this is the only round)
+      s_acc[group][l] = o;
+      if (l == 0) s_ml[group] = make_float2(m, sum);
+      __syncthreads();
+      if (mine && turn == 0)
+        for (int i = 1; i < shared_by; ++i) add(s_ml[group + i], s_acc[group + i][l]);
+    }
+    const bool ends = mine && turn == 0;
+    const int rt = t + (A.blocks > 1 ? 0 : r / G), rh = hk * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G), d = 4 * l;
+    bool fine = true;
+    if (ends) {
+      fine = sum == sum;
+      if (P.sinks && m != -INFINITY) sum += __builtin_amdgcn_exp2f(fmaf(P.sinks[rh], 1.4426950408889634f, T::SCALE) - m * c_exp);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      if (d < C.D) {
+        o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+        fine = fine && pt_fine<QT>(o.x) && pt_fine<QT>(o.y) && pt_fine<QT>(o.z) && pt_fine<QT>(o.w);
+        char* to = (char*)P.out + ((int64_t)rt * P.os_t + (int64_t)rh * P.os_h + d) * pg_size(QT);
+        if (QT == SAH_F32) *(float4*)to = o;
+        else *(uint2*)to = make_uint2(sah_pack2_hw<QT>(o.x, o.y), sah_pack2_hw<QT>(o.z, o.w));
+      }
+    }
+    // rows that are not finite are done again, one after the other, by the wave that has them
+    uint64_t again = __ballot(!fine);
+    while (again) {
+      const int at = __builtin_ctzll(again) / L * L;
+      again &= L == SAH_WAVE ? 0ull : ~(((1ull << L) - 1) << at);
+      pt_row_again<KT, QT>(A, req, __builtin_amdgcn_readlane(rt, at), __builtin_amdgcn_readlane(rh, at));
     }
   }
-  bool fine = l == l;
-  if (P.sinks && m != -INFINITY) l += __builtin_amdgcn_exp2f(fmaf(P.sinks[h], 1.4426950408889634f, T::SCALE) - m * c_exp);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int f = 0; f < F; ++f) {
-    const int d = lane * F + f;
-    if (d >= C.D) continue;
-    o[f] *= inv;
-    fine = fine && pt_fine<QT>(o[f]);
-    sah_store<QT>(P.out, (int64_t)t * P.os_t + (int64_t)h * P.os_h + d, o[f]);
-  }
-  if (__ballot(!fine)) pt_row_again<KT, QT>(A, req, t, h);
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-// How a call's tiles are shared. About PT_WGS workgroups, if that leaves each a round of keys; no more than PT_MOST keys of each, so that requests of uneven
-// lengths keep the card busy, but where there are many tiles.
-#define PT_WGS 1024
-static pt_args pt_plan(const sah_page_attention_args* a) {
+static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
   pt_args A;
   A.a = *a;
   const int G = a->Hq / a->cache.Hkv;
   A.tokens = a->pages || G >= PT_ROWS ? 1 : PT_ROWS / G;
   A.blocks = (G + PT_ROWS - 1) / PT_ROWS;
   A.unit = a->cache.page_size > PT_STEP ? a->cache.page_size : PT_STEP;
+  // About as many workgroups as the call has work for, at most what the card holds at once. Only how the work is shared depends on it.
   const int64_t table = (int64_t)a->requests.table_width * a->cache.page_size;
-  int64_t most = table;   // keys that a tile may see
-  if (a->pages) most = (int64_t)a->n_select * a->cache.page_size;
-  else if (a->window) {
-    const int64_t w = ((int64_t)a->sink + A.unit - 1) / A.unit * A.unit + a->window + A.tokens + 2 * (int64_t)A.unit;
-    most = w < table ? w : table;
+  int64_t keys = table;
+  if (a->pages) {
+    keys = (int64_t)a->n_select * a->cache.page_size;
+  } else {
+    if (a->max_context > 0 && a->max_context < keys) keys = a->max_context;
+    if (a->window && (int64_t)a->sink + a->window + 2 * (int64_t)A.unit < keys) keys = (int64_t)a->sink + a->window + 2 * (int64_t)A.unit;
   }
-  int64_t usual = most;   // ... about, by what the caller says
-  if (!a->pages && a->max_context > 0 && a->max_context < usual) usual = a->max_context;
   const double tiles = ((double)a->requests.n_tokens / A.tokens + (A.tokens > 1 ? a->requests.n_requests : 0)) * A.blocks * a->cache.Hkv;
-  const double limit = tiles > 4 * PT_WGS ? PT_MOST * tiles / (4 * PT_WGS) : PT_MOST;
-  const double each = fmin(tiles * (double)usual / PT_WGS, limit);
-  A.stretch = (int)((int64_t)(fmin(each, 1e9) + PT_ROUND - 1) / PT_ROUND * PT_ROUND);
-  if (A.stretch < PT_ROUND) A.stretch = PT_ROUND;
-  const int64_t splits = (usual + A.stretch - 1) / A.stretch;
-  A.splits = (int)(splits < 1 ? 1 : splits < PT_SPLITS ? splits : PT_SPLITS);
-  A.groups = (int64_t)a->requests.n_tokens * A.blocks * A.splits;
+  const double n = tiles * (double)(keys + PT_TILE_COST) / PT_LEAST;
+  const int most = PT_CUS * pt_per_cu(a->cache.dtype, a->cache.D);
+  wgs = n < most ? ((int)n / PT_XCDS + 1) * PT_XCDS : most;
   return A;
 }
 
@@ -716,12 +930,13 @@ extern "C" int64_t sah_page_attention_work_bytes(const sah_page_attention_args* 
     const sah_paged_attention_args p = pt_on_copy(a);
     return copy + 4 * sah_paged_attention_work_floats(&p);
   }
-  const pt_args A = pt_plan(a);
-  return A.splits > 1 ? (int64_t)a->requests.n_tokens * a->Hq * A.splits * (pt_dim(a) + 4) * 4 : 0;
+  int wgs;
+  (void)pt_plan(a, wgs);
+  return (int64_t)wgs * 2 * PT_ROWS * (pt_dim(a) + 4) * 4;
 }
 
 template <int KT, int QT, int DP>
-static int pt_launch(const pt_args& A, unsigned wgs) {
+static int pt_launch(const pt_args& A, int wgs) {
   hipStream_t st = (hipStream_t)A.a.stream;
   {
     sah_timed timed("k_page_attn", A.a.stream);
@@ -729,14 +944,13 @@ static int pt_launch(const pt_args& A, unsigned wgs) {
     else hipLaunchKernelGGL((k_page_attn<KT, QT, DP, false>), dim3(wgs), dim3(PT_NT), 0, st, A);
     if (int rc = sah_launch_status("sah_page_attention")) return rc;
   }
-  if (A.splits == 1) return SAH_OK;
   sah_timed timed("k_page_attn_join", A.a.stream);
-  const int64_t rows = (int64_t)A.a.requests.n_tokens * A.a.Hq;
-  hipLaunchKernelGGL((k_page_attn_join<KT, QT, DP>), dim3((unsigned)((rows + PT_NW - 1) / PT_NW)), dim3(PT_NT), 0, st, A);
+  const int64_t tiles = (int64_t)A.a.requests.n_tokens * A.a.cache.Hkv * A.blocks;
+  hipLaunchKernelGGL((k_page_attn_join<KT, QT, DP>), dim3((unsigned)tiles, tiles < 2 * PT_CUS ? 4 : 1), dim3(PT_NT), 0, st, A, wgs);
   return sah_launch_status("sah_page_attention(join)");
 }
 template <int KT, int QT>
-static int pt_launch_dim(const pt_args& A, unsigned wgs) {
+static int pt_launch_dim(const pt_args& A, int wgs) {
   const int dp = pt_dim(&A.a);
   return dp == 64 ? pt_launch<KT, QT, 64>(A, wgs) : dp == 128 ? pt_launch<KT, QT, 128>(A, wgs) : pt_launch<KT, QT, 256>(A, wgs);
 }
@@ -760,6 +974,9 @@ extern "C" int sah_page_attention(const sah_page_attention_args* given) {
   if (int rc = pg_check_requests(r, c.page_size, true, what)) return rc;
   if ((int64_t)a->n_select * c.page_size > INT32_MAX - 4096) return sah_fail(SAH_ESHAPE, "sah_page_attention: n_select * page_size passes 2^31 - 4097");
   if ((int64_t)r.n_tokens * a->Hq > 1 << 30) return sah_fail(SAH_ESHAPE, "sah_page_attention: n_tokens * Hq passes 2^30");
+  // the line of work is divided in doubles, also where running sums overlap
+  const double each = (a->pages ? (double)a->n_select : (double)r.table_width) * c.page_size + PT_TILE_COST;
+  if (((double)r.n_tokens + r.n_requests) * a->Hq * each * r.n_requests > 0x1p52) return sah_fail(SAH_ESHAPE, "sah_page_attention: too much work for one call");
   if (r.n_tokens == 0) return SAH_OK;
   if (!a->q || !a->out) return sah_fail(SAH_ENULL, "sah_page_attention: NULL pointer");
   if (r.n_tokens == 1) a->qs_t = a->os_t = 0;
@@ -795,13 +1012,12 @@ extern "C" int sah_page_attention(const sah_page_attention_args* given) {
     p.work_floats = (a->work_bytes - copy) / 4;
     return sah_paged_attention(&p);
   }
-  const pt_args A = pt_plan(a);
-  const int64_t wgs = (A.groups + 7) / 8 * 8 * c.Hkv;
-  if (wgs > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_attention: too much work for one call");
-  if (c.dtype == SAH_F32) return pt_launch_dim<SAH_F32, SAH_F32>(A, (unsigned)wgs);
-  if (c.dtype == SAH_BF16) return pt_launch_dim<SAH_BF16, SAH_BF16>(A, (unsigned)wgs);
-  if (c.dtype == SAH_F16) return pt_launch_dim<SAH_F16, SAH_F16>(A, (unsigned)wgs);
-  if (a->dtype == SAH_F32) return pt_launch_dim<SAH_E4M3, SAH_F32>(A, (unsigned)wgs);
-  if (a->dtype == SAH_BF16) return pt_launch_dim<SAH_E4M3, SAH_BF16>(A, (unsigned)wgs);
-  return pt_launch_dim<SAH_E4M3, SAH_F16>(A, (unsigned)wgs);
+  int wgs;
+  const pt_args A = pt_plan(a, wgs);
+  if (c.dtype == SAH_F32) return pt_launch_dim<SAH_F32, SAH_F32>(A, wgs);
+  if (c.dtype == SAH_BF16) return pt_launch_dim<SAH_BF16, SAH_BF16>(A, wgs);
+  if (c.dtype == SAH_F16) return pt_launch_dim<SAH_F16, SAH_F16>(A, wgs);
+  if (a->dtype == SAH_F32) return pt_launch_dim<SAH_E4M3, SAH_F32>(A, wgs);
+  if (a->dtype == SAH_BF16) return pt_launch_dim<SAH_E4M3, SAH_BF16>(A, wgs);
+  return pt_launch_dim<SAH_E4M3, SAH_F16>(A, wgs);
 }

@@ -52,10 +52,9 @@ struct pg_request {
   int64_t base;      // row t stands at position base + t
 };
 __device__ __forceinline__ pg_request pg_none() { return pg_request{-1, 0, 0, 0, 0}; }
-__device__ __forceinline__ pg_request pg_read(const sah_page_requests& R, int page_size, int b, int t) {
+// with begin in [0, n_tokens), begin < end
+__device__ __forceinline__ pg_request pg_make(const sah_page_requests& R, int page_size, int b, int begin, int end, int kv) {
   pg_request r;
-  const int begin = R.cu_new[b], end = R.cu_new[b + 1], kv = R.kv_lens[b];
-  if (begin < 0 || t < begin || t >= end) return pg_none();  // (running sums that fall: nobody's)
   const int last = end < R.n_tokens ? end : R.n_tokens, most = R.table_width * page_size;
   r.b = b;
   r.begin = begin;
@@ -64,6 +63,25 @@ __device__ __forceinline__ pg_request pg_read(const sah_page_requests& R, int pa
   r.base = (int64_t)kv - end;
   return r;
 }
+__device__ __forceinline__ pg_request pg_read(const sah_page_requests& R, int page_size, int b, int t) {
+  const int begin = R.cu_new[b], end = R.cu_new[b + 1], kv = R.kv_lens[b];
+  if (begin < 0 || t < begin || t >= end) return pg_none();  // (running sums that fall: nobody's)
+  return pg_make(R, page_size, b, begin, end, kv);
+}
+// What all lanes of the wave hold, in scalar registers (doubles are divided in vector ones)
+__device__ __forceinline__ int64_t pg_uniform(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+// a / b for 0 <= a < 2^53, 0 < b: exact. (The 64-bit division of integers is some 150 instructions.)
+__device__ __forceinline__ int64_t pg_div(int64_t a, int64_t b) {
+  int64_t q = (int64_t)((double)a / (double)b);
+  const int64_t r = a - q * b;
+  q -= r < 0;
+  q += r >= b;
+  return q;
+}
+
 // By a whole wave, for a row that all of its lanes ask for: 64 ends are looked at in one trip to memory.
 __device__ __forceinline__ pg_request pg_find_by_wave(const sah_page_requests& R, int page_size, int t) {
   const int lane = threadIdx.x & (SAH_WAVE - 1);
