@@ -19,7 +19,6 @@
 #define PT_NW (PT_NT / SAH_WAVE)
 #define PT_ROWS 16
 #define PT_STEP 32                      // keys of a wave's step
-#define PT_ROUND (PT_STEP * PT_NW)      // of a workgroup's
 #define PT_MOST 2048                    // keys whose pages a workgroup looks up at once
 #define PT_CUS 256
 #define PT_XCDS 8
@@ -31,6 +30,9 @@ struct pt_args {
   sah_page_attention_args a;
   int tokens, blocks;     // tokens of a tile; tiles that a token's query heads of a key head make
   int unit;               // window: keys that begin and end with one
+  // Key heads that a workgroup works on at once, each by as many of its waves: 4, 2 or 1. Their keys lie side by side (64 answers of 1K to 32K keys, 8
+  // heads: 4.9 TB/s one by one, 5.6 so); with a list each has pages of its own, and 1 it is.
+  int heads;
 };
 
 template <int KT, int QT>
@@ -99,7 +101,7 @@ __device__ __forceinline__ pt_keys pt_keys_of(const pt_args& A, const pg_request
 // Cost of a request's tiles, all of them alike: about the keys that its last tile reads. Only the balance depends on it.
 struct pt_cost {
   int64_t each;
-  int64_t tiles;  // of all key heads
+  int64_t tiles;  // of all groups of key heads
   __device__ __forceinline__ int64_t all() const { return each * tiles; }
 };
 struct pt_lens { int begin, end, kv; };
@@ -111,7 +113,7 @@ __device__ __forceinline__ pt_cost pt_cost_of(const pt_args& A, const pt_lens& l
   pt_cost c{PT_TILE_COST, 0};
   const int last = end < R.n_tokens ? end : R.n_tokens;
   if (begin < 0 || begin >= last) return c;
-  c.tiles = (int64_t)((last - begin + A.tokens - 1) / A.tokens) * A.blocks * P.cache.Hkv;
+  c.tiles = (int64_t)((last - begin + A.tokens - 1) / A.tokens) * A.blocks * (P.cache.Hkv / A.heads);
   int64_t n = (int64_t)kv - end + last;  // keys up to the last row's position
   const int64_t most = (int64_t)R.table_width * P.cache.page_size;
   if (P.pages) {
@@ -123,14 +125,28 @@ __device__ __forceinline__ pt_cost pt_cost_of(const pt_args& A, const pt_lens& l
   c.each += n > 0 ? n : 0;
   return c;
 }
-// workgroups that have a piece, and where workgroup w's begins
-__device__ __forceinline__ int pt_sharers(int64_t total, int wgs) {
-  const int64_t w = (total + PT_LEAST - 1) / PT_LEAST;
-  return (int)(w < wgs ? w : wgs);
-}
-__device__ __forceinline__ int64_t pt_bound(int64_t total, int n, int w) {
-  const int64_t each = pg_uniform(pg_div(total, n));
-  return each * w + pg_uniform(pg_div((total - each * n) * w, n));
+// How the line is shared: by `n` workgroups, and where workgroup w's piece begins
+struct pt_shares {
+  int64_t total, each;
+  uint32_t n, rest;
+  __device__ __forceinline__ int64_t bound(int w) const { return each * w + rest * (uint32_t)w / n; }  // (n is at most 1024)
+};
+__device__ __forceinline__ pt_shares pt_share(const pt_args& A, int64_t total, int wgs) {
+  const sah_page_attention_args& P = A.a;
+  pt_shares s;
+  const int64_t w = (total * A.heads + PT_LEAST - 1) / PT_LEAST;
+  s.total = total;
+  s.n = (uint32_t)(w < wgs ? w : wgs);
+  // Tiles that are all alike (lists; one request): so many workgroups that no piece holds parts of two. A second tile of a short piece costs as
+  // much as the first (1024 keys of 8 heads: 15 -> 9 us).
+  const pt_cost one = pt_cost_of(A, P.pages ? pt_lens{0, 1, 0x40000000} : pt_lens_of(P.requests, 0));
+  if ((P.pages || P.requests.n_requests == 1) && total >= one.each) {
+    const int64_t tiles = pg_uniform(pg_div(total, one.each));
+    if (tiles * one.each == total && tiles < s.n) s.n -= s.n % (uint32_t)tiles;
+  }
+  s.each = s.n ? pg_uniform(pg_div(total, s.n)) : 0;
+  s.rest = (uint32_t)(total - s.each * s.n);
+  return s;
 }
 // Neighbours on the line share keys' cache lines (scales, and what lies between two heads), so they get the same XCD.
 __device__ __forceinline__ int pt_number() { return (int)(blockIdx.x % PT_XCDS) * (int)(gridDim.x / PT_XCDS) + (int)(blockIdx.x / PT_XCDS); }
@@ -141,8 +157,7 @@ struct pt_place {
   pt_lens lens;
   int64_t tile, begin;
   pt_cost cost;
-  int64_t total, x0, x1;  // the workgroup's piece
-  int sharers;
+  int64_t x0, x1;  // the workgroup's piece
 };
 // s_sum: PT_NW + 4 words. All threads call. False: no piece.
 __device__ __forceinline__ bool pt_start(const pt_args& A, int w, int wgs, int64_t* s_sum, pt_place& at) {
@@ -169,10 +184,10 @@ __device__ __forceinline__ bool pt_start(const pt_args& A, int w, int wgs, int64
     lens = pt_lens_of(R, b);
     return pt_cost_of(A, lens).all();
   };
-  auto share = [&]() {
-    at.sharers = pt_sharers(at.total, wgs);
-    at.x0 = w < at.sharers ? pt_bound(at.total, at.sharers, w) : 0;
-    at.x1 = w < at.sharers ? pt_bound(at.total, at.sharers, w + 1) : 0;
+  auto share = [&](int64_t total) {
+    const pt_shares s = pt_share(A, total, wgs);
+    at.x0 = w < (int)s.n ? s.bound(w) : 0;
+    at.x1 = w < (int)s.n ? s.bound(w + 1) : 0;
   };
   auto claim = [&](int b, int64_t mine, int64_t end) {  // one thread's request holds x0
     if (mine && end > at.x0 && end - mine <= at.x0) {
@@ -181,15 +196,16 @@ __device__ __forceinline__ bool pt_start(const pt_args& A, int w, int wgs, int64
       s_sum[PT_NW + 2] = (int64_t)lens.end << 32 | (uint32_t)lens.begin;
     }
   };
+  int64_t total;
   if (R.n_requests <= PT_NT) {
-    const int64_t mine = cost_of(threadIdx.x), end = scan(mine, at.total);
-    share();
+    const int64_t mine = cost_of(threadIdx.x), end = scan(mine, total);
+    share(total);
     claim(threadIdx.x, mine, end);
   } else {
     int64_t sum = 0, run = 0, all;
     for (int b = threadIdx.x; b < R.n_requests; b += PT_NT) sum += cost_of(b);
-    (void)scan(sum, at.total);
-    share();
+    (void)scan(sum, total);
+    share(total);
     for (int b0 = 0; b0 < R.n_requests; b0 += PT_NT) {
       const int64_t mine = cost_of(b0 + threadIdx.x), end = run + scan(mine, all);
       claim(b0 + threadIdx.x, mine, end);
@@ -197,7 +213,7 @@ __device__ __forceinline__ bool pt_start(const pt_args& A, int w, int wgs, int64
     }
   }
   __syncthreads();
-  if (w >= at.sharers || at.x0 >= at.x1) return false;
+  if (at.x0 >= at.x1) return false;
   const int64_t own = pg_uniform(s_sum[PT_NW]), begin = pg_uniform(s_sum[PT_NW + 1]), rows = pg_uniform(s_sum[PT_NW + 2]);
   at.b = (int)own;
   at.lens = pt_lens{(int)rows, (int)(rows >> 32), (int)(own >> 32)};
@@ -222,7 +238,7 @@ __device__ __forceinline__ bool pt_next(const pt_args& A, pt_place& at) {
 __device__ __forceinline__ int pt_key_at(int64_t y, int64_t cost, int n) {
   if (y >= cost) return n;
   const int u = (int)((double)n * ((double)y / (double)cost));
-  return __builtin_amdgcn_readfirstlane(u / PT_ROUND * PT_ROUND);
+  return __builtin_amdgcn_readfirstlane(u / PT_STEP * PT_STEP);
 }
 
 // One row key by key, by one wave: what a row holds that came out not finite. The average so far is held, not the sum: of finite values it
@@ -336,7 +352,7 @@ __device__ __forceinline__ sah_f32x4 pt_mfma_f32(float a, float b, sah_f32x4 c) 
 
 // Workgroups of a CU, by the registers that an instance needs: waves of a SIMD
 __host__ __device__ constexpr int pt_per_cu(int cache_type, int dim) {
-  return cache_type == SAH_E4M3 ? (dim > 128 ? 2 : dim > 64 ? 3 : 4) : cache_type == SAH_F32 ? (dim > 64 ? 1 : 2) : dim > 128 ? 1 : dim > 64 ? 2 : 4;
+  return cache_type == SAH_F32 ? (dim > 64 ? 1 : 2) : dim > 128 ? 1 : dim > 64 ? 2 : 3;
 }
 
 // From a uniform address and an offset of the lane: told apart here, or the compiler adds them up in vector registers.
@@ -346,7 +362,7 @@ __device__ __forceinline__ W pt_load(const void* base, uint32_t offset) {
   return *(const W*)((const char*)base + offset);
 }
 
-// Where a 16-key tile (in small pages: a key) lies: bytes from the key head's first key and value, its scales, its number.
+// Where a 16-key tile (in small pages: a key) lies: bytes from a key head's first key and value, and scale; its number.
 struct __attribute__((aligned(16))) pt_where {
   int64_t k, v, scale;
   int first, pad;
@@ -365,12 +381,12 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
   constexpr int TILES = DP / 16;
   constexpr int PITCH = DP + 4;                                       // floats of a row in LDS
   // key tiles of a wave's step: fp32 rows of 256 dims leave no registers for two
-  constexpr int NA = KT == SAH_F32 && DP > 128 ? 1 : 2, STEP = 16 * NA, ROUND = STEP * PT_NW;
+  constexpr int NA = KT == SAH_F32 && DP > 128 ? 1 : 2, STEP = 16 * NA;
   constexpr int MOST = SMALL ? PT_MOST / 4 : PT_MOST, SLOTS = SMALL ? MOST : MOST / 16;
   __shared__ pt_where s_at[SLOTS];                                    // of the 16-key tiles (SMALL: keys) that are worked on
   __shared__ __align__(16) float s_acc[PT_NW][PT_ROWS][PITCH];
   __shared__ float s_ml[PT_NW][2][PT_ROWS];
-  __shared__ uint32_t s_bad;
+  __shared__ unsigned long long s_bad;  // a bit a head and row
 
   __shared__ int64_t s_sum[PT_NW + 4];
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id(), i16 = lane & 15, g = lane >> 4;
@@ -387,7 +403,8 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
   const int64_t y0 = x - at.begin, y1 = at.x1 - at.begin < at.cost.each ? at.x1 - at.begin : at.cost.each;
   const bool whole = y0 == 0 && y1 == at.cost.each;
   const int tile = __builtin_amdgcn_readfirstlane((int)at.tile);  // (n_tokens * Hq fits)
-  const int tb = tile / C.Hkv, hk = tile - tb * C.Hkv, block = tb % A.blocks, i0 = tb / A.blocks * A.tokens;
+  const int head_groups = C.Hkv / A.heads, tb = tile / head_groups, hk0 = (tile - tb * head_groups) * A.heads, block = tb % A.blocks, i0 = tb / A.blocks * A.tokens;
+  const int hk = hk0 + (wave & (A.heads - 1)), turns = PT_NW / A.heads, turn = wave / A.heads;  // this wave's head; a head's waves take turns
   const int t0 = at.lens.begin + i0;
   const pg_request req = pg_make(P.requests, C.page_size, at.b, at.lens.begin, at.lens.end, at.lens.kv);
   const int n_tok = A.tokens < req.n_new - i0 ? A.tokens : req.n_new - i0;
@@ -407,38 +424,81 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
   const int from_own = window_from(p), from_any = window_from(p_lo), from_all = window_from(p_hi);
   if (threadIdx.x == 0) s_bad = 0;
 
-  // queries as the second operand, in the order in which a lane's 16 bytes of a key come
+  // Queries as the second operand, in the order in which a lane's 16 bytes of a key come: requested here, made into it when the first keys are
+  // under way.
+  constexpr int QS = KT == SAH_F32 ? KL : DP / 32, QE = KT == SAH_F32 ? 4 : 8, QW = QE * pg_size(QT) / 16;  // pieces, elements, loads of a piece
   const char* qp = (const char*)P.q + ((int64_t)tok * P.qs_t + (int64_t)head * P.qs_h) * pg_size(QT);
-  uint4 qf[T::NQ][KT == SAH_F32 ? KL : DP / 32];
+  uint4 qf[T::NQ][QS];
+  sah_u4 q_raw[QS][QW];
 #pragma unroll
-  for (int s = 0; s < (KT == SAH_F32 ? KL : DP / 32); ++s) {
-    constexpr int E = KT == SAH_F32 ? 4 : 8;
+  for (int s = 0; s < QS; ++s) {
     const int d = KT == SAH_F32 ? 16 * s + 4 * g : KT == SAH_E4M3 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
-    float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    if (d < C.D && live) {
-      if constexpr (KT == SAH_F32) {
-        const float4 f = *(const float4*)(qp + 4 * d);
-        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-      } else {
-        sah_load8<QT>(qp, d, v);
-      }
+    for (int i = 0; i < QW; ++i) {
+      q_raw[s][i] = sah_u4{0, 0, 0, 0};
+      if (d < C.D && live) q_raw[s][i] = *(const sah_u4*)(qp + d * pg_size(QT) + 16 * i);
     }
+  }
+  // Where the keys from u0 on lie, MOST of them
+  auto look_up = [&](int u0) __attribute__((always_inline)) {
+    const int u1 = u_end - u0 < MOST ? u_end : u0 + MOST;
+    constexpr int EACH = SMALL ? 1 : 16;
+    const int n_slots = (u1 - u0 + STEP - 1) / STEP * (STEP / EACH);
+    const int32_t* list = P.pages ? P.pages + ((int64_t)t0 * C.Hkv + hk0) * P.n_select : nullptr;
+    for (int s = threadIdx.x; s < n_slots; s += PT_NT) {
+      const int u = u0 + s * EACH, e = u >> shift;
+      int64_t in = u & (C.page_size - 1);
+      int lg = e;
+      if (list) lg = e < P.n_select ? list[e] : -1;
+      else if (keys.skip && u >= keys.sinks) lg = e + (keys.skip >> shift);
+      int64_t page = -1;
+      if (lg >= 0 && lg < P.requests.table_width && lg <= keys.hi >> shift) page = P.requests.block_table[(int64_t)req.b * P.requests.table_pitch + lg];
+      pt_where at;
+      // a page that is not there: another one's keys, behind every position (table_width pages end before that)
+      at.first = (int)(0x80000000u - (uint32_t)C.page_size + (uint32_t)in);
+      if (page >= 0 && page < C.n_pages) at.first = (lg << shift) + (int)in;
+      else page = in = 0;
+      at.k = (page * C.ks_p + in * C.ks_t) * ES;
+      at.v = (page * C.vs_p + in * C.vs_t) * ES;
+      at.scale = page * C.Hkv * C.page_size + in;
+      s_at[s] = at;
+    }
+  };
+  __syncthreads();  // the sums of the tile before have been read
+  if (u_first < u_end) look_up(u_first);
+  {
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] *= sign;
-    if constexpr (KT == SAH_F32) {
-      qf[0][s] = make_uint4(sah_float_to_bits(v[0]), sah_float_to_bits(v[1]), sah_float_to_bits(v[2]), sah_float_to_bits(v[3]));
-    } else {
+    for (int s = 0; s < QS; ++s) {
+      float v[8];
 #pragma unroll
-      for (int i = 0; i < T::NQ; ++i) {
-        uint32_t w[4];
+      for (int i = 0; i < QW; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = pt_term<MT>(v[2 * k], v[2 * k + 1]);
-        qf[i][s] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t x = q_raw[s][i][k];
+          if constexpr (QT == SAH_F32) {
+            v[4 * i + k] = sign * sah_bits_to_float(x);
+          } else if constexpr (QT == SAH_BF16) {
+            v[2 * k] = sign * sah_bits_to_float(x << 16);
+            v[2 * k + 1] = sign * sah_bits_to_float(x & 0xffff0000u);
+          } else {
+            v[2 * k] = sign * sah_f16_to_float((uint16_t)x);
+            v[2 * k + 1] = sign * sah_f16_to_float((uint16_t)(x >> 16));
+          }
+        }
+      if constexpr (KT == SAH_F32) {
+        qf[0][s] = make_uint4(sah_float_to_bits(v[0]), sah_float_to_bits(v[1]), sah_float_to_bits(v[2]), sah_float_to_bits(v[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < T::NQ; ++i) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = pt_term<MT>(v[2 * k], v[2 * k + 1]);
+          qf[i][s] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
     }
   }
+  __syncthreads();
 
   float m_run = -INFINITY, l_run = 0.f;
   sah_f32x4 acc[TILES];
@@ -463,51 +523,50 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
   }
   const char* kbase = (const char*)C.k + (int64_t)hk * C.ks_h * ES;
   const char* vbase = (const char*)C.v + (int64_t)hk * C.vs_h * ES;
-  const uint8_t *k_scales = C.k_scales, *v_scales = C.v_scales;
+  const uint8_t *k_scales = C.k_scales + (int64_t)hk * C.page_size, *v_scales = C.v_scales + (int64_t)hk * C.page_size;
 
-  sah_u4 kr[NA][KL];
-  uint32_t vr[H][4 * NA][VW];
-  uint32_t k_scale[NA], v_scale[NA];   // bytes: of four keys, this lane's among them; of the four whose values it has
+  struct keys_of { sah_u4 r[NA][KL]; uint32_t scale[NA]; } kb;           // scales: bytes, of four keys, this lane's among them
+  struct values_of { uint32_t r[H][4 * NA][VW]; uint32_t scale[NA]; } vb; // ... of the four whose values a lane has
   int u0 = u_first;                  // of what s_at holds
-  auto fetch_k = [&](int u) __attribute__((always_inline)) {
+  auto fetch_k = [&](int u, keys_of& k) __attribute__((always_inline)) {
 #pragma unroll
     for (int a = 0; a < NA; ++a) {
       if constexpr (SMALL) {
         const pt_where& at = s_at[u + 16 * a + i16 - u0];
         const char* from = kbase + at.k;
-        if constexpr (KT == SAH_E4M3) k_scale[a] = k_scales[at.scale] * 0x01010101u;
+        if constexpr (KT == SAH_E4M3) k.scale[a] = k_scales[at.scale] * 0x01010101u;
 #pragma unroll
-        for (int s = 0; s < KL; ++s) kr[a][s] = *(const sah_u4*)(from + k_in[s]);
+        for (int s = 0; s < KL; ++s) k.r[a][s] = *(const sah_u4*)(from + k_in[s]);
       } else {
         const pt_where& at = s_at[(u - u0) / 16 + a];
         const char* from = kbase + pg_uniform(at.k);
-        if constexpr (KT == SAH_E4M3) k_scale[a] = pt_load<uint32_t>(k_scales + pg_uniform(at.scale), i16 & 12);
+        if constexpr (KT == SAH_E4M3) k.scale[a] = pt_load<uint32_t>(k_scales + pg_uniform(at.scale), i16 & 12);
 #pragma unroll
-        for (int s = 0; s < KL; ++s) kr[a][s] = pt_load<sah_u4>(from, k_in[s]);
+        for (int s = 0; s < KL; ++s) k.r[a][s] = pt_load<sah_u4>(from, k_in[s]);
       }
     }
   };
-  auto fetch_v = [&](int u) __attribute__((always_inline)) {
+  auto fetch_v = [&](int u, values_of& x) __attribute__((always_inline)) {
 #pragma unroll
     for (int a = 0; a < NA; ++a) {
       const char* from = nullptr;
       if constexpr (!SMALL) {
         const pt_where& at = s_at[(u - u0) / 16 + a];
         from = vbase + pg_uniform(at.v);
-        if constexpr (KT == SAH_E4M3) v_scale[a] = pt_load<uint32_t>(v_scales + pg_uniform(at.scale), 4 * g);
+        if constexpr (KT == SAH_E4M3) x.scale[a] = pt_load<uint32_t>(v_scales + pg_uniform(at.scale), 4 * g);
       } else if constexpr (KT == SAH_E4M3) {
-        v_scale[a] = 0;
+        x.scale[a] = 0;
       }
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         if constexpr (SMALL) {
           const pt_where& at = s_at[u + 16 * a + 4 * g + v - u0];
           from = vbase + at.v;
-          if constexpr (KT == SAH_E4M3) v_scale[a] |= (uint32_t)v_scales[at.scale] << (8 * v);
+          if constexpr (KT == SAH_E4M3) x.scale[a] |= (uint32_t)v_scales[at.scale] << (8 * v);
         }
 #pragma unroll
         for (int s = 0; s < H; ++s) {
-          uint32_t* to = vr[s][4 * a + v];
+          uint32_t* to = x.r[s][4 * a + v];
           typedef uint32_t words __attribute__((ext_vector_type(VW)));
           const words w = SMALL ? *(const words*)(from + v_in[s][v]) : pt_load<words>(from, v_in[s][v]);
 #pragma unroll
@@ -517,16 +576,16 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
     }
   };
 
-  auto step = [&](int u, auto k_read, auto v_read) __attribute__((always_inline)) {
+  auto step = [&](int u, int next, keys_of& kx, values_of& vx) __attribute__((always_inline)) {
     sah_f32x4 s[NA];
 #pragma unroll
     for (int a = 0; a < NA; ++a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[a][e] = 0.f;
-      const float scale = KT == SAH_E4M3 ? pg_scale_of(k_scale[a], i16 & 3) : 1.f;
+      const float scale = KT == SAH_E4M3 ? pg_scale_of(kx.scale[a], i16 & 3) : 1.f;
 #pragma unroll
       for (int c = 0; c < KL; ++c) {
-        const sah_u4 k = kr[a][c];
+        const sah_u4 k = kx.r[a][c];
         if constexpr (KT == SAH_F32) {
           s[a] = pt_mfma_f32(sah_bits_to_float(k.x), sah_bits_to_float(qf[0][c].x), s[a]);
           s[a] = pt_mfma_f32(sah_bits_to_float(k.y), sah_bits_to_float(qf[0][c].y), s[a]);
@@ -545,7 +604,7 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
         }
       }
     }
-    k_read();
+    fetch_k(next, kx);
     // keys that not every row sees; values of keys that no row sees are made 0
     int first[NA] = {};
     bool plain = !SMALL;   // uniform
@@ -567,7 +626,7 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
 #pragma unroll
           for (int c = 0; c < H; ++c)
 #pragma unroll
-            for (int w = 0; w < VW; ++w) vr[c][4 * a + e][w] = some ? vr[c][4 * a + e][w] : 0u;
+            for (int w = 0; w < VW; ++w) vx.r[c][4 * a + e][w] = some ? vx.r[c][4 * a + e][w] : 0u;
         }
     }
     float mx = s[0][0];
@@ -605,7 +664,7 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
 #pragma unroll
           for (int c = 0; c < H; ++c)
 #pragma unroll
-            for (int w = 0; w < NC; ++w) acc[c * NC + w] = pt_mfma_f32(sah_bits_to_float(vr[c][4 * a + e][w]), s[a][e], acc[c * NC + w]);
+            for (int w = 0; w < NC; ++w) acc[c * NC + w] = pt_mfma_f32(sah_bits_to_float(vx.r[c][4 * a + e][w]), s[a][e], acc[c * NC + w]);
     } else {
       uint32_t term[T::NP][4];
       float rest[8];
@@ -623,10 +682,10 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             if constexpr (KT == SAH_E4M3) {
-              const float scale = pg_scale_of(v_scale[k / 4], k % 4);
-              two[k] = pair % 2 ? pg_widen2<true>(vr[c][k][pair / 2], scale) : pg_widen2<false>(vr[c][k][pair / 2], scale);
+              const float scale = pg_scale_of(vx.scale[k / 4], k % 4);
+              two[k] = pair % 2 ? pg_widen2<true>(vx.r[c][k][pair / 2], scale) : pg_widen2<false>(vx.r[c][k][pair / 2], scale);
             } else {
-              two[k] = vr[c][k][pair];
+              two[k] = vx.r[c][k][pair];
             }
           }
           const uint4 lo = make_uint4(pt_low(two[0], two[1]), pt_low(two[2], two[3]), pt_low(two[4], two[5]), pt_low(two[6], two[7]));
@@ -639,47 +698,28 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
           }
         }
     }
-    v_read();
+    fetch_v(next, vx);
   };
   for (; u0 < u_end; u0 += MOST) {  // (uniform; the next one's first key fits 32 bits: the host has checked what a request can have)
     const int u1 = u_end - u0 < MOST ? u_end : u0 + MOST;
-    __syncthreads();                // the places before have been read, and the sums of the tile before
-    constexpr int EACH = SMALL ? 1 : 16;
-    const int n_slots = (u1 - u0 + STEP - 1) / STEP * (STEP / EACH);
-    const int32_t* list = P.pages ? P.pages + ((int64_t)t0 * C.Hkv + hk) * P.n_select : nullptr;
-    for (int s = threadIdx.x; s < n_slots; s += PT_NT) {
-      const int u = u0 + s * EACH, e = u >> shift;
-      int64_t in = u & (C.page_size - 1);
-      int lg = e;
-      if (list) lg = e < P.n_select ? list[e] : -1;
-      else if (keys.skip && u >= keys.sinks) lg = e + (keys.skip >> shift);
-      int64_t page = -1;
-      if (lg >= 0 && lg < P.requests.table_width && lg <= keys.hi >> shift) page = P.requests.block_table[(int64_t)req.b * P.requests.table_pitch + lg];
-      pt_where at;
-      // a page that is not there: another one's keys, behind every position (table_width pages end before that)
-      at.first = (int)(0x80000000u - (uint32_t)C.page_size + (uint32_t)in);
-      if (page >= 0 && page < C.n_pages) at.first = (lg << shift) + (int)in;
-      else page = in = 0;
-      at.k = (page * C.ks_p + in * C.ks_t) * ES;
-      at.v = (page * C.vs_p + in * C.vs_t) * ES;
-      at.scale = (page * C.Hkv + hk) * C.page_size + in;
-      s_at[s] = at;
+    if (u0 != u_first) {
+      __syncthreads();  // the places before have been read
+      look_up(u0);
+      __syncthreads();
     }
-    __syncthreads();
-    int u = u0 + STEP * wave;
+    const int round = STEP * turns;
+    int u = u0 + STEP * turn;
     if (u >= u1) continue;
-    fetch_k(u);
-    fetch_v(u);
-    // (the last step apart: a way through the loop that skips a request would have the compiler wait for all of them)
-#pragma unroll 1
-    for (; u + ROUND < u1; u += ROUND)
-      step(u, [&]() __attribute__((always_inline)) { fetch_k(u + ROUND); }, [&]() __attribute__((always_inline)) { fetch_v(u + ROUND); });
-    step(u, [] {}, [] {});
+    // Behind a wave's last step it is requested again, from the caches: a way through the loop that skips a request would have the compiler wait
+    // for all of them.
+    const int end = u + (u1 - 1 - u) / round * round;
+    fetch_k(u, kb);
+    fetch_v(u, vb);
+    for (; u < u1; u += round) step(u, u < end ? u + round : end, kb, vb);
   }
 
   // the four waves' sums, row by row in LDS
   l_run = pt_quad_sum(l_run);
-  if (u_first >= u_end) __syncthreads();  // those of the tile before have been read (else the wait above)
   if (live) {
     if (g == 0) {
       s_ml[wave][0][i16] = m_run;
@@ -695,14 +735,12 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
               make_float4(acc[c * NC + e][v], acc[c * NC + e + 1][v], acc[c * NC + e + 2][v], acc[c * NC + e + 3][v]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * (DP / 4); i += PT_NT) {
-    const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
+  for (int i = threadIdx.x; i < A.heads * rows * (DP / 4); i += PT_NT) {
+    const int of = i / (DP / 4), d = 4 * (i % (DP / 4)), hh = of / rows, r = of - hh * rows;
     float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < PT_NW; ++w) m = fmaxf(m, s_ml[w][0][r]);
+    for (int w = hh; w < PT_NW; w += A.heads) m = fmaxf(m, s_ml[w][0][r]);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < PT_NW; ++w) {
+    for (int w = hh; w < PT_NW; w += A.heads) {
       const float mw = s_ml[w][0][r], lw = s_ml[w][1][r], up = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - m) * c_exp);
       l += lw == lw ? lw * up : lw;  // (a wave whose sum is NaN has no maximum, perhaps)
       const float4 a = *(const float4*)&s_acc[w][r][d];
@@ -711,9 +749,9 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
       o.z += a.z * up;
       o.w += a.w * up;
     }
-    const int rt = t0 + (A.blocks > 1 ? 0 : r / G), rh = hk * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G);
+    const int rt = t0 + (A.blocks > 1 ? 0 : r / G), rh = (hk0 + hh) * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G);
     if (!whole) {  // a part: to slot 0 where the tile began before this workgroup's piece, else to slot 1
-      float* to = (float*)P.work + (((int64_t)w * 2 + (y0 ? 0 : 1)) * PT_ROWS + r) * (DP + 4);
+      float* to = (float*)P.work + ((((int64_t)w * 2 + (y0 ? 0 : 1)) * A.heads + hh) * PT_ROWS + r) * (DP + 4);
       if (d == 0) *(float2*)to = make_float2(m, l);
       *(float4*)(to + 4 + d) = o;
       continue;
@@ -724,19 +762,19 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
     o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
     if (d >= C.D) continue;
     fine = fine && pt_fine<QT>(o.x) && pt_fine<QT>(o.y) && pt_fine<QT>(o.z) && pt_fine<QT>(o.w);
-    if (!fine) atomicOr(&s_bad, 1u << r);
+    if (!fine) atomicOr(&s_bad, 1ull << (hh * PT_ROWS + r));
     char* to = (char*)P.out + ((int64_t)rt * P.os_t + (int64_t)rh * P.os_h + d) * pg_size(QT);
     if (QT == SAH_F32) *(float4*)to = o;
     else *(uint2*)to = make_uint2(sah_pack2_hw<QT>(o.x, o.y), sah_pack2_hw<QT>(o.z, o.w));
   }
   if (whole) {
     __syncthreads();
-    uint32_t bad = s_bad;  // rows that are not finite are done again, each by a wave
+    unsigned long long bad = s_bad;  // rows that are not finite are done again, each by a wave
     for (int i = 0; bad; ++i) {
-      const int r = __builtin_ctz(bad);
+      const int hh = __builtin_ctzll(bad) / PT_ROWS, r = __builtin_ctzll(bad) % PT_ROWS;
       bad &= bad - 1;
       if (i % PT_NW != wave) continue;
-      pt_row_again<KT, QT>(A, req, t0 + (A.blocks > 1 ? 0 : r / G), hk * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G));
+      pt_row_again<KT, QT>(A, req, t0 + (A.blocks > 1 ? 0 : r / G), (hk0 + hh) * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G));
     }
     if (at.begin + y1 < at.x1) __syncthreads();  // (s_bad has been read)
   }
@@ -758,33 +796,46 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A, int wgs) {
   __shared__ float2 s_ml[GROUPS];
   const int lane = threadIdx.x & (SAH_WAVE - 1), l = threadIdx.x % L, group = threadIdx.x / L;
   const int per_token = C.Hkv * A.blocks, t = (int)(blockIdx.x / per_token), in = (int)blockIdx.x - t * per_token, hk = in % C.Hkv, block = in / C.Hkv;
-  const pg_request req = pg_find_by_wave(P.requests, C.page_size, t);
-  if (req.b < 0) return;
+  // the token's request, and where its tiles begin on the line
+  int b_of = -1;
+  pt_lens lens{0, 0, 0};
+  int64_t before = 0, total = 0;
+  for (int b0 = 0; b0 < P.requests.n_requests; b0 += SAH_WAVE) {
+    const int b = b0 + lane;
+    pt_lens l{0, 0, 0};
+    if (b < P.requests.n_requests) l = pt_lens_of(P.requests, b);
+    const int64_t c = pt_cost_of(A, l).all();
+    const uint64_t has = __ballot(l.begin >= 0 && t >= l.begin && t < l.end);
+    total += c;
+    if (b_of < 0) {
+      const int at = has ? __builtin_ctzll(has) : SAH_WAVE;
+      before += lane < at ? c : 0;
+      if (has) {
+        b_of = b0 + at;
+        lens = pt_lens{__builtin_amdgcn_readlane(l.begin, at), __builtin_amdgcn_readlane(l.end, at), __builtin_amdgcn_readlane(l.kv, at)};
+      }
+    }
+  }
+  if (b_of < 0) return;
+  const pg_request req = pg_make(P.requests, C.page_size, b_of, lens.begin, lens.end, lens.kv);
   const int i = t - req.begin;
   if (i % A.tokens) return;  // not the first of its tile
   const int G = P.Hq / C.Hkv, n_tok = A.tokens < req.n_new - i ? A.tokens : req.n_new - i;
   const int all_rows = A.blocks > 1 ? (G - block * PT_ROWS < PT_ROWS ? G - block * PT_ROWS : PT_ROWS) : n_tok * G;
   const int rows = (all_rows - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;  // this workgroup's
   if (rows <= 0) return;
-  // the tile on the line
-  int64_t before = 0, total = 0;
-  for (int b0 = 0; b0 < P.requests.n_requests; b0 += SAH_WAVE) {
-    const int b = b0 + lane;
-    const int64_t c = b < P.requests.n_requests ? pt_cost_of(A, pt_lens_of(P.requests, b)).all() : 0;
-    total += c;
-    before += b < req.b ? c : 0;
-  }
   total = (int64_t)sah_lane_u64(sah_wave_incl_scan_u64((uint64_t)total), SAH_WAVE - 1);
   before = (int64_t)sah_lane_u64(sah_wave_incl_scan_u64((uint64_t)before), SAH_WAVE - 1);
-  const pt_cost cost = pt_cost_of(A, pt_lens_of(P.requests, req.b));
-  const int64_t begin = before + (((int64_t)(i / A.tokens) * A.blocks + block) * C.Hkv + hk) * cost.each, end = begin + cost.each;
+  const pt_cost cost = pt_cost_of(A, lens);
+  const int64_t begin = before + (((int64_t)(i / A.tokens) * A.blocks + block) * (C.Hkv / A.heads) + hk / A.heads) * cost.each, end = begin + cost.each;
   // the workgroups whose pieces hold its first and its last key
-  const int sharers = pt_sharers(total, wgs);
+  const pt_shares shares = pt_share(A, total, wgs);
+  const int sharers = (int)shares.n;
   auto holder = [&](int64_t x) {
-    int w = __builtin_amdgcn_readfirstlane((int)((double)x / (double)total * sharers));
+    int w = __builtin_amdgcn_readfirstlane((int)((float)x / (float)total * sharers));
     w = w < sharers ? w : sharers - 1;
-    while (w + 1 < sharers && pt_bound(total, sharers, w + 1) <= x) ++w;
-    while (w > 0 && pt_bound(total, sharers, w) > x) --w;
+    while (w + 1 < sharers && shares.bound(w + 1) <= x) ++w;
+    while (w > 0 && shares.bound(w) > x) --w;
     return w;
   };
   const int w0 = holder(begin), w1 = holder(end - 1);
@@ -793,7 +844,7 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A, int wgs) {
   int shared_by = 1;     // groups that share a row
   while (2 * shared_by * rows <= GROUPS) shared_by *= 2;
   const float c_exp = pt_log2(P.scaling);
-  const float* from = (const float*)P.work + (int64_t)w0 * 2 * PT_ROWS * (DP + 4);
+  const float* from = (const float*)P.work + ((int64_t)w0 * 2 * A.heads + hk % A.heads) * PT_ROWS * (DP + 4);
   float m, sum;
   float4 o;
   auto add = [&](float2 ml, const float4& v) __attribute__((always_inline)) {
@@ -820,7 +871,7 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A, int wgs) {
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int of = p0 + i * shared_by < parts ? p0 + i * shared_by : parts - 1;
-        const float* part = from + ((int64_t)(of ? 2 * of : 1) * PT_ROWS + r) * (DP + 4);
+        const float* part = from + ((int64_t)(of ? 2 * of : 1) * A.heads * PT_ROWS + r) * (DP + 4);
         ml[i] = *(const float2*)part;
         v[i] = *(const float4*)(part + 4 + 4 * l);
       }
@@ -870,6 +921,7 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
   A.tokens = a->pages || G >= PT_ROWS ? 1 : PT_ROWS / G;
   A.blocks = (G + PT_ROWS - 1) / PT_ROWS;
   A.unit = a->cache.page_size > PT_STEP ? a->cache.page_size : PT_STEP;
+  A.heads = a->pages || a->cache.Hkv % 2 ? 1 : a->cache.Hkv % 4 ? 2 : 4;
   // About as many workgroups as the call has work for, at most what the card holds at once. Only how the work is shared depends on it.
   const int64_t table = (int64_t)a->requests.table_width * a->cache.page_size;
   int64_t keys = table;
@@ -931,8 +983,8 @@ extern "C" int64_t sah_page_attention_work_bytes(const sah_page_attention_args* 
     return copy + 4 * sah_paged_attention_work_floats(&p);
   }
   int wgs;
-  (void)pt_plan(a, wgs);
-  return (int64_t)wgs * 2 * PT_ROWS * (pt_dim(a) + 4) * 4;
+  const pt_args A = pt_plan(a, wgs);
+  return (int64_t)wgs * 2 * A.heads * PT_ROWS * (pt_dim(a) + 4) * 4;
 }
 
 template <int KT, int QT, int DP>

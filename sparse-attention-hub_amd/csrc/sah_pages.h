@@ -63,11 +63,6 @@ __device__ __forceinline__ pg_request pg_make(const sah_page_requests& R, int pa
   r.base = (int64_t)kv - end;
   return r;
 }
-__device__ __forceinline__ pg_request pg_read(const sah_page_requests& R, int page_size, int b, int t) {
-  const int begin = R.cu_new[b], end = R.cu_new[b + 1], kv = R.kv_lens[b];
-  if (begin < 0 || t < begin || t >= end) return pg_none();  // (running sums that fall: nobody's)
-  return pg_make(R, page_size, b, begin, end, kv);
-}
 // What all lanes of the wave hold, in scalar registers (doubles are divided in vector ones)
 __device__ __forceinline__ int64_t pg_uniform(int64_t v) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
@@ -82,29 +77,26 @@ __device__ __forceinline__ int64_t pg_div(int64_t a, int64_t b) {
   return q;
 }
 
-// By a whole wave, for a row that all of its lanes ask for: 64 ends are looked at in one trip to memory.
+// By a whole wave, for a row that all of its lanes ask for: 64 requests are looked at in one trip to memory.
 __device__ __forceinline__ pg_request pg_find_by_wave(const sah_page_requests& R, int page_size, int t) {
   const int lane = threadIdx.x & (SAH_WAVE - 1);
-  int lo = 0, n = R.n_requests, step;
-  do {
-    step = (n + SAH_WAVE - 1) / SAH_WAVE;
+  int lo = 0, n = R.n_requests;
+  while (n > SAH_WAVE) {
+    const int step = (n + SAH_WAVE - 1) / SAH_WAVE;
     const int64_t i = (int64_t)(lane + 1) * step - 1;
     const uint64_t behind = __ballot(R.cu_new[lo + (i < n ? (int)i : n - 1) + 1] > t);
     if (!behind) return pg_none();
     const int from = __builtin_ctzll(behind) * step;  // (at most n - 1: lanes beyond it ask what the last one before asks)
     lo += from;
     n = n - from < step ? n - from : step;
-  } while (step > 1);
-  return pg_read(R, page_size, __builtin_amdgcn_readfirstlane(lo), t);
-}
-// By a lane of its own, for its row
-__device__ __forceinline__ pg_request pg_find(const sah_page_requests& R, int page_size, int t) {
-  int lo = 0, hi = R.n_requests;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (R.cu_new[mid + 1] > t) hi = mid; else lo = mid + 1;
   }
-  return lo < R.n_requests ? pg_read(R, page_size, lo, t) : pg_none();
+  const int b = lo + (lane < n ? lane : n - 1);
+  const int begin = R.cu_new[b], end = R.cu_new[b + 1], kv = R.kv_lens[b];
+  const uint64_t has = __ballot(begin >= 0 && begin <= t && t < end);  // (running sums that fall: the first one's)
+  if (!has) return pg_none();
+  const int at = __builtin_ctzll(has);
+  return pg_make(R, page_size, __builtin_amdgcn_readlane(b, at), __builtin_amdgcn_readlane(begin, at), __builtin_amdgcn_readlane(end, at),
+                 __builtin_amdgcn_readlane(kv, at));
 }
 
 // ---------------------------------------------------------------------------

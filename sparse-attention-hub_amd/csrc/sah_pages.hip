@@ -217,7 +217,8 @@ __global__ __launch_bounds__(PG_NT) void k_page_bounds(sah_page_bounds_args P, i
 // ---------------------------------------------------------------------------
 #define PG_ALWAYS ~0ull        // pages that are taken whatever they score
 #define PG_FIRST (~0ull - 1)   // scores that are not finite
-#define PG_WAVE_PAGES 32       // pages that a wave scores
+#define PG_WAVE_PAGES 32       // pages that a wave scores at once
+#define PG_SCORE_WGS 1024      // workgroups of a call, about: what the card holds at once
 
 __device__ __forceinline__ uint64_t pg_key(double score) {  // never 0
   if (!(score - score == 0.0)) return PG_FIRST;
@@ -227,6 +228,25 @@ __device__ __forceinline__ uint64_t pg_key(double score) {  // never 0
 template <int CTRL>
 __device__ __forceinline__ double pg_dpp(double v) {
   return __builtin_bit_cast(double, sah_dpp_u64<CTRL, 0xF, true>(__builtin_bit_cast(uint64_t, v)));
+}
+
+// N elements (8; of fp32 also 4, of 16-bit types 4 at 8-byte addresses)
+template <int T, int N>
+__device__ __forceinline__ void pg_load_some(const void* p, int64_t i, float (&o)[8]) {
+  if constexpr (N == 8) {
+    sah_load8<T>(p, i, o);
+  } else if constexpr (T == SAH_F32) {
+    const float4 f = *(const float4*)((const float*)p + i);
+    o[0] = f.x; o[1] = f.y; o[2] = f.z; o[3] = f.w;
+  } else {
+    const uint2 u = *(const uint2*)((const uint16_t*)p + i);
+    const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      o[2 * k] = T == SAH_BF16 ? sah_bits_to_float(w[k] << 16) : sah_f16_to_float((uint16_t)w[k]);
+      o[2 * k + 1] = T == SAH_BF16 ? sah_bits_to_float(w[k] & 0xffff0000u) : sah_f16_to_float((uint16_t)(w[k] >> 16));
+    }
+  }
 }
 
 struct pg_select {
@@ -256,21 +276,29 @@ __global__ __launch_bounds__(PG_NT) void k_page_scores(pg_select S) {
   if (p < 0) return;
   const int shift = 31 - __builtin_clz(P.page_size), n = (int)(p >> shift) + 1;
   if ((chunk * NW + wave) * PG_WAVE_PAGES >= n) return;
-  // the group's queries, the positive and the negative ones of a channel added up (G numbers of 24 bits: exact for what is not wide apart)
+  // the group's queries, the positive and the negative ones of a channel added up (numbers of at most 24 bits: exact for what is not wide apart)
   const int G = P.Hq / P.Hkv;
   double up[E], down[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) up[e] = down[e] = 0.0;
   if (in * E < P.D) {
-    for (int i = 0; i < G; ++i) {
-      const int64_t at = t * P.qs_t + (int64_t)(h * G + i) * P.qs_h + in * E;
+    const int64_t first = t * P.qs_t + (int64_t)h * G * P.qs_h + in * E;
+    auto add = [&](auto type) __attribute__((always_inline)) {
+      constexpr int QT = decltype(type)::value;
+#pragma unroll 4
+      for (int i = 0; i < G; ++i) {
+        float q[8];
+        pg_load_some<QT, E>(P.q, first + i * P.qs_h, q);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const double q = P.dtype == SAH_F32 ? sah_load<SAH_F32>(P.q, at + e) : P.dtype == SAH_BF16 ? sah_load<SAH_BF16>(P.q, at + e) : sah_load<SAH_F16>(P.q, at + e);
-        if (q < 0.0) down[e] += q;
-        else up[e] += q;  // (NaN too)
+        for (int e = 0; e < E; ++e) {
+          up[e] += q[e] < 0.f ? 0.0 : (double)q[e];  // (NaN too)
+          down[e] += q[e] < 0.f ? (double)q[e] : 0.0;
+        }
       }
-    }
+    };
+    if (P.dtype == SAH_F32) add(std::integral_constant<int, SAH_F32>());
+    else if (P.dtype == SAH_BF16) add(std::integral_constant<int, SAH_BF16>());
+    else add(std::integral_constant<int, SAH_F16>());
   }
   uint64_t* keys = (uint64_t*)P.work + row * S.pitch;
   const char* base = (const char*)P.bounds + (int64_t)h * 2 * P.D * ES;
@@ -334,15 +362,47 @@ __global__ __launch_bounds__(PG_NT) void k_page_scores(pg_select S) {
   }
 }
 
-// One workgroup a row: the n_select-th largest key by digits of 8 bits, from the highest bit on in which the row's keys differ, in LDS
-// histograms; then the places of what is taken, in the order of the table. A thread has neighbouring pages.
+// Sum of one number per thread before it, across the workgroup, and of all; `wsum`: PG_NT / 64 words that no other call uses.
+__device__ __forceinline__ int pg_before(int v, int* wsum, int& all) {
+  constexpr int NW = PG_NT / SAH_WAVE;
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
+  const int incl = sah_wave_incl_scan(v);
+  if (lane == SAH_WAVE - 1) wsum[wave] = incl;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    before += i < wave ? wsum[i] : 0;
+    all += wsum[i];
+  }
+  return before + incl - v;
+}
+// bits that any of the wave's lanes has set (in its last lane)
+__device__ __forceinline__ uint32_t pg_any_bits(uint32_t v) {
+  int x = (int)v;
+  x |= sah_dpp_i<0x111, 0xF, true>(x);
+  x |= sah_dpp_i<0x112, 0xF, true>(x);
+  x |= sah_dpp_i<0x114, 0xF, true>(x);
+  x |= sah_dpp_i<0x118, 0xF, true>(x);
+  x |= sah_dpp_i<0x142, 0xA, false>(x);
+  x |= sah_dpp_i<0x143, 0xC, false>(x);
+  return (uint32_t)x;
+}
+
+// One workgroup a row: the digit of 8 bits at which the count of the larger keys passes n_select, from the highest bit on in which the row's keys
+// differ, in an LDS histogram; again inside that digit, unless its keys fit a list of one wave, which ranks them against each other.
+// Then the places of what is taken, in the order of the table. A thread has neighbouring pages.
+#define PG_DIGIT 8
+#define PG_LIST SAH_WAVE
 __global__ __launch_bounds__(PG_NT) void k_page_top(pg_select S) {
   sah_touch_kernargs<sizeof(pg_select)>();
   const sah_page_select_args& P = S.a;
-  constexpr int NW = PG_NT / SAH_WAVE, KEEP = 8;
-  __shared__ int s_hist[256], s_scan[NW + 1];
-  __shared__ uint64_t s_min[NW], s_max[NW];
-  __shared__ int s_bin, s_above, s_count;
+  constexpr int NW = PG_NT / SAH_WAVE, KEEP = 8, BINS = 1 << PG_DIGIT, MINE = BINS / PG_NT;
+  __shared__ int s_hist[BINS];
+  __shared__ int s_sum[5][NW];
+  __shared__ uint64_t s_ones[NW], s_zeros[NW], s_key[PG_LIST], s_border;
+  __shared__ int s_at[PG_LIST], s_border_at, s_listed, s_bin, s_above, s_count;
   const int64_t row = blockIdx.x, t = row / P.Hkv;
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
   const pg_request r = pg_find_by_wave(P.requests, P.page_size, (int)t);
@@ -352,7 +412,7 @@ __global__ __launch_bounds__(PG_NT) void k_page_top(pg_select S) {
   int32_t* out = P.pages + row * P.n_select;
   const uint64_t* keys = (const uint64_t*)P.work + row * S.pitch;
   const int each = (n + PG_NT - 1) / PG_NT, first = (int)threadIdx.x * each;
-  const bool kept = each <= KEEP;  // in registers, else read again in every pass
+  const bool kept = each <= KEEP;  // in registers, else read again whenever they are looked at
   uint64_t mine[KEEP];
 #pragma unroll
   for (int i = 0; i < KEEP; ++i) mine[i] = kept && i < each && first + i < n ? keys[first + i] : 0;
@@ -365,96 +425,133 @@ __global__ __launch_bounds__(PG_NT) void k_page_top(pg_select S) {
       for (int i = 0; i < each; ++i) f(first + i, first + i < n ? keys[first + i] : 0);
     }
   };
-  // candidates, the smallest and the largest key of them
-  uint64_t least = ~0ull, most = 0;
-  int count = 0;
-  visit([&](int, uint64_t key) {
-    if (!key) return;
-    ++count;
-    least = key < least ? key : least;
-    most = key > most ? key : most;
-  });
+  auto clear = [&]() {
 #pragma unroll
-  for (int m = 1; m < SAH_WAVE; m *= 2) {
-    const uint64_t a = __shfl_xor(least, m), b = __shfl_xor(most, m);
-    least = a < least ? a : least;
-    most = b > most ? b : most;
+    for (int i = 0; i < MINE; ++i) s_hist[(int)threadIdx.x + i * PG_NT] = 0;
+    if (threadIdx.x == 0) s_listed = 0;
+  };
+  clear();
+  // Those that are ranked (not the ones that are taken anyway: their key would hide where the others' differ), and which bits are set, and which
+  // are not, in any of them
+  auto ranks = [](uint64_t key) { return (key != 0) & (key != PG_ALWAYS); };
+  uint64_t ones = 0, zeros = 0;
+  int count = 0, fixed = 0;
+  visit([&](int, uint64_t key) {
+    const bool in = ranks(key);
+    count += in;
+    fixed += key == PG_ALWAYS;
+    ones |= in ? key : 0;
+    zeros |= in ? ~key : 0;
+  });
+  const uint32_t o0 = pg_any_bits((uint32_t)ones), o1 = pg_any_bits((uint32_t)(ones >> 32));
+  const uint32_t z0 = pg_any_bits((uint32_t)zeros), z1 = pg_any_bits((uint32_t)(zeros >> 32));
+  if (lane == SAH_WAVE - 1) {
+    s_ones[wave] = (uint64_t)o1 << 32 | o0;
+    s_zeros[wave] = (uint64_t)z1 << 32 | z0;
   }
-  if (lane == 0) {
-    s_min[wave] = least;
-    s_max[wave] = most;
-  }
-  int total;
-  (void)sah_block_excl_scan<PG_NT>(count, s_scan, &total);
+  int total, always;
+  (void)pg_before(fixed, s_sum[2], always);
+  (void)pg_before(count, s_sum[0], total);
+  ones = zeros = 0;
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
-    least = s_min[i] < least ? s_min[i] : least;
-    most = s_max[i] > most ? s_max[i] : most;
+    ones |= s_ones[i];
+    zeros |= s_zeros[i];
   }
-  uint64_t border = 1;         // keys above it are taken, and the first `ties` that are equal
-  int ties = total;
-  if (total > P.n_select) {
-    int want = P.n_select;
-    const uint64_t differ = least ^ most;
-    int low = differ ? 64 - __builtin_clzll(differ) : 0;  // bits below it are still to be looked at
-    uint64_t prefix = low < 64 ? most >> low : 0;
-    border = most;
-    ties = want;
-    while (low > 0) {  // (at most 8 times)
-      const int width = low < 8 ? low : 8, next = low - width;
-      for (int i = threadIdx.x; i < 256; i += PG_NT) s_hist[i] = 0;
-      __syncthreads();
+  // Taken: keys whose bits from `low` on are more than `prefix`, and `want` of the `inside` ones for which they are just that.
+  int low = 64, want = total, inside = total;  // (no bits: all)
+  uint64_t prefix = 0;
+  auto upper = [&](uint64_t key) { return low < 64 ? key >> low : 0; };
+  if (total > P.n_select - always) {
+    const uint64_t differ = ones & zeros;
+    low = differ ? 64 - __builtin_clzll(differ) : 0;
+    prefix = upper(ones);
+    want = P.n_select - always;
+    int round = 0;
+    while (low > 0 && inside > PG_LIST && inside > want && want) {  // (at most 8 times)
+      const int width = low < PG_DIGIT ? low : PG_DIGIT, next = low - width;
       visit([&](int, uint64_t key) {
-        if (key && (low < 64 ? key >> low : 0) == prefix) atomicAdd(&s_hist[(key >> next) & ((1u << width) - 1)], 1);
+        if (ranks(key) && upper(key) == prefix) atomicAdd(&s_hist[(key >> next) & ((1u << width) - 1)], 1);
       });
       __syncthreads();
-      if (wave == 0) {  // the digit at which the count, from the largest down, reaches `want`: four digits a lane, the largest in lane 0
-        int c[4], sum = 0;
+      // a thread's neighbouring digits, the largest in thread 0
+      int c[MINE], sum = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += c[i] = s_hist[255 - 4 * lane - i];
-        int above = sah_wave_incl_scan(sum) - sum;
-        if (above < want && want <= above + sum) {
+      for (int i = 0; i < MINE; ++i) sum += c[i] = s_hist[BINS - 1 - MINE * (int)threadIdx.x - i];
+      int all;
+      int above = pg_before(sum, s_sum[1 + (round++ & 1)], all);  // (those of the round before may still be read)
+      if (above < want && want <= above + sum) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (above < want && want <= above + c[i]) {
-              s_bin = 255 - 4 * lane - i;
-              s_above = above;
-              s_count = c[i];
-            }
-            above += c[i];
+        for (int i = 0; i < MINE; ++i) {
+          if (above < want && want <= above + c[i]) {
+            s_bin = BINS - 1 - MINE * (int)threadIdx.x - i;
+            s_above = above;
+            s_count = c[i];
           }
+          above += c[i];
         }
       }
+      clear();          // (all have read their digits: the wait above)
       __syncthreads();
       want -= s_above;
+      inside = s_count;
       prefix = (low < 64 ? prefix << width : 0) | (uint64_t)s_bin;
       low = next;
-      border = prefix << low;
-      ties = want;
-      if (s_count == want) {  // all of the digit's keys: what is at least its first number
-        ties = total;
-        break;
-      }
-      // (the next write of s_bin and s_count lies behind two waits)
     }
   }
-  // keys above the border, and equal ones while they last; a digit that is taken whole begins at the border
-  int above = 0, equal = 0;
-  visit([&](int, uint64_t key) {
-    above += key > border;
-    equal += key == border;
-  });
-  int all_above, all_equal;
-  int before = sah_block_excl_scan<PG_NT>(above, s_scan, &all_above);
-  int ranked = sah_block_excl_scan<PG_NT>(equal, s_scan, &all_equal);
-  const int taken_equal = all_equal < ties ? all_equal : ties;
-  visit([&](int j, uint64_t key) {
-    const bool eq = key == border, take = key > border || (eq && ranked < ties);
-    if (take) out[before + (ranked < ties ? ranked : ties)] = j;
-    before += key > border;
-    ranked += eq;
-  });
-  for (int i = all_above + taken_equal + (int)threadIdx.x; i < P.n_select; i += PG_NT) out[i] = -1;
+  // the last one taken, by key and, of equal keys, place
+  uint64_t border = low < 64 ? (prefix << low) - 1 : 0;  // (all of the inside ones: what lies above their smallest number less one)
+  int border_at = -1;
+  if (want == 0) border = PG_ALWAYS - 1;
+  else if (want < inside && low > 0) {  // uniform: a list of at most PG_LIST
+    visit([&](int j, uint64_t key) {
+      if (!ranks(key) || upper(key) != prefix) return;
+      const int i = atomicAdd(&s_listed, 1);
+      s_key[i] = key;
+      s_at[i] = j;
+    });
+    __syncthreads();
+    if (wave == 0) {
+      const uint64_t key = s_key[lane];  // (lanes beyond the list hold nobody's)
+      const int at = s_at[lane];
+      int ahead = 0;
+#pragma unroll 4
+      for (int i = 0; i < inside; ++i) ahead += (s_key[i] > key) | ((s_key[i] == key) & (s_at[i] < at));
+      if (lane < inside && ahead == want - 1) {
+        s_border = key;
+        s_border_at = at;
+      }
+    }
+    __syncthreads();
+    border = s_border;
+    border_at = s_border_at;
+  }
+  int all, taken;
+  if (low == 0 && want && want < inside) {  // equal keys, more than the list holds: the first `want` of them
+    int n_larger = 0, n_equal = 0;
+    visit([&](int, uint64_t key) {
+      n_larger += key > prefix;
+      n_equal += key == prefix;
+    });
+    int larger = pg_before(n_larger, s_sum[3], all);
+    taken = all + want;
+    int ranked = pg_before(n_equal, s_sum[4], all);
+    visit([&](int j, uint64_t key) {
+      if (key < prefix) return;
+      if (key > prefix || ranked < want) out[larger + (ranked < want ? ranked : want)] = j;
+      larger += key > prefix;
+      ranked += key == prefix;
+    });
+  } else {
+    auto take = [&](int j, uint64_t key) { return (key > border) | ((key == border) & (j <= border_at)); };
+    int n_taken = 0;
+    visit([&](int j, uint64_t key) { n_taken += take(j, key); });
+    int at = pg_before(n_taken, s_sum[3], taken);
+    visit([&](int j, uint64_t key) {
+      if (take(j, key)) out[at++] = j;
+    });
+  }
+  for (int i = taken + (int)threadIdx.x; i < P.n_select; i += PG_NT) out[i] = -1;
 }
 
 // ---------------------------------------------------------------------------
@@ -571,15 +668,19 @@ extern "C" int sah_page_select(const sah_page_select_args* given) {
   if (int rc = pg_check_requests(a->requests, a->page_size, true, "sah_page_select")) return rc;
   if (a->requests.n_tokens == 0) return SAH_OK;
   if (!a->q || !a->bounds || !a->pages) return sah_fail(SAH_ENULL, "sah_page_select: NULL pointer");
-  if ((uint64_t)a->bounds % 16) return sah_fail(SAH_EINVAL, "sah_page_select: bounds must be 16-byte aligned");
   if (!a->work || a->work_bytes < sah_page_select_work_bytes(a) || (uint64_t)a->work % 16) return sah_fail(SAH_ECAPACITY, "sah_page_select: work is too small");
   if (a->requests.n_tokens == 1) a->qs_t = 0;
   if (a->Hq == 1) a->qs_h = 0;
+  if (((uint64_t)a->q | (uint64_t)a->bounds | (uint64_t)(pg_size(a->dtype) * (a->qs_t | a->qs_h))) % 16)
+    return sah_fail(SAH_EINVAL, "sah_page_select: addresses and strides must be multiples of 16 bytes");
   const int64_t rows = (int64_t)a->requests.n_tokens * a->Hkv;
   const int per = PG_WAVE_PAGES * (PG_NT / SAH_WAVE), width = a->requests.table_width;
   const int64_t hint = ((int64_t)a->max_context + a->page_size - 1) / a->page_size;
   const int usual = hint > 0 && hint < width ? (int)hint : width;  // pages of the longest request, by what the caller says
-  const pg_select s{*a, width, (usual + per - 1) / per};
+  int64_t chunks = (usual + per - 1) / per;
+  const int64_t room = PG_SCORE_WGS / rows > 1 ? PG_SCORE_WGS / rows : 1;
+  if (chunks > room) chunks = room;
+  const pg_select s{*a, width, (int)chunks};
   if (rows * s.chunks > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_select: too many rows");
   hipStream_t st = (hipStream_t)a->stream;
   const dim3 grid((unsigned)(rows * s.chunks));

@@ -115,7 +115,7 @@ def test_bounds_refuse(changes, code):
 @pytest.mark.parametrize("changes, code", _REQUEST_REFUSALS + _ROW_REFUSALS + [
     (dict(dtype=3), -5), (dict(bounds_dtype=3), -5), (dict(Hq=3), -1), (dict(Hkv=0), -1), (dict(n_pages=0), -1), (dict(max_context=-1), -1), (dict(D=60), -3),
     (dict(D=264), -3), (dict(page_size=3), -3), (dict(n_select=2), -1), (dict(sink_pages=-1), -1), (dict(window_pages=0), -1),
-    (dict(sink_pages=2 ** 31 - 1, window_pages=2 ** 31 - 1), -1), (dict(q=None), -2), (dict(bounds=None), -2), (dict(pages=None), -2), (dict(bounds=_FAR + 4), -1),
+    (dict(sink_pages=2 ** 31 - 1, window_pages=2 ** 31 - 1), -1), (dict(q=None), -2), (dict(bounds=None), -2), (dict(pages=None), -2), (dict(bounds=_FAR + 4), -1), (dict(q=_FAR + 8), -1), (dict(qs_t=260), -1), (dict(qs_h=68), -1),
     (dict(work=None), -4), (dict(work_bytes=100), -4), (dict(work=_FAR + 8), -4), (dict(requests__n_tokens=-1), -1),
     (dict(requests__n_tokens=2 ** 30, work_bytes=2 ** 60), -3),
 ])
@@ -167,8 +167,9 @@ def test_workspaces_follow_the_work():
                                    requests=N.PageRequests(table_width=width, n_requests=requests, n_tokens=tokens))
         return N.page_work_bytes("attention", args)
 
-    assert attention(1, 8) == 0 and attention(1, 1000, n_select=8) == 0  # 128 keys: one workgroup's
-    assert 0 < attention(1, 64) <= attention(1, 2048) <= 8 * 32 * 1024 * 132 * 4
+    # two parts of 16 rows for each key head of a workgroup, of which there are as many as there is work for, 4 a CU at most
+    assert 0 < attention(1, 8) <= attention(1, 64) <= attention(1, 2048) <= attention(1, 2 ** 20) <= 1024 * 2 * 2 * 16 * 132 * 4
+    assert attention(1, 1000, n_select=8) <= attention(1, 8) < 2 ** 20
     # a chunk: the contexts in 16 bits, their table, and what the attention over them needs
     copy = 2 * 2 * 2048 * 16 * 2 * 128 + 4 * 2048
     assert copy < attention(2048, 2048) < copy + 2 ** 28
