@@ -5,7 +5,7 @@
 #define PG_BOUND_WAVES 8192
 
 // ---------------------------------------------------------------------------
-// store: 16 lanes hold a row (token, key head) of one matrix, 8 elements each (16 beyond 128 dims)
+// store: 16 lanes hold a row (token, key head) of both matrices, 8 elements each (16 beyond 128 dims)
 // ---------------------------------------------------------------------------
 // exponent of the scale of a row whose largest magnitude is `most`: the least e >= -110 with most <= 448 * 2^e = 1.75 * 2^(e + 8)
 __device__ __forceinline__ int pg_exponent(float most) {
@@ -38,66 +38,70 @@ __global__ __launch_bounds__(PG_NT) void k_page_store(sah_page_store_args P) {
   const int l16 = threadIdx.x & 15;
   const int64_t t = row / C.Hkv;
   const int h = (int)(row - t * C.Hkv);
-  const bool v = blockIdx.y != 0;
-  // (all 16 lanes of a row go the same way)
-  if (t >= P.n_tokens) return;
+  if (t >= P.n_tokens) return;  // (all 16 lanes of a row go the same way)
+  const char* from[2] = {(const char*)P.k + (t * P.ks_t + h * P.ks_h) * ES, (const char*)P.v + (t * P.vs_t + h * P.vs_h) * ES};
+  float x[2][2][8];  // keys and values, requested with the slot
+#pragma unroll
+  for (int v = 0; v < 2; ++v)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = 8 * l16 + 128 * i;
+      if (d < C.D) {
+        sah_load8<T>(from[v], d, x[v][i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[v][i][e] = 0.f;
+      }
+    }
   const int64_t slot = P.slot_map[t];
   if (slot < 0 || slot >= (int64_t)C.n_pages * C.page_size) return;
-  const char* from = (const char*)(v ? P.v : P.k) + (t * (v ? P.vs_t : P.ks_t) + h * (v ? P.vs_h : P.ks_h)) * ES;
-  float x[2][8];
-  float most = 0.f;
+  const int shift = 31 - __builtin_clz(C.page_size);
+  const int64_t page = slot >> shift, entry = slot & (C.page_size - 1), scale = (page * C.Hkv + h) * C.page_size + entry;
+  uint8_t* to[2] = {(uint8_t*)C.k + page * C.ks_p + entry * C.ks_t + h * C.ks_h, (uint8_t*)C.v + page * C.vs_p + entry * C.vs_t + h * C.vs_h};
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int d = 8 * l16 + 128 * i;
-    if (d < C.D) {
-      sah_load8<T>(from, d, x[i]);
-    } else {
+  for (int v = 0; v < 2; ++v) {
+    float most = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = fabsf(x[v][i][e]);
+        most = fmaxf(most, a < INFINITY ? a : 0.f);
+      }
+    const int e = pg_exponent(pg_row16_max(most));
+    const float up = sah_bits_to_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = 8 * l16 + 128 * i;
+      if (d >= C.D) continue;
+      const float* y = x[v][i];
+      *(uint2*)(to[v] + d) = make_uint2(pg_narrow4(y[0] * up, y[1] * up, y[2] * up, y[3] * up), pg_narrow4(y[4] * up, y[5] * up, y[6] * up, y[7] * up));
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = fabsf(x[i][e]);
-      most = fmaxf(most, a < INFINITY ? a : 0.f);
-    }
+    if (l16 == 0) (v ? C.v_scales : C.k_scales)[scale] = (uint8_t)(e + 127);
   }
-  const int e = pg_exponent(pg_row16_max(most));
-  const float up = sah_bits_to_float((uint32_t)(127 - e) << 23);
-  const int64_t page = slot / C.page_size, entry = slot - page * C.page_size;
-  uint8_t* to = (uint8_t*)(v ? C.v : C.k) + page * (v ? C.vs_p : C.ks_p) + entry * (v ? C.vs_t : C.ks_t) + h * (v ? C.vs_h : C.ks_h);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int d = 8 * l16 + 128 * i;
-    if (d >= C.D) continue;
-    *(uint2*)(to + d) = make_uint2(pg_narrow4(x[i][0] * up, x[i][1] * up, x[i][2] * up, x[i][3] * up),
-                                   pg_narrow4(x[i][4] * up, x[i][5] * up, x[i][6] * up, x[i][7] * up));
-  }
-  if (l16 == 0) (v ? C.v_scales : C.k_scales)[(page * C.Hkv + h) * C.page_size + entry] = (uint8_t)(e + 127);
 }
 
 // ---------------------------------------------------------------------------
-// load: a thread holds 16 elements of the cache (8-bit) or 16 bytes of it (others: copied as they are)
+// load: a thread holds 8 elements of the cache (8-bit: what 16 bytes of a 16-bit result take) or 16 bytes of it (others: copied as they are)
 // ---------------------------------------------------------------------------
-// what 16 elements of e4m3 are in type T, stored at `to`
+// what 8 elements of e4m3 are in type T, stored at `to`
 template <int T>
-__device__ __forceinline__ void pg_put16(char* to, uint4 x, float scale) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+__device__ __forceinline__ void pg_put8(char* to, uint2 x, float scale) {
   if constexpr (T == SAH_BF16) {
-    ((uint4*)to)[0] = make_uint4(pg_widen2<false>(w[0], scale), pg_widen2<true>(w[0], scale), pg_widen2<false>(w[1], scale), pg_widen2<true>(w[1], scale));
-    ((uint4*)to)[1] = make_uint4(pg_widen2<false>(w[2], scale), pg_widen2<true>(w[2], scale), pg_widen2<false>(w[3], scale), pg_widen2<true>(w[3], scale));
+    *(uint4*)to = make_uint4(pg_widen2<false>(x.x, scale), pg_widen2<true>(x.x, scale), pg_widen2<false>(x.y, scale), pg_widen2<true>(x.y, scale));
   } else {
+    float f[2][4];
+    pg_widen4(x.x, scale, f[0]);
+    pg_widen4(x.y, scale, f[1]);
+    if constexpr (T == SAH_F32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[4];
-      pg_widen4(w[i], scale, f);
-      if constexpr (T == SAH_F32) {
-        ((float4*)to)[i] = make_float4(f[0], f[1], f[2], f[3]);
-      } else {
-        // (a row's largest may have been rounded up past the type's; NaN stays)
+      for (int i = 0; i < 2; ++i) ((float4*)to)[i] = make_float4(f[i][0], f[i][1], f[i][2], f[i][3]);
+    } else {
+      // (a row's largest may have been rounded up past the type's; NaN stays)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = f[e] > 65504.f ? 65504.f : (f[e] < -65504.f ? -65504.f : f[e]);
-        ((uint2*)to)[i] = make_uint2(sah_pack2_hw<SAH_F16>(f[0], f[1]), sah_pack2_hw<SAH_F16>(f[2], f[3]));
-      }
+      for (int i = 0; i < 8; ++i) f[i / 4][i % 4] = f[i / 4][i % 4] > 65504.f ? 65504.f : (f[i / 4][i % 4] < -65504.f ? -65504.f : f[i / 4][i % 4]);
+      *(uint4*)to = make_uint4(sah_pack2_hw<SAH_F16>(f[0][0], f[0][1]), sah_pack2_hw<SAH_F16>(f[0][2], f[0][3]), sah_pack2_hw<SAH_F16>(f[1][0], f[1][1]),
+                               sah_pack2_hw<SAH_F16>(f[1][2], f[1][3]));
     }
   }
 }
@@ -105,7 +109,7 @@ __device__ __forceinline__ void pg_put16(char* to, uint4 x, float scale) {
 template <int CT, int OT>
 __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_requests R, pg_load_out O, int64_t n_units) {
   sah_touch_kernargs<sizeof(sah_page_cache) + sizeof(sah_page_requests) + sizeof(pg_load_out) + 8>();
-  constexpr int CS = pg_size(CT), OS = pg_size(OT), E = 16 / CS;  // elements of a unit
+  constexpr int CS = pg_size(CT), OS = pg_size(OT), E = CT == SAH_E4M3 ? 8 : 16 / CS;  // elements of a unit
   const int units = C.D / E, unit_h = units * C.Hkv;
   const int64_t u = (int64_t)blockIdx.x * PG_NT + threadIdx.x;
   if (u >= n_units) return;
@@ -125,14 +129,16 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
     for (int i = 0; i < E * OS / 16; ++i) ((uint4*)ko)[i] = ((uint4*)vo)[i] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const uint4 k = *(const uint4*)((const char*)C.k + (page * C.ks_p + entry * C.ks_t + h * C.ks_h) * CS + 16 * c);
-  const uint4 v = *(const uint4*)((const char*)C.v + (page * C.vs_p + entry * C.vs_t + h * C.vs_h) * CS + 16 * c);
+  const char* kp = (const char*)C.k + (page * C.ks_p + entry * C.ks_t + h * C.ks_h + c * E) * CS;
+  const char* vp = (const char*)C.v + (page * C.vs_p + entry * C.vs_t + h * C.vs_h + c * E) * CS;
   if constexpr (CT == SAH_E4M3) {
+    const uint2 k = *(const uint2*)kp, v = *(const uint2*)vp;
     const int64_t s = ((int64_t)page * C.Hkv + h) * C.page_size + entry;
     const float ks = pg_scale(C.k_scales[s]), vs = pg_scale(C.v_scales[s]);
-    pg_put16<OT>(ko, k, ks);
-    pg_put16<OT>(vo, v, vs);
+    pg_put8<OT>(ko, k, ks);
+    pg_put8<OT>(vo, v, vs);
   } else {
+    const uint4 k = *(const uint4*)kp, v = *(const uint4*)vp;
     *(uint4*)ko = k;
     *(uint4*)vo = v;
   }
@@ -580,7 +586,7 @@ extern "C" int sah_page_store(const sah_page_store_args* given) {
   const int64_t wgs = ((int64_t)a->n_tokens * c.Hkv + PG_NT / 16 - 1) / (PG_NT / 16);
   if (wgs > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_store: too many rows");
   sah_timed timed("k_page_store", a->stream);
-  const dim3 grid((unsigned)wgs, 2);
+  const dim3 grid((unsigned)wgs);
   hipStream_t st = (hipStream_t)a->stream;
   if (a->dtype == SAH_F32) hipLaunchKernelGGL(k_page_store<SAH_F32>, grid, dim3(PG_NT), 0, st, *a);
   else if (a->dtype == SAH_BF16) hipLaunchKernelGGL(k_page_store<SAH_BF16>, grid, dim3(PG_NT), 0, st, *a);
@@ -590,7 +596,7 @@ extern "C" int sah_page_store(const sah_page_store_args* given) {
 
 // (also what the attention over chunks makes its copy with)
 int pg_load(const sah_page_cache& c, const sah_page_requests& r, int dtype, const pg_load_out& out, void* stream, const char* what) {
-  const int64_t units = (int64_t)c.D * pg_size(c.dtype) / 16 * c.Hkv * out.length * r.n_requests, wgs = (units + PG_NT - 1) / PG_NT;
+  const int64_t units = (int64_t)c.D / (c.dtype == SAH_E4M3 ? 8 : 16 / pg_size(c.dtype)) * c.Hkv * out.length * r.n_requests, wgs = (units + PG_NT - 1) / PG_NT;
   if (wgs > 0x7fffffff) return sah_fail(SAH_ESHAPE, "%s: too many elements", what);
   sah_timed timed("k_page_load", stream);
   const dim3 grid((unsigned)wgs);
