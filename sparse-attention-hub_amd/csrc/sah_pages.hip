@@ -317,16 +317,16 @@ __global__ __launch_bounds__(PG_NT) void k_page_scores(pg_select S) {
     const bool always = j < P.sink_pages || j >= n - P.window_pages;
     for (int i0 = 0; i0 < PG_WAVE_PAGES; i0 += U * AT_ONCE) {
       if (j0 + i0 >= n) break;
-      uint4 lo[U], hi[U];
+      sah_u4 lo[U], hi[U];
       int at[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         at[i] = __shfl(always ? -1 : page, i0 + i * AT_ONCE + who);
-        lo[i] = hi[i] = make_uint4(0, 0, 0, 0);
+        lo[i] = hi[i] = sah_u4{0, 0, 0, 0};
         if (at[i] >= 0 && in * E < P.D) {
           const char* b = base + (int64_t)at[i] * P.Hkv * 2 * P.D * ES + 16 * in;
-          lo[i] = *(const uint4*)b;
-          hi[i] = *(const uint4*)(b + P.D * ES);
+          lo[i] = __builtin_nontemporal_load((const sah_u4*)b);
+          hi[i] = __builtin_nontemporal_load((const sah_u4*)(b + P.D * ES));
         }
       }
 #pragma unroll
