@@ -627,6 +627,7 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
           for (int c = 0; c < H; ++c)
 #pragma unroll
             for (int w = 0; w < VW; ++w) vx.r[c][4 * a + e][w] = some ? vx.r[c][4 * a + e][w] : 0u;
+          if constexpr (KT == SAH_E4M3) vx.scale[a] = some ? vx.scale[a] : vx.scale[a] & ~(0xffu << (8 * e));  // (0 times the byte 255 is NaN)
         }
     }
     float mx = s[0][0];

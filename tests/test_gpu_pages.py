@@ -518,6 +518,56 @@ def test_attention_over_pages_head_groups(cuda, q_heads, kv_heads):
     _attention_case(cuda, torch.bfloat16, torch.bfloat16, [1, 3], [400, 20], q_heads, kv_heads, 64, 16, seed=q_heads, lists=_some_pages)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("q_heads, kv_heads", [(3, 3), (8, 4), (10, 5), (6, 6), (16, 8), (24, 12), (34, 2)])
+def test_attention_8bit_key_heads_side_by_side(cuda, dtype, q_heads, kv_heads):
+    """Workgroups work on four, two or one of the key heads at once."""
+    _attention_case(cuda, dtype, _E4M3, [1, 2], [900, 40], q_heads, kv_heads, 64, 16, sinks=True, seed=kv_heads)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+def test_attention_8bit_in_many_parts(cuda, dtype):
+    """Contexts of thousands of keys at the widest heads, single tokens and a few, beside short ones: tiles that many workgroups share."""
+    _attention_case(cuda, dtype, _E4M3, [1, 4, 1], [7001, 3500, 2], 4, 2, 256, 32, sinks=True, seed=8)
+
+
+@pytest.mark.parametrize("page, sink, window", [(2048, 0, 0), (4096, 5, 700), (8192, 4100, 33)])
+def test_attention_8bit_over_large_pages(cuda, page, sink, window):
+    """Pages of more tokens than a workgroup looks up at once."""
+    _attention_case(cuda, torch.bfloat16, _E4M3, [1, 2], [9000, 4095], 4, 2, 64, page, sink, window, seed=page)
+
+
+def _many_requests(n):
+    """Short contexts, now and then a longer one, a request without new tokens, one without any."""
+    rng = random.Random(n)
+    new = [rng.choice([0, 1, 1, 1, 2]) for _ in range(n - 1)] + [1]
+    return new, [rng.choice([0, 3, 17, 40, 900 if i % 50 == 7 else 5]) for i in range(n)]
+
+
+@pytest.mark.parametrize("n", [64, 65, 256, 257, 700])
+def test_attention_of_many_requests(cuda, n):
+    """Lengths are looked at 64 and 256 at a time."""
+    new, cached = _many_requests(n)
+    _attention_case(cuda, torch.bfloat16, _E4M3, new, cached, 4, 2, 32, 16, seed=n, pad=3)
+    _attention_case(cuda, torch.bfloat16, torch.bfloat16, new, cached, 4, 2, 32, 16, seed=n, pad=3, lists=_some_pages)
+
+
+@pytest.mark.parametrize("n", [64, 65, 257, 5000])
+def test_pages_of_many_requests(cuda, n):
+    """The rows of thousands of requests find theirs: bounds and selection."""
+    new, cached = _many_requests(n)
+    case = Case(cuda, torch.bfloat16, new, cached, 2, 16, 8, seed=n)
+    bounds = torch.full((case.caches[0].shape[0], 2, 2, 16), 7.0, dtype=torch.bfloat16, device=cuda)
+    P.update_page_bounds(bounds, case.caches[0], case.table, case.kv_lens, case.cu_new)
+    want = torch.full(bounds.shape, 7.0, dtype=torch.float64)
+    for b in range(n):
+        for j in range(cached[b] // 8, case.kv[b] // 8):
+            at = int(case.table_host[b, j])
+            want[at, :, 0], want[at, :, 1] = case.wide[0][at].amin(0), case.wide[0][at].amax(0)
+    assert torch.equal(bounds.double().cpu(), want)
+    _select_case(cuda, torch.bfloat16, torch.bfloat16, new, cached, 4, 2, 16, 8, 6, seed=n, pad=2)
+
+
 # ------------------------------------------------------------------------------------------------------ what is not finite
 @pytest.mark.parametrize("dtype", _TYPES)
 @pytest.mark.parametrize("new", [[1, 3], [1, 60]])
@@ -539,6 +589,31 @@ def test_attention_8bit_values_that_are_not_finite_stay_where_they_are_seen(cuda
     assert torch.isnan(got[:case.cu[1]]).all()
     assert torch.isfinite(got[case.cu[1]:-1]).all()
     assert torch.isnan(got[-1, :, 5]).all() and torch.isfinite(got[-1, :, :5]).all() and torch.isfinite(got[-1, :, 6:]).all()
+
+
+@pytest.mark.parametrize("byte", [0, 255])
+@pytest.mark.parametrize("page", [4, 16, 64])
+@pytest.mark.parametrize("new", [[1, 3], [1, 60]])
+def test_attention_8bit_scales_of_keys_that_no_row_sees(cuda, new, page, byte):
+    """Entries that hold no token yet may hold anything, their scales too: a call on a cache where those differ gives the same bits."""
+    case = Case(cuda, _E4M3, new, [100, 21], 2, 64, page, seed=6)
+    q = torch.randn(case.cu[-1], 4, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(cuda)
+    lists = _i32([[list(range(case.width))] * 2] * case.cu[-1], cuda)
+
+    def calls():
+        return [P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, **case.held, **o)
+                for o in ({}, dict(pages=lists), dict(sink_size=5, window_size=30))]
+
+    want = calls()
+    used = torch.zeros(case.caches[0].shape[0], page, dtype=torch.bool)
+    for b in range(2):
+        j = torch.arange(case.kv[b])
+        used[case.table_host[b, j // page].long(), j % page] = True
+    hidden = ~used[:, None].expand(-1, 2, -1).to(cuda)
+    for s in case.scales:
+        s.view(torch.uint8)[hidden] = byte
+    for have, plain in zip(calls(), want):
+        assert torch.isfinite(have).all() and torch.equal(have, plain)
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
