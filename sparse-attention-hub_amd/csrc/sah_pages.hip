@@ -2,6 +2,7 @@
 #include "sah_pages.h"
 
 #define PG_NT 256
+#define PG_LOAD_WGS 16384
 #define PG_BOUND_WAVES 8192
 
 // ---------------------------------------------------------------------------
@@ -105,42 +106,48 @@ __device__ __forceinline__ void pg_put8(char* to, uint2 x, float scale) {
     }
   }
 }
-// CT: type of the cache; OT: of the output (other caches than SAH_E4M3: the same)
+// CT: type of the cache; OT: of the output (other caches than SAH_E4M3: the same). `wgs` workgroups a request, which go through its tokens in
+// turn: what lies behind a context in a table of a hundred thousand tokens costs a copy nothing.
 template <int CT, int OT>
-__global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_requests R, pg_load_out O, int64_t n_units) {
-  sah_touch_kernargs<sizeof(sah_page_cache) + sizeof(sah_page_requests) + sizeof(pg_load_out) + 8>();
+__global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_requests R, pg_load_out O, int wgs) {
+  sah_touch_kernargs<sizeof(sah_page_cache) + sizeof(sah_page_requests) + sizeof(pg_load_out) + 4>();
   constexpr int CS = pg_size(CT), OS = pg_size(OT), E = CT == SAH_E4M3 ? 8 : 16 / CS;  // elements of a unit
-  const int units = C.D / E, unit_h = units * C.Hkv;
-  const int64_t u = (int64_t)blockIdx.x * PG_NT + threadIdx.x;
-  if (u >= n_units) return;
+  const uint32_t units = C.D / E, unit_h = units * C.Hkv, stride = (uint32_t)wgs * PG_NT, stride_t = stride / unit_h, stride_in = stride - stride_t * unit_h;
+  const int shift = 31 - __builtin_clz(C.page_size), b = (int)blockIdx.x / wgs, kv = R.kv_lens[b];
+  const uint32_t n = O.table && kv < O.length ? (kv > 0 ? kv : 0) : O.length, first = (blockIdx.x - (uint32_t)b * wgs) * PG_NT + threadIdx.x;
   // consecutive threads: a token's units, all heads of it, then the next token: as the cache lies
-  const int64_t token = u / unit_h;
-  const int in = (int)(u - token * unit_h), h = in / units, c = in - h * units;
-  const int b = (int)(token / O.length), t = (int)(token - (int64_t)b * O.length);
-  const int shift = 31 - __builtin_clz(C.page_size), j = t >> shift, entry = t & (C.page_size - 1);
-  const int page = t < R.kv_lens[b] && j < R.table_width ? R.block_table[(int64_t)b * R.table_pitch + j] : -1;
-  const bool there = page >= 0 && page < C.n_pages;
-  if (O.table && entry == 0 && in == 0) O.table[(int64_t)b * R.table_width + j] = there ? b * R.table_width + j : -1;
-  if (O.table && !there) return;
-  const int64_t to = (b * O.s_b + h * O.s_h + t * O.s_t + (int64_t)c * E) * OS;
-  char *ko = (char*)O.k + to, *vo = (char*)O.v + to;
-  if (!there) {
+  uint32_t at = first / unit_h, in = first - at * unit_h;
+  for (; at < n; at += stride_t, in += stride_in) {
+    if (in >= unit_h) {
+      in -= unit_h;
+      if (++at >= n) break;
+    }
+    const int t = (int)at, h = (int)(in / units), c = (int)(in - h * units);
+    const int j = t >> shift, entry = t & (C.page_size - 1);
+    const int page = t < kv && j < R.table_width ? R.block_table[(int64_t)b * R.table_pitch + j] : -1;
+    const bool there = page >= 0 && page < C.n_pages;
+    if (O.table && entry == 0 && in == 0) O.table[(int64_t)b * R.table_width + j] = there ? b * R.table_width + j : -1;
+    if (O.table && !there) continue;
+    const int64_t to = (b * O.s_b + h * O.s_h + t * O.s_t + (int64_t)c * E) * OS;
+    char *ko = (char*)O.k + to, *vo = (char*)O.v + to;
+    if (!there) {
 #pragma unroll
-    for (int i = 0; i < E * OS / 16; ++i) ((uint4*)ko)[i] = ((uint4*)vo)[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  const char* kp = (const char*)C.k + (page * C.ks_p + entry * C.ks_t + h * C.ks_h + c * E) * CS;
-  const char* vp = (const char*)C.v + (page * C.vs_p + entry * C.vs_t + h * C.vs_h + c * E) * CS;
-  if constexpr (CT == SAH_E4M3) {
-    const uint2 k = *(const uint2*)kp, v = *(const uint2*)vp;
-    const int64_t s = ((int64_t)page * C.Hkv + h) * C.page_size + entry;
-    const float ks = pg_scale(C.k_scales[s]), vs = pg_scale(C.v_scales[s]);
-    pg_put8<OT>(ko, k, ks);
-    pg_put8<OT>(vo, v, vs);
-  } else {
-    const uint4 k = *(const uint4*)kp, v = *(const uint4*)vp;
-    *(uint4*)ko = k;
-    *(uint4*)vo = v;
+      for (int i = 0; i < E * OS / 16; ++i) ((uint4*)ko)[i] = ((uint4*)vo)[i] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const char* kp = (const char*)C.k + (page * C.ks_p + entry * C.ks_t + h * C.ks_h + c * E) * CS;
+    const char* vp = (const char*)C.v + (page * C.vs_p + entry * C.vs_t + h * C.vs_h + c * E) * CS;
+    if constexpr (CT == SAH_E4M3) {
+      const uint2 k = *(const uint2*)kp, v = *(const uint2*)vp;
+      const int64_t s = ((int64_t)page * C.Hkv + h) * C.page_size + entry;
+      const float ks = pg_scale(C.k_scales[s]), vs = pg_scale(C.v_scales[s]);
+      pg_put8<OT>(ko, k, ks);
+      pg_put8<OT>(vo, v, vs);
+    } else {
+      const uint4 k = *(const uint4*)kp, v = *(const uint4*)vp;
+      *(uint4*)ko = k;
+      *(uint4*)vo = v;
+    }
   }
 }
 
@@ -150,6 +157,16 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
 // (a NaN is kept: comparisons with it are false)
 __device__ __forceinline__ float pg_lower(float a, float b) { return b < a || b != b ? b : a; }
 __device__ __forceinline__ float pg_upper(float a, float b) { return b > a || b != b ? b : a; }
+// what the lanes l and l ^ 16 hold, to both of them
+__device__ __forceinline__ void pg_swap16(float v, float& a, float& b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const auto r = __builtin_amdgcn_permlane16_swap(sah_float_to_bits(v), sah_float_to_bits(v), false, false);
+  a = sah_bits_to_float(r[0]);
+  b = sah_bits_to_float(r[1]);
+#else
+  a = b = v;
+#endif
+}
 template <int T>
 __global__ __launch_bounds__(PG_NT) void k_page_bounds(sah_page_bounds_args P, int n_waves) {
   sah_touch_kernargs<sizeof(sah_page_bounds_args) + 4>();
@@ -180,40 +197,75 @@ __global__ __launch_bounds__(PG_NT) void k_page_bounds(sah_page_bounds_args P, i
         lo[e] = INFINITY;
         hi[e] = -INFINITY;
       }
-      for (int i = g; i < C.page_size; i += 4) {
-        float x[E];
-        if constexpr (T == SAH_E4M3) {
-          const float scale = pg_scale(C.k_scales[(pg * C.Hkv + h) * C.page_size + i]);
-          const uint2 w = *(const uint2*)((const uint8_t*)C.k + pg * C.ks_p + i * C.ks_t + h * C.ks_h + (on ? d : 0));
-          float a[4], b[4];
-          pg_widen4(w.x, scale, a);
-          pg_widen4(w.y, scale, b);
+      constexpr int U = 4;
+      for (int i0 = g; i0 < C.page_size; i0 += 4 * U) {  // four rows requested at once; behind the last one it is taken again, which changes nothing
+        sah_u4 raw[U][T == SAH_F32 ? 2 : 1];
+        float scale[U];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = a[e];
-            x[4 + e] = b[e];
+        for (int u = 0; u < U; ++u) {
+          const int64_t i = i0 + 4 * u < C.page_size ? i0 + 4 * u : i0;
+          const char* from = (const char*)C.k + (pg * C.ks_p + i * C.ks_t + h * C.ks_h + (on ? d : 0)) * pg_size(T);
+          if constexpr (T == SAH_E4M3) {
+            const uint2 w = *(const uint2*)from;
+            raw[u][0] = sah_u4{w.x, w.y, 0, 0};
+            scale[u] = pg_scale(C.k_scales[(pg * C.Hkv + h) * C.page_size + i]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < (T == SAH_F32 ? 2 : 1); ++k) raw[u][k] = ((const sah_u4*)from)[k];
           }
-        } else {
-          sah_load8<T>(C.k, pg * C.ks_p + i * C.ks_t + h * C.ks_h + (on ? d : 0), x);
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          lo[e] = pg_lower(lo[e], x[e]);
-          hi[e] = pg_upper(hi[e], x[e]);
+        for (int u = 0; u < U; ++u) {
+          float x[E];
+          if constexpr (T == SAH_E4M3) {
+            float a[4], b[4];
+            pg_widen4(raw[u][0].x, scale[u], a);
+            pg_widen4(raw[u][0].y, scale[u], b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[e] = a[e];
+              x[4 + e] = b[e];
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              if constexpr (T == SAH_F32) x[e] = sah_bits_to_float(raw[u][e / 4][e % 4]);
+              else if constexpr (T == SAH_BF16) x[e] = sah_bits_to_float(e % 2 ? raw[u][0][e / 2] & 0xffff0000u : raw[u][0][e / 2] << 16);
+              else x[e] = sah_f16_to_float((uint16_t)(raw[u][0][e / 2] >> (16 * (e % 2))));
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            lo[e] = pg_lower(lo[e], x[e]);
+            hi[e] = pg_upper(hi[e], x[e]);
+          }
         }
       }
+      // the four groups' rows: lanes l, l + 16, l + 32 and l + 48
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-#pragma unroll
-        for (int m = 16; m < SAH_WAVE; m *= 2) {
-          lo[e] = pg_lower(lo[e], __shfl_xor(lo[e], m));
-          hi[e] = pg_upper(hi[e], __shfl_xor(hi[e], m));
-        }
+        float a, b;
+        pg_swap16(lo[e], a, b);
+        lo[e] = pg_lower(a, b);
+        pg_swap16(hi[e], a, b);
+        hi[e] = pg_upper(a, b);
+        uint32_t c, f;
+        sah_half_both(sah_float_to_bits(lo[e]), c, f);
+        lo[e] = pg_lower(sah_bits_to_float(c), sah_bits_to_float(f));
+        sah_half_both(sah_float_to_bits(hi[e]), c, f);
+        hi[e] = pg_upper(sah_bits_to_float(c), sah_bits_to_float(f));
       }
       if (!on || g > 1) continue;
-      const int64_t to = ((pg * C.Hkv + h) * 2 + g) * C.D + d;
+      char* to = (char*)P.bounds + (((pg * C.Hkv + h) * 2 + g) * C.D + d) * pg_size(BT);
+      float y[E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) sah_store<BT>(P.bounds, to + e, g ? hi[e] : lo[e]);
+      for (int e = 0; e < E; ++e) y[e] = g ? hi[e] : lo[e];
+      if constexpr (BT == SAH_F32) {
+        ((float4*)to)[0] = make_float4(y[0], y[1], y[2], y[3]);
+        ((float4*)to)[1] = make_float4(y[4], y[5], y[6], y[7]);
+      } else {
+        *(uint4*)to = make_uint4(sah_pack2_hw<BT>(y[0], y[1]), sah_pack2_hw<BT>(y[2], y[3]), sah_pack2_hw<BT>(y[4], y[5]), sah_pack2_hw<BT>(y[6], y[7]));
+      }
     }
   }
 }
@@ -596,16 +648,17 @@ extern "C" int sah_page_store(const sah_page_store_args* given) {
 
 // (also what the attention over chunks makes its copy with)
 int pg_load(const sah_page_cache& c, const sah_page_requests& r, int dtype, const pg_load_out& out, void* stream, const char* what) {
-  const int64_t units = (int64_t)c.D / (c.dtype == SAH_E4M3 ? 8 : 16 / pg_size(c.dtype)) * c.Hkv * out.length * r.n_requests, wgs = (units + PG_NT - 1) / PG_NT;
-  if (wgs > 0x7fffffff) return sah_fail(SAH_ESHAPE, "%s: too many elements", what);
+  const int64_t units = (int64_t)c.D / (c.dtype == SAH_E4M3 ? 8 : 16 / pg_size(c.dtype)) * c.Hkv * out.length, room = PG_LOAD_WGS / r.n_requests;
+  int64_t wgs = (units + PG_NT - 1) / PG_NT;
+  if (wgs > room) wgs = room > 1 ? room : 1;
   sah_timed timed("k_page_load", stream);
-  const dim3 grid((unsigned)wgs);
+  const dim3 grid((unsigned)(wgs * r.n_requests));
   hipStream_t st = (hipStream_t)stream;
-  if (c.dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_F32, SAH_F32>), grid, dim3(PG_NT), 0, st, c, r, out, units);
-  else if (c.dtype != SAH_E4M3) hipLaunchKernelGGL((k_page_load<SAH_BF16, SAH_BF16>), grid, dim3(PG_NT), 0, st, c, r, out, units);
-  else if (dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F32>), grid, dim3(PG_NT), 0, st, c, r, out, units);
-  else if (dtype == SAH_BF16) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_BF16>), grid, dim3(PG_NT), 0, st, c, r, out, units);
-  else hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F16>), grid, dim3(PG_NT), 0, st, c, r, out, units);
+  if (c.dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_F32, SAH_F32>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else if (c.dtype != SAH_E4M3) hipLaunchKernelGGL((k_page_load<SAH_BF16, SAH_BF16>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else if (dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F32>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else if (dtype == SAH_BF16) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_BF16>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F16>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
   return sah_launch_status(what);
 }
 
