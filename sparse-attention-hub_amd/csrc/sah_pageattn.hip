@@ -127,15 +127,22 @@ __device__ __forceinline__ pt_cost pt_cost_of(const pt_args& A, const pt_lens& l
 }
 // How the line is shared: by `n` workgroups, and where workgroup w's piece begins
 struct pt_shares {
-  int64_t total, each;
+  int64_t each;
   uint32_t n, rest;
   __device__ __forceinline__ int64_t bound(int w) const { return each * w + rest * (uint32_t)w / n; }  // (n is at most 1024)
+  // Whose piece has key x, `away` from where w's begins: asked for two keys at once, by the halves of a wave, whose lanes try a piece each. (The
+  // guess is off by one at most: pieces differ by one key.)
+  __device__ __forceinline__ void holders(int64_t x, int64_t away, int w, int& lower, int& upper) const {
+    const int lane = threadIdx.x & (SAH_WAVE - 1), guess = w - 16 + (int)floorf((float)away / ((float)each + (float)rest / (float)n)), c = guess + (lane & 31);
+    const uint64_t begun = __ballot((c >= 0) & (c < (int)n) & (bound(c) <= x));
+    lower = __builtin_amdgcn_readlane(guess, 0) + 31 - __builtin_clz((uint32_t)begun | 1u);
+    upper = __builtin_amdgcn_readlane(guess, 32) + 31 - __builtin_clz((uint32_t)(begun >> 32) | 1u);
+  }
 };
 __device__ __forceinline__ pt_shares pt_share(const pt_args& A, int64_t total, int wgs) {
   const sah_page_attention_args& P = A.a;
   pt_shares s;
   const int64_t w = (total * A.heads + PT_LEAST - 1) / PT_LEAST;
-  s.total = total;
   s.n = (uint32_t)(w < wgs ? w : wgs);
   // Tiles that are all alike (lists; one request): so many workgroups that no piece holds parts of two. A second tile of a short piece costs as
   // much as the first (1024 keys of 8 heads: 15 -> 9 us).
@@ -159,8 +166,8 @@ struct pt_place {
   pt_cost cost;
   int64_t x0, x1;  // the workgroup's piece
 };
-// s_sum: PT_NW + 4 words. All threads call. False: no piece.
-__device__ __forceinline__ bool pt_start(const pt_args& A, int w, int wgs, int64_t* s_sum, pt_place& at) {
+// s_sum: PT_NW + 3 words; s_shares: how the line is shared. All threads call. False: no piece.
+__device__ __forceinline__ bool pt_start(const pt_args& A, int w, int wgs, int64_t* s_sum, pt_shares& s_shares, pt_place& at) {
   const sah_page_requests& R = A.a.requests;
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
   auto scan = [&](int64_t v, int64_t& all) -> int64_t {  // inclusive
@@ -188,6 +195,7 @@ __device__ __forceinline__ bool pt_start(const pt_args& A, int w, int wgs, int64
     const pt_shares s = pt_share(A, total, wgs);
     at.x0 = w < (int)s.n ? s.bound(w) : 0;
     at.x1 = w < (int)s.n ? s.bound(w + 1) : 0;
+    if (threadIdx.x == 0) s_shares = s;
   };
   auto claim = [&](int b, int64_t mine, int64_t end) {  // one thread's request holds x0
     if (mine && end > at.x0 && end - mine <= at.x0) {
@@ -239,6 +247,18 @@ __device__ __forceinline__ int pt_key_at(int64_t y, int64_t cost, int n) {
   if (y >= cost) return n;
   const int u = (int)((double)n * ((double)y / (double)cost));
   return __builtin_amdgcn_readfirstlane(u / PT_STEP * PT_STEP);
+}
+
+// What the join has to know of a part: whose it is, and which workgroups have the tile's others. Every workgroup leaves two of them, of the
+// tile that began before its piece and of the one that ends behind it; parts 0: there is none.
+struct __attribute__((aligned(16))) pt_record {
+  int w0, parts;
+  int t0, rows, hk0, block;
+  int b, begin, end, kv;
+  int pad[2];
+};
+__device__ __forceinline__ pt_record* pt_records(const pt_args& A, int wgs, int dp, int w) {
+  return (pt_record*)((float*)A.a.work + (int64_t)wgs * 2 * A.heads * PT_ROWS * (dp + 4)) + 2 * w;
 }
 
 // One row key by key, by one wave: what a row holds that came out not finite. The average so far is held, not the sum: of finite values it
@@ -387,465 +407,437 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
   __shared__ __align__(16) float s_acc[PT_NW][PT_ROWS][PITCH];
   __shared__ float s_ml[PT_NW][2][PT_ROWS];
   __shared__ unsigned long long s_bad;  // a bit a head and row
-
-  __shared__ int64_t s_sum[PT_NW + 4];
+  __shared__ int64_t s_sum[PT_NW + 3];
+  __shared__ pt_shares s_shares;
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id(), i16 = lane & 15, g = lane >> 4;
   const int w = pt_number();
   pt_place at;
-  if (!pt_start(pt_arguments(), w, gridDim.x, s_sum, at)) return;
+  if (!pt_start(pt_arguments(), w, gridDim.x, s_sum, s_shares, at)) {
+    if (threadIdx.x < 2) pt_records(pt_arguments(), gridDim.x, DP, w)[threadIdx.x].parts = 0;
+    return;
+  }
+  int left = 0;  // records that have been written, a bit each
   int64_t x = at.x0;
   for (;;) {
-  const pt_args& A = pt_arguments();
-  const sah_page_attention_args& P = A.a;
-  const sah_page_cache& C = P.cache;
-  const int G = P.Hq / C.Hkv, shift = 31 - __builtin_clz(C.page_size);
-  const float c_exp = pt_log2(P.scaling), sign = P.scaling < 0.f ? -1.f : 1.f;
-  const int64_t y0 = x - at.begin, y1 = at.x1 - at.begin < at.cost.each ? at.x1 - at.begin : at.cost.each;
-  const bool whole = y0 == 0 && y1 == at.cost.each;
-  const int tile = __builtin_amdgcn_readfirstlane((int)at.tile);  // (n_tokens * Hq fits)
-  const int head_groups = C.Hkv / A.heads, tb = tile / head_groups, hk0 = (tile - tb * head_groups) * A.heads, block = tb % A.blocks, i0 = tb / A.blocks * A.tokens;
-  const int hk = hk0 + (wave & (A.heads - 1)), turns = PT_NW / A.heads, turn = wave / A.heads;  // this wave's head; a head's waves take turns
-  const int t0 = at.lens.begin + i0;
-  const pg_request req = pg_make(P.requests, C.page_size, at.b, at.lens.begin, at.lens.end, at.lens.kv);
-  const int n_tok = A.tokens < req.n_new - i0 ? A.tokens : req.n_new - i0;
-  const int rows = A.blocks > 1 ? (G - block * PT_ROWS < PT_ROWS ? G - block * PT_ROWS : PT_ROWS) : n_tok * G;
-  const int64_t p_lo = req.base + t0, p_hi = p_lo + n_tok - 1;
-  const pt_keys keys = pt_keys_of(A, req, p_lo, p_hi);
-  const int u_first = y0 ? pt_key_at(y0, at.cost.each, keys.n) : 0, u_end = pt_key_at(y1, at.cost.each, keys.n);
-  const bool live = i16 < rows;
-  const int rr = live ? i16 : rows - 1;
-  const int tok = t0 + (A.blocks > 1 ? 0 : rr / G), head = hk * G + (A.blocks > 1 ? block * PT_ROWS + rr : rr % G);
-  const int64_t p = req.base + tok;
-  const int last = p < keys.hi ? (p < -1 ? -1 : (int)p) : keys.hi;          // the last key that this lane's row sees
-  const int least = p_lo < keys.hi ? (p_lo < -1 ? -1 : (int)p_lo) : keys.hi; // ... that all rows see
-  // window: where it begins for this lane's row, for some row, for all rows
-  const int sink = P.window ? P.sink : 0;
-  auto window_from = [&](int64_t at_p) { return P.window && at_p >= P.window ? (int)(at_p - P.window + 1 < keys.hi + 1 ? at_p - P.window + 1 : keys.hi + 1) : 0; };
-  const int from_own = window_from(p), from_any = window_from(p_lo), from_all = window_from(p_hi);
-  if (threadIdx.x == 0) s_bad = 0;
+    const pt_args& A = pt_arguments();
+    const sah_page_attention_args& P = A.a;
+    const sah_page_cache& C = P.cache;
+    const int G = P.Hq / C.Hkv, shift = 31 - __builtin_clz(C.page_size);
+    const float c_exp = pt_log2(P.scaling), sign = P.scaling < 0.f ? -1.f : 1.f;
+    const int64_t y0 = x - at.begin, y1 = at.x1 - at.begin < at.cost.each ? at.x1 - at.begin : at.cost.each;
+    const bool whole = y0 == 0 && y1 == at.cost.each;
+    const int tile = __builtin_amdgcn_readfirstlane((int)at.tile);  // (n_tokens * Hq fits)
+    const int head_groups = C.Hkv / A.heads, tb = tile / head_groups, hk0 = (tile - tb * head_groups) * A.heads, block = tb % A.blocks, i0 = tb / A.blocks * A.tokens;
+    const int hk = hk0 + (wave & (A.heads - 1)), turns = PT_NW / A.heads, turn = wave / A.heads;  // this wave's head; a head's waves take turns
+    const int t0 = at.lens.begin + i0;
+    const pg_request req = pg_make(P.requests, C.page_size, at.b, at.lens.begin, at.lens.end, at.lens.kv);
+    const int n_tok = A.tokens < req.n_new - i0 ? A.tokens : req.n_new - i0;
+    const int rows = A.blocks > 1 ? (G - block * PT_ROWS < PT_ROWS ? G - block * PT_ROWS : PT_ROWS) : n_tok * G;
+    const int64_t p_lo = req.base + t0, p_hi = p_lo + n_tok - 1;
+    const pt_keys keys = pt_keys_of(A, req, p_lo, p_hi);
+    const int u_first = y0 ? pt_key_at(y0, at.cost.each, keys.n) : 0, u_end = pt_key_at(y1, at.cost.each, keys.n);
+    const bool live = i16 < rows;
+    const int rr = live ? i16 : rows - 1;
+    const int tok = t0 + (A.blocks > 1 ? 0 : rr / G), head = hk * G + (A.blocks > 1 ? block * PT_ROWS + rr : rr % G);
+    const int64_t p = req.base + tok;
+    const int last = p < keys.hi ? (p < -1 ? -1 : (int)p) : keys.hi;          // the last key that this lane's row sees
+    const int least = p_lo < keys.hi ? (p_lo < -1 ? -1 : (int)p_lo) : keys.hi; // ... that all rows see
+    // window: where it begins for this lane's row, for some row, for all rows
+    const int sink = P.window ? P.sink : 0;
+    auto window_from = [&](int64_t at_p) { return P.window && at_p >= P.window ? (int)(at_p - P.window + 1 < keys.hi + 1 ? at_p - P.window + 1 : keys.hi + 1) : 0; };
+    const int from_own = window_from(p), from_any = window_from(p_lo), from_all = window_from(p_hi);
+    if (threadIdx.x == 0) s_bad = 0;
 
-  // Queries as the second operand, in the order in which a lane's 16 bytes of a key come: requested here, made into it when the first keys are
-  // under way.
-  constexpr int QS = KT == SAH_F32 ? KL : DP / 32, QE = KT == SAH_F32 ? 4 : 8, QW = QE * pg_size(QT) / 16;  // pieces, elements, loads of a piece
-  const char* qp = (const char*)P.q + ((int64_t)tok * P.qs_t + (int64_t)head * P.qs_h) * pg_size(QT);
-  uint4 qf[T::NQ][QS];
-  sah_u4 q_raw[QS][QW];
-#pragma unroll
-  for (int s = 0; s < QS; ++s) {
-    const int d = KT == SAH_F32 ? 16 * s + 4 * g : KT == SAH_E4M3 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
-#pragma unroll
-    for (int i = 0; i < QW; ++i) {
-      q_raw[s][i] = sah_u4{0, 0, 0, 0};
-      if (d < C.D && live) q_raw[s][i] = *(const sah_u4*)(qp + d * pg_size(QT) + 16 * i);
-    }
-  }
-  // Where the keys from u0 on lie, MOST of them
-  auto look_up = [&](int u0) __attribute__((always_inline)) {
-    const int u1 = u_end - u0 < MOST ? u_end : u0 + MOST;
-    constexpr int EACH = SMALL ? 1 : 16;
-    const int n_slots = (u1 - u0 + STEP - 1) / STEP * (STEP / EACH);
-    const int32_t* list = P.pages ? P.pages + ((int64_t)t0 * C.Hkv + hk0) * P.n_select : nullptr;
-    for (int s = threadIdx.x; s < n_slots; s += PT_NT) {
-      const int u = u0 + s * EACH, e = u >> shift;
-      int64_t in = u & (C.page_size - 1);
-      int lg = e;
-      if (list) lg = e < P.n_select ? list[e] : -1;
-      else if (keys.skip && u >= keys.sinks) lg = e + (keys.skip >> shift);
-      int64_t page = -1;
-      if (lg >= 0 && lg < P.requests.table_width && lg <= keys.hi >> shift) page = P.requests.block_table[(int64_t)req.b * P.requests.table_pitch + lg];
-      pt_where at;
-      // a page that is not there: another one's keys, behind every position (table_width pages end before that)
-      at.first = (int)(0x80000000u - (uint32_t)C.page_size + (uint32_t)in);
-      if (page >= 0 && page < C.n_pages) at.first = (lg << shift) + (int)in;
-      else page = in = 0;
-      at.k = (page * C.ks_p + in * C.ks_t) * ES;
-      at.v = (page * C.vs_p + in * C.vs_t) * ES;
-      at.scale = page * C.Hkv * C.page_size + in;
-      s_at[s] = at;
-    }
-  };
-  __syncthreads();  // the sums of the tile before have been read
-  if (u_first < u_end) look_up(u_first);
-  {
+    // Queries as the second operand, in the order in which a lane's 16 bytes of a key come: requested here, made into it when the first keys are
+    // under way.
+    constexpr int QS = KT == SAH_F32 ? KL : DP / 32, QE = KT == SAH_F32 ? 4 : 8, QW = QE * pg_size(QT) / 16;  // pieces, elements, loads of a piece
+    const char* qp = (const char*)P.q + ((int64_t)tok * P.qs_t + (int64_t)head * P.qs_h) * pg_size(QT);
+    uint4 qf[T::NQ][QS];
+    sah_u4 q_raw[QS][QW];
 #pragma unroll
     for (int s = 0; s < QS; ++s) {
-      float v[8];
+      const int d = KT == SAH_F32 ? 16 * s + 4 * g : KT == SAH_E4M3 ? 64 * (s / 2) + 16 * g + 8 * (s % 2) : 32 * s + 8 * g;
 #pragma unroll
-      for (int i = 0; i < QW; ++i)
+      for (int i = 0; i < QW; ++i) {
+        q_raw[s][i] = sah_u4{0, 0, 0, 0};
+        if (d < C.D && live) q_raw[s][i] = *(const sah_u4*)(qp + d * pg_size(QT) + 16 * i);
+      }
+    }
+    // Where the keys from u0 on lie, MOST of them
+    auto look_up = [&](int u0) __attribute__((always_inline)) {
+      const int u1 = u_end - u0 < MOST ? u_end : u0 + MOST;
+      constexpr int EACH = SMALL ? 1 : 16;
+      const int n_slots = (u1 - u0 + STEP - 1) / STEP * (STEP / EACH);
+      const int32_t* list = P.pages ? P.pages + ((int64_t)t0 * C.Hkv + hk0) * P.n_select : nullptr;
+      for (int s = threadIdx.x; s < n_slots; s += PT_NT) {
+        const int u = u0 + s * EACH, e = u >> shift;
+        int64_t in = u & (C.page_size - 1);
+        int lg = e;
+        if (list) lg = e < P.n_select ? list[e] : -1;
+        else if (keys.skip && u >= keys.sinks) lg = e + (keys.skip >> shift);
+        int64_t page = -1;
+        if (lg >= 0 && lg < P.requests.table_width && lg <= keys.hi >> shift) page = P.requests.block_table[(int64_t)req.b * P.requests.table_pitch + lg];
+        pt_where at;
+        // a page that is not there: another one's keys, behind every position (table_width pages end before that)
+        at.first = (int)(0x80000000u - (uint32_t)C.page_size + (uint32_t)in);
+        if (page >= 0 && page < C.n_pages) at.first = (lg << shift) + (int)in;
+        else page = in = 0;
+        at.k = (page * C.ks_p + in * C.ks_t) * ES;
+        at.v = (page * C.vs_p + in * C.vs_t) * ES;
+        at.scale = page * C.Hkv * C.page_size + in;
+        s_at[s] = at;
+      }
+    };
+    __syncthreads();  // the sums of the tile before have been read
+    if (u_first < u_end) look_up(u_first);
+    {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t x = q_raw[s][i][k];
-          if constexpr (QT == SAH_F32) {
-            v[4 * i + k] = sign * sah_bits_to_float(x);
-          } else if constexpr (QT == SAH_BF16) {
-            v[2 * k] = sign * sah_bits_to_float(x << 16);
-            v[2 * k + 1] = sign * sah_bits_to_float(x & 0xffff0000u);
-          } else {
-            v[2 * k] = sign * sah_f16_to_float((uint16_t)x);
-            v[2 * k + 1] = sign * sah_f16_to_float((uint16_t)(x >> 16));
+      for (int s = 0; s < QS; ++s) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < QW; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t x = q_raw[s][i][k];
+            if constexpr (QT == SAH_F32) {
+              v[4 * i + k] = sign * sah_bits_to_float(x);
+            } else if constexpr (QT == SAH_BF16) {
+              v[2 * k] = sign * sah_bits_to_float(x << 16);
+              v[2 * k + 1] = sign * sah_bits_to_float(x & 0xffff0000u);
+            } else {
+              v[2 * k] = sign * sah_f16_to_float((uint16_t)x);
+              v[2 * k + 1] = sign * sah_f16_to_float((uint16_t)(x >> 16));
+            }
           }
-        }
-      if constexpr (KT == SAH_F32) {
-        qf[0][s] = make_uint4(sah_float_to_bits(v[0]), sah_float_to_bits(v[1]), sah_float_to_bits(v[2]), sah_float_to_bits(v[3]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < T::NQ; ++i) {
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = pt_term<MT>(v[2 * k], v[2 * k + 1]);
-          qf[i][s] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-    }
-  }
-  __syncthreads();
-
-  float m_run = -INFINITY, l_run = 0.f;
-  sah_f32x4 acc[TILES];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
-
-  // What lies behind a shorter head's end is its last piece again: the queries are 0 there, the results nobody's. Offsets of a lane from a
-  // key tile's first key (SMALL: from its own key).
-  uint32_t k_in[KL], v_in[H][4];
-#pragma unroll
-  for (int s = 0; s < KL; ++s) {
-    const int in = 64 * s + 16 * g;
-    k_in[s] = (uint32_t)((SMALL ? 0 : i16 * C.ks_t * ES) + (in < C.D * ES ? in : C.D * ES - 16));
-  }
-#pragma unroll
-  for (int s = 0; s < H; ++s) {
-    const int in = (s * 16 + i16) * NC;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) v_in[s][v] = (uint32_t)((SMALL ? 0 : (4 * g + v) * C.vs_t * ES) + (in < C.D ? in : C.D - NC) * ES);
-  }
-  const char* kbase = (const char*)C.k + (int64_t)hk * C.ks_h * ES;
-  const char* vbase = (const char*)C.v + (int64_t)hk * C.vs_h * ES;
-  const uint8_t *k_scales = C.k_scales + (int64_t)hk * C.page_size, *v_scales = C.v_scales + (int64_t)hk * C.page_size;
-
-  struct keys_of { sah_u4 r[NA][KL]; uint32_t scale[NA]; } kb;           // scales: bytes, of four keys, this lane's among them
-  struct values_of { uint32_t r[H][4 * NA][VW]; uint32_t scale[NA]; } vb; // ... of the four whose values a lane has
-  int u0 = u_first;                  // of what s_at holds
-  auto fetch_k = [&](int u, keys_of& k) __attribute__((always_inline)) {
-#pragma unroll
-    for (int a = 0; a < NA; ++a) {
-      if constexpr (SMALL) {
-        const pt_where& at = s_at[u + 16 * a + i16 - u0];
-        const char* from = kbase + at.k;
-        if constexpr (KT == SAH_E4M3) k.scale[a] = k_scales[at.scale] * 0x01010101u;
-#pragma unroll
-        for (int s = 0; s < KL; ++s) k.r[a][s] = *(const sah_u4*)(from + k_in[s]);
-      } else {
-        const pt_where& at = s_at[(u - u0) / 16 + a];
-        const char* from = kbase + pg_uniform(at.k);
-        if constexpr (KT == SAH_E4M3) k.scale[a] = pt_load<uint32_t>(k_scales + pg_uniform(at.scale), i16 & 12);
-#pragma unroll
-        for (int s = 0; s < KL; ++s) k.r[a][s] = pt_load<sah_u4>(from, k_in[s]);
-      }
-    }
-  };
-  auto fetch_v = [&](int u, values_of& x) __attribute__((always_inline)) {
-#pragma unroll
-    for (int a = 0; a < NA; ++a) {
-      const char* from = nullptr;
-      if constexpr (!SMALL) {
-        const pt_where& at = s_at[(u - u0) / 16 + a];
-        from = vbase + pg_uniform(at.v);
-        if constexpr (KT == SAH_E4M3) x.scale[a] = pt_load<uint32_t>(v_scales + pg_uniform(at.scale), 4 * g);
-      } else if constexpr (KT == SAH_E4M3) {
-        x.scale[a] = 0;
-      }
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        if constexpr (SMALL) {
-          const pt_where& at = s_at[u + 16 * a + 4 * g + v - u0];
-          from = vbase + at.v;
-          if constexpr (KT == SAH_E4M3) x.scale[a] |= (uint32_t)v_scales[at.scale] << (8 * v);
-        }
-#pragma unroll
-        for (int s = 0; s < H; ++s) {
-          uint32_t* to = x.r[s][4 * a + v];
-          typedef uint32_t words __attribute__((ext_vector_type(VW)));
-          const words w = SMALL ? *(const words*)(from + v_in[s][v]) : pt_load<words>(from, v_in[s][v]);
-#pragma unroll
-          for (int i = 0; i < VW; ++i) to[i] = w[i];
-        }
-      }
-    }
-  };
-
-  auto step = [&](int u, int next, keys_of& kx, values_of& vx) __attribute__((always_inline)) {
-    sah_f32x4 s[NA];
-#pragma unroll
-    for (int a = 0; a < NA; ++a) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[a][e] = 0.f;
-      const float scale = KT == SAH_E4M3 ? pg_scale_of(kx.scale[a], i16 & 3) : 1.f;
-#pragma unroll
-      for (int c = 0; c < KL; ++c) {
-        const sah_u4 k = kx.r[a][c];
         if constexpr (KT == SAH_F32) {
-          s[a] = pt_mfma_f32(sah_bits_to_float(k.x), sah_bits_to_float(qf[0][c].x), s[a]);
-          s[a] = pt_mfma_f32(sah_bits_to_float(k.y), sah_bits_to_float(qf[0][c].y), s[a]);
-          s[a] = pt_mfma_f32(sah_bits_to_float(k.z), sah_bits_to_float(qf[0][c].z), s[a]);
-          s[a] = pt_mfma_f32(sah_bits_to_float(k.w), sah_bits_to_float(qf[0][c].w), s[a]);
-        } else if constexpr (KT == SAH_E4M3) {
-          const uint4 k0 = make_uint4(pg_widen2<false>(k.x, scale), pg_widen2<true>(k.x, scale), pg_widen2<false>(k.y, scale), pg_widen2<true>(k.y, scale));
-          const uint4 k1 = make_uint4(pg_widen2<false>(k.z, scale), pg_widen2<true>(k.z, scale), pg_widen2<false>(k.w, scale), pg_widen2<true>(k.w, scale));
+          qf[0][s] = make_uint4(sah_float_to_bits(v[0]), sah_float_to_bits(v[1]), sah_float_to_bits(v[2]), sah_float_to_bits(v[3]));
+        } else {
 #pragma unroll
           for (int i = 0; i < T::NQ; ++i) {
-            s[a] = sah_mfma_16x16x32<MT>(k0, qf[i][2 * c], s[a]);
-            s[a] = sah_mfma_16x16x32<MT>(k1, qf[i][2 * c + 1], s[a]);
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = pt_term<MT>(v[2 * k], v[2 * k + 1]);
+            qf[i][s] = make_uint4(w[0], w[1], w[2], w[3]);
           }
-        } else {
-          s[a] = sah_mfma_16x16x32<MT>(make_uint4(k.x, k.y, k.z, k.w), qf[0][c], s[a]);
         }
       }
     }
-    fetch_k(next, kx);
-    // keys that not every row sees; values of keys that no row sees are made 0
-    int first[NA] = {};
-    bool plain = !SMALL;   // uniform
-    if constexpr (!SMALL) {
+    __syncthreads();
+
+    float m_run = -INFINITY, l_run = 0.f;
+    sah_f32x4 acc[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
+
+    // What lies behind a shorter head's end is its last piece again: the queries are 0 there, the results nobody's. Offsets of a lane from a
+    // key tile's first key (SMALL: from its own key).
+    uint32_t k_in[KL], v_in[H][4];
+#pragma unroll
+    for (int s = 0; s < KL; ++s) {
+      const int in = 64 * s + 16 * g;
+      k_in[s] = (uint32_t)((SMALL ? 0 : i16 * C.ks_t * ES) + (in < C.D * ES ? in : C.D * ES - 16));
+    }
+#pragma unroll
+    for (int s = 0; s < H; ++s) {
+      const int in = (s * 16 + i16) * NC;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) v_in[s][v] = (uint32_t)((SMALL ? 0 : (4 * g + v) * C.vs_t * ES) + (in < C.D ? in : C.D - NC) * ES);
+    }
+    const char* kbase = (const char*)C.k + (int64_t)hk * C.ks_h * ES;
+    const char* vbase = (const char*)C.v + (int64_t)hk * C.vs_h * ES;
+    const uint8_t *k_scales = C.k_scales + (int64_t)hk * C.page_size, *v_scales = C.v_scales + (int64_t)hk * C.page_size;
+
+    struct keys_of { sah_u4 r[NA][KL]; uint32_t scale[NA]; } kb;           // scales: bytes, of four keys, this lane's among them
+    struct values_of { uint32_t r[H][4 * NA][VW]; uint32_t scale[NA]; } vb; // ... of the four whose values a lane has
+    int u0 = u_first;                  // of what s_at holds
+    auto fetch_k = [&](int u, keys_of& k) __attribute__((always_inline)) {
 #pragma unroll
       for (int a = 0; a < NA; ++a) {
-        first[a] = __builtin_amdgcn_readfirstlane(s_at[(u - u0) / 16 + a].first);
-        plain = plain & (first[a] + 15 <= least) & ((first[a] >= from_all) | (first[a] + 15 < sink));
+        if constexpr (SMALL) {
+          const pt_where& at = s_at[u + 16 * a + i16 - u0];
+          const char* from = kbase + at.k;
+          if constexpr (KT == SAH_E4M3) k.scale[a] = k_scales[at.scale] * 0x01010101u;
+#pragma unroll
+          for (int s = 0; s < KL; ++s) k.r[a][s] = *(const sah_u4*)(from + k_in[s]);
+        } else {
+          const pt_where& at = s_at[(u - u0) / 16 + a];
+          const char* from = kbase + pg_uniform(at.k);
+          if constexpr (KT == SAH_E4M3) k.scale[a] = pt_load<uint32_t>(k_scales + pg_uniform(at.scale), i16 & 12);
+#pragma unroll
+          for (int s = 0; s < KL; ++s) k.r[a][s] = pt_load<sah_u4>(from, k_in[s]);
+        }
       }
-    }
-    if (!plain) {
+    };
+    auto fetch_v = [&](int u, values_of& x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int a = 0; a < NA; ++a) {
+        const char* from = nullptr;
+        if constexpr (!SMALL) {
+          const pt_where& at = s_at[(u - u0) / 16 + a];
+          from = vbase + pg_uniform(at.v);
+          if constexpr (KT == SAH_E4M3) x.scale[a] = pt_load<uint32_t>(v_scales + pg_uniform(at.scale), 4 * g);
+        } else if constexpr (KT == SAH_E4M3) {
+          x.scale[a] = 0;
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          if constexpr (SMALL) {
+            const pt_where& at = s_at[u + 16 * a + 4 * g + v - u0];
+            from = vbase + at.v;
+            if constexpr (KT == SAH_E4M3) x.scale[a] |= (uint32_t)v_scales[at.scale] << (8 * v);
+          }
+#pragma unroll
+          for (int s = 0; s < H; ++s) {
+            uint32_t* to = x.r[s][4 * a + v];
+            typedef uint32_t words __attribute__((ext_vector_type(VW)));
+            const words w = SMALL ? *(const words*)(from + v_in[s][v]) : pt_load<words>(from, v_in[s][v]);
+#pragma unroll
+            for (int i = 0; i < VW; ++i) to[i] = w[i];
+          }
+        }
+      }
+    };
+
+    auto step = [&](int u, int next, keys_of& kx, values_of& vx) __attribute__((always_inline)) {
+      sah_f32x4 s[NA];
+#pragma unroll
+      for (int a = 0; a < NA; ++a) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[a][e] = 0.f;
+        const float scale = KT == SAH_E4M3 ? pg_scale_of(kx.scale[a], i16 & 3) : 1.f;
+#pragma unroll
+        for (int c = 0; c < KL; ++c) {
+          const sah_u4 k = kx.r[a][c];
+          if constexpr (KT == SAH_F32) {
+            s[a] = pt_mfma_f32(sah_bits_to_float(k.x), sah_bits_to_float(qf[0][c].x), s[a]);
+            s[a] = pt_mfma_f32(sah_bits_to_float(k.y), sah_bits_to_float(qf[0][c].y), s[a]);
+            s[a] = pt_mfma_f32(sah_bits_to_float(k.z), sah_bits_to_float(qf[0][c].z), s[a]);
+            s[a] = pt_mfma_f32(sah_bits_to_float(k.w), sah_bits_to_float(qf[0][c].w), s[a]);
+          } else if constexpr (KT == SAH_E4M3) {
+            const uint4 k0 = make_uint4(pg_widen2<false>(k.x, scale), pg_widen2<true>(k.x, scale), pg_widen2<false>(k.y, scale), pg_widen2<true>(k.y, scale));
+            const uint4 k1 = make_uint4(pg_widen2<false>(k.z, scale), pg_widen2<true>(k.z, scale), pg_widen2<false>(k.w, scale), pg_widen2<true>(k.w, scale));
+#pragma unroll
+            for (int i = 0; i < T::NQ; ++i) {
+              s[a] = sah_mfma_16x16x32<MT>(k0, qf[i][2 * c], s[a]);
+              s[a] = sah_mfma_16x16x32<MT>(k1, qf[i][2 * c + 1], s[a]);
+            }
+          } else {
+            s[a] = sah_mfma_16x16x32<MT>(make_uint4(k.x, k.y, k.z, k.w), qf[0][c], s[a]);
+          }
+        }
+      }
+      fetch_k(next, kx);
+      // keys that not every row sees; values of keys that no row sees are made 0
+      int first[NA] = {};
+      bool plain = !SMALL;   // uniform
+      if constexpr (!SMALL) {
+#pragma unroll
+        for (int a = 0; a < NA; ++a) {
+          first[a] = __builtin_amdgcn_readfirstlane(s_at[(u - u0) / 16 + a].first);
+          plain = plain & (first[a] + 15 <= least) & ((first[a] >= from_all) | (first[a] + 15 < sink));
+        }
+      }
+      if (!plain) {
+#pragma unroll
+        for (int a = 0; a < NA; ++a)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = SMALL ? s_at[u + 16 * a + 4 * g + e - u0].first : first[a] + 4 * g + e;
+            const bool on = (j <= last) & ((j >= from_own) | (j < sink)), some = (j <= keys.hi) & ((j >= from_any) | (j < sink));
+            s[a][e] = on ? s[a][e] : -INFINITY;
+#pragma unroll
+            for (int c = 0; c < H; ++c)
+#pragma unroll
+              for (int w = 0; w < VW; ++w) vx.r[c][4 * a + e][w] = some ? vx.r[c][4 * a + e][w] : 0u;
+            if constexpr (KT == SAH_E4M3) vx.scale[a] = some ? vx.scale[a] : vx.scale[a] & ~(0xffu << (8 * e));  // (0 times the byte 255 is NaN)
+          }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int a = 0; a < NA; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[a][e]);
+      mx = pt_quad_max(mx);
+      // (-inf - -inf is NaN: no rise)
+      if (__ballot((mx - m_run) * c_exp > T::SLACK) != 0) {
+        const float m_new = fmaxf(m_run, mx);
+        const float up = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * c_exp);
+        m_run = m_new;
+        l_run *= up;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[t][e] *= up;
+      }
+      // (Products are compared and subtracted before they are scaled: a product times c_exp, rounded, beside the same unrounded leaves a difference of
+      // its own size where products are large.)
+      const float m_at = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
       for (int a = 0; a < NA; ++a)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int j = SMALL ? s_at[u + 16 * a + 4 * g + e - u0].first : first[a] + 4 * g + e;
-          const bool on = (j <= last) & ((j >= from_own) | (j < sink)), some = (j <= keys.hi) & ((j >= from_any) | (j < sink));
-          s[a][e] = on ? s[a][e] : -INFINITY;
-#pragma unroll
-          for (int c = 0; c < H; ++c)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vx.r[c][4 * a + e][w] = some ? vx.r[c][4 * a + e][w] : 0u;
-          if constexpr (KT == SAH_E4M3) vx.scale[a] = some ? vx.scale[a] : vx.scale[a] & ~(0xffu << (8 * e));  // (0 times the byte 255 is NaN)
+          s[a][e] = __builtin_amdgcn_exp2f(fmaf(s[a][e] - m_at, c_exp, T::SCALE));
+          l_run += s[a][e];
         }
-    }
-    float mx = s[0][0];
+      if constexpr (KT == SAH_F32) {
 #pragma unroll
-    for (int a = 0; a < NA; ++a)
+        for (int a = 0; a < NA; ++a)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[a][e]);
-    mx = pt_quad_max(mx);
-    // (-inf - -inf is NaN: no rise)
-    if (__ballot((mx - m_run) * c_exp > T::SLACK) != 0) {
-      const float m_new = fmaxf(m_run, mx);
-      const float up = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * c_exp);
-      m_run = m_new;
-      l_run *= up;
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int t = 0; t < TILES; ++t)
+            for (int c = 0; c < H; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[t][e] *= up;
-    }
-    // (Products are compared and subtracted before they are scaled: a product times c_exp, rounded, beside the same unrounded leaves a difference of
-    // its own size where products are large.)
-    const float m_at = m_run == -INFINITY ? 0.f : m_run;
+              for (int w = 0; w < NC; ++w) acc[c * NC + w] = pt_mfma_f32(sah_bits_to_float(vx.r[c][4 * a + e][w]), s[a][e], acc[c * NC + w]);
+      } else {
+        uint32_t term[T::NP][4];
+        float rest[8];
 #pragma unroll
-    for (int a = 0; a < NA; ++a)
+        for (int e = 0; e < 8; ++e) rest[e] = s[e / 4][e % 4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[a][e] = __builtin_amdgcn_exp2f(fmaf(s[a][e] - m_at, c_exp, T::SCALE));
-        l_run += s[a][e];
+        for (int i = 0; i < T::NP; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) term[i][k] = pt_term<MT>(rest[2 * k], rest[2 * k + 1]);
+#pragma unroll
+        for (int c = 0; c < H; ++c)
+#pragma unroll
+          for (int pair = 0; pair < NC / 2; ++pair) {
+            uint32_t two[8];  // the pair's dims of the 8 keys
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              if constexpr (KT == SAH_E4M3) {
+                const float scale = pg_scale_of(vx.scale[k / 4], k % 4);
+                two[k] = pair % 2 ? pg_widen2<true>(vx.r[c][k][pair / 2], scale) : pg_widen2<false>(vx.r[c][k][pair / 2], scale);
+              } else {
+                two[k] = vx.r[c][k][pair];
+              }
+            }
+            const uint4 lo = make_uint4(pt_low(two[0], two[1]), pt_low(two[2], two[3]), pt_low(two[4], two[5]), pt_low(two[6], two[7]));
+            const uint4 hi = make_uint4(pt_high(two[0], two[1]), pt_high(two[2], two[3]), pt_high(two[4], two[5]), pt_high(two[6], two[7]));
+#pragma unroll
+            for (int i = 0; i < T::NP; ++i) {
+              const uint4 w = make_uint4(term[i][0], term[i][1], term[i][2], term[i][3]);
+              acc[c * NC + 2 * pair] = sah_mfma_16x16x32<MT>(lo, w, acc[c * NC + 2 * pair]);
+              acc[c * NC + 2 * pair + 1] = sah_mfma_16x16x32<MT>(hi, w, acc[c * NC + 2 * pair + 1]);
+            }
+          }
       }
-    if constexpr (KT == SAH_F32) {
-#pragma unroll
-      for (int a = 0; a < NA; ++a)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int c = 0; c < H; ++c)
-#pragma unroll
-            for (int w = 0; w < NC; ++w) acc[c * NC + w] = pt_mfma_f32(sah_bits_to_float(vx.r[c][4 * a + e][w]), s[a][e], acc[c * NC + w]);
-    } else {
-      uint32_t term[T::NP][4];
-      float rest[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) rest[e] = s[e / 4][e % 4];
-#pragma unroll
-      for (int i = 0; i < T::NP; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) term[i][k] = pt_term<MT>(rest[2 * k], rest[2 * k + 1]);
+      fetch_v(next, vx);
+    };
+    for (; u0 < u_end; u0 += MOST) {  // (uniform; the next one's first key fits 32 bits: the host has checked what a request can have)
+      const int u1 = u_end - u0 < MOST ? u_end : u0 + MOST;
+      if (u0 != u_first) {
+        __syncthreads();  // the places before have been read
+        look_up(u0);
+        __syncthreads();
+      }
+      const int round = STEP * turns;
+      int u = u0 + STEP * turn;
+      if (u >= u1) continue;
+      // Behind a wave's last step it is requested again, from the caches: a way through the loop that skips a request would have the compiler wait
+      // for all of them.
+      const int end = u + (u1 - 1 - u) / round * round;
+      fetch_k(u, kb);
+      fetch_v(u, vb);
+      for (; u < u1; u += round) step(u, u < end ? u + round : end, kb, vb);
+    }
+
+    // the four waves' sums, row by row in LDS
+    l_run = pt_quad_sum(l_run);
+    if (live) {
+      if (g == 0) {
+        s_ml[wave][0][i16] = m_run;
+        s_ml[wave][1][i16] = l_run;
+      }
 #pragma unroll
       for (int c = 0; c < H; ++c)
 #pragma unroll
-        for (int pair = 0; pair < NC / 2; ++pair) {
-          uint32_t two[8];  // the pair's dims of the 8 keys
+        for (int v = 0; v < 4; ++v)
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if constexpr (KT == SAH_E4M3) {
-              const float scale = pg_scale_of(vx.scale[k / 4], k % 4);
-              two[k] = pair % 2 ? pg_widen2<true>(vx.r[c][k][pair / 2], scale) : pg_widen2<false>(vx.r[c][k][pair / 2], scale);
-            } else {
-              two[k] = vx.r[c][k][pair];
-            }
-          }
-          const uint4 lo = make_uint4(pt_low(two[0], two[1]), pt_low(two[2], two[3]), pt_low(two[4], two[5]), pt_low(two[6], two[7]));
-          const uint4 hi = make_uint4(pt_high(two[0], two[1]), pt_high(two[2], two[3]), pt_high(two[4], two[5]), pt_high(two[6], two[7]));
-#pragma unroll
-          for (int i = 0; i < T::NP; ++i) {
-            const uint4 w = make_uint4(term[i][0], term[i][1], term[i][2], term[i][3]);
-            acc[c * NC + 2 * pair] = sah_mfma_16x16x32<MT>(lo, w, acc[c * NC + 2 * pair]);
-            acc[c * NC + 2 * pair + 1] = sah_mfma_16x16x32<MT>(hi, w, acc[c * NC + 2 * pair + 1]);
-          }
-        }
+          for (int e = 0; e < NC; e += 4)
+            *(float4*)&s_acc[wave][i16][(c * 16 + 4 * g + v) * NC + e] =
+                make_float4(acc[c * NC + e][v], acc[c * NC + e + 1][v], acc[c * NC + e + 2][v], acc[c * NC + e + 3][v]);
     }
-    fetch_v(next, vx);
-  };
-  for (; u0 < u_end; u0 += MOST) {  // (uniform; the next one's first key fits 32 bits: the host has checked what a request can have)
-    const int u1 = u_end - u0 < MOST ? u_end : u0 + MOST;
-    if (u0 != u_first) {
-      __syncthreads();  // the places before have been read
-      look_up(u0);
-      __syncthreads();
-    }
-    const int round = STEP * turns;
-    int u = u0 + STEP * turn;
-    if (u >= u1) continue;
-    // Behind a wave's last step it is requested again, from the caches: a way through the loop that skips a request would have the compiler wait
-    // for all of them.
-    const int end = u + (u1 - 1 - u) / round * round;
-    fetch_k(u, kb);
-    fetch_v(u, vb);
-    for (; u < u1; u += round) step(u, u < end ? u + round : end, kb, vb);
-  }
-
-  // the four waves' sums, row by row in LDS
-  l_run = pt_quad_sum(l_run);
-  if (live) {
-    if (g == 0) {
-      s_ml[wave][0][i16] = m_run;
-      s_ml[wave][1][i16] = l_run;
-    }
-#pragma unroll
-    for (int c = 0; c < H; ++c)
-#pragma unroll
-      for (int v = 0; v < 4; ++v)
-#pragma unroll
-        for (int e = 0; e < NC; e += 4)
-          *(float4*)&s_acc[wave][i16][(c * 16 + 4 * g + v) * NC + e] =
-              make_float4(acc[c * NC + e][v], acc[c * NC + e + 1][v], acc[c * NC + e + 2][v], acc[c * NC + e + 3][v]);
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < A.heads * rows * (DP / 4); i += PT_NT) {
-    const int of = i / (DP / 4), d = 4 * (i % (DP / 4)), hh = of / rows, r = of - hh * rows;
-    float m = -INFINITY, l = 0.f;
-    for (int w = hh; w < PT_NW; w += A.heads) m = fmaxf(m, s_ml[w][0][r]);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = hh; w < PT_NW; w += A.heads) {
-      const float mw = s_ml[w][0][r], lw = s_ml[w][1][r], up = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - m) * c_exp);
-      l += lw == lw ? lw * up : lw;  // (a wave whose sum is NaN has no maximum, perhaps)
-      const float4 a = *(const float4*)&s_acc[w][r][d];
-      o.x += a.x * up;
-      o.y += a.y * up;
-      o.z += a.z * up;
-      o.w += a.w * up;
-    }
-    const int rt = t0 + (A.blocks > 1 ? 0 : r / G), rh = (hk0 + hh) * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G);
-    if (!whole) {  // a part: to slot 0 where the tile began before this workgroup's piece, else to slot 1
-      float* to = (float*)P.work + ((((int64_t)w * 2 + (y0 ? 0 : 1)) * A.heads + hh) * PT_ROWS + r) * (DP + 4);
-      if (d == 0) *(float2*)to = make_float2(m, l);
-      *(float4*)(to + 4 + d) = o;
-      continue;
-    }
-    bool fine = l == l;
-    if (P.sinks && m != -INFINITY) l += __builtin_amdgcn_exp2f(fmaf(P.sinks[rh], 1.4426950408889634f, T::SCALE) - m * c_exp);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
-    if (d >= C.D) continue;
-    fine = fine && pt_fine<QT>(o.x) && pt_fine<QT>(o.y) && pt_fine<QT>(o.z) && pt_fine<QT>(o.w);
-    if (!fine) atomicOr(&s_bad, 1ull << (hh * PT_ROWS + r));
-    char* to = (char*)P.out + ((int64_t)rt * P.os_t + (int64_t)rh * P.os_h + d) * pg_size(QT);
-    if (QT == SAH_F32) *(float4*)to = o;
-    else *(uint2*)to = make_uint2(sah_pack2_hw<QT>(o.x, o.y), sah_pack2_hw<QT>(o.z, o.w));
-  }
-  if (whole) {
     __syncthreads();
-    unsigned long long bad = s_bad;  // rows that are not finite are done again, each by a wave
-    for (int i = 0; bad; ++i) {
-      const int hh = __builtin_ctzll(bad) / PT_ROWS, r = __builtin_ctzll(bad) % PT_ROWS;
-      bad &= bad - 1;
-      if (i % PT_NW != wave) continue;
-      pt_row_again<KT, QT>(A, req, t0 + (A.blocks > 1 ? 0 : r / G), (hk0 + hh) * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G));
+    for (int i = threadIdx.x; i < A.heads * rows * (DP / 4); i += PT_NT) {
+      const int of = i / (DP / 4), d = 4 * (i % (DP / 4)), hh = of / rows, r = of - hh * rows;
+      float m = -INFINITY, l = 0.f;
+      for (int w = hh; w < PT_NW; w += A.heads) m = fmaxf(m, s_ml[w][0][r]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = hh; w < PT_NW; w += A.heads) {
+        const float mw = s_ml[w][0][r], lw = s_ml[w][1][r], up = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - m) * c_exp);
+        l += lw == lw ? lw * up : lw;  // (a wave whose sum is NaN has no maximum, perhaps)
+        const float4 a = *(const float4*)&s_acc[w][r][d];
+        o.x += a.x * up;
+        o.y += a.y * up;
+        o.z += a.z * up;
+        o.w += a.w * up;
+      }
+      const int rt = t0 + (A.blocks > 1 ? 0 : r / G), rh = (hk0 + hh) * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G);
+      if (!whole) {  // a part: to slot 0 where the tile began before this workgroup's piece, else to slot 1
+        float* to = (float*)P.work + ((((int64_t)w * 2 + (y0 ? 0 : 1)) * A.heads + hh) * PT_ROWS + r) * (DP + 4);
+        if (d == 0) *(float2*)to = make_float2(m, l);
+        *(float4*)(to + 4 + d) = o;
+        continue;
+      }
+      bool fine = l == l;
+      if (P.sinks && m != -INFINITY) l += __builtin_amdgcn_exp2f(fmaf(P.sinks[rh], 1.4426950408889634f, T::SCALE) - m * c_exp);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+      if (d >= C.D) continue;
+      fine = fine && pt_fine<QT>(o.x) && pt_fine<QT>(o.y) && pt_fine<QT>(o.z) && pt_fine<QT>(o.w);
+      if (!fine) atomicOr(&s_bad, 1ull << (hh * PT_ROWS + r));
+      char* to = (char*)P.out + ((int64_t)rt * P.os_t + (int64_t)rh * P.os_h + d) * pg_size(QT);
+      if (QT == SAH_F32) *(float4*)to = o;
+      else *(uint2*)to = make_uint2(sah_pack2_hw<QT>(o.x, o.y), sah_pack2_hw<QT>(o.z, o.w));
     }
-    if (at.begin + y1 < at.x1) __syncthreads();  // (s_bad has been read)
+    if (!whole && wave == PT_NW - 1) {
+      const pt_shares shares = s_shares;
+      const int64_t key = at.begin + (lane < 32 ? 0 : at.cost.each - 1);
+      int w0, w1;
+      shares.holders(key, key - at.x0, w, w0, w1);
+      pt_record rec{};
+      rec.w0 = w0 > 0 ? (w0 < w ? w0 : w) : 0;
+      rec.parts = (w1 > w ? (w1 < (int)shares.n ? w1 : (int)shares.n - 1) : w) - rec.w0 + 1;
+      rec.t0 = t0; rec.rows = rows; rec.hk0 = hk0; rec.block = block;
+      rec.b = at.b; rec.begin = at.lens.begin; rec.end = at.lens.end; rec.kv = at.lens.kv;
+      if (lane == 0) pt_records(A, gridDim.x, DP, w)[y0 ? 0 : 1] = rec;
+    }
+    left |= whole ? 0 : y0 ? 1 : 2;
+    if (whole) {
+      __syncthreads();
+      unsigned long long bad = s_bad;  // rows that are not finite are done again, each by a wave
+      for (int i = 0; bad; ++i) {
+        const int hh = __builtin_ctzll(bad) / PT_ROWS, r = __builtin_ctzll(bad) % PT_ROWS;
+        bad &= bad - 1;
+        if (i % PT_NW != wave) continue;
+        pt_row_again<KT, QT>(A, req, t0 + (A.blocks > 1 ? 0 : r / G), (hk0 + hh) * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G));
+      }
+      if (at.begin + y1 < at.x1) __syncthreads();  // (s_bad has been read)
+    }
+    x = at.begin + y1;
+    if (x >= at.x1 || !pt_next(pt_arguments(), at)) break;
   }
-  x = at.begin + y1;
-  if (x >= at.x1 || !pt_next(pt_arguments(), at)) break;
-  }
+  if (threadIdx.x < 2 && !(left >> threadIdx.x & 1)) pt_records(pt_arguments(), gridDim.x, DP, w)[threadIdx.x].parts = 0;
 }
 
-// Joins the parts of a tile's rows, a workgroup each tile. DP / 4 lanes hold a row's dims; where a tile has fewer rows than the workgroup has
-// such groups of lanes, a row's parts are shared by several. blockIdx.y: its rows are dealt to as many workgroups.
+// Joins the parts of tiles' rows: the workgroups that had a tile's parts deal its rows out among themselves. DP / 4 lanes hold a row's dims;
+// where a workgroup has fewer rows than such groups of lanes, a row's parts are shared by several.
 template <int KT, int QT, int DP>
-__global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A, int wgs) {
-  sah_touch_kernargs<sizeof(pt_args) + 4>();
+__global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A) {
+  sah_touch_kernargs<sizeof(pt_args)>();
   const sah_page_attention_args& P = A.a;
   const sah_page_cache& C = P.cache;
   typedef pt_types<KT, QT> T;
   constexpr int L = DP / 4, GROUPS = PT_NT / L, U = 8;
   __shared__ __align__(16) float4 s_acc[GROUPS][L];
   __shared__ float2 s_ml[GROUPS];
-  const int lane = threadIdx.x & (SAH_WAVE - 1), l = threadIdx.x % L, group = threadIdx.x / L;
-  const int per_token = C.Hkv * A.blocks, t = (int)(blockIdx.x / per_token), in = (int)blockIdx.x - t * per_token, hk = in % C.Hkv, block = in / C.Hkv;
-  // the token's request, and where its tiles begin on the line
-  int b_of = -1;
-  pt_lens lens{0, 0, 0};
-  int64_t before = 0, total = 0;
-  for (int b0 = 0; b0 < P.requests.n_requests; b0 += SAH_WAVE) {
-    const int b = b0 + lane;
-    pt_lens l{0, 0, 0};
-    if (b < P.requests.n_requests) l = pt_lens_of(P.requests, b);
-    const int64_t c = pt_cost_of(A, l).all();
-    const uint64_t has = __ballot(l.begin >= 0 && t >= l.begin && t < l.end);
-    total += c;
-    if (b_of < 0) {
-      const int at = has ? __builtin_ctzll(has) : SAH_WAVE;
-      before += lane < at ? c : 0;
-      if (has) {
-        b_of = b0 + at;
-        lens = pt_lens{__builtin_amdgcn_readlane(l.begin, at), __builtin_amdgcn_readlane(l.end, at), __builtin_amdgcn_readlane(l.kv, at)};
-      }
-    }
-  }
-  if (b_of < 0) return;
-  const pg_request req = pg_make(P.requests, C.page_size, b_of, lens.begin, lens.end, lens.kv);
-  const int i = t - req.begin;
-  if (i % A.tokens) return;  // not the first of its tile
-  const int G = P.Hq / C.Hkv, n_tok = A.tokens < req.n_new - i ? A.tokens : req.n_new - i;
-  const int all_rows = A.blocks > 1 ? (G - block * PT_ROWS < PT_ROWS ? G - block * PT_ROWS : PT_ROWS) : n_tok * G;
-  const int rows = (all_rows - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;  // this workgroup's
-  if (rows <= 0) return;
-  total = (int64_t)sah_lane_u64(sah_wave_incl_scan_u64((uint64_t)total), SAH_WAVE - 1);
-  before = (int64_t)sah_lane_u64(sah_wave_incl_scan_u64((uint64_t)before), SAH_WAVE - 1);
-  const pt_cost cost = pt_cost_of(A, lens);
-  const int64_t begin = before + (((int64_t)(i / A.tokens) * A.blocks + block) * (C.Hkv / A.heads) + hk / A.heads) * cost.each, end = begin + cost.each;
-  // the workgroups whose pieces hold its first and its last key
-  const pt_shares shares = pt_share(A, total, wgs);
-  const int sharers = (int)shares.n;
-  auto holder = [&](int64_t x) {
-    int w = __builtin_amdgcn_readfirstlane((int)((float)x / (float)total * sharers));
-    w = w < sharers ? w : sharers - 1;
-    while (w + 1 < sharers && shares.bound(w + 1) <= x) ++w;
-    while (w > 0 && shares.bound(w) > x) --w;
-    return w;
-  };
-  const int w0 = holder(begin), w1 = holder(end - 1);
-  if (w0 == w1) return;  // one workgroup's: written
-  const int parts = w1 - w0 + 1;
-  int shared_by = 1;     // groups that share a row
-  while (2 * shared_by * rows <= GROUPS) shared_by *= 2;
+  const int l = threadIdx.x % L, group = threadIdx.x / L, w = pt_number();
+  const pt_record* records = pt_records(A, gridDim.x, DP, w);
+  const pt_record first = records[0], second = records[1];
+  const int G = P.Hq / C.Hkv;
   const float c_exp = pt_log2(P.scaling);
-  const float* from = (const float*)P.work + ((int64_t)w0 * 2 * A.heads + hk % A.heads) * PT_ROWS * (DP + 4);
   float m, sum;
   float4 o;
   auto add = [&](float2 ml, const float4& v) __attribute__((always_inline)) {
@@ -860,54 +852,65 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A, int wgs) {
     o.z = o.z * a + v.z * z;
     o.w = o.w * a + v.w * z;
   };
-  for (int r0 = 0; r0 < rows; r0 += GROUPS / shared_by) {  // uniform
-    const int nth = r0 + group / shared_by, turn = group % shared_by, r = nth * (int)gridDim.y + (int)blockIdx.y;
-    const bool mine = nth < rows;
-    m = -INFINITY;
-    sum = 0.f;
-    o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = turn; mine && p0 < parts; p0 += U * shared_by) {  // several parts requested at once; behind the last one it is taken again, and not added
-      float2 ml[U];
-      float4 v[U];
+  for (int slot = 0; slot < 2; ++slot) {
+    const pt_record rec = slot ? second : first;
+    const int parts = rec.parts, w0 = rec.w0, all_rows = A.heads * rec.rows, nth_part = w - w0;
+    if (nth_part >= all_rows || parts == 0) continue;
+    const int rows = (all_rows - nth_part + parts - 1) / parts;  // this workgroup's: every parts-th
+    int shared_by = 1;     // groups that share a row
+    while (2 * shared_by * rows <= GROUPS) shared_by *= 2;
+    const float* from = (const float*)P.work + (int64_t)w0 * 2 * A.heads * PT_ROWS * (DP + 4);
+    for (int r0 = 0; r0 < rows; r0 += GROUPS / shared_by) {  // uniform
+      const int nth = r0 + group / shared_by, turn = group % shared_by, of_all = nth * parts + nth_part, hh = of_all / rec.rows, r = of_all - hh * rec.rows;
+      const bool mine = nth < rows;
+      m = -INFINITY;
+      sum = 0.f;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int p0 = turn; mine && p0 < parts; p0 += U * shared_by) {  // several parts requested at once; behind the last one it is taken again, and not added
+        float2 ml[U];
+        float4 v[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int of = p0 + i * shared_by < parts ? p0 + i * shared_by : parts - 1;
-        const float* part = from + ((int64_t)(of ? 2 * of : 1) * A.heads * PT_ROWS + r) * (DP + 4);
-        ml[i] = *(const float2*)part;
-        v[i] = *(const float4*)(part + 4 + 4 * l);
-      }
+        for (int i = 0; i < U; ++i) {
+          const int of = p0 + i * shared_by < parts ? p0 + i * shared_by : parts - 1;
+          const float* part = from + (((int64_t)(of ? 2 * of : 1) * A.heads + hh) * PT_ROWS + r) * (DP + 4);
+          ml[i] = *(const float2*)part;
+          v[i] = *(const float4*)(part + 4 + 4 * l);
+        }
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (p0 + i * shared_by < parts) add(ml[i], v[i]);
-    }
-    if (shared_by > 1) {  // (then this is the only round)
-      s_acc[group][l] = o;
-      if (l == 0) s_ml[group] = make_float2(m, sum);
-      __syncthreads();
-      if (mine && turn == 0)
-        for (int i = 1; i < shared_by; ++i) add(s_ml[group + i], s_acc[group + i][l]);
-    }
-    const bool ends = mine && turn == 0;
-    const int rt = t + (A.blocks > 1 ? 0 : r / G), rh = hk * G + (A.blocks > 1 ? block * PT_ROWS + r : r % G), d = 4 * l;
-    bool fine = true;
-    if (ends) {
-      fine = sum == sum;
-      if (P.sinks && m != -INFINITY) sum += __builtin_amdgcn_exp2f(fmaf(P.sinks[rh], 1.4426950408889634f, T::SCALE) - m * c_exp);
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      if (d < C.D) {
-        o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
-        fine = fine && pt_fine<QT>(o.x) && pt_fine<QT>(o.y) && pt_fine<QT>(o.z) && pt_fine<QT>(o.w);
-        char* to = (char*)P.out + ((int64_t)rt * P.os_t + (int64_t)rh * P.os_h + d) * pg_size(QT);
-        if (QT == SAH_F32) *(float4*)to = o;
-        else *(uint2*)to = make_uint2(sah_pack2_hw<QT>(o.x, o.y), sah_pack2_hw<QT>(o.z, o.w));
+        for (int i = 0; i < U; ++i)
+          if (p0 + i * shared_by < parts) add(ml[i], v[i]);
       }
-    }
-    // rows that are not finite are done again, one after the other, by the wave that has them
-    uint64_t again = __ballot(!fine);
-    while (again) {
-      const int at = __builtin_ctzll(again) / L * L;
-      again &= L == SAH_WAVE ? 0ull : ~(((1ull << L) - 1) << at);
-      pt_row_again<KT, QT>(A, req, __builtin_amdgcn_readlane(rt, at), __builtin_amdgcn_readlane(rh, at));
+      if (shared_by > 1) {  // (then this is the only round)
+        __syncthreads();    // (the other slot's have been read)
+        s_acc[group][l] = o;
+        if (l == 0) s_ml[group] = make_float2(m, sum);
+        __syncthreads();
+        if (mine && turn == 0)
+          for (int i = 1; i < shared_by; ++i) add(s_ml[group + i], s_acc[group + i][l]);
+      }
+      const bool ends = mine && turn == 0;
+      const int hk = rec.hk0 + hh, rt = rec.t0 + (A.blocks > 1 ? 0 : r / G), rh = hk * G + (A.blocks > 1 ? rec.block * PT_ROWS + r : r % G), d = 4 * l;
+      bool fine = true;
+      if (ends) {
+        fine = sum == sum;
+        if (P.sinks && m != -INFINITY) sum += __builtin_amdgcn_exp2f(fmaf(P.sinks[rh], 1.4426950408889634f, T::SCALE) - m * c_exp);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        if (d < C.D) {
+          o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+          fine = fine && pt_fine<QT>(o.x) && pt_fine<QT>(o.y) && pt_fine<QT>(o.z) && pt_fine<QT>(o.w);
+          char* to = (char*)P.out + ((int64_t)rt * P.os_t + (int64_t)rh * P.os_h + d) * pg_size(QT);
+          if (QT == SAH_F32) *(float4*)to = o;
+          else *(uint2*)to = make_uint2(sah_pack2_hw<QT>(o.x, o.y), sah_pack2_hw<QT>(o.z, o.w));
+        }
+      }
+      // rows that are not finite are done again, one after the other, by the wave that has them
+      uint64_t again = __ballot(!fine);
+      while (again) {
+        const int at = __builtin_ctzll(again) / L * L;
+        again &= L == SAH_WAVE ? 0ull : ~(((1ull << L) - 1) << at);
+        pt_row_again<KT, QT>(A, pg_make(P.requests, C.page_size, rec.b, rec.begin, rec.end, rec.kv), __builtin_amdgcn_readlane(rt, at),
+                             __builtin_amdgcn_readlane(rh, at));
+      }
     }
   }
 }
@@ -985,7 +988,7 @@ extern "C" int64_t sah_page_attention_work_bytes(const sah_page_attention_args* 
   }
   int wgs;
   const pt_args A = pt_plan(a, wgs);
-  return (int64_t)wgs * 2 * A.heads * PT_ROWS * (pt_dim(a) + 4) * 4;
+  return (int64_t)wgs * 2 * (A.heads * PT_ROWS * (pt_dim(a) + 4) * 4 + (int64_t)sizeof(pt_record));
 }
 
 template <int KT, int QT, int DP>
@@ -998,8 +1001,7 @@ static int pt_launch(const pt_args& A, int wgs) {
     if (int rc = sah_launch_status("sah_page_attention")) return rc;
   }
   sah_timed timed("k_page_attn_join", A.a.stream);
-  const int64_t tiles = (int64_t)A.a.requests.n_tokens * A.a.cache.Hkv * A.blocks;
-  hipLaunchKernelGGL((k_page_attn_join<KT, QT, DP>), dim3((unsigned)tiles, tiles < 2 * PT_CUS ? 4 : 1), dim3(PT_NT), 0, st, A, wgs);
+  hipLaunchKernelGGL((k_page_attn_join<KT, QT, DP>), dim3(wgs), dim3(PT_NT), 0, st, A);
   return sah_launch_status("sah_page_attention(join)");
 }
 template <int KT, int QT>

@@ -650,6 +650,7 @@ extern "C" int sah_page_store(const sah_page_store_args* given) {
 int pg_load(const sah_page_cache& c, const sah_page_requests& r, int dtype, const pg_load_out& out, void* stream, const char* what) {
   const int64_t units = (int64_t)c.D / (c.dtype == SAH_E4M3 ? 8 : 16 / pg_size(c.dtype)) * c.Hkv * out.length, room = PG_LOAD_WGS / r.n_requests;
   int64_t wgs = (units + PG_NT - 1) / PG_NT;
+  if (wgs > INT32_MAX / r.n_requests) return sah_fail(SAH_ESHAPE, "%s: too many elements", what);
   if (wgs > room) wgs = room > 1 ? room : 1;
   sah_timed timed("k_page_load", stream);
   const dim3 grid((unsigned)(wgs * r.n_requests));
