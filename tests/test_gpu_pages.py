@@ -347,9 +347,10 @@ def test_select_scores_that_are_not_finite_come_first(cuda):
 
 # -------------------------------------------------------------------------------------------------------------- attention
 def _attention_case(cuda, dtype, kind, new, cached, q_heads, kv_heads, dim, page, sink=0, window=0, sinks=False, pad=0, seed=0, layout="plain",
-                    missing=(), lists=None, max_context=None, scaling=None, scale=1.0, stride=False):
-    """`lists`: a function (token's last page, rng) -> a token's list of pages."""
+                    missing=(), lists=None, max_context=None, scaling=None, scale=1.0, stride=False, wide=0):
+    """`lists`: a function (token's last page, rng) -> a token's list of pages. `wide`: entries that the table has beyond the requests'."""
     case = Case(cuda, kind, new, cached, kv_heads, dim, page, seed=seed, missing=missing, layout=layout, scale=scale)
+    case.table = torch.cat([case.table, torch.full((len(new), wide), -1, dtype=torch.int32, device=cuda)], 1)
     g, rng = torch.Generator().manual_seed(seed + 7), random.Random(seed)
     tokens, group = case.cu[-1] + pad, q_heads // kv_heads
     q = torch.randn(tokens, q_heads, dim, generator=g).to(dtype)
@@ -529,6 +530,14 @@ def test_attention_8bit_key_heads_side_by_side(cuda, dtype, q_heads, kv_heads):
 def test_attention_8bit_in_many_parts(cuda, dtype):
     """Contexts of thousands of keys at the widest heads, single tokens and a few, beside short ones: tiles that many workgroups share."""
     _attention_case(cuda, dtype, _E4M3, [1, 4, 1], [7001, 3500, 2], 4, 2, 256, 32, sinks=True, seed=8)
+
+
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("dim", [64, 96, 256])
+def test_attention_8bit_in_tables_of_millions_of_keys(cuda, dtype, dim):
+    """Contexts that may be larger than every cache are read past the caches."""
+    _attention_case(cuda, dtype, _E4M3, [1, 1, 1], [3001, 700, 0], 4, 2, dim, 16, sinks=True, seed=dim, wide=2 ** 17)
+    _attention_case(cuda, dtype, _E4M3, [1, 1], [3001, 700], 4, 2, dim, 16, 40, 2 ** 21, seed=dim, wide=2 ** 17)
 
 
 @pytest.mark.parametrize("page, sink, window", [(2048, 0, 0), (4096, 5, 700), (8192, 4100, 33)])
