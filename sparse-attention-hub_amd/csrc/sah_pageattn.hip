@@ -23,14 +23,17 @@
 #define PT_CUS 256
 #define PT_XCDS 8
 #define PT_LAST_CACHE 0x1p28               // bytes
-// In keys: what starting and ending a tile takes, and the least that is worth a workgroup.
+// What starting and ending a tile takes, in keys: how pieces with many tiles are balanced against those with one (256 and 384: within 2 us of 400).
 #define PT_TILE_COST 128
+// The least that is worth a workgroup, in bytes of a key's element: keys of more bytes are worth one sooner. (512 keys of fp32 for each of 8 heads,
+// pieces of 64 keys: 18 us, of 256: 23; 8-bit keys within a window, of 256: 27 us, of 64: 30.)
 #define PT_LEAST 256
 
 struct pt_args {
   sah_page_attention_args a;
   int tokens, blocks;     // tokens of a tile; tiles that a token's query heads of a key head make
   int unit;               // window: keys that begin and end with one
+  int least;              // keys of a key head that are worth a workgroup
   // Key heads that a workgroup works on at once, each by as many of its waves: 4, 2 or 1. Their keys lie side by side (64 answers of 1K to 32K keys, 8
   // heads: 4.9 TB/s one by one, 5.6 so); with a list each has pages of its own, and 1 it is.
   int heads;
@@ -143,7 +146,7 @@ struct pt_shares {
 __device__ __forceinline__ pt_shares pt_share(const pt_args& A, int64_t total, int wgs) {
   const sah_page_attention_args& P = A.a;
   pt_shares s;
-  const int64_t w = (total * A.heads + PT_LEAST - 1) / PT_LEAST;
+  const int64_t w = (total * A.heads + A.least - 1) / A.least;
   s.n = (uint32_t)(w < wgs ? w : wgs);
   // Tiles that are all alike (lists; one request): so many workgroups that no piece holds parts of two. A second tile of a short piece costs as
   // much as the first (1024 keys of 8 heads: 15 -> 9 us).
@@ -928,6 +931,7 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
   A.tokens = a->pages || G >= PT_ROWS ? 1 : PT_ROWS / G;
   A.blocks = (G + PT_ROWS - 1) / PT_ROWS;
   A.unit = a->cache.page_size > PT_STEP ? a->cache.page_size : PT_STEP;
+  A.least = PT_LEAST / pg_size(a->cache.dtype);
   A.heads = a->pages || a->cache.Hkv % 2 ? 1 : a->cache.Hkv % 4 ? 2 : 4;
   // About as many workgroups as the call has work for, at most what the card holds at once. Only how the work is shared depends on it.
   const int64_t table = (int64_t)a->requests.table_width * a->cache.page_size;
@@ -939,7 +943,7 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
     if (a->window && (int64_t)a->sink + a->window + 2 * (int64_t)A.unit < keys) keys = (int64_t)a->sink + a->window + 2 * (int64_t)A.unit;
   }
   const double tiles = ((double)a->requests.n_tokens / A.tokens + (A.tokens > 1 ? a->requests.n_requests : 0)) * A.blocks * a->cache.Hkv;
-  const double n = tiles * (double)(keys + PT_TILE_COST) / PT_LEAST;
+  const double n = tiles * (double)(keys + PT_TILE_COST) / A.least;
   const int most = PT_CUS * pt_per_cu(a->cache.dtype, a->cache.D);
   wgs = n < most ? ((int)n / PT_XCDS + 1) * PT_XCDS : most;
   return A;
