@@ -1,4 +1,6 @@
-// Attention over pages in 8 bits, or over the pages that a list names for each token: few rows a request, so that memory bounds it.
+// Attention over pages in 8 bits, or over the pages that a list names for each token: few rows a request, so that reading keys and values bounds it
+// (64 answers of 1K to 32K 8-bit keys, 8 key heads of 128: 2.2 GB in 384 us, 5.8 TB/s), and where a call is small the time of a workgroup's chain of
+// reads: lengths, table, keys, values (one answer over 1024 listed keys: 11 us, 7 of them before the first product).
 //
 // Of a request's tokens (with a list: of one token) and a key head's query heads every (token, head) is a row; up to 16 are a tile. All
 // tiles of all requests are one line of work, measured in keys; every workgroup takes an equal piece of it, whatever the requests' lengths,
@@ -12,6 +14,7 @@
 // C i .. C i + C - 1 (a key's row is 16 lanes' pieces, one after the other), and a permutation of 16-bit halves inside the lane makes of
 // them the operand of dim C i + e, the output's tile e. 8-bit elements become bf16 on the way, their scale with them, in one instruction a pair: exact.
 // A 32-key step's K is requested as soon as the step before has been multiplied with its own, V likewise: half a step or more is under way at all times.
+// (Two steps ahead: 412 instead of 404 us, lists that several tokens share 85 instead of 59: the registers cost waves.)
 #include "sah_pages.h"
 #include "sah_spans.h"
 
@@ -35,7 +38,7 @@ struct pt_args {
   int unit;               // window: keys that begin and end with one
   int least;              // keys of a key head that are worth a workgroup
   // Key heads that a workgroup works on at once, each by as many of its waves: 4, 2 or 1. Their keys lie side by side (64 answers of 1K to 32K keys, 8
-  // heads: 4.9 TB/s one by one, 5.6 so); with a list each has pages of its own, and 1 it is.
+  // heads: 445 us one by one, 407 so); with a list each has pages of its own, and 1 it is.
   int heads;
 };
 
@@ -149,7 +152,7 @@ __device__ __forceinline__ pt_shares pt_share(const pt_args& A, int64_t total, i
   const int64_t w = (total * A.heads + A.least - 1) / A.least;
   s.n = (uint32_t)(w < wgs ? w : wgs);
   // Tiles that are all alike (lists; one request): so many workgroups that no piece holds parts of two. A second tile of a short piece costs as
-  // much as the first (1024 keys of 8 heads: 15 -> 9 us).
+  // much as the first (1024 listed keys, 8 heads: 15.4 us with pieces as they fall, 11.9 so).
   const pt_cost one = pt_cost_of(A, P.pages ? pt_lens{0, 1, 0x40000000} : pt_lens_of(P.requests, 0));
   if ((P.pages || P.requests.n_requests == 1) && total >= one.each) {
     const int64_t tiles = pg_uniform(pg_div(total, one.each));
@@ -828,8 +831,10 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
   if (threadIdx.x < 2 && !(left >> threadIdx.x & 1)) pt_records(pt_arguments(), gridDim.x, DP, w)[threadIdx.x].parts = 0;
 }
 
-// Joins the parts of tiles' rows: the workgroups that had a tile's parts deal its rows out among themselves. DP / 4 lanes hold a row's dims;
-// where a workgroup has fewer rows than such groups of lanes, a row's parts are shared by several.
+// Joins the parts of tiles' rows: sum over parts of 2^((m_part - m) c) (l, acc), then acc / l. The workgroups that had a tile's parts deal its rows out
+// among themselves; DP / 4 lanes hold a row's dims, and where a workgroup has fewer rows than such groups of lanes, a row's parts are shared by several. Two
+// trips to memory, the record's and the parts' (4 us; 256 parts a row, 32768 keys of one answer: 9.5). A join that finds a tile's place from the
+// lengths takes 2 to 4 us more, one by the last workgroup of a tile would need counters that are zero before the call.
 template <int KT, int QT, int DP>
 __global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A) {
   sah_touch_kernargs<sizeof(pt_args)>();
@@ -949,11 +954,13 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
   return A;
 }
 
-// Chunks of an 8-bit cache: bytes of the copies of K and V and of their table, and the call on them; 0 where the cache is attended to as it is.
+// Chunks of an 8-bit cache: bytes of the copies of K and V and of their table, and the call on them; 0 where the cache is attended to as it is. From some
+// 128 rows a request and key head on a copy for wide tiles is worth its making (32 heads on 8, head_dim 128, us as it is / by a copy: 4 requests of
+// 8192 keys, 64 rows 56 / 72, 128 rows 74 / 84, 256 rows 124 / 99, 512 rows 222 / 137; 2 of 32768, 128 rows 178 / 191, 256 rows 228 / 193).
 static int64_t pt_copy_bytes(const sah_page_attention_args* a) {
   if (a->pages || a->cache.dtype != SAH_E4M3) return 0;
   const int64_t rows = (int64_t)a->requests.n_tokens * (a->Hq / a->cache.Hkv);
-  if (rows <= 32 * (int64_t)a->requests.n_requests) return 0;
+  if (rows <= 128 * (int64_t)a->requests.n_requests) return 0;
   const double pages = (double)a->requests.n_requests * a->requests.table_width;
   const double bytes = pages * a->cache.page_size * a->cache.Hkv * a->cache.D * pg_size(a->dtype) * 2;
   if (bytes > 0x1p33 || pages * 4 > 0x1p33) return 0;

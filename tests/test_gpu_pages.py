@@ -372,7 +372,7 @@ def _attention_case(cuda, dtype, kind, new, cached, q_heads, kv_heads, dim, page
     got = got.double().cpu()
     assert got[case.cu[-1]:].eq(7).all(), "rows behind the last request's were written"
     half = _HALF_STEP[dtype]
-    chunk = pages is None and case.cu[-1] * group > 32 * len(new)
+    chunk = pages is None and tokens * group > 128 * len(new)
     off2 = norm2 = most = 0.0
     for b in range(len(new)):
         keys, there = case.context(b, 0)
@@ -447,13 +447,13 @@ def test_attention_8bit_single_tokens(cuda, dtype, cached):
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
-@pytest.mark.parametrize("new, cached", [([2], [0]), ([9, 8, 7], [1, 0, 64]), ([33], [100]), ([65, 1], [0, 300]), ([150], [17])])
+@pytest.mark.parametrize("new, cached", [([2], [0]), ([9, 8, 7], [1, 0, 64]), ([33], [100]), ([65, 1], [0, 300]), ([150], [17]), ([32, 32], [500, 0])])
 def test_attention_8bit_chunks(cuda, dtype, new, cached):
     _attention_case(cuda, dtype, _E4M3, new, cached, 8, 2, 64, 16, seed=sum(new), pad=1)
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
-@pytest.mark.parametrize("new", [[1, 4], [70, 9]])
+@pytest.mark.parametrize("new", [[1, 4], [70, 9], [150, 9]])
 @pytest.mark.parametrize("sink, window", [(0, 1), (0, 64), (1, 1), (4, 63), (128, 100), (100, 100000), (5000, 7)])
 def test_attention_8bit_sink_and_window(cuda, dtype, new, sink, window):
     for page in (8, 64):
@@ -461,7 +461,7 @@ def test_attention_8bit_sink_and_window(cuda, dtype, new, sink, window):
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
-@pytest.mark.parametrize("new", [[1, 1, 2], [40, 1, 2]])
+@pytest.mark.parametrize("new", [[1, 1, 2], [40, 1, 2], [210, 1, 2]])
 def test_attention_8bit_sink_logits_and_missing_pages(cuda, dtype, new):
     _attention_case(cuda, dtype, _E4M3, new, [300, 20, 0], 4, 2, 64, 16, sinks=True, missing=[(0, 2, -1), (0, 5, 10 ** 6), (1, 0, -3), (1, 1, -1), (2, 0, -1)], seed=3)
 
@@ -579,7 +579,7 @@ def test_pages_of_many_requests(cuda, n):
 
 # ------------------------------------------------------------------------------------------------------ what is not finite
 @pytest.mark.parametrize("dtype", _TYPES)
-@pytest.mark.parametrize("new", [[1, 3], [1, 60]])
+@pytest.mark.parametrize("new", [[1, 3], [1, 60], [1, 140]])
 def test_attention_8bit_values_that_are_not_finite_stay_where_they_are_seen(cuda, dtype, new):
     """NaN on a page's unused end, behind a row's position, on a page of another request: no row sees it. In a visible value: that channel
     of the rows that see it, in a visible key: all channels."""
@@ -602,7 +602,7 @@ def test_attention_8bit_values_that_are_not_finite_stay_where_they_are_seen(cuda
 
 @pytest.mark.parametrize("byte", [0, 255])
 @pytest.mark.parametrize("page", [4, 16, 64])
-@pytest.mark.parametrize("new", [[1, 3], [1, 60]])
+@pytest.mark.parametrize("new", [[1, 3], [1, 60], [1, 140]])
 def test_attention_8bit_scales_of_keys_that_no_row_sees(cuda, new, page, byte):
     """Entries that hold no token yet may hold anything, their scales too: a call on a cache where those differ gives the same bits."""
     case = Case(cuda, _E4M3, new, [100, 21], 2, 64, page, seed=6)
