@@ -104,9 +104,9 @@ int sah_page_select(const sah_page_select_args* a);
  * position are hidden also on the pages that are named. With pages there is no window. All else is as there, sinks, rows without a key, rows behind the last
  * request's and what out may share memory with. A row that comes out not finite is done again key by key.
  * Logits, softmax statistics and sums are fp32; q of more than bf16's bits and weights enter 16-bit products as several terms: as
- * exact as the result's own rounding. Chunks of an 8-bit cache (more than 128 rows of q a request and key head on average, and no more than 8 GiB of
- * work) are attended to through a copy of the contexts in q's type in work, by sah_paged_attention's kernels and with what it
- * says of weights. work: sah_page_attention_work_bytes(a) bytes, 16-byte aligned, no particular content. */
+ * exact as the result's own rounding. Chunks of an 8-bit cache under 16-bit q (more than 128 rows of q a request
+ * and key head on average, with a window as many times more as the table has keys beyond it, and no more than 8 GiB of work) are attended to through a
+ * copy of the contexts in q's type in work, by sah_paged_attention's kernels and with what it says of weights. work: sah_page_attention_work_bytes(a) bytes, 16-byte aligned, no particular content. */
 typedef struct sah_page_attention_args {
   const void* q; int64_t qs_t, qs_h;
   sah_page_cache cache;

@@ -954,13 +954,17 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
   return A;
 }
 
-// Chunks of an 8-bit cache: bytes of the copies of K and V and of their table, and the call on them; 0 where the cache is attended to as it is. From some
-// 128 rows a request and key head on a copy for wide tiles is worth its making (32 heads on 8, head_dim 128, us as it is / by a copy: 4 requests of
-// 8192 keys, 64 rows 56 / 72, 128 rows 74 / 84, 256 rows 124 / 99, 512 rows 222 / 137; 2 of 32768, 128 rows 178 / 191, 256 rows 228 / 193).
+// Chunks of an 8-bit cache: bytes of the copies of K and V and of their table, and the call on them; 0 where the cache is attended to as it is. A copy
+// for wide tiles costs some 1.2 ns a key (8 heads of 128), and saves 8 ps for each row and key that it sees: worth it from 128 rows or so a request and key
+// head on, with a window from so many times the context as it hides (32 heads on 8, us as it is / by a copy: 4 requests of 8192 keys, 64 rows 56 / 72,
+// 128 rows 74 / 84, 256 rows 124 / 99, 512 rows 222 / 137; of those keys 512 + 128 seen, 1024 rows 56 / 70, 4096 rows 191 / 129; 2 requests of
+// 32768, 2048 + 128 seen, 1024 rows 84 / 129, 4096 rows 248 / 175). Never for fp32 q: its terms go at the 16-bit matrix rate here, an fp32 copy at a
+// tenth of it (4 requests of 8192 keys, 128 rows 80 / 268, 2048 rows 947 / 2952).
 static int64_t pt_copy_bytes(const sah_page_attention_args* a) {
-  if (a->pages || a->cache.dtype != SAH_E4M3) return 0;
-  const int64_t rows = (int64_t)a->requests.n_tokens * (a->Hq / a->cache.Hkv);
-  if (rows <= 128 * (int64_t)a->requests.n_requests) return 0;
+  if (a->pages || a->cache.dtype != SAH_E4M3 || a->dtype == SAH_F32) return 0;
+  const double keys = (double)a->requests.table_width * a->cache.page_size, reach = (double)a->sink + a->window, seen = a->window && reach < keys ? reach : keys;
+  const double rows = (double)a->requests.n_tokens * (a->Hq / a->cache.Hkv);
+  if (rows * seen <= 128 * keys * a->requests.n_requests) return 0;
   const double pages = (double)a->requests.n_requests * a->requests.table_width;
   const double bytes = pages * a->cache.page_size * a->cache.Hkv * a->cache.D * pg_size(a->dtype) * 2;
   if (bytes > 0x1p33 || pages * 4 > 0x1p33) return 0;

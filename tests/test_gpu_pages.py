@@ -372,7 +372,8 @@ def _attention_case(cuda, dtype, kind, new, cached, q_heads, kv_heads, dim, page
     got = got.double().cpu()
     assert got[case.cu[-1]:].eq(7).all(), "rows behind the last request's were written"
     half = _HALF_STEP[dtype]
-    chunk = pages is None and tokens * group > 128 * len(new)
+    context = case.table.shape[1] * page
+    chunk = pages is None and tokens * group * (min(context, sink + window) if window else context) > 128 * len(new) * context
     off2 = norm2 = most = 0.0
     for b in range(len(new)):
         keys, there = case.context(b, 0)
@@ -458,6 +459,13 @@ def test_attention_8bit_chunks(cuda, dtype, new, cached):
 def test_attention_8bit_sink_and_window(cuda, dtype, new, sink, window):
     for page in (8, 64):
         _attention_case(cuda, dtype, _E4M3, new, [700, 130], 4, 2, 64, page, sink, window, seed=sink + window)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sink, window", [(0, 200), (128, 300), (7, 33)])
+def test_attention_8bit_long_chunks_under_a_window(cuda, dtype, sink, window):
+    """Rows enough for a copy of the contexts, and (the last one) not enough for what the window hides of them."""
+    _attention_case(cuda, dtype, _E4M3, [600], [300], 4, 2, 64, 16, sink, window, sinks=True, seed=window)
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
