@@ -802,6 +802,41 @@ def test_a_captured_step(cuda, kind):
     assert torch.equal(graphed.lens, eager.lens)
 
 
+@pytest.mark.parametrize("dtype", _TYPES)
+def test_a_captured_chunk_and_its_context_read_back(cuda, dtype):
+    """A chunk over 8-bit pages (in 16-bit types through a copy) and the contexts as tensors, replayed on other caches, tables and lengths between
+    eager calls."""
+    cases = [Case(cuda, _E4M3, [200], [n], 2, 64, 16, seed=n) for n in (1100, 1098, 1105)]
+    live = [x.clone() for x in (cases[0].caches[0].view(torch.uint8), cases[0].caches[1].view(torch.uint8), cases[0].scales[0].view(torch.uint8),
+                                cases[0].scales[1].view(torch.uint8), cases[0].table, cases[0].kv_lens)]
+    q = torch.randn(200, 4, 64, generator=torch.Generator().manual_seed(3)).to(dtype).to(cuda)
+
+    def calls(keys, values, key_scales, value_scales, table, kv_lens):
+        held = dict(key_scales=key_scales.view(_E8M0), value_scales=value_scales.view(_E8M0))
+        caches = (keys.view(_E4M3), values.view(_E4M3))
+        return (P.paged_attention(q, *caches, table, kv_lens, cases[0].cu_new, 0.125, **held), *P.load_paged(*caches, table, kv_lens, 1400, dtype=dtype, **held))
+
+    stream = torch.cuda.Stream(cuda)
+    stream.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(stream):
+        calls(*live)
+    torch.cuda.current_stream(cuda).wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls(*live)
+    for i in range(9):
+        case = cases[i % 3]
+        given = [case.caches[0].view(torch.uint8), case.caches[1].view(torch.uint8), case.scales[0].view(torch.uint8), case.scales[1].view(torch.uint8),
+                 case.table, case.kv_lens]
+        for to, x in zip(live, given):
+            to.copy_(x)
+        graph.replay()
+        want = calls(*live)
+        torch.cuda.synchronize(cuda)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), i
+
+
 def test_two_streams_at_once(cuda):
     """Calls on two streams share nothing."""
     cases = [Case(cuda, _E4M3, [1, 2], [3000, 500], 2, 64, 16, seed=s) for s in (1, 2)]
