@@ -7,7 +7,7 @@
 
 // ---------------------------------------------------------------------------
 // store: 16 lanes hold a row (token, key head) of both matrices, 8 elements each (16 beyond 128 dims)
-// Memory bounds it: 16384 tokens of 8 heads of 128 in bf16, 101 MB, 27.6 us (a large copy's rate: 21). Keys and values by one thread, so that the slot is
+// Memory bounds it: 16384 tokens of 8 heads of 128 in bf16, 101 MB, 24 us (a large copy's rate: 21). Keys and values by one thread, so that the slot is
 // read once and twice as many loads are under way: by a thread each 30.1 us.
 // ---------------------------------------------------------------------------
 // exponent of the scale of a row whose largest magnitude is `most`: the least e >= -110 with most <= 448 * 2^e = 1.75 * 2^(e + 8)
@@ -86,39 +86,47 @@ __global__ __launch_bounds__(PG_NT) void k_page_store(sah_page_store_args P) {
 
 // ---------------------------------------------------------------------------
 // load: a thread holds 8 elements of the cache (8-bit: what 16 bytes of a 16-bit result take) or 16 bytes of it (others: copied as they are)
-// Memory bounds it: 24575 tokens of 8 heads of 128 in four contexts of up to 8192, 50 MB, to bf16, 134 MB with the zeros: 35 us, 5.2 TB/s. 16 elements a
-// thread: 36.4.
+// Memory bounds it: 24575 tokens of 8 heads of 128 in four contexts of up to 8192, 50 MB, to bf16, 134 MB with the zeros: 29 us, 6.5 TB/s. Twice as many
+// elements a thread: 1.5 us more.
 // ---------------------------------------------------------------------------
+// 16 bytes of a result: past the L2 where it is the caller's (ONCE), of which it would hold a small part and displace what the next kernel reads (24575 tokens
+// read back 29 us, through it 35; the store after it 24, 28), through it where the attention reads it next.
+template <bool ONCE>
+__device__ __forceinline__ void pg_put16(char* to, sah_u4 x) {
+  if constexpr (ONCE) __builtin_nontemporal_store(x, (sah_u4*)to);
+  else *(sah_u4*)to = x;
+}
 // what 8 elements of e4m3 are in type T, stored at `to`
-template <int T>
+template <int T, bool ONCE>
 __device__ __forceinline__ void pg_put8(char* to, uint2 x, float scale) {
   if constexpr (T == SAH_BF16) {
-    *(uint4*)to = make_uint4(pg_widen2<false>(x.x, scale), pg_widen2<true>(x.x, scale), pg_widen2<false>(x.y, scale), pg_widen2<true>(x.y, scale));
+    pg_put16<ONCE>(to, sah_u4{pg_widen2<false>(x.x, scale), pg_widen2<true>(x.x, scale), pg_widen2<false>(x.y, scale), pg_widen2<true>(x.y, scale)});
   } else {
     float f[2][4];
     pg_widen4(x.x, scale, f[0]);
     pg_widen4(x.y, scale, f[1]);
     if constexpr (T == SAH_F32) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) ((float4*)to)[i] = make_float4(f[i][0], f[i][1], f[i][2], f[i][3]);
+      for (int i = 0; i < 2; ++i)
+        pg_put16<ONCE>(to + 16 * i, sah_u4{sah_float_to_bits(f[i][0]), sah_float_to_bits(f[i][1]), sah_float_to_bits(f[i][2]), sah_float_to_bits(f[i][3])});
     } else {
       // (a row's largest may have been rounded up past the type's; NaN stays)
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i / 4][i % 4] = f[i / 4][i % 4] > 65504.f ? 65504.f : (f[i / 4][i % 4] < -65504.f ? -65504.f : f[i / 4][i % 4]);
-      *(uint4*)to = make_uint4(sah_pack2_hw<SAH_F16>(f[0][0], f[0][1]), sah_pack2_hw<SAH_F16>(f[0][2], f[0][3]), sah_pack2_hw<SAH_F16>(f[1][0], f[1][1]),
-                               sah_pack2_hw<SAH_F16>(f[1][2], f[1][3]));
+      pg_put16<ONCE>(to, sah_u4{sah_pack2_hw<SAH_F16>(f[0][0], f[0][1]), sah_pack2_hw<SAH_F16>(f[0][2], f[0][3]), sah_pack2_hw<SAH_F16>(f[1][0], f[1][1]),
+                                sah_pack2_hw<SAH_F16>(f[1][2], f[1][3])});
     }
   }
 }
 // CT: type of the cache; OT: of the output (other caches than SAH_E4M3: the same). `wgs` workgroups a request, which go through its tokens in
-// turn: what lies behind a context in a table of a hundred thousand tokens costs a copy nothing.
-template <int CT, int OT>
+// turn: what lies behind a context in a table of a hundred thousand tokens costs a copy nothing. COPY: for the attention, with a table.
+template <int CT, int OT, bool COPY>
 __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_requests R, pg_load_out O, int wgs) {
   sah_touch_kernargs<sizeof(sah_page_cache) + sizeof(sah_page_requests) + sizeof(pg_load_out) + 4>();
   constexpr int CS = pg_size(CT), OS = pg_size(OT), E = CT == SAH_E4M3 ? 8 : 16 / CS;  // elements of a unit
   const uint32_t units = C.D / E, unit_h = units * C.Hkv, stride = (uint32_t)wgs * PG_NT, stride_t = stride / unit_h, stride_in = stride - stride_t * unit_h;
   const int shift = 31 - __builtin_clz(C.page_size), b = (int)blockIdx.x / wgs, kv = R.kv_lens[b];
-  const uint32_t n = O.table && kv < O.length ? (kv > 0 ? kv : 0) : O.length, first = (blockIdx.x - (uint32_t)b * wgs) * PG_NT + threadIdx.x;
+  const uint32_t n = COPY && kv < O.length ? (kv > 0 ? kv : 0) : O.length, first = (blockIdx.x - (uint32_t)b * wgs) * PG_NT + threadIdx.x;
   // consecutive threads: a token's units, all heads of it, then the next token: as the cache lies
   uint32_t at = first / unit_h, in = first - at * unit_h;
   for (; at < n; at += stride_t, in += stride_in) {
@@ -130,27 +138,32 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
     const int j = t >> shift, entry = t & (C.page_size - 1);
     const int page = t < kv && j < R.table_width ? R.block_table[(int64_t)b * R.table_pitch + j] : -1;
     const bool there = page >= 0 && page < C.n_pages;
-    if (O.table && entry == 0 && in == 0) O.table[(int64_t)b * R.table_width + j] = there ? b * R.table_width + j : -1;
-    if (O.table && !there) continue;
+    if (COPY && entry == 0 && in == 0) O.table[(int64_t)b * R.table_width + j] = there ? b * R.table_width + j : -1;
+    if (COPY && !there) continue;
     const int64_t to = (b * O.s_b + h * O.s_h + t * O.s_t + (int64_t)c * E) * OS;
     char *ko = (char*)O.k + to, *vo = (char*)O.v + to;
-    if (!there) {
-#pragma unroll
-      for (int i = 0; i < E * OS / 16; ++i) ((uint4*)ko)[i] = ((uint4*)vo)[i] = make_uint4(0, 0, 0, 0);
-      continue;
-    }
     const char* kp = (const char*)C.k + (page * C.ks_p + entry * C.ks_t + h * C.ks_h + c * E) * CS;
     const char* vp = (const char*)C.v + (page * C.vs_p + entry * C.vs_t + h * C.vs_h + c * E) * CS;
     if constexpr (CT == SAH_E4M3) {
-      const uint2 k = *(const uint2*)kp, v = *(const uint2*)vp;
-      const int64_t s = ((int64_t)page * C.Hkv + h) * C.page_size + entry;
-      const float ks = pg_scale(C.k_scales[s]), vs = pg_scale(C.v_scales[s]);
-      pg_put8<OT>(ko, k, ks);
-      pg_put8<OT>(vo, v, vs);
+      uint2 k = make_uint2(0, 0), v = k;
+      float ks = 1.f, vs = 1.f;
+      if (there) {
+        const int64_t s = ((int64_t)page * C.Hkv + h) * C.page_size + entry;
+        k = *(const uint2*)kp;
+        v = *(const uint2*)vp;
+        ks = pg_scale(C.k_scales[s]);
+        vs = pg_scale(C.v_scales[s]);
+      }
+      pg_put8<OT, !COPY>(ko, k, ks);
+      pg_put8<OT, !COPY>(vo, v, vs);
     } else {
-      const uint4 k = *(const uint4*)kp, v = *(const uint4*)vp;
-      *(uint4*)ko = k;
-      *(uint4*)vo = v;
+      sah_u4 k = {0, 0, 0, 0}, v = k;
+      if (there) {
+        k = *(const sah_u4*)kp;
+        v = *(const sah_u4*)vp;
+      }
+      pg_put16<!COPY>(ko, k);
+      pg_put16<!COPY>(vo, v);
     }
   }
 }
@@ -665,11 +678,13 @@ int pg_load(const sah_page_cache& c, const sah_page_requests& r, int dtype, cons
   sah_timed timed("k_page_load", stream);
   const dim3 grid((unsigned)(wgs * r.n_requests));
   hipStream_t st = (hipStream_t)stream;
-  if (c.dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_F32, SAH_F32>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
-  else if (c.dtype != SAH_E4M3) hipLaunchKernelGGL((k_page_load<SAH_BF16, SAH_BF16>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
-  else if (dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F32>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
-  else if (dtype == SAH_BF16) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_BF16>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
-  else hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F16>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  if (c.dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_F32, SAH_F32, false>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else if (c.dtype != SAH_E4M3) hipLaunchKernelGGL((k_page_load<SAH_BF16, SAH_BF16, false>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else if (dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F32, false>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else if (out.table && dtype == SAH_BF16) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_BF16, true>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else if (out.table) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F16, true>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else if (dtype == SAH_BF16) hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_BF16, false>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
+  else hipLaunchKernelGGL((k_page_load<SAH_E4M3, SAH_F16, false>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
   return sah_launch_status(what);
 }
 
