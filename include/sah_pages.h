@@ -37,7 +37,7 @@ typedef struct sah_page_requests {
 } sah_page_requests;
 
 /* Quantises row t of keys and values [n_tokens, Hkv, D] (dtype) into slot slot_map[t] of a SAH_E4M3 cache, the scales with it. Slots outside the cache
- * are passed over; two rows of one slot: which one it holds is not defined. */
+ * are passed over; two rows of one slot: which one it holds is not defined. Rows and slots share no memory with the cache. */
 typedef struct sah_page_store_args {
   sah_page_cache cache;
   const void* k; int64_t ks_t, ks_h;
@@ -82,7 +82,8 @@ int sah_page_bounds(const sah_page_bounds_args* a);
  * their ranks do not hang on the order of a sum; one that is not finite ranks above all others. Pages that the table does not have are no
  * candidates. pages [n_tokens, Hkv, n_select]: places in the request's row of the table, rising, -1 behind the last; -1 alone for rows behind the
  * last request's. Only bounds of candidates that are not taken anyway are read. sink_pages + window_pages <= n_select, window_pages >= 1.
- * Addresses and strides of q and bounds are multiples of 16 bytes. max_context: as for sah_paged_attention. work: sah_page_select_work_bytes(a) bytes, 16-byte aligned, no particular content. */
+ * Addresses and strides of q and bounds are multiples of 16 bytes. max_context: as for sah_paged_attention. work: sah_page_select_work_bytes(a) bytes,
+ * 16-byte aligned, no particular content. */
 typedef struct sah_page_select_args {
   const void* q; int64_t qs_t, qs_h;
   const void* bounds;
@@ -106,7 +107,8 @@ int sah_page_select(const sah_page_select_args* a);
  * Logits, softmax statistics and sums are fp32; q of more than bf16's bits and weights enter 16-bit products as several terms: as
  * exact as the result's own rounding. Chunks of an 8-bit cache under 16-bit q (more than 128 rows of q a request
  * and key head on average, with a window as many times more as the table has keys beyond it, and no more than 8 GiB of work) are attended to through a
- * copy of the contexts in q's type in work, by sah_paged_attention's kernels and with what it says of weights. work: sah_page_attention_work_bytes(a) bytes, 16-byte aligned, no particular content. */
+ * copy of the contexts in q's type in work, by sah_paged_attention's kernels and with what it says of weights. work:
+ * sah_page_attention_work_bytes(a) bytes, 16-byte aligned, no particular content. */
 typedef struct sah_page_attention_args {
   const void* q; int64_t qs_t, qs_h;
   sah_page_cache cache;

@@ -86,8 +86,8 @@ __global__ __launch_bounds__(PG_NT) void k_page_store(sah_page_store_args P) {
 
 // ---------------------------------------------------------------------------
 // load: a thread holds 8 elements of the cache (8-bit: what 16 bytes of a 16-bit result take) or 16 bytes of it (others: copied as they are)
-// Memory bounds it: 24575 tokens of 8 heads of 128 in four contexts of up to 8192, 50 MB, to bf16, 134 MB with the zeros: 29 us, 6.5 TB/s. Twice as many
-// elements a thread: 1.5 us more.
+// Memory bounds it: 24575 tokens of 8 heads of 128 in four contexts of up to 8192, 50 MB, to bf16, 134 MB with the zeros: 29 us, 6.5 TB/s. (Written
+// through the L2: 33.8, with 16 elements a thread 36.4.)
 // ---------------------------------------------------------------------------
 // 16 bytes of a result: past the L2 where it is the caller's (ONCE), of which it would hold a small part and displace what the next kernel reads (24575 tokens
 // read back 29 us, through it 35; the store after it 24, 28), through it where the attention reads it next.

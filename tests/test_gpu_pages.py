@@ -585,6 +585,46 @@ def test_pages_of_many_requests(cuda, n):
     _select_case(cuda, torch.bfloat16, torch.bfloat16, new, cached, 4, 2, 16, 8, 6, seed=n, pad=2)
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, _E4M3])
+def test_a_batch_of_padding_alone(cuda, kind):
+    """Rows, but no request that has one: nothing is written, nothing selected."""
+    if kind == _E4M3:
+        _attention_case(cuda, torch.bfloat16, kind, [0, 0], [20, 3], 4, 2, 64, 16, pad=3)
+        _attention_case(cuda, torch.bfloat16, kind, [0], [500], 4, 2, 64, 16, pad=200)
+    _attention_case(cuda, torch.bfloat16, kind, [0, 0], [20, 3], 4, 2, 64, 16, pad=3, lists=_some_pages)
+    _select_case(cuda, torch.bfloat16, kind, [0, 0], [20, 3], 4, 2, 64, 16, 4, pad=3)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, _E4M3])
+def test_lengths_that_no_table_holds(cuda, kind):
+    """A length below its new tokens, or below 0: rows that see nothing. One beyond the table: as the table's."""
+    case = Case(cuda, kind, [1, 2, 1], [47, 46, 30], 2, 64, 16, seed=5)
+    q = torch.randn(4, 4, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(cuda)
+    bounds = torch.zeros(case.caches[0].shape[0], 2, 2, 64, dtype=torch.bfloat16, device=cuda)
+    for b in range(3):
+        P.update_page_bounds(bounds, case.caches[0], case.table[b:b + 1], case.kv_lens[b:b + 1], _i32([0, 100], cuda), key_scales=case.scales[0])
+    lists = _i32([[[0, 1, 2, 3]] * 2] * 4, cuda)
+
+    def calls(kv_lens):
+        kv_lens = _i32(kv_lens, cuda)
+        out = [P.paged_attention(q, *case.caches, case.table, kv_lens, case.cu_new, 0.125, pages=lists, **case.held)]
+        if kind == _E4M3:
+            out += [P.paged_attention(q, *case.caches, case.table, kv_lens, case.cu_new, 0.125, **case.held, **o) for o in ({}, dict(sink_size=3, window_size=9))]
+        return out, P.select_pages(q, bounds, case.table, kv_lens, case.cu_new, 16, 3)
+
+    most = case.width * 16
+    (usual, chosen), (odd, odd_chosen) = calls([most, 1, 31]), calls([10 ** 9, -7, 31])
+    assert odd_chosen[1:3].eq(-1).all() and torch.equal(odd_chosen[[0, 3]], chosen[[0, 3]]) and chosen[1].eq(-1).all()
+    for i, (a, b) in enumerate(zip(usual, odd)):
+        assert b[1:3].eq(0).all() and a[1].eq(0).all() and torch.isfinite(a).all()
+        if i < 2:  # (a window lies at the row's position)
+            # Pieces of the work may end elsewhere, so sums are made in another order: each is off by (2 n + 16) 2^-24 and its weights by 2^-16 of the
+            # largest value, and a result may then round to the neighbour, 2^-7 of itself away.
+            x, y = a[[0, 3]].double().cpu(), b[[0, 3]].double().cpu()
+            off = 2 * ((2 * most + 16) * 2.0 ** -24 + 2.0 ** -16) * float(case.wide[1].abs().max())
+            assert ((x - y).abs() <= 2.0 ** -7 * torch.maximum(x.abs(), y.abs()) + off).all()
+
+
 # ------------------------------------------------------------------------------------------------------ what is not finite
 @pytest.mark.parametrize("dtype", _TYPES)
 @pytest.mark.parametrize("new", [[1, 3], [1, 60], [1, 140]])
