@@ -37,8 +37,9 @@ struct pt_args {
   int tokens, blocks;     // tokens of a tile; tiles that a token's query heads of a key head make
   int unit;               // window: keys that begin and end with one
   int least;              // keys of a key head that are worth a workgroup
-  // Key heads that a workgroup works on at once, each by as many of its waves: 4, 2 or 1. Their keys lie side by side (64 answers of 1K to 32K keys, 8
-  // heads: 445 us one by one, 407 so); with a list each has pages of its own, and 1 it is.
+  // Key heads that a workgroup works on at once, each by as many of its waves: 4, 2 or 1. Their keys lie side by side, which memory rewards (64
+  // answers of 1K to 32K keys, 8 heads: 445 us one by one, 407 by 4; 32 of 4K to 8K: 106 by 1, 97 by 2, 94 by 4); the fewer, the fewer parts
+  // there are to join (one answer of 32K keys: 32.1 us by 4, 27.6 by 2, 26.7 by 1; of 128K: 70.5, 66.8, 71.9). With a list each has pages of its own, and 1 it is.
   int heads;
 };
 
@@ -833,7 +834,7 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
 
 // Joins the parts of tiles' rows: sum over parts of 2^((m_part - m) c) (l, acc), then acc / l. The workgroups that had a tile's parts deal its rows out
 // among themselves; DP / 4 lanes hold a row's dims, and where a workgroup has fewer rows than such groups of lanes, a row's parts are shared by several. Two
-// trips to memory, the record's and the parts' (4 us; 256 parts a row, 32768 keys of one answer: 9.5). A join that finds a tile's place from the
+// trips to memory, the record's and the parts' (4 us; 128 parts a row, 32768 keys of one answer: 6.4). A join that finds a tile's place from the
 // lengths takes 2 to 4 us more, one by the last workgroup of a tile would need counters that are zero before the call.
 template <int KT, int QT, int DP>
 __global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A) {
@@ -929,6 +930,14 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A) {
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
+// What the contexts' keys and values may come to, by what the caller says
+static double pt_context_bytes(const sah_page_attention_args& a) {
+  double keys = (double)a.requests.table_width * a.cache.page_size;
+  if (a.max_context > 0 && a.max_context < keys) keys = a.max_context;
+  if (a.window && (double)a.sink + a.window < keys) keys = (double)a.sink + a.window;
+  return keys * a.requests.n_requests * a.cache.Hkv * a.cache.D * 2 * pg_size(a.cache.dtype);
+}
+
 static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
   pt_args A;
   A.a = *a;
@@ -937,7 +946,7 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
   A.blocks = (G + PT_ROWS - 1) / PT_ROWS;
   A.unit = a->cache.page_size > PT_STEP ? a->cache.page_size : PT_STEP;
   A.least = PT_LEAST / pg_size(a->cache.dtype);
-  A.heads = a->pages || a->cache.Hkv % 2 ? 1 : a->cache.Hkv % 4 ? 2 : 4;
+  A.heads = a->pages || a->cache.Hkv % 2 ? 1 : a->cache.Hkv % 4 || pt_context_bytes(*a) <= PT_LAST_CACHE ? 2 : 4;
   // About as many workgroups as the call has work for, at most what the card holds at once. Only how the work is shared depends on it.
   const int64_t table = (int64_t)a->requests.table_width * a->cache.page_size;
   int64_t keys = table;
@@ -1015,10 +1024,7 @@ extern "C" int64_t sah_page_attention_work_bytes(const sah_page_attention_args* 
 static bool pt_once(const pt_args& A) {
   const sah_page_attention_args& a = A.a;
   if (a.pages || A.blocks > 1 || a.requests.n_tokens > (int64_t)a.requests.n_requests * A.tokens) return false;
-  double keys = (double)a.requests.table_width * a.cache.page_size;
-  if (a.max_context > 0 && a.max_context < keys) keys = a.max_context;
-  if (a.window && (double)a.sink + a.window < keys) keys = (double)a.sink + a.window;
-  return keys * a.requests.n_requests * a.cache.Hkv * a.cache.D * 2 > PT_LAST_CACHE * 2;
+  return pt_context_bytes(a) > PT_LAST_CACHE * 2;
 }
 
 template <int KT, int QT, int DP>

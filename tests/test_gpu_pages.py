@@ -529,9 +529,11 @@ def test_attention_over_pages_head_groups(cuda, q_heads, kv_heads):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("q_heads, kv_heads", [(3, 3), (8, 4), (10, 5), (6, 6), (16, 8), (24, 12), (34, 2)])
-def test_attention_8bit_key_heads_side_by_side(cuda, dtype, q_heads, kv_heads):
-    """Workgroups work on four, two or one of the key heads at once."""
-    _attention_case(cuda, dtype, _E4M3, [1, 2], [900, 40], q_heads, kv_heads, 64, 16, sinks=True, seed=kv_heads)
+@pytest.mark.parametrize("wide", [0, 2 ** 14, 2 ** 17])
+def test_attention_8bit_key_heads_side_by_side(cuda, dtype, q_heads, kv_heads, wide):
+    """Workgroups work on two or one of the key heads at once, on four where contexts may be larger than a cache."""
+    _attention_case(cuda, dtype, _E4M3, [1, 2], [900, 40], q_heads, kv_heads, 64, 16, sinks=True, seed=kv_heads, wide=wide)
+    _attention_case(cuda, dtype, _E4M3, [3, 1, 1], [70, 900, 0], q_heads, kv_heads, 64, 8, seed=kv_heads, wide=wide)
 
 
 @pytest.mark.parametrize("dtype", _TYPES)
