@@ -833,7 +833,8 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
 }
 
 // Joins the parts of tiles' rows: sum over parts of 2^((m_part - m) c) (l, acc), then acc / l. The workgroups that had a tile's parts deal its rows out
-// among themselves; DP / 4 lanes hold a row's dims, and where a workgroup has fewer rows than such groups of lanes, a row's parts are shared by several. Two
+// among themselves; DP / 4 lanes hold a row's dims, and where a workgroup has fewer rows than such groups of lanes, a row's parts are shared by several. blockIdx.y: the
+// tile that began before the workgroup's piece, or the one that ends behind it. Two
 // trips to memory, the record's and the parts' (4 us; 128 parts a row, 32768 keys of one answer: 6.4). A join that finds a tile's place from the
 // lengths takes 2 to 4 us more, one by the last workgroup of a tile would need counters that are zero before the call.
 template <int KT, int QT, int DP>
@@ -846,8 +847,13 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A) {
   __shared__ __align__(16) float4 s_acc[GROUPS][L];
   __shared__ float2 s_ml[GROUPS];
   const int l = threadIdx.x % L, group = threadIdx.x / L, w = pt_number();
-  const pt_record* records = pt_records(A, gridDim.x, DP, w);
-  const pt_record first = records[0], second = records[1];
+  const pt_record rec = pt_records(A, gridDim.x, DP, w)[blockIdx.y];
+  const int parts = rec.parts, w0 = rec.w0, all_rows = A.heads * rec.rows, nth_part = w - w0;
+  if (parts == 0 || nth_part >= all_rows) return;
+  const int rows = (all_rows - nth_part + parts - 1) / parts;  // this workgroup's: every parts-th
+  int shared_by = 1;     // groups that share a row
+  while (2 * shared_by * rows <= GROUPS) shared_by *= 2;
+  const float* from = (const float*)P.work + (int64_t)w0 * 2 * A.heads * PT_ROWS * (DP + 4);
   const int G = P.Hq / C.Hkv;
   const float c_exp = pt_log2(P.scaling);
   float m, sum;
@@ -864,65 +870,55 @@ __global__ __launch_bounds__(PT_NT) void k_page_attn_join(pt_args A) {
     o.z = o.z * a + v.z * z;
     o.w = o.w * a + v.w * z;
   };
-  for (int slot = 0; slot < 2; ++slot) {
-    const pt_record rec = slot ? second : first;
-    const int parts = rec.parts, w0 = rec.w0, all_rows = A.heads * rec.rows, nth_part = w - w0;
-    if (nth_part >= all_rows || parts == 0) continue;
-    const int rows = (all_rows - nth_part + parts - 1) / parts;  // this workgroup's: every parts-th
-    int shared_by = 1;     // groups that share a row
-    while (2 * shared_by * rows <= GROUPS) shared_by *= 2;
-    const float* from = (const float*)P.work + (int64_t)w0 * 2 * A.heads * PT_ROWS * (DP + 4);
-    for (int r0 = 0; r0 < rows; r0 += GROUPS / shared_by) {  // uniform
-      const int nth = r0 + group / shared_by, turn = group % shared_by, of_all = nth * parts + nth_part, hh = of_all / rec.rows, r = of_all - hh * rec.rows;
-      const bool mine = nth < rows;
-      m = -INFINITY;
-      sum = 0.f;
-      o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int p0 = turn; mine && p0 < parts; p0 += U * shared_by) {  // several parts requested at once; behind the last one it is taken again, and not added
-        float2 ml[U];
-        float4 v[U];
+  for (int r0 = 0; r0 < rows; r0 += GROUPS / shared_by) {  // uniform
+    const int nth = r0 + group / shared_by, turn = group % shared_by, of_all = nth * parts + nth_part, hh = of_all / rec.rows, r = of_all - hh * rec.rows;
+    const bool mine = nth < rows;
+    m = -INFINITY;
+    sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = turn; mine && p0 < parts; p0 += U * shared_by) {  // several parts requested at once; behind the last one it is taken again, and not added
+      float2 ml[U];
+      float4 v[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) {
-          const int of = p0 + i * shared_by < parts ? p0 + i * shared_by : parts - 1;
-          const float* part = from + (((int64_t)(of ? 2 * of : 1) * A.heads + hh) * PT_ROWS + r) * (DP + 4);
-          ml[i] = *(const float2*)part;
-          v[i] = *(const float4*)(part + 4 + 4 * l);
-        }
+      for (int i = 0; i < U; ++i) {
+        const int of = p0 + i * shared_by < parts ? p0 + i * shared_by : parts - 1;
+        const float* part = from + (((int64_t)(of ? 2 * of : 1) * A.heads + hh) * PT_ROWS + r) * (DP + 4);
+        ml[i] = *(const float2*)part;
+        v[i] = *(const float4*)(part + 4 + 4 * l);
+      }
 #pragma unroll
-        for (int i = 0; i < U; ++i)
-          if (p0 + i * shared_by < parts) add(ml[i], v[i]);
+      for (int i = 0; i < U; ++i)
+        if (p0 + i * shared_by < parts) add(ml[i], v[i]);
+    }
+    if (shared_by > 1) {  // (then this is the only round)
+      s_acc[group][l] = o;
+      if (l == 0) s_ml[group] = make_float2(m, sum);
+      __syncthreads();
+      if (mine && turn == 0)
+        for (int i = 1; i < shared_by; ++i) add(s_ml[group + i], s_acc[group + i][l]);
+    }
+    const bool ends = mine && turn == 0;
+    const int hk = rec.hk0 + hh, rt = rec.t0 + (A.blocks > 1 ? 0 : r / G), rh = hk * G + (A.blocks > 1 ? rec.block * PT_ROWS + r : r % G), d = 4 * l;
+    bool fine = true;
+    if (ends) {
+      fine = sum == sum;
+      if (P.sinks && m != -INFINITY) sum += __builtin_amdgcn_exp2f(fmaf(P.sinks[rh], 1.4426950408889634f, T::SCALE) - m * c_exp);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      if (d < C.D) {
+        o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+        fine = fine && pt_fine<QT>(o.x) && pt_fine<QT>(o.y) && pt_fine<QT>(o.z) && pt_fine<QT>(o.w);
+        char* to = (char*)P.out + ((int64_t)rt * P.os_t + (int64_t)rh * P.os_h + d) * pg_size(QT);
+        if (QT == SAH_F32) *(float4*)to = o;
+        else *(uint2*)to = make_uint2(sah_pack2_hw<QT>(o.x, o.y), sah_pack2_hw<QT>(o.z, o.w));
       }
-      if (shared_by > 1) {  // (then this is the only round)
-        __syncthreads();    // (the other slot's have been read)
-        s_acc[group][l] = o;
-        if (l == 0) s_ml[group] = make_float2(m, sum);
-        __syncthreads();
-        if (mine && turn == 0)
-          for (int i = 1; i < shared_by; ++i) add(s_ml[group + i], s_acc[group + i][l]);
-      }
-      const bool ends = mine && turn == 0;
-      const int hk = rec.hk0 + hh, rt = rec.t0 + (A.blocks > 1 ? 0 : r / G), rh = hk * G + (A.blocks > 1 ? rec.block * PT_ROWS + r : r % G), d = 4 * l;
-      bool fine = true;
-      if (ends) {
-        fine = sum == sum;
-        if (P.sinks && m != -INFINITY) sum += __builtin_amdgcn_exp2f(fmaf(P.sinks[rh], 1.4426950408889634f, T::SCALE) - m * c_exp);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        if (d < C.D) {
-          o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
-          fine = fine && pt_fine<QT>(o.x) && pt_fine<QT>(o.y) && pt_fine<QT>(o.z) && pt_fine<QT>(o.w);
-          char* to = (char*)P.out + ((int64_t)rt * P.os_t + (int64_t)rh * P.os_h + d) * pg_size(QT);
-          if (QT == SAH_F32) *(float4*)to = o;
-          else *(uint2*)to = make_uint2(sah_pack2_hw<QT>(o.x, o.y), sah_pack2_hw<QT>(o.z, o.w));
-        }
-      }
-      // rows that are not finite are done again, one after the other, by the wave that has them
-      uint64_t again = __ballot(!fine);
-      while (again) {
-        const int at = __builtin_ctzll(again) / L * L;
-        again &= L == SAH_WAVE ? 0ull : ~(((1ull << L) - 1) << at);
-        pt_row_again<KT, QT>(A, pg_make(P.requests, C.page_size, rec.b, rec.begin, rec.end, rec.kv), __builtin_amdgcn_readlane(rt, at),
-                             __builtin_amdgcn_readlane(rh, at));
-      }
+    }
+    // rows that are not finite are done again, one after the other, by the wave that has them
+    uint64_t again = __ballot(!fine);
+    while (again) {
+      const int at = __builtin_ctzll(again) / L * L;
+      again &= L == SAH_WAVE ? 0ull : ~(((1ull << L) - 1) << at);
+      pt_row_again<KT, QT>(A, pg_make(P.requests, C.page_size, rec.b, rec.begin, rec.end, rec.kv), __builtin_amdgcn_readlane(rt, at),
+                           __builtin_amdgcn_readlane(rh, at));
     }
   }
 }
@@ -1038,7 +1034,7 @@ static int pt_launch(const pt_args& A, int wgs) {
     if (int rc = sah_launch_status("sah_page_attention")) return rc;
   }
   sah_timed timed("k_page_attn_join", A.a.stream);
-  hipLaunchKernelGGL((k_page_attn_join<KT, QT, DP>), dim3(wgs), dim3(PT_NT), 0, st, A);
+  hipLaunchKernelGGL((k_page_attn_join<KT, QT, DP>), dim3(wgs, 2), dim3(PT_NT), 0, st, A);
   return sah_launch_status("sah_page_attention(join)");
 }
 template <int KT, int QT>
