@@ -3,8 +3,8 @@
 // reads: lengths, table, keys, values (one answer over 1024 listed keys: 11 us, 7 of them before the first product).
 //
 // Of a request's tokens (with a list: of one token) and a key head's query heads every (token, head) is a row; up to 16 are a tile. All
-// tiles of all requests are one line of work, measured in keys; every workgroup takes an equal piece of it, whatever the requests' lengths,
-// finds its place from the lengths on the device, and works through tiles and parts of tiles. A part's (m, l, acc) goes to the workspace, a second
+// tiles of all requests are one line of work, measured in keys; every workgroup takes an equal piece of it, whatever the requests' lengths (where there is
+// little work, a piece of one tile), finds its place from the lengths on the device, and works through tiles and parts of tiles. A part's (m, l, acc) goes to the workspace, a second
 // kernel joins the parts of a row.
 //
 // The four waves of a workgroup take 32 keys of a tile in turn. Nothing is staged: keys and values
@@ -28,6 +28,9 @@
 #define PT_LAST_CACHE 0x1p28               // bytes
 // What starting and ending a tile takes, in keys: how pieces with many tiles are balanced against those with one (256 and 384: within 2 us of 400).
 #define PT_TILE_COST 128
+// Keys a workgroup below which every tile is cut by itself (16 answers of 1K to 2K keys 29.9 -> 24.9 us, drafts within a window 24.1 -> 19.6; what decides
+// it costs other calls 0.6 us). Beyond, the balance of equal pieces is worth more (8 answers of 8192 keys, 520 a workgroup: 36.4 us against 39.3).
+#define PT_FEW 512
 // The least that is worth a workgroup, in bytes of a key's element: keys of more bytes are worth one sooner. (512 keys of fp32 for each of 8 heads,
 // pieces of 64 keys: 18 us, of 256: 23; 8-bit keys within a window, of 256: 27 us, of 64: 30.)
 #define PT_LEAST 256
@@ -125,7 +128,7 @@ __device__ __forceinline__ pt_cost pt_cost_of(const pt_args& A, const pt_lens& l
   int64_t n = (int64_t)kv - end + last;  // keys up to the last row's position
   const int64_t most = (int64_t)R.table_width * P.cache.page_size;
   if (P.pages) {
-    n = n > 0 ? (int64_t)P.n_select * P.cache.page_size : 0;
+    n = (int64_t)P.n_select * P.cache.page_size;  // (the same for all tiles: pt_start counts on it)
   } else {
     n = n < most ? n : most;
     if (P.window && (int64_t)P.sink + P.window + 2 * (int64_t)A.unit < n) n = (int64_t)P.sink + P.window + 2 * (int64_t)A.unit;
@@ -137,6 +140,7 @@ __device__ __forceinline__ pt_cost pt_cost_of(const pt_args& A, const pt_lens& l
 struct pt_shares {
   int64_t each;
   uint32_t n, rest;
+  int w0, parts;  // parts > 0: the piece is one of so many of a tile, the first of them workgroup w0's
   __device__ __forceinline__ int64_t bound(int w) const { return each * w + rest * (uint32_t)w / n; }  // (n is at most 1024)
   // Whose piece has key x, `away` from where w's begins: asked for two keys at once, by the halves of a wave, whose lanes try a piece each. (The
   // guess is off by one at most: pieces differ by one key.)
@@ -148,19 +152,12 @@ struct pt_shares {
   }
 };
 __device__ __forceinline__ pt_shares pt_share(const pt_args& A, int64_t total, int wgs) {
-  const sah_page_attention_args& P = A.a;
   pt_shares s;
   const int64_t w = (total * A.heads + A.least - 1) / A.least;
   s.n = (uint32_t)(w < wgs ? w : wgs);
-  // Tiles that are all alike (lists; one request): so many workgroups that no piece holds parts of two. A second tile of a short piece costs as
-  // much as the first (1024 listed keys, 8 heads: 15.4 us with pieces as they fall, 11.9 so).
-  const pt_cost one = pt_cost_of(A, P.pages ? pt_lens{0, 1, 0x40000000} : pt_lens_of(P.requests, 0));
-  if ((P.pages || P.requests.n_requests == 1) && total >= one.each) {
-    const int64_t tiles = pg_uniform(pg_div(total, one.each));
-    if (tiles * one.each == total && tiles < s.n) s.n -= s.n % (uint32_t)tiles;
-  }
   s.each = s.n ? pg_uniform(pg_div(total, s.n)) : 0;
   s.rest = (uint32_t)(total - s.each * s.n);
+  s.w0 = s.parts = 0;
   return s;
 }
 // Neighbours on the line share keys' cache lines (scales, and what lies between two heads), so they get the same XCD.
@@ -174,68 +171,107 @@ struct pt_place {
   pt_cost cost;
   int64_t x0, x1;  // the workgroup's piece
 };
-// s_sum: PT_NW + 3 words; s_shares: how the line is shared. All threads call. False: no piece.
+// Cost of a piece where no piece holds parts of two tiles, or 0 where pieces are equal. A second tile costs a workgroup as much as its first one's start, some 7
+// us, so calls of little work a workgroup cut every tile by itself, and those whose tiles are alike or few do, which lose no balance by it. At most
+// `wgs` pieces: total / target + tiles.
+__device__ __forceinline__ int64_t pt_target(const pt_args& A, int64_t total, int64_t tiles, int wgs) {
+  if (tiles == 0 || tiles > wgs) return 0;
+  const int64_t least = A.least / A.heads, room = wgs - tiles, target = room ? pg_uniform(pg_div(total + room - 1, room)) : total;
+  if (!A.a.pages && A.a.requests.n_requests > 1 && tiles * 16 >= wgs && target > PT_FEW) return 0;
+  return target > least ? target : least;
+}
+// s_sum: 2 PT_NW + 3 words; s_shares: how the line is shared. All threads call. False: no piece.
 __device__ __forceinline__ bool pt_start(const pt_args& A, int w, int wgs, int64_t* s_sum, pt_shares& s_shares, pt_place& at) {
   const sah_page_requests& R = A.a.requests;
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
-  auto scan = [&](int64_t v, int64_t& all) -> int64_t {  // inclusive
-    const int64_t incl = (int64_t)sah_wave_incl_scan_u64((uint64_t)v);
+  // inclusive sum of v, and the sums of v and u over all threads
+  auto scan = [&](int64_t v, int64_t u, int64_t& all, int64_t& all_u) -> int64_t {
+    const int64_t incl = (int64_t)sah_wave_incl_scan_u64((uint64_t)v), incl_u = (int64_t)sah_wave_incl_scan_u64((uint64_t)u);
     __syncthreads();
-    if (lane == SAH_WAVE - 1) s_sum[wave] = incl;
+    if (lane == SAH_WAVE - 1) {
+      s_sum[wave] = incl;
+      s_sum[PT_NW + wave] = incl_u;
+    }
     __syncthreads();
     int64_t before = 0;
-    all = 0;
+    all = all_u = 0;
 #pragma unroll
     for (int i = 0; i < PT_NW; ++i) {
       before += i < wave ? s_sum[i] : 0;
       all += s_sum[i];
+      all_u += s_sum[PT_NW + i];
     }
     all = pg_uniform(all);
+    all_u = pg_uniform(all_u);
     return before + incl;
   };
   pt_lens lens{0, 0, 0};
-  auto cost_of = [&](int b) -> int64_t {
-    if (b >= R.n_requests) return 0;
+  auto cost_of = [&](int b) -> pt_cost {
+    if (b >= R.n_requests) return pt_cost{PT_TILE_COST, 0};
     lens = pt_lens_of(R, b);
-    return pt_cost_of(A, lens).all();
+    return pt_cost_of(A, lens);
   };
-  auto share = [&](int64_t total) {
-    const pt_shares s = pt_share(A, total, wgs);
-    at.x0 = w < (int)s.n ? s.bound(w) : 0;
-    at.x1 = w < (int)s.n ? s.bound(w + 1) : 0;
-    if (threadIdx.x == 0) s_shares = s;
-  };
-  auto claim = [&](int b, int64_t mine, int64_t end) {  // one thread's request holds x0
-    if (mine && end > at.x0 && end - mine <= at.x0) {
-      s_sum[PT_NW] = (int64_t)lens.kv << 32 | (uint32_t)b;
-      s_sum[PT_NW + 1] = end - mine;
-      s_sum[PT_NW + 2] = (int64_t)lens.end << 32 | (uint32_t)lens.begin;
-    }
-  };
-  int64_t total;
-  if (R.n_requests <= PT_NT) {
-    const int64_t mine = cost_of(threadIdx.x), end = scan(mine, total);
-    share(total);
-    claim(threadIdx.x, mine, end);
-  } else {
-    int64_t sum = 0, run = 0, all;
-    for (int b = threadIdx.x; b < R.n_requests; b += PT_NT) sum += cost_of(b);
-    (void)scan(sum, total);
-    share(total);
-    for (int b0 = 0; b0 < R.n_requests; b0 += PT_NT) {
-      const int64_t mine = cost_of(b0 + threadIdx.x), end = run + scan(mine, all);
-      claim(b0 + threadIdx.x, mine, end);
-      run += all;
-    }
+  // requests' costs and tiles, then where each one's pieces begin (of a line in keys, or in pieces), PT_NT requests at a time
+  int64_t total = 0, tiles = 0, unused;
+  pt_cost c{PT_TILE_COST, 0};
+  for (int b = threadIdx.x; b < R.n_requests; b += PT_NT) {
+    c = cost_of(b);
+    total += c.all();
+    tiles += c.tiles;
   }
+  if (threadIdx.x == 0) s_sum[2 * PT_NW] = -1;
+  const int64_t end_0 = scan(total, tiles, total, tiles);
+  const int64_t target = pt_target(A, total, tiles, wgs);
+  at.x0 = w;
+  if (!target) {
+    const pt_shares shares = pt_share(A, total, wgs);
+    if (w >= (int)shares.n) return false;
+    at.x0 = shares.bound(w);
+    at.x1 = shares.bound(w + 1);
+    if (threadIdx.x == 0) s_shares = shares;
+  }
+  int64_t run = 0;
+  const bool alike = (A.a.pages || R.n_requests == 1) && tiles > 0;
+  const int64_t each = alike ? pg_uniform(pg_div(total, tiles)) : 0;
+  for (int b0 = 0; b0 < R.n_requests; b0 += PT_NT) {
+    const int b = b0 + (int)threadIdx.x;
+    if (R.n_requests > PT_NT) c = cost_of(b);
+    const int64_t k = target ? pg_div((alike ? each : c.each) + target - 1, target) : 1, mine = target ? c.tiles * k : c.all();
+    int64_t all = 0, end = end_0;
+    if (R.n_requests > PT_NT || (target && !alike)) {
+      end = run + scan(mine, 0, all, unused);
+    } else if (target) {  // tiles of one cost: the first scan tells them, too
+      end = pg_div(end_0, each) * k;
+      all = tiles * pg_uniform(k);
+    }
+    if (mine && end > at.x0 && end - mine <= at.x0) {  // one thread's request holds x0
+      s_sum[2 * PT_NW] = (int64_t)lens.kv << 32 | (uint32_t)b;
+      s_sum[2 * PT_NW + 1] = end - mine;
+      s_sum[2 * PT_NW + 2] = (int64_t)lens.end << 32 | (uint32_t)lens.begin;
+    }
+    run += all;
+  }
+  if (target && w >= run) return false;
   __syncthreads();
-  if (at.x0 >= at.x1) return false;
-  const int64_t own = pg_uniform(s_sum[PT_NW]), begin = pg_uniform(s_sum[PT_NW + 1]), rows = pg_uniform(s_sum[PT_NW + 2]);
+  const int64_t own = pg_uniform(s_sum[2 * PT_NW]), begin = pg_uniform(s_sum[2 * PT_NW + 1]), rows = pg_uniform(s_sum[2 * PT_NW + 2]);
   at.b = (int)own;
+  if (at.b < 0) return false;  // (lengths changed under way: a program's error, but one that ends)
   at.lens = pt_lens{(int)rows, (int)(rows >> 32), (int)(own >> 32)};
   at.cost = pt_cost_of(A, at.lens);
-  at.tile = pg_uniform(pg_div(at.x0 - begin, at.cost.each));
-  at.begin = begin + at.tile * at.cost.each;
+  if (target) {
+    const int k = (int)pg_uniform(pg_div(at.cost.each + target - 1, target)), nth = w - (int)begin, tile = nth / k, part = nth - tile * k;
+    at.tile = tile;
+    at.begin = 0;
+    at.x0 = pg_uniform(pg_div(at.cost.each * part, k));
+    at.x1 = pg_uniform(pg_div(at.cost.each * (part + 1), k));
+    if (threadIdx.x == 0) {
+      s_shares.w0 = w - part;
+      s_shares.parts = k;
+    }
+  } else {
+    at.tile = pg_uniform(pg_div(at.x0 - begin, at.cost.each));
+    at.begin = begin + at.tile * at.cost.each;
+  }
   return true;
 }
 // The next tile on the line; there is one, unless lengths changed under way (an error of the program's, but one that ends)
@@ -417,7 +453,7 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
   __shared__ __align__(16) float s_acc[PT_NW][PT_ROWS][PITCH];
   __shared__ float s_ml[PT_NW][2][PT_ROWS];
   __shared__ unsigned long long s_bad;  // a bit a head and row
-  __shared__ int64_t s_sum[PT_NW + 3];
+  __shared__ int64_t s_sum[2 * PT_NW + 3];
   __shared__ pt_shares s_shares;
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id(), i16 = lane & 15, g = lane >> 4;
   const int w = pt_number();
@@ -805,11 +841,11 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
     if (!whole && wave == PT_NW - 1) {
       const pt_shares shares = s_shares;
       const int64_t key = at.begin + (lane < 32 ? 0 : at.cost.each - 1);
-      int w0, w1;
-      shares.holders(key, key - at.x0, w, w0, w1);
+      int w0 = shares.w0, w1 = shares.w0 + shares.parts - 1;
+      if (shares.parts == 0) shares.holders(key, key - at.x0, w, w0, w1);
       pt_record rec{};
       rec.w0 = w0 > 0 ? (w0 < w ? w0 : w) : 0;
-      rec.parts = (w1 > w ? (w1 < (int)shares.n ? w1 : (int)shares.n - 1) : w) - rec.w0 + 1;
+      rec.parts = (w1 > w ? (w1 < (int)gridDim.x ? w1 : (int)gridDim.x - 1) : w) - rec.w0 + 1;
       rec.t0 = t0; rec.rows = rows; rec.hk0 = hk0; rec.block = block;
       rec.b = at.b; rec.begin = at.lens.begin; rec.end = at.lens.end; rec.kv = at.lens.kv;
       if (lane == 0) pt_records(A, gridDim.x, DP, w)[y0 ? 0 : 1] = rec;
