@@ -31,8 +31,8 @@
 // Keys a workgroup below which every tile is cut by itself (16 answers of 1K to 2K keys 29.9 -> 24.9 us, drafts within a window 24.1 -> 19.6; what decides
 // it costs other calls 0.6 us). Beyond, the balance of equal pieces is worth more (8 answers of 8192 keys, 520 a workgroup: 36.4 us against 39.3).
 #define PT_FEW 512
-// The least that is worth a workgroup, in bytes of a key's element: keys of more bytes are worth one sooner. (512 keys of fp32 for each of 8 heads,
-// pieces of 64 keys: 18 us, of 256: 23; 8-bit keys within a window, of 256: 27 us, of 64: 30.)
+// The least that is worth a workgroup, in keys of one byte an element: wider ones are worth one sooner. (272 listed fp32 keys a token, 2 key heads: pieces
+// of 64 keys 18 us, of 256 23; 8-bit drafts within a window: of 256 keys 27 us, of 64 30.)
 #define PT_LEAST 256
 
 struct pt_args {
