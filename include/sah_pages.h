@@ -78,7 +78,8 @@ int sah_page_bounds(const sah_page_bounds_args* a);
 /* The pages that a token attends to, for each key head h: of those at or before its own position's page, which are its candidates,
  * the first sink_pages and the last window_pages (its own is the last one), and of the others, up to n_select in all, those of the largest
  *     score(page) = sum over h's query heads and over channels c of max(q_c * smallest_c, q_c * largest_c),
- * ties to the lower page. (What is summed over c is the largest q . k that a key of the page can reach.) Scores are held in 64 bits, so that
+ * ties to the lower page. (What is summed over c is the largest q . k that a key of the page can reach. An infinite bound counts where its product is the larger
+ * one; 0 times it is no number.) Scores are held in 64 bits, so that
  * their ranks do not hang on the order of a sum; one that is not finite ranks above all others. Pages that the table does not have are no
  * candidates. pages [n_tokens, Hkv, n_select]: places in the request's row of the table, rising, -1 behind the last; -1 alone for rows behind the
  * last request's. Only bounds of candidates that are not taken anyway are read. sink_pages + window_pages <= n_select, window_pages >= 1.

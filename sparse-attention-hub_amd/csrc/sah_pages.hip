@@ -291,8 +291,8 @@ __global__ __launch_bounds__(PG_NT) void k_page_bounds(sah_page_bounds_args P, i
 
 // ---------------------------------------------------------------------------
 // select: a 64-bit key per candidate (larger: rather taken), then the largest of a row
-// The sum over heads of max(q a, q b) with a <= b is Q+ . b + Q- . a, Q+ (Q-) the sum of the heads' positive (negative) elements: the heads share one
-// reading of the bounds and one pair of products. In fp64, so that no order of sums changes a rank; fp32 is no faster (72 us against 70): reading the
+// The sum over heads of max(q a, q b) with a <= b, both finite, is Q+ . b + Q- . a, Q+ (Q-) the sum of the heads' positive (negative) elements: the heads
+// share one reading of the bounds and one pair of products (pages of infinite bounds: pg_score_again). In fp64, so that no order of sums changes a rank; fp32 is no faster (72 us against 70): reading the
 // bounds is what it costs. 64 answers of 1K to 32K keys in pages of 16, 8 heads: 277 MB of bf16 bounds, 61 us, 4.5 TB/s; they are read past the caches, which
 // they would go through once (71 us). All heads of a page by one wave 97 us, smallest and largest by neighbouring lanes 80.
 // ---------------------------------------------------------------------------
@@ -336,9 +336,39 @@ struct pg_select {
   int chunks;   // workgroups a row, which take its pages in turn
 };
 
+__device__ __forceinline__ float pg_load_as(int dtype, const void* p, int64_t i) {
+  return dtype == SAH_F32 ? sah_load<SAH_F32>(p, i) : dtype == SAH_BF16 ? sah_load<SAH_BF16>(p, i) : sah_load<SAH_F16>(p, i);
+}
+// The score of a page by a whole wave, for those whose sum of Q+ . max + Q- . min is not finite: an infinite smallest element counts only where
+// some head is not positive, a largest one where some head is not negative. Elsewhere the larger product is the other one, not 0 times infinity.
+__device__ __forceinline__ double pg_score_again(const sah_page_select_args& P, int64_t t, int h, int page) {
+  const int lane = threadIdx.x & (SAH_WAVE - 1), G = P.Hq / P.Hkv;
+  const int64_t q = t * P.qs_t + (int64_t)h * G * P.qs_h, b = ((int64_t)page * P.Hkv + h) * 2 * P.D;
+  double sum = 0.0;
+#pragma unroll 1
+  for (int d = lane; d < P.D; d += SAH_WAVE) {
+    double up = 0.0, down = 0.0;
+    bool positive = true, negative = true;  // all heads
+#pragma unroll 1
+    for (int i = 0; i < G; ++i) {
+      const float x = pg_load_as(P.dtype, P.q, q + i * P.qs_h + d);
+      up += x < 0.f ? 0.0 : (double)x;
+      down += x < 0.f ? (double)x : 0.0;
+      positive &= x > 0.f;
+      negative &= x < 0.f;
+    }
+    const float lo = pg_load_as(P.bounds_dtype, P.bounds, b + d), hi = pg_load_as(P.bounds_dtype, P.bounds, b + P.D + d);
+    if (!(positive && fabsf(lo) == INFINITY)) sum = fma(down, (double)lo, sum);
+    if (!(negative && fabsf(hi) == INFINITY)) sum = fma(up, (double)hi, sum);
+  }
+#pragma unroll
+  for (int i = 1; i < SAH_WAVE; i *= 2) sum += __shfl_xor(sum, i);
+  return sum;
+}
+
 // BT: type of the bounds, DP: D up to 64, 128 or 256. L lanes hold a page's row of bounds, E elements of each of the two.
 template <int BT, int DP>
-__global__ __launch_bounds__(PG_NT) void k_page_scores(pg_select S) {
+__global__ __launch_bounds__(PG_NT, (BT == SAH_F32 || DP <= 128 ? 4 : 3)) void k_page_scores(pg_select S) {
   sah_touch_kernargs<sizeof(pg_select)>();
   const sah_page_select_args& P = S.a;
   const sah_page_requests& R = P.requests;
@@ -383,6 +413,7 @@ __global__ __launch_bounds__(PG_NT) void k_page_scores(pg_select S) {
   }
   uint64_t* keys = (uint64_t*)P.work + row * S.pitch;
   const char* base = (const char*)P.bounds + (int64_t)h * 2 * P.D * ES;
+  bool odd = false;  // a score that is not finite
   for (int64_t from = (chunk * NW + wave) * PG_WAVE_PAGES; from < n; from += (int64_t)S.chunks * NW * PG_WAVE_PAGES) {
     // a lane's page
     const int j0 = (int)from, j = j0 + lane;
@@ -436,10 +467,19 @@ __global__ __launch_bounds__(PG_NT) void k_page_scores(pg_select S) {
         if constexpr (L >= 32) sum += __shfl_xor(sum, 16);
         if constexpr (L >= 64) sum += __shfl_xor(sum, 32);
         const int to = j0 + i0 + i * AT_ONCE + who;
+        odd |= !(sum - sum == 0.0);
         if (in == 0 && at[i] >= 0 && to < n) keys[to] = pg_key(sum);
       }
     }
     if (mine && (always || page < 0)) keys[j] = page < 0 ? 0 : PG_ALWAYS;
+    if (!__ballot(odd)) continue;
+    odd = false;
+    for (int i = 0; i < PG_WAVE_PAGES && j0 + i < n; ++i) {
+      const int page_of = __builtin_amdgcn_readlane(always ? -1 : page, i);
+      if (page_of < 0) continue;
+      const double sum = pg_score_again(P, t, h, page_of);
+      if (lane == 0) keys[j0 + i] = pg_key(sum);
+    }
   }
 }
 

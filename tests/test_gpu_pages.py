@@ -345,6 +345,35 @@ def test_select_scores_that_are_not_finite_come_first(cuda):
     assert got[0, 0].tolist() == [0, 1, 2, 3, 39]
 
 
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim, q_heads, kv_heads", [(16, 1, 1), (64, 6, 2), (128, 4, 1), (256, 2, 2), (96, 12, 1)])
+def test_select_where_bounds_are_infinite(cuda, kind, dim, q_heads, kv_heads):
+    """A smallest element of -inf is no product's larger one where all of a group's queries are positive, nor a largest of +inf where all are
+    negative: such a page ranks by its finite score. Where a head has the other sign, or 0, it is not finite and comes first."""
+    case = Case(cuda, kind, [1, 2], [900, 333], kv_heads, dim, 8, seed=dim)
+    g = torch.Generator().manual_seed(dim + q_heads)
+    bounds = torch.stack([case.wide[0].amin(1), case.wide[0].amax(1)], 2)
+    q = torch.randn(3, q_heads, dim, generator=g).abs() + 0.01
+    q[:, :, 1::2] *= -1  # channels of one sign in all heads
+    q[:, :, 2] = torch.randn(3, q_heads, generator=g)
+    q[:, -1, 4] = 0.0
+    q = q.to(kind)
+    for page in range(bounds.shape[0]):
+        for h in range(kv_heads):
+            if torch.rand((), generator=g) < 0.6:
+                c = int(torch.randint(0, 2, (), generator=g))
+                c += 8 if dim == 16 else 2 * int(torch.randint(4, dim // 2, (), generator=g))
+                bounds[page, h, c % 2, c] = math.inf if c % 2 else -math.inf
+            if torch.rand((), generator=g) < 0.04:
+                c = (2, 4, 10, 11)[int(torch.randint(0, 4, (), generator=g))]  # both signs (of several heads), a 0, the bound that counts
+                which = 1 - c % 2 if c > 4 else 0
+                bounds[page, h, which, c] = math.inf if which else -math.inf
+    bounds = bounds.to(kind)
+    want = _plain_select(q, bounds.double(), case, q_heads // kv_heads, 30, 1, 1)
+    got = P.select_pages(q.to(cuda), bounds.to(cuda), case.table, case.kv_lens, case.cu_new, 8, 30)
+    assert torch.equal(got.long().cpu(), want)
+
+
 # -------------------------------------------------------------------------------------------------------------- attention
 def _attention_case(cuda, dtype, kind, new, cached, q_heads, kv_heads, dim, page, sink=0, window=0, sinks=False, pad=0, seed=0, layout="plain",
                     missing=(), lists=None, max_context=None, scaling=None, scale=1.0, stride=False, wide=0):
