@@ -22,7 +22,7 @@ extern "C" {
 typedef struct sah_page_cache {
   void* k; int64_t ks_p, ks_t, ks_h;
   void* v; int64_t vs_p, vs_t, vs_h;
-  uint8_t* k_scales;       /* SAH_E4M3: [n_pages, Hkv, page_size], 4-byte aligned; else not looked at */
+  uint8_t* k_scales;       /* SAH_E4M3: [n_pages, Hkv, page_size], from a page_size of 16 on 4-byte aligned; else not looked at */
   uint8_t* v_scales;
   int32_t dtype;
   int32_t n_pages, page_size, Hkv, D;

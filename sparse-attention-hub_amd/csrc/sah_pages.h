@@ -121,7 +121,9 @@ static inline int pg_check_cache(sah_page_cache& c, bool with_v, const char* wha
   const int es = pg_size(c.dtype);
   if (((uint64_t)c.k | (uint64_t)c.v | (uint64_t)(es * (c.ks_p | c.ks_t | c.ks_h | c.vs_p | c.vs_t | c.vs_h))) % 16)
     return sah_fail(SAH_EINVAL, "%s: the cache's addresses and strides must be multiples of 16 bytes", what);
-  if (c.dtype == SAH_E4M3 && ((uint64_t)c.k_scales | (uint64_t)c.v_scales) % 4) return sah_fail(SAH_EINVAL, "%s: scales must be 4-byte aligned", what);
+  // (four scales of a page are read at once where a page has 16 tokens or more, single ones elsewhere: a layer's of small pages may begin anywhere)
+  if (c.dtype == SAH_E4M3 && c.page_size >= 16 && ((uint64_t)c.k_scales | (uint64_t)c.v_scales) % 4)
+    return sah_fail(SAH_EINVAL, "%s: scales must be 4-byte aligned", what);
   if (c.ks_t < 0 || c.vs_t < 0 || c.ks_t >= 1 << 26 || c.vs_t >= 1 << 26)  // a few tokens of a page: 32-bit offsets
     return sah_fail(SAH_ESHAPE, "%s: a page's tokens are 2^26 elements or more apart", what);
   return SAH_OK;

@@ -813,6 +813,31 @@ def test_a_server_with_selected_pages(cuda, dtype, kind):
             assert torch.equal(got[which].double().cpu(), want)
 
 
+@pytest.mark.parametrize("page, kv_heads, pages", [(1, 1, 103), (1, 3, 81), (2, 1, 61), (2, 3, 63), (4, 1, 41)])
+@pytest.mark.parametrize("chunk", [3, 50, 140])
+def test_layers_of_small_pages(cuda, page, kv_heads, pages, chunk):
+    """The layers of an 8-bit cache whose scales begin at odd bytes: stored, read back, their bounds, attention over all keys and over some."""
+    torch.manual_seed(page + chunk)
+    dim, heads = 16, 2 * kv_heads
+    chunk = min(chunk, pages * page - 1)
+    cache = P.PagedKVCache(3, pages, page, kv_heads, dim, 1, pages * page, _E4M3, cuda, page_bounds=True)
+    rows = [[torch.randn(n, m, dim).to(torch.bfloat16) for m in (heads, kv_heads, kv_heads)] for n in (chunk, 1) for _ in range(3)]
+    for i, n in enumerate((chunk, 1)):
+        step = cache.assign(_i32([n], cuda), n)
+        for layer in range(3):
+            q, k, v = (x.to(cuda) for x in rows[3 * i + layer])
+            out = cache.attend(layer, q, k, v, step, 0.25, n_select=None if i == 0 else pages).double().cpu()
+            keys, values = (torch.cat([_plain_quantise(rows[3 * r + layer][which])[0] for r in range(i + 1)]) for which in (1, 2))
+            got = cache.load(layer, keys.shape[0], torch.float32)
+            assert torch.equal(got[0][0].transpose(0, 1).double().cpu(), keys) and torch.equal(got[1][0].transpose(0, 1).double().cpu(), values)
+            for t in range(n):
+                p = keys.shape[0] - n + t
+                for h in range(heads):
+                    want = _plain_step(None, rows[3 * i + layer][0][t, h], keys[:p + 1, h // 2], values[:p + 1, h // 2], 0.25)
+                    # the result's rounding and in chunks that of the weights, logits of a few units
+                    assert (out[t, h] - want).abs().max() <= 2.2 * _HALF_STEP[torch.bfloat16] * max(1.0, float(values.abs().max()))
+
+
 def test_a_context_read_back_goes_into_research_attention(cuda):
     """An 8-bit context as the maskers' contiguous cache: Sink + Local over it is paged attention's window over the pages."""
     from sparse_attention_hub_amd.sparse_attention import LocalMaskerConfig, ResearchAttentionConfig, SinkMaskerConfig

@@ -161,6 +161,20 @@ def test_nothing_to_do_is_no_error():
     assert _call("sah_page_select", args, requests__n_tokens=0) == 0
 
 
+@pytest.mark.parametrize("page_size, ok", [(1, True), (2, True), (4, True), (8, True), (16, False), (64, False)])
+def test_scales_of_small_pages_may_begin_anywhere(page_size, ok):
+    """A layer's scales are a slice of all layers': where its pages hold few tokens, it begins at any byte."""
+    for offset in (1, 2, 3):
+        changes = dict(cache__page_size=page_size, cache__k_scales=3 * _FAR + offset, cache__v_scales=4 * _FAR + offset)
+        # nothing to do, or a refusal that comes behind those of the cache
+        store = N.PageStoreArgs(_cache(), 8 * _FAR, 128, 64, 9 * _FAR, 128, 64, 10 * _FAR, 1, 0, None)
+        assert _call("sah_page_store", store, **changes) == (0 if ok else -1)
+        load = N.PageLoadArgs(_cache(), _requests(), 8 * _FAR, 9 * _FAR, 1, 0, None)
+        assert _call("sah_page_load", load, **changes) == (0 if ok else -1)
+        assert _call("sah_page_bounds", N.PageBoundsArgs(_cache(v=None), _requests(), None, None), **changes) == (-2 if ok else -1)
+        assert _attention(requests__n_tokens=0, **changes) == (0 if ok else -1)
+
+
 def test_workspaces_follow_the_work():
     def attention(tokens, width, requests=1, n_select=0, Hq=8):
         args = N.PageAttentionArgs(dtype=1, Hq=Hq, n_select=n_select, pages=_PTR if n_select else None, cache=N.PageCache(dtype=3, n_pages=9, page_size=16, Hkv=2, D=128),
