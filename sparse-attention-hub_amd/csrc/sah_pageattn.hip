@@ -1092,9 +1092,10 @@ extern "C" int sah_page_attention(const sah_page_attention_args* given) {
   if (a->Hq <= 0 || a->Hq % c.Hkv || a->max_context < 0 || a->sink < 0 || a->window < 0 || a->n_select < 0)
     return sah_fail(SAH_EINVAL, "sah_page_attention: bad sizes (heads %d / %d, max_context %d, sink %d, window %d, n_select %d)", a->Hq, c.Hkv, a->max_context,
                     a->sink, a->window, a->n_select);
-  if ((a->pages != nullptr) != (a->n_select > 0)) return sah_fail(SAH_EINVAL, "sah_page_attention: pages and n_select go together");
-  if (a->pages && (a->window || a->sink)) return sah_fail(SAH_EINVAL, "sah_page_attention: pages and a window do not go together");
-  if (!a->pages && c.dtype != SAH_E4M3) return sah_fail(SAH_EDTYPE, "sah_page_attention: neither pages nor an 8-bit cache: sah_paged_attention's");
+  // (lists of no tokens lie nowhere)
+  if (a->pages ? a->n_select == 0 : a->n_select > 0 && r.n_tokens > 0) return sah_fail(SAH_EINVAL, "sah_page_attention: pages and n_select go together");
+  if (a->n_select && (a->window || a->sink)) return sah_fail(SAH_EINVAL, "sah_page_attention: pages and a window do not go together");
+  if (!a->n_select && c.dtype != SAH_E4M3) return sah_fail(SAH_EDTYPE, "sah_page_attention: neither pages nor an 8-bit cache: sah_paged_attention's");
   if (int rc = pg_check_requests(r, c.page_size, true, what)) return rc;
   if ((int64_t)a->n_select * c.page_size > INT32_MAX - 4096) return sah_fail(SAH_ESHAPE, "sah_page_attention: n_select * page_size passes 2^31 - 4097");
   if ((int64_t)r.n_tokens * a->Hq > 1 << 30) return sah_fail(SAH_ESHAPE, "sah_page_attention: n_tokens * Hq passes 2^30");

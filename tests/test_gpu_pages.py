@@ -967,6 +967,21 @@ def test_calls_of_no_tokens(cuda):
     assert bounds.eq(0).all()
 
 
+@pytest.mark.parametrize("kind", _KINDS)
+def test_selection_and_attention_of_no_tokens(cuda, kind):
+    """A step without a token: its lists are as empty as its queries."""
+    case = Case(cuda, kind, [0, 0], [20, 3], 2, 64, 16)
+    dtype = torch.bfloat16 if kind == _E4M3 else kind
+    q, out = torch.zeros(0, 4, 64, dtype=dtype, device=cuda), torch.zeros(0, 4, 64, dtype=dtype, device=cuda)
+    bounds = torch.zeros(case.caches[0].shape[0], 2, 2, 64, dtype=dtype, device=cuda)
+    pages = P.select_pages(q, bounds, case.table, case.kv_lens, case.cu_new, 16, 4)
+    for o in (None, out):
+        assert P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, pages=pages, out=o, **case.held).shape == (0, 4, 64)
+    cache = P.PagedKVCache(1, 9, 16, 2, 64, 2, 100, kind, cuda, page_bounds=True)
+    rows = torch.zeros(0, 2, 64, dtype=dtype, device=cuda)
+    assert cache.attend(0, q, rows, rows, cache.assign(_i32([0, 0], cuda), 0), 0.125, n_select=3).shape == (0, 4, 64)
+
+
 def test_pages_beyond_32_bits(cuda):
     """A cache of more than 2^32 bytes and elements, its last pages in use."""
     heads, dim, page = 1, 256, 16

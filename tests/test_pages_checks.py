@@ -175,6 +175,14 @@ def test_scales_of_small_pages_may_begin_anywhere(page_size, ok):
         assert _attention(requests__n_tokens=0, **changes) == (0 if ok else -1)
 
 
+@pytest.mark.parametrize("dtype", [N.SAH_E4M3, 1])
+def test_lists_of_no_tokens_are_no_error(dtype):
+    """An empty tensor has no address."""
+    nothing = dict(requests__n_tokens=0, q=None, out=None, work=None, cache__dtype=dtype)
+    assert _attention(n_select=4, pages=None, **nothing) == 0 and _attention(n_select=4, pages=11 * _FAR, **nothing) == 0
+    assert _attention(n_select=4, pages=None, window=4, **nothing) == -1 and _attention(n_select=0, pages=11 * _FAR, **nothing) == -1
+
+
 def test_workspaces_follow_the_work():
     def attention(tokens, width, requests=1, n_select=0, Hq=8):
         args = N.PageAttentionArgs(dtype=1, Hq=Hq, n_select=n_select, pages=_PTR if n_select else None, cache=N.PageCache(dtype=3, n_pages=9, page_size=16, Hkv=2, D=128),
