@@ -6,7 +6,8 @@
  * 2^e, e the same for all of a token's elements of one key head: the least whole number from -110 up at which the row's
  * largest finite magnitude is at most 448 * 2^e. The scale is held as the byte e + 127 (torch.float8_e8m0fnu), scales [n_pages, Hkv, page_size].
  * A power of two divides and multiplies exactly: an element is rounded once, to the nearest, ties to even, and what it stands
- * for is a bf16 number. An element that is not finite is held as NaN. */
+ * for is a bf16 number; but magnitudes from 248 * 2^120 (3.297e38) on are rounded to 2^128, which bf16 and fp32 do not have, and count as infinite wherever
+ * they are read. An element that is not finite is held as NaN. */
 #ifndef SAH_PAGES_H
 #define SAH_PAGES_H
 #include "sah_serve.h"

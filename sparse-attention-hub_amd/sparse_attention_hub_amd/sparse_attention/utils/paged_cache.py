@@ -176,7 +176,7 @@ def store_paged(keys: torch.Tensor, values: torch.Tensor, key_cache: torch.Tenso
     (or any other outside the cache) are passed over. No two rows may name the same slot: which of them it would hold is
     not defined. An 8-bit cache takes float32, bfloat16 or float16 rows (addresses and strides multiples of 16 bytes, head_dim of
     16): each is rounded once to e4m3 times the least power of two, from 2^-110 up, at which its largest element fits; what is not finite
-    becomes NaN."""
+    becomes NaN, and magnitudes from 248 * 2^120 (3.297e38) on are rounded to 2^128: infinite when they are read."""
     _check_cache(key_cache, value_cache)
     _check_scales(key_scales, "key_scales", key_cache)
     _check_scales(value_scales, "value_scales", value_cache)

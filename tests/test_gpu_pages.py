@@ -106,6 +106,29 @@ def test_store_quantises(cuda, dtype, tokens, heads, dim, page, layout):
         assert _same_values(_wide(caches[i], scales[i]), want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_largest_numbers_are_infinite_when_they_are_read(cuda, dtype):
+    """From 248 * 2^120 on an element is rounded to 2^128, below it to a bf16 number: contexts read back, bounds and attention."""
+    rows = torch.zeros(2, 1, 16)
+    rows[0, 0, :4] = torch.tensor([torch.finfo(dtype).max, -248.0 * 2.0 ** 120, 247.0 * 2.0 ** 120, -232.0 * 2.0 ** 120])
+    rows = rows.to(dtype)
+    want = torch.zeros(2, 16, dtype=torch.float64)
+    want[0, :4] = torch.tensor([math.inf, -math.inf, 240.0 * 2.0 ** 120, -224.0 * 2.0 ** 120], dtype=torch.float64)
+    cache = P.PagedKVCache(1, 1, 2, 1, 16, 1, 2, _E4M3, cuda, page_bounds=True)
+    q = torch.zeros(2, 1, 16, dtype=dtype, device=cuda)
+    keys = torch.zeros_like(rows)  # equal weights, so that the value alone decides
+    step = cache.assign(_i32([2], cuda), 2)
+    out = cache.attend(0, q, keys.to(cuda), rows.to(cuda), step, 0.25).double().cpu()[0, 0]
+    assert torch.equal(out, want[0])
+    cache.release(torch.ones(1, dtype=torch.bool, device=cuda))
+    cache.attend(0, q, rows.to(cuda), rows.to(cuda), cache.assign(_i32([2], cuda), 2), 0.25)
+    for given in (torch.float32, torch.bfloat16):
+        for got in cache.load(0, 2, given):
+            assert torch.equal(got[0, 0].double().cpu(), want)
+    assert torch.equal(cache.bounds[0, 0, 0].double().cpu(), torch.stack([want.amin(0), want.amax(0)]))
+    assert cache.load(0, 2, torch.float16)[0][0, 0, 0, :4].tolist() == [65504.0, -65504.0, 65504.0, -65504.0]
+
+
 def test_store_of_no_tokens(cuda):
     cache, scales = torch.zeros(2, 4, 2, 16, device=cuda).to(_E4M3), torch.zeros(2, 2, 4, dtype=torch.uint8, device=cuda).view(_E8M0)
     rows = torch.zeros(0, 2, 16, device=cuda)
