@@ -5,6 +5,7 @@ import random
 import pytest
 import torch
 
+from sparse_attention_hub_amd import _native as N
 from sparse_attention_hub_amd.sparse_attention.utils import paged_cache as P
 
 pytestmark = pytest.mark.gpu
@@ -535,6 +536,34 @@ def test_attention_8bit_does_not_depend_on_the_hint(cuda, dtype, max_context):
 @pytest.mark.parametrize("scaling", [-0.2, 0.0, 2.0])
 def test_attention_8bit_scaling(cuda, scaling):
     _attention_case(cuda, torch.bfloat16, _E4M3, [1, 3], [500, 77], 4, 2, 64, 16, scaling=scaling)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_8bit_chunks_copy_no_context_without_a_row(cuda, dtype):
+    """A chunk beside requests that have nothing new in this step: their contexts are not read, and their part of the workspace stays as it was."""
+    new, cached, page, dim = [0, 700, 0, 3], [300, 100, 400, 50], 16, 64
+    case = Case(cuda, _E4M3, new, cached, 1, dim, page, seed=1)
+    q = torch.randn(case.cu[-1], 2, dim, generator=torch.Generator().manual_seed(1)).to(dtype).to(cuda)
+    want = P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, **case.held)
+    out = torch.empty_like(q)
+    args = N.PageAttentionArgs(
+        q.data_ptr(), q.stride(0), q.stride(1), P._cache_block(*case.caches, *case.scales),
+        N.PageRequests(case.table.data_ptr(), case.width, case.width, case.kv_lens.data_ptr(), case.cu_new.data_ptr(), 4, case.cu[-1]), None, 0, None,
+        N.dtype_code(dtype), 2, 0, 0, 0, 0.125, out.data_ptr(), out.stride(0), out.stride(1), None, 0, N.stream_ptr(cuda))
+    size = N.page_work_bytes("attention", args)
+    work = torch.full((size,), 0x5a, dtype=torch.uint8, device=cuda)
+    args.work, args.work_bytes = work.data_ptr(), size
+    N.call_on(cuda, "sah_page_attention", args)
+    assert torch.equal(out, want)
+    contexts = work[:2 * 4 * case.width * page * dim * 2].view(2, 4, -1)  # keys and values, request by request
+    for b in range(4):
+        length = case.kv[b] * dim * 2
+        assert all(contexts[which, b, :length].eq(0x5a).all() == (new[b] == 0) for which in range(2)), b
+    # scales that no request with a row has
+    for b in (0, 2):
+        for s in case.scales:
+            s.view(torch.uint8)[case.table_host[b, :-(-case.kv[b] // page)].long().to(cuda)] = 255
+    assert torch.equal(P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, **case.held), want)
 
 
 def _some_pages(last, rng):
