@@ -109,7 +109,8 @@ int sah_page_select(const sah_page_select_args* a);
  * Logits, softmax statistics and sums are fp32; q of more than bf16's bits and weights enter 16-bit products as several terms: as
  * exact as the result's own rounding. Chunks of an 8-bit cache under 16-bit q (more than 128 rows of q a request
  * and key head on average, with a window as many times more as the table has keys beyond it, and no more than 8 GiB of work) are attended to through a
- * copy of the contexts in q's type in work, by sah_paged_attention's kernels and with what it says of weights. work:
+ * copy of the contexts in q's type in work, by sah_paged_attention's kernels and with what it says of weights; a cache that holds what SAH_F16 does not
+ * (beyond 65504, finer than 2^-24) is then attended to as it is all the same. work:
  * sah_page_attention_work_bytes(a) bytes, 16-byte aligned, no particular content. */
 typedef struct sah_page_attention_args {
   const void* q; int64_t qs_t, qs_h;

@@ -44,6 +44,8 @@ struct pt_args {
   // answers of 1K to 32K keys, 8 heads: 445 us one by one, 407 by 4; 32 of 4K to 8K: 106 by 1, 97 by 2, 94 by 4); the fewer, the fewer parts
   // there are to join (one answer of 32K keys: 32.1 us by 4, 27.6 by 2, 26.7 by 1; of 128K: 70.5, 66.8, 71.9). With a list each has pages of its own, and 1 it is.
   int heads;
+  int n_lost;             // the call that stands in for one over a copy: bytes that tell whether it has to
+  const uint8_t* lost;
 };
 
 template <int KT, int QT>
@@ -305,6 +307,14 @@ __device__ __forceinline__ pt_record* pt_records(const pt_args& A, int wgs, int 
   return (pt_record*)((float*)A.a.work + (int64_t)wgs * 2 * A.heads * PT_ROWS * (dp + 4)) + 2 * w;
 }
 
+// Whether one of the bytes is set. All threads call.
+__device__ __forceinline__ bool pt_any(const uint8_t* bytes, int n) {
+  uint32_t any = 0;
+  for (int i = threadIdx.x; i < n / 4; i += PT_NT) any |= ((const uint32_t*)bytes)[i];
+  for (int i = n / 4 * 4 + threadIdx.x; i < n; i += PT_NT) any |= bytes[i];
+  return __syncthreads_or(any != 0);
+}
+
 // One row key by key, by one wave: what a row holds that came out not finite. The average so far is held, not the sum: of finite values it
 // is finite, however large they are.
 template <int KT, int QT>
@@ -458,7 +468,8 @@ __global__ __launch_bounds__(PT_NT, (pt_per_cu(KT, DP))) void k_page_attn(pt_arg
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id(), i16 = lane & 15, g = lane >> 4;
   const int w = pt_number();
   pt_place at;
-  if (!pt_start(pt_arguments(), w, gridDim.x, s_sum, s_shares, at)) {
+  const uint8_t* lost = pt_arguments().lost;
+  if ((lost && !pt_any(lost, pt_arguments().n_lost)) || !pt_start(pt_arguments(), w, gridDim.x, s_sum, s_shares, at)) {
     if (threadIdx.x < 2) pt_records(pt_arguments(), gridDim.x, DP, w)[threadIdx.x].parts = 0;
     return;
   }
@@ -973,6 +984,8 @@ static double pt_context_bytes(const sah_page_attention_args& a) {
 static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
   pt_args A;
   A.a = *a;
+  A.n_lost = 0;
+  A.lost = nullptr;
   const int G = a->Hq / a->cache.Hkv;
   A.tokens = a->pages || G >= PT_ROWS ? 1 : PT_ROWS / G;
   A.blocks = (G + PT_ROWS - 1) / PT_ROWS;
@@ -1001,15 +1014,27 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
 // 128 rows 74 / 84, 256 rows 124 / 99, 512 rows 222 / 137; of those keys 512 + 128 seen, 1024 rows 56 / 70, 4096 rows 191 / 129; 2 requests of
 // 32768, 2048 + 128 seen, 1024 rows 84 / 129, 4096 rows 248 / 175). Never for fp32 q: its terms go at the 16-bit matrix rate here, an fp32 copy at a
 // tenth of it (4 requests of 8192 keys, 128 rows 80 / 268, 2048 rows 947 / 2952).
-static int64_t pt_copy_bytes(const sah_page_attention_args* a) {
-  if (a->pages || a->cache.dtype != SAH_E4M3 || a->dtype == SAH_F32) return 0;
+// fp16 does not hold all that an 8-bit cache can: the copy's workgroups tell where it does not, and the cache is then attended to as it is, all rows
+// once more (fp16 copies that hold everything pay for it with two launches that end at once: 4 requests of 64 tokens over 8192 keys 104 -> 113 us).
+struct pt_copy {
+  int64_t bytes;    // K, V, their table and what was lost; 0: none
+  int64_t lost_at;  // where the last of these begins
+  int n_lost;       // 0: the copy's type holds everything
+};
+static pt_copy pt_copy_of(const sah_page_attention_args* a) {
+  const pt_copy none{0, 0, 0};
+  if (a->pages || a->cache.dtype != SAH_E4M3 || a->dtype == SAH_F32) return none;
   const double keys = (double)a->requests.table_width * a->cache.page_size, reach = (double)a->sink + a->window, seen = a->window && reach < keys ? reach : keys;
   const double rows = (double)a->requests.n_tokens * (a->Hq / a->cache.Hkv);
-  if (rows * seen <= 128 * keys * a->requests.n_requests) return 0;
+  if (rows * seen <= 128 * keys * a->requests.n_requests) return none;
   const double pages = (double)a->requests.n_requests * a->requests.table_width;
   const double bytes = pages * a->cache.page_size * a->cache.Hkv * a->cache.D * pg_size(a->dtype) * 2;
-  if (bytes > 0x1p33 || pages * 4 > 0x1p33) return 0;
-  return (int64_t)bytes + ((int64_t)pages * 4 + 15) / 16 * 16;
+  if (bytes > 0x1p33 || pages * 4 > 0x1p33) return none;
+  pt_copy c;
+  c.lost_at = (int64_t)bytes + ((int64_t)pages * 4 + 15) / 16 * 16;
+  c.n_lost = a->dtype == SAH_F16 ? (int)pg_load_workgroups(a->cache, a->requests, a->requests.table_width * a->cache.page_size) : 0;
+  c.bytes = c.lost_at + (c.n_lost + 15) / 16 * 16;
+  return c;
 }
 static sah_paged_attention_args pt_on_copy(const sah_page_attention_args* a) {
   const sah_page_cache& c = a->cache;
@@ -1041,13 +1066,14 @@ extern "C" int64_t sah_page_attention_work_bytes(const sah_page_attention_args* 
   if (!a || a->requests.n_tokens <= 0 || a->requests.n_requests <= 0 || a->requests.table_width <= 0 || a->cache.Hkv <= 0 || a->Hq < a->cache.Hkv ||
       a->cache.D <= 0 || a->cache.D > PG_MAX_D || a->cache.page_size <= 0 || (a->pages && a->n_select <= 0))
     return 0;
-  if (const int64_t copy = pt_copy_bytes(a)) {
-    const sah_paged_attention_args p = pt_on_copy(a);
-    return copy + 4 * sah_paged_attention_work_floats(&p);
-  }
   int wgs;
   const pt_args A = pt_plan(a, wgs);
-  return (int64_t)wgs * 2 * (A.heads * PT_ROWS * (pt_dim(a) + 4) * 4 + (int64_t)sizeof(pt_record));
+  const int64_t own = (int64_t)wgs * 2 * (A.heads * PT_ROWS * (pt_dim(a) + 4) * 4 + (int64_t)sizeof(pt_record));
+  const pt_copy copy = pt_copy_of(a);
+  if (!copy.bytes) return own;
+  const sah_paged_attention_args p = pt_on_copy(a);
+  const int64_t others = 4 * sah_paged_attention_work_floats(&p);
+  return copy.bytes + (copy.n_lost && own > others ? own : others);  // (one after the other)
 }
 
 // Whether keys and values are read past the caches: where every key is one tile's alone and the contexts, as far as the caller says, are twice what the
@@ -1127,18 +1153,22 @@ extern "C" int sah_page_attention(const sah_page_attention_args* given) {
       (a->pages && sah_meet(out, sah_span_of<1>(a->pages, 4, (int64_t)r.n_tokens * c.Hkv * a->n_select, {0}, {1}))) ||
       (a->sinks && sah_meet(out, sah_span_of<1>(a->sinks, 4, 1, {1}, {a->Hq}))))
     return sah_fail(SAH_EINVAL, "sah_page_attention: out lies within the cache, the table, the lists or the lengths");
-  if (const int64_t copy = pt_copy_bytes(a)) {
+  int wgs;
+  pt_args A = pt_plan(a, wgs);
+  const pt_copy copy = pt_copy_of(a);
+  if (copy.bytes) {
     sah_paged_attention_args p = pt_on_copy(a);
     const int64_t row = c.D, token = row * c.Hkv, request = token * c.page_size * r.table_width;
-    if (int rc = pg_load(c, r, a->dtype, pg_load_out{(void*)p.k, (void*)p.v, request, row, token, r.table_width * c.page_size, (int32_t*)p.block_table},
-                         a->stream, what))
-      return rc;
-    p.work = (float*)((char*)a->work + copy);
-    p.work_floats = (a->work_bytes - copy) / 4;
-    return sah_paged_attention(&p);
+    A.n_lost = copy.n_lost;
+    if (copy.n_lost) A.lost = (const uint8_t*)a->work + copy.lost_at;
+    const pg_load_out to{(void*)p.k, (void*)p.v, request, row, token, r.table_width * c.page_size, (int32_t*)p.block_table, (uint8_t*)A.lost};
+    if (int rc = pg_load(c, r, a->dtype, to, a->stream, what)) return rc;
+    p.work = (float*)((char*)a->work + copy.bytes);
+    p.work_floats = (a->work_bytes - copy.bytes) / 4;
+    if (int rc = sah_paged_attention(&p)) return rc;
+    if (!copy.n_lost) return SAH_OK;
+    A.a.work = p.work;
   }
-  int wgs;
-  const pt_args A = pt_plan(a, wgs);
   if (c.dtype == SAH_F32) return pt_launch_dim<SAH_F32, SAH_F32>(A, wgs);
   if (c.dtype == SAH_BF16) return pt_launch_dim<SAH_BF16, SAH_BF16>(A, wgs);
   if (c.dtype == SAH_F16) return pt_launch_dim<SAH_F16, SAH_F16>(A, wgs);

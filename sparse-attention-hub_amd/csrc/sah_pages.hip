@@ -118,6 +118,20 @@ __device__ __forceinline__ void pg_put8(char* to, uint2 x, float scale) {
     }
   }
 }
+// Whether one of 8 elements of e4m3 is a number that fp16 does not hold. All of them are multiples of 2^(e - 9) up to 448 * 2^e: from e = -15 to 7 none is.
+__device__ __forceinline__ bool pg_none_of_f16(uint2 x, uint32_t scale) {
+  if (scale >= 127 - 15 && scale <= 127 + 7) return false;
+  float f[2][4];
+  pg_widen4(x.x, pg_scale(scale), f[0]);
+  pg_widen4(x.y, pg_scale(scale), f[1]);
+  [[maybe_unused]] bool lost = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = f[i / 4][i % 4];
+    lost |= v == v && (fabsf(v) > 65504.f || sah_f16_to_float(sah_float_to_f16(v)) != v);
+  }
+  return lost;
+}
 // CT: type of the cache; OT: of the output (other caches than SAH_E4M3: the same). `wgs` workgroups a request, which go through its tokens in
 // turn: what lies behind a context in a table of a hundred thousand tokens costs a copy nothing. COPY: for the attention, with a table; requests without a row
 // have no use for one (a chunk of 1024 tokens over 4024 keys beside 7 contexts of 32768 without one: 109 us, with copies of theirs 377).
@@ -129,8 +143,12 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
   const int shift = 31 - __builtin_clz(C.page_size), b = (int)blockIdx.x / wgs, kv = R.kv_lens[b];
   if constexpr (COPY) {
     const int begin = R.cu_new[b], end = R.cu_new[b + 1];
-    if ((begin > 0 ? begin : 0) >= (end < R.n_tokens ? end : R.n_tokens)) return;
+    if ((begin > 0 ? begin : 0) >= (end < R.n_tokens ? end : R.n_tokens)) {
+      if (O.lost && threadIdx.x == 0) O.lost[blockIdx.x] = 0;
+      return;
+    }
   }
+  [[maybe_unused]] bool lost = false;
   const uint32_t n = COPY && kv < O.length ? (kv > 0 ? kv : 0) : O.length, first = (blockIdx.x - (uint32_t)b * wgs) * PG_NT + threadIdx.x;
   // consecutive threads: a token's units, all heads of it, then the next token: as the cache lies
   uint32_t at = first / unit_h, in = first - at * unit_h;
@@ -154,10 +172,12 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
       float ks = 1.f, vs = 1.f;
       if (there) {
         const int64_t s = ((int64_t)page * C.Hkv + h) * C.page_size + entry;
+        const uint32_t k_byte = C.k_scales[s], v_byte = C.v_scales[s];
         k = *(const uint2*)kp;
         v = *(const uint2*)vp;
-        ks = pg_scale(C.k_scales[s]);
-        vs = pg_scale(C.v_scales[s]);
+        ks = pg_scale(k_byte);
+        vs = pg_scale(v_byte);
+        if constexpr (COPY && OT == SAH_F16) lost = lost || pg_none_of_f16(k, k_byte) || pg_none_of_f16(v, v_byte);
       }
       pg_put8<OT, !COPY>(ko, k, ks);
       pg_put8<OT, !COPY>(vo, v, vs);
@@ -170,6 +190,11 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
       pg_put16<!COPY>(ko, k);
       pg_put16<!COPY>(vo, v);
     }
+  }
+  if constexpr (COPY) {
+    if (!O.lost) return;
+    const int any = __syncthreads_or(lost);
+    if (threadIdx.x == 0) O.lost[blockIdx.x] = any != 0;
   }
 }
 
@@ -714,14 +739,19 @@ extern "C" int sah_page_store(const sah_page_store_args* given) {
   return sah_launch_status(what);
 }
 
+int64_t pg_load_workgroups(const sah_page_cache& c, const sah_page_requests& r, int length) {
+  const int64_t units = (int64_t)c.D / (c.dtype == SAH_E4M3 ? 8 : 16 / pg_size(c.dtype)) * c.Hkv * length, room = PG_LOAD_WGS / r.n_requests;
+  int64_t wgs = (units + PG_NT - 1) / PG_NT;
+  if (wgs > INT32_MAX / r.n_requests) return 0;
+  if (wgs > room) wgs = room > 1 ? room : 1;
+  return wgs * r.n_requests;
+}
 // (also what the attention over chunks makes its copy with)
 int pg_load(const sah_page_cache& c, const sah_page_requests& r, int dtype, const pg_load_out& out, void* stream, const char* what) {
-  const int64_t units = (int64_t)c.D / (c.dtype == SAH_E4M3 ? 8 : 16 / pg_size(c.dtype)) * c.Hkv * out.length, room = PG_LOAD_WGS / r.n_requests;
-  int64_t wgs = (units + PG_NT - 1) / PG_NT;
-  if (wgs > INT32_MAX / r.n_requests) return sah_fail(SAH_ESHAPE, "%s: too many elements", what);
-  if (wgs > room) wgs = room > 1 ? room : 1;
+  const int64_t all = pg_load_workgroups(c, r, out.length), wgs = all / r.n_requests;
+  if (!all) return sah_fail(SAH_ESHAPE, "%s: too many elements", what);
   sah_timed timed("k_page_load", stream);
-  const dim3 grid((unsigned)(wgs * r.n_requests));
+  const dim3 grid((unsigned)all);
   hipStream_t st = (hipStream_t)stream;
   if (c.dtype == SAH_F32) hipLaunchKernelGGL((k_page_load<SAH_F32, SAH_F32, false>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
   else if (c.dtype != SAH_E4M3) hipLaunchKernelGGL((k_page_load<SAH_BF16, SAH_BF16, false>), grid, dim3(PG_NT), 0, st, c, r, out, (int)wgs);
@@ -748,7 +778,7 @@ extern "C" int sah_page_load(const sah_page_load_args* given) {
   if (!a->k_out || !a->v_out) return sah_fail(SAH_ENULL, "sah_page_load: NULL pointer");
   if (((uint64_t)a->k_out | (uint64_t)a->v_out) % 16) return sah_fail(SAH_EINVAL, "sah_page_load: addresses must be multiples of 16 bytes");
   const int64_t row = c.D, head = row * a->length;
-  return pg_load(c, a->requests, a->dtype, pg_load_out{a->k_out, a->v_out, head * c.Hkv, head, row, a->length, nullptr}, a->stream, what);
+  return pg_load(c, a->requests, a->dtype, pg_load_out{a->k_out, a->v_out, head * c.Hkv, head, row, a->length, nullptr, nullptr}, a->stream, what);
 }
 
 extern "C" int sah_page_bounds(const sah_page_bounds_args* given) {

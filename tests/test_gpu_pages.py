@@ -566,6 +566,82 @@ def test_attention_8bit_chunks_copy_no_context_without_a_row(cuda, dtype):
     assert torch.equal(P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, **case.held), want)
 
 
+def _over_a_context(case, q, scaling, dtype, term):
+    """(want, bound) of a chunk alone in its table, in 64 bits: bounds as derived for _attention_case, a weight off by `term` of itself."""
+    keys, values = (case.context(0, which)[0] for which in range(2))
+    heads, group = q.shape[1], q.shape[1] // case.kv_heads
+    p = case.cached[0] + torch.arange(case.new[0])
+    want, bound = torch.empty(q.shape, dtype=torch.float64), torch.empty(q.shape, dtype=torch.float64)
+    n = case.kv[0]
+    hidden = torch.arange(n)[None] > p[:, None]
+    for h in range(heads):
+        kk, vv, qq = keys[:, h // group], values[:, h // group], q[:case.new[0], h].double().cpu()
+        weights = torch.softmax((qq @ kk.T * scaling).masked_fill(hidden, -math.inf), 1)
+        reach = float((qq.abs() @ kk.abs().T).max()) * abs(scaling)
+        off = (case.dim + 4) * 2.0 ** -24 * reach + 8 * 2.0 ** -24
+        want[:, h] = weights @ vv
+        bound[:, h] = want[:, h].abs() * _HALF_STEP[dtype] + weights @ vv.abs() * (term + 2 * off + (2 * n + 16) * 2.0 ** -24) + torch.finfo(dtype).smallest_normal * _HALF_STEP[dtype]
+    return want, bound * 1.001
+
+
+@pytest.mark.parametrize("which, exponent, scaling", [(0, 6, 2.0 ** -12), (0, 12, 2.0 ** -18), (0, -17, 2.0 ** 10), (0, -30, 2.0 ** 24), (1, -17, 0.125), (1, 7, 0.125)])
+@pytest.mark.parametrize("new, cached", [(3, 150), (150, 40), (200, 1100)])
+def test_attention_8bit_under_float16_queries_of_what_float16_does_not_hold(cuda, which, exponent, scaling, new, cached):
+    """Elements beyond 65504 and finer than 2^-24, under few rows and under many: the same numbers, whatever way a call takes."""
+    case = Case(cuda, _E4M3, [new], [cached], 2, 64, 16, seed=new)
+    case.scales[which].view(torch.uint8).add_(exponent)
+    case.wide[which] = _wide(case.caches[which].view(torch.uint8).cpu().view(_E4M3), case.scales[which])
+    if which == 1 and exponent > 0:  # of both signs and beyond the type, their averages within it
+        raw = case.caches[1].view(torch.uint8)
+        raw[:, 0::2, :, 3] = 0x7e
+        raw[:, 1::2, :, 3] = 0xfe
+        case.scales[1].view(torch.uint8).fill_(127 + 8)
+        case.wide[1] = _wide(case.caches[1].view(torch.uint8).cpu().view(_E4M3), case.scales[1])
+    q = torch.randn(new, 4, 64, generator=torch.Generator().manual_seed(1)).to(torch.float16)
+    if which == 1 and exponent > 0:
+        q *= 2.0 ** -6
+    got = P.paged_attention(q.to(cuda), *case.caches, case.table, case.kv_lens, case.cu_new, scaling, **case.held).double().cpu()
+    want, bound = _over_a_context(case, q, scaling, torch.float16, _HALF_STEP[torch.float16])
+    inside = want.abs() < 65000
+    assert torch.isfinite(want).all() and inside[1:].all() and ((got - want).abs() <= bound)[inside].all()
+
+
+def test_a_captured_float16_chunk_over_what_float16_holds_and_what_not(cuda):
+    """One graph, replayed on caches that fp16 holds and on ones that it does not, between eager calls: the eager results, which are the definition's."""
+    cases = [Case(cuda, _E4M3, [200], [1100], 2, 64, 16, seed=n) for n in range(3)]
+    cases[1].scales[0].view(torch.uint8).add_(12)
+    q = torch.randn(200, 4, 64, generator=torch.Generator().manual_seed(3)).to(torch.float16)
+    queries, out = q.to(cuda), torch.empty(200, 4, 64, dtype=torch.float16, device=cuda)
+    live = [x.clone() for x in (cases[0].caches[0].view(torch.uint8), cases[0].caches[1].view(torch.uint8), cases[0].scales[0].view(torch.uint8),
+                                cases[0].scales[1].view(torch.uint8), cases[0].table)]
+
+    def call(o):
+        return P.paged_attention(queries, live[0].view(_E4M3), live[1].view(_E4M3), live[4], cases[0].kv_lens, cases[0].cu_new, 2.0 ** -18, out=o,
+                                 key_scales=live[2].view(_E8M0), value_scales=live[3].view(_E8M0))
+
+    stream = torch.cuda.Stream(cuda)
+    stream.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(stream):
+        call(out)
+    torch.cuda.current_stream(cuda).wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for i in range(9):
+        case = cases[i % 3]
+        for to, x in zip(live, (case.caches[0].view(torch.uint8), case.caches[1].view(torch.uint8), case.scales[0].view(torch.uint8),
+                                case.scales[1].view(torch.uint8), case.table)):
+            to.copy_(x)
+        graph.replay()
+        eager = call(torch.empty_like(out))
+        torch.cuda.synchronize(cuda)
+        assert torch.equal(out, eager), i
+        if i == 1:
+            case.wide[0] = _wide(case.caches[0].view(torch.uint8).cpu().view(_E4M3), case.scales[0])
+            want, bound = _over_a_context(case, q, 2.0 ** -18, torch.float16, _HALF_STEP[torch.float16])
+            assert ((eager.double().cpu() - want).abs() <= bound).all()
+
+
 def _some_pages(last, rng):
     """A token's own page and others, in disorder, one behind its position, one that does not exist, an entry of -1 in between."""
     some = rng.sample(range(last + 1), min(last + 1, 5)) + [last + 1, 10 ** 6, -1]
