@@ -1014,39 +1014,49 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
 // 128 rows 74 / 84, 256 rows 124 / 99, 512 rows 222 / 137; of those keys 512 + 128 seen, 1024 rows 56 / 70, 4096 rows 191 / 129; 2 requests of
 // 32768, 2048 + 128 seen, 1024 rows 84 / 129, 4096 rows 248 / 175). Never for fp32 q: its terms go at the 16-bit matrix rate here, an fp32 copy at a
 // tenth of it (4 requests of 8192 keys, 128 rows 80 / 268, 2048 rows 947 / 2952).
-// fp16 does not hold all that an 8-bit cache can: the copy's workgroups tell where it does not, and the cache is then attended to as it is, all rows
-// once more (fp16 copies that hold everything pay for it with two launches that end at once: 4 requests of 64 tokens over 8192 keys 104 -> 113 us).
+// A copy has room for max_context tokens a request where that is given: tables are as wide as a server's longest request may become (16 of 131072 tokens,
+// 8 heads of 128: 8 GiB, of 4096 tokens 256 MiB). It is no more than 2 GiB, under a hundredth of the card's memory; beyond, the cache is attended to as it is.
+// (2048 tokens of one request over 4096 keys, 32 tables of 131072: 149 us by a copy of 4096 tokens each, 407 as it is; 543 where the copy was too short. 1024
+// tokens, 16 such tables: 108, 202.)
+//
+// fp16 does not hold all that an 8-bit cache can, and a context may be longer than max_context says: the copy's workgroups tell where that is so, and the
+// cache is then attended to as it is, all rows once more (copies that hold everything pay for it with two launches that end at once: 4 requests of 64 fp16
+// tokens over 8192 keys 104 -> 113 us).
+#define PT_COPY_BYTES 0x1p31
 struct pt_copy {
   int64_t bytes;    // K, V, their table and what was lost; 0: none
+  int width;        // pages of a request
   int64_t lost_at;  // where the last of these begins
-  int n_lost;       // 0: the copy's type holds everything
+  int n_lost;       // 0: the copy holds everything
 };
 static pt_copy pt_copy_of(const sah_page_attention_args* a) {
-  const pt_copy none{0, 0, 0};
+  const pt_copy none{0, 0, 0, 0};
   if (a->pages || a->cache.dtype != SAH_E4M3 || a->dtype == SAH_F32) return none;
-  const double keys = (double)a->requests.table_width * a->cache.page_size, reach = (double)a->sink + a->window, seen = a->window && reach < keys ? reach : keys;
+  const int table = a->requests.table_width, page_size = a->cache.page_size;
+  const double keys = (double)table * page_size, reach = (double)a->sink + a->window, seen = a->window && reach < keys ? reach : keys;
   const double rows = (double)a->requests.n_tokens * (a->Hq / a->cache.Hkv);
   if (rows * seen <= 128 * keys * a->requests.n_requests) return none;
-  const double pages = (double)a->requests.n_requests * a->requests.table_width;
-  const double bytes = pages * a->cache.page_size * a->cache.Hkv * a->cache.D * pg_size(a->dtype) * 2;
-  if (bytes > 0x1p33 || pages * 4 > 0x1p33) return none;
   pt_copy c;
+  const int64_t hint = ((int64_t)a->max_context + page_size - 1) / page_size;
+  c.width = hint > 0 && hint < table ? (int)hint : table;
+  const double pages = (double)a->requests.n_requests * c.width, bytes = pages * page_size * a->cache.Hkv * a->cache.D * pg_size(a->dtype) * 2;
+  if (bytes > PT_COPY_BYTES || pages * 4 > PT_COPY_BYTES) return none;
   c.lost_at = (int64_t)bytes + ((int64_t)pages * 4 + 15) / 16 * 16;
-  c.n_lost = a->dtype == SAH_F16 ? (int)pg_load_workgroups(a->cache, a->requests, a->requests.table_width * a->cache.page_size) : 0;
+  c.n_lost = a->dtype == SAH_F16 || c.width < table ? (int)pg_load_workgroups(a->cache, a->requests, c.width * page_size) : 0;
   c.bytes = c.lost_at + (c.n_lost + 15) / 16 * 16;
   return c;
 }
-static sah_paged_attention_args pt_on_copy(const sah_page_attention_args* a) {
+static sah_paged_attention_args pt_on_copy(const sah_page_attention_args* a, int width) {
   const sah_page_cache& c = a->cache;
   sah_paged_attention_args p = {};
-  const int64_t row = c.D, token = row * c.Hkv, page = token * c.page_size, pages = (int64_t)a->requests.n_requests * a->requests.table_width;
+  const int64_t row = c.D, token = row * c.Hkv, page = token * c.page_size, pages = (int64_t)a->requests.n_requests * width;
   const int es = pg_size(a->dtype);
   char* k = (char*)a->work;
   p.q = a->q; p.qs_t = a->qs_t; p.qs_h = a->qs_h;
   p.k = k; p.ks_p = page; p.ks_t = token; p.ks_h = row;
   p.v = k + pages * page * es; p.vs_p = page; p.vs_t = token; p.vs_h = row;
   p.block_table = (const int32_t*)(k + 2 * pages * page * es);
-  p.table_pitch = p.table_width = a->requests.table_width;
+  p.table_pitch = p.table_width = width;
   p.kv_lens = a->requests.kv_lens;
   p.cu_new = a->requests.cu_new;
   p.sinks = a->sinks;
@@ -1071,7 +1081,7 @@ extern "C" int64_t sah_page_attention_work_bytes(const sah_page_attention_args* 
   const int64_t own = (int64_t)wgs * 2 * (A.heads * PT_ROWS * (pt_dim(a) + 4) * 4 + (int64_t)sizeof(pt_record));
   const pt_copy copy = pt_copy_of(a);
   if (!copy.bytes) return own;
-  const sah_paged_attention_args p = pt_on_copy(a);
+  const sah_paged_attention_args p = pt_on_copy(a, copy.width);
   const int64_t others = 4 * sah_paged_attention_work_floats(&p);
   return copy.bytes + (copy.n_lost && own > others ? own : others);  // (one after the other)
 }
@@ -1157,11 +1167,11 @@ extern "C" int sah_page_attention(const sah_page_attention_args* given) {
   pt_args A = pt_plan(a, wgs);
   const pt_copy copy = pt_copy_of(a);
   if (copy.bytes) {
-    sah_paged_attention_args p = pt_on_copy(a);
-    const int64_t row = c.D, token = row * c.Hkv, request = token * c.page_size * r.table_width;
+    sah_paged_attention_args p = pt_on_copy(a, copy.width);
+    const int64_t row = c.D, token = row * c.Hkv, request = token * c.page_size * copy.width;
     A.n_lost = copy.n_lost;
     if (copy.n_lost) A.lost = (const uint8_t*)a->work + copy.lost_at;
-    const pg_load_out to{(void*)p.k, (void*)p.v, request, row, token, r.table_width * c.page_size, (int32_t*)p.block_table, (uint8_t*)A.lost};
+    const pg_load_out to{(void*)p.k, (void*)p.v, request, row, token, copy.width * c.page_size, (int32_t*)p.block_table, (uint8_t*)A.lost};
     if (int rc = pg_load(c, r, a->dtype, to, a->stream, what)) return rc;
     p.work = (float*)((char*)a->work + copy.bytes);
     p.work_floats = (a->work_bytes - copy.bytes) / 4;

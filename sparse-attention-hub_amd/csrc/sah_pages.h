@@ -138,8 +138,8 @@ static inline int pg_check_requests(const sah_page_requests& r, int page_size, b
 }
 
 // Where a context's copy goes. Strides of the outputs in elements. A table, where given, names the copies' pages (of a cache whose pages follow
-// each other, table_width a request): what the attention over a copy goes by; what lies behind a context is left as it is then. `lost`, where given with
-// it: a byte for each of pg_load_workgroups() workgroups, whether one of its elements is none of the copy's type.
+// each other, as many a request as `length` has): what the attention over a copy goes by; what lies behind a context is left as it is then. `lost`, where
+// given with it: a byte for each of pg_load_workgroups() workgroups, whether its request has tokens behind `length`, or an element that is none of the copy's type.
 struct pg_load_out {
   void *k, *v;
   int64_t s_b, s_h, s_t;

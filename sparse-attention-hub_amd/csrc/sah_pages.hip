@@ -141,6 +141,7 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
   constexpr int CS = pg_size(CT), OS = pg_size(OT), E = CT == SAH_E4M3 ? 8 : 16 / CS;  // elements of a unit
   const uint32_t units = C.D / E, unit_h = units * C.Hkv, stride = (uint32_t)wgs * PG_NT, stride_t = stride / unit_h, stride_in = stride - stride_t * unit_h;
   const int shift = 31 - __builtin_clz(C.page_size), b = (int)blockIdx.x / wgs, kv = R.kv_lens[b];
+  const int copied = O.length >> shift;  // pages of a copy
   if constexpr (COPY) {
     const int begin = R.cu_new[b], end = R.cu_new[b + 1];
     if ((begin > 0 ? begin : 0) >= (end < R.n_tokens ? end : R.n_tokens)) {
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
       return;
     }
   }
-  [[maybe_unused]] bool lost = false;
+  [[maybe_unused]] bool lost = kv > O.length && R.table_width > copied;
   const uint32_t n = COPY && kv < O.length ? (kv > 0 ? kv : 0) : O.length, first = (blockIdx.x - (uint32_t)b * wgs) * PG_NT + threadIdx.x;
   // consecutive threads: a token's units, all heads of it, then the next token: as the cache lies
   uint32_t at = first / unit_h, in = first - at * unit_h;
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
     const int j = t >> shift, entry = t & (C.page_size - 1);
     const int page = t < kv && j < R.table_width ? R.block_table[(int64_t)b * R.table_pitch + j] : -1;
     const bool there = page >= 0 && page < C.n_pages;
-    if (COPY && entry == 0 && in == 0) O.table[(int64_t)b * R.table_width + j] = there ? b * R.table_width + j : -1;
+    if (COPY && entry == 0 && in == 0) O.table[(int64_t)b * copied + j] = there ? b * copied + j : -1;
     if (COPY && !there) continue;
     const int64_t to = (b * O.s_b + h * O.s_h + t * O.s_t + (int64_t)c * E) * OS;
     char *ko = (char*)O.k + to, *vo = (char*)O.v + to;

@@ -566,6 +566,50 @@ def test_attention_8bit_chunks_copy_no_context_without_a_row(cuda, dtype):
     assert torch.equal(P.paged_attention(q, *case.caches, case.table, case.kv_lens, case.cu_new, 0.125, **case.held), want)
 
 
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("max_context", [1, 300, 512, 799, 800, 801, 10 ** 9])
+@pytest.mark.parametrize("sink, window", [(0, 0), (20, 90)])
+def test_attention_8bit_chunks_do_not_depend_on_the_hint(cuda, dtype, max_context, sink, window):
+    """A copy with room for less than a context, for just that, for more: long chunks beside a short one and an idle request, in a wide table."""
+    _attention_case(cuda, dtype, _E4M3, [400, 0, 170, 250], [400, 900, 300, 0], 4, 2, 64, 16, sink, window, sinks=True, seed=5, max_context=max_context, wide=60, pad=2,
+                    missing=[(0, 2, -1), (0, 45, 10 ** 6), (2, 0, -3)])
+
+
+def test_a_captured_chunk_whose_contexts_pass_the_hint(cuda):
+    """One graph, replayed on contexts that the copy has room for and on longer ones, between eager calls."""
+    cases = [Case(cuda, _E4M3, [300, 200], [n, 30], 2, 64, 16, seed=n) for n in (200, 212, 600)]
+    width = max(c.width for c in cases) + 20
+    tables = [torch.cat([c.table, torch.full((2, width - c.width), -1, dtype=torch.int32, device=cuda)], 1) for c in cases]
+    most = max(c.caches[0].shape[0] for c in cases)
+    grow = lambda x: torch.cat([x, torch.zeros(most - x.shape[0], *x.shape[1:], dtype=x.dtype, device=cuda)])
+    held = [[*(grow(x.view(torch.uint8)) for x in (*c.caches, *c.scales)), t, c.kv_lens] for c, t in zip(cases, tables)]
+    live = [x.clone() for x in held[0]]
+    q = torch.randn(500, 4, 64, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    queries, out = q.to(cuda), torch.empty(500, 4, 64, dtype=torch.bfloat16, device=cuda)
+
+    def call(o):
+        return P.paged_attention(queries, live[0].view(_E4M3), live[1].view(_E4M3), live[4], live[5], cases[0].cu_new, 0.125, out=o, max_context=512,
+                                 key_scales=live[2].view(_E8M0), value_scales=live[3].view(_E8M0))
+
+    stream = torch.cuda.Stream(cuda)
+    stream.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(stream):
+        call(out)
+    torch.cuda.current_stream(cuda).wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for i in range(9):
+        for to, x in zip(live, held[i % 3]):
+            to.copy_(x)
+        graph.replay()
+        eager = call(torch.empty_like(out))
+        torch.cuda.synchronize(cuda)
+        assert torch.equal(out, eager), i
+        want, bound = _over_a_context(cases[i % 3], q[:300], 0.125, torch.bfloat16, _HALF_STEP[torch.bfloat16])
+        assert ((eager[:300].double().cpu() - want).abs() <= bound).all(), i
+
+
 def _over_a_context(case, q, scaling, dtype, term):
     """(want, bound) of a chunk alone in its table, in 64 bits: bounds as derived for _attention_case, a weight off by `term` of itself."""
     keys, values = (case.context(0, which)[0] for which in range(2))

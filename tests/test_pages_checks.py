@@ -201,6 +201,27 @@ def test_workspaces_follow_the_work():
     assert N.page_work_bytes("select", select) == 7 * 2 * 1000 * 8
 
 
+@pytest.mark.parametrize("dtype", [1, 2])
+def test_the_copy_of_a_chunk_has_room_for_what_the_caller_says(dtype):
+    def attention(slots, tokens, max_context, width=8192, page_size=16, window=0):
+        args = N.PageAttentionArgs(dtype=dtype, Hq=32, max_context=max_context, window=window, cache=N.PageCache(dtype=3, n_pages=9, page_size=page_size, Hkv=8, D=128),
+                                   requests=N.PageRequests(table_width=width, n_requests=slots, n_tokens=tokens))
+        return N.page_work_bytes("attention", args)
+
+    def copy(slots, pages, page_size=16):
+        return slots * (4 * pages * page_size * 8 * 128 + 4 * pages)
+
+    rest = 2 ** 27  # what the kernels need beside it, and what was lost
+    for slots, hint in ((1, 4096), (16, 4096), (16, 4081), (16, 5000), (64, 8192)):
+        assert copy(slots, -(-hint // 16)) <= attention(slots, 4096, hint) <= copy(slots, -(-hint // 16)) + rest
+    assert copy(1, 8192) <= attention(1, 4096, 0) <= copy(1, 8192) + rest        # not said: the table's
+    assert copy(1, 8192) <= attention(1, 4096, 2 ** 31 - 1) <= copy(1, 8192) + rest
+    assert copy(4, 1, 4096) <= attention(4, 4096, 7, 32, 4096) <= copy(4, 1, 4096) + rest
+    for slots, hint in ((16, 0), (16, 131072), (64, 16384), (2, 2 ** 31 - 1)):     # no copy of more than 2 GiB
+        width = 8192 if slots > 2 else 2 ** 20
+        assert attention(slots, 4096, hint, width) <= rest
+
+
 def test_tensors_on_the_host_are_refused():
     i32, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32)
     cache = torch.zeros(8, 16, 2, 64).to(_E4M3)
