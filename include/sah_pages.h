@@ -84,8 +84,8 @@ int sah_page_bounds(const sah_page_bounds_args* a);
  * their ranks do not hang on the order of a sum; one that is not finite ranks above all others. Pages that the table does not have are no
  * candidates. pages [n_tokens, Hkv, n_select]: places in the request's row of the table, rising, -1 behind the last; -1 alone for rows behind the
  * last request's. Only bounds of candidates that are not taken anyway are read. sink_pages + window_pages <= n_select, window_pages >= 1.
- * Addresses and strides of q and bounds are multiples of 16 bytes. max_context: as for sah_paged_attention. work: sah_page_select_work_bytes(a) bytes,
- * 16-byte aligned, no particular content. */
+ * Addresses and strides of q and bounds are multiples of 16 bytes. max_context: as for sah_paged_attention. work: sah_page_select_work_bytes(a) bytes
+ * (8 a token, key head and entry of the table, up to 256 MiB or a single row's), 16-byte aligned, no particular content. */
 typedef struct sah_page_select_args {
   const void* q; int64_t qs_t, qs_h;
   const void* bounds;

@@ -363,8 +363,9 @@ __device__ __forceinline__ void pg_load_some(const void* p, int64_t i, float (&o
 
 struct pg_select {
   sah_page_select_args a;
-  int pitch;    // keys of a row
-  int chunks;   // workgroups a row, which take its pages in turn
+  int64_t row0;  // the first of the rows (token, key head) that are looked at: a call goes through them in slices that its workspace has room for
+  int pitch;     // keys of a row
+  int chunks;    // workgroups a row, which take its pages in turn
 };
 
 __device__ __forceinline__ float pg_load_as(int dtype, const void* p, int64_t i) {
@@ -409,8 +410,8 @@ __global__ __launch_bounds__(PG_NT, (BT == SAH_F32 || DP <= 128 ? 4 : 3)) void k
   const int lane = threadIdx.x & (SAH_WAVE - 1), in = lane % L, who = lane / L, wave = sah_wave_id();
   const int64_t row = blockIdx.x / S.chunks;
   const int chunk = (int)(blockIdx.x - row * S.chunks);
-  const int64_t t = row / P.Hkv;
-  const int h = (int)(row - t * P.Hkv);
+  const int64_t t = (S.row0 + row) / P.Hkv;
+  const int h = (int)(S.row0 + row - t * P.Hkv);
   const pg_request r = pg_find_by_wave(R, P.page_size, (int)t);
   if (r.b < 0) return;
   int64_t p = r.base + t;
@@ -555,14 +556,14 @@ __global__ __launch_bounds__(PG_NT) void k_page_top(pg_select S) {
   __shared__ int s_sum[5][NW];
   __shared__ uint64_t s_ones[NW], s_zeros[NW], s_key[PG_LIST], s_border;
   __shared__ int s_at[PG_LIST], s_border_at, s_listed, s_bin, s_above, s_count;
-  const int64_t row = blockIdx.x, t = row / P.Hkv;
+  const int64_t row = S.row0 + blockIdx.x, t = row / P.Hkv;
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id();
   const pg_request r = pg_find_by_wave(P.requests, P.page_size, (int)t);
   int64_t p = r.b < 0 ? -1 : r.base + t;
   if (p >= r.kv) p = r.kv - 1;
   const int shift = 31 - __builtin_clz(P.page_size), n = p < 0 ? 0 : (int)(p >> shift) + 1;
   int32_t* out = P.pages + row * P.n_select;
-  const uint64_t* keys = (const uint64_t*)P.work + row * S.pitch;
+  const uint64_t* keys = (const uint64_t*)P.work + (int64_t)blockIdx.x * S.pitch;
   const int each = (n + PG_NT - 1) / PG_NT, first = (int)threadIdx.x * each;
   const bool kept = each <= KEEP;  // in registers, else read again whenever they are looked at
   uint64_t mine[KEEP];
@@ -808,9 +809,16 @@ extern "C" int sah_page_bounds(const sah_page_bounds_args* given) {
   return sah_launch_status(what);
 }
 
+// Rows of a slice: all of them up to 256 MiB of keys (2048 tokens, 8 key heads, tables of 131072 tokens in pages of
+// 16: 1 GiB; in slices 16.1 ms instead of 18.7 over 130000 keys, 0.97 instead of 0.91 over 20000).
+#define PG_SELECT_BYTES (1 << 28)
+static int64_t pg_select_rows(const sah_page_select_args* a) {
+  const int64_t rows = (int64_t)a->requests.n_tokens * a->Hkv, room = PG_SELECT_BYTES / ((int64_t)a->requests.table_width * 8);
+  return rows < room ? rows : room > 1 ? room : 1;
+}
 extern "C" int64_t sah_page_select_work_bytes(const sah_page_select_args* a) {
   if (!a || a->requests.n_tokens <= 0 || a->Hkv <= 0 || a->requests.table_width <= 0) return 0;
-  return (int64_t)a->requests.n_tokens * a->Hkv * a->requests.table_width * 8;
+  return pg_select_rows(a) * a->requests.table_width * 8;
 }
 
 extern "C" int sah_page_select(const sah_page_select_args* given) {
@@ -838,24 +846,28 @@ extern "C" int sah_page_select(const sah_page_select_args* given) {
   const int per = PG_WAVE_PAGES * (PG_NT / SAH_WAVE), width = a->requests.table_width;
   const int64_t hint = ((int64_t)a->max_context + a->page_size - 1) / a->page_size;
   const int usual = hint > 0 && hint < width ? (int)hint : width;  // pages of the longest request, by what the caller says
+  if (rows > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_select: too many rows");
+  const int64_t most = pg_select_rows(a), room = PG_SCORE_WGS / most > 1 ? PG_SCORE_WGS / most : 1;
   int64_t chunks = (usual + per - 1) / per;
-  const int64_t room = PG_SCORE_WGS / rows > 1 ? PG_SCORE_WGS / rows : 1;
   if (chunks > room) chunks = room;
-  const pg_select s{*a, width, (int)chunks};
-  if (rows * s.chunks > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_select: too many rows");
   hipStream_t st = (hipStream_t)a->stream;
-  const dim3 grid((unsigned)(rows * s.chunks));
-  {
-    sah_timed timed("k_page_scores", a->stream);
-    const int dp = a->D <= 64 ? 64 : a->D <= 128 ? 128 : 256;
+  for (int64_t row0 = 0; row0 < rows; row0 += most) {
+    const int64_t n = rows - row0 < most ? rows - row0 : most;
+    const pg_select s{*a, row0, width, (int)chunks};
+    {
+      sah_timed timed("k_page_scores", a->stream);
+      const dim3 grid((unsigned)(n * chunks));
+      const int dp = a->D <= 64 ? 64 : a->D <= 128 ? 128 : 256;
 #define PG_CASE(bt, d) if (a->bounds_dtype == bt && dp == d) hipLaunchKernelGGL((k_page_scores<bt, d>), grid, dim3(PG_NT), 0, st, s);
-    PG_CASE(SAH_F32, 64) PG_CASE(SAH_F32, 128) PG_CASE(SAH_F32, 256)
-    PG_CASE(SAH_BF16, 64) PG_CASE(SAH_BF16, 128) PG_CASE(SAH_BF16, 256)
-    PG_CASE(SAH_F16, 64) PG_CASE(SAH_F16, 128) PG_CASE(SAH_F16, 256)
+      PG_CASE(SAH_F32, 64) PG_CASE(SAH_F32, 128) PG_CASE(SAH_F32, 256)
+      PG_CASE(SAH_BF16, 64) PG_CASE(SAH_BF16, 128) PG_CASE(SAH_BF16, 256)
+      PG_CASE(SAH_F16, 64) PG_CASE(SAH_F16, 128) PG_CASE(SAH_F16, 256)
 #undef PG_CASE
-    if (int rc = sah_launch_status("sah_page_select")) return rc;
+      if (int rc = sah_launch_status("sah_page_select")) return rc;
+    }
+    sah_timed timed("k_page_top", a->stream);
+    hipLaunchKernelGGL(k_page_top, dim3((unsigned)n), dim3(PG_NT), 0, st, s);
+    if (int rc = sah_launch_status("sah_page_select(top)")) return rc;
   }
-  sah_timed timed("k_page_top", a->stream);
-  hipLaunchKernelGGL(k_page_top, dim3((unsigned)rows), dim3(PG_NT), 0, st, s);
-  return sah_launch_status("sah_page_select(top)");
+  return SAH_OK;
 }

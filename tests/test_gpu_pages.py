@@ -788,6 +788,21 @@ def test_pages_of_many_requests(cuda, n):
     _select_case(cuda, torch.bfloat16, torch.bfloat16, new, cached, 4, 2, 16, 8, 6, seed=n, pad=2)
 
 
+@pytest.mark.parametrize("new, cached, kv_heads", [([9, 0, 5], [700, 3, 90], 3), ([1, 30], [2000, 0], 1)])
+def test_select_in_slices(cuda, new, cached, kv_heads):
+    """Tables so wide that a call's workspace has room for a few of its rows at a time: 5 rows a slice, which end inside a token's key heads."""
+    case = Case(cuda, torch.bfloat16, new, cached, kv_heads, 32, 8, seed=3)
+    width = 2 ** 28 // 8 // 5
+    table = torch.full((len(new), width), -1, dtype=torch.int32, device=cuda)
+    table[:, :case.width] = case.table
+    bounds = torch.stack([case.wide[0].amin(1), case.wide[0].amax(1)], 2).to(torch.bfloat16)
+    q = torch.randn(case.cu[-1] + 4, 2 * kv_heads, 32, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    want = _plain_select(q, bounds.double(), case, 2, 12, 1, 1)
+    for max_context in (None, 100, 2100):
+        got = P.select_pages(q.to(cuda), bounds.to(cuda), table, case.kv_lens, case.cu_new, 8, 12, max_context=max_context)
+        assert torch.equal(got.long().cpu(), want)
+
+
 @pytest.mark.parametrize("kind", [torch.bfloat16, _E4M3])
 def test_a_batch_of_padding_alone(cuda, kind):
     """Rows, but no request that has one: nothing is written, nothing selected."""

@@ -222,6 +222,16 @@ def test_the_copy_of_a_chunk_has_room_for_what_the_caller_says(dtype):
         assert attention(slots, 4096, hint, width) <= rest
 
 
+def test_the_workspace_of_a_selection_is_bounded():
+    def select(tokens, width, Hkv=8):
+        return N.page_work_bytes("select", N.PageSelectArgs(Hkv=Hkv, requests=N.PageRequests(table_width=width, n_tokens=tokens)))
+
+    assert select(100, 8192) == 100 * 8 * 8192 * 8
+    assert select(512, 8192) == 2 ** 28 == select(513, 8192) == select(2 ** 20, 8192)
+    assert 2 ** 28 - 3000 * 8 < select(2 ** 20, 3000) <= 2 ** 28
+    assert select(9, 2 ** 26) == 2 ** 29  # a row's keys are a row's
+
+
 def test_tensors_on_the_host_are_refused():
     i32, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32)
     cache = torch.zeros(8, 16, 2, 64).to(_E4M3)
