@@ -52,7 +52,7 @@ int sah_page_store(const sah_page_store_args* a);
 
 /* Reads requests' contexts back: k_out and v_out [n_requests, Hkv, length, D] (contiguous) hold the tokens at positions below kv_lens[b], and 0 from
  * there on and on pages that are not there. dtype: the cache's, or for SAH_E4M3 any of the three; SAH_F16 then ends at its
- * largest number, +-65504. Of `requests` cu_new and n_tokens are not looked at. */
+ * largest number, +-65504. Of `requests` cu_new and n_tokens are not looked at. k_out and v_out share no memory with each other or with what is read (refused). */
 typedef struct sah_page_load_args {
   sah_page_cache cache;
   sah_page_requests requests;
@@ -67,7 +67,7 @@ int sah_page_load(const sah_page_load_args* a);
 /* Bounds [n_pages, Hkv, 2, D] (contiguous; the cache's type, for SAH_E4M3 bf16, which holds them exactly): the smallest and, behind it, the largest
  * element of each channel of a page's keys, NaN where one of them is. Brings those of the pages that the step has filled up to date: pages whose last
  * token is one of the cu_new[b + 1] - cu_new[b] last ones of kv_lens[b]. All others stay as they were. Keys have been written before; v, its strides and scales
- * and n_tokens are not looked at. */
+ * and n_tokens are not looked at. Bounds share no memory with what is read (refused). */
 typedef struct sah_page_bounds_args {
   sah_page_cache cache;
   sah_page_requests requests;
@@ -84,7 +84,7 @@ int sah_page_bounds(const sah_page_bounds_args* a);
  * their ranks do not hang on the order of a sum; one that is not finite ranks above all others. Pages that the table does not have are no
  * candidates. pages [n_tokens, Hkv, n_select]: places in the request's row of the table, rising, -1 behind the last; -1 alone for rows behind the
  * last request's. Only bounds of candidates that are not taken anyway are read. sink_pages + window_pages <= n_select, window_pages >= 1.
- * Addresses and strides of q and bounds are multiples of 16 bytes. max_context: as for sah_paged_attention. work: sah_page_select_work_bytes(a) bytes
+ * Addresses and strides of q and bounds are multiples of 16 bytes; pages share no memory with what is read (refused). max_context: as for sah_paged_attention. work: sah_page_select_work_bytes(a) bytes
  * (8 a token, key head and entry of the table, up to 256 MiB or a single row's), 16-byte aligned, no particular content. */
 typedef struct sah_page_select_args {
   const void* q; int64_t qs_t, qs_h;

@@ -16,7 +16,6 @@
 // A 32-key step's K is requested as soon as the step before has been multiplied with its own, V likewise: half a step or more is under way at all times.
 // (Two steps ahead: 412 instead of 404 us, lists that several tokens share 85 instead of 59: the registers cost waves.)
 #include "sah_pages.h"
-#include "sah_spans.h"
 
 #define PT_NT 256
 #define PT_NW (PT_NT / SAH_WAVE)
@@ -1153,14 +1152,8 @@ extern "C" int sah_page_attention(const sah_page_attention_args* given) {
   const sah_span out = sah_span_of<2>(a->out, es, c.D, {a->os_t, a->os_h}, {r.n_tokens, a->Hq});
   if (sah_out_on_queries(a->q, a->qs_t, a->qs_h, a->out, a->os_t, a->os_h, r.n_tokens, a->Hq, c.D, es))
     return sah_fail(SAH_EINVAL, "sah_page_attention: out shares memory with q");
-  const int ces = pg_size(c.dtype);
-  const int64_t scales = c.dtype == SAH_E4M3 ? (int64_t)c.n_pages * c.Hkv * c.page_size : 0;
-  if (sah_meet(out, sah_span_of<3>(c.k, ces, c.D, {c.ks_p, c.ks_t, c.ks_h}, {c.n_pages, c.page_size, c.Hkv})) ||
-      sah_meet(out, sah_span_of<3>(c.v, ces, c.D, {c.vs_p, c.vs_t, c.vs_h}, {c.n_pages, c.page_size, c.Hkv})) ||
-      (scales && (sah_meet(out, sah_span_of<1>(c.k_scales, 1, scales, {0}, {1})) || sah_meet(out, sah_span_of<1>(c.v_scales, 1, scales, {0}, {1})))) ||
-      sah_meet(out, sah_span_of<1>(r.block_table, 4, r.table_width, {r.table_pitch}, {r.n_requests})) ||
-      sah_meet(out, sah_span_of<1>(r.kv_lens, 4, 1, {1}, {r.n_requests})) || sah_meet(out, sah_span_of<1>(r.cu_new, 4, 1, {1}, {r.n_requests + 1})) ||
-      (a->pages && sah_meet(out, sah_span_of<1>(a->pages, 4, (int64_t)r.n_tokens * c.Hkv * a->n_select, {0}, {1}))) ||
+  if (pg_on_cache(out, c) || pg_on_requests(out, r, true) ||
+      (a->pages && sah_meet(out, pg_span(a->pages, r.n_tokens, c.Hkv, a->n_select, 4))) ||
       (a->sinks && sah_meet(out, sah_span_of<1>(a->sinks, 4, 1, {1}, {a->Hq}))))
     return sah_fail(SAH_EINVAL, "sah_page_attention: out lies within the cache, the table, the lists or the lengths");
   int wgs;

@@ -1,6 +1,7 @@
 // What the kernels on 8-bit pages and on pages' bounds share: a token's request, elements of e4m3, checks of arguments.
 #pragma once
 #include "sah_common.h"
+#include "sah_spans.h"
 #include "../../include/sah_pages.h"
 
 #define PG_MAX_D 256
@@ -135,6 +136,25 @@ static inline int pg_check_requests(const sah_page_requests& r, int page_size, b
   if (r.table_pitch < r.table_width) return sah_fail(SAH_EINVAL, "%s: table_pitch is less than table_width", what);
   if (!r.block_table || !r.kv_lens || (with_rows && !r.cu_new)) return sah_fail(SAH_ENULL, "%s: NULL pointer", what);
   return SAH_OK;
+}
+
+// A contiguous tensor of a * b * c elements (more than memory has: as far as addresses go)
+static inline sah_span pg_span(const void* p, int64_t a, int64_t b, int64_t c, int es) {
+  const double bytes = (double)a * b * c * es;
+  return sah_span{(int64_t)(uint64_t)p, bytes < 0x1p62 ? (int64_t)(uint64_t)p + a * b * c * es : INT64_MAX};
+}
+// Whether an output lies on keys, values (which stand for keys where a call has none) or their scales
+static inline bool pg_on_cache(const sah_span& out, const sah_page_cache& c) {
+  const int es = pg_size(c.dtype);
+  return sah_meet(out, sah_span_of<3>(c.k, es, c.D, {c.ks_p, c.ks_t, c.ks_h}, {c.n_pages, c.page_size, c.Hkv})) ||
+         sah_meet(out, sah_span_of<3>(c.v, es, c.D, {c.vs_p, c.vs_t, c.vs_h}, {c.n_pages, c.page_size, c.Hkv})) ||
+         (c.dtype == SAH_E4M3 && (sah_meet(out, pg_span(c.k_scales, c.n_pages, c.Hkv, c.page_size, 1)) || sah_meet(out, pg_span(c.v_scales, c.n_pages, c.Hkv, c.page_size, 1))));
+}
+// ... on the table or the lengths
+static inline bool pg_on_requests(const sah_span& out, const sah_page_requests& r, bool with_rows) {
+  return sah_meet(out, sah_span_of<1>(r.block_table, 4, r.table_width, {r.table_pitch}, {r.n_requests})) ||
+         sah_meet(out, sah_span_of<1>(r.kv_lens, 4, 1, {1}, {r.n_requests})) ||
+         (with_rows && sah_meet(out, sah_span_of<1>(r.cu_new, 4, 1, {1}, {r.n_requests + 1})));
 }
 
 // Where a context's copy goes. Strides of the outputs in elements. A table, where given, names the copies' pages (of a cache whose pages follow

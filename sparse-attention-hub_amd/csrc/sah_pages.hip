@@ -779,7 +779,11 @@ extern "C" int sah_page_load(const sah_page_load_args* given) {
   if (a->length == 0) return SAH_OK;
   if (!a->k_out || !a->v_out) return sah_fail(SAH_ENULL, "sah_page_load: NULL pointer");
   if (((uint64_t)a->k_out | (uint64_t)a->v_out) % 16) return sah_fail(SAH_EINVAL, "sah_page_load: addresses must be multiples of 16 bytes");
+  if (!pg_load_workgroups(c, a->requests, a->length)) return sah_fail(SAH_ESHAPE, "sah_page_load: too many elements");
   const int64_t row = c.D, head = row * a->length;
+  const sah_span k = pg_span(a->k_out, a->requests.n_requests, c.Hkv, head, pg_size(a->dtype)), v = pg_span(a->v_out, a->requests.n_requests, c.Hkv, head, pg_size(a->dtype));
+  if (sah_meet(k, v) || pg_on_cache(k, c) || pg_on_cache(v, c) || pg_on_requests(k, a->requests, false) || pg_on_requests(v, a->requests, false))
+    return sah_fail(SAH_EINVAL, "sah_page_load: k_out or v_out shares memory with the other, the cache, the table or the lengths");
   return pg_load(c, a->requests, a->dtype, pg_load_out{a->k_out, a->v_out, head * c.Hkv, head, row, a->length, nullptr, nullptr}, a->stream, what);
 }
 
@@ -793,6 +797,9 @@ extern "C" int sah_page_bounds(const sah_page_bounds_args* given) {
   if (int rc = pg_check_requests(a->requests, c.page_size, true, what)) return rc;
   if (!a->bounds) return sah_fail(SAH_ENULL, "sah_page_bounds: NULL pointer");
   if ((uint64_t)a->bounds % 16) return sah_fail(SAH_EINVAL, "sah_page_bounds: addresses must be multiples of 16 bytes");
+  const sah_span bounds = pg_span(a->bounds, c.n_pages, c.Hkv, 2 * c.D, c.dtype == SAH_E4M3 ? 2 : pg_size(c.dtype));
+  if (pg_on_cache(bounds, c) || pg_on_requests(bounds, a->requests, true))
+    return sah_fail(SAH_EINVAL, "sah_page_bounds: bounds share memory with the keys, the table or the lengths");
   // Enough waves for the card where few requests have filled many pages; each of many requests' fills few.
   const int64_t rows = (int64_t)a->requests.n_requests * c.Hkv;
   int64_t n_waves = PG_BOUND_WAVES / rows;
@@ -843,10 +850,14 @@ extern "C" int sah_page_select(const sah_page_select_args* given) {
   if (((uint64_t)a->q | (uint64_t)a->bounds | (uint64_t)(pg_size(a->dtype) * (a->qs_t | a->qs_h))) % 16)
     return sah_fail(SAH_EINVAL, "sah_page_select: addresses and strides must be multiples of 16 bytes");
   const int64_t rows = (int64_t)a->requests.n_tokens * a->Hkv;
+  if (rows > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_select: too many rows");
+  const sah_span pages = pg_span(a->pages, rows, a->n_select, 1, 4);
+  if (sah_meet(pages, sah_span_of<2>(a->q, pg_size(a->dtype), a->D, {a->qs_t, a->qs_h}, {a->requests.n_tokens, a->Hq})) ||
+      sah_meet(pages, pg_span(a->bounds, a->n_pages, a->Hkv, 2 * a->D, pg_size(a->bounds_dtype))) || pg_on_requests(pages, a->requests, true))
+    return sah_fail(SAH_EINVAL, "sah_page_select: pages share memory with the queries, the bounds, the table or the lengths");
   const int per = PG_WAVE_PAGES * (PG_NT / SAH_WAVE), width = a->requests.table_width;
   const int64_t hint = ((int64_t)a->max_context + a->page_size - 1) / a->page_size;
   const int usual = hint > 0 && hint < width ? (int)hint : width;  // pages of the longest request, by what the caller says
-  if (rows > 0x7fffffff) return sah_fail(SAH_ESHAPE, "sah_page_select: too many rows");
   const int64_t most = pg_select_rows(a), room = PG_SCORE_WGS / most > 1 ? PG_SCORE_WGS / most : 1;
   int64_t chunks = (usual + per - 1) / per;
   if (chunks > room) chunks = room;

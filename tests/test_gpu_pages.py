@@ -278,6 +278,27 @@ def test_page_bounds_of_refused_requests_and_bad_lengths(cuda):
     assert torch.equal(bounds.double().cpu(), want)
 
 
+@pytest.mark.parametrize("kind", _KINDS)
+def test_page_bounds_beside_the_keys_and_on_them(cuda, kind):
+    """One buffer: right before the keys and right behind them, and 16 bytes further in, where they are refused."""
+    case = Case(cuda, kind, [70], [5], 2, 64, 16)
+    cache, held = case.caches[0], torch.bfloat16 if kind == _E4M3 else kind
+    pages, size = cache.shape[0], cache.numel() * cache.element_size()
+    room = pages * 2 * 2 * 64 * (2 if kind == _E4M3 else cache.element_size())
+    buffer = torch.zeros(2 * room + size, dtype=torch.uint8, device=cuda)
+    buffer[room:room + size] = cache.view(torch.uint8).flatten()
+    keys = buffer[room:room + size].view(cache.dtype).view(cache.shape)
+    want = torch.zeros(pages, 2, 2, 64, dtype=held, device=cuda)
+    P.update_page_bounds(want, cache, case.table, case.kv_lens, case.cu_new, key_scales=case.scales[0])
+    for at in (0, room + size):
+        bounds = buffer[at:at + room].view(held).view(want.shape)
+        P.update_page_bounds(bounds, keys, case.table, case.kv_lens, case.cu_new, key_scales=case.scales[0])
+        assert torch.equal(bounds, want)
+    for at in (16, room + size - 16):
+        with pytest.raises(ValueError, match="share memory"):
+            P.update_page_bounds(buffer[at:at + room].view(held).view(want.shape), keys, case.table, case.kv_lens, case.cu_new, key_scales=case.scales[0])
+
+
 # ----------------------------------------------------------------------------------------------------------------- select
 def _plain_select(q, bounds, case, group, n_select, sink, window):
     """By the rule, one row after the other. `bounds`: (pages, kv_heads, 2, dim) in 64 bits."""

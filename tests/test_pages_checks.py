@@ -232,6 +232,28 @@ def test_the_workspace_of_a_selection_is_bounded():
     assert select(9, 2 ** 26) == 2 ** 29  # a row's keys are a row's
 
 
+# _cache(): 8 pages of 16 tokens and 2 heads of 64, its scales 256 bytes; _requests(): a table of 4 entries, one length, two sums
+@pytest.mark.parametrize("dtype, size", [(0, 4), (1, 2)])
+def test_outputs_on_what_a_call_reads_are_refused(dtype, size):
+    out = 2 * 40 * 64 * size  # bytes of a context read back
+    held = N.PageLoadArgs(_cache(), _requests(), 8 * _FAR, 9 * _FAR, dtype, 40, None)
+    ends = [_FAR + 8 * 2048 - 16, 2 * _FAR + 8 * 2048 - 16, 3 * _FAR + 240, 4 * _FAR + 240, 5 * _FAR, 6 * _FAR, _FAR - out + 16]
+    for field in ("k_out", "v_out"):
+        for at in ends + [8 * _FAR + out - 16 if field == "v_out" else 9 * _FAR - out + 16]:
+            assert _call("sah_page_load", N.PageLoadArgs.from_buffer_copy(held), **{field: at}) == -1, at
+    for cache_dtype, unit in ((N.SAH_E4M3, 1), (1, 2), (0, 4)):
+        whole = 8 * 2 * 2 * 64 * (2 if cache_dtype == N.SAH_E4M3 else unit)  # bytes of bounds
+        for at in [_FAR + 8 * 2048 * unit - 16, 5 * _FAR, 6 * _FAR, 7 * _FAR, _FAR - whole + 16] + ([3 * _FAR + 240] if unit == 1 else []):
+            assert _call("sah_page_bounds", N.PageBoundsArgs(_cache(v=None, dtype=cache_dtype), _requests(), at, None)) == -1, at
+
+    def select(**changes):  # 3 tokens of 4 heads of 64 in 16 bits, bounds 8 * 2 * 2 * 64
+        args = N.PageSelectArgs(8 * _FAR, 256, 64, 9 * _FAR, 1, 1, 4, 2, 64, 8, 16, _requests(), 3, 1, 2, 0, 10 * _FAR, 11 * _FAR, 2 ** 20, None)
+        return _call("sah_page_select", args, **changes)
+
+    for at in (8 * _FAR + 3 * 512 - 4, 9 * _FAR + 8 * 2 * 2 * 64 * 2 - 4, 8 * _FAR - 3 * 2 * 3 * 4 + 4, 5 * _FAR + 12, 6 * _FAR, 7 * _FAR + 4):
+        assert select(pages=at) == -1, at
+
+
 def test_tensors_on_the_host_are_refused():
     i32, table = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32)
     cache = torch.zeros(8, 16, 2, 64).to(_E4M3)
