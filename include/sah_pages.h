@@ -1,5 +1,7 @@
 /* Entry points of libsah_mi355.so for a paged cache (sah_serve.h) that is held in 8 bits, and for attention over the pages that matter to
- * a token. The reference has no counterpart: its caches are contiguous, in the model's type, and its maskers select single keys.
+ * a token. The reference's caches are contiguous and in the model's type; its QuestTopKMasker (maskers/fixed/implementations/quest_top_k.py:58) takes pages
+ * by the smallest and largest elements of their keys into a mask over a contiguous cache. That score was published as Quest (Tang et al., 2024); here it is summed
+ * over the query heads that share a key head, and pages that are not selected are not read.
  * Conventions and error codes are sah.h's, what a cache, a table, a slot and a step are is sah_serve.h's.
  *
  * Eight bits: an element is a number of e4m3 (4 bits of exponent, 3 of mantissa, NaN but no infinity; torch.float8_e4m3fn) times
@@ -80,8 +82,9 @@ int sah_page_bounds(const sah_page_bounds_args* a);
  * the first sink_pages and the last window_pages (its own is the last one), and of the others, up to n_select in all, those of the largest
  *     score(page) = sum over h's query heads and over channels c of max(q_c * smallest_c, q_c * largest_c),
  * ties to the lower page. (What is summed over c is the largest q . k that a key of the page can reach. An infinite bound counts where its product is the larger
- * one; 0 times it is no number.) Scores are held in 64 bits, so that
- * their ranks do not hang on the order of a sum; one that is not finite ranks above all others. Pages that the table does not have are no
+ * one; 0 times it is no number.) Scores are held in 64 bits and summed in
+ * an order that D and the bounds' type fix: equal bounds score the same and results repeat; scores that are closer to each other than some 4 D * 2^-53 of the sum of
+ * their terms' sizes may rank either way. One that is not finite ranks above all others. Pages that the table does not have are no
  * candidates. pages [n_tokens, Hkv, n_select]: places in the request's row of the table, rising, -1 behind the last; -1 alone for rows behind the
  * last request's. Only bounds of candidates that are not taken anyway are read. sink_pages + window_pages <= n_select, window_pages >= 1.
  * Addresses and strides of q and bounds are multiples of 16 bytes; pages share no memory with what is read (refused). max_context: as for sah_paged_attention. work: sah_page_select_work_bytes(a) bytes

@@ -323,7 +323,7 @@ __global__ __launch_bounds__(PG_NT) void k_page_bounds(sah_page_bounds_args P, i
 // ---------------------------------------------------------------------------
 // select: a 64-bit key per candidate (larger: rather taken), then the largest of a row
 // The sum over heads of max(q a, q b) with a <= b, both finite, is Q+ . b + Q- . a, Q+ (Q-) the sum of the heads' positive (negative) elements: the heads
-// share one reading of the bounds and one pair of products (pages of infinite bounds: pg_score_again). In fp64, so that no order of sums changes a rank; fp32 is no faster (72 us against 70): reading the
+// share one reading of the bounds and one pair of products (pages of infinite bounds: pg_score_again). In fp64, in which rounding decides between almost equal scores alone; fp32 is no faster (72 us against 70): reading the
 // bounds is what it costs. 64 answers of 1K to 32K keys in pages of 16, 8 heads: 277 MB of bf16 bounds, 61 us, 4.5 TB/s; they are read past the caches, which
 // they would go through once (71 us). All heads of a page by one wave 97 us, smallest and largest by neighbouring lanes 80.
 // ---------------------------------------------------------------------------

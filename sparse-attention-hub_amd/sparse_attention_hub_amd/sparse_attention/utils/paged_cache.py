@@ -17,7 +17,8 @@ A cache may be held in 8 bits: `torch.float8_e4m3fn` tensors of the same shape a
 with such a cache. `load_paged` reads contexts back, as the contiguous tensors that the maskers and `ResearchAttention` take.
 
 A token may attend to a few pages instead of all: `update_page_bounds` keeps the smallest and largest element of every channel of the pages'
-keys, `select_pages` chooses a token's pages by how large a logit they can hold, `paged_attention(..., pages=...)` attends to them.
+keys, `select_pages` chooses a token's pages by how large a logit they can hold (the score of Quest, Tang et al., 2024, which the reference has as a masker:
+`maskers/fixed/implementations/quest_top_k.py:58`), `paged_attention(..., pages=...)` attends to them.
 """
 from __future__ import annotations
 
@@ -348,7 +349,7 @@ def select_pages(queries: torch.Tensor, bounds: torch.Tensor, block_table: torch
     Of the pages at or before the token's own: the first `sink_pages`, the last `window_pages` (at least 1, its own), and of the others as many as
     make `n_select` with the largest `sum over the key head's query heads and over channels of max(q * smallest, q * largest)`, the most
     that the heads' products with a key of the page can come to together; ties to the lower page, scores that are not finite first. Scores are
-    held in 64 bits: the same pages whatever the order of sums. Pages that are not there are no candidates. `bounds` as
+    held in 64 bits and summed in one order: results repeat, and only scores within 4 head_dim * 2^-53 of the sum of their terms' sizes may rank either way. Pages that are not there are no candidates. `bounds` as
     `update_page_bounds` keeps them. `max_context` as for `paged_attention`.
     """
     N.require_device(queries, "queries")
