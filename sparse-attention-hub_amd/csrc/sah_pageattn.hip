@@ -1013,55 +1013,63 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
 // 128 rows 74 / 84, 256 rows 124 / 99, 512 rows 222 / 137; of those keys 512 + 128 seen, 1024 rows 56 / 70, 4096 rows 191 / 129; 2 requests of
 // 32768, 2048 + 128 seen, 1024 rows 84 / 129, 4096 rows 248 / 175). Never for fp32 q: its terms go at the 16-bit matrix rate here, an fp32 copy at a
 // tenth of it (4 requests of 8192 keys, 128 rows 80 / 268, 2048 rows 947 / 2952).
-// A copy has room for max_context tokens a request where that is given: tables are as wide as a server's longest request may become (16 of 131072 tokens,
-// 8 heads of 128: 8 GiB, of 4096 tokens 256 MiB). It is no more than 2 GiB, under a hundredth of the card's memory; beyond, the cache is attended to as it is.
-// (2048 tokens of one request over 4096 keys, 32 tables of 131072: 149 us by a copy of 4096 tokens each, 407 as it is; 543 where the copy was too short. 1024
-// tokens, 16 such tables: 108, 202.)
+// A copy has room for max_context tokens of every request (the table's where that is not given) while this comes to no more than 2 GiB. Tables are as wide as a
+// server's longest request may become (16 of 131072 tokens, 8 heads of 128: 8 GiB): beyond that contexts are copied one behind the other, into as many
+// pages as the cache has, 2 GiB at most. (2048 tokens of one request over 16384 keys, 32 tables of 18432: 662 us; as it is 1699, alone in its table 658.)
 //
-// fp16 does not hold all that an 8-bit cache can, and a context may be longer than max_context says: the copy's workgroups tell where that is so, and the
-// cache is then attended to as it is, all rows once more (copies that hold everything pay for it with two launches that end at once: 4 requests of 64 fp16
-// tokens over 8192 keys 104 -> 113 us).
+// fp16 does not hold all that an 8-bit cache can, a context may be longer than max_context says, and all of them may need more room than there is: the copy's
+// workgroups tell where that is so, and the cache is then attended to as it is, all rows once more (copies that hold everything pay for it with two launches that end at
+// once: 4 requests of 64 fp16 tokens over 8192 keys 104 -> 113 us).
 #define PT_COPY_BYTES 0x1p31
 struct pt_copy {
-  int64_t bytes;    // K, V, their table and what was lost; 0: none
-  int width;        // pages of a request
-  int64_t lost_at;  // where the last of these begins
+  int64_t bytes;    // K, V, their table, places and what was lost; 0: none
+  int width;        // pages of a request, at most
+  int64_t pages;    // of all
+  int64_t table_at, placed_at, lost_at;  // placed_at: first pages and lengths, where contexts lie one behind the other, else 0
   int n_lost;       // 0: the copy holds everything
 };
 static pt_copy pt_copy_of(const sah_page_attention_args* a) {
-  const pt_copy none{0, 0, 0, 0};
-  if (a->pages || a->cache.dtype != SAH_E4M3 || a->dtype == SAH_F32) return none;
-  const int table = a->requests.table_width, page_size = a->cache.page_size;
+  pt_copy c = {};
+  if (a->pages || a->cache.dtype != SAH_E4M3 || a->dtype == SAH_F32) return c;
+  const int table = a->requests.table_width, page_size = a->cache.page_size, n = a->requests.n_requests;
   const double keys = (double)table * page_size, reach = (double)a->sink + a->window, seen = a->window && reach < keys ? reach : keys;
   const double rows = (double)a->requests.n_tokens * (a->Hq / a->cache.Hkv);
-  if (rows * seen <= 128 * keys * a->requests.n_requests) return none;
-  pt_copy c;
+  if (rows * seen <= 128 * keys * n) return c;
   const int64_t hint = ((int64_t)a->max_context + page_size - 1) / page_size;
   c.width = hint > 0 && hint < table ? (int)hint : table;
-  const double pages = (double)a->requests.n_requests * c.width, bytes = pages * page_size * a->cache.Hkv * a->cache.D * pg_size(a->dtype) * 2;
-  if (bytes > PT_COPY_BYTES || pages * 4 > PT_COPY_BYTES) return none;
-  c.lost_at = (int64_t)bytes + ((int64_t)pages * 4 + 15) / 16 * 16;
-  c.n_lost = a->dtype == SAH_F16 || c.width < table ? (int)pg_load_workgroups(a->cache, a->requests, c.width * page_size) : 0;
-  c.bytes = c.lost_at + (c.n_lost + 15) / 16 * 16;
+  const double page = (double)page_size * a->cache.Hkv * a->cache.D * pg_size(a->dtype) * 2;
+  c.pages = (int64_t)n * c.width;
+  if (c.pages * 4.0 > PT_COPY_BYTES / 8) return c;  // (their table)
+  const bool placed = c.pages * page > PT_COPY_BYTES;
+  if (placed) {
+    const int64_t room = (int64_t)(PT_COPY_BYTES / page), least = a->cache.n_pages < room ? a->cache.n_pages : room;
+    if (least < c.pages) c.pages = least;
+    if (c.pages == 0) return c;
+  }
+  auto round = [](int64_t v) { return (v + 15) / 16 * 16; };
+  c.table_at = c.pages * (int64_t)page;
+  c.placed_at = placed ? round(c.table_at + (int64_t)n * c.width * 4) : 0;
+  c.lost_at = placed ? round(c.placed_at + (int64_t)n * 8) : round(c.table_at + (int64_t)n * c.width * 4);
+  c.n_lost = a->dtype == SAH_F16 || c.width < table || placed ? (int)pg_load_workgroups(a->cache, a->requests, c.width * page_size) : 0;
+  c.bytes = round(c.lost_at + c.n_lost);
   return c;
 }
-static sah_paged_attention_args pt_on_copy(const sah_page_attention_args* a, int width) {
+static sah_paged_attention_args pt_on_copy(const sah_page_attention_args* a, const pt_copy& copy) {
   const sah_page_cache& c = a->cache;
   sah_paged_attention_args p = {};
-  const int64_t row = c.D, token = row * c.Hkv, page = token * c.page_size, pages = (int64_t)a->requests.n_requests * width;
-  const int es = pg_size(a->dtype);
+  const int64_t row = c.D, token = row * c.Hkv, page = token * c.page_size;
   char* k = (char*)a->work;
   p.q = a->q; p.qs_t = a->qs_t; p.qs_h = a->qs_h;
   p.k = k; p.ks_p = page; p.ks_t = token; p.ks_h = row;
-  p.v = k + pages * page * es; p.vs_p = page; p.vs_t = token; p.vs_h = row;
-  p.block_table = (const int32_t*)(k + 2 * pages * page * es);
-  p.table_pitch = p.table_width = width;
-  p.kv_lens = a->requests.kv_lens;
+  p.v = k + copy.table_at / 2; p.vs_p = page; p.vs_t = token; p.vs_h = row;
+  p.block_table = (const int32_t*)(k + copy.table_at);
+  p.table_pitch = p.table_width = copy.width;
+  p.kv_lens = copy.placed_at ? (const int32_t*)(k + copy.placed_at) + a->requests.n_requests : a->requests.kv_lens;
   p.cu_new = a->requests.cu_new;
   p.sinks = a->sinks;
   p.dtype = a->dtype;
   p.n_requests = a->requests.n_requests; p.n_tokens = a->requests.n_tokens; p.Hq = a->Hq; p.Hkv = c.Hkv; p.D = c.D;
-  p.n_pages = (int)pages; p.page_size = c.page_size;
+  p.n_pages = (int)copy.pages; p.page_size = c.page_size;
   p.max_context = a->max_context; p.sink = a->sink; p.window = a->window;
   p.scaling = a->scaling;
   p.out = a->out; p.os_t = a->os_t; p.os_h = a->os_h;
@@ -1080,7 +1088,7 @@ extern "C" int64_t sah_page_attention_work_bytes(const sah_page_attention_args* 
   const int64_t own = (int64_t)wgs * 2 * (A.heads * PT_ROWS * (pt_dim(a) + 4) * 4 + (int64_t)sizeof(pt_record));
   const pt_copy copy = pt_copy_of(a);
   if (!copy.bytes) return own;
-  const sah_paged_attention_args p = pt_on_copy(a, copy.width);
+  const sah_paged_attention_args p = pt_on_copy(a, copy);
   const int64_t others = 4 * sah_paged_attention_work_floats(&p);
   return copy.bytes + (copy.n_lost && own > others ? own : others);  // (one after the other)
 }
@@ -1160,11 +1168,16 @@ extern "C" int sah_page_attention(const sah_page_attention_args* given) {
   pt_args A = pt_plan(a, wgs);
   const pt_copy copy = pt_copy_of(a);
   if (copy.bytes) {
-    sah_paged_attention_args p = pt_on_copy(a, copy.width);
+    sah_paged_attention_args p = pt_on_copy(a, copy);
     const int64_t row = c.D, token = row * c.Hkv, request = token * c.page_size * copy.width;
+    char* work = (char*)a->work;
+    int32_t* first = copy.placed_at ? (int32_t*)(work + copy.placed_at) : nullptr;
     A.n_lost = copy.n_lost;
-    if (copy.n_lost) A.lost = (const uint8_t*)a->work + copy.lost_at;
-    const pg_load_out to{(void*)p.k, (void*)p.v, request, row, token, copy.width * c.page_size, (int32_t*)p.block_table, (uint8_t*)A.lost};
+    if (copy.n_lost) A.lost = (const uint8_t*)work + copy.lost_at;
+    if (first) {
+      if (int rc = pg_place(r, c.page_size, copy.width, copy.pages, first, first + r.n_requests, a->stream, what)) return rc;
+    }
+    const pg_load_out to{(void*)p.k, (void*)p.v, request, row, token, copy.width * c.page_size, (int32_t*)p.block_table, (uint8_t*)A.lost, first};
     if (int rc = pg_load(c, r, a->dtype, to, a->stream, what)) return rc;
     p.work = (float*)((char*)a->work + copy.bytes);
     p.work_floats = (a->work_bytes - copy.bytes) / 4;

@@ -158,14 +158,19 @@ static inline bool pg_on_requests(const sah_span& out, const sah_page_requests& 
 }
 
 // Where a context's copy goes. Strides of the outputs in elements. A table, where given, names the copies' pages (of a cache whose pages follow
-// each other, as many a request as `length` has): what the attention over a copy goes by; what lies behind a context is left as it is then. `lost`, where
-// given with it: a byte for each of pg_load_workgroups() workgroups, whether its request has tokens behind `length`, or an element that is none of the copy's type.
+// each other, as many a request as `length` has, or from page first[b] on): what the attention over a copy goes by; what lies behind a context is left as it is
+// then. `lost`, where given with it: a byte for each of pg_load_workgroups() workgroups, whether its request has tokens behind `length`, or no place, or an element that
+// is none of the copy's type.
 struct pg_load_out {
   void *k, *v;
   int64_t s_b, s_h, s_t;
   int length;
   int32_t* table;
   uint8_t* lost;
+  const int32_t* first;
 };
 int64_t pg_load_workgroups(const sah_page_cache& c, const sah_page_requests& r, int length);  // 0: too many
 int pg_load(const sah_page_cache& c, const sah_page_requests& r, int dtype, const pg_load_out& out, void* stream, const char* what);
+// Places for the contexts of requests with new tokens, one behind the other: first[b], the first of its pages, and lens[b], its length; where `width` pages of a
+// request or `room` in all are not enough -1 and 0 for every request.
+int pg_place(const sah_page_requests& r, int page_size, int width, int64_t room, int32_t* first, int32_t* lens, void* stream, const char* what);

@@ -144,11 +144,13 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
   const int copied = O.length >> shift;  // pages of a copy
   if constexpr (COPY) {
     const int begin = R.cu_new[b], end = R.cu_new[b + 1];
-    if ((begin > 0 ? begin : 0) >= (end < R.n_tokens ? end : R.n_tokens)) {
-      if (O.lost && threadIdx.x == 0) O.lost[blockIdx.x] = 0;
+    const bool idle = (begin > 0 ? begin : 0) >= (end < R.n_tokens ? end : R.n_tokens);
+    if (idle || (O.first && O.first[b] < 0)) {
+      if (O.lost && threadIdx.x == 0) O.lost[blockIdx.x] = !idle;
       return;
     }
   }
+  const int64_t page0 = COPY && O.first ? O.first[b] : (int64_t)b * copied;
   [[maybe_unused]] bool lost = kv > O.length && R.table_width > copied;
   const uint32_t n = COPY && kv < O.length ? (kv > 0 ? kv : 0) : O.length, first = (blockIdx.x - (uint32_t)b * wgs) * PG_NT + threadIdx.x;
   // consecutive threads: a token's units, all heads of it, then the next token: as the cache lies
@@ -162,9 +164,9 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
     const int j = t >> shift, entry = t & (C.page_size - 1);
     const int page = t < kv && j < R.table_width ? R.block_table[(int64_t)b * R.table_pitch + j] : -1;
     const bool there = page >= 0 && page < C.n_pages;
-    if (COPY && entry == 0 && in == 0) O.table[(int64_t)b * copied + j] = there ? b * copied + j : -1;
+    if (COPY && entry == 0 && in == 0) O.table[(int64_t)b * copied + j] = there ? (int)page0 + j : -1;
     if (COPY && !there) continue;
-    const int64_t to = (b * O.s_b + h * O.s_h + t * O.s_t + (int64_t)c * E) * OS;
+    const int64_t to = ((COPY ? page0 * C.page_size * O.s_t : b * O.s_b) + h * O.s_h + t * O.s_t + (int64_t)c * E) * OS;
     char *ko = (char*)O.k + to, *vo = (char*)O.v + to;
     const char* kp = (const char*)C.k + (page * C.ks_p + entry * C.ks_t + h * C.ks_h + c * E) * CS;
     const char* vp = (const char*)C.v + (page * C.vs_p + entry * C.vs_t + h * C.vs_h + c * E) * CS;
@@ -196,6 +198,55 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
     if (!O.lost) return;
     const int any = __syncthreads_or(lost);
     if (threadIdx.x == 0) O.lost[blockIdx.x] = any != 0;
+  }
+}
+
+// One workgroup: how many pages each request needs, then where each one's begin (4 us for 64 requests, nearly all of it the launch and two readings).
+__global__ __launch_bounds__(PG_NT) void k_page_place(sah_page_requests R, int page_size, int width, int64_t room, int32_t* first, int32_t* lens) {
+  __shared__ int64_t s_sum[2][PG_NT / SAH_WAVE];
+  const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id(), shift = 31 - __builtin_clz(page_size), most = R.table_width << shift;
+  auto need = [&](int b, int& kv) -> int {  // pages; 0 also for requests without a row
+    kv = 0;
+    if (b >= R.n_requests) return 0;
+    const int begin = R.cu_new[b], end = R.cu_new[b + 1];
+    if ((begin > 0 ? begin : 0) >= (end < R.n_tokens ? end : R.n_tokens)) return 0;
+    kv = R.kv_lens[b];
+    const int held = kv < 0 ? 0 : (kv < most ? kv : most);
+    return (held >> shift) + ((held & (page_size - 1)) != 0);
+  };
+  int turn = 0;
+  auto before = [&](int64_t v, int64_t& all) -> int64_t {
+    const int64_t incl = (int64_t)sah_wave_incl_scan_u64((uint64_t)v);
+    if (lane == SAH_WAVE - 1) s_sum[turn][wave] = incl;
+    __syncthreads();
+    int64_t sum = incl - v;
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < PG_NT / SAH_WAVE; ++i) {
+      sum += i < wave ? s_sum[turn][i] : 0;
+      all += s_sum[turn][i];
+    }
+    turn ^= 1;  // (the sums of the one before may still be read)
+    return sum;
+  };
+  int64_t total = 0, run = 0, all;
+  int kv;
+  bool more = false;
+  for (int b = threadIdx.x; b < R.n_requests; b += PG_NT) {
+    const int n = need(b, kv);
+    total += n;
+    more |= n > width;
+  }
+  (void)before(total, total);
+  const bool fits = !__syncthreads_or(more) && total <= room;
+  for (int b0 = 0; b0 < R.n_requests; b0 += PG_NT) {
+    const int b = b0 + (int)threadIdx.x, n = need(b, kv);
+    const int64_t at = run + before(n, all);
+    if (b < R.n_requests) {
+      first[b] = fits ? (int)at : -1;
+      lens[b] = fits ? kv : 0;
+    }
+    run += all;
   }
 }
 
@@ -324,7 +375,7 @@ __global__ __launch_bounds__(PG_NT) void k_page_bounds(sah_page_bounds_args P, i
 // select: a 64-bit key per candidate (larger: rather taken), then the largest of a row
 // The sum over heads of max(q a, q b) with a <= b, both finite, is Q+ . b + Q- . a, Q+ (Q-) the sum of the heads' positive (negative) elements: the heads
 // share one reading of the bounds and one pair of products (pages of infinite bounds: pg_score_again). In fp64, in which rounding decides between almost equal scores alone; fp32 is no faster (72 us against 70): reading the
-// bounds is what it costs. 64 answers of 1K to 32K keys in pages of 16, 8 heads: 277 MB of bf16 bounds, 61 us, 4.5 TB/s; they are read past the caches, which
+// bounds is what it costs. 64 answers of 1K to 32K keys in pages of 16, 8 heads: 277 MB of bf16 bounds, 62 us, 4.5 TB/s; they are read past the caches, which
 // they would go through once (71 us). All heads of a page by one wave 97 us, smallest and largest by neighbouring lanes 80.
 // ---------------------------------------------------------------------------
 #define PG_ALWAYS ~0ull        // pages that are taken whatever they score
@@ -765,6 +816,12 @@ int pg_load(const sah_page_cache& c, const sah_page_requests& r, int dtype, cons
   return sah_launch_status(what);
 }
 
+int pg_place(const sah_page_requests& r, int page_size, int width, int64_t room, int32_t* first, int32_t* lens, void* stream, const char* what) {
+  sah_timed timed("k_page_place", stream);
+  hipLaunchKernelGGL(k_page_place, dim3(1), dim3(PG_NT), 0, (hipStream_t)stream, r, page_size, width, room, first, lens);
+  return sah_launch_status(what);
+}
+
 extern "C" int sah_page_load(const sah_page_load_args* given) {
   static const char* what = "sah_page_load";
   if (!given) return sah_fail(SAH_ENULL, "sah_page_load: args is NULL");
@@ -784,7 +841,7 @@ extern "C" int sah_page_load(const sah_page_load_args* given) {
   const sah_span k = pg_span(a->k_out, a->requests.n_requests, c.Hkv, head, pg_size(a->dtype)), v = pg_span(a->v_out, a->requests.n_requests, c.Hkv, head, pg_size(a->dtype));
   if (sah_meet(k, v) || pg_on_cache(k, c) || pg_on_cache(v, c) || pg_on_requests(k, a->requests, false) || pg_on_requests(v, a->requests, false))
     return sah_fail(SAH_EINVAL, "sah_page_load: k_out or v_out shares memory with the other, the cache, the table or the lengths");
-  return pg_load(c, a->requests, a->dtype, pg_load_out{a->k_out, a->v_out, head * c.Hkv, head, row, a->length, nullptr, nullptr}, a->stream, what);
+  return pg_load(c, a->requests, a->dtype, pg_load_out{a->k_out, a->v_out, head * c.Hkv, head, row, a->length, nullptr, nullptr, nullptr}, a->stream, what);
 }
 
 extern "C" int sah_page_bounds(const sah_page_bounds_args* given) {

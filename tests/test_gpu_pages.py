@@ -631,6 +631,72 @@ def test_a_captured_chunk_whose_contexts_pass_the_hint(cuda):
         assert ((eager[:300].double().cpu() - want).abs() <= bound).all(), i
 
 
+@pytest.mark.parametrize("dtype", _TYPES)
+@pytest.mark.parametrize("max_context", [None, 500, 800, 2 ** 20])
+@pytest.mark.parametrize("sink, window", [(0, 0), (40, 1200000)])
+def test_attention_8bit_chunks_in_tables_of_millions_of_keys(cuda, dtype, max_context, sink, window):
+    """Copies of the tables' width would take 4 GiB: contexts with new tokens lie one behind the other."""
+    _attention_case(cuda, dtype, _E4M3, [400, 0, 170, 250], [400, 900, 300, 0], 4, 2, 64, 16, sink, window, sinks=True, seed=5, max_context=max_context, wide=2 ** 17, pad=2,
+                    missing=[(0, 2, -1), (0, 45, 10 ** 6), (2, 0, -3)])
+
+
+def test_attention_8bit_chunks_of_many_requests_in_wide_tables(cuda):
+    """Places are found 256 requests at a time."""
+    rng = random.Random(3)
+    new = [rng.choice([0, 1, 1, 9]) for _ in range(300)]
+    new[7], new[260] = 300, 200
+    cached = [rng.choice([0, 3, 17, 40]) for _ in new]
+    assert sum(new) * 40 > 128 * len(new)
+    _attention_case(cuda, torch.bfloat16, _E4M3, new, cached, 40, 1, 64, 16, seed=4, wide=2 ** 11, pad=3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_captured_chunk_in_wide_tables_that_share_pages_or_not(cuda, dtype):
+    """Requests that share their pages need more room for copies than the cache has pages, and are attended to as they are. One graph, replayed on tables that
+    share and tables that do not, between eager calls."""
+    case = Case(cuda, _E4M3, [300, 300], [500, 500], 2, 64, 16, seed=2, spare=0)
+    apart = torch.cat([case.table, torch.full((2, 2 ** 18), -1, dtype=torch.int32, device=cuda)], 1)
+    shared = apart.clone()
+    shared[1] = shared[0]
+    caches = [c.view(torch.uint8)[:60].clone().view(_E4M3) if c.shape[0] > 60 else c for c in case.caches]  # 50 pages a request: room for one
+    scales = [x.view(torch.uint8)[:60].clone().view(_E8M0) for x in case.scales]
+    order = torch.arange(50, dtype=torch.int32, device=cuda)
+    shared[0, :50] = shared[1, :50] = order
+    apart[0, :50], apart[1, :50] = order, torch.where(order < 10, order + 50, -1)  # of the second request's pages ten are there
+    case.wide = [w[:60] for w in case.wide]
+    lens = [_i32([800, 800], cuda), _i32([800, 0], cuda)]  # the second one is refused where pages are apart: its rows see nothing
+    q = torch.randn(600, 4, 64, generator=torch.Generator().manual_seed(3)).to(dtype)
+    queries, out, table, kv_lens = q.to(cuda), torch.empty(600, 4, 64, dtype=dtype, device=cuda), apart.clone(), lens[1].clone()
+
+    def call(o):
+        return P.paged_attention(queries, *caches, table, kv_lens, case.cu_new, 0.125, out=o, key_scales=scales[0], value_scales=scales[1])
+
+    stream = torch.cuda.Stream(cuda)
+    stream.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(stream):
+        call(out)
+    torch.cuda.current_stream(cuda).wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    case.table_host[0, :50] = order.cpu()
+    want, bound = _over_a_context(case, q[:300], 0.125, dtype, _HALF_STEP[dtype])
+    other, other_bound = _over_a_context(case, q[300:], 0.125, dtype, _HALF_STEP[dtype])
+    for i in range(8):
+        table.copy_(shared if i % 2 else apart)
+        kv_lens.copy_(lens[0] if i % 2 else lens[1])
+        graph.replay()
+        eager = call(torch.empty_like(out))
+        torch.cuda.synchronize(cuda)
+        assert torch.equal(out, eager), i
+        got = eager.double().cpu()
+        assert ((got[:300] - want).abs() <= bound).all(), i
+        if i % 2:
+            assert ((got[300:] - other).abs() <= other_bound).all(), i
+        else:
+            assert got[300:].eq(0).all(), i
+
+
 def _over_a_context(case, q, scaling, dtype, term):
     """(want, bound) of a chunk alone in its table, in 64 bits: bounds as derived for _attention_case, a weight off by `term` of itself."""
     keys, values = (case.context(0, which)[0] for which in range(2))

@@ -203,8 +203,8 @@ def test_workspaces_follow_the_work():
 
 @pytest.mark.parametrize("dtype", [1, 2])
 def test_the_copy_of_a_chunk_has_room_for_what_the_caller_says(dtype):
-    def attention(slots, tokens, max_context, width=8192, page_size=16, window=0):
-        args = N.PageAttentionArgs(dtype=dtype, Hq=32, max_context=max_context, window=window, cache=N.PageCache(dtype=3, n_pages=9, page_size=page_size, Hkv=8, D=128),
+    def attention(slots, tokens, max_context, width=8192, page_size=16, n_pages=9):
+        args = N.PageAttentionArgs(dtype=dtype, Hq=32, max_context=max_context, cache=N.PageCache(dtype=3, n_pages=n_pages, page_size=page_size, Hkv=8, D=128),
                                    requests=N.PageRequests(table_width=width, n_requests=slots, n_tokens=tokens))
         return N.page_work_bytes("attention", args)
 
@@ -217,9 +217,11 @@ def test_the_copy_of_a_chunk_has_room_for_what_the_caller_says(dtype):
     assert copy(1, 8192) <= attention(1, 4096, 0) <= copy(1, 8192) + rest        # not said: the table's
     assert copy(1, 8192) <= attention(1, 4096, 2 ** 31 - 1) <= copy(1, 8192) + rest
     assert copy(4, 1, 4096) <= attention(4, 4096, 7, 32, 4096) <= copy(4, 1, 4096) + rest
-    for slots, hint in ((16, 0), (16, 131072), (64, 16384), (2, 2 ** 31 - 1)):     # no copy of more than 2 GiB
-        width = 8192 if slots > 2 else 2 ** 20
-        assert attention(slots, 4096, hint, width) <= rest
+    # rooms of more than 2 GiB: as many pages as the cache has, 2 GiB at most, and a table
+    for slots, hint, width in ((16, 0, 8192), (16, 131072, 8192), (64, 16384, 8192), (2, 2 ** 31 - 1, 2 ** 20)):
+        for n_pages in (9, 1000, 30000, 2 ** 22):
+            least = 4 * min(n_pages, 2 ** 15) * 16 * 8 * 128
+            assert least <= attention(slots, 4096, hint, width, n_pages=n_pages) <= least + rest
 
 
 def test_the_workspace_of_a_selection_is_bounded():
