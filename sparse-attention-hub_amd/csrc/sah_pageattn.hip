@@ -1050,7 +1050,9 @@ static pt_copy pt_copy_of(const sah_page_attention_args* a) {
   c.table_at = c.pages * (int64_t)page;
   c.placed_at = placed ? round(c.table_at + (int64_t)n * c.width * 4) : 0;
   c.lost_at = placed ? round(c.placed_at + (int64_t)n * 8) : round(c.table_at + (int64_t)n * c.width * 4);
-  c.n_lost = a->dtype == SAH_F16 || c.width < table || placed ? (int)pg_load_workgroups(a->cache, a->requests, c.width * page_size) : 0;
+  const int64_t wgs = pg_load_workgroups(a->cache, a->requests, c.width * page_size);
+  if (!wgs) return c;
+  c.n_lost = a->dtype == SAH_F16 || c.width < table || placed ? (int)wgs : 0;
   c.bytes = round(c.lost_at + c.n_lost);
   return c;
 }

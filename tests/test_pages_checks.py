@@ -222,6 +222,8 @@ def test_the_copy_of_a_chunk_has_room_for_what_the_caller_says(dtype):
         for n_pages in (9, 1000, 30000, 2 ** 22):
             least = 4 * min(n_pages, 2 ** 15) * 16 * 8 * 128
             assert least <= attention(slots, 4096, hint, width, n_pages=n_pages) <= least + rest
+    # tables whose copy is more than a launch's workgroups, or whose own table is large: the cache as it is
+    assert attention(1024, 40000, 0, 2 ** 12, 4096, 9) <= rest and attention(2 ** 14, 2 ** 20, 0, 2 ** 13, 1, 9) <= rest
 
 
 def test_the_workspace_of_a_selection_is_bounded():
