@@ -40,7 +40,7 @@ typedef struct sah_page_requests {
 } sah_page_requests;
 
 /* Quantises row t of keys and values [n_tokens, Hkv, D] (dtype) into slot slot_map[t] of a SAH_E4M3 cache, the scales with it. Slots outside the cache
- * are passed over; two rows of one slot: which one it holds is not defined. Rows and slots share no memory with the cache. */
+ * are passed over; two rows of one slot: what it holds is not defined (elements of one, the scale of the other). Rows and slots share no memory with the cache. */
 typedef struct sah_page_store_args {
   sah_page_cache cache;
   const void* k; int64_t ks_t, ks_h;
