@@ -113,7 +113,7 @@ int sah_page_select(const sah_page_select_args* a);
  * exact as the result's own rounding. Chunks of an 8-bit cache under 16-bit q (more than 128 rows of q a request
  * and key head on average, with a window as many times more as the table has keys beyond it) are attended to through a
  * copy in q's type, in work, of the contexts of requests with new tokens, by sah_paged_attention's kernels and with what it says of weights. The copy has room for
- * max_context tokens of every request (the table's where that is 0), or, where this passes 2 GiB, for as many tokens as the cache or 2 GiB hold. Where a context is
+ * the table's tokens of every request up to 256 MiB, else max_context ones (0: the table's), or, where this passes 2 GiB, for as many tokens as the cache or 2 GiB hold. Where a context is
  * longer, all of them need more room (requests that share pages), or the cache holds what SAH_F16 does not (beyond 65504, finer than 2^-24), it is attended to as it is
  * all the same. work: sah_page_attention_work_bytes(a) bytes, 16-byte aligned, no particular content. */
 typedef struct sah_page_attention_args {

@@ -1013,14 +1013,16 @@ static pt_args pt_plan(const sah_page_attention_args* a, int& wgs) {
 // 128 rows 74 / 84, 256 rows 124 / 99, 512 rows 222 / 137; of those keys 512 + 128 seen, 1024 rows 56 / 70, 4096 rows 191 / 129; 2 requests of
 // 32768, 2048 + 128 seen, 1024 rows 84 / 129, 4096 rows 248 / 175). Never for fp32 q: its terms go at the 16-bit matrix rate here, an fp32 copy at a
 // tenth of it (4 requests of 8192 keys, 128 rows 80 / 268, 2048 rows 947 / 2952).
-// A copy has room for max_context tokens of every request (the table's where that is not given) while this comes to no more than 2 GiB. Tables are as wide as a
-// server's longest request may become (16 of 131072 tokens, 8 heads of 128: 8 GiB): beyond that contexts are copied one behind the other, into as many
-// pages as the cache has, 2 GiB at most. (2048 tokens of one request over 16384 keys, 32 tables of 18432: 662 us; as it is 1699, alone in its table 658.)
+// A copy has room for the table's tokens of every request while this comes to no more than 256 MiB, else for max_context ones, where that is given. Tables are as
+// wide as a server's longest request may become (16 of 131072 tokens, 8 heads of 128: 8 GiB): from 2 GiB on contexts are copied one behind the other, into as many
+// pages as the cache has, 2 GiB at most. (A smaller room saves no time: 4 requests of 64 tokens over 8192 keys in tables of 16384 98 us, with room for 8192 and asking
+// whether that was enough 107. 2048 tokens of one request over 16384 keys, 32 tables of 18432: 662 us; as it is 1699, alone in its table 658.)
 //
 // fp16 does not hold all that an 8-bit cache can, a context may be longer than max_context says, and all of them may need more room than there is: the copy's
 // workgroups tell where that is so, and the cache is then attended to as it is, all rows once more (copies that hold everything pay for it with two launches that end at
 // once: 4 requests of 64 fp16 tokens over 8192 keys 104 -> 113 us).
 #define PT_COPY_BYTES 0x1p31
+#define PT_COPY_WHOLE 0x1p28
 struct pt_copy {
   int64_t bytes;    // K, V, their table, places and what was lost; 0: none
   int width;        // pages of a request, at most
@@ -1036,8 +1038,8 @@ static pt_copy pt_copy_of(const sah_page_attention_args* a) {
   const double rows = (double)a->requests.n_tokens * (a->Hq / a->cache.Hkv);
   if (rows * seen <= 128 * keys * n) return c;
   const int64_t hint = ((int64_t)a->max_context + page_size - 1) / page_size;
-  c.width = hint > 0 && hint < table ? (int)hint : table;
   const double page = (double)page_size * a->cache.Hkv * a->cache.D * pg_size(a->dtype) * 2;
+  c.width = hint > 0 && hint < table && (double)n * table * page > PT_COPY_WHOLE ? (int)hint : table;
   c.pages = (int64_t)n * c.width;
   if (c.pages * 4.0 > PT_COPY_BYTES / 8) return c;  // (their table)
   const bool placed = c.pages * page > PT_COPY_BYTES;

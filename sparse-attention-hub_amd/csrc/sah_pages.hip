@@ -124,7 +124,7 @@ __device__ __forceinline__ bool pg_none_of_f16(uint2 x, uint32_t scale) {
   float f[2][4];
   pg_widen4(x.x, pg_scale(scale), f[0]);
   pg_widen4(x.y, pg_scale(scale), f[1]);
-  [[maybe_unused]] bool lost = false;
+  bool lost = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float v = f[i / 4][i % 4];
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(PG_NT) void k_page_load(sah_page_cache C, sah_page_
   }
 }
 
-// One workgroup: how many pages each request needs, then where each one's begin (4 us for 64 requests, nearly all of it the launch and two readings).
+// One workgroup: how many pages each request needs, then where each one's begin (4.5 us for 64 requests, nearly all of it the launch and two readings).
 __global__ __launch_bounds__(PG_NT) void k_page_place(sah_page_requests R, int page_size, int width, int64_t room, int32_t* first, int32_t* lens) {
   __shared__ int64_t s_sum[2][PG_NT / SAH_WAVE];
   const int lane = threadIdx.x & (SAH_WAVE - 1), wave = sah_wave_id(), shift = 31 - __builtin_clz(page_size), most = R.table_width << shift;
@@ -374,8 +374,8 @@ __global__ __launch_bounds__(PG_NT) void k_page_bounds(sah_page_bounds_args P, i
 // ---------------------------------------------------------------------------
 // select: a 64-bit key per candidate (larger: rather taken), then the largest of a row
 // The sum over heads of max(q a, q b) with a <= b, both finite, is Q+ . b + Q- . a, Q+ (Q-) the sum of the heads' positive (negative) elements: the heads
-// share one reading of the bounds and one pair of products (pages of infinite bounds: pg_score_again). In fp64, in which rounding decides between almost equal scores alone; fp32 is no faster (72 us against 70): reading the
-// bounds is what it costs. 64 answers of 1K to 32K keys in pages of 16, 8 heads: 277 MB of bf16 bounds, 62 us, 4.5 TB/s; they are read past the caches, which
+// share one reading of the bounds and one pair of products (pages of infinite bounds: pg_score_again). In fp64, in which rounding decides between almost equal
+// scores alone; fp32 is no faster (72 us against 70): reading the bounds is what it costs. 64 answers of 1K to 32K keys in pages of 16, 8 heads: 277 MB of bf16 bounds, 62 us, 4.5 TB/s; they are read past the caches, which
 // they would go through once (71 us). All heads of a page by one wave 97 us, smallest and largest by neighbouring lanes 80.
 // ---------------------------------------------------------------------------
 #define PG_ALWAYS ~0ull        // pages that are taken whatever they score

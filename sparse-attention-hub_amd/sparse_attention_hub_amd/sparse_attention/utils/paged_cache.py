@@ -221,8 +221,8 @@ def paged_attention(queries: torch.Tensor, key_cache: torch.Tensor, value_cache:
     the queries may be slices of one buffer, their tokens equally far apart). Returns `(n_tokens, heads, head_dim)`.
 
     An 8-bit cache (head_dim a multiple of 16) takes float32, bfloat16 or float16 queries, the result's type. Long chunks under 16-bit ones are attended
-    to through a copy of their contexts with room for `max_context` tokens of every request, at most 2 GiB: where the table is much wider, what the
-    step's longest request has saves memory (a longer context costs time, and changes nothing else than whether weights are rounded to 16 bits). `pages`, int32 `(n_tokens,
+    to through a copy of their contexts, from 256 MiB on with room for `max_context` tokens of every request, 2 GiB at most: where the table is much wider, what
+    the step's longest request has saves memory (a longer context costs time, and changes nothing else than whether weights are rounded to 16 bits). `pages`, int32 `(n_tokens,
     kv_heads, n)` as from `select_pages`: row t's heads of a key head see the keys at or before its position on these pages of its request
     alone (places in its row of `block_table`; others, and -1, stand for nothing; one named twice counts twice); not with `window_size`.
     """

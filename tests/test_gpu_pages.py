@@ -589,17 +589,18 @@ def test_attention_8bit_chunks_copy_no_context_without_a_row(cuda, dtype):
 
 @pytest.mark.parametrize("dtype", _TYPES)
 @pytest.mark.parametrize("max_context", [1, 300, 512, 799, 800, 801, 10 ** 9])
-@pytest.mark.parametrize("sink, window", [(0, 0), (20, 90)])
-def test_attention_8bit_chunks_do_not_depend_on_the_hint(cuda, dtype, max_context, sink, window):
-    """A copy with room for less than a context, for just that, for more: long chunks beside a short one and an idle request, in a wide table."""
-    _attention_case(cuda, dtype, _E4M3, [400, 0, 170, 250], [400, 900, 300, 0], 4, 2, 64, 16, sink, window, sinks=True, seed=5, max_context=max_context, wide=60, pad=2,
+@pytest.mark.parametrize("sink, window, wide", [(0, 0, 60), (0, 0, 2 ** 14), (40, 200000, 2 ** 14)])
+def test_attention_8bit_chunks_do_not_depend_on_the_hint(cuda, dtype, max_context, sink, window, wide):
+    """A copy with room for less than a context, for just that, for more: long chunks beside a short one and an idle request, in a table whose copy is small, and
+    where the hint decides its size."""
+    _attention_case(cuda, dtype, _E4M3, [400, 0, 170, 250], [400, 900, 300, 0], 4, 2, 64, 16, sink, window, sinks=True, seed=5, max_context=max_context, wide=wide, pad=2,
                     missing=[(0, 2, -1), (0, 45, 10 ** 6), (2, 0, -3)])
 
 
 def test_a_captured_chunk_whose_contexts_pass_the_hint(cuda):
     """One graph, replayed on contexts that the copy has room for and on longer ones, between eager calls."""
     cases = [Case(cuda, _E4M3, [300, 200], [n, 30], 2, 64, 16, seed=n) for n in (200, 212, 600)]
-    width = max(c.width for c in cases) + 20
+    width = max(c.width for c in cases) + 2 ** 15  # 512 MiB: the hint decides the copy's size
     tables = [torch.cat([c.table, torch.full((2, width - c.width), -1, dtype=torch.int32, device=cuda)], 1) for c in cases]
     most = max(c.caches[0].shape[0] for c in cases)
     grow = lambda x: torch.cat([x, torch.zeros(most - x.shape[0], *x.shape[1:], dtype=x.dtype, device=cuda)])
